@@ -289,6 +289,68 @@ typedef struct NtRlReadoutScoreArgs {
 } NtRlReadoutScoreArgs;
 int nt_hip_rl_readout_score(const NtRlReadoutScoreArgs *a);
 
+/* The readout-fused scorer of a training step: nt_hip_rl_readout_score for a weight that changes between
+ * steps (not packed), any number of rows, any sizes, bf16 or f16 on the matrix cores as they are (f32 sums),
+ * every mask, and the log-sum-exps that the backward needs; the logits are never written. For each row, with
+ * z = tempered_logits(hidden . W, T, mask) (rl.rs:475-486):
+ *   logp[r]    = token_log_probs(z, tokens)[r]      (rl.rs:134-141; minus it is the cross entropy,
+ *                                                    src/nn/loss.rs:10-16)
+ *   entropy[r] = categorical_entropy(z)[r]          (rl.rs:405-414)
+ *   lse_base[r] + lse_rest[r] = ln sum exp z, lse_base the maximum of z.
+ * A token that the mask excludes has logp -inf; one outside [0, vocab) has logp NaN and NT_ROW_BAD_TOKEN.
+ * A row with no allowed token has logp and entropy NaN, lse_base -inf, lse_rest 0 and NT_ROW_NO_TOKEN; one
+ * whose allowed logits hold a NaN or +inf has NaNs and NT_ROW_NAN. Rows of 16-byte-aligned operands whose
+ * strides and contiguous lengths are multiples of 8 are read in place; others are first copied into such rows.
+ * The workspace is 8 (12 with the entropy) bytes per row and 128 columns, and those copies. */
+typedef struct NtRlReadoutStatsArgs {
+    const void *hidden;        /* [rows, ldh] */
+    const void *weight;        /* [dim, ldw] (NT_READOUT_W_DV) or [vocab, ldw] (NT_READOUT_W_VD) */
+    int32_t dtype;             /* NT_BF16 | NT_F16 (both) */
+    int32_t layout;            /* NT_READOUT_W_* */
+    int64_t rows, vocab, dim;  /* rows <= 2^24, vocab <= 2^20, dim <= 65536 */
+    int64_t ldh, ldw;          /* row strides in elements, at most 2^21 */
+    const void *mask;          /* rows of vocab entries; NULL with NT_MASK_NONE */
+    int64_t mask_ld;           /* mask row stride; 0 = one row shared */
+    int32_t mask_kind;         /* NT_MASK_NONE | NT_MASK_U8 | NT_MASK_F32 */
+    int32_t pad0;
+    double temperature;        /* > 0 and finite */
+    const int32_t *tokens;     /* [rows] */
+    float *logp;               /* [rows] out */
+    float *entropy;            /* [rows] out or NULL */
+    float *lse_base;           /* [rows] out or NULL */
+    float *lse_rest;           /* [rows] out or NULL */
+    uint8_t *status;           /* [rows] out: NT_ROW_* */
+} NtRlReadoutStatsArgs;
+int nt_hip_rl_readout_score_stats(const NtRlReadoutStatsArgs *a);
+
+/* Its backward: the gradients of sum_r g_logp[r] logp[r] + g_entropy[r] entropy[r] with respect to the hidden
+ * states and the weight, in the operands' type. With p = exp(z - lse),
+ *   G = (g_logp (onehot(token) - p) - g_entropy p (ln p + entropy)) / T     (score_backward's dL/dx)
+ *   grad_hidden = G W^T  [rows, grad_hidden_ld],   grad_weight = H^T G, laid out as the weight.
+ * The logits are computed again, a piece of the vocabulary at a time; G, at most 512 MiB of it (256 columns
+ * at the least), is rounded to the operands' type, every sum is f32 and in a fixed order. A row whose
+ * upstream gradients are zero, and one that has no allowed token, adds nothing, whatever its hidden states
+ * hold; a token outside [0, vocab) has no log-probability to differentiate. rows 0 gives a zero
+ * grad_weight. Inputs as the forward's, with its outputs. */
+typedef struct NtRlReadoutStatsGradArgs {
+    const void *hidden, *weight;
+    int32_t dtype, layout;
+    int64_t rows, vocab, dim, ldh, ldw;
+    const void *mask;
+    int64_t mask_ld;
+    int32_t mask_kind;
+    int32_t pad0;
+    double temperature;
+    const int32_t *tokens;
+    const float *lse_base, *lse_rest;  /* [rows] from the forward */
+    const float *entropy;              /* [rows] the forward's; needed when g_entropy is given */
+    const float *g_logp, *g_entropy;   /* [rows] upstream gradients, or NULL (zero) */
+    void *grad_hidden;                 /* [rows, grad_hidden_ld] out or NULL */
+    void *grad_weight;                 /* the weight's layout, row stride grad_weight_ld, out or NULL (one of the two) */
+    int64_t grad_hidden_ld, grad_weight_ld;
+} NtRlReadoutStatsGradArgs;
+int nt_hip_rl_readout_score_backward(const NtRlReadoutStatsGradArgs *a);
+
 /* Fused row scoring: for each row, any of
  *   logp[r]     = token_log_probs(z, tokens)[r]                 (rl.rs:134-141)
  *   ref_logp[r] = token_log_probs(zr, tokens)[r]                (rl.rs:134-141, reference)

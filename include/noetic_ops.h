@@ -169,6 +169,27 @@ int nt_hip_matmul_half(const float *a, const NtLayout *al, const float *b, const
  * NUL-terminated into buf. */
 int nt_hip_half_gemm_key(char *buf, size_t cap);
 
+/* Rows in 8 bits (no counterpart in the reference: beside cast and matmul_half, for weights and activations
+ * held or multiplied in integers). Each row of the view x (f32, bf16 or f16; a row is the last dimension, so a
+ * swapped view quantizes columns) becomes q = round(x / s), ties to even, of the exact quotient, |q| <= 127,
+ * and its scale s = max |x| / 127 in f32: q contiguous over the view's shape, scale over its leading
+ * dimensions. A row of zeros has scale 0; one that holds a NaN or an infinity has scale NaN and zeros; a row
+ * of no elements scale 0. A view whose leading dimensions do not fold into one stride, or whose rows are not
+ * contiguous (nor its columns), is first copied to scratch. */
+int nt_hip_quantize_int8(const void *x, const NtLayout *xl, int32_t dtype, int8_t *q, float *scale);
+
+/* out = q scale, the values the 8 bits stand for, rounded to nearest even into dtype: q and out [rows, cols]
+ * contiguous, scale [rows]. */
+int nt_hip_dequantize_int8(const int8_t *q, const float *scale, int64_t rows, int64_t cols, int32_t dtype, void *out);
+
+/* The product of quantized rows: out[i, j] = (sum_k a[i, k] b[j, k]) a_scale[i] b_scale[j], a scale for each
+ * token (row of a) and each channel (row of b, the weight [n, k]). The integer sums are exact in 32 bits
+ * (k <= 131071), then rounded to f32, scaled, and rounded into dtype (f32, bf16 or f16). Row strides lda, ldb
+ * (at most 2^22) and ldo in elements. Operands whose base and stride are not multiples of 16, or whose k is not, are first
+ * copied to scratch rows that are. k = 0 gives zeros. */
+int nt_hip_matmul_int8(const int8_t *a, int64_t lda, const float *a_scale, const int8_t *b, int64_t ldb, const float *b_scale,
+                       int64_t m, int64_t n, int64_t k, int32_t dtype, void *out, int64_t ldo);
+
 /* GpuBackend::sort_desc (gpu/mod.rs:186-191; CpuRef's order, kernels.rs:374-413): along the
  * middle of contiguous f32 x [outer, n, inner], descending: every NaN first (all NaNs equal),
  * then total_cmp (+0 before -0), ties in ascending source position. vals gets the source values

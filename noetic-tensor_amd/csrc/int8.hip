@@ -1,0 +1,370 @@
+// 8-bit rows and their product: a row (a token's activations, an output channel's weights) held as integers
+// q = round(x / s) with one f32 scale s = max |x| / 127, and C = (qa qb^T) sa sb on the matrix cores.
+//
+// The reference has no 8-bit type; these stand beside its cast and its reduced-precision product
+// (src/tensor/gpu/mod.rs:142-144, 157-162), as MatmulPrecision::Half's bf16 operands do
+// (src/tensor/precision.rs:4-8).
+//
+// Quantizing: the quotient's nearest integer, ties to even, of the exact x / s, so that the integers depend on
+// no rounding of the quotient: r = round(x (1/s)) is at most one off next to a border, and the remainder
+// x - r s, exact in one fma, says which side x is on. Bounded by HBM: the values in, a byte each out.
+//
+// The product: v_mfma_i32_32x32x32_i8 sums exactly in 32 bits (k up to 131071 keeps |sum| under 2^31), so the
+// only roundings are the sum's to f32, the two scales' products and the output type's.
+#include <hip/hip_runtime.h>
+
+#include <algorithm>
+#include <cmath>
+#include <cstdint>
+#include <string>
+#include <type_traits>
+
+#include "../../include/noetic_ops.h"
+#include "nt_internal.hpp"
+#include "nt_tile.hpp"
+
+namespace nt {
+namespace {
+
+using namespace tile;
+
+typedef u32x4 u32x4u __attribute__((aligned(1)));
+
+int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
+int64_t round_up(int64_t a, int64_t b) { return ceil_div(a, b) * b; }
+
+template <int T>
+__device__ __forceinline__ float load_f32(const void *p, int64_t i) {
+    if constexpr (T == NT_F32) return static_cast<const float *>(p)[i];
+    else if constexpr (T == NT_BF16) return __builtin_bit_cast(float, uint32_t(static_cast<const uint16_t *>(p)[i]) << 16);
+    else return float(static_cast<const _Float16 *>(p)[i]);
+}
+
+// A row's scale from its largest magnitude, NaN where it holds a NaN or an infinity.
+__device__ __forceinline__ float scale_of(float amax, bool finite) { return finite ? amax / 127.0f : NAN; }
+
+// The 8-bit value of x at scale s; `inv` is 1 / s rounded. A row of zeros (s 0) is zeros, as is one whose scale
+// is NaN. Scales under 2^-100, whose reciprocal or products may leave f32, take the quotient in f64, which is
+// as exact here: |x / s - (n + 1/2)| is 0 or over 2^-33.
+__device__ __forceinline__ int quantized(float x, float s, float inv) {
+    if (!(s >= 0x1p-100f)) {
+        if (!(s > 0.0f)) return 0;
+        const double r = rint(double(x) / double(s));
+        return int(fmin(fmax(r, -127.0), 127.0));  // (a subnormal scale's own rounding may pass 127)
+    }
+    float r = rintf(x * inv);
+    const float d = 2.0f * fmaf(-r, s, x);  // twice the exact remainder
+    const bool odd = (int(r) & 1) != 0;
+    if (d > s || (d == s && odd)) r += 1.0f;
+    else if (-d > s || (-d == s && odd)) r -= 1.0f;
+    return int(r);
+}
+
+// A workgroup a row.
+template <int T>
+__global__ __launch_bounds__(256) void k_quantize_rows(const void *xv, int64_t cols, int64_t ld, int8_t *q, float *scale) {
+    __shared__ float s_max[4];
+    __shared__ int s_bad[4];
+    const int64_t row = blockIdx.x, at = row * ld;
+    float m = 0.0f;
+    bool bad = false;
+    for (int64_t c = threadIdx.x; c < cols; c += 256) {
+        const float a = fabsf(load_f32<T>(xv, at + c));
+        bad |= !(a < INFINITY);
+        m = fmaxf(m, a);
+    }
+#pragma unroll
+    for (int d = 32; d; d /= 2) m = fmaxf(m, __shfl_xor(m, d, 64));
+    const bool any = __any(bad);
+    if (threadIdx.x % 64 == 0) s_max[threadIdx.x / 64] = m, s_bad[threadIdx.x / 64] = any;
+    __syncthreads();
+    m = fmaxf(fmaxf(s_max[0], s_max[1]), fmaxf(s_max[2], s_max[3]));
+    const float s = scale_of(m, !(s_bad[0] | s_bad[1] | s_bad[2] | s_bad[3])), inv = 1.0f / s;
+    if (threadIdx.x == 0) scale[row] = s;
+    for (int64_t c = threadIdx.x; c < cols; c += 256) q[row * cols + c] = int8_t(quantized(load_f32<T>(xv, at + c), s, inv));
+}
+
+// Rows that are the columns of x [n, ld]: a workgroup takes 64 of them.
+template <int T>
+__global__ __launch_bounds__(256) void k_quantize_columns(const void *xv, int64_t rows, int64_t n, int64_t ld, int8_t *q,
+                                                          float *scale) {
+    __shared__ float s_max[4][64];
+    __shared__ int s_bad[4][64];
+    __shared__ int8_t tile[64][65];
+    const int lc = threadIdx.x % 64, seg = threadIdx.x / 64;
+    const int64_t c0 = int64_t(blockIdx.x) * 64, c = c0 + lc;
+    const bool live = c < rows;
+    float m = 0.0f;
+    bool bad = false;
+    if (live)
+        for (int64_t k = seg; k < n; k += 4) {
+            const float a = fabsf(load_f32<T>(xv, k * ld + c));
+            bad |= !(a < INFINITY);
+            m = fmaxf(m, a);
+        }
+    s_max[seg][lc] = m, s_bad[seg][lc] = bad;
+    __syncthreads();
+    m = fmaxf(fmaxf(s_max[0][lc], s_max[1][lc]), fmaxf(s_max[2][lc], s_max[3][lc]));
+    const float s = scale_of(m, !(s_bad[0][lc] | s_bad[1][lc] | s_bad[2][lc] | s_bad[3][lc])), inv = 1.0f / s;
+    if (seg == 0 && live) scale[c] = s;
+    for (int64_t k0 = 0; k0 < n; k0 += 64) {
+        for (int k = seg; k < 64; k += 4)
+            tile[k][lc] = live && k0 + k < n ? int8_t(quantized(load_f32<T>(xv, (k0 + k) * ld + c), s, inv)) : int8_t(0);
+        __syncthreads();
+        for (int r = seg; r < 64; r += 4)
+            if (c0 + r < rows && k0 + lc < n) q[(c0 + r) * n + k0 + lc] = tile[lc][r];
+        __syncthreads();
+    }
+}
+
+template <int T>
+__global__ __launch_bounds__(256) void k_dequantize(const int8_t *q, const float *scale, int64_t rows, int64_t cols, void *out) {
+    const int64_t total = rows * cols;
+    for (int64_t i = blockIdx.x * int64_t(256) + threadIdx.x; i < total; i += int64_t(gridDim.x) * 256) {
+        float x = float(q[i]) * scale[i / cols];
+        asm("" : "+v"(x));  // (rounded to f32 first for every type: the f16 product is not made one instruction)
+        if constexpr (T == NT_F32) static_cast<float *>(out)[i] = x;
+        else if constexpr (T == NT_BF16) static_cast<uint16_t *>(out)[i] = uint16_t(pair16<Bf16>(x, 0.0f));
+        else static_cast<uint16_t *>(out)[i] = uint16_t(pair16<F16>(x, 0.0f));
+    }
+}
+
+// Bytes of rows into rows of `ldo` (a multiple of 16) bytes, zeros from `cols` on.
+__global__ __launch_bounds__(256) void k_pad_bytes(const uint8_t *src, int64_t rows, int64_t cols, int64_t ld, uint8_t *out,
+                                                   int64_t ldo) {
+    const int64_t per = ldo / 16, total = rows * per;
+    for (int64_t i = blockIdx.x * int64_t(256) + threadIdx.x; i < total; i += int64_t(gridDim.x) * 256) {
+        const int64_t r = i / per, c = (i - r * per) * 16;
+        const uint8_t *s = src + r * ld + c;
+        union {
+            u32x4 v;
+            uint8_t b[16];
+        } x;
+        if (c + 16 <= cols) x.v = *reinterpret_cast<const u32x4u *>(s);
+        else
+            for (int e = 0; e < 16; e++) x.b[e] = c + e < cols ? s[e] : uint8_t(0);
+        *reinterpret_cast<u32x4 *>(out + r * ldo + c) = x.v;
+    }
+}
+
+struct Int8P {
+    const uint8_t *a, *b;
+    int64_t lda, ldb, m, n, kb;
+    uint32_t tm, tn;
+    const float *sa, *sb;
+    void *out;
+    int64_t ldo;
+};
+
+template <int T>
+__device__ __forceinline__ void store4(void *out, int64_t at, const float (&x)[4], int have) {
+    if constexpr (T == NT_F32) {
+        float *o = static_cast<float *>(out) + at;
+        if (have == 4) __builtin_memcpy(o, x, 16);
+        else
+            for (int e = 0; e < have; e++) o[e] = x[e];
+    } else {
+        typedef typename std::conditional<T == NT_BF16, Bf16, F16>::type E;
+        uint16_t *o = static_cast<uint16_t *>(out) + at;
+        const uint32_t w[2] = {pair16<E>(x[0], x[1]), pair16<E>(x[2], x[3])};
+        if (have == 4) __builtin_memcpy(o, w, 8);
+        else
+            for (int e = 0; e < have; e++) o[e] = uint16_t(w[e / 2] >> (16 * (e % 2)));
+    }
+}
+
+template <int TM, int TN, int WM, int WN, int OUT>
+__global__ __launch_bounds__(256, 1) void k_int8_tiles(Int8P p) {
+    typedef Tile<I8, TM, TN, WM, WN, false, false> T;
+    __shared__ __attribute__((aligned(16))) uint8_t lds[T::kLds];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    int im, in;
+    tile_of(blockIdx.x, p.tm, p.tn, im, in);
+    const int64_t m0 = int64_t(im) * T::BM, n0 = int64_t(in) * T::BN;
+    T t;
+    t.run(lds, Operand{p.a + m0 * p.lda, p.lda, p.m - m0, p.kb}, Operand{p.b + n0 * p.ldb, p.ldb, p.n - n0, p.kb}, p.kb, wave, lane);
+    const int wm = wave / WN, wn = wave % WN;
+#pragma unroll
+    for (int i = 0; i < TM; i++) {
+        const int64_t row = m0 + 32 * (TM * wm + i) + lane % 32;
+        if (row >= p.m) continue;
+        const float sa = p.sa[row];
+#pragma unroll
+        for (int j = 0; j < TN; j++)
+#pragma unroll
+            for (int q = 0; q < 4; q++) {
+                const int64_t col = n0 + 32 * (TN * wn + j) + 8 * q + 4 * (lane / 32);
+                const int have = p.n - col >= 4 ? 4 : int(p.n - col);
+                if (have <= 0) continue;
+                float x[4];
+#pragma unroll
+                for (int e = 0; e < 4; e++) x[e] = float(t.acc[i][j][4 * q + e]) * sa * (e < have ? p.sb[col + e] : 0.0f);
+                store4<OUT>(p.out, row * p.ldo + col, x, have);
+            }
+    }
+}
+
+int pad_rows(const int8_t *src, int64_t rows, int64_t cols, int64_t ld, uint8_t *out, int64_t ldo) {
+    const int64_t n = rows * (ldo / 16);
+    hipLaunchKernelGGL(k_pad_bytes, dim3(unsigned(std::min<int64_t>(ceil_div(n, 256), 8192))), dim3(256), 0, ctx().stream,
+                       reinterpret_cast<const uint8_t *>(src), rows, cols, ld, out, ldo);
+    return launched("k_pad_bytes");
+}
+
+bool aligned(const void *p, int64_t cols, int64_t ld) {
+    return reinterpret_cast<uintptr_t>(p) % 16 == 0 && ld % 16 == 0 && cols % 16 == 0;
+}
+
+constexpr int64_t kMaxK = 131071, kMaxLd = int64_t(1) << 22;
+
+int product(const int8_t *a, int64_t lda, const float *sa, const int8_t *b, int64_t ldb, const float *sb, int64_t m, int64_t n,
+            int64_t k, int32_t dtype, void *out, int64_t ldo) {
+    const bool ad = aligned(a, k, lda), bd = aligned(b, k, ldb);
+    const int64_t kp = round_up(k, 16);
+    const int64_t abytes = ad ? 0 : m * kp;
+    const int64_t need = abytes + (bd ? 0 : n * kp);
+    void *ws = nullptr;
+    if (need > 0)
+        if (int rc = scratch_alloc(size_t(need), &ws)) return rc;
+    uint8_t *pa = static_cast<uint8_t *>(ws), *pb = pa + abytes;
+    Int8P p{reinterpret_cast<const uint8_t *>(a), reinterpret_cast<const uint8_t *>(b), lda, ldb, m, n, kp, 0, 0, sa, sb, out,
+            ldo};
+    int rc = 0;
+    if (!ad) {
+        rc = pad_rows(a, m, k, lda, pa, kp);
+        p.a = pa, p.lda = kp;
+    }
+    if (!rc && !bd) {
+        rc = pad_rows(b, n, k, ldb, pb, kp);
+        p.b = pb, p.ldb = kp;
+    }
+    if (!rc) {
+        p.tm = uint32_t(ceil_div(m, 256)), p.tn = uint32_t(ceil_div(n, 256));
+        const dim3 grid(p.tm * p.tn), block(256);
+        if (dtype == NT_F32) hipLaunchKernelGGL((k_int8_tiles<4, 4, 2, 2, NT_F32>), grid, block, 0, ctx().stream, p);
+        else if (dtype == NT_BF16) hipLaunchKernelGGL((k_int8_tiles<4, 4, 2, 2, NT_BF16>), grid, block, 0, ctx().stream, p);
+        else hipLaunchKernelGGL((k_int8_tiles<4, 4, 2, 2, NT_F16>), grid, block, 0, ctx().stream, p);
+        rc = launched("k_int8_tiles");
+    }
+    const int rf = scratch_release(ws);
+    return rc ? rc : rf;
+}
+
+bool float_type(int32_t t) { return t == NT_F32 || t == NT_BF16 || t == NT_F16; }
+int size_of(int32_t t) { return t == NT_F32 ? 4 : 2; }
+
+// A view as rows of its last dimension: {rows, columns, strides of both}, if its leading dimensions fold into
+// one stride.
+struct Rows {
+    int64_t rows, cols, row_stride, col_stride;
+};
+bool as_rows(const NtLayout *l, Rows *o) {
+    const int r = l->rank;
+    o->rows = 1, o->cols = l->shape[r - 1], o->col_stride = l->strides[r - 1], o->row_stride = 0;
+    for (int d = r - 2; d >= 0; d--) {
+        if (l->shape[d] == 1) continue;
+        if (o->rows == 1) o->row_stride = l->strides[d];
+        else if (l->strides[d] != o->row_stride * o->rows) return false;
+        o->rows *= l->shape[d];
+    }
+    return true;
+}
+
+}  // namespace
+}  // namespace nt
+
+using namespace nt;
+
+extern "C" {
+
+int nt_hip_quantize_int8(const void *x, const NtLayout *xl, int32_t dtype, int8_t *q, float *scale) {
+    const char *who = "quantize_int8";
+    if (!xl || xl->rank < 1 || xl->rank > NT_MAX_RANK) return fail(NT_E_ARG, std::string(who) + ": a view of rank 1 to 8");
+    if (!float_type(dtype)) return fail(NT_E_ARG, std::string(who) + ": dtype " + std::to_string(dtype) + " (f32, bf16 or f16)");
+    int64_t total = 1;
+    for (int d = 0; d < xl->rank; d++) {
+        if (xl->shape[d] < 0 || xl->strides[d] < 0 || xl->offset < 0)
+            return fail(NT_E_ARG, std::string(who) + ": negative shape, stride or offset");
+        total *= xl->shape[d];
+    }
+    int64_t rows = 1;
+    for (int d = 0; d + 1 < xl->rank; d++) rows *= xl->shape[d];
+    const int64_t cols = xl->shape[xl->rank - 1];
+    if (rows > 0x7fffffff || cols > (int64_t(1) << 40))
+        return fail(NT_E_ARG, std::string(who) + ": " + std::to_string(rows) + " rows (at most 2^31 - 1)");
+    if (rows > 0 && (!scale || (total > 0 && (!x || !q))))
+        return fail(NT_E_ARG, std::string(who) + ": null buffer");
+    std::unique_lock<std::mutex> lk;
+    if (int rc = enter(&lk)) return rc;
+    if (rows == 0) return 0;
+    Rows v;
+    void *ws = nullptr;
+    const uint8_t *src = static_cast<const uint8_t *>(x) + xl->offset * size_of(dtype);
+    const bool folds = as_rows(xl, &v);
+    const bool columns = folds && v.rows > 1 && v.cols > 1 && v.row_stride == 1 && v.col_stride != 1;
+    if (!columns && !(folds && (v.col_stride == 1 || v.cols == 1))) {  // any other view: its values in order first
+        if (int rc = scratch_alloc(size_t(total) * size_of(dtype), &ws)) return rc;
+        lk.unlock();
+        int rc = nt_hip_copy(x, xl, size_of(dtype), ws);
+        if (int re = enter(&lk)) return rc ? rc : re;
+        if (rc) {
+            (void)scratch_release(ws);
+            return rc;
+        }
+        src = static_cast<const uint8_t *>(ws);
+        v = Rows{rows, cols, cols, 1};
+    }
+    hipStream_t st = ctx().stream;
+    if (columns) {
+        const dim3 grid(unsigned(ceil_div(v.rows, 64)));
+        if (dtype == NT_F32) hipLaunchKernelGGL(k_quantize_columns<NT_F32>, grid, dim3(256), 0, st, src, v.rows, v.cols, v.col_stride, q, scale);
+        else if (dtype == NT_BF16) hipLaunchKernelGGL(k_quantize_columns<NT_BF16>, grid, dim3(256), 0, st, src, v.rows, v.cols, v.col_stride, q, scale);
+        else hipLaunchKernelGGL(k_quantize_columns<NT_F16>, grid, dim3(256), 0, st, src, v.rows, v.cols, v.col_stride, q, scale);
+    } else {
+        const dim3 grid{unsigned(v.rows)};
+        if (dtype == NT_F32) hipLaunchKernelGGL(k_quantize_rows<NT_F32>, grid, dim3(256), 0, st, src, v.cols, v.row_stride, q, scale);
+        else if (dtype == NT_BF16) hipLaunchKernelGGL(k_quantize_rows<NT_BF16>, grid, dim3(256), 0, st, src, v.cols, v.row_stride, q, scale);
+        else hipLaunchKernelGGL(k_quantize_rows<NT_F16>, grid, dim3(256), 0, st, src, v.cols, v.row_stride, q, scale);
+    }
+    const int rc = launched("k_quantize");
+    const int rf = scratch_release(ws);
+    return rc ? rc : rf;
+}
+
+int nt_hip_dequantize_int8(const int8_t *q, const float *scale, int64_t rows, int64_t cols, int32_t dtype, void *out) {
+    const char *who = "dequantize_int8";
+    if (!float_type(dtype)) return fail(NT_E_ARG, std::string(who) + ": dtype " + std::to_string(dtype) + " (f32, bf16 or f16)");
+    if (rows < 0 || cols < 0 || (cols > 0 && rows > (int64_t(1) << 40) / cols))
+        return fail(NT_E_ARG, std::string(who) + ": " + std::to_string(rows) + " rows of " + std::to_string(cols));
+    if (rows * cols > 0 && (!q || !scale || !out)) return fail(NT_E_ARG, std::string(who) + ": null buffer");
+    std::unique_lock<std::mutex> lk;
+    if (int rc = enter(&lk)) return rc;
+    if (rows * cols == 0) return 0;
+    const dim3 grid(unsigned(std::min<int64_t>(ceil_div(rows * cols, 256), 16384)));
+    if (dtype == NT_F32) hipLaunchKernelGGL(k_dequantize<NT_F32>, grid, dim3(256), 0, ctx().stream, q, scale, rows, cols, out);
+    else if (dtype == NT_BF16) hipLaunchKernelGGL(k_dequantize<NT_BF16>, grid, dim3(256), 0, ctx().stream, q, scale, rows, cols, out);
+    else hipLaunchKernelGGL(k_dequantize<NT_F16>, grid, dim3(256), 0, ctx().stream, q, scale, rows, cols, out);
+    return launched("k_dequantize");
+}
+
+int nt_hip_matmul_int8(const int8_t *a, int64_t lda, const float *a_scale, const int8_t *b, int64_t ldb, const float *b_scale,
+                       int64_t m, int64_t n, int64_t k, int32_t dtype, void *out, int64_t ldo) {
+    const char *who = "matmul_int8";
+    if (!float_type(dtype)) return fail(NT_E_ARG, std::string(who) + ": dtype " + std::to_string(dtype) + " (f32, bf16 or f16)");
+    if (m < 0 || n < 0 || k < 0 || m > (1 << 24) || n > (1 << 24) || k > kMaxK || lda < k || ldb < k || ldo < n || lda > kMaxLd ||
+        ldb > kMaxLd || ceil_div(m, 256) * ceil_div(n, 256) >= (1 << 23))
+        return fail(NT_E_ARG, std::string(who) + ": [" + std::to_string(m) + ", " + std::to_string(k) + "] x [" + std::to_string(n) +
+                                  ", " + std::to_string(k) + "], row strides " + std::to_string(lda) + ", " +
+                                  std::to_string(ldb) + ", " + std::to_string(ldo) +
+                                  " (m and n at most 2^24 and 2^39 outputs, k at most 131071, strides at least the row, "
+                                  "the operands' at most 2^22)");
+    if (m > 0 && n > 0 && (!a_scale || !b_scale || !out || (k > 0 && (!a || !b))))
+        return fail(NT_E_ARG, std::string(who) + ": null buffer");
+    if (reinterpret_cast<uintptr_t>(out) % size_of(dtype)) return fail(NT_E_ARG, std::string(who) + ": unaligned out");
+    std::unique_lock<std::mutex> lk;
+    if (int rc = enter(&lk)) return rc;
+    if (m == 0 || n == 0) return 0;
+    return product(a, lda, a_scale, b, ldb, b_scale, m, n, k, dtype, out, ldo);
+}
+
+}  // extern "C"

@@ -1,0 +1,862 @@
+// The training readout: token log-probabilities, entropies and log-sum-exps of logits x = H W from the
+// hidden states, and their gradients with respect to H and W, the logits never kept.
+//
+// The reference multiplies (the decoder's head, src/nn/decoder.rs:272,286; linear.rs:1-3), keeps [rows, V]
+// logits, and differentiates log_softmax, gather and categorical_entropy on them (activation.rs:30-42,
+// rl.rs:134-141, 405-414). Here, with z = x / T + mask and y = z log2 e:
+//
+//  Forward: k_readout_stats computes a tile of x on the matrix cores (nt_tile.hpp) and reduces it where it
+//  stands: per row and block of columns the reference ref = max y, sum 2^(y - ref) and, for the entropy,
+//  sum 2^(y - ref) (y - ref) (f32: at most 128 terms). k_readout_merge joins a row's blocks in f64:
+//    lse = ln sum e^z, logp = z[token] - lse, entropy = lse - sum p z.
+//
+//  Backward: p = 2^(y - lse log2 e) comes from the logits computed once more, piece by piece of the
+//  vocabulary, so that
+//    G = dL/dx = (g_logp (onehot - p) - g_entropy p (ln p + entropy)) / T
+//  is held for one piece at a time, in the operands' 16-bit type: three products per piece, x = H W,
+//  dW = G^T H (the piece's rows of it, whole) and dH += G W^T (f32 sums over the pieces). 8 rows V dim
+//  operations with the forward's, against 6 where the logits are kept: the least there is without them.
+//
+//  Rounding: G is the one value that is rounded on the way (2^-9 of itself for bf16, 2^-12 for f16, as the
+//  gradients are when they are written); every sum is f32. For f16, whose range G would leave, a row of G is
+//  held in units of 2^(e - 14), 2^e over |g_logp| + 16 |g_entropy| (p |ln p + entropy| is under 14 for a
+//  vocabulary of 2^20), its share of dW being scaled through the row of H by a power of two.
+#include <hip/hip_runtime.h>
+
+#include <algorithm>
+#include <cmath>
+#include <cstdint>
+#include <string>
+#include <type_traits>
+
+#include "../../include/noetic_hip.h"
+#include "nt_internal.hpp"
+#include "nt_tile.hpp"
+
+namespace nt {
+namespace {
+
+using namespace tile;
+
+constexpr float kLog2e = 1.44269504088896340736f;
+constexpr double kLog2eD = 1.4426950408889634074, kLn2 = 0.69314718055994530942;
+
+typedef uint32_t u32u __attribute__((aligned(1)));
+typedef u32x4 u32x4u __attribute__((aligned(1)));
+typedef f32x16 f32x16_t;
+
+// The mask of a readout call: none, a u8 keep-mask or an additive f32 one, a row per logits row (ld > 0) or
+// one for all (ld 0), from the piece's first column on.
+struct MaskP {
+    const uint8_t *u8;
+    const float *f32;
+    int64_t ld;
+};
+
+// y = x c (+ mask log2 e) of four neighbouring columns of a row, -inf where the mask excludes them or past
+// the vocabulary's `n` columns.
+__device__ __forceinline__ void tempered4(const MaskP &m, int64_t row, int col, int n, float c, float (&y)[4]) {
+#pragma unroll
+    for (int e = 0; e < 4; e++) y[e] *= c;
+    if (col + 4 <= n) {
+        if (m.u8) {
+            const uint32_t k = *reinterpret_cast<const u32u *>(m.u8 + row * m.ld + col);
+#pragma unroll
+            for (int e = 0; e < 4; e++) y[e] = (k >> (8 * e)) & 0xffu ? y[e] : -INFINITY;
+        } else if (m.f32) {
+            float f[4];
+            __builtin_memcpy(f, m.f32 + row * m.ld + col, 16);
+#pragma unroll
+            for (int e = 0; e < 4; e++) y[e] = fmaf(f[e], kLog2e, y[e]);
+        }
+        return;
+    }
+#pragma unroll
+    for (int e = 0; e < 4; e++) {
+        if (col + e >= n) y[e] = -INFINITY;
+        else if (m.u8) y[e] = m.u8[row * m.ld + col + e] ? y[e] : -INFINITY;
+        else if (m.f32) y[e] = fmaf(m.f32[row * m.ld + col + e], kLog2e, y[e]);
+    }
+}
+
+// A piece of the vocabulary: x[r, v] = sum_k H(r, k) W(v, k) for `n` columns from v0 on.
+struct PieceP {
+    const uint8_t *h;  // k-contiguous [rows, ldh bytes]
+    const uint8_t *w;  // the piece's rows [n, ldw bytes] (VD) or columns of [dim, ldw bytes] (DV)
+    int64_t ldh, ldw, wwidth;  // wwidth: bytes of a row of the piece (a multiple of 16)
+    int64_t rows, kbytes, dim;
+    int n;
+    int64_t v0;
+    uint32_t tm, tn;
+    float c;           // log2(e) / T
+    MaskP mask;
+    const int32_t *tokens;
+    // forward
+    float *ref, *sum, *esum;  // [block][rows_p]
+    int64_t rows_p, block0;   // rows padded for those, the piece's first block
+    float *xtok;              // [rows] the token's raw logit
+    // backward
+    const float4 *coef;       // [rows] {lse log2 e (+inf: nothing flows), a, b, the token's term}
+    uint8_t *g;               // [rows, ldg bytes], zeros from n to the row's end
+    int64_t ldg;
+};
+
+template <class T, bool BTR>
+__device__ __forceinline__ Operand weight_rows(const PieceP &p, int in) {
+    const int64_t n0 = int64_t(in) * T::BN;
+    if constexpr (BTR) return Operand{p.w + n0 * 2, p.ldw, p.dim, p.wwidth - n0 * 2};
+    else return Operand{p.w + n0 * p.ldw, p.ldw, p.n - n0, p.kbytes};
+}
+
+template <class E, int TM, int TN, int WM, int WN, bool BTR, bool ENT>
+__global__ __launch_bounds__(256, 1) void k_readout_stats(PieceP p) {
+    typedef Tile<E, TM, TN, WM, WN, false, BTR> T;
+    __shared__ __attribute__((aligned(16))) uint8_t lds[T::kLds];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    int im, in;
+    tile_of(blockIdx.x, p.tm, p.tn, im, in);
+    T t;
+    t.run(lds, Operand{p.h + int64_t(im) * T::BM * p.ldh, p.ldh, p.rows - int64_t(im) * T::BM, p.kbytes},
+          weight_rows<T, BTR>(p, in), p.kbytes, wave, lane);
+    const int wm = wave / WN, wn = wave % WN;
+    const int col0 = in * T::BN + 32 * TN * wn + 4 * (lane / 32);
+    const int64_t block = p.block0 + int64_t(in) * WN + wn;
+#pragma unroll
+    for (int i = 0; i < TM; i++) {
+        const int64_t row = int64_t(im) * T::BM + 32 * (TM * wm + i) + lane % 32;
+        const bool live = row < p.rows;
+        const int64_t r = live ? row : 0;
+        // the token's logit, if it is one of this lane's columns
+        const int64_t tok = p.tokens[r] - p.v0 - col0;
+        if (live && tok >= 0 && tok < 32 * TN && (tok & 4) == 0 && tok + col0 < p.n) {
+            const int tj = int(tok / 32), tv = int(4 * ((tok % 32) / 8) + tok % 4);
+            float x = 0.0f;
+#pragma unroll
+            for (int j = 0; j < TN; j++)
+#pragma unroll
+                for (int v = 0; v < 16; v++)
+                    if (j == tj && v == tv) x = t.acc[i][j][v];
+            p.xtok[row] = x;
+        }
+        float m = -INFINITY;
+#pragma unroll
+        for (int j = 0; j < TN; j++)
+#pragma unroll
+            for (int a = 0; a < 4; a++) {
+                float y[4] = {t.acc[i][j][4 * a], t.acc[i][j][4 * a + 1], t.acc[i][j][4 * a + 2], t.acc[i][j][4 * a + 3]};
+                tempered4(p.mask, r, col0 + 32 * j + 8 * a, p.n, p.c, y);
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    t.acc[i][j][4 * a + e] = y[e];
+                    m = fmaxf(m, y[e]);
+                }
+            }
+        m = fmaxf(m, __shfl_xor(m, 32, 64));
+        const float ref = m == -INFINITY ? 0.0f : m;
+        float s = 0.0f, es = 0.0f;
+#pragma unroll
+        for (int j = 0; j < TN; j++)
+#pragma unroll
+            for (int v = 0; v < 16; v++) {
+                const float d = t.acc[i][j][v] - ref, w = __builtin_amdgcn_exp2f(d);
+                s += w;
+                if constexpr (ENT) es += w > 0.0f ? w * d : 0.0f;
+            }
+        s += __shfl_xor(s, 32, 64);
+        if constexpr (ENT) es += __shfl_xor(es, 32, 64);
+        if (live && lane < 32) {
+            p.ref[block * p.rows_p + row] = m;
+            p.sum[block * p.rows_p + row] = s;
+            if constexpr (ENT) p.esum[block * p.rows_p + row] = es;
+        }
+    }
+}
+
+struct MergeP {
+    const float *ref, *sum, *esum;
+    int64_t rows, rows_p;
+    int blocks;
+    int64_t vocab;
+    const float *xtok;
+    const int32_t *tokens;
+    MaskP mask;
+    double tau;
+    float *logp, *entropy, *base, *rest;
+    uint8_t *status;
+};
+
+// A workgroup joins the blocks of 32 rows, eight threads a row, in f64 and in the same order always.
+__global__ __launch_bounds__(256) void k_readout_merge(MergeP p) {
+    __shared__ float sm[8][32];
+    __shared__ double ss[8][32], st[8][32];
+    const int lr = threadIdx.x % 32, seg = threadIdx.x / 32;
+    const int64_t row = int64_t(blockIdx.x) * 32 + lr;
+    const bool live = row < p.rows;
+    float m = -INFINITY;
+    if (live)
+        for (int b = seg; b < p.blocks; b += 8) m = fmaxf(m, p.ref[b * p.rows_p + row]);
+    sm[seg][lr] = m;
+    __syncthreads();
+    for (int k = 0; k < 8; k++) m = fmaxf(m, sm[k][lr]);
+    double s = 0.0, t = 0.0;
+    if (live && m > -INFINITY)
+        for (int b = seg; b < p.blocks; b += 8) {
+            const float r = p.ref[b * p.rows_p + row];
+            // (a block with nothing allowed has ref -inf and sum 0; with a NaN in it, sum NaN)
+            const double d = double(r) - double(m);
+            const float q = p.sum[b * p.rows_p + row];
+            if (r == -INFINITY && q == 0.0f) continue;
+            const double f = exp2(d);
+            s += f * double(q);
+            if (p.esum) t += f * (double(p.esum[b * p.rows_p + row]) + d * double(q));
+        }
+    else if (live)  // no maximum: NaNs alone leave sums that are NaN
+        for (int b = seg; b < p.blocks; b += 8) s += double(p.sum[b * p.rows_p + row]);
+    ss[seg][lr] = s;
+    st[seg][lr] = t;
+    __syncthreads();
+    if (seg != 0 || !live) return;
+    s = t = 0.0;
+    for (int k = 0; k < 8; k++) s += ss[k][lr], t += st[k][lr];
+    const int64_t tok = p.tokens[row];
+    const bool bad = tok < 0 || tok >= p.vocab;
+    const bool none = m == -INFINITY && s == 0.0;
+    const bool ok = !none && s > 0.0 && s < INFINITY && m < INFINITY;
+    uint8_t status = ok ? NT_ROW_OK : (none ? NT_ROW_NO_TOKEN : NT_ROW_NAN);
+    const double lse2 = double(m) + log2(s), lse = lse2 * kLn2;
+    float base = float(double(m) * kLn2);
+    if (p.base) p.base[row] = ok ? base : (none ? -INFINITY : NAN);
+    if (p.rest) p.rest[row] = ok ? float(lse - double(base)) : (none ? 0.0f : NAN);
+    if (p.entropy) p.entropy[row] = ok ? float(kLn2 * (log2(s) - t / s)) : NAN;
+    float lp = NAN;
+    if (ok && !bad) {
+        double z = double(p.xtok[row]) / p.tau;
+        if (p.mask.u8 && !p.mask.u8[row * p.mask.ld + tok]) z = -INFINITY;
+        else if (p.mask.f32) z += double(p.mask.f32[row * p.mask.ld + tok]);
+        lp = float(z - lse);
+    }
+    p.logp[row] = lp;
+    if (ok && bad) status = NT_ROW_BAD_TOKEN;
+    p.status[row] = status;
+}
+
+// ---------------------------------------------------------------------------------- backward
+
+struct CoefP {
+    const float *base, *rest, *entropy, *g_logp, *g_entropy;
+    const int32_t *tokens;
+    int64_t rows, vocab;
+    double tau;
+    int f16;
+    float4 *coef;
+    float *up;     // [rows] f16: what a row of G was divided by
+    float *top;    // [1] f16: the largest of them
+};
+
+// What a row's upstream gradients make of it (one workgroup: the largest row's scale is a maximum over all).
+__global__ __launch_bounds__(1024) void k_readout_coef(CoefP p) {
+    __shared__ float s_top[16];
+    float top = 0.0f;
+    for (int64_t r = threadIdx.x; r < p.rows; r += 1024) {
+        const int64_t tok = p.tokens[r];
+        double gl = p.g_logp ? double(p.g_logp[r]) : 0.0;
+        if (tok < 0 || tok >= p.vocab) gl = 0.0;
+        const double ge = p.g_entropy ? double(p.g_entropy[r]) : 0.0;
+        const double h = p.g_entropy ? double(p.entropy[r]) : 0.0;
+        const double lse = double(p.base[r]) + double(p.rest[r]);
+        const bool dead = (gl == 0.0 && ge == 0.0) || lse == -INFINITY;
+        double unit = 1.0;  // f16: G's unit, a power of two
+        float up = 0.0f;
+        if (p.f16 && !dead) {
+            const double size = fabs(gl) + 16.0 * fabs(ge);
+            int e = 0;
+            if (size > 0.0 && size < INFINITY) {
+                (void)frexp(size, &e);  // size < 2^e
+                e = e < -126 ? -126 : (e > 127 ? 127 : e);
+            }
+            up = ldexpf(1.0f, e);
+            unit = ldexp(1.0, 14 - e);
+            top = fmaxf(top, up);
+        } else if (!p.f16) {
+            unit = 1.0 / p.tau;
+        }
+        if (p.f16) p.up[r] = up;
+        const float a = float(-(gl + ge * h) * unit), b = float(-ge * kLn2 * unit);
+        p.coef[r] = dead ? float4{INFINITY, 0.0f, 0.0f, 0.0f} : float4{float(lse * kLog2eD), a, b, float(gl * unit)};
+    }
+    if (!p.f16) return;
+#pragma unroll
+    for (int d = 32; d; d /= 2) top = fmaxf(top, __shfl_xor(top, d, 64));
+    if (threadIdx.x % 64 == 0) s_top[threadIdx.x / 64] = top;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        for (int k = 1; k < 16; k++) top = fmaxf(top, s_top[k]);
+        *p.top = top == 0.0f ? 1.0f : top;
+    }
+}
+
+// Rows of 16-bit values into rows of `ldo` bytes, zeros from `cols` to their end: an operand that is not laid
+// out as the copies need it. With `coef`, the rows that nothing flows through are zeros (whatever they hold, a
+// NaN too, stays out of dW) and with `up`, f16 rows are scaled by up / top, a power of two.
+__global__ __launch_bounds__(256) void k_readout_rows(const uint16_t *src, int64_t rows, int64_t cols, int64_t ld,
+                                                      uint8_t *out, int64_t ldo, const float4 *coef, const float *up,
+                                                      const float *top) {
+    const int64_t per = ldo / 16, total = rows * per;
+    for (int64_t i = blockIdx.x * int64_t(256) + threadIdx.x; i < total; i += int64_t(gridDim.x) * 256) {
+        const int64_t r = i / per, c = (i - r * per) * 8;
+        const uint16_t *s = src + r * ld + c;
+        union {
+            u32x4 v;
+            uint16_t h[8];
+            _Float16 f[8];
+        } x;
+        x.v = u32x4{0, 0, 0, 0};
+        if (!coef || coef[r].x != INFINITY) {
+            if (c + 8 <= cols) x.v = *reinterpret_cast<const u32x4u *>(s);
+            else
+                for (int e = 0; e < 8; e++) x.h[e] = c + e < cols ? s[e] : uint16_t(0);
+            if (up) {
+                const float f = up[r] / *top;
+#pragma unroll
+                for (int e = 0; e < 8; e++) x.f[e] = _Float16(float(x.f[e]) * f);
+            }
+        }
+        *reinterpret_cast<u32x4 *>(out + r * ldo + c * 2) = x.v;
+    }
+}
+
+template <class E, int TM, int TN, int WM, int WN, bool BTR>
+__global__ __launch_bounds__(256, 1) void k_readout_g(PieceP p) {
+    typedef Tile<E, TM, TN, WM, WN, false, BTR> T;
+    __shared__ __attribute__((aligned(16))) uint8_t lds[T::kLds];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    int im, in;
+    tile_of(blockIdx.x, p.tm, p.tn, im, in);
+    T t;
+    t.run(lds, Operand{p.h + int64_t(im) * T::BM * p.ldh, p.ldh, p.rows - int64_t(im) * T::BM, p.kbytes},
+          weight_rows<T, BTR>(p, in), p.kbytes, wave, lane);
+    const int wm = wave / WN, wn = wave % WN;
+    const int col0 = in * T::BN + 32 * TN * wn + 4 * (lane / 32);
+    const int ncol = int(p.ldg / 2);
+#pragma unroll
+    for (int i = 0; i < TM; i++) {
+        const int64_t row = int64_t(im) * T::BM + 32 * (TM * wm + i) + lane % 32;
+        if (row >= p.rows) continue;
+        const float4 k = p.coef[row];
+        const int64_t tok64 = p.tokens[row] - p.v0;
+        const int tok = tok64 >= 0 && tok64 < p.n ? int(tok64) : -1;
+        const bool dead = k.x == INFINITY;
+#pragma unroll
+        for (int j = 0; j < TN; j++)
+#pragma unroll
+            for (int a = 0; a < 4; a++) {
+                const int col = col0 + 32 * j + 8 * a;
+                float y[4] = {t.acc[i][j][4 * a], t.acc[i][j][4 * a + 1], t.acc[i][j][4 * a + 2], t.acc[i][j][4 * a + 3]};
+                tempered4(p.mask, row, col, p.n, p.c, y);
+                float g[4];
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    const float lp = y[e] - k.x, pr = __builtin_amdgcn_exp2f(lp);  // log2 p, p
+                    g[e] = pr == 0.0f ? 0.0f : pr * fmaf(k.z, lp, k.y);
+                    if (col + e == tok) g[e] += k.w;
+                    g[e] = dead || col + e >= p.n ? 0.0f : g[e];
+                }
+                if (col < ncol)
+                    *reinterpret_cast<u32x2 *>(p.g + row * p.ldg + col * 2) = u32x2{pair16<E>(g[0], g[1]), pair16<E>(g[2], g[3])};
+            }
+    }
+}
+
+// C[m, n] = sum_k A(m, k) B(n, k) over the k of split z: into the gradient itself (16-bit, scaled), or into
+// the split's f32 slab, set or added to.
+struct GradP {
+    const uint8_t *a, *b;
+    int64_t lda, ldb, wa, wb; // strides, and bytes of a row of a transposed operand (a multiple of 16)
+    int64_t m, n, k;          // k in elements (a k-contiguous operand's row is padded with zeros to 16 bytes)
+    int64_t per;              // k of a split, a multiple of 32
+    uint32_t tm, tn;
+    uint16_t *out;            // [m, ldo] or null
+    int64_t ldo;
+    float *slab;              // [splits][m][n] f32
+    int add;
+    const float *row_scale;   // f16: [m] or null
+    const float *scale;       // f16: [1] or null
+    float fixed;
+};
+
+template <class E>
+__device__ __forceinline__ void store4(uint16_t *o, const float (&x)[4], int have) {
+    const u32x2 v = {pair16<E>(x[0], x[1]), pair16<E>(x[2], x[3])};
+    if (have >= 4) {
+        __builtin_memcpy(o, &v, 8);
+        return;
+    }
+    const uint32_t w[2] = {v.x, v.y};
+    for (int e = 0; e < have; e++) o[e] = uint16_t(w[e / 2] >> (16 * (e % 2)));
+}
+
+template <class E, int TM, int TN, int WM, int WN, bool ATR, bool BTR>
+__global__ __launch_bounds__(256, 1) void k_readout_grad(GradP p) {
+    typedef Tile<E, TM, TN, WM, WN, ATR, BTR> T;
+    __shared__ __attribute__((aligned(16))) uint8_t lds[T::kLds];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    int im, in;
+    tile_of(blockIdx.x, p.tm, p.tn, im, in);
+    const int64_t k0 = blockIdx.y * p.per, left = p.k - k0 < p.per ? p.k - k0 : p.per;
+    const int64_t kn = left > 0 ? left : 0;  // (a shorter last piece may leave a split nothing: zeros)
+    const int64_t m0 = int64_t(im) * T::BM, n0 = int64_t(in) * T::BN;
+    const int64_t kb = (kn * 2 + 15) / 16 * 16;
+    const Operand a = ATR ? Operand{p.a + k0 * p.lda + m0 * 2, p.lda, kn, p.wa - m0 * 2}
+                          : Operand{p.a + m0 * p.lda + k0 * 2, p.lda, p.m - m0, kb};
+    const Operand b = BTR ? Operand{p.b + k0 * p.ldb + n0 * 2, p.ldb, kn, p.wb - n0 * 2}
+                          : Operand{p.b + n0 * p.ldb + k0 * 2, p.ldb, p.n - n0, kb};
+    T t;
+    t.run(lds, a, b, kb, wave, lane);
+    const int wm = wave / WN, wn = wave % WN;
+    const float whole = p.scale ? *p.scale * p.fixed : p.fixed;
+#pragma unroll
+    for (int i = 0; i < TM; i++) {
+        const int64_t row = m0 + 32 * (TM * wm + i) + lane % 32;
+        if (row >= p.m) continue;
+        const float f = p.row_scale ? p.row_scale[row] * whole : whole;
+#pragma unroll
+        for (int j = 0; j < TN; j++)
+#pragma unroll
+            for (int q = 0; q < 4; q++) {
+                const int64_t col = n0 + 32 * (TN * wn + j) + 8 * q + 4 * (lane / 32);
+                const int have = p.n - col >= 4 ? 4 : int(p.n - col);
+                if (have <= 0) continue;
+                float x[4] = {t.acc[i][j][4 * q], t.acc[i][j][4 * q + 1], t.acc[i][j][4 * q + 2], t.acc[i][j][4 * q + 3]};
+                if (p.out) {
+#pragma unroll
+                    for (int e = 0; e < 4; e++) x[e] *= f;
+                    store4<E>(p.out + row * p.ldo + col, x, have);
+                } else {
+                    float *o = p.slab + (int64_t(blockIdx.y) * p.m + row) * p.n + col;
+                    if (have == 4) {
+                        float c[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+                        if (p.add) __builtin_memcpy(c, o, 16);
+#pragma unroll
+                        for (int e = 0; e < 4; e++) c[e] += x[e];
+                        __builtin_memcpy(o, c, 16);
+                    } else {
+                        for (int e = 0; e < have; e++) o[e] = (p.add ? o[e] : 0.0f) + x[e];
+                    }
+                }
+            }
+    }
+}
+
+// The slabs' sum in their order, scaled and rounded.
+template <class E>
+__global__ __launch_bounds__(256) void k_readout_fold(const float *slab, int splits, int64_t m, int64_t n, uint16_t *out,
+                                                      int64_t ldo, const float *row_scale, const float *scale, float fixed) {
+    const int64_t per = (n + 3) / 4, total = m * per;
+    for (int64_t i = blockIdx.x * int64_t(256) + threadIdx.x; i < total; i += int64_t(gridDim.x) * 256) {
+        const int64_t r = i / per, c = (i - r * per) * 4;
+        const int have = n - c >= 4 ? 4 : int(n - c);
+        float x[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+        for (int z = 0; z < splits; z++) {
+            const float *s = slab + (z * m + r) * n + c;
+            float v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+            if (have == 4) __builtin_memcpy(v, s, 16);
+            else
+                for (int e = 0; e < have; e++) v[e] = s[e];
+#pragma unroll
+            for (int e = 0; e < 4; e++) x[e] += v[e];
+        }
+        float f = scale ? *scale * fixed : fixed;
+        if (row_scale) f *= row_scale[r];
+#pragma unroll
+        for (int e = 0; e < 4; e++) x[e] *= f;
+        store4<E>(out + r * ldo + c, x, have);
+    }
+}
+
+// ---------------------------------------------------------------------------------- host
+
+int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
+int64_t round_up(int64_t a, int64_t b) { return ceil_div(a, b) * b; }
+
+// Scratch of one call, cut from one allocation: sizes are asked for first, then the places.
+struct Scratch {
+    size_t need = 0;
+    uint8_t *base = nullptr;
+    size_t add(int64_t bytes) {
+        const size_t at = need;
+        need += (size_t(bytes) + 255) & ~size_t(255);
+        return at;
+    }
+    template <class P>
+    P *at(size_t o) const {
+        return reinterpret_cast<P *>(base + o);
+    }
+    ~Scratch() {
+        if (base) (void)scratch_release(base);
+    }
+};
+
+constexpr int64_t kMaxDim = 65536, kMaxVocab = 1 << 20, kMaxRows = 1 << 24;
+
+// What both entries check of the operands. `dv`: the weight is [dim, vocab].
+int check(const char *who, const void *hidden, const void *weight, int32_t dtype, int32_t layout, int64_t rows, int64_t vocab,
+          int64_t dim, int64_t ldh, int64_t ldw, int32_t mask_kind, const void *mask, int64_t mask_ld, double tau,
+          const int32_t *tokens) {
+    if (dtype != NT_BF16 && dtype != NT_F16)
+        return fail(NT_E_ARG, std::string(who) + ": dtype " + std::to_string(dtype) + " (NT_BF16 or NT_F16)");
+    if (layout != NT_READOUT_W_DV && layout != NT_READOUT_W_VD)
+        return fail(NT_E_ARG, std::string(who) + ": layout " + std::to_string(layout) + " (NT_READOUT_W_DV or _VD)");
+    const int64_t wrow = layout == NT_READOUT_W_DV ? vocab : dim;
+    if (rows < 0 || rows > kMaxRows || vocab < 1 || vocab > kMaxVocab || dim < 1 || dim > kMaxDim || ldh < dim || ldw < wrow ||
+        ldh > (int64_t(1) << 21) || ldw > (int64_t(1) << 21))
+        return fail(NT_E_ARG, std::string(who) + ": rows " + std::to_string(rows) + " (at most 2^24), vocab " +
+                                  std::to_string(vocab) + " (1 to 2^20), dim " + std::to_string(dim) +
+                                  " (1 to 65536), ldh " + std::to_string(ldh) + ", ldw " + std::to_string(ldw) +
+                                  " (at least the row, at most 2^21)");
+    if (mask_kind != NT_MASK_NONE && mask_kind != NT_MASK_U8 && mask_kind != NT_MASK_F32)
+        return fail(NT_E_ARG, std::string(who) + ": mask kind " + std::to_string(mask_kind));
+    if ((mask_kind == NT_MASK_NONE) != (mask == nullptr))
+        return fail(NT_E_ARG, std::string(who) + ": mask kind and mask pointer disagree");
+    if (mask && mask_ld != 0 && mask_ld < vocab)
+        return fail(NT_E_ARG, std::string(who) + ": mask_ld " + std::to_string(mask_ld) + " (0, or at least vocab)");
+    if (mask_kind == NT_MASK_F32 && reinterpret_cast<uintptr_t>(mask) % 4)
+        return fail(NT_E_ARG, std::string(who) + ": unaligned mask");
+    if (!(tau > 0.0) || !std::isfinite(tau) || !(float(kLog2eD / tau) > 0.0f) || std::isinf(float(kLog2eD / tau)))
+        return fail(NT_E_ARG, "tempered_logits: temperature " + std::to_string(tau) + " (must be positive)");
+    if (rows > 0 && (!hidden || !weight || !tokens || reinterpret_cast<uintptr_t>(hidden) % 2 ||
+                     reinterpret_cast<uintptr_t>(weight) % 2))
+        return fail(NT_E_ARG, std::string(who) + ": null or unaligned hidden or weight, or null tokens");
+    return 0;
+}
+
+bool aligned(const void *p, int64_t cols, int64_t ld) {
+    return reinterpret_cast<uintptr_t>(p) % 16 == 0 && ld % 8 == 0 && cols % 8 == 0;
+}
+
+int copy_rows(const void *src, int64_t rows, int64_t cols, int64_t ld, uint8_t *out, int64_t ldo, const float4 *coef,
+              const float *up, const float *top) {
+    const int64_t n = rows * (ldo / 16);
+    hipLaunchKernelGGL(k_readout_rows, dim3(unsigned(std::min<int64_t>(ceil_div(n, 256), 8192))), dim3(256), 0,
+                       ctx().stream, static_cast<const uint16_t *>(src), rows, cols, ld, out, ldo, coef, up, top);
+    return launched("k_readout_rows");
+}
+
+// A piece of the weight as the copies need it: in place, or copied into `buf` where it is not aligned.
+int piece_weight(const void *weight, bool dv, bool direct, int64_t v0, int64_t n, int64_t dim, int64_t ldw, uint8_t *buf,
+                 PieceP *p) {
+    const uint16_t *s = static_cast<const uint16_t *>(weight) + (dv ? v0 : v0 * ldw);
+    p->wwidth = round_up(dv ? n : dim, 8) * 2;
+    if (direct) {
+        p->w = reinterpret_cast<const uint8_t *>(s);
+        p->ldw = ldw * 2;
+        return 0;
+    }
+    p->w = buf;
+    p->ldw = p->wwidth;
+    return copy_rows(s, dv ? dim : n, dv ? n : dim, ldw, buf, p->ldw, nullptr, nullptr, nullptr);
+}
+
+MaskP mask_at(int32_t kind, const void *mask, int64_t ld, int64_t v0) {
+    MaskP m{nullptr, nullptr, ld};
+    if (kind == NT_MASK_U8) m.u8 = static_cast<const uint8_t *>(mask) + v0;
+    if (kind == NT_MASK_F32) m.f32 = static_cast<const float *>(mask) + v0;
+    return m;
+}
+
+constexpr int kBlockCols = 128;  // columns of a forward block: a wave's of a 256-column tile
+constexpr int kTile = 256;
+
+// The vocabulary's pieces: whole tiles, `cols` of them at most.
+int64_t piece_cols(int64_t vocab, int64_t cols) {
+    const int64_t most = std::max<int64_t>(kTile, cols / kTile * kTile);
+    const int64_t pieces = ceil_div(vocab, most);
+    return std::min(round_up(ceil_div(vocab, pieces), kTile), round_up(vocab, kTile));
+}
+
+template <class E, bool BTR>
+int launch_stats(const PieceP &p, bool ent) {
+    const dim3 grid(p.tm * p.tn), block(256);
+    if (ent) k_readout_stats<E, 4, 4, 2, 2, BTR, true><<<grid, block, 0, ctx().stream>>>(p);
+    else k_readout_stats<E, 4, 4, 2, 2, BTR, false><<<grid, block, 0, ctx().stream>>>(p);
+    return launched("k_readout_stats");
+}
+
+int forward(const NtRlReadoutStatsArgs *a) {
+    const bool dv = a->layout == NT_READOUT_W_DV;
+    const int64_t R = a->rows, V = a->vocab, d = a->dim, kp = round_up(d, 8);
+    const bool hdirect = aligned(a->hidden, d, a->ldh);
+    const bool wdirect = aligned(a->weight, dv ? V : d, a->ldw);
+    // one launch for the whole vocabulary, but for a copied weight (pieces of 256 MiB) and more than 2^23 tiles
+    int64_t most = (int64_t(1) << 23) / ceil_div(R, kTile) * kTile;
+    if (!wdirect) most = std::min(most, (int64_t(1) << 27) / kp);
+    const int64_t cols = piece_cols(V, most);
+    const int64_t blocks = ceil_div(V, kTile) * 2, rows_p = round_up(R, 32);
+    Scratch s;
+    const size_t o_h = s.add(hdirect ? 0 : R * kp * 2);
+    const size_t o_w = s.add(wdirect ? 0 : (dv ? d * cols : cols * kp) * 2);
+    const size_t o_ref = s.add(blocks * rows_p * 4), o_sum = s.add(blocks * rows_p * 4);
+    const size_t o_es = s.add(a->entropy ? blocks * rows_p * 4 : 0), o_x = s.add(R * 4);
+    void *ws = nullptr;
+    if (int rc = scratch_alloc(s.need, &ws)) return rc;
+    s.base = static_cast<uint8_t *>(ws);
+    PieceP p{};
+    p.h = static_cast<const uint8_t *>(a->hidden);
+    p.ldh = a->ldh * 2;
+    if (!hdirect) {
+        if (int rc = copy_rows(a->hidden, R, d, a->ldh, s.at<uint8_t>(o_h), kp * 2, nullptr, nullptr, nullptr)) return rc;
+        p.h = s.at<uint8_t>(o_h);
+        p.ldh = kp * 2;
+    }
+    p.rows = R;
+    p.dim = d;
+    p.kbytes = kp * 2;
+    p.c = float(kLog2eD / a->temperature);
+    p.tokens = a->tokens;
+    p.ref = s.at<float>(o_ref);
+    p.sum = s.at<float>(o_sum);
+    p.esum = a->entropy ? s.at<float>(o_es) : nullptr;
+    p.rows_p = rows_p;
+    p.xtok = s.at<float>(o_x);
+    for (int64_t v0 = 0; v0 < V; v0 += cols) {
+        const int64_t n = std::min(cols, V - v0);
+        if (int rc = piece_weight(a->weight, dv, wdirect, v0, n, d, a->ldw, s.at<uint8_t>(o_w), &p)) return rc;
+        p.n = int(n);
+        p.v0 = v0;
+        p.block0 = v0 / kBlockCols;
+        p.mask = mask_at(a->mask_kind, a->mask, a->mask_ld, v0);
+        p.tm = uint32_t(ceil_div(R, kTile));
+        p.tn = uint32_t(ceil_div(n, kTile));
+        const bool bf16 = a->dtype == NT_BF16, ent = a->entropy != nullptr;
+        const int rc = dv ? (bf16 ? launch_stats<Bf16, true>(p, ent) : launch_stats<F16, true>(p, ent))
+                          : (bf16 ? launch_stats<Bf16, false>(p, ent) : launch_stats<F16, false>(p, ent));
+        if (rc) return rc;
+    }
+    MergeP q{};
+    q.ref = p.ref;
+    q.sum = p.sum;
+    q.esum = p.esum;
+    q.rows = R;
+    q.rows_p = rows_p;
+    q.blocks = int(blocks);
+    q.vocab = V;
+    q.xtok = p.xtok;
+    q.tokens = a->tokens;
+    q.mask = mask_at(a->mask_kind, a->mask, a->mask_ld, 0);
+    q.tau = a->temperature;
+    q.logp = a->logp;
+    q.entropy = a->entropy;
+    q.base = a->lse_base;
+    q.rest = a->lse_rest;
+    q.status = a->status;
+    hipLaunchKernelGGL(k_readout_merge, dim3(unsigned(ceil_div(R, 32))), dim3(256), 0, ctx().stream, q);
+    return launched("k_readout_merge");
+}
+
+// One product of the backward: tiles, and splits of k where the tiles alone leave CUs idle.
+struct Split {
+    int64_t per, splits;
+};
+Split split_k(int64_t m, int64_t n, int64_t k) {
+    const int64_t tiles = ceil_div(m, kTile) * ceil_div(n, kTile);
+    const int64_t want = std::min(std::max<int64_t>(1, 256 / tiles), std::max<int64_t>(1, k / 256));
+    const int64_t per = round_up(ceil_div(k, want), 32);
+    return Split{per, ceil_div(k, per)};
+}
+
+template <class E>
+int fold(const GradP &p, int64_t splits, uint16_t *out) {
+    const int64_t n = p.m * ceil_div(p.n, 4);
+    hipLaunchKernelGGL(k_readout_fold<E>, dim3(unsigned(std::min<int64_t>(ceil_div(n, 256), 8192))), dim3(256), 0,
+                       ctx().stream, p.slab, int(splits), p.m, p.n, out, p.ldo, p.row_scale, p.scale, p.fixed);
+    return launched("k_readout_fold");
+}
+
+template <class E, bool ATR, bool BTR>
+int product(GradP p, const Split &s) {
+    p.per = s.per;
+    p.tm = uint32_t(ceil_div(p.m, kTile));
+    p.tn = uint32_t(ceil_div(p.n, kTile));
+    hipLaunchKernelGGL((k_readout_grad<E, 4, 4, 2, 2, ATR, BTR>), dim3(p.tm * p.tn, unsigned(s.splits)), dim3(256), 0,
+                       ctx().stream, p);
+    return launched("k_readout_grad");
+}
+
+// One piece of the vocabulary: its G, its rows of dW, its share of dH.
+struct BackP {
+    const NtRlReadoutStatsGradArgs *a;
+    PieceP p;
+    Split sh, sw;
+    bool hslab;
+    const uint8_t *hs;  // the scaled hidden states, [rows, ldhs bytes]
+    int64_t ldhs;
+    float *slab_h, *slab_w;
+    const float *up, *top;
+    float fixed;
+    bool last;
+};
+
+template <class E, bool DV>
+int piece(const BackP &b) {
+    const NtRlReadoutStatsGradArgs *a = b.a;
+    const PieceP &p = b.p;
+    k_readout_g<E, 4, 4, 2, 2, DV><<<dim3(p.tm * p.tn), dim3(256), 0, ctx().stream>>>(p);
+    if (int rc = launched("k_readout_g")) return rc;
+    if (a->grad_weight) {
+        GradP w{};
+        w.a = DV ? b.hs : p.g;
+        w.lda = w.wa = DV ? b.ldhs : p.ldg;
+        w.b = DV ? p.g : b.hs;
+        w.ldb = w.wb = DV ? p.ldg : b.ldhs;
+        w.m = DV ? p.dim : p.n;
+        w.n = DV ? p.n : p.dim;
+        w.k = p.rows;
+        uint16_t *out = static_cast<uint16_t *>(a->grad_weight) + (DV ? p.v0 : p.v0 * a->grad_weight_ld);
+        w.ldo = a->grad_weight_ld;
+        w.out = b.sw.splits > 1 ? nullptr : out;
+        w.slab = b.slab_w;
+        w.scale = b.top;
+        w.fixed = b.fixed;
+        if (int rc = product<E, true, true>(w, b.sw)) return rc;
+        if (b.sw.splits > 1)
+            if (int rc = fold<E>(w, b.sw.splits, out)) return rc;
+    }
+    if (a->grad_hidden) {
+        GradP h{};
+        h.a = p.g;
+        h.lda = p.ldg;
+        h.b = p.w;
+        h.ldb = p.ldw;
+        h.wb = p.wwidth;
+        h.m = p.rows;
+        h.n = p.dim;
+        h.k = p.n;
+        h.ldo = a->grad_hidden_ld;
+        uint16_t *out = static_cast<uint16_t *>(a->grad_hidden);
+        h.out = b.hslab ? nullptr : out;
+        h.slab = b.slab_h;
+        h.add = p.v0 > 0;
+        h.row_scale = b.up;
+        h.fixed = b.fixed;
+        if (int rc = product<E, false, !DV>(h, b.sh)) return rc;
+        if (b.hslab && b.last)
+            if (int rc = fold<E>(h, b.sh.splits, out)) return rc;
+    }
+    return 0;
+}
+
+int backward(const NtRlReadoutStatsGradArgs *a) {
+    const bool dv = a->layout == NT_READOUT_W_DV, f16 = a->dtype == NT_F16;
+    const int64_t R = a->rows, V = a->vocab, d = a->dim, kp = round_up(d, 8);
+    if (R == 0) {  // a sum over no rows
+        GradP w{};
+        w.m = dv ? d : V;
+        w.n = dv ? V : d;
+        w.ldo = a->grad_weight_ld;
+        return a->grad_weight ? fold<Bf16>(w, 0, static_cast<uint16_t *>(a->grad_weight)) : 0;
+    }
+    const bool hdirect = aligned(a->hidden, d, a->ldh);
+    const bool wdirect = aligned(a->weight, dv ? V : d, a->ldw);
+    // G of a piece takes at most 512 MiB (a copied piece of the weight 256 MiB)
+    int64_t most = (int64_t(1) << 28) / R;
+    if (!wdirect) most = std::min(most, (int64_t(1) << 27) / kp);
+    const int64_t cols = piece_cols(V, most), pieces = ceil_div(V, cols);
+    // dH: [rows, dim], k the piece's columns; dW: [vocab, dim] or [dim, vocab], k the rows
+    const Split sh = split_k(R, d, round_up(std::min(cols, V), 8));
+    const Split sw = dv ? split_k(d, std::min(cols, V), R) : split_k(std::min(cols, V), d, R);
+    const bool hslab = sh.splits > 1 || pieces > 1;
+    Scratch s;
+    const size_t o_h = s.add(hdirect ? 0 : R * kp * 2), o_hs = s.add(R * kp * 2);
+    const size_t o_w = s.add(wdirect ? 0 : (dv ? d * cols : cols * kp) * 2);
+    const size_t o_coef = s.add(R * 16), o_up = s.add(R * 4), o_top = s.add(4);
+    const size_t o_g = s.add(R * cols * 2);
+    const size_t o_sh = s.add(a->grad_hidden && hslab ? sh.splits * R * d * 4 : 0);
+    const size_t o_sw = s.add(a->grad_weight && sw.splits > 1 ? sw.splits * std::min(cols, V) * d * 4 : 0);
+    void *ws = nullptr;
+    if (int rc = scratch_alloc(s.need, &ws)) return rc;
+    s.base = static_cast<uint8_t *>(ws);
+    const float *up = f16 ? s.at<float>(o_up) : nullptr, *top = f16 ? s.at<float>(o_top) : nullptr;
+    const float fixed = f16 ? float(ldexp(1.0, -14) / a->temperature) : 1.0f;
+    CoefP c{};
+    c.base = a->lse_base;
+    c.rest = a->lse_rest;
+    c.entropy = a->entropy;
+    c.g_logp = a->g_logp;
+    c.g_entropy = a->g_entropy;
+    c.tokens = a->tokens;
+    c.rows = R;
+    c.vocab = V;
+    c.tau = a->temperature;
+    c.f16 = f16;
+    c.coef = s.at<float4>(o_coef);
+    c.up = s.at<float>(o_up);
+    c.top = s.at<float>(o_top);
+    hipLaunchKernelGGL(k_readout_coef, dim3(1), dim3(1024), 0, ctx().stream, c);
+    if (int rc = launched("k_readout_coef")) return rc;
+    if (a->grad_weight)
+        if (int rc = copy_rows(a->hidden, R, d, a->ldh, s.at<uint8_t>(o_hs), kp * 2, c.coef, up, top)) return rc;
+    PieceP p{};
+    p.h = static_cast<const uint8_t *>(a->hidden);
+    p.ldh = a->ldh * 2;
+    if (!hdirect) {
+        if (int rc = copy_rows(a->hidden, R, d, a->ldh, s.at<uint8_t>(o_h), kp * 2, nullptr, nullptr, nullptr)) return rc;
+        p.h = s.at<uint8_t>(o_h);
+        p.ldh = kp * 2;
+    }
+    p.rows = R;
+    p.dim = d;
+    p.kbytes = kp * 2;
+    p.c = float(kLog2eD / a->temperature);
+    p.tokens = a->tokens;
+    p.coef = c.coef;
+    p.g = s.at<uint8_t>(o_g);
+    for (int64_t v0 = 0; v0 < V; v0 += cols) {
+        const int64_t n = std::min(cols, V - v0);
+        if (int rc = piece_weight(a->weight, dv, wdirect, v0, n, d, a->ldw, s.at<uint8_t>(o_w), &p)) return rc;
+        p.n = int(n);
+        p.v0 = v0;
+        p.ldg = round_up(n, 8) * 2;
+        p.mask = mask_at(a->mask_kind, a->mask, a->mask_ld, v0);
+        p.tm = uint32_t(ceil_div(R, kTile));
+        p.tn = uint32_t(ceil_div(n, kTile));
+        BackP b{a, p, sh, sw, hslab, s.at<uint8_t>(o_hs), kp * 2, s.at<float>(o_sh), s.at<float>(o_sw), up, top, fixed,
+                v0 + cols >= V};
+        const int rc = dv ? (f16 ? piece<F16, true>(b) : piece<Bf16, true>(b)) : (f16 ? piece<F16, false>(b) : piece<Bf16, false>(b));
+        if (rc) return rc;
+    }
+    return 0;
+}
+
+}  // namespace
+}  // namespace nt
+
+using namespace nt;
+
+extern "C" int nt_hip_rl_readout_score_stats(const NtRlReadoutStatsArgs *a) {
+    const char *who = "nt_hip_rl_readout_score_stats";
+    if (!a) return fail(NT_E_ARG, std::string(who) + ": null args");
+    if (int rc = check(who, a->hidden, a->weight, a->dtype, a->layout, a->rows, a->vocab, a->dim, a->ldh, a->ldw, a->mask_kind,
+                       a->mask, a->mask_ld, a->temperature, a->tokens))
+        return rc;
+    if (a->rows > 0 && (!a->logp || !a->status)) return fail(NT_E_ARG, std::string(who) + ": null logp or status");
+    std::unique_lock<std::mutex> lk;
+    if (int rc = enter(&lk)) return rc;
+    return a->rows == 0 ? 0 : forward(a);
+}
+
+extern "C" int nt_hip_rl_readout_score_backward(const NtRlReadoutStatsGradArgs *a) {
+    const char *who = "nt_hip_rl_readout_score_backward";
+    if (!a) return fail(NT_E_ARG, std::string(who) + ": null args");
+    if (int rc = check(who, a->hidden, a->weight, a->dtype, a->layout, a->rows, a->vocab, a->dim, a->ldh, a->ldw, a->mask_kind,
+                       a->mask, a->mask_ld, a->temperature, a->tokens))
+        return rc;
+    if (!a->grad_hidden && !a->grad_weight) return fail(NT_E_ARG, std::string(who) + ": no gradient asked for");
+    const int64_t wrow = a->layout == NT_READOUT_W_DV ? a->vocab : a->dim;
+    if ((a->grad_hidden && (a->grad_hidden_ld < a->dim || reinterpret_cast<uintptr_t>(a->grad_hidden) % 2)) ||
+        (a->grad_weight && (a->grad_weight_ld < wrow || reinterpret_cast<uintptr_t>(a->grad_weight) % 2)))
+        return fail(NT_E_ARG, std::string(who) + ": a gradient's row stride is under its row, or it is unaligned");
+    if (a->rows > 0 && (!a->lse_base || !a->lse_rest || (a->g_entropy && !a->entropy)))
+        return fail(NT_E_ARG, std::string(who) + ": null lse_base or lse_rest, or g_entropy without the entropy");
+    std::unique_lock<std::mutex> lk;
+    if (int rc = enter(&lk)) return rc;
+    return backward(a);
+}

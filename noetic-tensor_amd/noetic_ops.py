@@ -364,6 +364,56 @@ def matmul(a: Tensor, al: Layout, b: Tensor, bl: Layout,
     return y, shape
 
 
+def quantize_int8(x: Tensor, xl: Layout) -> Tuple[Tensor, Tensor]:
+    """Rows of a view (its last dimension; `swapped` for columns) in 8 bits: (q, scale), q = round(x / scale) of
+    the exact quotient, ties to even, over the view's shape, scale = max |x| / 127 in f32 over its leading
+    dimensions. A row with a NaN or an infinity has scale NaN; one of zeros scale 0."""
+    if x.dtype not in ("f32", "bf16", "f16"):
+        raise TypeError(f"quantize_int8 of {x.dtype} storage (f32, bf16 or f16)")
+    if not xl.shape:
+        raise ValueError("quantize_int8: a view of rank 1 or more")
+    _inside(x, xl, "quantize_int8")
+    q, scale = Tensor(xl.shape, "i8"), Tensor(xl.shape[:-1], "f32")
+    _check(_dev().nt_hip_quantize_int8(C.c_void_p(x.ptr), C.byref(xl.c()), _DT[x.dtype], C.c_void_p(q.ptr),
+                                       C.c_void_p(scale.ptr)), "quantize_int8")
+    return q, scale
+
+
+def _quantized(q: Tensor, scale: Tensor, what: str):
+    if q.dtype != "i8" or scale.dtype != "f32":
+        raise TypeError(f"{what}: {q.dtype} values with {scale.dtype} scales (i8 and f32)")
+    if not q.shape or q.numel != scale.numel * q.shape[-1]:
+        raise ValueError(f"{what}: {list(scale.shape)} scales for the rows of {list(q.shape)}")
+
+
+def dequantize_int8(q: Tensor, scale: Tensor, dtype: str = "f32") -> Tensor:
+    """The values quantized rows stand for, q scale, rounded to nearest even into `dtype`."""
+    _quantized(q, scale, "dequantize_int8")
+    if dtype not in ("f32", "bf16", "f16"):
+        raise TypeError(f"dequantize_int8 into {dtype} (f32, bf16 or f16)")
+    y = Tensor(q.shape, dtype)
+    _check(_dev().nt_hip_dequantize_int8(C.c_void_p(q.ptr), C.c_void_p(scale.ptr), scale.numel, q.shape[-1], _DT[dtype],
+                                         C.c_void_p(y.ptr)), "dequantize_int8")
+    return y
+
+
+def matmul_int8(a: Tensor, a_scale: Tensor, b: Tensor, b_scale: Tensor, dtype: str = "f32") -> Tensor:
+    """The product of quantized rows a [.., m, k] (a scale for each token) and b [n, k] (the weight, a scale for
+    each output channel), as `quantize_int8` gives them: [.., m, n] of `dtype`, the integer sums exact."""
+    _quantized(a, a_scale, "matmul_int8")
+    _quantized(b, b_scale, "matmul_int8")
+    if dtype not in ("f32", "bf16", "f16"):
+        raise TypeError(f"matmul_int8 into {dtype} (f32, bf16 or f16)")
+    if len(b.shape) != 2 or a.shape[-1] != b.shape[1]:
+        raise ValueError(f"matmul_int8 {list(a.shape)} × {list(b.shape)} (b [n, k], its rows as long as a's)")
+    n, k = b.shape
+    y = Tensor(a.shape[:-1] + (n,), dtype)
+    _check(_dev().nt_hip_matmul_int8(C.c_void_p(a.ptr), k, C.c_void_p(a_scale.ptr), C.c_void_p(b.ptr), k,
+                                     C.c_void_p(b_scale.ptr), a_scale.numel, n, k, _DT[dtype], C.c_void_p(y.ptr), n),
+           "matmul_int8")
+    return y
+
+
 def half_gemm_key() -> str:
     """GpuBackend::half_gemm_key: the reduced-precision product's key part."""
     buf = C.create_string_buffer(256)

@@ -153,6 +153,23 @@ class NtRlReadoutScoreArgs(C.Structure):
                 ("logits", C.c_void_p)]
 
 
+class NtRlReadoutStatsArgs(C.Structure):
+    _fields_ = [("hidden", C.c_void_p), ("weight", C.c_void_p), ("dtype", C.c_int32), ("layout", C.c_int32),
+                ("rows", C.c_int64), ("vocab", C.c_int64), ("dim", C.c_int64), ("ldh", C.c_int64), ("ldw", C.c_int64),
+                ("mask", C.c_void_p), ("mask_ld", C.c_int64), ("mask_kind", C.c_int32), ("pad0", C.c_int32),
+                ("temperature", C.c_double), ("tokens", C.c_void_p), ("logp", C.c_void_p), ("entropy", C.c_void_p),
+                ("lse_base", C.c_void_p), ("lse_rest", C.c_void_p), ("status", C.c_void_p)]
+
+
+class NtRlReadoutStatsGradArgs(C.Structure):
+    _fields_ = [("hidden", C.c_void_p), ("weight", C.c_void_p), ("dtype", C.c_int32), ("layout", C.c_int32),
+                ("rows", C.c_int64), ("vocab", C.c_int64), ("dim", C.c_int64), ("ldh", C.c_int64), ("ldw", C.c_int64),
+                ("mask", C.c_void_p), ("mask_ld", C.c_int64), ("mask_kind", C.c_int32), ("pad0", C.c_int32),
+                ("temperature", C.c_double), ("tokens", C.c_void_p), ("lse_base", C.c_void_p), ("lse_rest", C.c_void_p),
+                ("entropy", C.c_void_p), ("g_logp", C.c_void_p), ("g_entropy", C.c_void_p), ("grad_hidden", C.c_void_p),
+                ("grad_weight", C.c_void_p), ("grad_hidden_ld", C.c_int64), ("grad_weight_ld", C.c_int64)]
+
+
 class NtRlScoreArgs(C.Structure):
     _fields_ = [("logits", C.c_void_p), ("ref_logits", C.c_void_p), ("dtype", C.c_int32),
                 ("mask_kind", C.c_int32), ("rows", C.c_int64), ("vocab", C.c_int64), ("ld", C.c_int64),
@@ -226,6 +243,8 @@ _SIGS = {
     "nt_hip_rl_readout_packed_bytes": (C.c_int64, [C.c_int64, C.c_int64]),
     "nt_hip_rl_readout_pack_weight": (C.c_int, [C.c_void_p, C.c_int32, C.c_int32, C.c_int64, C.c_int64, C.c_int64,
                                                 C.c_void_p]),
+    "nt_hip_rl_readout_score_stats": (C.c_int, [C.POINTER(NtRlReadoutStatsArgs)]),
+    "nt_hip_rl_readout_score_backward": (C.c_int, [C.POINTER(NtRlReadoutStatsGradArgs)]),
     "nt_hip_rl_sample_noalloc": (C.c_int, [C.POINTER(NtRlSampleArgs)]),
     "nt_hip_rl_score": (C.c_int, [C.POINTER(NtRlScoreArgs)]),
     "nt_hip_rl_score_backward": (C.c_int, [C.POINTER(NtRlScoreGradArgs)]),
@@ -264,6 +283,10 @@ _SIGS = {
     "nt_hip_matmul": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p]),
     "nt_hip_matmul_half": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p]),
     "nt_hip_half_gemm_key": (C.c_int, [C.c_char_p, C.c_size_t]),
+    "nt_hip_quantize_int8": (C.c_int, [C.c_void_p, C.POINTER(NtLayout), C.c_int32, C.c_void_p, C.c_void_p]),
+    "nt_hip_dequantize_int8": (C.c_int, [C.c_void_p, C.c_void_p, C.c_int64, C.c_int64, C.c_int32, C.c_void_p]),
+    "nt_hip_matmul_int8": (C.c_int, [C.c_void_p, C.c_int64, C.c_void_p, C.c_void_p, C.c_int64, C.c_void_p, C.c_int64,
+                                     C.c_int64, C.c_int64, C.c_int32, C.c_void_p, C.c_int64]),
     "nt_hip_sort_desc": (C.c_int, [C.c_void_p, C.c_int64, C.c_int64, C.c_int64, C.c_void_p, C.c_void_p]),
     # noetic_rng.h
     "nt_rng_derive": (C.c_int, [C.POINTER(NtRng), C.c_uint64, C.c_char_p, C.c_size_t]),
@@ -387,8 +410,8 @@ def launches() -> int:
 
 # ----------------------------------------------------------------------------------- storage
 
-_NP = {"f32": np.float32, "bf16": np.uint16, "f16": np.uint16, "u8": np.uint8, "bool": np.uint8, "i32": np.int32,
-       "i64": np.int64, "f64": np.float64}
+_NP = {"f32": np.float32, "bf16": np.uint16, "f16": np.uint16, "u8": np.uint8, "bool": np.uint8, "i8": np.int8,
+       "i32": np.int32, "i64": np.int64, "f64": np.float64}
 
 
 class Buffer:
@@ -411,8 +434,8 @@ class Buffer:
 
 
 class Tensor:
-    """Device storage with a shape and a dtype ("f32", "bf16" or "f16" bits, "u8", "bool" bytes, "i32",
-    "i64", "f64")."""
+    """Device storage with a shape and a dtype ("f32", "bf16" or "f16" bits, "u8", "bool" bytes, "i8",
+    "i32", "i64", "f64")."""
 
     def __init__(self, shape: Sequence[int], dtype: str, buf: Optional[Buffer] = None):
         self.shape = tuple(int(s) for s in shape)
@@ -430,7 +453,7 @@ class Tensor:
     def from_numpy(a: np.ndarray, dtype: Optional[str] = None) -> "Tensor":
         if dtype is None:
             dtype = {np.dtype(np.float32): "f32", np.dtype(np.uint16): "bf16", np.dtype(np.uint8): "u8",
-                     np.dtype(np.int32): "i32", np.dtype(np.float64): "f64"}[a.dtype]
+                     np.dtype(np.int8): "i8", np.dtype(np.int32): "i32", np.dtype(np.float64): "f64"}[a.dtype]
         a = np.ascontiguousarray(a, dtype=_NP[dtype])
         t = Tensor(a.shape, dtype)
         _check(_dev().nt_hip_upload(C.c_void_p(t.ptr), a.ctypes.data_as(C.c_void_p), t.nbytes), "upload")
@@ -927,6 +950,133 @@ def readout_score(hidden: Tensor, weight: PackedReadout, temperature: float, mas
         if bad.size:
             raise IndexError(f"gather index out of range {V} at position {bad[0]}")
     return (lp, ent, logits) if debug else (lp, ent)
+
+
+def _readout_weight(hidden: Tensor, weight: Tensor, layout: str, who: str):
+    """(seeds, rows per seed, d, V, a seed's weight elements) of hidden [.., d] against a weight [d, V] ("dv")
+    or [V, d] ("vd"), or [S, N, d] against a seed-batched one, with _readout_shape's refusals."""
+    if layout not in ("dv", "vd"):
+        raise ValueError(f"readout weight layout {layout!r} (dv or vd)")
+    if weight.dtype not in _HALF or len(weight.shape) not in (2, 3):
+        raise ValueError(f"{who}: a bf16 or f16 weight [d, V] or [S, d, V] (casts are explicit)")
+    if hidden.dtype not in _ESIZE or len(hidden.shape) < 2:
+        raise ValueError(f"{who}: hidden [.., d]")
+    batched = len(weight.shape) == 3
+    d, V = weight.shape[-2:] if layout == "dv" else weight.shape[:-3:-1]
+    if batched and (len(hidden.shape) != 3 or hidden.shape[0] != weight.shape[0]):
+        raise ValueError(f"{who}: hidden {list(hidden.shape)} against a weight of {weight.shape[0]} seeds "
+                         "(hidden [S, N, d])")
+    if hidden.shape[-1] != d:
+        raise ValueError(f"{who}: hidden's d {hidden.shape[-1]} against the weight's {d}")
+    same_dtype(hidden.dtype, weight.dtype, "matmul")
+    rows = int(np.prod(hidden.shape[:-1]))
+    S = weight.shape[0] if batched else 1
+    return S, rows // S if S else 0, d, V, d * V
+
+
+def _readout_vocab_mask(mask: Optional[Tensor], logits_shape, rows: int, V: int, seeds: int):
+    """(kind, mask tensor, row stride, seed stride) of a vocabulary mask: a u8 keep-mask or an additive f32,
+    bf16 or f16 one, with a row per logits row, one shared row, one per seed ([S, 1, V]), or any other shape
+    that broadcasts to the logits' (broadcast on the device first)."""
+    if mask is None:
+        return NT_MASK_NONE, None, 0, 0
+    import noetic_ops as ops  # (noetic_ops imports this module)
+    if mask.dtype in _HALF:  # (added in f32: widened exactly)
+        mask = ops.cast(mask, ops.Layout.contiguous(mask.shape), "f32")
+    if mask.dtype not in ("u8", "f32"):
+        raise ValueError(f"vocabulary mask of dtype {mask.dtype} (u8 keep-mask, or additive f32, bf16 or f16)")
+    kind = NT_MASK_U8 if mask.dtype == "u8" else NT_MASK_F32
+    sh, full = tuple(mask.shape), tuple(logits_shape)
+    by_row = kind, mask, V, (rows // seeds) * V
+    if sh and sh[-1] == V and mask.numel == V:
+        return kind, mask, 0, 0
+    if len(sh) != len(full):  # rows of another rank: one per logits row
+        if sh and sh[-1] == V and mask.numel == rows * V:
+            return by_row
+    elif sh == full:
+        return by_row
+    elif seeds > 1 and sh == (seeds, 1, V):
+        return kind, mask, 0, V
+    elif all(a == b or a == 1 for a, b in zip(sh, full)):
+        return kind, ops.copy(mask, ops.Layout.contiguous(sh).broadcast(full)), V, (rows // seeds) * V
+    raise ValueError(f"readout: a mask {list(sh)} that does not broadcast to the logits {list(full)}")
+
+
+def readout_score_with_stats(hidden: Tensor, weight: Tensor, temperature: float, mask: Optional[Tensor], tokens: Tensor,
+                             entropy: bool = True, layout: str = "dv", check: bool = True):
+    """The scoring pass of a training step fused with the head at MatmulPrecision::Half: logits = hidden . W
+    (decoder.rs:272,286) tempered and masked (rl.rs:475-486), then token_log_probs (rl.rs:134-141) of `tokens`
+    (minus them is the cross entropy, loss.rs:10-16) and, with `entropy`, categorical_entropy (rl.rs:405-414),
+    the logits never written. `weight` is the head's own bf16 or f16 tensor, [d, V] ("dv") or [V, d] ("vd"), or
+    seed-batched; hidden has its dtype. Returns (logp, entropy or None, RowStats) for `readout_score_grad`.
+    `check` reads the per-row status and refuses a token outside the vocabulary."""
+    who = "readout_score_with_stats"
+    _readout_gate(who)
+    if not (temperature > 0.0 and math.isfinite(temperature)):
+        raise ValueError(f"tempered_logits: temperature {temperature} (must be positive)")
+    S, N, d, V, wn = _readout_weight(hidden, weight, layout, who)
+    rows, out_shape = S * N, hidden.shape[:-1]
+    if tokens.dtype != "i32" or tokens.numel != rows:
+        raise ValueError("token_log_probs: tokens shape (the logits' without the vocabulary axis)")
+    kind, mask, mld, msd = _readout_vocab_mask(mask, out_shape + (V,), rows, V, S)
+    lp, base, rest = (Tensor(out_shape, "f32") for _ in range(3))
+    ent = Tensor(out_shape, "f32") if entropy else None
+    status = Tensor(out_shape, "u8")
+    at = lambda t, i: None if t is None else t.ptr + i  # noqa: E731
+    msize = 4 if kind == NT_MASK_F32 else 1
+    for k in range(S):
+        r = k * N
+        a = NtRlReadoutStatsArgs(at(hidden, r * d * 2), at(weight, k * wn * 2), _DTCODE[hidden.dtype],
+                                 NT_READOUT_W_DV if layout == "dv" else NT_READOUT_W_VD, N, V, d, d,
+                                 V if layout == "dv" else d, at(mask, k * msd * msize), mld, kind, 0, float(temperature),
+                                 at(tokens, r * 4), at(lp, r * 4), at(ent, r * 4), at(base, r * 4), at(rest, r * 4),
+                                 at(status, r))
+        _check(_dev().nt_hip_rl_readout_score_stats(C.byref(a)), "readout score")
+    if check and rows:
+        bad = np.nonzero(status.to_numpy().ravel() == NT_ROW_BAD_TOKEN)[0]
+        if bad.size:
+            raise IndexError(f"gather index out of range {V} at position {bad[0]}")
+    return lp, ent, RowStats(base, rest)
+
+
+def readout_score_grad(hidden: Tensor, weight: Tensor, temperature: float, mask: Optional[Tensor], tokens: Tensor,
+                       stats: "RowStats", entropy: Optional[Tensor] = None, g_logp: Optional[Tensor] = None,
+                       g_entropy: Optional[Tensor] = None, layout: str = "dv", want_hidden: bool = True,
+                       want_weight: bool = True):
+    """The backward of `readout_score_with_stats`: (d hidden, d weight) of sum_r g_logp[r] logp[r] + g_entropy[r]
+    entropy[r] (g_logp from a loss of logp, as policy_gradient_loss_backward or reduce_tokens_backward give it),
+    in the operands' dtype, the logits computed again by pieces of the vocabulary; None for one not wanted. A
+    position whose upstream gradients are zero adds nothing, whatever it holds."""
+    who = "readout_score_grad"
+    _readout_gate(who)
+    if not (temperature > 0.0 and math.isfinite(temperature)):
+        raise ValueError(f"tempered_logits: temperature {temperature} (must be positive)")
+    S, N, d, V, wn = _readout_weight(hidden, weight, layout, who)
+    rows, out_shape = S * N, hidden.shape[:-1]
+    if tokens.dtype != "i32" or tokens.numel != rows:
+        raise ValueError("token_log_probs: tokens shape (the logits' without the vocabulary axis)")
+    if not (want_hidden or want_weight):
+        raise ValueError(f"{who}: no gradient asked for")
+    if g_entropy is not None and entropy is None:
+        raise ValueError(f"{who}: g_entropy needs the forward's entropy")
+    entropy, g_logp, g_entropy = (_row_arg(t, rows, "f32", f"{who}: {n}") for t, n in
+                                  ((entropy, "entropy"), (g_logp, "g_logp"), (g_entropy, "g_entropy")))
+    base, rest = (_row_arg(t, rows, "f32", f"{who}: stats") for t in (stats.lse_base, stats.lse_rest))
+    kind, mask, mld, msd = _readout_vocab_mask(mask, out_shape + (V,), rows, V, S)
+    gh = Tensor(hidden.shape, hidden.dtype) if want_hidden else None
+    gw = Tensor(weight.shape, weight.dtype) if want_weight else None
+    at = lambda t, i: None if t is None else t.ptr + i  # noqa: E731
+    msize = 4 if kind == NT_MASK_F32 else 1
+    wld = V if layout == "dv" else d
+    for k in range(S):
+        r = k * N
+        a = NtRlReadoutStatsGradArgs(at(hidden, r * d * 2), at(weight, k * wn * 2), _DTCODE[hidden.dtype],
+                                     NT_READOUT_W_DV if layout == "dv" else NT_READOUT_W_VD, N, V, d, d, wld,
+                                     at(mask, k * msd * msize), mld, kind, 0, float(temperature), at(tokens, r * 4),
+                                     at(base, r * 4), at(rest, r * 4), at(entropy, r * 4), at(g_logp, r * 4),
+                                     at(g_entropy, r * 4), at(gh, r * d * 2), at(gw, k * wn * 2), d, wld)
+        _check(_dev().nt_hip_rl_readout_score_backward(C.byref(a)), "readout score backward")
+    return gh, gw
 
 
 def _score(policy, ref, tokens, want_logp, want_ref_logp, want_kl, want_ent, want_stats=False):
