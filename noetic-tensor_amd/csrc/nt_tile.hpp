@@ -116,6 +116,7 @@ struct Side {
             }
         }
         if constexpr (!TR) {
+            src = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t *>(base), short(0), int((rows - 1) * ld + width), kWord3);
             const int row = 32 * first_tile + lane % 32, s = (row >> 2) & 3;
             addr[0] = row * kStageK + ((lane / 32) ^ s) * 16;
             addr[1] = row * kStageK + ((2 + lane / 32) ^ s) * 16;
@@ -127,53 +128,60 @@ struct Side {
         }
     }
 
-    // The copies of stage `t` into `lds` (this operand's part of the stage's buffer).
-    __device__ __forceinline__ void copy(uint8_t *lds, int t, int wave) const {
+    // Stage `t`'s copies, q of them: begin(t), then each into `lds` (this operand's part of the buffer).
+    __amdgpu_buffer_rsrc_t src;
+    uint32_t koff;
+    __device__ __forceinline__ void begin(int t) {
         if constexpr (!TR) {
             // a chunk past the row's end is pushed past the range
-            const int64_t last = (rows - 1) * ld + width;
-            const __amdgpu_buffer_rsrc_t r =
-                __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t *>(base), short(0), int(last), kWord3);
             const uint32_t k0 = t * kStageK;
-            const uint32_t koff = int64_t(k0) + chunk * 16 < width ? k0 : 0x80000000u;
-#pragma unroll
-            for (int q = 0; q < kCopies; q++)
-                __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (lds_ptr)(lds + (wave * kCopies + q) * 1024), 16,
-                                                         voff[q] + koff, 0, 0, 0);
+            koff = int64_t(k0) + chunk * 16 < width ? k0 : 0x80000000u;
         } else {
             const int64_t left = rows - int64_t(t) * 32;
             const int64_t bytes = left <= 0 ? 0 : (left < 32 ? left - 1 : 31) * ld + width;
-            const __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc(
-                const_cast<uint8_t *>(base + (left <= 0 ? 0 : int64_t(t) * 32 * ld)), short(0), int(bytes), kWord3);
-#pragma unroll
-            for (int q = 0; q < kCopies; q++)
-                __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (lds_ptr)(lds + (wave * kCopies + q) * 1024), 16, voff[q], 0,
-                                                         0, 0);
+            src = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t *>(base + (left <= 0 ? 0 : int64_t(t) * 32 * ld)),
+                                                    short(0), int(bytes), kWord3);
         }
+    }
+    template <int Q>
+    __device__ __forceinline__ void copy(uint8_t *lds, int wave) const {
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(src, (lds_ptr)(lds + (wave * kCopies + Q) * 1024), 16,
+                                                 TR ? voff[Q] : voff[Q] + koff, 0, 0, 0);
     }
 
-    // Fragment i of k half j of a stage (`at`: the stage's LDS address plus this operand's), waited for.
-    template <int I, int J>
-    __device__ __forceinline__ u32x4 read(uint32_t at) const {
-        if constexpr (!TR) {
-            u32x4 d;
-            asm volatile("ds_read_b128 %0, %1 offset:%2\n\ts_waitcnt lgkmcnt(0)"
-                         : "=&v"(d)
-                         : "v"(at + addr[J]), "i"(I * 32 * kStageK)
+    // The fragments of one k half of a stage: T tiles of 32 rows, by one read each (k-contiguous) or two (TR).
+    static constexpr int kReads = TR ? 2 : 1;
+    typedef typename std::conditional<TR, u32x2, u32x4>::type Part;
+
+    // Read R of half J (`at`: the stage's LDS address plus this operand's), issued only: the register is in
+    // flight until landed() below.
+    template <int R, int J>
+    __device__ __forceinline__ void issue(uint32_t at, Part &d) const {
+        if constexpr (!TR)
+            asm volatile("ds_read_b128 %0, %1 offset:%2" : "=v"(d) : "v"(at + addr[J]), "i"(R * 32 * kStageK) : "memory");
+        else
+            asm volatile("ds_read_b64_tr_b16 %0, %1 offset:%2"
+                         : "=v"(d)
+                         : "v"(at + addr[R / 2]), "i"(J * 32 * B + (R % 2) * 8 * B)
                          : "memory");
-            return d;
-        } else {
-            static_assert(I < 4, "addr");
-            u32x2 d, e;
-            asm volatile("ds_read_b64_tr_b16 %0, %2 offset:%3\n\tds_read_b64_tr_b16 %1, %2 offset:%4\n\t"
-                         "s_waitcnt lgkmcnt(0)"
-                         : "=&v"(d), "=&v"(e)
-                         : "v"(at + addr[I]), "i"(J * 32 * B), "i"(J * 32 * B + 8 * B)
-                         : "memory");
-            return u32x4{d.x, d.y, e.x, e.y};
-        }
+    }
+    template <int N>
+    static __device__ __forceinline__ u32x4 fragment(const Part (&f)[N], int i) {
+        if constexpr (!TR) return f[i];
+        else return u32x4{f[2 * i].x, f[2 * i].y, f[2 * i + 1].x, f[2 * i + 1].y};
     }
 };
+
+// The wait for every LDS read issued, and each register taken through it: nothing that uses one can be placed
+// before, and none is free while its read is in flight.
+template <class P, int N, class Q, int M>
+__device__ __forceinline__ void landed(P (&a)[N], Q (&b)[M]) {
+    asm volatile("s_waitcnt lgkmcnt(0)" : "+v"(a[0]) : : "memory");
+#pragma unroll
+    for (int i = 1; i < N; i++) asm volatile("" : "+v"(a[i]) : : "memory");
+#pragma unroll
+    for (int i = 0; i < M; i++) asm volatile("" : "+v"(b[i]) : : "memory");
+}
 
 // The tile. Lane l of wave (wm, wn) holds in acc[i][j][v] the output of row 32 (TM wm + i) + l % 32 at column
 // 32 (TN wn + j) + 8 (v / 4) + 4 (l / 32) + v % 4: B is the MFMA's first operand, so that a lane's values are
@@ -185,11 +193,26 @@ struct Tile {
     typedef Side<BM, kWaves, ATR> SideA;
     typedef Side<BN, kWaves, BTR> SideB;
     static constexpr int kStageBytes = SideA::kBytes + SideB::kBytes;
-    static constexpr int kStages = 2;
+    static constexpr int kStages = 163840 / kStageBytes < 8 ? 163840 / kStageBytes : 8;
     static constexpr int kLds = kStages * kStageBytes;
+    static constexpr int kCopies = SideA::kCopies + SideB::kCopies;  // of a wave per stage
+    static constexpr int kReadsA = TM * SideA::kReads, kReadsB = TN * SideB::kReads;
+    static_assert(kStages >= 3 && (kStages - 2) * kCopies < 64, "vmcnt's range");
     typename E::Acc acc[TM][TN];
 
-    // acc = the product over `kb` bytes of k (of a k-contiguous row; 2 bytes a row of a transposed operand)
+    struct Frags {
+        typename SideA::Part a[kReadsA];
+        typename SideB::Part b[kReadsB];
+    };
+
+    // acc = the product over `kb` bytes of k (of a k-contiguous row; 2 bytes a row of a transposed operand).
+    //
+    // Stage t sits in buffer t % kStages; its two k halves are steps of TM TN MFMAs. One wave runs on each
+    // SIMD, so whatever is not an MFMA is placed between two of them, where it runs while the first executes:
+    //  - in a stage's first step the second half's fragments are read; in its second step, which begins with
+    //    the wait for the next stage's copies and the barrier, the next stage's first half, and stage
+    //    t + kStages is copied into this stage's buffer (every wave's reads of it have landed by that barrier);
+    //  - so a stage's copies have kStages - 1 stages of MFMAs to land (4 of 1024 cycles for the 256 x 256 tile).
     __device__ __forceinline__ void run(uint8_t *lds, const Operand &a, const Operand &b, int64_t kb, int wave, int lane) {
 #ifdef __HIP_DEVICE_COMPILE__  // (the host pass, which drops the body, cannot emit its lambdas' asm)
         SideA sa;
@@ -204,31 +227,67 @@ struct Tile {
 #pragma unroll
                 for (int v = 0; v < 16; v++) acc[i][j][v] = 0;
         const int n = int((kb + kStageK - 1) / kStageK);
-        sa.copy(lds, 0, wave);
-        sb.copy(lds + SideA::kBytes, 0, wave);
+#pragma unroll
+        for (int t = 0; t < kStages; t++) {
+            sa.begin(t);
+            sb.begin(t);
+            unrolled<SideA::kCopies>([&](auto q) { sa.template copy<q>(lds + t * kStageBytes, wave); });
+            unrolled<SideB::kCopies>([&](auto q) { sb.template copy<q>(lds + t * kStageBytes + SideA::kBytes, wave); });
+        }
         const uint32_t at = uint32_t((uintptr_t)(lds_ptr)(lds));
+        Frags x, y;
+        wait_copies<(kStages - 1) * kCopies>();
+        asm volatile("s_barrier" ::: "memory");
+        unrolled<kReadsA>([&](auto r) { sa.template issue<r, 0>(at, x.a[r]); });
+        unrolled<kReadsB>([&](auto r) { sb.template issue<r, 0>(at + SideA::kBytes, x.b[r]); });
+        landed(x.a, x.b);
+        uint32_t now = 0;  // the stage's buffer
         for (int t = 0; t < n; t++) {
-            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-            __syncthreads();
-            uint8_t *next = lds + ((t + 1) % kStages) * kStageBytes;
-            sa.copy(next, t + 1, wave);
-            sb.copy(next + SideA::kBytes, t + 1, wave);
-            const uint32_t now = at + (t % kStages) * kStageBytes;
-            unrolled<2>([&](auto j_c) {
-                constexpr int J = decltype(j_c)::value;
-                u32x4 fa[TM], fb[TN];
-                unrolled<TM>([&](auto i_c) { fa[i_c] = sa.template read<i_c, J>(now); });
-                unrolled<TN>([&](auto i_c) { fb[i_c] = sb.template read<i_c, J>(now + SideA::kBytes); });
-#pragma unroll
-                for (int i = 0; i < TM; i++)
-#pragma unroll
-                    for (int k = 0; k < TN; k++) acc[i][k] = E::mfma(fb[k], fa[i], acc[i][k]);
-            });
+            const uint32_t next = now + kStageBytes == kLds ? 0 : now + kStageBytes;
+            step<0, 0>(sa, sb, x, y, at + now, nullptr, wave);
+            landed(y.a, y.b);
+            wait_copies<(kStages - 2) * kCopies>();
+            asm volatile("s_barrier" ::: "memory");
+            sa.begin(t + kStages);
+            sb.begin(t + kStages);
+            step<1, kCopies>(sa, sb, y, x, at + next, lds + now, wave);
+            landed(x.a, x.b);
+            now = next;
         }
         // every copy has landed, and every wave is past its last read, before the caller uses the LDS
-        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-        __syncthreads();
+        wait_copies<0>();
+        asm volatile("s_barrier" ::: "memory");
 #endif
+    }
+
+private:
+    template <int N>
+    static __device__ __forceinline__ void wait_copies() {
+        asm volatile("s_waitcnt vmcnt(%0)" : : "i"(N) : "memory");
+    }
+
+    // A step's MFMAs on `f`, the reads of half 1 - J at `at` into `g` and `COPIES` copies into `to` between them.
+    template <int J, int COPIES>
+    __device__ __forceinline__ void step(SideA &sa, SideB &sb, const Frags &f, Frags &g, uint32_t at, uint8_t *to, int wave) {
+        constexpr int kMfmas = TM * TN, kOps = kReadsA + kReadsB + COPIES;
+        unrolled<kMfmas>([&](auto m_c) {
+            constexpr int M = decltype(m_c)::value, I = M / TN, K = M % TN;
+            acc[I][K] = E::mfma(SideB::fragment(f.b, K), SideA::fragment(f.a, I), acc[I][K]);
+            __builtin_amdgcn_sched_barrier(0);
+            // ops M kOps / kMfmas .. : all of them by the last but one MFMA, so that the reads land meanwhile
+            constexpr int kSpread = kMfmas > 4 ? kMfmas - 4 : kMfmas;
+            constexpr int kFrom = M * kOps / kSpread < kOps ? M * kOps / kSpread : kOps;
+            constexpr int kTo = (M + 1) * kOps / kSpread < kOps ? (M + 1) * kOps / kSpread : kOps;
+            unrolled<kTo - kFrom>([&](auto o_c) {
+                constexpr int O = kFrom + decltype(o_c)::value;
+                if constexpr (O < kReadsB) sb.template issue<O, 1 - J>(at + SideA::kBytes, g.b[O]);
+                else if constexpr (O < kReadsB + kReadsA) sa.template issue<O - kReadsB, 1 - J>(at, g.a[O - kReadsB]);
+                else if constexpr (O < kReadsB + kReadsA + SideA::kCopies)
+                    sa.template copy<O - kReadsB - kReadsA>(to, wave);
+                else sb.template copy<O - kReadsB - kReadsA - SideA::kCopies>(to + SideA::kBytes, wave);
+                __builtin_amdgcn_sched_barrier(0);
+            });
+        });
     }
 };
 
