@@ -116,7 +116,7 @@ struct Side {
             }
         }
         if constexpr (!TR) {
-            src = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t *>(base), short(0), int((rows - 1) * ld + width), kWord3);
+            src[0] = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t *>(base), short(0), int((rows - 1) * ld + width), kWord3);
             const int row = 32 * first_tile + lane % 32, s = (row >> 2) & 3;
             addr[0] = row * kStageK + ((lane / 32) ^ s) * 16;
             addr[1] = row * kStageK + ((2 + lane / 32) ^ s) * 16;
@@ -128,25 +128,29 @@ struct Side {
         }
     }
 
-    // Stage `t`'s copies, q of them: begin(t), then each into `lds` (this operand's part of the buffer).
-    __amdgpu_buffer_rsrc_t src;
-    uint32_t koff;
+    // The copies of stages `t` (even) and t + 1: begin(t), then each by the half it belongs to, into `lds` (this
+    // operand's part of that stage's buffer).
+    __amdgpu_buffer_rsrc_t src[TR ? 2 : 1];
+    uint32_t koff[2];
     __device__ __forceinline__ void begin(int t) {
-        if constexpr (!TR) {
-            // a chunk past the row's end is pushed past the range
-            const uint32_t k0 = t * kStageK;
-            koff = int64_t(k0) + chunk * 16 < width ? k0 : 0x80000000u;
-        } else {
-            const int64_t left = rows - int64_t(t) * 32;
-            const int64_t bytes = left <= 0 ? 0 : (left < 32 ? left - 1 : 31) * ld + width;
-            src = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t *>(base + (left <= 0 ? 0 : int64_t(t) * 32 * ld)),
-                                                    short(0), int(bytes), kWord3);
+#pragma unroll
+        for (int h = 0; h < 2; h++) {
+            if constexpr (!TR) {
+                // a chunk past the row's end is pushed past the range
+                const uint32_t k0 = (t + h) * kStageK;
+                koff[h] = int64_t(k0) + chunk * 16 < width ? k0 : 0x80000000u;
+            } else {
+                const int64_t k0 = int64_t(t + h) * 32, left = rows - k0;
+                const int64_t bytes = left <= 0 ? 0 : (left < 32 ? left - 1 : 31) * ld + width;
+                src[h] = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t *>(base + (left <= 0 ? 0 : k0 * ld)), short(0),
+                                                           int(bytes), kWord3);
+            }
         }
     }
-    template <int Q>
+    template <int Q, int H>
     __device__ __forceinline__ void copy(uint8_t *lds, int wave) const {
-        __builtin_amdgcn_raw_ptr_buffer_load_lds(src, (lds_ptr)(lds + (wave * kCopies + Q) * 1024), 16,
-                                                 TR ? voff[Q] : voff[Q] + koff, 0, 0, 0);
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(src[TR ? H : 0], (lds_ptr)(lds + (wave * kCopies + Q) * 1024), 16,
+                                                 TR ? voff[Q] : voff[Q] + koff[H], 0, 0, 0);
     }
 
     // The fragments of one k half of a stage: T tiles of 32 rows, by one read each (k-contiguous) or two (TR).
@@ -193,11 +197,11 @@ struct Tile {
     typedef Side<BM, kWaves, ATR> SideA;
     typedef Side<BN, kWaves, BTR> SideB;
     static constexpr int kStageBytes = SideA::kBytes + SideB::kBytes;
-    static constexpr int kStages = 163840 / kStageBytes < 8 ? 163840 / kStageBytes : 8;
+    static constexpr int kStages = 5;
     static constexpr int kLds = kStages * kStageBytes;
     static constexpr int kCopies = SideA::kCopies + SideB::kCopies;  // of a wave per stage
     static constexpr int kReadsA = TM * SideA::kReads, kReadsB = TN * SideB::kReads;
-    static_assert(kStages >= 3 && (kStages - 2) * kCopies < 64, "vmcnt's range");
+    static_assert(kLds <= 163840 && 4 * kCopies < 64, "LDS, and vmcnt's range");
     typename E::Acc acc[TM][TN];
 
     struct Frags {
@@ -207,12 +211,14 @@ struct Tile {
 
     // acc = the product over `kb` bytes of k (of a k-contiguous row; 2 bytes a row of a transposed operand).
     //
-    // Stage t sits in buffer t % kStages; its two k halves are steps of TM TN MFMAs. One wave runs on each
-    // SIMD, so whatever is not an MFMA is placed between two of them, where it runs while the first executes:
-    //  - in a stage's first step the second half's fragments are read; in its second step, which begins with
-    //    the wait for the next stage's copies and the barrier, the next stage's first half, and stage
-    //    t + kStages is copied into this stage's buffer (every wave's reads of it have landed by that barrier);
-    //  - so a stage's copies have kStages - 1 stages of MFMAs to land (4 of 1024 cycles for the 256 x 256 tile).
+    // Stage t sits in buffer t % 5; its two k halves are steps of TM TN MFMAs. One wave runs on each SIMD, so
+    // whatever is not an MFMA is placed between two of them, where it runs while the first executes: in a
+    // stage's first step the reads of its second half, in its second step those of the next stage's first.
+    // Stages go in pairs, whose copies are issued side by side: a k-contiguous row's two 64 bytes are one
+    // cache line, and an L1 of 32 KiB does not keep it from one stage to the next (4096 x 4096 x 128256 scored
+    // in 4188 us with single stages). During an even stage t the pair t + 4 goes into the buffers of t - 1
+    // and t, which every wave has read by the barrier in front; it has three stages of 1024 cycles (256 x 256
+    // tile) to land.
     __device__ __forceinline__ void run(uint8_t *lds, const Operand &a, const Operand &b, int64_t kb, int wave, int lane) {
 #ifdef __HIP_DEVICE_COMPILE__  // (the host pass, which drops the body, cannot emit its lambdas' asm)
         SideA sa;
@@ -228,31 +234,37 @@ struct Tile {
                 for (int v = 0; v < 16; v++) acc[i][j][v] = 0;
         const int n = int((kb + kStageK - 1) / kStageK);
 #pragma unroll
-        for (int t = 0; t < kStages; t++) {
+        for (int t = 0; t < 4; t += 2) {
             sa.begin(t);
             sb.begin(t);
-            unrolled<SideA::kCopies>([&](auto q) { sa.template copy<q>(lds + t * kStageBytes, wave); });
-            unrolled<SideB::kCopies>([&](auto q) { sb.template copy<q>(lds + t * kStageBytes + SideA::kBytes, wave); });
+            unrolled<2 * kCopies>([&](auto o) { copy<o>(sa, sb, lds + t * kStageBytes, lds + (t + 1) * kStageBytes, wave); });
         }
         const uint32_t at = uint32_t((uintptr_t)(lds_ptr)(lds));
         Frags x, y;
-        wait_copies<(kStages - 1) * kCopies>();
+        wait_copies<2 * kCopies>();
         asm volatile("s_barrier" ::: "memory");
         unrolled<kReadsA>([&](auto r) { sa.template issue<r, 0>(at, x.a[r]); });
         unrolled<kReadsB>([&](auto r) { sb.template issue<r, 0>(at + SideA::kBytes, x.b[r]); });
         landed(x.a, x.b);
-        uint32_t now = 0;  // the stage's buffer
-        for (int t = 0; t < n; t++) {
-            const uint32_t next = now + kStageBytes == kLds ? 0 : now + kStageBytes;
-            step<0, 0>(sa, sb, x, y, at + now, nullptr, wave);
+        uint32_t b0 = 0, free = 4 * kStageBytes;  // stage t's buffer, stage t - 1's
+        auto after = [](uint32_t o) { return o + kStageBytes == kLds ? 0u : o + kStageBytes; };
+        for (int t = 0; t < n; t += 2) {
+            const uint32_t b1 = after(b0), b2 = after(b1);
+            step<0, 0, 0>(sa, sb, x, y, at + b0, nullptr, nullptr, wave);
             landed(y.a, y.b);
-            wait_copies<(kStages - 2) * kCopies>();
-            asm volatile("s_barrier" ::: "memory");
-            sa.begin(t + kStages);
-            sb.begin(t + kStages);
-            step<1, kCopies>(sa, sb, y, x, at + next, lds + now, wave);
+            asm volatile("s_barrier" ::: "memory");  // every wave has read stage t
+            sa.begin(t + 4);
+            sb.begin(t + 4);
+            step<1, 0, kCopies>(sa, sb, y, x, at + b1, lds + free, lds + b0, wave);
             landed(x.a, x.b);
-            now = next;
+            step<0, kCopies, 2 * kCopies>(sa, sb, x, y, at + b1, lds + free, lds + b0, wave);
+            landed(y.a, y.b);
+            wait_copies<2 * kCopies>();  // the pair t + 2
+            asm volatile("s_barrier" ::: "memory");
+            step<1, 0, 0>(sa, sb, y, x, at + b2, nullptr, nullptr, wave);
+            landed(x.a, x.b);
+            free = b1;
+            b0 = b2;
         }
         // every copy has landed, and every wave is past its last read, before the caller uses the LDS
         wait_copies<0>();
@@ -266,25 +278,34 @@ private:
         asm volatile("s_waitcnt vmcnt(%0)" : : "i"(N) : "memory");
     }
 
-    // A step's MFMAs on `f`, the reads of half 1 - J at `at` into `g` and `COPIES` copies into `to` between them.
-    template <int J, int COPIES>
-    __device__ __forceinline__ void step(SideA &sa, SideB &sb, const Frags &f, Frags &g, uint32_t at, uint8_t *to, int wave) {
-        constexpr int kMfmas = TM * TN, kOps = kReadsA + kReadsB + COPIES;
+    // Copy O of a pair of stages: both halves of one copy side by side.
+    template <int O>
+    static __device__ __forceinline__ void copy(const SideA &sa, const SideB &sb, uint8_t *even, uint8_t *odd, int wave) {
+        constexpr int Q = O / 2, H = O % 2;
+        uint8_t *to = H ? odd : even;
+        if constexpr (Q < SideA::kCopies) sa.template copy<Q, H>(to, wave);
+        else sb.template copy<Q - SideA::kCopies, H>(to + SideA::kBytes, wave);
+    }
+
+    // A step's MFMAs on `f`, between them the reads of half 1 - J at `at` into `g` and copies FROM .. TO - 1 of the
+    // pair into its buffers.
+    template <int J, int FROM, int TO>
+    __device__ __forceinline__ void step(const SideA &sa, const SideB &sb, const Frags &f, Frags &g, uint32_t at, uint8_t *even,
+                                         uint8_t *odd, int wave) {
+        constexpr int kMfmas = TM * TN, kReads = kReadsA + kReadsB, kOps = kReads + TO - FROM;
         unrolled<kMfmas>([&](auto m_c) {
             constexpr int M = decltype(m_c)::value, I = M / TN, K = M % TN;
             acc[I][K] = E::mfma(SideB::fragment(f.b, K), SideA::fragment(f.a, I), acc[I][K]);
             __builtin_amdgcn_sched_barrier(0);
-            // ops M kOps / kMfmas .. : all of them by the last but one MFMA, so that the reads land meanwhile
+            // all of them by the last but four MFMAs, so that the reads land meanwhile
             constexpr int kSpread = kMfmas > 4 ? kMfmas - 4 : kMfmas;
             constexpr int kFrom = M * kOps / kSpread < kOps ? M * kOps / kSpread : kOps;
             constexpr int kTo = (M + 1) * kOps / kSpread < kOps ? (M + 1) * kOps / kSpread : kOps;
             unrolled<kTo - kFrom>([&](auto o_c) {
                 constexpr int O = kFrom + decltype(o_c)::value;
                 if constexpr (O < kReadsB) sb.template issue<O, 1 - J>(at + SideA::kBytes, g.b[O]);
-                else if constexpr (O < kReadsB + kReadsA) sa.template issue<O - kReadsB, 1 - J>(at, g.a[O - kReadsB]);
-                else if constexpr (O < kReadsB + kReadsA + SideA::kCopies)
-                    sa.template copy<O - kReadsB - kReadsA>(to, wave);
-                else sb.template copy<O - kReadsB - kReadsA - SideA::kCopies>(to + SideA::kBytes, wave);
+                else if constexpr (O < kReads) sa.template issue<O - kReadsB, 1 - J>(at, g.a[O - kReadsB]);
+                else copy<O - kReads + FROM>(sa, sb, even, odd, wave);
                 __builtin_amdgcn_sched_barrier(0);
             });
         });
