@@ -60,28 +60,97 @@ __device__ __forceinline__ int quantized(float x, float s, float inv) {
     return int(r);
 }
 
-// A workgroup a row.
+// Eight neighbouring values, at the elements' own alignment.
 template <int T>
-__global__ __launch_bounds__(256) void k_quantize_rows(const void *xv, int64_t cols, int64_t ld, int8_t *q, float *scale) {
+__device__ __forceinline__ void load8(const void *p, int64_t i, float (&x)[8]) {
+    if constexpr (T == NT_F32) {
+        __builtin_memcpy(x, static_cast<const float *>(p) + i, 32);
+    } else {
+        uint16_t h[8];
+        __builtin_memcpy(h, static_cast<const uint16_t *>(p) + i, 16);
+#pragma unroll
+        for (int e = 0; e < 8; e++) {
+            if constexpr (T == NT_BF16) x[e] = __builtin_bit_cast(float, uint32_t(h[e]) << 16);
+            else x[e] = float(__builtin_bit_cast(_Float16, h[e]));
+        }
+    }
+}
+
+// THREADS threads a row, ROWS rows a workgroup: a wave a row while that leaves a lane at most 8 chunks of eight
+// values (4096 columns), else 256 threads a row. A lane's first KEEP chunks stay in registers between the two passes; past those
+// (16384 columns) the row is read again, from the caches.
+template <int T, int THREADS, int KEEP>
+__global__ __launch_bounds__(256) void k_quantize_rows(const void *xv, int64_t rows, int64_t cols, int64_t ld, int8_t *q,
+                                                       float *scale) {
+    constexpr int ROWS = 256 / THREADS;
     __shared__ float s_max[4];
     __shared__ int s_bad[4];
-    const int64_t row = blockIdx.x, at = row * ld;
+    const int t = threadIdx.x % THREADS;
+    const int64_t row = blockIdx.x * int64_t(ROWS) + threadIdx.x / THREADS;
+    if (ROWS > 1 && row >= rows) return;
+    const int64_t at = row * ld, chunks = cols / 8;
+    float x[KEEP][8];
     float m = 0.0f;
     bool bad = false;
-    for (int64_t c = threadIdx.x; c < cols; c += 256) {
-        const float a = fabsf(load_f32<T>(xv, at + c));
+    auto see = [&](float v) {
+        const float a = fabsf(v);
         bad |= !(a < INFINITY);
         m = fmaxf(m, a);
+    };
+#pragma unroll
+    for (int k = 0; k < KEEP; k++) {
+        const int64_t c = t + int64_t(k) * THREADS;
+        if (c < chunks) {
+            load8<T>(xv, at + c * 8, x[k]);
+#pragma unroll
+            for (int e = 0; e < 8; e++) see(x[k][e]);
+        }
     }
+    for (int64_t c = t + int64_t(KEEP) * THREADS; c < chunks; c += THREADS) {
+        float y[8];
+        load8<T>(xv, at + c * 8, y);
+#pragma unroll
+        for (int e = 0; e < 8; e++) see(y[e]);
+    }
+    if (chunks * 8 + t < cols && t < 8) see(load_f32<T>(xv, at + chunks * 8 + t));
 #pragma unroll
     for (int d = 32; d; d /= 2) m = fmaxf(m, __shfl_xor(m, d, 64));
-    const bool any = __any(bad);
-    if (threadIdx.x % 64 == 0) s_max[threadIdx.x / 64] = m, s_bad[threadIdx.x / 64] = any;
-    __syncthreads();
-    m = fmaxf(fmaxf(s_max[0], s_max[1]), fmaxf(s_max[2], s_max[3]));
-    const float s = scale_of(m, !(s_bad[0] | s_bad[1] | s_bad[2] | s_bad[3])), inv = 1.0f / s;
-    if (threadIdx.x == 0) scale[row] = s;
-    for (int64_t c = threadIdx.x; c < cols; c += 256) q[row * cols + c] = int8_t(quantized(load_f32<T>(xv, at + c), s, inv));
+    bool any = __any(bad);
+    if constexpr (THREADS > 64) {
+        if (t % 64 == 0) s_max[t / 64] = m, s_bad[t / 64] = any;
+        __syncthreads();
+        m = fmaxf(fmaxf(s_max[0], s_max[1]), fmaxf(s_max[2], s_max[3]));
+        any = s_bad[0] | s_bad[1] | s_bad[2] | s_bad[3];
+    }
+    const float s = scale_of(m, !any), inv = 1.0f / s;
+    if (t == 0) scale[row] = s;
+    int8_t *o = q + row * cols;
+    auto put = [&](int64_t c, const float (&v)[8]) {
+        uint32_t w[2] = {0, 0};
+#pragma unroll
+        for (int e = 0; e < 8; e++) w[e / 4] |= uint32_t(quantized(v[e], s, inv) & 255) << (8 * (e % 4));
+        __builtin_memcpy(o + c * 8, w, 8);
+    };
+#pragma unroll
+    for (int k = 0; k < KEEP; k++) {
+        const int64_t c = t + int64_t(k) * THREADS;
+        if (c < chunks) put(c, x[k]);
+    }
+    for (int64_t c = t + int64_t(KEEP) * THREADS; c < chunks; c += THREADS) {
+        float y[8];
+        load8<T>(xv, at + c * 8, y);
+        put(c, y);
+    }
+    if (chunks * 8 + t < cols && t < 8) o[chunks * 8 + t] = int8_t(quantized(load_f32<T>(xv, at + chunks * 8 + t), s, inv));
+}
+
+template <int T>
+int launch_rows(const void *x, int64_t rows, int64_t cols, int64_t ld, int8_t *q, float *scale) {
+    if (cols <= 4096)
+        k_quantize_rows<T, 64, 8><<<dim3(unsigned(ceil_div(rows, 4))), dim3(256), 0, ctx().stream>>>(x, rows, cols, ld, q, scale);
+    else
+        k_quantize_rows<T, 256, 8><<<dim3(unsigned(rows)), dim3(256), 0, ctx().stream>>>(x, rows, cols, ld, q, scale);
+    return launched("k_quantize_rows");
 }
 
 // Rows that are the columns of x [n, ld]: a workgroup takes 64 of them.
@@ -117,15 +186,52 @@ __global__ __launch_bounds__(256) void k_quantize_columns(const void *xv, int64_
     }
 }
 
+// A thread takes eight neighbouring values at a time, of one row or, where rows are not whole chunks, of two or more.
 template <int T>
 __global__ __launch_bounds__(256) void k_dequantize(const int8_t *q, const float *scale, int64_t rows, int64_t cols, void *out) {
-    const int64_t total = rows * cols;
-    for (int64_t i = blockIdx.x * int64_t(256) + threadIdx.x; i < total; i += int64_t(gridDim.x) * 256) {
-        float x = float(q[i]) * scale[i / cols];
+    const int64_t total = rows * cols, chunks = total / 8;
+    const bool whole = cols % 8 == 0;
+    auto value = [](int8_t b, float s) {
+        float x = float(b) * s;
         asm("" : "+v"(x));  // (rounded to f32 first for every type: the f16 product is not made one instruction)
+        return x;
+    };
+    auto put = [&](int64_t i, float x) {
         if constexpr (T == NT_F32) static_cast<float *>(out)[i] = x;
         else if constexpr (T == NT_BF16) static_cast<uint16_t *>(out)[i] = uint16_t(pair16<Bf16>(x, 0.0f));
         else static_cast<uint16_t *>(out)[i] = uint16_t(pair16<F16>(x, 0.0f));
+    };
+    for (int64_t c = blockIdx.x * int64_t(256) + threadIdx.x; c < chunks; c += int64_t(gridDim.x) * 256) {
+        const int64_t i = c * 8;
+        int8_t b[8];
+        __builtin_memcpy(b, q + i, 8);
+        // (a 32-bit quotient where it does: an index division of 64 bits costs more than the chunk)
+        const int64_t r = total <= 0xffffffffu ? int64_t(uint32_t(i) / uint32_t(cols)) : i / cols;
+        float x[8];
+        if (whole) {
+            const float s = scale[r];
+#pragma unroll
+            for (int e = 0; e < 8; e++) x[e] = value(b[e], s);
+        } else {
+            int64_t row = r, left = cols - (i - r * cols);
+            float s = scale[row];
+            for (int e = 0; e < 8; e++) {
+                if (left == 0) s = scale[++row], left = cols;
+                x[e] = value(b[e], s);
+                left--;
+            }
+        }
+        if constexpr (T == NT_F32) {
+            __builtin_memcpy(static_cast<float *>(out) + i, x, 32);
+        } else {
+            typedef typename std::conditional<T == NT_BF16, Bf16, F16>::type E;
+            const uint32_t w[4] = {pair16<E>(x[0], x[1]), pair16<E>(x[2], x[3]), pair16<E>(x[4], x[5]), pair16<E>(x[6], x[7])};
+            __builtin_memcpy(static_cast<uint16_t *>(out) + i, w, 16);
+        }
+    }
+    if (blockIdx.x == 0 && chunks * 8 + threadIdx.x < total) {
+        const int64_t i = chunks * 8 + threadIdx.x;
+        put(i, value(q[i], scale[i / cols]));
     }
 }
 
@@ -156,23 +262,6 @@ struct Int8P {
     int64_t ldo;
 };
 
-template <int T>
-__device__ __forceinline__ void store4(void *out, int64_t at, const float (&x)[4], int have) {
-    if constexpr (T == NT_F32) {
-        float *o = static_cast<float *>(out) + at;
-        if (have == 4) __builtin_memcpy(o, x, 16);
-        else
-            for (int e = 0; e < have; e++) o[e] = x[e];
-    } else {
-        typedef typename std::conditional<T == NT_BF16, Bf16, F16>::type E;
-        uint16_t *o = static_cast<uint16_t *>(out) + at;
-        const uint32_t w[2] = {pair16<E>(x[0], x[1]), pair16<E>(x[2], x[3])};
-        if (have == 4) __builtin_memcpy(o, w, 8);
-        else
-            for (int e = 0; e < have; e++) o[e] = uint16_t(w[e / 2] >> (16 * (e % 2)));
-    }
-}
-
 template <int TM, int TN, int WM, int WN, int OUT>
 __global__ __launch_bounds__(256, 1) void k_int8_tiles(Int8P p) {
     typedef Tile<I8, TM, TN, WM, WN, false, false> T;
@@ -184,23 +273,45 @@ __global__ __launch_bounds__(256, 1) void k_int8_tiles(Int8P p) {
     T t;
     t.run(lds, Operand{p.a + m0 * p.lda, p.lda, p.m - m0, p.kb}, Operand{p.b + n0 * p.ldb, p.ldb, p.n - n0, p.kb}, p.kb, wave, lane);
     const int wm = wave / WN, wn = wave % WN;
+    typedef typename std::conditional<OUT == NT_F32, u32x4, u32x2>::type V;
+    typedef typename std::conditional<OUT == NT_F16, F16, Bf16>::type E;
+    constexpr int kSize = OUT == NT_F32 ? 4 : 2;
+    static_assert(store_bytes<TN>(kSize) * WM * WN <= T::kLds, "the blocks fit");
+    const int64_t col0 = n0 + 32 * TN * wn;
+    // (every scale before the first store, which the compiler takes to change them)
+    float sb[4 * TN][4];
+#pragma unroll
+    for (int q = 0; q < 4 * TN; q++)
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+            const int64_t col = col0 + 8 * q + 4 * (lane / 32) + e;
+            sb[q][e] = p.sb[col < p.n ? col : p.n - 1];
+        }
+    float sa[TM];
 #pragma unroll
     for (int i = 0; i < TM; i++) {
         const int64_t row = m0 + 32 * (TM * wm + i) + lane % 32;
-        if (row >= p.m) continue;
-        const float sa = p.sa[row];
+        sa[i] = p.sa[row < p.m ? row : p.m - 1];
+    }
+    if (col0 >= p.n) return;
 #pragma unroll
-        for (int j = 0; j < TN; j++)
+    for (int i = 0; i < TM; i++) {
+        const int64_t row0 = m0 + 32 * (TM * wm + i);
+        if (row0 >= p.m) break;
+        V v[4 * TN];
 #pragma unroll
-            for (int q = 0; q < 4; q++) {
-                const int64_t col = n0 + 32 * (TN * wn + j) + 8 * q + 4 * (lane / 32);
-                const int have = p.n - col >= 4 ? 4 : int(p.n - col);
-                if (have <= 0) continue;
-                float x[4];
+        for (int q = 0; q < 4 * TN; q++) {
+            float x[4];
 #pragma unroll
-                for (int e = 0; e < 4; e++) x[e] = float(t.acc[i][j][4 * q + e]) * sa * (e < have ? p.sb[col + e] : 0.0f);
-                store4<OUT>(p.out, row * p.ldo + col, x, have);
-            }
+            for (int e = 0; e < 4; e++) x[e] = float(t.acc[i][q / 4][4 * (q % 4) + e]) * sa[i] * sb[q][e];
+            if constexpr (OUT == NT_F32) v[q] = V{__builtin_bit_cast(uint32_t, x[0]), __builtin_bit_cast(uint32_t, x[1]),
+                                                  __builtin_bit_cast(uint32_t, x[2]), __builtin_bit_cast(uint32_t, x[3])};
+            else v[q] = V{pair16<E>(x[0], x[1]), pair16<E>(x[2], x[3])};
+        }
+        const int64_t rows = p.m - row0, bytes = (p.n - col0) * kSize;
+        store_block<TN>(lds + wave * store_bytes<TN>(kSize), v, lane,
+                        static_cast<uint8_t *>(p.out) + (row0 * p.ldo + col0) * kSize, p.ldo * kSize,
+                        rows < 32 ? int(rows) : 32, bytes < 32 * TN * kSize ? int(bytes) : 32 * TN * kSize);
     }
 }
 
@@ -321,10 +432,11 @@ int nt_hip_quantize_int8(const void *x, const NtLayout *xl, int32_t dtype, int8_
         else if (dtype == NT_BF16) hipLaunchKernelGGL(k_quantize_columns<NT_BF16>, grid, dim3(256), 0, st, src, v.rows, v.cols, v.col_stride, q, scale);
         else hipLaunchKernelGGL(k_quantize_columns<NT_F16>, grid, dim3(256), 0, st, src, v.rows, v.cols, v.col_stride, q, scale);
     } else {
-        const dim3 grid{unsigned(v.rows)};
-        if (dtype == NT_F32) hipLaunchKernelGGL(k_quantize_rows<NT_F32>, grid, dim3(256), 0, st, src, v.cols, v.row_stride, q, scale);
-        else if (dtype == NT_BF16) hipLaunchKernelGGL(k_quantize_rows<NT_BF16>, grid, dim3(256), 0, st, src, v.cols, v.row_stride, q, scale);
-        else hipLaunchKernelGGL(k_quantize_rows<NT_F16>, grid, dim3(256), 0, st, src, v.cols, v.row_stride, q, scale);
+        const int rc = dtype == NT_F32 ? launch_rows<NT_F32>(src, v.rows, v.cols, v.row_stride, q, scale)
+                       : dtype == NT_BF16 ? launch_rows<NT_BF16>(src, v.rows, v.cols, v.row_stride, q, scale)
+                                          : launch_rows<NT_F16>(src, v.rows, v.cols, v.row_stride, q, scale);
+        const int rf = scratch_release(ws);
+        return rc ? rc : rf;
     }
     const int rc = launched("k_quantize");
     const int rf = scratch_release(ws);
@@ -340,7 +452,7 @@ int nt_hip_dequantize_int8(const int8_t *q, const float *scale, int64_t rows, in
     std::unique_lock<std::mutex> lk;
     if (int rc = enter(&lk)) return rc;
     if (rows * cols == 0) return 0;
-    const dim3 grid(unsigned(std::min<int64_t>(ceil_div(rows * cols, 256), 16384)));
+    const dim3 grid(unsigned(std::min<int64_t>(ceil_div(rows * cols, 2048), 16384)));
     if (dtype == NT_F32) hipLaunchKernelGGL(k_dequantize<NT_F32>, grid, dim3(256), 0, ctx().stream, q, scale, rows, cols, out);
     else if (dtype == NT_BF16) hipLaunchKernelGGL(k_dequantize<NT_BF16>, grid, dim3(256), 0, ctx().stream, q, scale, rows, cols, out);
     else hipLaunchKernelGGL(k_dequantize<NT_F16>, grid, dim3(256), 0, ctx().stream, q, scale, rows, cols, out);

@@ -200,6 +200,8 @@ struct Tile {
     static constexpr int kStages = 5;
     static constexpr int kLds = kStages * kStageBytes;
     static constexpr int kCopies = SideA::kCopies + SideB::kCopies;  // of a wave per stage
+    static constexpr int kPair = 2 * kCopies;
+    static constexpr int part(int q) { return kPair * q / 4; }
     static constexpr int kReadsA = TM * SideA::kReads, kReadsB = TN * SideB::kReads;
     static_assert(kLds <= 163840 && 4 * kCopies < 64, "LDS, and vmcnt's range");
     typename E::Acc acc[TM][TN];
@@ -216,9 +218,9 @@ struct Tile {
     // stage's first step the reads of its second half, in its second step those of the next stage's first.
     // Stages go in pairs, whose copies are issued side by side: a k-contiguous row's two 64 bytes are one
     // cache line, and an L1 of 32 KiB does not keep it from one stage to the next (4096 x 4096 x 128256 scored
-    // in 4188 us with single stages). During an even stage t the pair t + 4 goes into the buffers of t - 1
-    // and t, which every wave has read by the barrier in front; it has three stages of 1024 cycles (256 x 256
-    // tile) to land.
+    // in 4188 us with single stages). From an even stage t on the pair t + 4 goes into the buffers of t - 1 and
+    // t, which every wave has read by the barrier in front, a quarter of its copies in each of four steps: the
+    // load unit takes about 24 cycles for a copy of 1 KiB, and a wave whose copy has to wait issues no MFMAs.
     __device__ __forceinline__ void run(uint8_t *lds, const Operand &a, const Operand &b, int64_t kb, int wave, int lane) {
 #ifdef __HIP_DEVICE_COMPILE__  // (the host pass, which drops the body, cannot emit its lambdas' asm)
         SideA sa;
@@ -233,37 +235,39 @@ struct Tile {
 #pragma unroll
                 for (int v = 0; v < 16; v++) acc[i][j][v] = 0;
         const int n = int((kb + kStageK - 1) / kStageK);
-#pragma unroll
-        for (int t = 0; t < 4; t += 2) {
-            sa.begin(t);
-            sb.begin(t);
-            unrolled<2 * kCopies>([&](auto o) { copy<o>(sa, sb, lds + t * kStageBytes, lds + (t + 1) * kStageBytes, wave); });
-        }
         const uint32_t at = uint32_t((uintptr_t)(lds_ptr)(lds));
         Frags x, y;
-        wait_copies<2 * kCopies>();
+        sa.begin(0);
+        sb.begin(0);
+        unrolled<kPair>([&](auto o) { copy<o>(sa, sb, lds, lds + kStageBytes, wave); });
+        sa.begin(2);
+        sb.begin(2);
+        unrolled<part(3)>([&](auto o) { copy<o>(sa, sb, lds + 2 * kStageBytes, lds + 3 * kStageBytes, wave); });
+        wait_copies<part(3)>();
         asm volatile("s_barrier" ::: "memory");
         unrolled<kReadsA>([&](auto r) { sa.template issue<r, 0>(at, x.a[r]); });
         unrolled<kReadsB>([&](auto r) { sb.template issue<r, 0>(at + SideA::kBytes, x.b[r]); });
         landed(x.a, x.b);
-        uint32_t b0 = 0, free = 4 * kStageBytes;  // stage t's buffer, stage t - 1's
+        // the buffers of stage t, of the pair being copied
+        uint32_t b0 = 0, even = 2 * kStageBytes, odd = 3 * kStageBytes;
         auto after = [](uint32_t o) { return o + kStageBytes == kLds ? 0u : o + kStageBytes; };
         for (int t = 0; t < n; t += 2) {
             const uint32_t b1 = after(b0), b2 = after(b1);
-            step<0, 0, 0>(sa, sb, x, y, at + b0, nullptr, nullptr, wave);
+            step<0, part(3), kPair>(sa, sb, x, y, at + b0, lds + even, lds + odd, wave);
             landed(y.a, y.b);
             asm volatile("s_barrier" ::: "memory");  // every wave has read stage t
             sa.begin(t + 4);
             sb.begin(t + 4);
-            step<1, 0, kCopies>(sa, sb, y, x, at + b1, lds + free, lds + b0, wave);
+            even = after(odd);  // (stage t - 1's)
+            odd = b0;
+            step<1, 0, part(1)>(sa, sb, y, x, at + b1, lds + even, lds + odd, wave);
             landed(x.a, x.b);
-            step<0, kCopies, 2 * kCopies>(sa, sb, x, y, at + b1, lds + free, lds + b0, wave);
+            step<0, part(1), part(2)>(sa, sb, x, y, at + b1, lds + even, lds + odd, wave);
             landed(y.a, y.b);
-            wait_copies<2 * kCopies>();  // the pair t + 2
+            wait_copies<part(2)>();  // the pair t + 2
             asm volatile("s_barrier" ::: "memory");
-            step<1, 0, 0>(sa, sb, y, x, at + b2, nullptr, nullptr, wave);
+            step<1, part(2), part(3)>(sa, sb, y, x, at + b2, lds + even, lds + odd, wave);
             landed(x.a, x.b);
-            free = b1;
             b0 = b2;
         }
         // every copy has landed, and every wave is past its last read, before the caller uses the LDS
@@ -287,25 +291,28 @@ private:
         else sb.template copy<Q - SideA::kCopies, H>(to + SideA::kBytes, wave);
     }
 
-    // A step's MFMAs on `f`, between them the reads of half 1 - J at `at` into `g` and copies FROM .. TO - 1 of the
-    // pair into its buffers.
+    // A step's MFMAs on `f`, between them the reads of half 1 - J at `at` into `g`, by the last but four of them
+    // so that they land meanwhile, and copies FROM .. TO - 1 of the pair into its buffers, evenly.
     template <int J, int FROM, int TO>
     __device__ __forceinline__ void step(const SideA &sa, const SideB &sb, const Frags &f, Frags &g, uint32_t at, uint8_t *even,
                                          uint8_t *odd, int wave) {
-        constexpr int kMfmas = TM * TN, kReads = kReadsA + kReadsB, kOps = kReads + TO - FROM;
+        constexpr int kMfmas = TM * TN, kReads = kReadsA + kReadsB;
         unrolled<kMfmas>([&](auto m_c) {
             constexpr int M = decltype(m_c)::value, I = M / TN, K = M % TN;
             acc[I][K] = E::mfma(SideB::fragment(f.b, K), SideA::fragment(f.a, I), acc[I][K]);
             __builtin_amdgcn_sched_barrier(0);
-            // all of them by the last but four MFMAs, so that the reads land meanwhile
             constexpr int kSpread = kMfmas > 4 ? kMfmas - 4 : kMfmas;
-            constexpr int kFrom = M * kOps / kSpread < kOps ? M * kOps / kSpread : kOps;
-            constexpr int kTo = (M + 1) * kOps / kSpread < kOps ? (M + 1) * kOps / kSpread : kOps;
+            constexpr int kFrom = M * kReads / kSpread < kReads ? M * kReads / kSpread : kReads;
+            constexpr int kTo = (M + 1) * kReads / kSpread < kReads ? (M + 1) * kReads / kSpread : kReads;
             unrolled<kTo - kFrom>([&](auto o_c) {
                 constexpr int O = kFrom + decltype(o_c)::value;
                 if constexpr (O < kReadsB) sb.template issue<O, 1 - J>(at + SideA::kBytes, g.b[O]);
-                else if constexpr (O < kReads) sa.template issue<O - kReadsB, 1 - J>(at, g.a[O - kReadsB]);
-                else copy<O - kReads + FROM>(sa, sb, even, odd, wave);
+                else sa.template issue<O - kReadsB, 1 - J>(at, g.a[O - kReadsB]);
+                __builtin_amdgcn_sched_barrier(0);
+            });
+            constexpr int cFrom = FROM + M * (TO - FROM) / kMfmas, cTo = FROM + (M + 1) * (TO - FROM) / kMfmas;
+            unrolled<cTo - cFrom>([&](auto o_c) {
+                copy<cFrom + decltype(o_c)::value>(sa, sb, even, odd, wave);
                 __builtin_amdgcn_sched_barrier(0);
             });
         });
@@ -336,6 +343,56 @@ __device__ __forceinline__ uint32_t pair16(float lo, float hi) {
         const uint16_t a = __builtin_bit_cast(uint16_t, _Float16(lo)), b = __builtin_bit_cast(uint16_t, _Float16(hi));
         return uint32_t(a) | (uint32_t(b) << 16);
     }
+}
+
+// A wave's 32 x 32 TN block of the output as whole cache lines: the tile's layout gives a lane four neighbouring
+// columns of a row, 32 rows a store, so that a line would be written eight bytes at a time. Through LDS (wave
+// `lds`: 32 rows of 32 TN values, the caller's barrier in front) a store's lanes cover whole rows of the block. In
+// LDS, row r's 16-byte chunk c is at c ^ (r % 16), 16-bit values with their chunk's halves swapped in rows
+// 16 .. 31: writes and reads free of bank conflicts.
+// V: u32x2 (four 16-bit values) or u32x4 (four 32-bit ones); v[4 j + a] is columns 32 j + 8 a + 4 (lane / 32) ...
+// `out`: the block's first value, rows ldo bytes apart; `rows` and `bytes` of the block are stored.
+template <int TN, class V>
+__device__ __forceinline__ void store_block(uint8_t *lds, const V (&v)[4 * TN], int lane, uint8_t *out, int64_t ldo,
+                                            int rows, int bytes) {
+    constexpr bool kHalf = sizeof(V) == 8;
+    constexpr int kRow = 32 * TN * int(sizeof(V)) / 4, kPer = kRow / 16, kAt = 64 / kPer;  // chunks a row, rows a store
+    static_assert(kPer >= 16 && kPer <= 64, "chunks of a row");
+    const int r = lane % 32, h = lane / 32;
+#pragma unroll
+    for (int q = 0; q < 4 * TN; q++) {
+        if constexpr (kHalf)
+            *reinterpret_cast<u32x2 *>(lds + r * kRow + (q ^ (r % 16)) * 16 + (h ^ (r / 16)) * 8) = v[q];
+        else
+            *reinterpret_cast<u32x4 *>(lds + r * kRow + ((2 * q + h) ^ (r % 16)) * 16) = v[q];
+    }
+    // (the compiler orders a wave's own LDS accesses; no other wave touches these)
+    const int c = lane % kPer;
+#pragma unroll
+    for (int g = 0; g < 32 / kAt; g++) {
+        const int row = g * kAt + lane / kPer;
+        u32x4 x = *reinterpret_cast<const u32x4 *>(lds + row * kRow + (c ^ (row % 16)) * 16);
+        if (kHalf && row >= 16) x = u32x4{x.z, x.w, x.x, x.y};
+        if (row >= rows) continue;
+        uint8_t *o = out + row * ldo + c * 16;
+        const int left = bytes - c * 16;
+        if (left >= 16) __builtin_memcpy(o, &x, 16);
+        else {
+            const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+            if constexpr (kHalf) {
+                for (int e = 0; e < 8; e++)
+                    if (2 * e < left) reinterpret_cast<uint16_t *>(o)[e] = uint16_t(w[e / 2] >> (16 * (e % 2)));
+            } else {
+                for (int e = 0; e < 4; e++)
+                    if (4 * e < left) reinterpret_cast<uint32_t *>(o)[e] = w[e];
+            }
+        }
+    }
+}
+// The LDS a wave's blocks take.
+template <int TN>
+constexpr int store_bytes(int value_bytes) {
+    return 32 * 32 * TN * value_bytes;
 }
 
 }  // namespace tile

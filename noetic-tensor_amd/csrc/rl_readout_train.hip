@@ -53,29 +53,27 @@ struct MaskP {
     int64_t ld;
 };
 
-// y = x c (+ mask log2 e) of four neighbouring columns of a row, -inf where the mask excludes them or past
-// the vocabulary's `n` columns.
-__device__ __forceinline__ void tempered4(const MaskP &m, int64_t row, int col, int n, float c, float (&y)[4]) {
-#pragma unroll
-    for (int e = 0; e < 4; e++) y[e] *= c;
+// Four neighbouring columns of a row of logits under the mask: -inf where it excludes them or past the
+// vocabulary's `n` columns; under an additive mask x c + mask log2 e, else x itself (y = x c follows in the sum's fma).
+__device__ __forceinline__ void masked4(const MaskP &m, int64_t row, int col, int n, float c, float (&x)[4]) {
     if (col + 4 <= n) {
         if (m.u8) {
             const uint32_t k = *reinterpret_cast<const u32u *>(m.u8 + row * m.ld + col);
 #pragma unroll
-            for (int e = 0; e < 4; e++) y[e] = (k >> (8 * e)) & 0xffu ? y[e] : -INFINITY;
+            for (int e = 0; e < 4; e++) x[e] = (k >> (8 * e)) & 0xffu ? x[e] : -INFINITY;
         } else if (m.f32) {
             float f[4];
             __builtin_memcpy(f, m.f32 + row * m.ld + col, 16);
 #pragma unroll
-            for (int e = 0; e < 4; e++) y[e] = fmaf(f[e], kLog2e, y[e]);
+            for (int e = 0; e < 4; e++) x[e] = fmaf(f[e], kLog2e, x[e] * c);
         }
         return;
     }
 #pragma unroll
     for (int e = 0; e < 4; e++) {
-        if (col + e >= n) y[e] = -INFINITY;
-        else if (m.u8) y[e] = m.u8[row * m.ld + col + e] ? y[e] : -INFINITY;
-        else if (m.f32) y[e] = fmaf(m.f32[row * m.ld + col + e], kLog2e, y[e]);
+        if (col + e >= n) x[e] = -INFINITY;
+        else if (m.u8) x[e] = m.u8[row * m.ld + col + e] ? x[e] : -INFINITY;
+        else if (m.f32) x[e] = fmaf(m.f32[row * m.ld + col + e], kLog2e, x[e] * c);
     }
 }
 
@@ -120,45 +118,47 @@ __global__ __launch_bounds__(256, 1) void k_readout_stats(PieceP p) {
           weight_rows<T, BTR>(p, in), p.kbytes, wave, lane);
     const int wm = wave / WN, wn = wave % WN;
     const int col0 = in * T::BN + 32 * TN * wn + 4 * (lane / 32);
+    const bool plain = !p.mask.u8 && !p.mask.f32 && in * T::BN + T::BN <= p.n;  // every column as it is
+    const float c = p.mask.f32 ? 1.0f : p.c;                                   // y = acc c from here on
     const int64_t block = p.block0 + int64_t(in) * WN + wn;
 #pragma unroll
     for (int i = 0; i < TM; i++) {
         const int64_t row = int64_t(im) * T::BM + 32 * (TM * wm + i) + lane % 32;
         const bool live = row < p.rows;
         const int64_t r = live ? row : 0;
-        // the token's logit, if it is one of this lane's columns
+        // the token's logit, if it is one of this lane's columns (of 32 rows few have it among the wave's)
         const int64_t tok = p.tokens[r] - p.v0 - col0;
-        if (live && tok >= 0 && tok < 32 * TN && (tok & 4) == 0 && tok + col0 < p.n) {
-            const int tj = int(tok / 32), tv = int(4 * ((tok % 32) / 8) + tok % 4);
-            float x = 0.0f;
+        const bool mine = live && tok >= 0 && tok < 32 * TN && (tok & 4) == 0 && tok + col0 < p.n;
+        if (__any(mine)) {
+            float xt = 0.0f;
 #pragma unroll
-            for (int j = 0; j < TN; j++)
+            for (int q = 0; q < 4 * TN; q++)
 #pragma unroll
-                for (int v = 0; v < 16; v++)
-                    if (j == tj && v == tv) x = t.acc[i][j][v];
-            p.xtok[row] = x;
+                for (int e = 0; e < 4; e++)
+                    if (tok == 8 * q + e) xt = t.acc[i][q / 4][4 * (q % 4) + e];
+            if (mine) p.xtok[row] = xt;
         }
+        float x[4 * TN][4];
+#pragma unroll
+        for (int q = 0; q < 4 * TN; q++)
+#pragma unroll
+            for (int e = 0; e < 4; e++) x[q][e] = t.acc[i][q / 4][4 * (q % 4) + e];
+        if (!plain)
+#pragma unroll
+            for (int q = 0; q < 4 * TN; q++) masked4(p.mask, r, col0 + 8 * q, p.n, p.c, x[q]);
         float m = -INFINITY;
 #pragma unroll
-        for (int j = 0; j < TN; j++)
+        for (int q = 0; q < 4 * TN; q++)
 #pragma unroll
-            for (int a = 0; a < 4; a++) {
-                float y[4] = {t.acc[i][j][4 * a], t.acc[i][j][4 * a + 1], t.acc[i][j][4 * a + 2], t.acc[i][j][4 * a + 3]};
-                tempered4(p.mask, r, col0 + 32 * j + 8 * a, p.n, p.c, y);
-#pragma unroll
-                for (int e = 0; e < 4; e++) {
-                    t.acc[i][j][4 * a + e] = y[e];
-                    m = fmaxf(m, y[e]);
-                }
-            }
-        m = fmaxf(m, __shfl_xor(m, 32, 64));
+            for (int e = 0; e < 4; e++) m = fmaxf(m, x[q][e]);
+        m = fmaxf(m, __shfl_xor(m, 32, 64)) * c;
         const float ref = m == -INFINITY ? 0.0f : m;
         float s = 0.0f, es = 0.0f;
 #pragma unroll
-        for (int j = 0; j < TN; j++)
+        for (int q = 0; q < 4 * TN; q++)
 #pragma unroll
-            for (int v = 0; v < 16; v++) {
-                const float d = t.acc[i][j][v] - ref, w = __builtin_amdgcn_exp2f(d);
+            for (int e = 0; e < 4; e++) {
+                const float d = fmaf(x[q][e], c, -ref), w = __builtin_amdgcn_exp2f(d);
                 s += w;
                 if constexpr (ENT) es += w > 0.0f ? w * d : 0.0f;
             }
@@ -185,39 +185,39 @@ struct MergeP {
     uint8_t *status;
 };
 
-// A workgroup joins the blocks of 32 rows, eight threads a row, in f64 and in the same order always.
-__global__ __launch_bounds__(256) void k_readout_merge(MergeP p) {
-    __shared__ float sm[8][32];
-    __shared__ double ss[8][32], st[8][32];
+// A workgroup joins the blocks of 32 rows, 32 threads a row, in f64 and in the same order always.
+__global__ __launch_bounds__(1024) void k_readout_merge(MergeP p) {
+    constexpr int kSegs = 32;
+    __shared__ float sm[kSegs][32];
+    __shared__ double ss[kSegs][32], st[kSegs][32];
     const int lr = threadIdx.x % 32, seg = threadIdx.x / 32;
     const int64_t row = int64_t(blockIdx.x) * 32 + lr;
     const bool live = row < p.rows;
     float m = -INFINITY;
     if (live)
-        for (int b = seg; b < p.blocks; b += 8) m = fmaxf(m, p.ref[b * p.rows_p + row]);
+        for (int b = seg; b < p.blocks; b += kSegs) m = fmaxf(m, p.ref[b * p.rows_p + row]);
     sm[seg][lr] = m;
     __syncthreads();
-    for (int k = 0; k < 8; k++) m = fmaxf(m, sm[k][lr]);
+    for (int k = 0; k < kSegs; k++) m = fmaxf(m, sm[k][lr]);
     double s = 0.0, t = 0.0;
     if (live && m > -INFINITY)
-        for (int b = seg; b < p.blocks; b += 8) {
-            const float r = p.ref[b * p.rows_p + row];
+        for (int b = seg; b < p.blocks; b += kSegs) {
+            const float r = p.ref[b * p.rows_p + row], q = p.sum[b * p.rows_p + row];
             // (a block with nothing allowed has ref -inf and sum 0; with a NaN in it, sum NaN)
-            const double d = double(r) - double(m);
-            const float q = p.sum[b * p.rows_p + row];
             if (r == -INFINITY && q == 0.0f) continue;
-            const double f = exp2(d);
+            const float d = r - m;
+            const double f = double(__builtin_amdgcn_exp2f(d));
             s += f * double(q);
-            if (p.esum) t += f * (double(p.esum[b * p.rows_p + row]) + d * double(q));
+            if (p.esum) t += f * (double(p.esum[b * p.rows_p + row]) + double(d) * double(q));
         }
     else if (live)  // no maximum: NaNs alone leave sums that are NaN
-        for (int b = seg; b < p.blocks; b += 8) s += double(p.sum[b * p.rows_p + row]);
+        for (int b = seg; b < p.blocks; b += kSegs) s += double(p.sum[b * p.rows_p + row]);
     ss[seg][lr] = s;
     st[seg][lr] = t;
     __syncthreads();
     if (seg != 0 || !live) return;
     s = t = 0.0;
-    for (int k = 0; k < 8; k++) s += ss[k][lr], t += st[k][lr];
+    for (int k = 0; k < kSegs; k++) s += ss[k][lr], t += st[k][lr];
     const int64_t tok = p.tokens[row];
     const bool bad = tok < 0 || tok >= p.vocab;
     const bool none = m == -INFINITY && s == 0.0;
@@ -337,33 +337,54 @@ __global__ __launch_bounds__(256, 1) void k_readout_g(PieceP p) {
           weight_rows<T, BTR>(p, in), p.kbytes, wave, lane);
     const int wm = wave / WN, wn = wave % WN;
     const int col0 = in * T::BN + 32 * TN * wn + 4 * (lane / 32);
-    const int ncol = int(p.ldg / 2);
+    const bool plain = !p.mask.u8 && !p.mask.f32 && in * T::BN + T::BN <= p.n;
+    const float c = p.mask.f32 ? 1.0f : p.c;
+    const int64_t bytes = p.ldg - (in * T::BN + 32 * TN * wn) * 2;
+    static_assert(store_bytes<TN>(2) * WM * WN <= T::kLds, "the blocks fit");
+    float4 coef[TM];
+    int tok[TM];  // the token's column from this lane's first, or -1
 #pragma unroll
     for (int i = 0; i < TM; i++) {
-        const int64_t row = int64_t(im) * T::BM + 32 * (TM * wm + i) + lane % 32;
-        if (row >= p.rows) continue;
-        const float4 k = p.coef[row];
-        const int64_t tok64 = p.tokens[row] - p.v0;
-        const int tok = tok64 >= 0 && tok64 < p.n ? int(tok64) : -1;
+        const int64_t row = int64_t(im) * T::BM + 32 * (TM * wm + i) + lane % 32, r = row < p.rows ? row : p.rows - 1;
+        coef[i] = p.coef[r];
+        const int64_t at = p.tokens[r] - p.v0;
+        tok[i] = at >= 0 && at < p.n ? int(at) - col0 : -1;
+    }
+    if (bytes <= 0) return;
+#pragma unroll
+    for (int i = 0; i < TM; i++) {
+        const int64_t row0 = int64_t(im) * T::BM + 32 * (TM * wm + i), row = row0 + lane % 32;
+        if (row0 >= p.rows) break;
+        const float4 k = coef[i];
         const bool dead = k.x == INFINITY;
+        // (of 32 rows few have their token among this wave's columns)
+        const bool mine = __any(tok[i] >= 0 && tok[i] < 32 * TN);
+        u32x2 v[4 * TN];
+        float x[4 * TN][4];
 #pragma unroll
-        for (int j = 0; j < TN; j++)
+        for (int q = 0; q < 4 * TN; q++)
 #pragma unroll
-            for (int a = 0; a < 4; a++) {
-                const int col = col0 + 32 * j + 8 * a;
-                float y[4] = {t.acc[i][j][4 * a], t.acc[i][j][4 * a + 1], t.acc[i][j][4 * a + 2], t.acc[i][j][4 * a + 3]};
-                tempered4(p.mask, row, col, p.n, p.c, y);
-                float g[4];
+            for (int e = 0; e < 4; e++) x[q][e] = t.acc[i][q / 4][4 * (q % 4) + e];
+        if (!plain)
 #pragma unroll
-                for (int e = 0; e < 4; e++) {
-                    const float lp = y[e] - k.x, pr = __builtin_amdgcn_exp2f(lp);  // log2 p, p
-                    g[e] = pr == 0.0f ? 0.0f : pr * fmaf(k.z, lp, k.y);
-                    if (col + e == tok) g[e] += k.w;
-                    g[e] = dead || col + e >= p.n ? 0.0f : g[e];
-                }
-                if (col < ncol)
-                    *reinterpret_cast<u32x2 *>(p.g + row * p.ldg + col * 2) = u32x2{pair16<E>(g[0], g[1]), pair16<E>(g[2], g[3])};
+            for (int q = 0; q < 4 * TN; q++) masked4(p.mask, row < p.rows ? row : p.rows - 1, col0 + 8 * q, p.n, p.c, x[q]);
+#pragma unroll
+        for (int q = 0; q < 4 * TN; q++) {
+            float g[4];
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                const float lp = fmaf(x[q][e], c, -k.x), pr = __builtin_amdgcn_exp2f(lp);  // log2 p, p
+                g[e] = pr * fmaf(k.z, fmaxf(lp, -200.0f), k.y);  // (p 0: 0, and a NaN stays in p)
             }
+            if (mine)
+#pragma unroll
+                for (int e = 0; e < 4; e++)
+                    if (tok[i] == 8 * q + e) g[e] += k.w;
+            v[q] = dead ? u32x2{0, 0} : u32x2{pair16<E>(g[0], g[1]), pair16<E>(g[2], g[3])};
+        }
+        const int64_t rows = p.rows - row0;
+        store_block<TN>(lds + wave * store_bytes<TN>(2), v, lane, p.g + row0 * p.ldg + (in * T::BN + 32 * TN * wn) * 2, p.ldg,
+                        rows < 32 ? int(rows) : 32, bytes < 64 * TN ? int(bytes) : 64 * TN);
     }
 }
 
@@ -414,36 +435,54 @@ __global__ __launch_bounds__(256, 1) void k_readout_grad(GradP p) {
     t.run(lds, a, b, kb, wave, lane);
     const int wm = wave / WN, wn = wave % WN;
     const float whole = p.scale ? *p.scale * p.fixed : p.fixed;
+    const int64_t col0 = n0 + 32 * TN * wn;
+    if (col0 >= p.n) return;
+    float f[TM];
 #pragma unroll
     for (int i = 0; i < TM; i++) {
         const int64_t row = m0 + 32 * (TM * wm + i) + lane % 32;
-        if (row >= p.m) continue;
-        const float f = p.row_scale ? p.row_scale[row] * whole : whole;
+        f[i] = p.row_scale ? p.row_scale[row < p.m ? row : p.m - 1] * whole : whole;
+    }
 #pragma unroll
-        for (int j = 0; j < TN; j++)
+    for (int i = 0; i < TM; i++) {
+        const int64_t row0 = m0 + 32 * (TM * wm + i);
+        if (row0 >= p.m) break;
+        const int rows = p.m - row0 < 32 ? int(p.m - row0) : 32;
+        const int cols = p.n - col0 < 32 * TN ? int(p.n - col0) : 32 * TN;
+        if (p.out) {
+            u32x2 v[4 * TN];
 #pragma unroll
-            for (int q = 0; q < 4; q++) {
-                const int64_t col = n0 + 32 * (TN * wn + j) + 8 * q + 4 * (lane / 32);
-                const int have = p.n - col >= 4 ? 4 : int(p.n - col);
-                if (have <= 0) continue;
-                float x[4] = {t.acc[i][j][4 * q], t.acc[i][j][4 * q + 1], t.acc[i][j][4 * q + 2], t.acc[i][j][4 * q + 3]};
-                if (p.out) {
-#pragma unroll
-                    for (int e = 0; e < 4; e++) x[e] *= f;
-                    store4<E>(p.out + row * p.ldo + col, x, have);
-                } else {
-                    float *o = p.slab + (int64_t(blockIdx.y) * p.m + row) * p.n + col;
-                    if (have == 4) {
-                        float c[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-                        if (p.add) __builtin_memcpy(c, o, 16);
-#pragma unroll
-                        for (int e = 0; e < 4; e++) c[e] += x[e];
-                        __builtin_memcpy(o, c, 16);
-                    } else {
-                        for (int e = 0; e < have; e++) o[e] = (p.add ? o[e] : 0.0f) + x[e];
-                    }
-                }
+            for (int q = 0; q < 4 * TN; q++) {
+                v[q] = u32x2{pair16<E>(t.acc[i][q / 4][4 * (q % 4)] * f[i], t.acc[i][q / 4][4 * (q % 4) + 1] * f[i]),
+                             pair16<E>(t.acc[i][q / 4][4 * (q % 4) + 2] * f[i], t.acc[i][q / 4][4 * (q % 4) + 3] * f[i])};
             }
+            store_block<TN>(lds + wave * store_bytes<TN>(2), v, lane, reinterpret_cast<uint8_t *>(p.out + row0 * p.ldo + col0),
+                            p.ldo * 2, rows, cols * 2);
+            continue;
+        }
+        float *o = p.slab + (int64_t(blockIdx.y) * p.m + row0) * p.n + col0;
+        float c[4 * TN][4];
+#pragma unroll
+        for (int q = 0; q < 4 * TN; q++) c[q][0] = c[q][1] = c[q][2] = c[q][3] = 0.0f;
+        if (p.add) {  // (every load before the first store)
+#pragma unroll
+            for (int q = 0; q < 4 * TN; q++) {
+                const int r = lane % 32, at = 8 * q + 4 * (lane / 32), have = r < rows ? cols - at : 0;
+                const float *s = o + int64_t(r) * p.n + at;
+                if (have >= 4) __builtin_memcpy(c[q], s, 16);
+                else
+                    for (int e = 0; e < 4; e++)
+                        if (e < have) c[q][e] = s[e];
+            }
+        }
+        u32x4 v[4 * TN];
+#pragma unroll
+        for (int q = 0; q < 4 * TN; q++) {
+#pragma unroll
+            for (int e = 0; e < 4; e++) c[q][e] += t.acc[i][q / 4][4 * (q % 4) + e];
+            __builtin_memcpy(&v[q], c[q], 16);
+        }
+        store_block<TN>(lds + wave * store_bytes<TN>(4), v, lane, reinterpret_cast<uint8_t *>(o), p.n * 4, rows, cols * 4);
     }
 }
 
@@ -648,7 +687,7 @@ int forward(const NtRlReadoutStatsArgs *a) {
     q.base = a->lse_base;
     q.rest = a->lse_rest;
     q.status = a->status;
-    hipLaunchKernelGGL(k_readout_merge, dim3(unsigned(ceil_div(R, 32))), dim3(256), 0, ctx().stream, q);
+    hipLaunchKernelGGL(k_readout_merge, dim3(unsigned(ceil_div(R, 32))), dim3(1024), 0, ctx().stream, q);
     return launched("k_readout_merge");
 }
 
