@@ -77,7 +77,7 @@ __device__ __forceinline__ void load8(const void *p, int64_t i, float (&x)[8]) {
 }
 
 // THREADS threads a row, ROWS rows a workgroup: a wave a row while that leaves a lane at most 8 chunks of eight
-// values (4096 columns), else 256 threads a row. A lane's first KEEP chunks stay in registers between the two passes; past those
+// values (4096 columns) and gives every CU a row, else 256 threads a row. A lane's first KEEP chunks stay in registers between the two passes; past those
 // (16384 columns) the row is read again, from the caches.
 template <int T, int THREADS, int KEEP>
 __global__ __launch_bounds__(256) void k_quantize_rows(const void *xv, int64_t rows, int64_t cols, int64_t ld, int8_t *q,
@@ -146,43 +146,119 @@ __global__ __launch_bounds__(256) void k_quantize_rows(const void *xv, int64_t r
 
 template <int T>
 int launch_rows(const void *x, int64_t rows, int64_t cols, int64_t ld, int8_t *q, float *scale) {
-    if (cols <= 4096)
+    if (cols <= 4096 && rows >= 1024)
         k_quantize_rows<T, 64, 8><<<dim3(unsigned(ceil_div(rows, 4))), dim3(256), 0, ctx().stream>>>(x, rows, cols, ld, q, scale);
     else
         k_quantize_rows<T, 256, 8><<<dim3(unsigned(rows)), dim3(256), 0, ctx().stream>>>(x, rows, cols, ld, q, scale);
     return launched("k_quantize_rows");
 }
 
-// Rows that are the columns of x [n, ld]: a workgroup takes 64 of them.
+// Rows that are the columns of x [n, ld]: a workgroup takes 64 of them, a thread four neighbouring ones (16 bytes of f32,
+// 8 of a 16-bit type) of every 32nd row of x. The first KEEP of these stay in registers between the two passes
+// (n 1024); past those x is read again, from the caches. The integers go out through LDS, 128 of a column side by side.
 template <int T>
-__global__ __launch_bounds__(256) void k_quantize_columns(const void *xv, int64_t rows, int64_t n, int64_t ld, int8_t *q,
+__global__ __launch_bounds__(512) void k_quantize_columns(const void *xv, int64_t cols, int64_t n, int64_t ld, int8_t *q,
                                                           float *scale) {
-    __shared__ float s_max[4][64];
-    __shared__ int s_bad[4][64];
-    __shared__ int8_t tile[64][65];
-    const int lc = threadIdx.x % 64, seg = threadIdx.x / 64;
+    constexpr int KEEP = 32, kStep = 4;  // kStep rows of x in flight in the second pass: 128 in all
+    __shared__ float s_max[32][64];
+    __shared__ int s_bad[32][64];
+    __shared__ uint32_t tile[64][33];  // [column][32 words of 4 rows of x]
+    const int t = threadIdx.x, g = t / 16, lc = (t % 16) * 4;
     const int64_t c0 = int64_t(blockIdx.x) * 64, c = c0 + lc;
-    const bool live = c < rows;
-    float m = 0.0f;
-    bool bad = false;
-    if (live)
-        for (int64_t k = seg; k < n; k += 4) {
-            const float a = fabsf(load_f32<T>(xv, k * ld + c));
-            bad |= !(a < INFINITY);
-            m = fmaxf(m, a);
+    const int have = cols - c >= 4 ? 4 : (cols > c ? int(cols - c) : 0);
+    auto load4 = [&](int64_t k, float (&x)[4]) {
+        x[0] = x[1] = x[2] = x[3] = 0.0f;
+        if (k >= n) return;
+        if (have == 4) {
+            if constexpr (T == NT_F32) {
+                __builtin_memcpy(x, static_cast<const float *>(xv) + k * ld + c, 16);
+            } else {
+                uint16_t h[4];
+                __builtin_memcpy(h, static_cast<const uint16_t *>(xv) + k * ld + c, 8);
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    if constexpr (T == NT_BF16) x[e] = __builtin_bit_cast(float, uint32_t(h[e]) << 16);
+                    else x[e] = float(__builtin_bit_cast(_Float16, h[e]));
+                }
+            }
+        } else {
+            for (int e = 0; e < have; e++) x[e] = load_f32<T>(xv, k * ld + c + e);
         }
-    s_max[seg][lc] = m, s_bad[seg][lc] = bad;
+    };
+    float kept[KEEP][4], m[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+    bool bad[4] = {false, false, false, false};
+    auto see = [&](const float (&x)[4]) {
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+            const float a = fabsf(x[e]);
+            bad[e] |= !(a < INFINITY);
+            m[e] = fmaxf(m[e], a);
+        }
+    };
+#pragma unroll
+    for (int k = 0; k < KEEP; k++) load4(g + 32 * k, kept[k]);
+#pragma unroll
+    for (int k = 0; k < KEEP; k++) see(kept[k]);
+    for (int64_t k = g + 32 * KEEP; k < n; k += 32 * kStep) {
+        float x[kStep][4];
+#pragma unroll
+        for (int u = 0; u < kStep; u++) load4(k + 32 * u, x[u]);
+#pragma unroll
+        for (int u = 0; u < kStep; u++) see(x[u]);
+    }
+#pragma unroll
+    for (int e = 0; e < 4; e++) s_max[g][lc + e] = m[e], s_bad[g][lc + e] = bad[e];
     __syncthreads();
-    m = fmaxf(fmaxf(s_max[0][lc], s_max[1][lc]), fmaxf(s_max[2][lc], s_max[3][lc]));
-    const float s = scale_of(m, !(s_bad[0][lc] | s_bad[1][lc] | s_bad[2][lc] | s_bad[3][lc])), inv = 1.0f / s;
-    if (seg == 0 && live) scale[c] = s;
-    for (int64_t k0 = 0; k0 < n; k0 += 64) {
-        for (int k = seg; k < 64; k += 4)
-            tile[k][lc] = live && k0 + k < n ? int8_t(quantized(load_f32<T>(xv, (k0 + k) * ld + c), s, inv)) : int8_t(0);
+    if (t < 64) {
+        float top = 0.0f;
+        int any = 0;
+        for (int k = 0; k < 32; k++) top = fmaxf(top, s_max[k][t]), any |= s_bad[k][t];
+        const float s = scale_of(top, !any);
+        s_max[0][t] = s;
+        if (c0 + t < cols) scale[c0 + t] = s;
+    }
+    __syncthreads();
+    float s[4], inv[4];
+#pragma unroll
+    for (int e = 0; e < 4; e++) s[e] = s_max[0][lc + e], inv[e] = 1.0f / s[e];
+    // 128 rows of x at a time: this thread's four, of row g + 32 u, byte by byte into its columns
+    auto put = [&](int64_t k0, const float (&x)[kStep][4]) {
+#pragma unroll
+        for (int u = 0; u < kStep; u++)
+#pragma unroll
+            for (int e = 0; e < 4; e++)
+                reinterpret_cast<int8_t *>(tile[lc + e])[32 * u + g] = int8_t(quantized(x[u][e], s[e], inv[e]));
         __syncthreads();
-        for (int r = seg; r < 64; r += 4)
-            if (c0 + r < rows && k0 + lc < n) q[(c0 + r) * n + k0 + lc] = tile[lc][r];
+        // 8 threads a column, 16 bytes each
+        const int col = t / 8, b = (t % 8) * 16;
+        const int64_t left = n - k0 - b;
+        if (c0 + col < cols && left > 0) {
+            uint32_t w[4];
+#pragma unroll
+            for (int e = 0; e < 4; e++) w[e] = tile[col][b / 4 + e];
+            int8_t *o = q + (c0 + col) * n + k0 + b;
+            if (left >= 16) __builtin_memcpy(o, w, 16);
+            else
+                for (int e = 0; e < 16; e++)
+                    if (e < left) o[e] = int8_t(w[e / 4] >> (8 * (e % 4)));
+        }
         __syncthreads();
+    };
+#pragma unroll
+    for (int k = 0; k < KEEP; k += kStep)
+        if (32 * k < n) {
+            float x[kStep][4];
+#pragma unroll
+            for (int u = 0; u < kStep; u++)
+#pragma unroll
+                for (int e = 0; e < 4; e++) x[u][e] = kept[k + u][e];
+            put(32 * k, x);
+        }
+    for (int64_t k = 32 * KEEP; k < n; k += 32 * kStep) {
+        float x[kStep][4];
+#pragma unroll
+        for (int u = 0; u < kStep; u++) load4(k + g + 32 * u, x[u]);
+        put(k, x);
     }
 }
 
@@ -263,7 +339,7 @@ struct Int8P {
 };
 
 template <int TM, int TN, int WM, int WN, int OUT>
-__global__ __launch_bounds__(256, 1) void k_int8_tiles(Int8P p) {
+__global__ __launch_bounds__(64 * WM * WN, 1) void k_int8_tiles(Int8P p) {
     typedef Tile<I8, TM, TN, WM, WN, false, false> T;
     __shared__ __attribute__((aligned(16))) uint8_t lds[T::kLds];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -315,6 +391,21 @@ __global__ __launch_bounds__(256, 1) void k_int8_tiles(Int8P p) {
     }
 }
 
+template <int TM, int WM, int WN, int OUT>
+int launch_tiles(Int8P p) {
+    p.tm = uint32_t(ceil_div(p.m, 32 * TM * WM)), p.tn = uint32_t(ceil_div(p.n, 128 * WN));
+    k_int8_tiles<TM, 4, WM, WN, OUT><<<dim3(p.tm * p.tn), dim3(64 * WM * WN), 0, ctx().stream>>>(p);
+    return launched("k_int8_tiles");
+}
+
+// 64 x 128 tiles for up to 64 rows, 128 x 256 for up to 128, else 256 x 256.
+template <int OUT>
+int tiles(const Int8P &p) {
+    if (p.m <= 64) return launch_tiles<1, 2, 1, OUT>(p);
+    if (p.m <= 128) return launch_tiles<2, 2, 2, OUT>(p);
+    return launch_tiles<4, 2, 2, OUT>(p);
+}
+
 int pad_rows(const int8_t *src, int64_t rows, int64_t cols, int64_t ld, uint8_t *out, int64_t ldo) {
     const int64_t n = rows * (ldo / 16);
     hipLaunchKernelGGL(k_pad_bytes, dim3(unsigned(std::min<int64_t>(ceil_div(n, 256), 8192))), dim3(256), 0, ctx().stream,
@@ -350,12 +441,7 @@ int product(const int8_t *a, int64_t lda, const float *sa, const int8_t *b, int6
         p.b = pb, p.ldb = kp;
     }
     if (!rc) {
-        p.tm = uint32_t(ceil_div(m, 256)), p.tn = uint32_t(ceil_div(n, 256));
-        const dim3 grid(p.tm * p.tn), block(256);
-        if (dtype == NT_F32) hipLaunchKernelGGL((k_int8_tiles<4, 4, 2, 2, NT_F32>), grid, block, 0, ctx().stream, p);
-        else if (dtype == NT_BF16) hipLaunchKernelGGL((k_int8_tiles<4, 4, 2, 2, NT_BF16>), grid, block, 0, ctx().stream, p);
-        else hipLaunchKernelGGL((k_int8_tiles<4, 4, 2, 2, NT_F16>), grid, block, 0, ctx().stream, p);
-        rc = launched("k_int8_tiles");
+        rc = dtype == NT_F32 ? tiles<NT_F32>(p) : dtype == NT_BF16 ? tiles<NT_BF16>(p) : tiles<NT_F16>(p);
     }
     const int rf = scratch_release(ws);
     return rc ? rc : rf;
@@ -428,9 +514,9 @@ int nt_hip_quantize_int8(const void *x, const NtLayout *xl, int32_t dtype, int8_
     hipStream_t st = ctx().stream;
     if (columns) {
         const dim3 grid(unsigned(ceil_div(v.rows, 64)));
-        if (dtype == NT_F32) hipLaunchKernelGGL(k_quantize_columns<NT_F32>, grid, dim3(256), 0, st, src, v.rows, v.cols, v.col_stride, q, scale);
-        else if (dtype == NT_BF16) hipLaunchKernelGGL(k_quantize_columns<NT_BF16>, grid, dim3(256), 0, st, src, v.rows, v.cols, v.col_stride, q, scale);
-        else hipLaunchKernelGGL(k_quantize_columns<NT_F16>, grid, dim3(256), 0, st, src, v.rows, v.cols, v.col_stride, q, scale);
+        if (dtype == NT_F32) hipLaunchKernelGGL(k_quantize_columns<NT_F32>, grid, dim3(512), 0, st, src, v.rows, v.cols, v.col_stride, q, scale);
+        else if (dtype == NT_BF16) hipLaunchKernelGGL(k_quantize_columns<NT_BF16>, grid, dim3(512), 0, st, src, v.rows, v.cols, v.col_stride, q, scale);
+        else hipLaunchKernelGGL(k_quantize_columns<NT_F16>, grid, dim3(512), 0, st, src, v.rows, v.cols, v.col_stride, q, scale);
     } else {
         const int rc = dtype == NT_F32 ? launch_rows<NT_F32>(src, v.rows, v.cols, v.row_stride, q, scale)
                        : dtype == NT_BF16 ? launch_rows<NT_BF16>(src, v.rows, v.cols, v.row_stride, q, scale)

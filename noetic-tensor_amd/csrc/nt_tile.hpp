@@ -6,7 +6,7 @@
 // transposed (TR: row k at base + k ld, its m side by side), so that a product and both of its gradients
 // read the same tensors: logits = H W^T, dH = G W, dW = G^T H, none of them copied or transposed first.
 //
-// A workgroup of four waves owns a (32 TM WM) x (32 TN WN) tile, a wave 32 TM x 32 TN of it as TM x TN MFMA
+// A workgroup of WM x WN waves owns a (32 TM WM) x (32 TN WN) tile, a wave 32 TM x 32 TN of it as TM x TN MFMA
 // tiles of 32 x 32. k goes by stages of 64 bytes of a row (32 k of a 16-bit type, 64 of an 8-bit one): both
 // operands' panels are copied by the load unit straight into LDS.
 //

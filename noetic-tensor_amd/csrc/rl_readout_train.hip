@@ -106,8 +106,20 @@ __device__ __forceinline__ Operand weight_rows(const PieceP &p, int in) {
     else return Operand{p.w + n0 * p.ldw, p.ldw, p.n - n0, p.kbytes};
 }
 
-template <class E, int TM, int TN, int WM, int WN, bool BTR, bool ENT>
-__global__ __launch_bounds__(256, 1) void k_readout_stats(PieceP p) {
+// A workgroup's tile: 32 TM WM rows by 128 WN columns (a wave takes 128 columns whatever the tile, so that a
+// row's sums are in the same order whatever rows are scored with it).
+template <int TM_, int WM_, int WN_>
+struct Shape {
+    static constexpr int TM = TM_, TN = 4, WM = WM_, WN = WN_;
+    static constexpr int kThreads = 64 * WM * WN, kRows = 32 * TM * WM, kCols = 128 * WN;
+};
+typedef Shape<4, 2, 2> Large;   // 256 x 256
+typedef Shape<2, 2, 2> Medium;  // 128 x 256
+typedef Shape<1, 2, 1> Small;   // 64 x 128
+
+template <class E, class S, bool BTR, bool ENT>
+__global__ __launch_bounds__(S::kThreads, 1) void k_readout_stats(PieceP p) {
+    constexpr int TM = S::TM, TN = S::TN, WM = S::WM, WN = S::WN;
     typedef Tile<E, TM, TN, WM, WN, false, BTR> T;
     __shared__ __attribute__((aligned(16))) uint8_t lds[T::kLds];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -185,39 +197,65 @@ struct MergeP {
     uint8_t *status;
 };
 
-// A workgroup joins the blocks of 32 rows, 32 threads a row, in f64 and in the same order always.
+// A workgroup joins the blocks of 32 rows, 32 threads a row, in f64 and in the same order always: a thread its
+// blocks by eights (loads in flight together), each eight against its own maximum.
 __global__ __launch_bounds__(1024) void k_readout_merge(MergeP p) {
-    constexpr int kSegs = 32;
+    constexpr int kSegs = 32, kBatch = 8;
     __shared__ float sm[kSegs][32];
     __shared__ double ss[kSegs][32], st[kSegs][32];
     const int lr = threadIdx.x % 32, seg = threadIdx.x / 32;
     const int64_t row = int64_t(blockIdx.x) * 32 + lr;
     const bool live = row < p.rows;
-    float m = -INFINITY;
-    if (live)
-        for (int b = seg; b < p.blocks; b += kSegs) m = fmaxf(m, p.ref[b * p.rows_p + row]);
-    sm[seg][lr] = m;
-    __syncthreads();
-    for (int k = 0; k < kSegs; k++) m = fmaxf(m, sm[k][lr]);
+    float m = -INFINITY;  // the maximum so far, s and t in its units
     double s = 0.0, t = 0.0;
-    if (live && m > -INFINITY)
-        for (int b = seg; b < p.blocks; b += kSegs) {
-            const float r = p.ref[b * p.rows_p + row], q = p.sum[b * p.rows_p + row];
-            // (a block with nothing allowed has ref -inf and sum 0; with a NaN in it, sum NaN)
-            if (r == -INFINITY && q == 0.0f) continue;
-            const float d = r - m;
-            const double f = double(__builtin_amdgcn_exp2f(d));
-            s += f * double(q);
-            if (p.esum) t += f * (double(p.esum[b * p.rows_p + row]) + double(d) * double(q));
+    for (int b0 = seg; b0 < p.blocks; b0 += kBatch * kSegs) {
+        float r[kBatch], q[kBatch], e[kBatch];
+#pragma unroll
+        for (int k = 0; k < kBatch; k++) {
+            const int b = b0 + k * kSegs;
+            const bool in = b < p.blocks && live;
+            r[k] = in ? p.ref[b * p.rows_p + row] : -INFINITY;
+            q[k] = in ? p.sum[b * p.rows_p + row] : 0.0f;
+            e[k] = in && p.esum ? p.esum[b * p.rows_p + row] : 0.0f;
         }
-    else if (live)  // no maximum: NaNs alone leave sums that are NaN
-        for (int b = seg; b < p.blocks; b += kSegs) s += double(p.sum[b * p.rows_p + row]);
+        float top = m;
+#pragma unroll
+        for (int k = 0; k < kBatch; k++) top = fmaxf(top, r[k]);
+        const float base = top == -INFINITY ? 0.0f : top;
+        if (m > -INFINITY) {
+            const double d = double(m) - double(base), f = double(__builtin_amdgcn_exp2f(float(d)));
+            t = f * (t + d * s);
+            s *= f;
+        }
+        m = top;
+#pragma unroll
+        for (int k = 0; k < kBatch; k++) {
+            // (a block with nothing allowed has ref -inf and sum 0; with NaNs alone, sum NaN)
+            if (r[k] == -INFINITY && q[k] == 0.0f) continue;
+            const float d = r[k] - base;
+            const double f = r[k] == -INFINITY ? 1.0 : double(__builtin_amdgcn_exp2f(d));
+            s += f * double(q[k]);
+            t += f * (double(e[k]) + double(d) * double(q[k]));
+        }
+    }
+    sm[seg][lr] = m;
     ss[seg][lr] = s;
     st[seg][lr] = t;
     __syncthreads();
     if (seg != 0 || !live) return;
+    for (int k = 0; k < kSegs; k++) m = fmaxf(m, sm[k][lr]);
     s = t = 0.0;
-    for (int k = 0; k < kSegs; k++) s += ss[k][lr], t += st[k][lr];
+    for (int k = 0; k < kSegs; k++) {
+        const double q = ss[k][lr];
+        if (sm[k][lr] == -INFINITY) {
+            s += q;  // 0, or NaN
+            continue;
+        }
+        const float d = sm[k][lr] - m;
+        const double f = double(__builtin_amdgcn_exp2f(d));
+        s += f * q;
+        t += f * (st[k][lr] + double(d) * q);
+    }
     const int64_t tok = p.tokens[row];
     const bool bad = tok < 0 || tok >= p.vocab;
     const bool none = m == -INFINITY && s == 0.0;
@@ -300,7 +338,7 @@ __global__ __launch_bounds__(1024) void k_readout_coef(CoefP p) {
 // NaN too, stays out of dW) and with `up`, f16 rows are scaled by up / top, a power of two.
 __global__ __launch_bounds__(256) void k_readout_rows(const uint16_t *src, int64_t rows, int64_t cols, int64_t ld,
                                                       uint8_t *out, int64_t ldo, const float4 *coef, const float *up,
-                                                      const float *top) {
+                                                      const float *top, int64_t again) {
     const int64_t per = ldo / 16, total = rows * per;
     for (int64_t i = blockIdx.x * int64_t(256) + threadIdx.x; i < total; i += int64_t(gridDim.x) * 256) {
         const int64_t r = i / per, c = (i - r * per) * 8;
@@ -322,11 +360,22 @@ __global__ __launch_bounds__(256) void k_readout_rows(const uint16_t *src, int64
             }
         }
         *reinterpret_cast<u32x4 *>(out + r * ldo + c * 2) = x.v;
+        if (again) *reinterpret_cast<u32x4 *>(out + (r + again) * ldo + c * 2) = x.v;
     }
 }
 
-template <class E, int TM, int TN, int WM, int WN, bool BTR>
-__global__ __launch_bounds__(256, 1) void k_readout_g(PieceP p) {
+template <class E>
+__device__ __forceinline__ float widened(uint32_t h) {
+    if constexpr (std::is_same<E, Bf16>::value) return __builtin_bit_cast(float, h << 16);
+    else return float(__builtin_bit_cast(_Float16, uint16_t(h)));
+}
+
+// A piece's G. TWO: up to 64 rows, where one rounding of a row's largest entries (its token's above all) is not averaged away in
+// the gradients' sums: what the rounding left goes into rows `rows` .. 2 rows - 1, and the products take both.
+// A stage of 32 k or a 64-row tile costs the same at twice so few rows.
+template <class E, class S, bool BTR, bool TWO>
+__global__ __launch_bounds__(S::kThreads, 1) void k_readout_g(PieceP p) {
+    constexpr int TM = S::TM, TN = S::TN, WM = S::WM, WN = S::WN;
     typedef Tile<E, TM, TN, WM, WN, false, BTR> T;
     __shared__ __attribute__((aligned(16))) uint8_t lds[T::kLds];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -359,7 +408,7 @@ __global__ __launch_bounds__(256, 1) void k_readout_g(PieceP p) {
         const bool dead = k.x == INFINITY;
         // (of 32 rows few have their token among this wave's columns)
         const bool mine = __any(tok[i] >= 0 && tok[i] < 32 * TN);
-        u32x2 v[4 * TN];
+        u32x2 v[4 * TN], lo[TWO ? 4 * TN : 1];
         float x[4 * TN][4];
 #pragma unroll
         for (int q = 0; q < 4 * TN; q++)
@@ -381,10 +430,16 @@ __global__ __launch_bounds__(256, 1) void k_readout_g(PieceP p) {
                 for (int e = 0; e < 4; e++)
                     if (tok[i] == 8 * q + e) g[e] += k.w;
             v[q] = dead ? u32x2{0, 0} : u32x2{pair16<E>(g[0], g[1]), pair16<E>(g[2], g[3])};
+            if constexpr (TWO) {
+                const float r[4] = {g[0] - widened<E>(v[q].x), g[1] - widened<E>(v[q].x >> 16), g[2] - widened<E>(v[q].y),
+                                    g[3] - widened<E>(v[q].y >> 16)};
+                lo[q] = dead ? u32x2{0, 0} : u32x2{pair16<E>(r[0], r[1]), pair16<E>(r[2], r[3])};
+            }
         }
-        const int64_t rows = p.rows - row0;
-        store_block<TN>(lds + wave * store_bytes<TN>(2), v, lane, p.g + row0 * p.ldg + (in * T::BN + 32 * TN * wn) * 2, p.ldg,
-                        rows < 32 ? int(rows) : 32, bytes < 64 * TN ? int(bytes) : 64 * TN);
+        const int rows = p.rows - row0 < 32 ? int(p.rows - row0) : 32, have = bytes < 64 * TN ? int(bytes) : 64 * TN;
+        uint8_t *o = p.g + row0 * p.ldg + (in * T::BN + 32 * TN * wn) * 2;
+        store_block<TN>(lds + wave * store_bytes<TN>(2), v, lane, o, p.ldg, rows, have);
+        if constexpr (TWO) store_block<TN>(lds + wave * store_bytes<TN>(2), lo, lane, o + p.rows * p.ldg, p.ldg, rows, have);
     }
 }
 
@@ -405,19 +460,9 @@ struct GradP {
     float fixed;
 };
 
-template <class E>
-__device__ __forceinline__ void store4(uint16_t *o, const float (&x)[4], int have) {
-    const u32x2 v = {pair16<E>(x[0], x[1]), pair16<E>(x[2], x[3])};
-    if (have >= 4) {
-        __builtin_memcpy(o, &v, 8);
-        return;
-    }
-    const uint32_t w[2] = {v.x, v.y};
-    for (int e = 0; e < have; e++) o[e] = uint16_t(w[e / 2] >> (16 * (e % 2)));
-}
-
-template <class E, int TM, int TN, int WM, int WN, bool ATR, bool BTR>
-__global__ __launch_bounds__(256, 1) void k_readout_grad(GradP p) {
+template <class E, class S, bool ATR, bool BTR>
+__global__ __launch_bounds__(S::kThreads, 1) void k_readout_grad(GradP p) {
+    constexpr int TM = S::TM, TN = S::TN, WM = S::WM, WN = S::WN;
     typedef Tile<E, TM, TN, WM, WN, ATR, BTR> T;
     __shared__ __attribute__((aligned(16))) uint8_t lds[T::kLds];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -486,29 +531,41 @@ __global__ __launch_bounds__(256, 1) void k_readout_grad(GradP p) {
     }
 }
 
-// The slabs' sum in their order, scaled and rounded.
+// The slabs' sum in their order, scaled and rounded; with `two` > 0, of rows r and r + two of each.
 template <class E>
-__global__ __launch_bounds__(256) void k_readout_fold(const float *slab, int splits, int64_t m, int64_t n, uint16_t *out,
-                                                      int64_t ldo, const float *row_scale, const float *scale, float fixed) {
-    const int64_t per = (n + 3) / 4, total = m * per;
+__global__ __launch_bounds__(256) void k_readout_fold(const float *slab, int splits, int64_t m, int64_t n, int64_t two,
+                                                      uint16_t *out, int64_t ldo, const float *row_scale, const float *scale,
+                                                      float fixed) {
+    const int64_t per = (n + 3) / 4, rows = two ? two : m, total = rows * per;
+    const int terms = two ? 2 * splits : splits;
     for (int64_t i = blockIdx.x * int64_t(256) + threadIdx.x; i < total; i += int64_t(gridDim.x) * 256) {
         const int64_t r = i / per, c = (i - r * per) * 4;
         const int have = n - c >= 4 ? 4 : int(n - c);
         float x[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-        for (int z = 0; z < splits; z++) {
-            const float *s = slab + (z * m + r) * n + c;
-            float v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-            if (have == 4) __builtin_memcpy(v, s, 16);
-            else
-                for (int e = 0; e < have; e++) v[e] = s[e];
+        for (int z0 = 0; z0 < terms; z0 += 8) {  // (eight loads in flight)
+            float v[8][4];
 #pragma unroll
-            for (int e = 0; e < 4; e++) x[e] += v[e];
+            for (int k = 0; k < 8; k++) {
+                v[k][0] = v[k][1] = v[k][2] = v[k][3] = 0.0f;
+                const int z = z0 + k;
+                if (z >= terms) continue;
+                const float *s = slab + (two ? (z / 2) * m + r + (z % 2) * two : z * m + r) * n + c;
+                if (have == 4) __builtin_memcpy(v[k], s, 16);
+                else
+                    for (int e = 0; e < have; e++) v[k][e] = s[e];
+            }
+#pragma unroll
+            for (int k = 0; k < 8; k++)
+#pragma unroll
+                for (int e = 0; e < 4; e++) x[e] += v[k][e];
         }
         float f = scale ? *scale * fixed : fixed;
         if (row_scale) f *= row_scale[r];
-#pragma unroll
-        for (int e = 0; e < 4; e++) x[e] *= f;
-        store4<E>(out + r * ldo + c, x, have);
+        uint16_t *o = out + r * ldo + c;
+        const uint32_t w[2] = {pair16<E>(x[0] * f, x[1] * f), pair16<E>(x[2] * f, x[3] * f)};
+        if (have == 4) __builtin_memcpy(o, w, 8);
+        else
+            for (int e = 0; e < have; e++) o[e] = uint16_t(w[e / 2] >> (16 * (e % 2)));
     }
 }
 
@@ -573,10 +630,10 @@ bool aligned(const void *p, int64_t cols, int64_t ld) {
 }
 
 int copy_rows(const void *src, int64_t rows, int64_t cols, int64_t ld, uint8_t *out, int64_t ldo, const float4 *coef,
-              const float *up, const float *top) {
+              const float *up, const float *top, int64_t again = 0) {
     const int64_t n = rows * (ldo / 16);
     hipLaunchKernelGGL(k_readout_rows, dim3(unsigned(std::min<int64_t>(ceil_div(n, 256), 8192))), dim3(256), 0,
-                       ctx().stream, static_cast<const uint16_t *>(src), rows, cols, ld, out, ldo, coef, up, top);
+                       ctx().stream, static_cast<const uint16_t *>(src), rows, cols, ld, out, ldo, coef, up, top, again);
     return launched("k_readout_rows");
 }
 
@@ -612,13 +669,48 @@ int64_t piece_cols(int64_t vocab, int64_t cols) {
     return std::min(round_up(ceil_div(vocab, pieces), kTile), round_up(vocab, kTile));
 }
 
-template <class E, bool BTR>
-int launch_stats(const PieceP &p, bool ent) {
-    const dim3 grid(p.tm * p.tn), block(256);
-    if (ent) k_readout_stats<E, 4, 4, 2, 2, BTR, true><<<grid, block, 0, ctx().stream>>>(p);
-    else k_readout_stats<E, 4, 4, 2, 2, BTR, false><<<grid, block, 0, ctx().stream>>>(p);
+// The tile of a product of `rows` rows and `cols` columns.
+enum class Size { kSmall, kMedium, kLarge };
+Size size_of(int64_t rows) {
+    return rows <= 64 ? Size::kSmall : rows <= 128 ? Size::kMedium : Size::kLarge;
+}
+
+template <class E, class S, bool BTR>
+int launch_stats(PieceP p, bool ent) {
+    p.tm = uint32_t(ceil_div(p.rows, S::kRows));
+    p.tn = uint32_t(ceil_div(p.n, S::kCols));
+    const dim3 grid(p.tm * p.tn), block(S::kThreads);
+    if (ent) k_readout_stats<E, S, BTR, true><<<grid, block, 0, ctx().stream>>>(p);
+    else k_readout_stats<E, S, BTR, false><<<grid, block, 0, ctx().stream>>>(p);
     return launched("k_readout_stats");
 }
+
+template <class E, bool BTR>
+int stats(const PieceP &p, bool ent) {
+    switch (size_of(p.rows)) {
+        case Size::kSmall: return launch_stats<E, Small, BTR>(p, ent);
+        case Size::kMedium: return launch_stats<E, Medium, BTR>(p, ent);
+        default: return launch_stats<E, Large, BTR>(p, ent);
+    }
+}
+
+template <class E, class S, bool BTR, bool TWO>
+int launch_g(PieceP p) {
+    p.tm = uint32_t(ceil_div(p.rows, S::kRows));
+    p.tn = uint32_t(ceil_div(p.n, S::kCols));
+    k_readout_g<E, S, BTR, TWO><<<dim3(p.tm * p.tn), dim3(S::kThreads), 0, ctx().stream>>>(p);
+    return launched("k_readout_g");
+}
+
+template <class E, bool BTR>
+int g_piece(const PieceP &p) {
+    switch (size_of(p.rows)) {
+        case Size::kSmall: return launch_g<E, Small, BTR, true>(p);
+        case Size::kMedium: return launch_g<E, Medium, BTR, false>(p);
+        default: return launch_g<E, Large, BTR, false>(p);
+    }
+}
+constexpr int64_t kTwoRows = 64;  // G in two terms for so many rows: the Small tile's
 
 int forward(const NtRlReadoutStatsArgs *a) {
     const bool dv = a->layout == NT_READOUT_W_DV;
@@ -629,7 +721,7 @@ int forward(const NtRlReadoutStatsArgs *a) {
     int64_t most = (int64_t(1) << 23) / ceil_div(R, kTile) * kTile;
     if (!wdirect) most = std::min(most, (int64_t(1) << 27) / kp);
     const int64_t cols = piece_cols(V, most);
-    const int64_t blocks = ceil_div(V, kTile) * 2, rows_p = round_up(R, 32);
+    const int64_t blocks = ceil_div(V, kTile) * 2, rows_p = round_up(R, 32);  // (a large tile writes whole ones)
     Scratch s;
     const size_t o_h = s.add(hdirect ? 0 : R * kp * 2);
     const size_t o_w = s.add(wdirect ? 0 : (dv ? d * cols : cols * kp) * 2);
@@ -663,11 +755,9 @@ int forward(const NtRlReadoutStatsArgs *a) {
         p.v0 = v0;
         p.block0 = v0 / kBlockCols;
         p.mask = mask_at(a->mask_kind, a->mask, a->mask_ld, v0);
-        p.tm = uint32_t(ceil_div(R, kTile));
-        p.tn = uint32_t(ceil_div(n, kTile));
         const bool bf16 = a->dtype == NT_BF16, ent = a->entropy != nullptr;
-        const int rc = dv ? (bf16 ? launch_stats<Bf16, true>(p, ent) : launch_stats<F16, true>(p, ent))
-                          : (bf16 ? launch_stats<Bf16, false>(p, ent) : launch_stats<F16, false>(p, ent));
+        const int rc = dv ? (bf16 ? stats<Bf16, true>(p, ent) : stats<F16, true>(p, ent))
+                          : (bf16 ? stats<Bf16, false>(p, ent) : stats<F16, false>(p, ent));
         if (rc) return rc;
     }
     MergeP q{};
@@ -676,7 +766,7 @@ int forward(const NtRlReadoutStatsArgs *a) {
     q.esum = p.esum;
     q.rows = R;
     q.rows_p = rows_p;
-    q.blocks = int(blocks);
+    q.blocks = int(ceil_div(V, kBlockCols));
     q.vocab = V;
     q.xtok = p.xtok;
     q.tokens = a->tokens;
@@ -703,21 +793,27 @@ Split split_k(int64_t m, int64_t n, int64_t k) {
 }
 
 template <class E>
-int fold(const GradP &p, int64_t splits, uint16_t *out) {
-    const int64_t n = p.m * ceil_div(p.n, 4);
+int fold(const GradP &p, int64_t splits, uint16_t *out, int64_t two = 0) {
+    const int64_t n = (two ? two : p.m) * ceil_div(p.n, 4);
     hipLaunchKernelGGL(k_readout_fold<E>, dim3(unsigned(std::min<int64_t>(ceil_div(n, 256), 8192))), dim3(256), 0,
-                       ctx().stream, p.slab, int(splits), p.m, p.n, out, p.ldo, p.row_scale, p.scale, p.fixed);
+                       ctx().stream, p.slab, int(splits), p.m, p.n, two, out, p.ldo, p.row_scale, p.scale, p.fixed);
     return launched("k_readout_fold");
 }
 
-template <class E, bool ATR, bool BTR>
-int product(GradP p, const Split &s) {
+template <class E, class S, bool ATR, bool BTR>
+int launch_product(GradP p, const Split &s) {
     p.per = s.per;
-    p.tm = uint32_t(ceil_div(p.m, kTile));
-    p.tn = uint32_t(ceil_div(p.n, kTile));
-    hipLaunchKernelGGL((k_readout_grad<E, 4, 4, 2, 2, ATR, BTR>), dim3(p.tm * p.tn, unsigned(s.splits)), dim3(256), 0,
-                       ctx().stream, p);
+    p.tm = uint32_t(ceil_div(p.m, S::kRows));
+    p.tn = uint32_t(ceil_div(p.n, S::kCols));
+    k_readout_grad<E, S, ATR, BTR><<<dim3(p.tm * p.tn, unsigned(s.splits)), dim3(S::kThreads), 0, ctx().stream>>>(p);
     return launched("k_readout_grad");
+}
+
+template <class E, bool ATR, bool BTR>
+int product(const GradP &p, const Split &s) {
+    if constexpr (!ATR)  // (dH: as many rows as there are, or twice them)
+        if (p.m <= 128) return launch_product<E, Medium, ATR, BTR>(p, s);
+    return launch_product<E, Large, ATR, BTR>(p, s);
 }
 
 // One piece of the vocabulary: its G, its rows of dW, its share of dH.
@@ -738,8 +834,8 @@ template <class E, bool DV>
 int piece(const BackP &b) {
     const NtRlReadoutStatsGradArgs *a = b.a;
     const PieceP &p = b.p;
-    k_readout_g<E, 4, 4, 2, 2, DV><<<dim3(p.tm * p.tn), dim3(256), 0, ctx().stream>>>(p);
-    if (int rc = launched("k_readout_g")) return rc;
+    if (int rc = g_piece<E, DV>(p)) return rc;
+    const int64_t two = p.rows <= kTwoRows ? p.rows : 0;  // (rows of G's second term)
     if (a->grad_weight) {
         GradP w{};
         w.a = DV ? b.hs : p.g;
@@ -748,7 +844,7 @@ int piece(const BackP &b) {
         w.ldb = w.wb = DV ? p.ldg : b.ldhs;
         w.m = DV ? p.dim : p.n;
         w.n = DV ? p.n : p.dim;
-        w.k = p.rows;
+        w.k = p.rows + two;
         uint16_t *out = static_cast<uint16_t *>(a->grad_weight) + (DV ? p.v0 : p.v0 * a->grad_weight_ld);
         w.ldo = a->grad_weight_ld;
         w.out = b.sw.splits > 1 ? nullptr : out;
@@ -766,7 +862,7 @@ int piece(const BackP &b) {
         h.b = p.w;
         h.ldb = p.ldw;
         h.wb = p.wwidth;
-        h.m = p.rows;
+        h.m = p.rows + two;
         h.n = p.dim;
         h.k = p.n;
         h.ldo = a->grad_hidden_ld;
@@ -778,7 +874,7 @@ int piece(const BackP &b) {
         h.fixed = b.fixed;
         if (int rc = product<E, false, !DV>(h, b.sh)) return rc;
         if (b.hslab && b.last)
-            if (int rc = fold<E>(h, b.sh.splits, out)) return rc;
+            if (int rc = fold<E>(h, b.sh.splits, out, two)) return rc;
     }
     return 0;
 }
@@ -800,15 +896,16 @@ int backward(const NtRlReadoutStatsGradArgs *a) {
     if (!wdirect) most = std::min(most, (int64_t(1) << 27) / kp);
     const int64_t cols = piece_cols(V, most), pieces = ceil_div(V, cols);
     // dH: [rows, dim], k the piece's columns; dW: [vocab, dim] or [dim, vocab], k the rows
+    const int64_t two = R <= kTwoRows ? R : 0;
     const Split sh = split_k(R, d, round_up(std::min(cols, V), 8));
-    const Split sw = dv ? split_k(d, std::min(cols, V), R) : split_k(std::min(cols, V), d, R);
-    const bool hslab = sh.splits > 1 || pieces > 1;
+    const Split sw = dv ? split_k(d, std::min(cols, V), R + two) : split_k(std::min(cols, V), d, R + two);
+    const bool hslab = sh.splits > 1 || pieces > 1 || two;
     Scratch s;
-    const size_t o_h = s.add(hdirect ? 0 : R * kp * 2), o_hs = s.add(R * kp * 2);
+    const size_t o_h = s.add(hdirect ? 0 : R * kp * 2), o_hs = s.add((R + two) * kp * 2);
     const size_t o_w = s.add(wdirect ? 0 : (dv ? d * cols : cols * kp) * 2);
     const size_t o_coef = s.add(R * 16), o_up = s.add(R * 4), o_top = s.add(4);
-    const size_t o_g = s.add(R * cols * 2);
-    const size_t o_sh = s.add(a->grad_hidden && hslab ? sh.splits * R * d * 4 : 0);
+    const size_t o_g = s.add((R + two) * cols * 2);
+    const size_t o_sh = s.add(a->grad_hidden && hslab ? sh.splits * (R + two) * d * 4 : 0);
     const size_t o_sw = s.add(a->grad_weight && sw.splits > 1 ? sw.splits * std::min(cols, V) * d * 4 : 0);
     void *ws = nullptr;
     if (int rc = scratch_alloc(s.need, &ws)) return rc;
@@ -832,7 +929,7 @@ int backward(const NtRlReadoutStatsGradArgs *a) {
     hipLaunchKernelGGL(k_readout_coef, dim3(1), dim3(1024), 0, ctx().stream, c);
     if (int rc = launched("k_readout_coef")) return rc;
     if (a->grad_weight)
-        if (int rc = copy_rows(a->hidden, R, d, a->ldh, s.at<uint8_t>(o_hs), kp * 2, c.coef, up, top)) return rc;
+        if (int rc = copy_rows(a->hidden, R, d, a->ldh, s.at<uint8_t>(o_hs), kp * 2, c.coef, up, top, two)) return rc;
     PieceP p{};
     p.h = static_cast<const uint8_t *>(a->hidden);
     p.ldh = a->ldh * 2;
@@ -855,8 +952,6 @@ int backward(const NtRlReadoutStatsGradArgs *a) {
         p.v0 = v0;
         p.ldg = round_up(n, 8) * 2;
         p.mask = mask_at(a->mask_kind, a->mask, a->mask_ld, v0);
-        p.tm = uint32_t(ceil_div(R, kTile));
-        p.tn = uint32_t(ceil_div(n, kTile));
         BackP b{a, p, sh, sw, hslab, s.at<uint8_t>(o_hs), kp * 2, s.at<float>(o_sh), s.at<float>(o_sw), up, top, fixed,
                 v0 + cols >= V};
         const int rc = dv ? (f16 ? piece<F16, true>(b) : piece<Bf16, true>(b)) : (f16 ? piece<F16, false>(b) : piece<Bf16, false>(b));
