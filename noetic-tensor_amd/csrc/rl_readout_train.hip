@@ -41,7 +41,6 @@ using namespace tile;
 constexpr float kLog2e = 1.44269504088896340736f;
 constexpr double kLog2eD = 1.4426950408889634074, kLn2 = 0.69314718055994530942;
 
-typedef uint32_t u32u __attribute__((aligned(1)));
 typedef u32x4 u32x4u __attribute__((aligned(1)));
 typedef f32x16 f32x16_t;
 
@@ -53,27 +52,81 @@ struct MaskP {
     int64_t ld;
 };
 
-// Four neighbouring columns of a row of logits under the mask: -inf where it excludes them or past the
-// vocabulary's `n` columns; under an additive mask x c + mask log2 e, else x itself (y = x c follows in the sum's fma).
-__device__ __forceinline__ void masked4(const MaskP &m, int64_t row, int col, int n, float c, float (&x)[4]) {
-    if (col + 4 <= n) {
+// A wave's block of the mask, 32 rows by 32 TN columns, through LDS: whole 16-byte pieces of its rows in (a lane's
+// own four columns of 32 rows would be 16 scattered loads), a lane's four columns of its row out. Columns past the
+// vocabulary's `n` count as excluded.
+template <int TN>
+struct MaskBlock {
+    static constexpr int kU8 = 32 * TN + 16, kF32 = 128 * TN + 16;  // bytes of a row in LDS
+    static constexpr int kLds = 32 * kF32;
+    // (row: this lane's rows of the loads below are row0 .. row0 + 31, clamped to `rows` of them)
+    static __device__ __forceinline__ void in(uint8_t *lds, const MaskP &m, int64_t row0, int rows, int col, int n, int lane) {
         if (m.u8) {
-            const uint32_t k = *reinterpret_cast<const u32u *>(m.u8 + row * m.ld + col);
+            constexpr int kPer = 2 * TN, kRows = 64 / kPer, kLoads = 32 / kRows;
+            const int c = (lane % kPer) * 16, left = n - col - c;
+            u32x4 v[kLoads];
 #pragma unroll
-            for (int e = 0; e < 4; e++) x[e] = (k >> (8 * e)) & 0xffu ? x[e] : -INFINITY;
-        } else if (m.f32) {
-            float f[4];
-            __builtin_memcpy(f, m.f32 + row * m.ld + col, 16);
+            for (int g = 0; g < kLoads; g++) {
+                const int r = g * kRows + lane / kPer;
+                const uint8_t *s = m.u8 + (row0 + (r < rows ? r : rows - 1)) * m.ld + col + c;
+                v[g] = u32x4{0, 0, 0, 0};
+                if (left >= 16) v[g] = *reinterpret_cast<const u32x4u *>(s);
+                else
+                    for (int e = 0; e < left; e++) v[g][e / 4] |= uint32_t(s[e]) << (8 * (e % 4));
+            }
 #pragma unroll
-            for (int e = 0; e < 4; e++) x[e] = fmaf(f[e], kLog2e, x[e] * c);
+            for (int g = 0; g < kLoads; g++)
+                *reinterpret_cast<u32x4 *>(lds + (g * kRows + lane / kPer) * kU8 + c) = v[g];
+        } else {
+            constexpr int kPer = 8 * TN, kRows = 64 / kPer, kLoads = 32 / kRows, kBatch = 8;
+            const int c = (lane % kPer) * 4, left = n - col - c;
+#pragma unroll
+            for (int b = 0; b < kLoads; b += kBatch) {
+                float v[kBatch][4];
+#pragma unroll
+                for (int g = 0; g < kBatch; g++) {
+                    const int r = (b + g) * kRows + lane / kPer;
+                    const float *s = m.f32 + (row0 + (r < rows ? r : rows - 1)) * m.ld + col + c;
+                    if (left >= 4) __builtin_memcpy(v[g], s, 16);
+                    else
+                        for (int e = 0; e < 4; e++) v[g][e] = e < left ? s[e] : -INFINITY;
+                }
+#pragma unroll
+                for (int g = 0; g < kBatch; g++) __builtin_memcpy(lds + ((b + g) * kRows + lane / kPer) * kF32 + c * 4, v[g], 16);
+            }
         }
-        return;
     }
+    // x under it: -inf where excluded; under an additive mask x c + mask log2 e, else x itself (y = x c follows in
+    // the sum's fma)
+    static __device__ __forceinline__ void out(const uint8_t *lds, const MaskP &m, float c, int lane, float (&x)[4 * TN][4]) {
+        const int r = lane % 32, h = lane / 32;
+        if (m.u8) {
 #pragma unroll
-    for (int e = 0; e < 4; e++) {
-        if (col + e >= n) x[e] = -INFINITY;
-        else if (m.u8) x[e] = m.u8[row * m.ld + col + e] ? x[e] : -INFINITY;
-        else if (m.f32) x[e] = fmaf(m.f32[row * m.ld + col + e], kLog2e, x[e] * c);
+            for (int q = 0; q < 4 * TN; q++) {
+                const uint32_t k = *reinterpret_cast<const uint32_t *>(lds + r * kU8 + 8 * q + 4 * h);
+#pragma unroll
+                for (int e = 0; e < 4; e++) x[q][e] = (k >> (8 * e)) & 0xffu ? x[q][e] : -INFINITY;
+            }
+        } else {
+#pragma unroll
+            for (int q = 0; q < 4 * TN; q++) {
+                float f[4];
+                __builtin_memcpy(f, lds + r * kF32 + 32 * q + 16 * h, 16);
+#pragma unroll
+                for (int e = 0; e < 4; e++) x[q][e] = fmaf(f[e], kLog2e, x[q][e] * c);
+            }
+        }
+    }
+};
+
+// Without a mask: the columns past the vocabulary's end, `left` columns from this lane's first.
+template <int Q>
+__device__ __forceinline__ void ended(float (&x)[Q][4], int left) {
+#pragma unroll
+    for (int q = 0; q < Q; q++) {
+#pragma unroll
+        for (int e = 0; e < 4; e++) x[q][e] = 8 * q + e < left ? x[q][e] : -INFINITY;
+        __builtin_amdgcn_sched_barrier(0);  // (or every comparison is made at once, into more registers than there are)
     }
 }
 
@@ -117,7 +170,7 @@ typedef Shape<4, 2, 2> Large;   // 256 x 256
 typedef Shape<2, 2, 2> Medium;  // 128 x 256
 typedef Shape<1, 2, 1> Small;   // 64 x 128
 
-template <class E, class S, bool BTR, bool ENT>
+template <class E, class S, bool BTR, bool ENT, bool MASK>
 __global__ __launch_bounds__(S::kThreads, 1) void k_readout_stats(PieceP p) {
     constexpr int TM = S::TM, TN = S::TN, WM = S::WM, WN = S::WN;
     typedef Tile<E, TM, TN, WM, WN, false, BTR> T;
@@ -130,8 +183,9 @@ __global__ __launch_bounds__(S::kThreads, 1) void k_readout_stats(PieceP p) {
           weight_rows<T, BTR>(p, in), p.kbytes, wave, lane);
     const int wm = wave / WN, wn = wave % WN;
     const int col0 = in * T::BN + 32 * TN * wn + 4 * (lane / 32);
-    const bool plain = !p.mask.u8 && !p.mask.f32 && in * T::BN + T::BN <= p.n;  // every column as it is
-    const float c = p.mask.f32 ? 1.0f : p.c;                                   // y = acc c from here on
+    const float c = MASK && p.mask.f32 ? 1.0f : p.c;  // y = x c under the mask
+    static_assert(MaskBlock<TN>::kLds * WM * WN <= T::kLds, "the mask's blocks fit");
+    uint8_t *const mlds = lds + wave * MaskBlock<TN>::kLds;
     const int64_t block = p.block0 + int64_t(in) * WN + wn;
 #pragma unroll
     for (int i = 0; i < TM; i++) {
@@ -155,9 +209,14 @@ __global__ __launch_bounds__(S::kThreads, 1) void k_readout_stats(PieceP p) {
         for (int q = 0; q < 4 * TN; q++)
 #pragma unroll
             for (int e = 0; e < 4; e++) x[q][e] = t.acc[i][q / 4][4 * (q % 4) + e];
-        if (!plain)
-#pragma unroll
-            for (int q = 0; q < 4 * TN; q++) masked4(p.mask, r, col0 + 8 * q, p.n, p.c, x[q]);
+        if constexpr (MASK) {
+            const int64_t row0 = row - lane % 32;
+            if (row0 < p.rows)
+                MaskBlock<TN>::in(mlds, p.mask, row0, p.rows - row0 < 32 ? int(p.rows - row0) : 32, in * T::BN + 32 * TN * wn, p.n, lane);
+            MaskBlock<TN>::out(mlds, p.mask, p.c, lane, x);
+        } else if (in * T::BN + T::BN > p.n) {
+            ended(x, p.n - col0);
+        }
         float m = -INFINITY;
 #pragma unroll
         for (int q = 0; q < 4 * TN; q++)
@@ -373,7 +432,7 @@ __device__ __forceinline__ float widened(uint32_t h) {
 // A piece's G. TWO: up to 64 rows, where one rounding of a row's largest entries (its token's above all) is not averaged away in
 // the gradients' sums: what the rounding left goes into rows `rows` .. 2 rows - 1, and the products take both.
 // A stage of 32 k or a 64-row tile costs the same at twice so few rows.
-template <class E, class S, bool BTR, bool TWO>
+template <class E, class S, bool BTR, bool TWO, bool MASK>
 __global__ __launch_bounds__(S::kThreads, 1) void k_readout_g(PieceP p) {
     constexpr int TM = S::TM, TN = S::TN, WM = S::WM, WN = S::WN;
     typedef Tile<E, TM, TN, WM, WN, false, BTR> T;
@@ -386,10 +445,11 @@ __global__ __launch_bounds__(S::kThreads, 1) void k_readout_g(PieceP p) {
           weight_rows<T, BTR>(p, in), p.kbytes, wave, lane);
     const int wm = wave / WN, wn = wave % WN;
     const int col0 = in * T::BN + 32 * TN * wn + 4 * (lane / 32);
-    const bool plain = !p.mask.u8 && !p.mask.f32 && in * T::BN + T::BN <= p.n;
-    const float c = p.mask.f32 ? 1.0f : p.c;
+    const float c = MASK && p.mask.f32 ? 1.0f : p.c;
     const int64_t bytes = p.ldg - (in * T::BN + 32 * TN * wn) * 2;
-    static_assert(store_bytes<TN>(2) * WM * WN <= T::kLds, "the blocks fit");
+    constexpr int kMask = MASK ? MaskBlock<TN>::kLds : 0, kWave = store_bytes<TN>(2) + kMask;
+    static_assert(kWave * WM * WN <= T::kLds, "the blocks fit");
+    uint8_t *const mlds = lds + wave * kWave, *const slds = mlds + kMask;
     float4 coef[TM];
     int tok[TM];  // the token's column from this lane's first, or -1
 #pragma unroll
@@ -402,7 +462,7 @@ __global__ __launch_bounds__(S::kThreads, 1) void k_readout_g(PieceP p) {
     if (bytes <= 0) return;
 #pragma unroll
     for (int i = 0; i < TM; i++) {
-        const int64_t row0 = int64_t(im) * T::BM + 32 * (TM * wm + i), row = row0 + lane % 32;
+        const int64_t row0 = int64_t(im) * T::BM + 32 * (TM * wm + i);
         if (row0 >= p.rows) break;
         const float4 k = coef[i];
         const bool dead = k.x == INFINITY;
@@ -414,9 +474,12 @@ __global__ __launch_bounds__(S::kThreads, 1) void k_readout_g(PieceP p) {
         for (int q = 0; q < 4 * TN; q++)
 #pragma unroll
             for (int e = 0; e < 4; e++) x[q][e] = t.acc[i][q / 4][4 * (q % 4) + e];
-        if (!plain)
-#pragma unroll
-            for (int q = 0; q < 4 * TN; q++) masked4(p.mask, row < p.rows ? row : p.rows - 1, col0 + 8 * q, p.n, p.c, x[q]);
+        if constexpr (MASK) {
+            MaskBlock<TN>::in(mlds, p.mask, row0, p.rows - row0 < 32 ? int(p.rows - row0) : 32, in * T::BN + 32 * TN * wn, p.n, lane);
+            MaskBlock<TN>::out(mlds, p.mask, p.c, lane, x);
+        } else if (in * T::BN + T::BN > p.n) {
+            ended(x, p.n - col0);
+        }
 #pragma unroll
         for (int q = 0; q < 4 * TN; q++) {
             float g[4];
@@ -438,8 +501,8 @@ __global__ __launch_bounds__(S::kThreads, 1) void k_readout_g(PieceP p) {
         }
         const int rows = p.rows - row0 < 32 ? int(p.rows - row0) : 32, have = bytes < 64 * TN ? int(bytes) : 64 * TN;
         uint8_t *o = p.g + row0 * p.ldg + (in * T::BN + 32 * TN * wn) * 2;
-        store_block<TN>(lds + wave * store_bytes<TN>(2), v, lane, o, p.ldg, rows, have);
-        if constexpr (TWO) store_block<TN>(lds + wave * store_bytes<TN>(2), lo, lane, o + p.rows * p.ldg, p.ldg, rows, have);
+        store_block<TN>(slds, v, lane, o, p.ldg, rows, have);
+        if constexpr (TWO) store_block<TN>(slds, lo, lane, o + p.rows * p.ldg, p.ldg, rows, have);
     }
 }
 
@@ -542,23 +605,20 @@ __global__ __launch_bounds__(256) void k_readout_fold(const float *slab, int spl
         const int64_t r = i / per, c = (i - r * per) * 4;
         const int have = n - c >= 4 ? 4 : int(n - c);
         float x[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-        for (int z0 = 0; z0 < terms; z0 += 8) {  // (eight loads in flight)
-            float v[8][4];
+        auto at = [&](int z) { return slab + (two ? (z / 2) * m + r + (z % 2) * two : z * m + r) * n + c; };
+        int z = 0;
+        if (have == 4)
+            for (; z + 8 <= terms; z += 8) {  // (eight loads in flight)
+                float v[8][4];
 #pragma unroll
-            for (int k = 0; k < 8; k++) {
-                v[k][0] = v[k][1] = v[k][2] = v[k][3] = 0.0f;
-                const int z = z0 + k;
-                if (z >= terms) continue;
-                const float *s = slab + (two ? (z / 2) * m + r + (z % 2) * two : z * m + r) * n + c;
-                if (have == 4) __builtin_memcpy(v[k], s, 16);
-                else
-                    for (int e = 0; e < have; e++) v[k][e] = s[e];
+                for (int k = 0; k < 8; k++) __builtin_memcpy(v[k], at(z + k), 16);
+#pragma unroll
+                for (int k = 0; k < 8; k++)
+#pragma unroll
+                    for (int e = 0; e < 4; e++) x[e] += v[k][e];
             }
-#pragma unroll
-            for (int k = 0; k < 8; k++)
-#pragma unroll
-                for (int e = 0; e < 4; e++) x[e] += v[k][e];
-        }
+        for (; z < terms; z++)
+            for (int e = 0; e < have; e++) x[e] += at(z)[e];
         float f = scale ? *scale * fixed : fixed;
         if (row_scale) f *= row_scale[r];
         uint16_t *o = out + r * ldo + c;
@@ -680,8 +740,14 @@ int launch_stats(PieceP p, bool ent) {
     p.tm = uint32_t(ceil_div(p.rows, S::kRows));
     p.tn = uint32_t(ceil_div(p.n, S::kCols));
     const dim3 grid(p.tm * p.tn), block(S::kThreads);
-    if (ent) k_readout_stats<E, S, BTR, true><<<grid, block, 0, ctx().stream>>>(p);
-    else k_readout_stats<E, S, BTR, false><<<grid, block, 0, ctx().stream>>>(p);
+    hipStream_t st = ctx().stream;
+    if (p.mask.u8 || p.mask.f32) {
+        if (ent) k_readout_stats<E, S, BTR, true, true><<<grid, block, 0, st>>>(p);
+        else k_readout_stats<E, S, BTR, false, true><<<grid, block, 0, st>>>(p);
+    } else {
+        if (ent) k_readout_stats<E, S, BTR, true, false><<<grid, block, 0, st>>>(p);
+        else k_readout_stats<E, S, BTR, false, false><<<grid, block, 0, st>>>(p);
+    }
     return launched("k_readout_stats");
 }
 
@@ -698,7 +764,9 @@ template <class E, class S, bool BTR, bool TWO>
 int launch_g(PieceP p) {
     p.tm = uint32_t(ceil_div(p.rows, S::kRows));
     p.tn = uint32_t(ceil_div(p.n, S::kCols));
-    k_readout_g<E, S, BTR, TWO><<<dim3(p.tm * p.tn), dim3(S::kThreads), 0, ctx().stream>>>(p);
+    const dim3 grid(p.tm * p.tn), block(S::kThreads);
+    if (p.mask.u8 || p.mask.f32) k_readout_g<E, S, BTR, TWO, true><<<grid, block, 0, ctx().stream>>>(p);
+    else k_readout_g<E, S, BTR, TWO, false><<<grid, block, 0, ctx().stream>>>(p);
     return launched("k_readout_g");
 }
 
