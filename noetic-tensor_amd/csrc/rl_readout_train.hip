@@ -148,8 +148,8 @@ struct PieceP {
     float *xtok;              // [rows] the token's raw logit
     // backward
     const float4 *coef;       // [rows] {lse log2 e (+inf: nothing flows), a, b, the token's term}
-    uint8_t *g;               // [rows, ldg bytes], zeros from n to the row's end
-    int64_t ldg;
+    uint8_t *g;               // [rows, ldg bytes], of which gbytes are written: zeros past n
+    int64_t ldg, gbytes;
 };
 
 template <class T, bool BTR>
@@ -166,9 +166,9 @@ struct Shape {
     static constexpr int TM = TM_, TN = 4, WM = WM_, WN = WN_;
     static constexpr int kThreads = 64 * WM * WN, kRows = 32 * TM * WM, kCols = 128 * WN;
 };
-typedef Shape<4, 2, 2> Large;   // 256 x 256
-typedef Shape<2, 2, 2> Medium;  // 128 x 256
-typedef Shape<1, 2, 1> Small;   // 64 x 128
+typedef Shape<4, 2, 2> Large;   // 256 x 256, a workgroup a CU
+typedef Shape<1, 4, 1> Medium;  // 128 x 128, two workgroups a CU: one's output while the other multiplies
+typedef Shape<1, 2, 1> Small;   // 64 x 128, two workgroups of two waves a CU
 
 template <class E, class S, bool BTR, bool ENT, bool MASK>
 __global__ __launch_bounds__(S::kThreads, 1) void k_readout_stats(PieceP p) {
@@ -446,10 +446,10 @@ __global__ __launch_bounds__(S::kThreads, 1) void k_readout_g(PieceP p) {
     const int wm = wave / WN, wn = wave % WN;
     const int col0 = in * T::BN + 32 * TN * wn + 4 * (lane / 32);
     const float c = MASK && p.mask.f32 ? 1.0f : p.c;
-    const int64_t bytes = p.ldg - (in * T::BN + 32 * TN * wn) * 2;
-    constexpr int kMask = MASK ? MaskBlock<TN>::kLds : 0, kWave = store_bytes<TN>(2) + kMask;
+    const int64_t bytes = p.gbytes - (in * T::BN + 32 * TN * wn) * 2;
+    constexpr int kMask = MASK ? MaskBlock<TN>::kLds : 0, kWave = store_bytes<TN>(2) > kMask ? store_bytes<TN>(2) : kMask;
     static_assert(kWave * WM * WN <= T::kLds, "the blocks fit");
-    uint8_t *const mlds = lds + wave * kWave, *const slds = mlds + kMask;
+    uint8_t *const mlds = lds + wave * kWave, *const slds = mlds;  // (the mask's block is read before G's is written)
     float4 coef[TM];
     int tok[TM];  // the token's column from this lane's first, or -1
 #pragma unroll
@@ -729,10 +729,68 @@ int64_t piece_cols(int64_t vocab, int64_t cols) {
     return std::min(round_up(ceil_div(vocab, pieces), kTile), round_up(vocab, kTile));
 }
 
-// The tile of a product of `rows` rows and `cols` columns.
+// The tile of a product [m, k] x [k, n] and the splits of k (`split`), by what they cost: rounds of the workgroups
+// that run at once, each its stages of 32 k and its output. Measured (us a stage, a round full): 0.92, 0.57 and
+// 0.36 for Large, Medium and Small, or 0.33 and 0.25 for a round of one workgroup a CU; an output of Large 5 us
+// (Medium's and Small's are half and a quarter of the CU's, and go on beside the other workgroup's products), the
+// slabs of split k 4 us and their bytes at 4 TB/s. So 4096 x 128256 takes Large, 333 x 50257 x 1001 Medium
+// (G 99 -> 72 us), 64 rows Small.
 enum class Size { kSmall, kMedium, kLarge };
-Size size_of(int64_t rows) {
-    return rows <= 64 ? Size::kSmall : rows <= 128 ? Size::kMedium : Size::kLarge;
+struct Plan {
+    Size size;
+    int64_t per, splits;  // k of a split, a multiple of 32
+    double cost;
+};
+Plan plan(int64_t m, int64_t n, int64_t k, bool split) {
+    struct Kind {
+        Size size;
+        int64_t rows, cols, slots;
+        double stage, alone, output;
+    };
+    static const Kind kinds[] = {{Size::kLarge, Large::kRows, Large::kCols, 256, 0.92, 0.92, 6.0},
+                                 {Size::kMedium, Medium::kRows, Medium::kCols, 512, 0.57, 0.33, 2.5},
+                                 {Size::kSmall, Small::kRows, Small::kCols, 512, 0.36, 0.25, 1.5}};
+    Plan best{};
+    for (const Kind &c : kinds) {
+        const int64_t tiles = ceil_div(m, c.rows) * ceil_div(n, c.cols);
+        for (int64_t s = 1; s <= 64; s = s < 4 ? s + 1 : s + s / 4) {
+            const int64_t per = round_up(ceil_div(k, s), 32), splits = ceil_div(k, per);
+            if (s > 1 && (!split || splits < s || per < 256)) continue;
+            const int64_t wgs = tiles * splits, rounds = ceil_div(wgs, c.slots);
+            const double stage = wgs <= 256 ? c.alone : c.stage;
+            const double cost = double(rounds) * (double(per / 32) * stage + c.output) +
+                                (splits > 1 ? 4.0 + double(splits) * double(m) * double(n) * 8e-6 / 4.0 : 0.0);
+            if (best.per == 0 || cost < best.cost) best = Plan{c.size, per, splits, cost};
+        }
+    }
+    return best;
+}
+
+// The columns of [m, n] that go by Large tiles in whole rounds of 256, where the rest by itself costs less than
+// one more round of them does (a multiple of a tile's; 0: no such split). 2048 x 50304 is 1576 tiles: 1536 and the
+// last 1152 columns apart (stats 828 -> 748 us).
+int64_t whole_rounds(int64_t m, int64_t n, int64_t k) {
+    const Plan all = plan(m, n, k, false);
+    if (all.size != Size::kLarge) return 0;
+    const int64_t tm = ceil_div(m, Large::kRows), tiles = tm * ceil_div(n, Large::kCols);
+    const int64_t cols = tiles / 256 * 256 / tm * Large::kCols;
+    if (cols <= 0 || cols >= n) return 0;
+    return plan(m, cols, k, false).cost + plan(m, n - cols, k, false).cost + 4.0 < all.cost ? cols : 0;
+}
+
+// Columns c0 .. c0 + n - 1 of a piece (c0 a multiple of 256).
+PieceP part_of(const PieceP &p, bool dv, int64_t c0, int64_t n) {
+    PieceP q = p;
+    q.w += dv ? c0 * 2 : c0 * p.ldw;
+    q.wwidth -= dv ? c0 * 2 : 0;
+    q.n = int(n);
+    q.v0 += c0;
+    q.block0 += c0 / 128;
+    q.g += c0 * 2;
+    q.gbytes = c0 + n < p.n ? n * 2 : p.gbytes - c0 * 2;
+    if (p.mask.u8) q.mask.u8 += c0;
+    if (p.mask.f32) q.mask.f32 += c0;
+    return q;
 }
 
 template <class E, class S, bool BTR>
@@ -753,7 +811,11 @@ int launch_stats(PieceP p, bool ent) {
 
 template <class E, bool BTR>
 int stats(const PieceP &p, bool ent) {
-    switch (size_of(p.rows)) {
+    if (const int64_t c = whole_rounds(p.rows, p.n, p.dim)) {
+        if (int rc = launch_stats<E, Large, BTR>(part_of(p, BTR, 0, c), ent)) return rc;
+        return stats<E, BTR>(part_of(p, BTR, c, p.n - c), ent);
+    }
+    switch (plan(p.rows, p.n, p.dim, false).size) {
         case Size::kSmall: return launch_stats<E, Small, BTR>(p, ent);
         case Size::kMedium: return launch_stats<E, Medium, BTR>(p, ent);
         default: return launch_stats<E, Large, BTR>(p, ent);
@@ -770,15 +832,21 @@ int launch_g(PieceP p) {
     return launched("k_readout_g");
 }
 
+constexpr int64_t kTwoRows = 64;  // G in two terms for so many rows: the Small tile's
+
 template <class E, bool BTR>
 int g_piece(const PieceP &p) {
-    switch (size_of(p.rows)) {
-        case Size::kSmall: return launch_g<E, Small, BTR, true>(p);
+    if (p.rows <= kTwoRows) return launch_g<E, Small, BTR, true>(p);
+    if (const int64_t c = whole_rounds(p.rows, p.n, p.dim)) {
+        if (int rc = launch_g<E, Large, BTR, false>(part_of(p, BTR, 0, c))) return rc;
+        return g_piece<E, BTR>(part_of(p, BTR, c, p.n - c));
+    }
+    switch (plan(p.rows, p.n, p.dim, false).size) {
+        case Size::kSmall: return launch_g<E, Small, BTR, false>(p);
         case Size::kMedium: return launch_g<E, Medium, BTR, false>(p);
         default: return launch_g<E, Large, BTR, false>(p);
     }
 }
-constexpr int64_t kTwoRows = 64;  // G in two terms for so many rows: the Small tile's
 
 int forward(const NtRlReadoutStatsArgs *a) {
     const bool dv = a->layout == NT_READOUT_W_DV;
@@ -849,17 +917,6 @@ int forward(const NtRlReadoutStatsArgs *a) {
     return launched("k_readout_merge");
 }
 
-// One product of the backward: tiles, and splits of k where the tiles alone leave CUs idle.
-struct Split {
-    int64_t per, splits;
-};
-Split split_k(int64_t m, int64_t n, int64_t k) {
-    const int64_t tiles = ceil_div(m, kTile) * ceil_div(n, kTile);
-    const int64_t want = std::min(std::max<int64_t>(1, 256 / tiles), std::max<int64_t>(1, k / 256));
-    const int64_t per = round_up(ceil_div(k, want), 32);
-    return Split{per, ceil_div(k, per)};
-}
-
 template <class E>
 int fold(const GradP &p, int64_t splits, uint16_t *out, int64_t two = 0) {
     const int64_t n = (two ? two : p.m) * ceil_div(p.n, 4);
@@ -869,7 +926,7 @@ int fold(const GradP &p, int64_t splits, uint16_t *out, int64_t two = 0) {
 }
 
 template <class E, class S, bool ATR, bool BTR>
-int launch_product(GradP p, const Split &s) {
+int launch_product(GradP p, const Plan &s) {
     p.per = s.per;
     p.tm = uint32_t(ceil_div(p.m, S::kRows));
     p.tn = uint32_t(ceil_div(p.n, S::kCols));
@@ -878,17 +935,19 @@ int launch_product(GradP p, const Split &s) {
 }
 
 template <class E, bool ATR, bool BTR>
-int product(const GradP &p, const Split &s) {
-    if constexpr (!ATR)  // (dH: as many rows as there are, or twice them)
-        if (p.m <= 128) return launch_product<E, Medium, ATR, BTR>(p, s);
-    return launch_product<E, Large, ATR, BTR>(p, s);
+int product(const GradP &p, const Plan &s) {
+    switch (s.size) {
+        case Size::kSmall: return launch_product<E, Small, ATR, BTR>(p, s);
+        case Size::kMedium: return launch_product<E, Medium, ATR, BTR>(p, s);
+        default: return launch_product<E, Large, ATR, BTR>(p, s);
+    }
 }
 
 // One piece of the vocabulary: its G, its rows of dW, its share of dH.
 struct BackP {
     const NtRlReadoutStatsGradArgs *a;
     PieceP p;
-    Split sh, sw;
+    Plan sh, sw;
     bool hslab;
     const uint8_t *hs;  // the scaled hidden states, [rows, ldhs bytes]
     int64_t ldhs;
@@ -919,7 +978,19 @@ int piece(const BackP &b) {
         w.slab = b.slab_w;
         w.scale = b.top;
         w.fixed = b.fixed;
-        if (int rc = product<E, true, true>(w, b.sw)) return rc;
+        const int64_t c = b.sw.splits > 1 ? 0 : whole_rounds(DV ? w.m : w.n, DV ? w.n : w.m, w.k);
+        if (c) {  // whole rounds of the vocabulary's side, and its rest
+            GradP first = w, rest = w;
+            (DV ? first.n : first.m) = c;
+            (DV ? rest.n : rest.m) -= c;
+            (DV ? rest.b : rest.a) += c * 2;
+            (DV ? rest.wb : rest.wa) -= c * 2;
+            rest.out += DV ? c : c * rest.ldo;
+            if (int rc = launch_product<E, Large, true, true>(first, b.sw)) return rc;
+            if (int rc = product<E, true, true>(rest, plan(rest.m, rest.n, rest.k, false))) return rc;
+        } else if (int rc = product<E, true, true>(w, b.sw)) {
+            return rc;
+        }
         if (b.sw.splits > 1)
             if (int rc = fold<E>(w, b.sw.splits, out)) return rc;
     }
@@ -965,8 +1036,9 @@ int backward(const NtRlReadoutStatsGradArgs *a) {
     const int64_t cols = piece_cols(V, most), pieces = ceil_div(V, cols);
     // dH: [rows, dim], k the piece's columns; dW: [vocab, dim] or [dim, vocab], k the rows
     const int64_t two = R <= kTwoRows ? R : 0;
-    const Split sh = split_k(R, d, round_up(std::min(cols, V), 8));
-    const Split sw = dv ? split_k(d, std::min(cols, V), R + two) : split_k(std::min(cols, V), d, R + two);
+    const int64_t width = std::min(cols, V);
+    const Plan sh = plan(R + two, d, round_up(width, 8), true);
+    const Plan sw = dv ? plan(d, width, R + two, true) : plan(width, d, R + two, true);
     const bool hslab = sh.splits > 1 || pieces > 1 || two;
     Scratch s;
     const size_t o_h = s.add(hdirect ? 0 : R * kp * 2), o_hs = s.add((R + two) * kp * 2);
@@ -1018,7 +1090,7 @@ int backward(const NtRlReadoutStatsGradArgs *a) {
         if (int rc = piece_weight(a->weight, dv, wdirect, v0, n, d, a->ldw, s.at<uint8_t>(o_w), &p)) return rc;
         p.n = int(n);
         p.v0 = v0;
-        p.ldg = round_up(n, 8) * 2;
+        p.ldg = p.gbytes = round_up(n, 8) * 2;
         p.mask = mask_at(a->mask_kind, a->mask, a->mask_ld, v0);
         BackP b{a, p, sh, sw, hslab, s.at<uint8_t>(o_hs), kp * 2, s.at<float>(o_sh), s.at<float>(o_sw), up, top, fixed,
                 v0 + cols >= V};

@@ -17,6 +17,7 @@ from __future__ import annotations
 
 import ctypes as C
 import enum
+import math
 from typing import List, Optional, Sequence, Tuple
 
 import numpy as np
@@ -86,8 +87,8 @@ class Layout:
     """src/tensor/layout.rs:8-81: shape, element strides and element offset of a view."""
 
     def __init__(self, shape: Sequence[int], strides: Optional[Sequence[int]] = None, offset: int = 0):
-        self.shape = [int(d) for d in shape]
-        self.strides = [int(s) for s in (strides if strides is not None else _row_major(self.shape))]
+        self.shape = list(map(int, shape))
+        self.strides = list(map(int, strides)) if strides is not None else _row_major(self.shape)
         self.offset = int(offset)
         if len(self.shape) > MAX_RANK:
             raise ValueError(f"rank {len(self.shape)} (at most {MAX_RANK} on the device)")
@@ -97,7 +98,7 @@ class Layout:
         return Layout(shape)
 
     def numel(self) -> int:
-        return int(np.prod(self.shape)) if self.shape else 1
+        return math.prod(self.shape)
 
     def is_contiguous(self) -> bool:
         return self.strides == _row_major(self.shape)

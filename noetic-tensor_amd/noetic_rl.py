@@ -412,6 +412,7 @@ def launches() -> int:
 
 _NP = {"f32": np.float32, "bf16": np.uint16, "f16": np.uint16, "u8": np.uint8, "bool": np.uint8, "i8": np.int8,
        "i32": np.int32, "i64": np.int64, "f64": np.float64}
+_ITEMSIZE = {k: np.dtype(v).itemsize for k, v in _NP.items()}
 
 
 class Buffer:
@@ -438,10 +439,10 @@ class Tensor:
     "i32", "i64", "f64")."""
 
     def __init__(self, shape: Sequence[int], dtype: str, buf: Optional[Buffer] = None):
-        self.shape = tuple(int(s) for s in shape)
+        self.shape = tuple(map(int, shape))
         self.dtype = dtype
-        self.numel = int(np.prod(self.shape)) if self.shape else 1
-        nbytes = self.numel * np.dtype(_NP[dtype]).itemsize
+        self.numel = math.prod(self.shape)
+        nbytes = self.numel * _ITEMSIZE[dtype]
         self.buf = buf if buf is not None else Buffer(nbytes)
         self.nbytes = nbytes
 
@@ -969,7 +970,7 @@ def _readout_weight(hidden: Tensor, weight: Tensor, layout: str, who: str):
     if hidden.shape[-1] != d:
         raise ValueError(f"{who}: hidden's d {hidden.shape[-1]} against the weight's {d}")
     same_dtype(hidden.dtype, weight.dtype, "matmul")
-    rows = int(np.prod(hidden.shape[:-1]))
+    rows = math.prod(hidden.shape[:-1])
     S = weight.shape[0] if batched else 1
     return S, rows // S if S else 0, d, V, d * V
 
