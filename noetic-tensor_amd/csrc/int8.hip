@@ -21,6 +21,7 @@
 
 #include "../../include/noetic_ops.h"
 #include "nt_internal.hpp"
+#include "nt_plan.hpp"
 #include "nt_tile.hpp"
 
 namespace nt {
@@ -29,9 +30,6 @@ namespace {
 using namespace tile;
 
 typedef u32x4 u32x4u __attribute__((aligned(1)));
-
-int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
-int64_t round_up(int64_t a, int64_t b) { return ceil_div(a, b) * b; }
 
 template <int T>
 __device__ __forceinline__ float load_f32(const void *p, int64_t i) {
@@ -348,24 +346,51 @@ struct Int8P {
     const float *sa, *sb;
     void *out;
     int64_t ldo;
+    int64_t per;   // bytes of k of a split
+    int32_t *slab; // [splits][m][n] integer sums, or null: the outputs themselves
 };
 
-template <int TM, int TN, int WM, int WN, int OUT>
-__global__ __launch_bounds__(64 * WM * WN, 1) void k_int8_tiles(Int8P p) {
+constexpr int kSlab = -1;  // OUT: the integer sums of a split of k
+
+template <class S, int OUT>
+__global__ __launch_bounds__(S::kThreads, 1) void k_int8_tiles(Int8P p) {
+    constexpr int TM = S::TM, TN = S::TN, WM = S::WM, WN = S::WN;
     typedef Tile<I8, TM, TN, WM, WN, false, false> T;
     __shared__ __attribute__((aligned(16))) uint8_t lds[T::kLds];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     int im, in;
     tile_of(blockIdx.x, p.tm, p.tn, im, in);
     const int64_t m0 = int64_t(im) * T::BM, n0 = int64_t(in) * T::BN;
+    const int64_t k0 = blockIdx.y * p.per, kb = p.kb - k0 < p.per ? p.kb - k0 : p.per;
     T t;
-    t.run(lds, Operand{p.a + m0 * p.lda, p.lda, p.m - m0, p.kb}, Operand{p.b + n0 * p.ldb, p.ldb, p.n - n0, p.kb}, p.kb, wave, lane);
+    t.run(lds, Operand{p.a + m0 * p.lda + k0, p.lda, p.m - m0, kb}, Operand{p.b + n0 * p.ldb + k0, p.ldb, p.n - n0, kb}, kb, wave,
+          lane);
     const int wm = wave / WN, wn = wave % WN;
-    typedef typename std::conditional<OUT == NT_F32, u32x4, u32x2>::type V;
+    constexpr bool kWide = OUT == NT_F32 || OUT == kSlab;
+    typedef typename std::conditional<kWide, u32x4, u32x2>::type V;
     typedef typename std::conditional<OUT == NT_F16, F16, Bf16>::type E;
-    constexpr int kSize = OUT == NT_F32 ? 4 : 2;
+    constexpr int kSize = kWide ? 4 : 2;
     static_assert(store_bytes<TN>(kSize) * WM * WN <= T::kLds, "the blocks fit");
     const int64_t col0 = n0 + 32 * TN * wn;
+    if constexpr (OUT == kSlab) {
+        if (col0 >= p.n) return;
+#pragma unroll
+        for (int i = 0; i < TM; i++) {
+            const int64_t row0 = m0 + 32 * (TM * wm + i);
+            if (row0 >= p.m) break;
+            V v[4 * TN];
+#pragma unroll
+            for (int q = 0; q < 4 * TN; q++) {
+                const int x[4] = {t.acc[i][q / 4][4 * (q % 4)], t.acc[i][q / 4][4 * (q % 4) + 1], t.acc[i][q / 4][4 * (q % 4) + 2],
+                                  t.acc[i][q / 4][4 * (q % 4) + 3]};
+                v[q] = V{uint32_t(x[0]), uint32_t(x[1]), uint32_t(x[2]), uint32_t(x[3])};
+            }
+            store_block<TN>(lds + wave * store_bytes<TN>(4), v, lane,
+                            reinterpret_cast<uint8_t *>(p.slab + (int64_t(blockIdx.y) * p.m + row0) * p.n + col0), p.n * 4,
+                            p.m - row0 < 32 ? int(p.m - row0) : 32, p.n - col0 < 32 * TN ? int(p.n - col0) * 4 : 128 * TN);
+        }
+        return;
+    } else {
     // (every scale before the first store, which the compiler takes to change them)
     float sb[4 * TN][4];
 #pragma unroll
@@ -400,6 +425,34 @@ __global__ __launch_bounds__(64 * WM * WN, 1) void k_int8_tiles(Int8P p) {
         store_block<TN>(lds + wave * store_bytes<TN>(kSize), v, lane,
                         static_cast<uint8_t *>(p.out) + (row0 * p.ldo + col0) * kSize, p.ldo * kSize,
                         rows < 32 ? int(rows) : 32, bytes < 32 * TN * kSize ? int(bytes) : 32 * TN * kSize);
+    }
+    }
+}
+
+template <int T>
+__device__ __forceinline__ void put(void *out, int64_t at, float x) {
+    if constexpr (T == NT_F32) static_cast<float *>(out)[at] = x;
+    else if constexpr (T == NT_BF16) static_cast<uint16_t *>(out)[at] = uint16_t(pair16<Bf16>(x, 0.0f));
+    else static_cast<uint16_t *>(out)[at] = uint16_t(pair16<F16>(x, 0.0f));
+}
+
+// The splits' sums (integers: their order does not matter), scaled and rounded.
+template <int OUT>
+__global__ __launch_bounds__(256) void k_int8_fold(Int8P p, int splits) {
+    const int64_t total = p.m * p.n;
+    for (int64_t i = blockIdx.x * int64_t(256) + threadIdx.x; i < total; i += int64_t(gridDim.x) * 256) {
+        const int64_t r = i / p.n, c = i - r * p.n;
+        int sum = 0;
+        int z = 0;
+        for (; z + 8 <= splits; z += 8) {  // (eight loads in flight)
+            int v[8];
+#pragma unroll
+            for (int k = 0; k < 8; k++) v[k] = p.slab[(z + k) * total + i];
+#pragma unroll
+            for (int k = 0; k < 8; k++) sum += v[k];
+        }
+        for (; z < splits; z++) sum += p.slab[z * total + i];
+        put<OUT>(p.out, r * p.ldo + c, float(sum) * p.sa[r] * p.sb[c]);
     }
 }
 
@@ -455,10 +508,7 @@ __global__ __launch_bounds__(256) void k_int8_few(Int8P p) {
         for (int ii = 0; ii < M; ii++)
             if (rr == r && ii == i) sum = acc[rr][ii];
     const float x = float(sum) * p.sa[i] * p.sb[n0 + r];
-    const int64_t o = i * p.ldo + n0 + r;
-    if constexpr (OUT == NT_F32) static_cast<float *>(p.out)[o] = x;
-    else if constexpr (OUT == NT_BF16) static_cast<uint16_t *>(p.out)[o] = uint16_t(pair16<Bf16>(x, 0.0f));
-    else static_cast<uint16_t *>(p.out)[o] = uint16_t(pair16<F16>(x, 0.0f));
+    put<OUT>(p.out, i * p.ldo + n0 + r, x);
 }
 
 template <int M, int OUT>
@@ -467,16 +517,25 @@ int launch_few(const Int8P &p) {
     return launched("k_int8_few");
 }
 
-template <int TM, int WM, int WN, int OUT>
-int launch_tiles(Int8P p) {
-    p.tm = uint32_t(ceil_div(p.m, 32 * TM * WM)), p.tn = uint32_t(ceil_div(p.n, 128 * WN));
-    k_int8_tiles<TM, 4, WM, WN, OUT><<<dim3(p.tm * p.tn), dim3(64 * WM * WN), 0, ctx().stream>>>(p);
+template <class S, int OUT>
+int launch_tiles(Int8P p, int64_t splits) {
+    p.tm = uint32_t(ceil_div(p.m, S::kRows)), p.tn = uint32_t(ceil_div(p.n, S::kCols));
+    k_int8_tiles<S, OUT><<<dim3(p.tm * p.tn, unsigned(splits)), dim3(S::kThreads), 0, ctx().stream>>>(p);
     return launched("k_int8_tiles");
 }
 
-// Up to four rows row by row, 64 x 128 tiles for up to 64 rows, 128 x 256 for up to 128, else 256 x 256.
 template <int OUT>
-int tiles(const Int8P &p) {
+int by_size(const Int8P &p, const Plan &s) {
+    switch (s.size) {
+        case Size::kSmall: return launch_tiles<Small, OUT>(p, s.splits);
+        case Size::kMedium: return launch_tiles<Medium, OUT>(p, s.splits);
+        default: return launch_tiles<Large, OUT>(p, s.splits);
+    }
+}
+
+// Up to four rows row by row, else by tiles (`s`); a split k's sums through slabs.
+template <int OUT>
+int tiles(const Int8P &p, const Plan &s) {
     switch (p.m) {
         case 1: return launch_few<1, OUT>(p);
         case 2: return launch_few<2, OUT>(p);
@@ -484,9 +543,11 @@ int tiles(const Int8P &p) {
         case 4: return launch_few<4, OUT>(p);
         default: break;
     }
-    if (p.m <= 64) return launch_tiles<1, 2, 1, OUT>(p);
-    if (p.m <= 128) return launch_tiles<2, 2, 2, OUT>(p);
-    return launch_tiles<4, 2, 2, OUT>(p);
+    if (!p.slab) return by_size<OUT>(p, s);
+    if (int rc = by_size<kSlab>(p, s)) return rc;
+    k_int8_fold<OUT><<<dim3(unsigned(std::min<int64_t>(ceil_div(p.m * p.n, 256), 8192))), dim3(256), 0, ctx().stream>>>(
+        p, int(s.splits));
+    return launched("k_int8_fold");
 }
 
 int pad_rows(const int8_t *src, int64_t rows, int64_t cols, int64_t ld, uint8_t *out, int64_t ldo) {
@@ -506,14 +567,16 @@ int product(const int8_t *a, int64_t lda, const float *sa, const int8_t *b, int6
             int64_t k, int32_t dtype, void *out, int64_t ldo) {
     const bool ad = aligned(a, k, lda), bd = aligned(b, k, ldb);
     const int64_t kp = round_up(k, 16);
-    const int64_t abytes = ad ? 0 : m * kp;
-    const int64_t need = abytes + (bd ? 0 : n * kp);
+    const Plan s = plan(m, n, kp, true);
+    const int64_t abytes = ad ? 0 : round_up(m * kp, 256), bbytes = bd ? 0 : round_up(n * kp, 256);
+    const bool slabs = m > 4 && s.splits > 1;
+    const int64_t need = abytes + bbytes + (slabs ? s.splits * m * n * 4 : 0);
     void *ws = nullptr;
     if (need > 0)
         if (int rc = scratch_alloc(size_t(need), &ws)) return rc;
     uint8_t *pa = static_cast<uint8_t *>(ws), *pb = pa + abytes;
     Int8P p{reinterpret_cast<const uint8_t *>(a), reinterpret_cast<const uint8_t *>(b), lda, ldb, m, n, kp, 0, 0, sa, sb, out,
-            ldo};
+            ldo, s.per, slabs ? reinterpret_cast<int32_t *>(pb + bbytes) : nullptr};
     int rc = 0;
     if (!ad) {
         rc = pad_rows(a, m, k, lda, pa, kp);
@@ -524,7 +587,7 @@ int product(const int8_t *a, int64_t lda, const float *sa, const int8_t *b, int6
         p.b = pb, p.ldb = kp;
     }
     if (!rc) {
-        rc = dtype == NT_F32 ? tiles<NT_F32>(p) : dtype == NT_BF16 ? tiles<NT_BF16>(p) : tiles<NT_F16>(p);
+        rc = dtype == NT_F32 ? tiles<NT_F32>(p, s) : dtype == NT_BF16 ? tiles<NT_BF16>(p, s) : tiles<NT_F16>(p, s);
     }
     const int rf = scratch_release(ws);
     return rc ? rc : rf;

@@ -190,20 +190,20 @@ __device__ __forceinline__ void landed(P (&a)[N], Q (&b)[M]) {
 // The tile. Lane l of wave (wm, wn) holds in acc[i][j][v] the output of row 32 (TM wm + i) + l % 32 at column
 // 32 (TN wn + j) + 8 (v / 4) + 4 (l / 32) + v % 4: B is the MFMA's first operand, so that a lane's values are
 // of one row and by four of neighbouring columns.
-template <class E, int TM, int TN, int WM, int WN, bool ATR, bool BTR>
+template <class E, int TM, int TN, int WM, int WN, bool ATR, bool BTR, int PAIRS = 2>
 struct Tile {
     static constexpr int kWaves = WM * WN, kThreads = 64 * kWaves;
     static constexpr int BM = 32 * TM * WM, BN = 32 * TN * WN;
     typedef Side<BM, kWaves, ATR> SideA;
     typedef Side<BN, kWaves, BTR> SideB;
     static constexpr int kStageBytes = SideA::kBytes + SideB::kBytes;
-    static constexpr int kStages = 5;
+    static constexpr int kStages = 2 * PAIRS + 1;
     static constexpr int kLds = kStages * kStageBytes;
     static constexpr int kCopies = SideA::kCopies + SideB::kCopies;  // of a wave per stage
     static constexpr int kPair = 2 * kCopies;
     static constexpr int part(int q) { return kPair * q / 4; }
     static constexpr int kReadsA = TM * SideA::kReads, kReadsB = TN * SideB::kReads;
-    static_assert(kLds <= 163840 && 4 * kCopies < 64, "LDS, and vmcnt's range");
+    static_assert(PAIRS >= 2 && kLds <= 163840 && (PAIRS - 2) * kPair + part(3) < 64, "LDS, and vmcnt's range");
     typename E::Acc acc[TM][TN];
 
     struct Frags {
@@ -213,12 +213,12 @@ struct Tile {
 
     // acc = the product over `kb` bytes of k (of a k-contiguous row; 2 bytes a row of a transposed operand).
     //
-    // Stage t sits in buffer t % 5; its two k halves are steps of TM TN MFMAs. One wave runs on each SIMD, so
+    // Stage t sits in buffer t % kStages; its two k halves are steps of TM TN MFMAs. One wave runs on each SIMD, so
     // whatever is not an MFMA is placed between two of them, where it runs while the first executes: in a
     // stage's first step the reads of its second half, in its second step those of the next stage's first.
     // Stages go in pairs, whose copies are issued side by side: a k-contiguous row's two 64 bytes are one
     // cache line, and an L1 of 32 KiB does not keep it from one stage to the next (4096 x 4096 x 128256 scored
-    // in 4188 us with single stages). From an even stage t on the pair t + 4 goes into the buffers of t - 1 and
+    // in 4188 us with single stages). From an even stage t on the pair t + 2 PAIRS goes into the buffers of t - 1 and
     // t, which every wave has read by the barrier in front, a quarter of its copies in each of four steps: the
     // load unit takes about 24 cycles for a copy of 1 KiB, and a wave whose copy has to wait issues no MFMAs.
     __device__ __forceinline__ void run(uint8_t *lds, const Operand &a, const Operand &b, int64_t kb, int wave, int lane) {
@@ -237,34 +237,37 @@ struct Tile {
         const int n = int((kb + kStageK - 1) / kStageK);
         const uint32_t at = uint32_t((uintptr_t)(lds_ptr)(lds));
         Frags x, y;
-        sa.begin(0);
-        sb.begin(0);
-        unrolled<kPair>([&](auto o) { copy<o>(sa, sb, lds, lds + kStageBytes, wave); });
-        sa.begin(2);
-        sb.begin(2);
-        unrolled<part(3)>([&](auto o) { copy<o>(sa, sb, lds + 2 * kStageBytes, lds + 3 * kStageBytes, wave); });
-        wait_copies<part(3)>();
+        unrolled<PAIRS - 1>([&](auto u) {
+            uint8_t *to = lds + 2 * u * kStageBytes;
+            sa.begin(2 * u);
+            sb.begin(2 * u);
+            unrolled<kPair>([&](auto o) { copy<o>(sa, sb, to, to + kStageBytes, wave); });
+        });
+        uint32_t even = (2 * PAIRS - 2) * kStageBytes, odd = even + kStageBytes;  // the buffers of the pair being copied
+        sa.begin(2 * PAIRS - 2);
+        sb.begin(2 * PAIRS - 2);
+        unrolled<part(3)>([&](auto o) { copy<o>(sa, sb, lds + even, lds + odd, wave); });
+        wait_copies<(PAIRS - 2) * kPair + part(3)>();
         asm volatile("s_barrier" ::: "memory");
         unrolled<kReadsA>([&](auto r) { sa.template issue<r, 0>(at, x.a[r]); });
         unrolled<kReadsB>([&](auto r) { sb.template issue<r, 0>(at + SideA::kBytes, x.b[r]); });
         landed(x.a, x.b);
-        // the buffers of stage t, of the pair being copied
-        uint32_t b0 = 0, even = 2 * kStageBytes, odd = 3 * kStageBytes;
+        uint32_t b0 = 0;  // stage t's buffer
         auto after = [](uint32_t o) { return o + kStageBytes == kLds ? 0u : o + kStageBytes; };
         for (int t = 0; t < n; t += 2) {
             const uint32_t b1 = after(b0), b2 = after(b1);
             step<0, part(3), kPair>(sa, sb, x, y, at + b0, lds + even, lds + odd, wave);
             landed(y.a, y.b);
             asm volatile("s_barrier" ::: "memory");  // every wave has read stage t
-            sa.begin(t + 4);
-            sb.begin(t + 4);
+            sa.begin(t + 2 * PAIRS);
+            sb.begin(t + 2 * PAIRS);
             even = after(odd);  // (stage t - 1's)
             odd = b0;
             step<1, 0, part(1)>(sa, sb, y, x, at + b1, lds + even, lds + odd, wave);
             landed(x.a, x.b);
             step<0, part(1), part(2)>(sa, sb, x, y, at + b1, lds + even, lds + odd, wave);
             landed(y.a, y.b);
-            wait_copies<part(2)>();  // the pair t + 2
+            wait_copies<(PAIRS - 2) * kPair + part(2)>();  // the pair t + 2
             asm volatile("s_barrier" ::: "memory");
             step<1, part(2), part(3)>(sa, sb, y, x, at + b2, lds + even, lds + odd, wave);
             landed(x.a, x.b);

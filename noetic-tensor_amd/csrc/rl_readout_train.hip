@@ -31,6 +31,7 @@
 
 #include "../../include/noetic_hip.h"
 #include "nt_internal.hpp"
+#include "nt_plan.hpp"
 #include "nt_tile.hpp"
 
 namespace nt {
@@ -59,8 +60,24 @@ template <int TN>
 struct MaskBlock {
     static constexpr int kU8 = 32 * TN + 16, kF32 = 128 * TN + 16;  // bytes of a row in LDS
     static constexpr int kLds = 32 * kF32;
-    // (row: this lane's rows of the loads below are row0 .. row0 + 31, clamped to `rows` of them)
-    static __device__ __forceinline__ void in(uint8_t *lds, const MaskP &m, int64_t row0, int rows, int col, int n, int lane) {
+    // Rows row0 .. row0 + rows - 1 of the mask (a row that all share, ld 0, once, before the first block).
+    static __device__ __forceinline__ void in(uint8_t *lds, const MaskP &m, int64_t row0, int rows, int col, int n, int lane,
+                                              bool first) {
+        if (m.ld == 0) {
+            if (!first || lane >= 8 * TN) return;
+            const int c = lane * 4;
+            if (m.u8) {
+                uint32_t k = 0;
+                for (int e = 0; e < 4; e++)
+                    if (col + c + e < n) k |= uint32_t(m.u8[col + c + e]) << (8 * e);
+                *reinterpret_cast<uint32_t *>(lds + c) = k;
+            } else {
+                float f[4];
+                for (int e = 0; e < 4; e++) f[e] = col + c + e < n ? m.f32[col + c + e] : -INFINITY;
+                __builtin_memcpy(lds + c * 4, f, 16);
+            }
+            return;
+        }
         if (m.u8) {
             constexpr int kPer = 2 * TN, kRows = 64 / kPer, kLoads = 32 / kRows;
             const int c = (lane % kPer) * 16, left = n - col - c;
@@ -99,7 +116,7 @@ struct MaskBlock {
     // x under it: -inf where excluded; under an additive mask x c + mask log2 e, else x itself (y = x c follows in
     // the sum's fma)
     static __device__ __forceinline__ void out(const uint8_t *lds, const MaskP &m, float c, int lane, float (&x)[4 * TN][4]) {
-        const int r = lane % 32, h = lane / 32;
+        const int r = m.ld == 0 ? 0 : lane % 32, h = lane / 32;
         if (m.u8) {
 #pragma unroll
             for (int q = 0; q < 4 * TN; q++) {
@@ -159,17 +176,6 @@ __device__ __forceinline__ Operand weight_rows(const PieceP &p, int in) {
     else return Operand{p.w + n0 * p.ldw, p.ldw, p.n - n0, p.kbytes};
 }
 
-// A workgroup's tile: 32 TM WM rows by 128 WN columns (a wave takes 128 columns whatever the tile, so that a
-// row's sums are in the same order whatever rows are scored with it).
-template <int TM_, int WM_, int WN_>
-struct Shape {
-    static constexpr int TM = TM_, TN = 4, WM = WM_, WN = WN_;
-    static constexpr int kThreads = 64 * WM * WN, kRows = 32 * TM * WM, kCols = 128 * WN;
-};
-typedef Shape<4, 2, 2> Large;   // 256 x 256, a workgroup a CU
-typedef Shape<1, 4, 1> Medium;  // 128 x 128, two workgroups a CU: one's output while the other multiplies
-typedef Shape<1, 2, 1> Small;   // 64 x 128, two workgroups of two waves a CU
-
 template <class E, class S, bool BTR, bool ENT, bool MASK>
 __global__ __launch_bounds__(S::kThreads, 1) void k_readout_stats(PieceP p) {
     constexpr int TM = S::TM, TN = S::TN, WM = S::WM, WN = S::WN;
@@ -212,7 +218,7 @@ __global__ __launch_bounds__(S::kThreads, 1) void k_readout_stats(PieceP p) {
         if constexpr (MASK) {
             const int64_t row0 = row - lane % 32;
             if (row0 < p.rows)
-                MaskBlock<TN>::in(mlds, p.mask, row0, p.rows - row0 < 32 ? int(p.rows - row0) : 32, in * T::BN + 32 * TN * wn, p.n, lane);
+                MaskBlock<TN>::in(mlds, p.mask, row0, p.rows - row0 < 32 ? int(p.rows - row0) : 32, in * T::BN + 32 * TN * wn, p.n, lane, i == 0);
             MaskBlock<TN>::out(mlds, p.mask, p.c, lane, x);
         } else if (in * T::BN + T::BN > p.n) {
             ended(x, p.n - col0);
@@ -475,7 +481,7 @@ __global__ __launch_bounds__(S::kThreads, 1) void k_readout_g(PieceP p) {
 #pragma unroll
             for (int e = 0; e < 4; e++) x[q][e] = t.acc[i][q / 4][4 * (q % 4) + e];
         if constexpr (MASK) {
-            MaskBlock<TN>::in(mlds, p.mask, row0, p.rows - row0 < 32 ? int(p.rows - row0) : 32, in * T::BN + 32 * TN * wn, p.n, lane);
+            MaskBlock<TN>::in(mlds, p.mask, row0, p.rows - row0 < 32 ? int(p.rows - row0) : 32, in * T::BN + 32 * TN * wn, p.n, lane, i == 0);
             MaskBlock<TN>::out(mlds, p.mask, p.c, lane, x);
         } else if (in * T::BN + T::BN > p.n) {
             ended(x, p.n - col0);
@@ -631,9 +637,6 @@ __global__ __launch_bounds__(256) void k_readout_fold(const float *slab, int spl
 
 // ---------------------------------------------------------------------------------- host
 
-int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
-int64_t round_up(int64_t a, int64_t b) { return ceil_div(a, b) * b; }
-
 // Scratch of one call, cut from one allocation: sizes are asked for first, then the places.
 struct Scratch {
     size_t need = 0;
@@ -729,55 +732,6 @@ int64_t piece_cols(int64_t vocab, int64_t cols) {
     return std::min(round_up(ceil_div(vocab, pieces), kTile), round_up(vocab, kTile));
 }
 
-// The tile of a product [m, k] x [k, n] and the splits of k (`split`), by what they cost: rounds of the workgroups
-// that run at once, each its stages of 32 k and its output. Measured (us a stage, a round full): 0.92, 0.57 and
-// 0.36 for Large, Medium and Small, or 0.33 and 0.25 for a round of one workgroup a CU; an output of Large 5 us
-// (Medium's and Small's are half and a quarter of the CU's, and go on beside the other workgroup's products), the
-// slabs of split k 4 us and their bytes at 4 TB/s. So 4096 x 128256 takes Large, 333 x 50257 x 1001 Medium
-// (G 99 -> 72 us), 64 rows Small.
-enum class Size { kSmall, kMedium, kLarge };
-struct Plan {
-    Size size;
-    int64_t per, splits;  // k of a split, a multiple of 32
-    double cost;
-};
-Plan plan(int64_t m, int64_t n, int64_t k, bool split) {
-    struct Kind {
-        Size size;
-        int64_t rows, cols, slots;
-        double stage, alone, output;
-    };
-    static const Kind kinds[] = {{Size::kLarge, Large::kRows, Large::kCols, 256, 0.92, 0.92, 6.0},
-                                 {Size::kMedium, Medium::kRows, Medium::kCols, 512, 0.57, 0.33, 2.5},
-                                 {Size::kSmall, Small::kRows, Small::kCols, 512, 0.36, 0.25, 1.5}};
-    Plan best{};
-    for (const Kind &c : kinds) {
-        const int64_t tiles = ceil_div(m, c.rows) * ceil_div(n, c.cols);
-        for (int64_t s = 1; s <= 64; s = s < 4 ? s + 1 : s + s / 4) {
-            const int64_t per = round_up(ceil_div(k, s), 32), splits = ceil_div(k, per);
-            if (s > 1 && (!split || splits < s || per < 256)) continue;
-            const int64_t wgs = tiles * splits, rounds = ceil_div(wgs, c.slots);
-            const double stage = wgs <= 256 ? c.alone : c.stage;
-            const double cost = double(rounds) * (double(per / 32) * stage + c.output) +
-                                (splits > 1 ? 4.0 + double(splits) * double(m) * double(n) * 8e-6 / 4.0 : 0.0);
-            if (best.per == 0 || cost < best.cost) best = Plan{c.size, per, splits, cost};
-        }
-    }
-    return best;
-}
-
-// The columns of [m, n] that go by Large tiles in whole rounds of 256, where the rest by itself costs less than
-// one more round of them does (a multiple of a tile's; 0: no such split). 2048 x 50304 is 1576 tiles: 1536 and the
-// last 1152 columns apart (stats 828 -> 748 us).
-int64_t whole_rounds(int64_t m, int64_t n, int64_t k) {
-    const Plan all = plan(m, n, k, false);
-    if (all.size != Size::kLarge) return 0;
-    const int64_t tm = ceil_div(m, Large::kRows), tiles = tm * ceil_div(n, Large::kCols);
-    const int64_t cols = tiles / 256 * 256 / tm * Large::kCols;
-    if (cols <= 0 || cols >= n) return 0;
-    return plan(m, cols, k, false).cost + plan(m, n - cols, k, false).cost + 4.0 < all.cost ? cols : 0;
-}
-
 // Columns c0 .. c0 + n - 1 of a piece (c0 a multiple of 256).
 PieceP part_of(const PieceP &p, bool dv, int64_t c0, int64_t n) {
     PieceP q = p;
@@ -811,11 +765,11 @@ int launch_stats(PieceP p, bool ent) {
 
 template <class E, bool BTR>
 int stats(const PieceP &p, bool ent) {
-    if (const int64_t c = whole_rounds(p.rows, p.n, p.dim)) {
+    if (const int64_t c = whole_rounds(p.rows, p.n, p.kbytes)) {
         if (int rc = launch_stats<E, Large, BTR>(part_of(p, BTR, 0, c), ent)) return rc;
         return stats<E, BTR>(part_of(p, BTR, c, p.n - c), ent);
     }
-    switch (plan(p.rows, p.n, p.dim, false).size) {
+    switch (plan(p.rows, p.n, p.kbytes, false).size) {
         case Size::kSmall: return launch_stats<E, Small, BTR>(p, ent);
         case Size::kMedium: return launch_stats<E, Medium, BTR>(p, ent);
         default: return launch_stats<E, Large, BTR>(p, ent);
@@ -837,11 +791,11 @@ constexpr int64_t kTwoRows = 64;  // G in two terms for so many rows: the Small 
 template <class E, bool BTR>
 int g_piece(const PieceP &p) {
     if (p.rows <= kTwoRows) return launch_g<E, Small, BTR, true>(p);
-    if (const int64_t c = whole_rounds(p.rows, p.n, p.dim)) {
+    if (const int64_t c = whole_rounds(p.rows, p.n, p.kbytes)) {
         if (int rc = launch_g<E, Large, BTR, false>(part_of(p, BTR, 0, c))) return rc;
         return g_piece<E, BTR>(part_of(p, BTR, c, p.n - c));
     }
-    switch (plan(p.rows, p.n, p.dim, false).size) {
+    switch (plan(p.rows, p.n, p.kbytes, false).size) {
         case Size::kSmall: return launch_g<E, Small, BTR, false>(p);
         case Size::kMedium: return launch_g<E, Medium, BTR, false>(p);
         default: return launch_g<E, Large, BTR, false>(p);
@@ -927,7 +881,7 @@ int fold(const GradP &p, int64_t splits, uint16_t *out, int64_t two = 0) {
 
 template <class E, class S, bool ATR, bool BTR>
 int launch_product(GradP p, const Plan &s) {
-    p.per = s.per;
+    p.per = s.per / 2;
     p.tm = uint32_t(ceil_div(p.m, S::kRows));
     p.tn = uint32_t(ceil_div(p.n, S::kCols));
     k_readout_grad<E, S, ATR, BTR><<<dim3(p.tm * p.tn, unsigned(s.splits)), dim3(S::kThreads), 0, ctx().stream>>>(p);
@@ -978,7 +932,7 @@ int piece(const BackP &b) {
         w.slab = b.slab_w;
         w.scale = b.top;
         w.fixed = b.fixed;
-        const int64_t c = b.sw.splits > 1 ? 0 : whole_rounds(DV ? w.m : w.n, DV ? w.n : w.m, w.k);
+        const int64_t c = b.sw.splits > 1 ? 0 : whole_rounds(DV ? w.m : w.n, DV ? w.n : w.m, w.k * 2);
         if (c) {  // whole rounds of the vocabulary's side, and its rest
             GradP first = w, rest = w;
             (DV ? first.n : first.m) = c;
@@ -987,7 +941,7 @@ int piece(const BackP &b) {
             (DV ? rest.wb : rest.wa) -= c * 2;
             rest.out += DV ? c : c * rest.ldo;
             if (int rc = launch_product<E, Large, true, true>(first, b.sw)) return rc;
-            if (int rc = product<E, true, true>(rest, plan(rest.m, rest.n, rest.k, false))) return rc;
+            if (int rc = product<E, true, true>(rest, plan(rest.m, rest.n, rest.k * 2, false))) return rc;
         } else if (int rc = product<E, true, true>(w, b.sw)) {
             return rc;
         }
@@ -1037,8 +991,8 @@ int backward(const NtRlReadoutStatsGradArgs *a) {
     // dH: [rows, dim], k the piece's columns; dW: [vocab, dim] or [dim, vocab], k the rows
     const int64_t two = R <= kTwoRows ? R : 0;
     const int64_t width = std::min(cols, V);
-    const Plan sh = plan(R + two, d, round_up(width, 8), true);
-    const Plan sw = dv ? plan(d, width, R + two, true) : plan(width, d, R + two, true);
+    const Plan sh = plan(R + two, d, round_up(width, 8) * 2, true);
+    const Plan sw = dv ? plan(d, width, (R + two) * 2, true) : plan(width, d, (R + two) * 2, true);
     const bool hslab = sh.splits > 1 || pieces > 1 || two;
     Scratch s;
     const size_t o_h = s.add(hdirect ? 0 : R * kp * 2), o_hs = s.add((R + two) * kp * 2);
