@@ -31,7 +31,7 @@ struct Plan {
 // at once, each its stages of 64 bytes and its output. Measured (us a stage, a round full): 0.92, 0.57 and 0.36 for
 // Large, Medium and Small, or 0.33 and 0.25 in a round of one workgroup a CU; an output of Large about 6 us, of
 // Medium and Small less than their share of it, since it goes on beside the other workgroup's products; the slabs of a
-// split k 4 us and their bytes, written and read, at 4 TB/s. So 4096 x 128256 takes Large, 333 x 50257 x 1001 Medium (a
+// split k 4 us, 0.15 a slab and their bytes, written and read, at 4 TB/s. So 4096 x 128256 takes Large, 333 x 50257 x 1001 Medium (a
 // pass over the logits 99 -> 77 us), 64 rows Small (29 -> 16 us at 32000 x 1024).
 inline Plan plan(int64_t m, int64_t n, int64_t kb, bool split) {
     if (kb < 64) kb = 64;
@@ -46,12 +46,15 @@ inline Plan plan(int64_t m, int64_t n, int64_t kb, bool split) {
     Plan best{};
     for (const Kind &c : kinds) {
         const int64_t tiles = ceil_div(m, c.rows) * ceil_div(n, c.cols);
-        for (int64_t s = 1; s <= 64; s = s < 4 ? s + 1 : s + s / 4) {
+        for (int64_t r = 0; r <= 3; r++) {  // unsplit, and the splits that fill one to three rounds
+            int64_t s = r == 0 ? 1 : c.slots * r / tiles;
+            s = s > 64 ? 64 : s;
+            if (s < 1 || (s > 1 && !split)) continue;
             const int64_t per = round_up(ceil_div(kb, s), 64), splits = ceil_div(kb, per);
-            if (s > 1 && (!split || splits < s || per < 512)) continue;
+            if (splits > 1 && per < 512) continue;
             const int64_t wgs = tiles * splits, rounds = ceil_div(wgs, c.slots);
             const double cost = double(rounds) * (double(per / 64) * (wgs <= 256 ? c.alone : c.stage) + c.output) +
-                                (splits > 1 ? 4.0 + double(splits) * double(m) * double(n) * 8e-6 / 4.0 : 0.0);
+                                (splits > 1 ? 4.0 + double(splits) * (0.15 + double(m) * double(n) * 8e-6 / 4.0) : 0.0);
             if (best.per == 0 || cost < best.cost) best = Plan{c.size, per, splits, cost};
         }
     }

@@ -637,21 +637,42 @@ __global__ __launch_bounds__(256) void k_readout_fold(const float *slab, int spl
 
 // ---------------------------------------------------------------------------------- host
 
-// Scratch of one call, cut from one allocation: sizes are asked for first, then the places.
+// Scratch of one call: sizes are asked for first, then allocated, the large ones each by itself (the library keeps
+// blocks of up to 128 MiB for the next call; a larger one is the device pool's, and its allocation may wait for the
+// stream), then the places.
 struct Scratch {
-    size_t need = 0;
-    uint8_t *base = nullptr;
-    size_t add(int64_t bytes) {
-        const size_t at = need;
-        need += (size_t(bytes) + 255) & ~size_t(255);
-        return at;
+    static constexpr int kMost = 12;
+    static constexpr size_t kAlone = size_t(1) << 20;
+    size_t size[kMost], together = 0;
+    void *place[kMost], *shared = nullptr;
+    int n = 0;
+    int add(int64_t bytes) {
+        size[n] = (size_t(bytes) + 255) & ~size_t(255);
+        place[n] = nullptr;
+        if (size[n] < kAlone) together += size[n];
+        return n++;
+    }
+    int allocate() {
+        if (int rc = scratch_alloc(together, &shared)) return rc;
+        uint8_t *at = static_cast<uint8_t *>(shared);
+        for (int i = 0; i < n; i++) {
+            if (size[i] >= kAlone) {
+                if (int rc = scratch_alloc(size[i], &place[i])) return rc;
+            } else {
+                place[i] = at;
+                at += size[i];
+            }
+        }
+        return 0;
     }
     template <class P>
-    P *at(size_t o) const {
-        return reinterpret_cast<P *>(base + o);
+    P *at(int i) const {
+        return static_cast<P *>(place[i]);
     }
     ~Scratch() {
-        if (base) (void)scratch_release(base);
+        for (int i = 0; i < n; i++)
+            if (size[i] >= kAlone && place[i]) (void)scratch_release(place[i]);
+        if (shared) (void)scratch_release(shared);
     }
 };
 
@@ -807,19 +828,17 @@ int forward(const NtRlReadoutStatsArgs *a) {
     const int64_t R = a->rows, V = a->vocab, d = a->dim, kp = round_up(d, 8);
     const bool hdirect = aligned(a->hidden, d, a->ldh);
     const bool wdirect = aligned(a->weight, dv ? V : d, a->ldw);
-    // one launch for the whole vocabulary, but for a copied weight (pieces of 256 MiB) and more than 2^23 tiles
+    // one launch for the whole vocabulary, but for a copied weight (pieces of 128 MiB) and more than 2^23 tiles
     int64_t most = (int64_t(1) << 23) / ceil_div(R, kTile) * kTile;
-    if (!wdirect) most = std::min(most, (int64_t(1) << 27) / kp);
+    if (!wdirect) most = std::min(most, (int64_t(1) << 26) / kp);
     const int64_t cols = piece_cols(V, most);
     const int64_t blocks = ceil_div(V, kTile) * 2, rows_p = round_up(R, 32);  // (a large tile writes whole ones)
     Scratch s;
-    const size_t o_h = s.add(hdirect ? 0 : R * kp * 2);
-    const size_t o_w = s.add(wdirect ? 0 : (dv ? d * cols : cols * kp) * 2);
-    const size_t o_ref = s.add(blocks * rows_p * 4), o_sum = s.add(blocks * rows_p * 4);
-    const size_t o_es = s.add(a->entropy ? blocks * rows_p * 4 : 0), o_x = s.add(R * 4);
-    void *ws = nullptr;
-    if (int rc = scratch_alloc(s.need, &ws)) return rc;
-    s.base = static_cast<uint8_t *>(ws);
+    const int o_h = s.add(hdirect ? 0 : R * kp * 2);
+    const int o_w = s.add(wdirect ? 0 : (dv ? d * cols : cols * kp) * 2);
+    const int o_ref = s.add(blocks * rows_p * 4), o_sum = s.add(blocks * rows_p * 4);
+    const int o_es = s.add(a->entropy ? blocks * rows_p * 4 : 0), o_x = s.add(R * 4);
+    if (int rc = s.allocate()) return rc;
     PieceP p{};
     p.h = static_cast<const uint8_t *>(a->hidden);
     p.ldh = a->ldh * 2;
@@ -984,9 +1003,11 @@ int backward(const NtRlReadoutStatsGradArgs *a) {
     }
     const bool hdirect = aligned(a->hidden, d, a->ldh);
     const bool wdirect = aligned(a->weight, dv ? V : d, a->ldw);
-    // G of a piece takes at most 512 MiB (a copied piece of the weight 256 MiB)
+    // G of a piece takes at most 512 MiB, a copied piece of the weight 128 MiB. (Pieces of 128 MiB of G, which the
+    // memory-side cache would hold between the products, lost: dH's sums are read and written for each piece. 4096 x
+    // 4096 x 128256 13.8 against 13.5 ms.)
     int64_t most = (int64_t(1) << 28) / R;
-    if (!wdirect) most = std::min(most, (int64_t(1) << 27) / kp);
+    if (!wdirect) most = std::min(most, (int64_t(1) << 26) / kp);
     const int64_t cols = piece_cols(V, most), pieces = ceil_div(V, cols);
     // dH: [rows, dim], k the piece's columns; dW: [vocab, dim] or [dim, vocab], k the rows
     const int64_t two = R <= kTwoRows ? R : 0;
@@ -995,15 +1016,13 @@ int backward(const NtRlReadoutStatsGradArgs *a) {
     const Plan sw = dv ? plan(d, width, (R + two) * 2, true) : plan(width, d, (R + two) * 2, true);
     const bool hslab = sh.splits > 1 || pieces > 1 || two;
     Scratch s;
-    const size_t o_h = s.add(hdirect ? 0 : R * kp * 2), o_hs = s.add((R + two) * kp * 2);
-    const size_t o_w = s.add(wdirect ? 0 : (dv ? d * cols : cols * kp) * 2);
-    const size_t o_coef = s.add(R * 16), o_up = s.add(R * 4), o_top = s.add(4);
-    const size_t o_g = s.add((R + two) * cols * 2);
-    const size_t o_sh = s.add(a->grad_hidden && hslab ? sh.splits * (R + two) * d * 4 : 0);
-    const size_t o_sw = s.add(a->grad_weight && sw.splits > 1 ? sw.splits * std::min(cols, V) * d * 4 : 0);
-    void *ws = nullptr;
-    if (int rc = scratch_alloc(s.need, &ws)) return rc;
-    s.base = static_cast<uint8_t *>(ws);
+    const int o_h = s.add(hdirect ? 0 : R * kp * 2), o_hs = s.add((R + two) * kp * 2);
+    const int o_w = s.add(wdirect ? 0 : (dv ? d * cols : cols * kp) * 2);
+    const int o_coef = s.add(R * 16), o_up = s.add(R * 4), o_top = s.add(4);
+    const int o_g = s.add((R + two) * cols * 2);
+    const int o_sh = s.add(a->grad_hidden && hslab ? sh.splits * (R + two) * d * 4 : 0);
+    const int o_sw = s.add(a->grad_weight && sw.splits > 1 ? sw.splits * std::min(cols, V) * d * 4 : 0);
+    if (int rc = s.allocate()) return rc;
     const float *up = f16 ? s.at<float>(o_up) : nullptr, *top = f16 ? s.at<float>(o_top) : nullptr;
     const float fixed = f16 ? float(ldexp(1.0, -14) / a->temperature) : 1.0f;
     CoefP c{};

@@ -132,7 +132,10 @@ def agree(got, want, dtype):
 
 
 PRODUCTS = [(1, 1, 1), (1, 5, 16), (2, 300, 48), (16, 64, 64), (33, 100, 77), (64, 1000, 128), (65, 257, 1000),
-            (128, 128, 4096), (300, 520, 208), (257, 255, 33), (1, 4099, 512), (5, 40, 20000), (700, 31, 96)]
+            (128, 128, 4096), (300, 520, 208), (257, 255, 33), (1, 4099, 512), (5, 40, 20000), (700, 31, 96),
+            # every tile and a split k; up to four rows beside five
+            (6, 276, 12096), (100, 152, 10496), (3, 33, 1040), (4, 1001, 2064), (5, 1001, 2064), (600, 5000, 272),
+            (2049, 4100, 96), (70, 33000, 64)]
 
 
 @pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])

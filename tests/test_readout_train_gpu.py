@@ -452,3 +452,53 @@ def test_a_policy_step_with_an_8_bit_rollout():
     agree(values(lp).ravel(), want["logp"], tol["logp"], "logp")
     agree(values(gh).reshape(c.rows, d), want["grad_hidden"], tol["grad_hidden"], "grad_hidden")
     agree(values(gw), want["grad_weight"], tol["grad_weight"], "grad_weight")
+
+
+# Sizes that every tile, split and cut of the products is taken at: 256 x 256 tiles in whole rounds with a rest beside them
+# (2100 x 16640, dim 1100 for its k), 128 x 128 and 64 x 128 ones, k split and not, in both layouts.
+@pytest.mark.parametrize("rows,V,d,dtype,layout,mask", [
+    (2100, 16640, 1100, "bf16", "dv", "u8"), (2100, 16640, 1100, "f16", "vd", "none"), (2050, 17001, 1096, "bf16", "vd", "f32_shared"),
+    (700, 9000, 200, "bf16", "vd", "f32"), (130, 30011, 520, "f16", "dv", "none"), (64, 20000, 300, "bf16", "dv", "none"),
+    (65, 20000, 304, "bf16", "vd", "u8_shared"), (1, 50257, 128, "bf16", "vd", "none")])
+def test_large_sizes(rows, V, d, dtype, layout, mask):
+    c = Case(rows, V, d, dtype, layout, mask, tau=0.9)
+    got = c.run()
+    for name in ("h", "w", "tokens", "g_logp", "g_entropy", "add"):
+        setattr(c, name, getattr(c, name).to("cuda"))
+    device = torch.get_default_device()
+    torch.set_default_device("cuda")
+    try:
+        want, tol = c.want()
+    finally:
+        torch.set_default_device(device)
+    for k in got:
+        agree(values(got[k]).to("cuda"), want[k], tol[k], k)
+    if rows <= 64:  # G in two terms: the gradients are off by their own rounding and the sums'
+        u = HALF_STEP[dtype]
+        for k in ("grad_hidden", "grad_weight"):
+            off = (values(got[k]).to("cuda") - want[k]).norm() / want[k].norm()
+            assert off <= 0.6 * u, (k, float(off))  # (a rounding alone: u / sqrt(3) at the most)
+
+
+def test_a_padded_batch_holds_nothing_back():
+    """Half the positions padded (upstream gradients zero, hidden states NaN, tokens -1): the others' results are those of
+    the batch without them."""
+    c = Case(96, 1000, 64, "bf16", "vd")
+    pad = torch.arange(96) % 2 == 1
+    c.h[pad], c.tokens[pad], c.g_logp[pad], c.g_entropy[pad] = math.nan, -1, 0.0, 0.0
+    full = {k: values(v) for k, v in c.run(check=False).items()}
+    d = Case(96, 1000, 64, "bf16", "vd")
+    d.rows, d.h, d.tokens, d.g_logp, d.g_entropy = 48, c.h[~pad], c.tokens[~pad], c.g_logp[~pad], c.g_entropy[~pad]
+    part = {k: values(v) for k, v in d.run().items()}
+    for k in ("logp", "entropy", "base", "rest"):
+        assert torch.equal(full[k][~pad], part[k]), k
+    want, tol = d.want()
+    agree(full["grad_hidden"][~pad], want["grad_hidden"], tol["grad_hidden"], "grad_hidden")
+    agree(full["grad_weight"], want["grad_weight"], tol["grad_weight"], "grad_weight")
+    assert (full["grad_hidden"][pad] == 0).all()
+
+
+def test_the_same_token_at_every_position():
+    c = Case(300, 700, 40, "bf16", "dv", tau=0.8)
+    c.tokens[:] = 699
+    check(c)
