@@ -161,13 +161,21 @@ __global__ __launch_bounds__(256) void k_quantize_rows(const void *xv, int64_t r
     if (chunks * 8 + t < cols && t < 8) o[chunks * 8 + t] = int8_t(quantized(load_f32<T>(xv, at + chunks * 8 + t), s, inv));
 }
 
+// (a launch holds fewer than 2^32 threads: 2^23 rows at a time)
 template <int T>
-int launch_rows(const void *x, int64_t rows, int64_t cols, int64_t ld, int8_t *q, float *scale) {
-    if (cols <= 4096 && rows >= 1024)
-        k_quantize_rows<T, 64, 8><<<dim3(unsigned(ceil_div(rows, 4))), dim3(256), 0, ctx().stream>>>(x, rows, cols, ld, q, scale);
-    else
-        k_quantize_rows<T, 256, 8><<<dim3(unsigned(rows)), dim3(256), 0, ctx().stream>>>(x, rows, cols, ld, q, scale);
-    return launched("k_quantize_rows");
+int launch_rows(const uint8_t *x, int64_t rows, int64_t cols, int64_t ld, int8_t *q, float *scale) {
+    constexpr int64_t kMost = int64_t(1) << 23, kSize = T == NT_F32 ? 4 : 2;
+    for (int64_t r = 0; r < rows; r += kMost) {
+        const int64_t n = std::min(kMost, rows - r);
+        const uint8_t *from = x + r * ld * kSize;
+        int8_t *to = q + r * cols;
+        if (cols <= 4096 && rows >= 1024)
+            k_quantize_rows<T, 64, 8><<<dim3(unsigned(ceil_div(n, 4))), dim3(256), 0, ctx().stream>>>(from, n, cols, ld, to, scale + r);
+        else
+            k_quantize_rows<T, 256, 8><<<dim3(unsigned(n)), dim3(256), 0, ctx().stream>>>(from, n, cols, ld, to, scale + r);
+        if (int rc = launched("k_quantize_rows")) return rc;
+    }
+    return 0;
 }
 
 // Rows that are the columns of x [n, ld]: a workgroup takes 64 of them, a thread four neighbouring ones (16 bytes of f32,
@@ -270,6 +278,17 @@ __global__ __launch_bounds__(512) void k_quantize_columns(const void *xv, int64_
 #pragma unroll
             for (int e = 0; e < 4; e++) x[u][e] = y[u][e];
     }
+}
+
+template <int T>
+int launch_columns(const uint8_t *x, int64_t cols, int64_t n, int64_t ld, int8_t *q, float *scale) {
+    constexpr int64_t kMost = int64_t(1) << 28, kSize = T == NT_F32 ? 4 : 2;
+    for (int64_t c = 0; c < cols; c += kMost) {
+        const int64_t w = std::min(kMost, cols - c);
+        k_quantize_columns<T><<<dim3(unsigned(ceil_div(w, 64))), dim3(512), 0, ctx().stream>>>(x + c * kSize, w, n, ld, q + c * n, scale + c);
+        if (int rc = launched("k_quantize_columns")) return rc;
+    }
+    return 0;
 }
 
 // A thread takes eight neighbouring values at a time, of one row or, where rows are not whole chunks, of two or more.
@@ -628,13 +647,14 @@ int nt_hip_quantize_int8(const void *x, const NtLayout *xl, int32_t dtype, int8_
     for (int d = 0; d < xl->rank; d++) {
         if (xl->shape[d] < 0 || xl->strides[d] < 0 || xl->offset < 0)
             return fail(NT_E_ARG, std::string(who) + ": negative shape, stride or offset");
-        total *= xl->shape[d];
+        if (__builtin_mul_overflow(total, xl->shape[d], &total) || total > (int64_t(1) << 40))
+            return fail(NT_E_ARG, std::string(who) + ": more than 2^40 values");
     }
-    int64_t rows = 1;
-    for (int d = 0; d + 1 < xl->rank; d++) rows *= xl->shape[d];
+    int64_t rows = 1;  // (of no columns there may be any number: as many scales)
+    for (int d = 0; d + 1 < xl->rank; d++)
+        if (__builtin_mul_overflow(rows, xl->shape[d], &rows) || rows > (int64_t(1) << 40))
+            return fail(NT_E_ARG, std::string(who) + ": more than 2^40 rows");
     const int64_t cols = xl->shape[xl->rank - 1];
-    if (rows > 0x7fffffff || cols > (int64_t(1) << 40))
-        return fail(NT_E_ARG, std::string(who) + ": " + std::to_string(rows) + " rows (at most 2^31 - 1)");
     if (rows > 0 && (!scale || (total > 0 && (!x || !q))))
         return fail(NT_E_ARG, std::string(who) + ": null buffer");
     std::unique_lock<std::mutex> lk;
@@ -657,20 +677,14 @@ int nt_hip_quantize_int8(const void *x, const NtLayout *xl, int32_t dtype, int8_
         src = static_cast<const uint8_t *>(ws);
         v = Rows{rows, cols, cols, 1};
     }
-    hipStream_t st = ctx().stream;
-    if (columns) {
-        const dim3 grid(unsigned(ceil_div(v.rows, 64)));
-        if (dtype == NT_F32) hipLaunchKernelGGL(k_quantize_columns<NT_F32>, grid, dim3(512), 0, st, src, v.rows, v.cols, v.col_stride, q, scale);
-        else if (dtype == NT_BF16) hipLaunchKernelGGL(k_quantize_columns<NT_BF16>, grid, dim3(512), 0, st, src, v.rows, v.cols, v.col_stride, q, scale);
-        else hipLaunchKernelGGL(k_quantize_columns<NT_F16>, grid, dim3(512), 0, st, src, v.rows, v.cols, v.col_stride, q, scale);
-    } else {
-        const int rc = dtype == NT_F32 ? launch_rows<NT_F32>(src, v.rows, v.cols, v.row_stride, q, scale)
-                       : dtype == NT_BF16 ? launch_rows<NT_BF16>(src, v.rows, v.cols, v.row_stride, q, scale)
-                                          : launch_rows<NT_F16>(src, v.rows, v.cols, v.row_stride, q, scale);
-        const int rf = scratch_release(ws);
-        return rc ? rc : rf;
-    }
-    const int rc = launched("k_quantize");
+    auto launch = [&](auto type) {
+        constexpr int T = decltype(type)::value;
+        return columns ? launch_columns<T>(src, v.rows, v.cols, v.col_stride, q, scale)
+                       : launch_rows<T>(src, v.rows, v.cols, v.row_stride, q, scale);
+    };
+    const int rc = dtype == NT_F32 ? launch(std::integral_constant<int, NT_F32>{})
+                   : dtype == NT_BF16 ? launch(std::integral_constant<int, NT_BF16>{})
+                                      : launch(std::integral_constant<int, NT_F16>{});
     const int rf = scratch_release(ws);
     return rc ? rc : rf;
 }

@@ -356,11 +356,11 @@ struct CoefP {
     float *top;    // [1] f16: the largest of them
 };
 
-// What a row's upstream gradients make of it (one workgroup: the largest row's scale is a maximum over all).
+// What a row's upstream gradients make of it (f16: one workgroup, the largest row's scale is a maximum over all).
 __global__ __launch_bounds__(1024) void k_readout_coef(CoefP p) {
     __shared__ float s_top[16];
     float top = 0.0f;
-    for (int64_t r = threadIdx.x; r < p.rows; r += 1024) {
+    for (int64_t r = blockIdx.x * int64_t(1024) + threadIdx.x; r < p.rows; r += int64_t(gridDim.x) * 1024) {
         const int64_t tok = p.tokens[r];
         double gl = p.g_logp ? double(p.g_logp[r]) : 0.0;
         if (tok < 0 || tok >= p.vocab) gl = 0.0;
@@ -828,8 +828,9 @@ int forward(const NtRlReadoutStatsArgs *a) {
     const int64_t R = a->rows, V = a->vocab, d = a->dim, kp = round_up(d, 8);
     const bool hdirect = aligned(a->hidden, d, a->ldh);
     const bool wdirect = aligned(a->weight, dv ? V : d, a->ldw);
-    // one launch for the whole vocabulary, but for a copied weight (pieces of 128 MiB) and more than 2^23 tiles
-    int64_t most = (int64_t(1) << 23) / ceil_div(R, kTile) * kTile;
+    // one launch for the whole vocabulary, but for a copied weight (pieces of 128 MiB) and more than 2^20 large tiles (a
+    // launch holds fewer than 2^32 threads: 2^23 small ones of 128)
+    int64_t most = (int64_t(1) << 20) / ceil_div(R, kTile) * kTile;
     if (!wdirect) most = std::min(most, (int64_t(1) << 26) / kp);
     const int64_t cols = piece_cols(V, most);
     const int64_t blocks = ceil_div(V, kTile) * 2, rows_p = round_up(R, 32);  // (a large tile writes whole ones)
@@ -1039,7 +1040,7 @@ int backward(const NtRlReadoutStatsGradArgs *a) {
     c.coef = s.at<float4>(o_coef);
     c.up = s.at<float>(o_up);
     c.top = s.at<float>(o_top);
-    hipLaunchKernelGGL(k_readout_coef, dim3(1), dim3(1024), 0, ctx().stream, c);
+    hipLaunchKernelGGL(k_readout_coef, dim3(f16 ? 1 : unsigned(std::min<int64_t>(ceil_div(R, 1024), 256))), dim3(1024), 0, ctx().stream, c);
     if (int rc = launched("k_readout_coef")) return rc;
     if (a->grad_weight)
         if (int rc = copy_rows(a->hidden, R, d, a->ldh, s.at<uint8_t>(o_hs), kp * 2, c.coef, up, top, two)) return rc;

@@ -502,3 +502,46 @@ def test_the_same_token_at_every_position():
     c = Case(300, 700, 40, "bf16", "dv", tau=0.8)
     c.tokens[:] = 699
     check(c)
+
+
+class Held:
+    """A torch allocation as the buffer behind a tensor."""
+
+    def __init__(self, t):
+        self.t, self.ptr = t, t.data_ptr()
+
+
+def test_offsets_past_32_bits():
+    """A keep-mask of 4.8 GB and G in 19 pieces: the last rows and the first against the formulas."""
+    R, V, d = 40000, 120001, 8
+    c = Case(R, V, d, "bf16", "vd", entropy=False)
+    g = torch.Generator(device="cuda").manual_seed(3)
+    keep = torch.empty(R, V, dtype=torch.uint8, device="cuda").random_(0, 3, generator=g)  # a third excluded
+    keep[torch.arange(R), c.tokens.long()] = 1
+    torch.cuda.synchronize()
+    m = nr.Tensor((R, V), "u8", Held(keep))
+    h, w, t = given(c.h), given(c.w), given(c.tokens)
+    lp, _, stats = nr.readout_score_with_stats(h, w, 1.0, m, t, entropy=False, layout="vd")
+    gh, gw = nr.readout_score_grad(h, w, 1.0, m, t, stats, g_logp=given(c.g_logp), layout="vd")
+    lp, gh, gw = values(lp), values(gh), values(gw)
+    for at in (slice(0, 40), slice(R // 2, R // 2 + 40), slice(R - 40, R)):
+        e = Case(40, V, d, "bf16", "vd", entropy=False)
+        e.h, e.w, e.tokens, e.g_logp = c.h[at], c.w, c.tokens[at], c.g_logp[at]
+        e.add = torch.where(keep[at].cpu() > 0, 0.0, -math.inf).double()
+        want, tol = e.want()
+        agree(lp[at], want["logp"], tol["logp"], "logp")
+        agree(gh[at], want["grad_hidden"], tol["grad_hidden"], "grad_hidden")
+    # a column's gradient from all rows, at both ends of the vocabulary
+    W, H, at = c.w.double().cuda(), c.h.double().cuda(), c.tokens.long().cuda()
+    gl = c.g_logp.double().cuda()
+    cols = torch.tensor([0, 1, 65000, V - 2, V - 1], device="cuda")
+    G = torch.zeros(R, 5, dtype=torch.float64, device="cuda")
+    for r in range(0, R, 2000):
+        s = slice(r, r + 2000)
+        z = (H[s] @ W.t()).masked_fill_(keep[s] == 0, -math.inf)
+        G[s] = -gl[s, None] * (z[:, cols] - torch.logsumexp(z, 1, keepdim=True)).exp()
+    G += gl[:, None] * (at[:, None] == cols[None, :])
+    want, size = G.t() @ H, G.abs().t() @ H.abs()
+    u = HALF_STEP["bf16"]
+    # (dp under 2^-12; each piece's sum of 40000 f32 terms)
+    assert ((gw.cuda()[cols] - want).abs() <= (u + 2.0 ** -12 + R * 2.0 ** -24) * size + u * want.abs()).all()
