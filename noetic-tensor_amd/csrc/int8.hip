@@ -60,7 +60,7 @@ __device__ __forceinline__ int quantized(float x, float s, float inv) {
 
 // Four of them as bytes of a word. x (1/s) + 1.5 2^23 rounds to the integer in one fma and leaves it in the low
 // byte; only where some remainder reaches half the scale (a value next to a border) are the four taken again as
-// above. (5 operations a value instead of 15: 4096 x 4096 bf16 rows 19.2 -> 12.4 us.)
+// above. (5 operations a value instead of 15: 4096 x 4096 bf16 rows 19.2 -> 16.5 us.)
 __device__ __forceinline__ uint32_t quantized4(const float (&x)[4], float s, float inv) {
     constexpr float kMagic = 12582912.0f;
     uint32_t b[4];
@@ -178,84 +178,126 @@ int launch_rows(const uint8_t *x, int64_t rows, int64_t cols, int64_t ld, int8_t
     return 0;
 }
 
-// Rows that are the columns of x [n, ld]: a workgroup takes 64 of them, a thread four neighbouring ones (16 bytes of f32,
-// 8 of a 16-bit type) in four rows of x at a time: a word of each of its columns. Both passes read x, the second from
-// the caches where they hold it. The words go out through LDS, 128 values of a column side by side.
-template <int T>
-__global__ __launch_bounds__(512) void k_quantize_columns(const void *xv, int64_t cols, int64_t n, int64_t ld, int8_t *q,
-                                                          float *scale) {
-    __shared__ float s_max[32][64];
-    __shared__ int s_bad[32][64];
-    __shared__ uint32_t tile[64][33];  // [column][words of 4 rows of x]
-    const int t = threadIdx.x, g = t / 16, lc = (t % 16) * 4;
-    const int64_t c0 = int64_t(blockIdx.x) * 64, c = c0 + lc;
-    const int have = cols - c >= 4 ? 4 : (cols > c ? int(cols - c) : 0);
+// Rows that are the columns of x [n, ld]. A workgroup takes W of them and `per` rows of x, a thread four neighbouring ones
+// (16 bytes of f32, 8 of a 16-bit type) in four rows of x at a time: a word of each of its columns. Bounded by HBM and
+// the last-level cache: x is read for the magnitudes and again for the values, which do not fit on the chip: 1024 x 50304
+// f32 takes 73 us where that cache holds x, 89 cold (its bytes once, at a copy's rate: 54).
+template <int T, int W>
+struct Columns {
+    const void *x;
+    int64_t cols, n, ld, c;
+    int have;
+
+    __device__ __forceinline__ Columns(const void *x, int64_t cols, int64_t n, int64_t ld, int64_t c)
+        : x(x), cols(cols), n(n), ld(ld), c(c), have(cols - c >= 4 ? 4 : (cols > c ? int(cols - c) : 0)) {}
+
     // rows k .. k + 3 of x
-    auto load = [&](int64_t k, float (&x)[4][4]) {
+    __device__ __forceinline__ void load(int64_t k, float (&v)[4][4]) const {
 #pragma unroll
-        for (int u = 0; u < 4; u++) x[u][0] = x[u][1] = x[u][2] = x[u][3] = 0.0f;
+        for (int u = 0; u < 4; u++) v[u][0] = v[u][1] = v[u][2] = v[u][3] = 0.0f;
         if (have == 4 && k + 4 <= n) {
             if constexpr (T == NT_F32) {
 #pragma unroll
-                for (int u = 0; u < 4; u++) __builtin_memcpy(x[u], static_cast<const float *>(xv) + (k + u) * ld + c, 16);
+                for (int u = 0; u < 4; u++) __builtin_memcpy(v[u], static_cast<const float *>(x) + (k + u) * ld + c, 16);
             } else {
                 uint16_t h[4][4];
 #pragma unroll
-                for (int u = 0; u < 4; u++) __builtin_memcpy(h[u], static_cast<const uint16_t *>(xv) + (k + u) * ld + c, 8);
+                for (int u = 0; u < 4; u++) __builtin_memcpy(h[u], static_cast<const uint16_t *>(x) + (k + u) * ld + c, 8);
 #pragma unroll
                 for (int u = 0; u < 4; u++)
 #pragma unroll
                     for (int e = 0; e < 4; e++) {
-                        if constexpr (T == NT_BF16) x[u][e] = __builtin_bit_cast(float, uint32_t(h[u][e]) << 16);
-                        else x[u][e] = float(__builtin_bit_cast(_Float16, h[u][e]));
+                        if constexpr (T == NT_BF16) v[u][e] = __builtin_bit_cast(float, uint32_t(h[u][e]) << 16);
+                        else v[u][e] = float(__builtin_bit_cast(_Float16, h[u][e]));
                     }
             }
             return;
         }
         for (int u = 0; u < 4; u++)
             for (int e = 0; e < 4; e++)
-                if (e < have && k + u < n) x[u][e] = load_f32<T>(xv, (k + u) * ld + c + e);
-    };
-    float m[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-    bool bad[4] = {false, false, false, false};
-    for (int64_t k0 = 0; k0 < n; k0 += 256) {
-        float x[2][4][4];
-        load(k0 + 4 * g, x[0]);
-        load(k0 + 128 + 4 * g, x[1]);
-#pragma unroll
-        for (int v = 0; v < 2; v++)
-#pragma unroll
-            for (int u = 0; u < 4; u++)
-#pragma unroll
-                for (int e = 0; e < 4; e++) {
-                    const float a = fabsf(x[v][u][e]);
-                    bad[e] |= !(a < INFINITY);
-                    m[e] = fmaxf(m[e], a);
-                }
+                if (e < have && k + u < n) v[u][e] = load_f32<T>(x, (k + u) * ld + c + e);
     }
+
+    // The largest magnitude of each column over rows r0 .. r1 - 1 as the bits of an f32, which order as their values do,
+    // infinities and NaN at the end; the workgroup's, in s_top[0].
+    __device__ __forceinline__ void top(int64_t r0, int64_t r1, uint32_t (&s_top)[32][W]) const {
+        const int g = threadIdx.x / (W / 4), lc = threadIdx.x % (W / 4) * 4;
+        uint32_t m[4] = {0, 0, 0, 0};
+        for (int64_t k0 = r0; k0 < r1; k0 += 256) {
+            float v[2][4][4];
+            load(k0 + 4 * g, v[0]);
+            load(k0 + 128 + 4 * g, v[1]);
 #pragma unroll
-    for (int e = 0; e < 4; e++) s_max[g][lc + e] = m[e], s_bad[g][lc + e] = bad[e];
-    __syncthreads();
-    if (t < 64) {
-        float top = 0.0f;
-        int any = 0;
-        for (int k = 0; k < 32; k++) top = fmaxf(top, s_max[k][t]), any |= s_bad[k][t];
-        const float s = scale_of(top, !any);
-        s_max[0][t] = s;
-        if (c0 + t < cols) scale[c0 + t] = s;
+            for (int w = 0; w < 2; w++)
+#pragma unroll
+                for (int u = 0; u < 4; u++)
+#pragma unroll
+                    for (int e = 0; e < 4; e++) m[e] = max(m[e], __builtin_bit_cast(uint32_t, v[w][u][e]) & 0x7fffffffu);
+        }
+#pragma unroll
+        for (int e = 0; e < 4; e++) s_top[g][lc + e] = m[e];
+        __syncthreads();
+        if (threadIdx.x < W) {
+            uint32_t t = 0;
+            for (int k = 0; k < 32; k++) t = max(t, s_top[k][threadIdx.x]);
+            s_top[0][threadIdx.x] = t;
+        }
+    }
+};
+
+// The largest magnitudes of `per` rows (a multiple of 256), [parts, cols].
+template <int T, int W>
+__global__ __launch_bounds__(W * 8) void k_column_tops(const void *x, int64_t cols, int64_t n, int64_t ld, int64_t per,
+                                                       uint32_t *tops) {
+    __shared__ uint32_t s_top[32][W];
+    const int64_t c0 = int64_t(blockIdx.x) * W, r0 = blockIdx.y * per;
+    const Columns<T, W> at(x, cols, n, ld, c0 + threadIdx.x % (W / 4) * 4);
+    at.top(r0, min(n, r0 + per), s_top);
+    if (threadIdx.x < W && c0 + threadIdx.x < cols) tops[blockIdx.y * cols + c0 + threadIdx.x] = s_top[0][threadIdx.x];
+}
+
+// `tops` null: all of n, whose second reading comes from the caches where they hold it. The words go out through LDS, 128
+// values of a column side by side.
+template <int T, int W>
+__global__ __launch_bounds__(W * 8) void k_quantize_columns(const void *x, int64_t cols, int64_t n, int64_t ld, int64_t per,
+                                                            const uint32_t *tops, int parts, int8_t *q, float *scale) {
+    __shared__ uint32_t s_top[32][W];
+    __shared__ float s_scale[W];
+    __shared__ uint32_t tile[W][33];  // [column][words of 4 rows of x]
+    const int t = threadIdx.x, g = t / (W / 4), lc = (t % (W / 4)) * 4;
+    const int64_t c0 = int64_t(blockIdx.x) * W, r0 = blockIdx.y * per, r1 = min(n, r0 + per);
+    const Columns<T, W> at(x, cols, n, ld, c0 + lc);
+    float v[4][4];
+    if (tops) {
+        at.load(r0 + 4 * g, v);
+        uint32_t m = 0;
+        const int64_t c = c0 + t % W;
+        if (c < cols)
+            for (int k = t / W; k < parts; k += 8) m = max(m, tops[k * cols + c]);
+        s_top[t / W][t % W] = m;
+        __syncthreads();
+        if (t < W)
+            for (int k = 1; k < 8; k++) m = max(m, s_top[k][t]);
+        if (t < W) s_top[0][t] = m;
+    } else {
+        at.top(0, n, s_top);
+        at.load(4 * g, v);
+    }
+    if (t < W) {
+        const float top = __builtin_bit_cast(float, s_top[0][t]), s = scale_of(top, top < INFINITY);
+        s_scale[t] = s;
+        if (c0 + t < cols && blockIdx.y == 0) scale[c0 + t] = s;
     }
     __syncthreads();
     float s[4], inv[4];
 #pragma unroll
-    for (int e = 0; e < 4; e++) s[e] = s_max[0][lc + e], inv[e] = 1.0f / s[e];
-    float x[4][4];
-    load(4 * g, x);
-    for (int64_t k0 = 0; k0 < n; k0 += 128) {  // 128 rows of x at a time, the next ones' loads ahead
-        float y[4][4];
-        load(k0 + 128 + 4 * g, y);
+    for (int e = 0; e < 4; e++) s[e] = s_scale[lc + e], inv[e] = 1.0f / s[e];
+    for (int64_t k0 = r0; k0 < r1; k0 += 128) {  // 128 rows of x at a time, the next ones' loads ahead
+        float next[4][4];
+        at.load(k0 + 128 + 4 * g, next);
 #pragma unroll
         for (int e = 0; e < 4; e++) {
-            const float a[4] = {x[0][e], x[1][e], x[2][e], x[3][e]};
+            const float a[4] = {v[0][e], v[1][e], v[2][e], v[3][e]};
             tile[lc + e][g] = quantized4(a, s[e], inv[e]);
         }
         __syncthreads();
@@ -276,16 +318,40 @@ __global__ __launch_bounds__(512) void k_quantize_columns(const void *xv, int64_
 #pragma unroll
         for (int u = 0; u < 4; u++)
 #pragma unroll
-            for (int e = 0; e < 4; e++) x[u][e] = y[u][e];
+            for (int e = 0; e < 4; e++) v[u][e] = next[u][e];
     }
 }
 
 template <int T>
 int launch_columns(const uint8_t *x, int64_t cols, int64_t n, int64_t ld, int8_t *q, float *scale) {
-    constexpr int64_t kMost = int64_t(1) << 28, kSize = T == NT_F32 ? 4 : 2;
+    constexpr int64_t kMost = int64_t(1) << 28, kSize = T == NT_F32 ? 4 : 2, W = 64;
+    const int64_t blocks = ceil_div(cols, W);
+    int64_t per = n, parts = 1;
+    void *tops = nullptr;
+    // Fewer workgroups than CUs: the rows of x in parts, two workgroups a CU, the magnitudes in a launch of their own (us,
+    // f32, whole and in parts: 4096 x 12576 144 and 108, 4096 x 4096 60 and 39, 11008 x 92 236 and 16; but 1024 x 16384,
+    // as many as there are CUs, 32 and 38).
+    if (blocks < 256 && n > 256) {
+        per = round_up(ceil_div(n, ceil_div(512, blocks)), 256);
+        parts = ceil_div(n, per);
+    }
+    if (parts > 1) {
+        if (int rc = scratch_alloc(size_t(parts * cols * 4), &tops)) return rc;
+        k_column_tops<T, W><<<dim3(unsigned(blocks), unsigned(parts)), dim3(W * 8), 0, ctx().stream>>>(
+            x, cols, n, ld, per, static_cast<uint32_t *>(tops));
+        int rc = launched("k_column_tops");
+        if (!rc) {
+            k_quantize_columns<T, W><<<dim3(unsigned(blocks), unsigned(parts)), dim3(W * 8), 0, ctx().stream>>>(
+                x, cols, n, ld, per, static_cast<uint32_t *>(tops), int(parts), q, scale);
+            rc = launched("k_quantize_columns");
+        }
+        const int rf = scratch_release(tops);
+        return rc ? rc : rf;
+    }
     for (int64_t c = 0; c < cols; c += kMost) {
         const int64_t w = std::min(kMost, cols - c);
-        k_quantize_columns<T><<<dim3(unsigned(ceil_div(w, 64))), dim3(512), 0, ctx().stream>>>(x + c * kSize, w, n, ld, q + c * n, scale + c);
+        k_quantize_columns<T, W><<<dim3(unsigned(ceil_div(w, W))), dim3(W * 8), 0, ctx().stream>>>(x + c * kSize, w, n, ld, n, nullptr, 0,
+                                                                                                  q + c * n, scale + c);
         if (int rc = launched("k_quantize_columns")) return rc;
     }
     return 0;
@@ -381,9 +447,13 @@ __global__ __launch_bounds__(S::kThreads, 1) void k_int8_tiles(Int8P p) {
     tile_of(blockIdx.x, p.tm, p.tn, im, in);
     const int64_t m0 = int64_t(im) * T::BM, n0 = int64_t(in) * T::BN;
     const int64_t k0 = blockIdx.y * p.per, kb = p.kb - k0 < p.per ? p.kb - k0 : p.per;
+    // One row of tiles: each from a stage of k of its own on (the sums are exact in any order). Weight rows a power of two
+    // of bytes apart fall on the same HBM channels where every tile reads the same k at once: 64 x 50304 x 4096 59 -> 53 us.
+    // With more rows of tiles those of a column share its panel, and stay together.
+    const int first = p.tm == 1 ? 2 * (in % int((kb + 127) / 128)) : 0;
     T t;
     t.run(lds, Operand{p.a + m0 * p.lda + k0, p.lda, p.m - m0, kb}, Operand{p.b + n0 * p.ldb + k0, p.ldb, p.n - n0, kb}, kb, wave,
-          lane);
+          lane, first);
     const int wm = wave / WN, wn = wave % WN;
     constexpr bool kWide = OUT == NT_F32 || OUT == kSlab;
     typedef typename std::conditional<kWide, u32x4, u32x2>::type V;

@@ -46,8 +46,8 @@ inline Plan plan(int64_t m, int64_t n, int64_t kb, bool split) {
     Plan best{};
     for (const Kind &c : kinds) {
         const int64_t tiles = ceil_div(m, c.rows) * ceil_div(n, c.cols);
-        for (int64_t r = 0; r <= 3; r++) {  // unsplit, and the splits that fill one to three rounds
-            int64_t s = r == 0 ? 1 : c.slots * r / tiles;
+        for (int64_t r = 0; r <= 4; r++) {  // unsplit, and the splits that give every CU one to four workgroups
+            int64_t s = r == 0 ? 1 : 256 * r / tiles;
             s = s > 64 ? 64 : s;
             if (s < 1 || (s > 1 && !split)) continue;
             const int64_t per = round_up(ceil_div(kb, s), 64), splits = ceil_div(kb, per);

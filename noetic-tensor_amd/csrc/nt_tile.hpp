@@ -221,7 +221,10 @@ struct Tile {
     // in 4188 us with single stages). From an even stage t on the pair t + 2 PAIRS goes into the buffers of t - 1 and
     // t, which every wave has read by the barrier in front, a quarter of its copies in each of four steps: the
     // load unit takes about 24 cycles for a copy of 1 KiB, and a wave whose copy has to wait issues no MFMAs.
-    __device__ __forceinline__ void run(uint8_t *lds, const Operand &a, const Operand &b, int64_t kb, int wave, int lane) {
+    //
+    // The stages are taken from stage `first` (even) on, those in front of it last.
+    __device__ __forceinline__ void run(uint8_t *lds, const Operand &a, const Operand &b, int64_t kb, int wave, int lane,
+                                        int first = 0) {
 #ifdef __HIP_DEVICE_COMPILE__  // (the host pass, which drops the body, cannot emit its lambdas' asm)
         SideA sa;
         SideB sb;
@@ -235,17 +238,23 @@ struct Tile {
 #pragma unroll
                 for (int v = 0; v < 16; v++) acc[i][j][v] = 0;
         const int n = int((kb + kStageK - 1) / kStageK);
+        const int n2 = (n + 1) / 2 * 2;
+        auto turn = [&](int t) {
+            if (t >= n2) return t;
+            const int u = t + first;
+            return u >= n2 ? u - n2 : u;
+        };
         const uint32_t at = uint32_t((uintptr_t)(lds_ptr)(lds));
         Frags x, y;
         unrolled<PAIRS - 1>([&](auto u) {
             uint8_t *to = lds + 2 * u * kStageBytes;
-            sa.begin(2 * u);
-            sb.begin(2 * u);
+            sa.begin(turn(2 * u));
+            sb.begin(turn(2 * u));
             unrolled<kPair>([&](auto o) { copy<o>(sa, sb, to, to + kStageBytes, wave); });
         });
         uint32_t even = (2 * PAIRS - 2) * kStageBytes, odd = even + kStageBytes;  // the buffers of the pair being copied
-        sa.begin(2 * PAIRS - 2);
-        sb.begin(2 * PAIRS - 2);
+        sa.begin(turn(2 * PAIRS - 2));
+        sb.begin(turn(2 * PAIRS - 2));
         unrolled<part(3)>([&](auto o) { copy<o>(sa, sb, lds + even, lds + odd, wave); });
         wait_copies<(PAIRS - 2) * kPair + part(3)>();
         asm volatile("s_barrier" ::: "memory");
@@ -259,8 +268,8 @@ struct Tile {
             step<0, part(3), kPair>(sa, sb, x, y, at + b0, lds + even, lds + odd, wave);
             landed(y.a, y.b);
             asm volatile("s_barrier" ::: "memory");  // every wave has read stage t
-            sa.begin(t + 2 * PAIRS);
-            sb.begin(t + 2 * PAIRS);
+            sa.begin(turn(t + 2 * PAIRS));
+            sb.begin(turn(t + 2 * PAIRS));
             even = after(odd);  // (stage t - 1's)
             odd = b0;
             step<1, 0, part(1)>(sa, sb, y, x, at + b1, lds + even, lds + odd, wave);

@@ -66,6 +66,26 @@ def test_rows_and_columns(rows, cols, dtype):
     same(q, s, quantized(x.t()))
 
 
+@pytest.mark.parametrize("n,cols", [(256, 1), (257, 1), (511, 65), (513, 64), (1500, 700), (4099, 130), (70001, 3),
+                                    (300, 16400), (515, 16321), (260, 16319)])
+def test_long_columns(n, cols):
+    """Columns of one workgroup and of several, at the borders between them: a column's largest value, its NaN or its
+    infinity in the first part, the last, or alone in the last row."""
+    g = torch.Generator().manual_seed(n + cols)
+    x = torch.randn(n, cols, generator=g)
+    x[n - 1] *= 100.0
+    x[n // 2, ::3] *= 1000.0
+    x[:, 0] = 0.0
+    x[n - 1, 0] = -1e-30
+    if cols > 2:
+        x[n - 1, 1] = math.nan
+        x[0, 2] = -math.inf
+    for dtype in TORCH.values():
+        y = x.to(dtype)
+        q, s = ops.quantize_int8(given(y), ops.Layout([cols, n], [1, cols]))
+        same(q, s, quantized(y.t()))
+
+
 def test_borders():
     """Quotients at and next to halves: rows whose largest value is 127 times a power of two or three of it, so that
     the scale and the halves are exact, and each half's neighbours in f32."""
