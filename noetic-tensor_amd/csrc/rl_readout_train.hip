@@ -21,6 +21,11 @@
 //  gradients are when they are written); every sum is f32. For f16, whose range G would leave, a row of G is
 //  held in units of 2^(e - 14), 2^e over |g_logp| + 16 |g_entropy| (p |ln p + entropy| is under 14 for a
 //  vocabulary of 2^20), its share of dW being scaled through the row of H by a power of two.
+//
+//  Bound by the matrix cores for many rows, and those by power: 4096 x 4096 x 128256 bf16 is scored in 3.2-3.3 ms (1.33
+//  PFLOP/s at a clock near 1.5 GHz; a library product alone 2.99) and scored and differentiated in 13.4 ms (1.29 at its 8
+//  R V dim). Few rows are bound by the weight's bytes and the launches: 64 x 1024 x 32000 scored in 26.5 us
+//  (of 14 at a copy's rate), 128 rows differentiated with it in 104 (28).
 #include <hip/hip_runtime.h>
 
 #include <algorithm>

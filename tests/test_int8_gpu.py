@@ -192,6 +192,8 @@ def test_scales_that_are_not_plain():
     assert np.isnan(y[2]).all() and (y[3] == 0).all() and np.isfinite(y[[0, 1, 3, 4]]).all()
     y = ops.matmul_int8(nr.Tensor((2, 0), "i8"), given(torch.ones(2)), nr.Tensor((3, 0), "i8"), given(torch.ones(3)))
     assert (y.to_numpy() == 0).all()
+    y = ops.matmul_int8(nr.Tensor((70, 0), "i8"), given(torch.ones(70)), nr.Tensor((300, 0), "i8"), given(torch.ones(300)))
+    assert (y.to_numpy() == 0).all()
     assert ops.matmul_int8(nr.Tensor((0, 4), "i8"), nr.Tensor((0,), "f32"), nr.Tensor((3, 4), "i8"),
                            given(torch.ones(3))).shape == (0, 3)
 
