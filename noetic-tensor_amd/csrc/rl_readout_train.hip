@@ -64,7 +64,7 @@ struct MaskP {
 template <int TN>
 struct MaskBlock {
     static constexpr int kU8 = 32 * TN + 16, kF32 = 128 * TN + 16;  // bytes of a row in LDS
-    static constexpr int kLds = 32 * kF32;
+    static constexpr int kLds = 32 * kF32, kShared = 128 * TN;  // (of 32 rows, and of one that all share)
     // Rows row0 .. row0 + rows - 1 of the mask (a row that all share, ld 0, once, before the first block).
     static __device__ __forceinline__ void in(uint8_t *lds, const MaskP &m, int64_t row0, int rows, int col, int n, int lane,
                                               bool first) {
@@ -458,9 +458,11 @@ __global__ __launch_bounds__(S::kThreads, 1) void k_readout_g(PieceP p) {
     const int col0 = in * T::BN + 32 * TN * wn + 4 * (lane / 32);
     const float c = MASK && p.mask.f32 ? 1.0f : p.c;
     const int64_t bytes = p.gbytes - (in * T::BN + 32 * TN * wn) * 2;
-    constexpr int kMask = MASK ? MaskBlock<TN>::kLds : 0, kWave = store_bytes<TN>(2) > kMask ? store_bytes<TN>(2) : kMask;
-    static_assert(kWave * WM * WN <= T::kLds, "the blocks fit");
-    uint8_t *const mlds = lds + wave * kWave, *const slds = mlds;  // (the mask's block is read before G's is written)
+    // (a mask's 32 rows are read before G's block is written over them; a row that all share stays in front of it)
+    constexpr int kShared = MASK ? MaskBlock<TN>::kShared : 0, kMask = MASK ? MaskBlock<TN>::kLds : 0;
+    constexpr int kStore = kShared + store_bytes<TN>(2), kWave = kStore > kMask ? kStore : kMask;
+    static_assert(kWave * WM * WN <= T::kLds && kWave % 16 == 0, "the blocks fit");
+    uint8_t *const mlds = lds + wave * kWave, *const slds = mlds + kShared;
     float4 coef[TM];
     int tok[TM];  // the token's column from this lane's first, or -1
 #pragma unroll

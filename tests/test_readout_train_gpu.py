@@ -454,9 +454,12 @@ def test_a_policy_step_with_an_8_bit_rollout():
     agree(values(gw), want["grad_weight"], tol["grad_weight"], "grad_weight")
 
 
-# Sizes that every tile, split and cut of the products is taken at: 256 x 256 tiles in whole rounds with a rest beside them
-# (2100 x 16640, dim 1100 for its k), 128 x 128 and 64 x 128 ones, k split and not, in both layouts.
+# Sizes that every tile, split and cut of the products is taken at: 256 x 256 tiles (300 x 32768, 1500 x 17001), those in
+# whole rounds with a rest beside them (2100 x 32768), 128 x 128 and 64 x 128 ones, k split and not, in both layouts.
 @pytest.mark.parametrize("rows,V,d,dtype,layout,mask", [
+    (300, 32768, 512, "bf16", "dv", "none"), (1500, 17001, 520, "f16", "vd", "u8_shared"),
+    (1500, 17001, 512, "bf16", "vd", "f32_shared"), (2100, 32768, 512, "bf16", "dv", "u8"),
+    (2100, 32768, 512, "bf16", "dv", "f32_shared"), (2100, 32768, 520, "f16", "vd", "f32"),
     (2100, 16640, 1100, "bf16", "dv", "u8"), (2100, 16640, 1100, "f16", "vd", "none"), (2050, 17001, 1096, "bf16", "vd", "f32_shared"),
     (700, 9000, 200, "bf16", "vd", "f32"), (130, 30011, 520, "f16", "dv", "none"), (64, 20000, 300, "bf16", "dv", "none"),
     (65, 20000, 304, "bf16", "vd", "u8_shared"), (1, 50257, 128, "bf16", "vd", "none")])
