@@ -18,14 +18,17 @@
 //  operations with the forward's, against 6 where the logits are kept: the least there is without them.
 //
 //  Rounding: G is the one value that is rounded on the way (2^-9 of itself for bf16, 2^-12 for f16, as the
-//  gradients are when they are written); every sum is f32. For f16, whose range G would leave, a row of G is
+//  gradients are when they are written); every sum is f32. A row's entry at its token is most of G, and its rounding
+//  would show in the gradients as their own does: for up to 512 rows what it left goes into both of them in f32, times the
+//  token's row of W and the row of H (128 x 1024 x 32000 bf16: the error is 0.0017 of the norm, which is the written
+//  values' own, instead of 0.0022, for 112 us instead of 104). For f16, whose range G would leave, a row of G is
 //  held in units of 2^(e - 14), 2^e over |g_logp| + 16 |g_entropy| (p |ln p + entropy| is under 14 for a
 //  vocabulary of 2^20), its share of dW being scaled through the row of H by a power of two.
 //
 //  Bound by the matrix cores for many rows, and those by power: 4096 x 4096 x 128256 bf16 is scored in 3.2-3.3 ms (1.33
 //  PFLOP/s at a clock near 1.5 GHz; a library product alone 2.99) and scored and differentiated in 13.4 ms (1.29 at its 8
 //  R V dim). Few rows are bound by the weight's bytes and the launches: 64 x 1024 x 32000 scored in 26.5 us
-//  (of 14 at a copy's rate), 128 rows differentiated with it in 104 (28).
+//  (of 14 at a copy's rate), 128 rows differentiated with it in 112 (28).
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -172,6 +175,7 @@ struct PieceP {
     const float4 *coef;       // [rows] {lse log2 e (+inf: nothing flows), a, b, the token's term}
     uint8_t *g;               // [rows, ldg bytes], of which gbytes are written: zeros past n
     int64_t ldg, gbytes;
+    float *left;              // [rows] what the rounding of G's entry at the row's token left, or null
 };
 
 template <class T, bool BTR>
@@ -357,6 +361,7 @@ struct CoefP {
     double tau;
     int f16;
     float4 *coef;
+    float *left;   // [rows] zeros here, or null
     float *up;     // [rows] f16: what a row of G was divided by
     float *top;    // [1] f16: the largest of them
 };
@@ -389,6 +394,7 @@ __global__ __launch_bounds__(1024) void k_readout_coef(CoefP p) {
             unit = 1.0 / p.tau;
         }
         if (p.f16) p.up[r] = up;
+        if (p.left) p.left[r] = 0.0f;
         const float a = float(-(gl + ge * h) * unit), b = float(-ge * kLn2 * unit);
         p.coef[r] = dead ? float4{INFINITY, 0.0f, 0.0f, 0.0f} : float4{float(lse * kLog2eD), a, b, float(gl * unit)};
     }
@@ -408,7 +414,7 @@ __global__ __launch_bounds__(1024) void k_readout_coef(CoefP p) {
 // NaN too, stays out of dW) and with `up`, f16 rows are scaled by up / top, a power of two.
 __global__ __launch_bounds__(256) void k_readout_rows(const uint16_t *src, int64_t rows, int64_t cols, int64_t ld,
                                                       uint8_t *out, int64_t ldo, const float4 *coef, const float *up,
-                                                      const float *top, int64_t again) {
+                                                      const float *top) {
     const int64_t per = ldo / 16, total = rows * per;
     for (int64_t i = blockIdx.x * int64_t(256) + threadIdx.x; i < total; i += int64_t(gridDim.x) * 256) {
         const int64_t r = i / per, c = (i - r * per) * 8;
@@ -430,7 +436,6 @@ __global__ __launch_bounds__(256) void k_readout_rows(const uint16_t *src, int64
             }
         }
         *reinterpret_cast<u32x4 *>(out + r * ldo + c * 2) = x.v;
-        if (again) *reinterpret_cast<u32x4 *>(out + (r + again) * ldo + c * 2) = x.v;
     }
 }
 
@@ -440,10 +445,8 @@ __device__ __forceinline__ float widened(uint32_t h) {
     else return float(__builtin_bit_cast(_Float16, uint16_t(h)));
 }
 
-// A piece's G. TWO: up to 64 rows, where one rounding of a row's largest entries (its token's above all) is not averaged away in
-// the gradients' sums: what the rounding left goes into rows `rows` .. 2 rows - 1, and the products take both.
-// A stage of 32 k or a 64-row tile costs the same at twice so few rows.
-template <class E, class S, bool BTR, bool TWO, bool MASK>
+// A piece's G.
+template <class E, class S, bool BTR, bool MASK>
 __global__ __launch_bounds__(S::kThreads, 1) void k_readout_g(PieceP p) {
     constexpr int TM = S::TM, TN = S::TN, WM = S::WM, WN = S::WN;
     typedef Tile<E, TM, TN, WM, WN, false, BTR> T;
@@ -470,7 +473,7 @@ __global__ __launch_bounds__(S::kThreads, 1) void k_readout_g(PieceP p) {
         const int64_t row = int64_t(im) * T::BM + 32 * (TM * wm + i) + lane % 32, r = row < p.rows ? row : p.rows - 1;
         coef[i] = p.coef[r];
         const int64_t at = p.tokens[r] - p.v0;
-        tok[i] = at >= 0 && at < p.n ? int(at) - col0 : -1;
+        tok[i] = at >= 0 && at < p.n && row < p.rows ? int(at) - col0 : -1;
     }
     if (bytes <= 0) return;
 #pragma unroll
@@ -481,7 +484,7 @@ __global__ __launch_bounds__(S::kThreads, 1) void k_readout_g(PieceP p) {
         const bool dead = k.x == INFINITY;
         // (of 32 rows few have their token among this wave's columns)
         const bool mine = __any(tok[i] >= 0 && tok[i] < 32 * TN);
-        u32x2 v[4 * TN], lo[TWO ? 4 * TN : 1];
+        u32x2 v[4 * TN];
         float x[4 * TN][4];
 #pragma unroll
         for (int q = 0; q < 4 * TN; q++)
@@ -506,16 +509,15 @@ __global__ __launch_bounds__(S::kThreads, 1) void k_readout_g(PieceP p) {
                 for (int e = 0; e < 4; e++)
                     if (tok[i] == 8 * q + e) g[e] += k.w;
             v[q] = dead ? u32x2{0, 0} : u32x2{pair16<E>(g[0], g[1]), pair16<E>(g[2], g[3])};
-            if constexpr (TWO) {
-                const float r[4] = {g[0] - widened<E>(v[q].x), g[1] - widened<E>(v[q].x >> 16), g[2] - widened<E>(v[q].y),
-                                    g[3] - widened<E>(v[q].y >> 16)};
-                lo[q] = dead ? u32x2{0, 0} : u32x2{pair16<E>(r[0], r[1]), pair16<E>(r[2], r[3])};
-            }
+            if (mine && p.left)
+#pragma unroll
+                for (int e = 0; e < 4; e++)
+                    if (tok[i] == 8 * q + e && !dead)
+                        p.left[row0 + lane % 32] = g[e] - widened<E>((e < 2 ? v[q].x : v[q].y) >> (16 * (e % 2)) & 0xffffu);
         }
         const int rows = p.rows - row0 < 32 ? int(p.rows - row0) : 32, have = bytes < 64 * TN ? int(bytes) : 64 * TN;
         uint8_t *o = p.g + row0 * p.ldg + (in * T::BN + 32 * TN * wn) * 2;
         store_block<TN>(slds, v, lane, o, p.ldg, rows, have);
-        if constexpr (TWO) store_block<TN>(slds, lo, lane, o + p.rows * p.ldg, p.ldg, rows, have);
     }
 }
 
@@ -534,10 +536,61 @@ struct GradP {
     const float *row_scale;   // f16: [m] or null
     const float *scale;       // f16: [1] or null
     float fixed;
+    // dW: what the rounding of G left of the tokens' entries (null: dH)
+    const float *left;        // [k]
+    const int32_t *tokens;    // [k]
+    int64_t v0;               // the vocabulary's first row of the output (VD) or column (DV)
+    bool dv;
 };
 
+// acc += left[r] H(r, .) at row r's token, for the rows whose token is among this wave's vocabulary from v0 on (its 32 rows,
+// or its columns, DV), in the order of r. `h` is H as the product reads it, [k, ldh bytes], `wh` bytes of each row.
+// `mine` and `lefts`: those of rows lane, lane + 64, .. (token -1 past the last), loaded in front of the product: a tile of so
+// few k takes no longer than a load.
+//
+// More than kLeftRows rows average their entries' roundings: the gradients' error is the written values' own and as much
+// again, within 6% of 1.41 of it, where with 128 rows a few upstream gradients far larger than the others make it 1.5 and
+// more; and the 256 x 256 tiles, which take over there, have no registers to add it in.
+constexpr int kLeftRows = 512, kLefts = kLeftRows / 64;
+template <class E, bool DV, int TN, class Acc>
+__device__ __forceinline__ void add_left(Acc (&acc)[TN], const GradP &p, const int (&mine)[kLefts], const float (&lefts)[kLefts],
+                                         int64_t v0, const uint8_t *h, int64_t ldh, int64_t wh, int64_t row0, int64_t col0, int lane) {
+    constexpr int BV = DV ? 32 * TN : 32;
+    const int first = int(v0);
+#pragma unroll
+    for (int b = 0; b < kLefts; b++) {
+        uint64_t hits = __ballot(mine[b] >= first && mine[b] < first + BV);
+        while (hits) {
+            const int at = __builtin_ctzll(hits), c = __builtin_amdgcn_readlane(mine[b], at) - first, k0 = 64 * b;
+            hits &= hits - 1;
+            const float left = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, lefts[b]), at));
+            const uint16_t *hr = reinterpret_cast<const uint16_t *>(h + (k0 + at) * ldh);
+            if constexpr (DV) {
+                const int64_t row = row0 + lane % 32;
+                const float x = left * widened<E>(hr[row < p.m ? row : 0]);
+                const int k = lane / 32 == c / 4 % 2 ? c / 8 * 4 + c % 4 : -1;
+#pragma unroll
+                for (int q = 0; q < 16 * TN; q++) acc[q / 16][q % 16] += k == q ? x : 0.0f;
+            } else {
+                uint16_t w[4 * TN][4];
+#pragma unroll
+                for (int q = 0; q < 4 * TN; q++) {  // (every load before the first use; columns past the end are not stored)
+                    const int64_t col = col0 + 8 * q + 4 * (lane / 32);
+                    __builtin_memcpy(w[q], hr + (col * 2 + 8 <= wh ? col : 0), 8);
+                }
+                const float f = lane % 32 == c ? left : 0.0f;
+#pragma unroll
+                for (int q = 0; q < 4 * TN; q++)
+#pragma unroll
+                    for (int e = 0; e < 4; e++) acc[q / 4][4 * (q % 4) + e] = fmaf(f, widened<E>(w[q][e]), acc[q / 4][4 * (q % 4) + e]);
+            }
+        }
+    }
+}
+
+// (Two waves a SIMD, 256 registers each, or the smaller tiles' second workgroup waits: dW 128 x 1024 x 32000 54 -> 30 us.)
 template <class E, class S, bool ATR, bool BTR>
-__global__ __launch_bounds__(S::kThreads, 1) void k_readout_grad(GradP p) {
+__global__ __launch_bounds__(S::kThreads, S::TM == 1 ? 2 : 1) void k_readout_grad(GradP p) {
     constexpr int TM = S::TM, TN = S::TN, WM = S::WM, WN = S::WN;
     typedef Tile<E, TM, TN, WM, WN, ATR, BTR> T;
     __shared__ __attribute__((aligned(16))) uint8_t lds[T::kLds];
@@ -552,9 +605,28 @@ __global__ __launch_bounds__(S::kThreads, 1) void k_readout_grad(GradP p) {
                           : Operand{p.a + m0 * p.lda + k0 * 2, p.lda, p.m - m0, kb};
     const Operand b = BTR ? Operand{p.b + k0 * p.ldb + n0 * 2, p.ldb, kn, p.wb - n0 * 2}
                           : Operand{p.b + n0 * p.ldb + k0 * 2, p.ldb, p.n - n0, kb};
+    constexpr bool kLeft = ATR && BTR && TM == 1;
+    int mine[kLeft ? kLefts : 1];
+    float lefts[kLeft ? kLefts : 1];
+    if (kLeft && p.left) {
+#pragma unroll
+        for (int q = 0; q < kLefts; q++) {
+            const int r = 64 * q + lane < p.k ? 64 * q + lane : 0;
+            mine[q] = p.tokens[r];
+            lefts[q] = p.left[r];
+            if (64 * q + lane >= p.k) mine[q] = -1;
+        }
+    }
     T t;
     t.run(lds, a, b, kb, wave, lane);
     const int wm = wave / WN, wn = wave % WN;
+    if constexpr (kLeft) {
+        if (p.left && blockIdx.y == 0) {
+            const int64_t row0 = m0 + 32 * wm, c0 = n0 + 32 * TN * wn;
+            if (p.dv) add_left<E, true>(t.acc[0], p, mine, lefts, p.v0 + c0, p.a, p.lda, p.wa, row0, c0, lane);
+            else add_left<E, false>(t.acc[0], p, mine, lefts, p.v0 + row0, p.b, p.ldb, p.wb, row0, c0, lane);
+        }
+    }
     const float whole = p.scale ? *p.scale * p.fixed : p.fixed;
     const int64_t col0 = n0 + 32 * TN * wn;
     if (col0 >= p.n) return;
@@ -607,21 +679,33 @@ __global__ __launch_bounds__(S::kThreads, 1) void k_readout_grad(GradP p) {
     }
 }
 
-// The slabs' sum in their order, scaled and rounded; with `two` > 0, of rows r and r + two of each.
+// The slabs' sum in their order, scaled and rounded; with `left`, first each row's times the token's row of W (a column
+// of it, DV).
+struct LeftP {
+    const float *left;      // [m] or null
+    const int32_t *tokens;  // [m]
+    const uint16_t *w;
+    int64_t ldw;
+    int dv;
+};
+
 template <class E>
-__global__ __launch_bounds__(256) void k_readout_fold(const float *slab, int splits, int64_t m, int64_t n, int64_t two,
-                                                      uint16_t *out, int64_t ldo, const float *row_scale, const float *scale,
-                                                      float fixed) {
-    const int64_t per = (n + 3) / 4, rows = two ? two : m, total = rows * per;
-    const int terms = two ? 2 * splits : splits;
+__global__ __launch_bounds__(256) void k_readout_fold(const float *slab, int splits, int64_t m, int64_t n, LeftP p, uint16_t *out,
+                                                      int64_t ldo, const float *row_scale, const float *scale, float fixed) {
+    const int64_t per = (n + 3) / 4, total = m * per;
     for (int64_t i = blockIdx.x * int64_t(256) + threadIdx.x; i < total; i += int64_t(gridDim.x) * 256) {
         const int64_t r = i / per, c = (i - r * per) * 4;
         const int have = n - c >= 4 ? 4 : int(n - c);
         float x[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-        auto at = [&](int z) { return slab + (two ? (z / 2) * m + r + (z % 2) * two : z * m + r) * n + c; };
+        const float left = p.left ? p.left[r] : 0.0f;
+        if (left != 0.0f) {
+            const uint16_t *w = p.w + (p.dv ? c * p.ldw + p.tokens[r] : p.tokens[r] * p.ldw + c);
+            for (int e = 0; e < have; e++) x[e] = left * widened<E>(w[p.dv ? e * p.ldw : e]);
+        }
+        auto at = [&](int z) { return slab + (z * m + r) * n + c; };
         int z = 0;
         if (have == 4)
-            for (; z + 8 <= terms; z += 8) {  // (eight loads in flight)
+            for (; z + 8 <= splits; z += 8) {  // (eight loads in flight)
                 float v[8][4];
 #pragma unroll
                 for (int k = 0; k < 8; k++) __builtin_memcpy(v[k], at(z + k), 16);
@@ -630,7 +714,7 @@ __global__ __launch_bounds__(256) void k_readout_fold(const float *slab, int spl
 #pragma unroll
                     for (int e = 0; e < 4; e++) x[e] += v[k][e];
             }
-        for (; z < terms; z++)
+        for (; z < splits; z++)
             for (int e = 0; e < have; e++) x[e] += at(z)[e];
         float f = scale ? *scale * fixed : fixed;
         if (row_scale) f *= row_scale[r];
@@ -721,10 +805,10 @@ bool aligned(const void *p, int64_t cols, int64_t ld) {
 }
 
 int copy_rows(const void *src, int64_t rows, int64_t cols, int64_t ld, uint8_t *out, int64_t ldo, const float4 *coef,
-              const float *up, const float *top, int64_t again = 0) {
+              const float *up, const float *top) {
     const int64_t n = rows * (ldo / 16);
     hipLaunchKernelGGL(k_readout_rows, dim3(unsigned(std::min<int64_t>(ceil_div(n, 256), 8192))), dim3(256), 0,
-                       ctx().stream, static_cast<const uint16_t *>(src), rows, cols, ld, out, ldo, coef, up, top, again);
+                       ctx().stream, static_cast<const uint16_t *>(src), rows, cols, ld, out, ldo, coef, up, top);
     return launched("k_readout_rows");
 }
 
@@ -804,29 +888,26 @@ int stats(const PieceP &p, bool ent) {
     }
 }
 
-template <class E, class S, bool BTR, bool TWO>
+template <class E, class S, bool BTR>
 int launch_g(PieceP p) {
     p.tm = uint32_t(ceil_div(p.rows, S::kRows));
     p.tn = uint32_t(ceil_div(p.n, S::kCols));
     const dim3 grid(p.tm * p.tn), block(S::kThreads);
-    if (p.mask.u8 || p.mask.f32) k_readout_g<E, S, BTR, TWO, true><<<grid, block, 0, ctx().stream>>>(p);
-    else k_readout_g<E, S, BTR, TWO, false><<<grid, block, 0, ctx().stream>>>(p);
+    if (p.mask.u8 || p.mask.f32) k_readout_g<E, S, BTR, true><<<grid, block, 0, ctx().stream>>>(p);
+    else k_readout_g<E, S, BTR, false><<<grid, block, 0, ctx().stream>>>(p);
     return launched("k_readout_g");
 }
 
-constexpr int64_t kTwoRows = 64;  // G in two terms for so many rows: the Small tile's
-
 template <class E, bool BTR>
 int g_piece(const PieceP &p) {
-    if (p.rows <= kTwoRows) return launch_g<E, Small, BTR, true>(p);
     if (const int64_t c = whole_rounds(p.rows, p.n, p.kbytes)) {
-        if (int rc = launch_g<E, Large, BTR, false>(part_of(p, BTR, 0, c))) return rc;
+        if (int rc = launch_g<E, Large, BTR>(part_of(p, BTR, 0, c))) return rc;
         return g_piece<E, BTR>(part_of(p, BTR, c, p.n - c));
     }
     switch (plan(p.rows, p.n, p.kbytes, false).size) {
-        case Size::kSmall: return launch_g<E, Small, BTR, false>(p);
-        case Size::kMedium: return launch_g<E, Medium, BTR, false>(p);
-        default: return launch_g<E, Large, BTR, false>(p);
+        case Size::kSmall: return launch_g<E, Small, BTR>(p);
+        case Size::kMedium: return launch_g<E, Medium, BTR>(p);
+        default: return launch_g<E, Large, BTR>(p);
     }
 }
 
@@ -899,10 +980,10 @@ int forward(const NtRlReadoutStatsArgs *a) {
 }
 
 template <class E>
-int fold(const GradP &p, int64_t splits, uint16_t *out, int64_t two = 0) {
-    const int64_t n = (two ? two : p.m) * ceil_div(p.n, 4);
+int fold(const GradP &p, int64_t splits, uint16_t *out, const LeftP &left = {}) {
+    const int64_t n = p.m * ceil_div(p.n, 4);
     hipLaunchKernelGGL(k_readout_fold<E>, dim3(unsigned(std::min<int64_t>(ceil_div(n, 256), 8192))), dim3(256), 0,
-                       ctx().stream, p.slab, int(splits), p.m, p.n, two, out, p.ldo, p.row_scale, p.scale, p.fixed);
+                       ctx().stream, p.slab, int(splits), p.m, p.n, left, out, p.ldo, p.row_scale, p.scale, p.fixed);
     return launched("k_readout_fold");
 }
 
@@ -943,7 +1024,6 @@ int piece(const BackP &b) {
     const NtRlReadoutStatsGradArgs *a = b.a;
     const PieceP &p = b.p;
     if (int rc = g_piece<E, DV>(p)) return rc;
-    const int64_t two = p.rows <= kTwoRows ? p.rows : 0;  // (rows of G's second term)
     if (a->grad_weight) {
         GradP w{};
         w.a = DV ? b.hs : p.g;
@@ -952,14 +1032,18 @@ int piece(const BackP &b) {
         w.ldb = w.wb = DV ? p.ldg : b.ldhs;
         w.m = DV ? p.dim : p.n;
         w.n = DV ? p.n : p.dim;
-        w.k = p.rows + two;
+        w.k = p.rows;
+        w.left = p.left;
+        w.tokens = p.tokens;
+        w.v0 = p.v0;
+        w.dv = DV;
         uint16_t *out = static_cast<uint16_t *>(a->grad_weight) + (DV ? p.v0 : p.v0 * a->grad_weight_ld);
         w.ldo = a->grad_weight_ld;
         w.out = b.sw.splits > 1 ? nullptr : out;
         w.slab = b.slab_w;
         w.scale = b.top;
         w.fixed = b.fixed;
-        const int64_t c = b.sw.splits > 1 ? 0 : whole_rounds(DV ? w.m : w.n, DV ? w.n : w.m, w.k * 2);
+        const int64_t c = b.sw.splits > 1 || p.left ? 0 : whole_rounds(DV ? w.m : w.n, DV ? w.n : w.m, w.k * 2);
         if (c) {  // whole rounds of the vocabulary's side, and its rest
             GradP first = w, rest = w;
             (DV ? first.n : first.m) = c;
@@ -967,6 +1051,7 @@ int piece(const BackP &b) {
             (DV ? rest.b : rest.a) += c * 2;
             (DV ? rest.wb : rest.wa) -= c * 2;
             rest.out += DV ? c : c * rest.ldo;
+            rest.v0 += c;
             if (int rc = launch_product<E, Large, true, true>(first, b.sw)) return rc;
             if (int rc = product<E, true, true>(rest, plan(rest.m, rest.n, rest.k * 2, false))) return rc;
         } else if (int rc = product<E, true, true>(w, b.sw)) {
@@ -982,7 +1067,7 @@ int piece(const BackP &b) {
         h.b = p.w;
         h.ldb = p.ldw;
         h.wb = p.wwidth;
-        h.m = p.rows + two;
+        h.m = p.rows;
         h.n = p.dim;
         h.k = p.n;
         h.ldo = a->grad_hidden_ld;
@@ -993,8 +1078,10 @@ int piece(const BackP &b) {
         h.row_scale = b.up;
         h.fixed = b.fixed;
         if (int rc = product<E, false, !DV>(h, b.sh)) return rc;
-        if (b.hslab && b.last)
-            if (int rc = fold<E>(h, b.sh.splits, out, two)) return rc;
+        if (b.hslab && b.last) {
+            const LeftP left{p.left, p.tokens, static_cast<const uint16_t *>(a->weight), a->ldw, DV};
+            if (int rc = fold<E>(h, b.sh.splits, out, left)) return rc;
+        }
     }
     return 0;
 }
@@ -1016,19 +1103,20 @@ int backward(const NtRlReadoutStatsGradArgs *a) {
     // 4096 x 128256 13.8 against 13.5 ms.)
     int64_t most = (int64_t(1) << 28) / R;
     if (!wdirect) most = std::min(most, (int64_t(1) << 26) / kp);
-    const int64_t cols = piece_cols(V, most), pieces = ceil_div(V, cols);
+    const int64_t cols = piece_cols(V, most);
     // dH: [rows, dim], k the piece's columns; dW: [vocab, dim] or [dim, vocab], k the rows
-    const int64_t two = R <= kTwoRows ? R : 0;
     const int64_t width = std::min(cols, V);
-    const Plan sh = plan(R + two, d, round_up(width, 8) * 2, true);
-    const Plan sw = dv ? plan(d, width, (R + two) * 2, true) : plan(width, d, (R + two) * 2, true);
-    const bool hslab = sh.splits > 1 || pieces > 1 || two;
+    const bool kept = R <= kLeftRows;
+    const Plan sh = plan(R, d, round_up(width, 8) * 2, true);
+    const Size most_w = kept ? Size::kMedium : Size::kLarge;
+    const Plan sw = dv ? plan(d, width, R * 2, true, most_w) : plan(width, d, R * 2, true, most_w);
+    const bool hslab = sh.splits > 1 || cols < V || kept;
     Scratch s;
-    const int o_h = s.add(hdirect ? 0 : R * kp * 2), o_hs = s.add((R + two) * kp * 2);
+    const int o_h = s.add(hdirect ? 0 : R * kp * 2), o_hs = s.add(R * kp * 2);
     const int o_w = s.add(wdirect ? 0 : (dv ? d * cols : cols * kp) * 2);
-    const int o_coef = s.add(R * 16), o_up = s.add(R * 4), o_top = s.add(4);
-    const int o_g = s.add((R + two) * cols * 2);
-    const int o_sh = s.add(a->grad_hidden && hslab ? sh.splits * (R + two) * d * 4 : 0);
+    const int o_coef = s.add(R * 16), o_left = s.add(kept ? R * 4 : 0), o_up = s.add(R * 4), o_top = s.add(4);
+    const int o_g = s.add(R * cols * 2);
+    const int o_sh = s.add(a->grad_hidden && hslab ? sh.splits * R * d * 4 : 0);
     const int o_sw = s.add(a->grad_weight && sw.splits > 1 ? sw.splits * std::min(cols, V) * d * 4 : 0);
     if (int rc = s.allocate()) return rc;
     const float *up = f16 ? s.at<float>(o_up) : nullptr, *top = f16 ? s.at<float>(o_top) : nullptr;
@@ -1045,12 +1133,13 @@ int backward(const NtRlReadoutStatsGradArgs *a) {
     c.tau = a->temperature;
     c.f16 = f16;
     c.coef = s.at<float4>(o_coef);
+    c.left = kept ? s.at<float>(o_left) : nullptr;
     c.up = s.at<float>(o_up);
     c.top = s.at<float>(o_top);
     hipLaunchKernelGGL(k_readout_coef, dim3(f16 ? 1 : unsigned(std::min<int64_t>(ceil_div(R, 1024), 256))), dim3(1024), 0, ctx().stream, c);
     if (int rc = launched("k_readout_coef")) return rc;
     if (a->grad_weight)
-        if (int rc = copy_rows(a->hidden, R, d, a->ldh, s.at<uint8_t>(o_hs), kp * 2, c.coef, up, top, two)) return rc;
+        if (int rc = copy_rows(a->hidden, R, d, a->ldh, s.at<uint8_t>(o_hs), kp * 2, c.coef, up, top)) return rc;
     PieceP p{};
     p.h = static_cast<const uint8_t *>(a->hidden);
     p.ldh = a->ldh * 2;
@@ -1066,6 +1155,7 @@ int backward(const NtRlReadoutStatsGradArgs *a) {
     p.tokens = a->tokens;
     p.coef = c.coef;
     p.g = s.at<uint8_t>(o_g);
+    p.left = c.left;
     for (int64_t v0 = 0; v0 < V; v0 += cols) {
         const int64_t n = std::min(cols, V - v0);
         if (int rc = piece_weight(a->weight, dv, wdirect, v0, n, d, a->ldw, s.at<uint8_t>(o_w), &p)) return rc;

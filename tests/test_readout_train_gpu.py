@@ -476,7 +476,7 @@ def test_large_sizes(rows, V, d, dtype, layout, mask):
         torch.set_default_device(device)
     for k in got:
         agree(values(got[k]).to("cuda"), want[k], tol[k], k)
-    if rows <= 64:  # G in two terms: the gradients are off by their own rounding and the sums'
+    if rows <= 512:  # the tokens' entries of G whole: the gradients are off by their own rounding and the other entries'
         u = HALF_STEP[dtype]
         for k in ("grad_hidden", "grad_weight"):
             off = (values(got[k]).to("cuda") - want[k]).norm() / want[k].norm()
