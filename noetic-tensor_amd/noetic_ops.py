@@ -383,7 +383,7 @@ def quantize_int8(x: Tensor, xl: Layout) -> Tuple[Tensor, Tensor]:
 def _quantized(q: Tensor, scale: Tensor, what: str):
     if q.dtype != "i8" or scale.dtype != "f32":
         raise TypeError(f"{what}: {q.dtype} values with {scale.dtype} scales (i8 and f32)")
-    if not q.shape or q.numel != scale.numel * q.shape[-1]:
+    if not q.shape or scale.numel != math.prod(q.shape[:-1]):  # (rows of no elements have their scales too)
         raise ValueError(f"{what}: {list(scale.shape)} scales for the rows of {list(q.shape)}")
 
 
@@ -408,9 +408,10 @@ def matmul_int8(a: Tensor, a_scale: Tensor, b: Tensor, b_scale: Tensor, dtype: s
     if len(b.shape) != 2 or a.shape[-1] != b.shape[1]:
         raise ValueError(f"matmul_int8 {list(a.shape)} × {list(b.shape)} (b [n, k], its rows as long as a's)")
     n, k = b.shape
+    m = math.prod(a.shape[:-1])
     y = Tensor(a.shape[:-1] + (n,), dtype)
     _check(_dev().nt_hip_matmul_int8(C.c_void_p(a.ptr), k, C.c_void_p(a_scale.ptr), C.c_void_p(b.ptr), k,
-                                     C.c_void_p(b_scale.ptr), a_scale.numel, n, k, _DT[dtype], C.c_void_p(y.ptr), n),
+                                     C.c_void_p(b_scale.ptr), m, n, k, _DT[dtype], C.c_void_p(y.ptr), n),
            "matmul_int8")
     return y
 

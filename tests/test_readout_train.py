@@ -128,6 +128,17 @@ def test_mirror_refusals():
         ops.matmul_int8(Fake((6, 16), "u8"), s, q, s)
 
 
+@pytest.mark.parametrize("rows,scales", [(2, 100), (100, 2), (0, 1), (1, 0)])
+def test_scales_of_rows_without_elements_are_counted(rows, scales):
+    """Rows of no elements have a scale each: another number of them is refused, on either side of the product."""
+    q, s = Fake((rows, 0), "i8"), Fake((scales,), "f32")
+    other, one = Fake((3, 0), "i8"), Fake((3,), "f32")
+    for call in (lambda: ops.dequantize_int8(q, s), lambda: ops.matmul_int8(q, s, other, one),
+                 lambda: ops.matmul_int8(other, one, q, s)):
+        with pytest.raises(ValueError, match="scales for the rows"):
+            call()
+
+
 def test_argument_struct_layouts_match_the_header(tmp_path):
     names = ("NtRlReadoutStatsArgs", "NtRlReadoutStatsGradArgs")
     lines = []
