@@ -659,7 +659,7 @@ constexpr int64_t kMaxK = 131071, kMaxLd = int64_t(1) << 22;
 
 int product(const int8_t *a, int64_t lda, const float *sa, const int8_t *b, int64_t ldb, const float *sb, int64_t m, int64_t n,
             int64_t k, int32_t dtype, void *out, int64_t ldo) {
-    const bool ad = aligned(a, k, lda), bd = aligned(b, k, ldb);
+    const bool ad = k == 0 || aligned(a, k, lda), bd = k == 0 || aligned(b, k, ldb);  // (no k: nothing is read)
     const int64_t kp = round_up(k, 16);
     const Plan s = plan(m, n, kp, true);
     const int64_t abytes = ad ? 0 : round_up(m * kp, 256), bbytes = bd ? 0 : round_up(n * kp, 256);

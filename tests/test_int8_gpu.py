@@ -225,6 +225,20 @@ def test_strides_and_leading_dimensions(dtype):
     agree(nr.Tensor((m, n), dtype, y.buf), product(a, sa, b, sb), dtype)
 
 
+@pytest.mark.parametrize("m", [1, 4, 5, 70, 300])
+def test_no_k_at_any_stride(m):
+    """k = 0: zeros, whatever the operands' addresses and strides."""
+    n = 300
+    sa, sb, out = given(torch.rand(m)), given(torch.rand(n)), given(torch.full((m, n), 5.0))
+    for lda, ldb, at in ((0, 0, 0), (5, 16, 0), (16, 7, 0), (3, 1, 1), (64, 64, 8)):
+        some = nr.Tensor((64,), "i8")
+        nr._check(nr.lib().nt_hip_matmul_int8(some.ptr + at, lda, sa.ptr, some.ptr + at, ldb, sb.ptr, m, n, 0, 0, out.ptr, n),
+                  "matmul_int8")
+        assert (out.to_numpy() == 0).all()
+        nr._check(nr.lib().nt_hip_matmul_int8(None, lda, sa.ptr, None, ldb, sb.ptr, m, n, 0, 0, out.ptr, n), "matmul_int8")
+        assert (out.to_numpy() == 0).all()
+
+
 def test_captured_calls_replay():
     m, n, k = 33, 500, 100
     g = torch.Generator().manual_seed(9)
