@@ -3,15 +3,17 @@
 //
 // The reference multiplies (the decoder's head, src/nn/decoder.rs:272,286; linear.rs:1-3), keeps [rows, V]
 // logits, and differentiates log_softmax, gather and categorical_entropy on them (activation.rs:30-42,
-// rl.rs:134-141, 405-414). Here, with z = x / T + mask and y = z log2 e:
+// rl.rs:134-141, 405-414). Here, with z = x / T + mask:
 //
 //  Forward: k_readout_stats computes a tile of x on the matrix cores (nt_tile.hpp) and reduces it where it
-//  stands: per row and block of columns the reference ref = max y, sum 2^(y - ref) and, for the entropy,
-//  sum 2^(y - ref) (y - ref) (f32: at most 128 terms). k_readout_merge joins a row's blocks in f64:
+//  stands: per row and block of columns the reference, the largest value (x, or z in f32 where an additive mask makes
+//  it), and the sums of w = 2^d and, for the entropy, w d over the differences d from it in units of ln 2 (f32: at
+//  most 128 terms). Differences first, products after: logits of any size, or a bias of -1e9 in every column, lose no
+//  more than their own f32 rounding. k_readout_merge joins a row's blocks in f64:
 //    lse = ln sum e^z, logp = z[token] - lse, entropy = lse - sum p z.
 //
-//  Backward: p = 2^(y - lse log2 e) comes from the logits computed once more, piece by piece of the
-//  vocabulary, so that
+//  Backward: p = e^(z - base - rest), of the forward's two parts of the log-sum-exp, the difference from the base taken
+//  first, comes from the logits computed once more, piece by piece of the vocabulary, so that
 //    G = dL/dx = (g_logp (onehot - p) - g_entropy p (ln p + entropy)) / T
 //  is held for one piece at a time, in the operands' 16-bit type: three products per piece, x = H W,
 //  dW = G^T H (the piece's rows of it, whole) and dH += G W^T (f32 sums over the pieces). 8 rows V dim
@@ -121,9 +123,8 @@ struct MaskBlock {
             }
         }
     }
-    // x under it: -inf where excluded; under an additive mask x c + mask log2 e, else x itself (y = x c follows in
-    // the sum's fma)
-    static __device__ __forceinline__ void out(const uint8_t *lds, const MaskP &m, float c, int lane, float (&x)[4 * TN][4]) {
+    // x's values under it: -inf where a keep-mask excludes; z = x / T + mask in f32 under an additive one (`invt`: 1 / T)
+    static __device__ __forceinline__ void out(const uint8_t *lds, const MaskP &m, float invt, int lane, float (&x)[4 * TN][4]) {
         const int r = m.ld == 0 ? 0 : lane % 32, h = lane / 32;
         if (m.u8) {
 #pragma unroll
@@ -138,7 +139,7 @@ struct MaskBlock {
                 float f[4];
                 __builtin_memcpy(f, lds + r * kF32 + 32 * q + 16 * h, 16);
 #pragma unroll
-                for (int e = 0; e < 4; e++) x[q][e] = fmaf(f[e], kLog2e, x[q][e] * c);
+                for (int e = 0; e < 4; e++) x[q][e] = x[q][e] * invt + f[e];
             }
         }
     }
@@ -164,15 +165,15 @@ struct PieceP {
     int n;
     int64_t v0;
     uint32_t tm, tn;
-    float c;           // log2(e) / T
+    float c, invt;     // log2(e) / T (under an additive mask log2(e)), 1 / T
     MaskP mask;
     const int32_t *tokens;
     // forward
-    float *ref, *sum, *esum;  // [block][rows_p]
+    float *ref, *sum, *esum;  // [block][rows_p]: the largest value, the sums relative to it
     int64_t rows_p, block0;   // rows padded for those, the piece's first block
     float *xtok;              // [rows] the token's raw logit
     // backward
-    const float4 *coef;       // [rows] {lse log2 e (+inf: nothing flows), a, b, the token's term}
+    const float4 *coef;       // [rows] {the largest value (+inf: nothing flows), a, b, the token's term}
     uint8_t *g;               // [rows, ldg bytes], of which gbytes are written: zeros past n
     int64_t ldg, gbytes;
     float *left;              // [rows] what the rounding of G's entry at the row's token left, or null
@@ -198,7 +199,6 @@ __global__ __launch_bounds__(S::kThreads, 1) void k_readout_stats(PieceP p) {
           weight_rows<T, BTR>(p, in), p.kbytes, wave, lane);
     const int wm = wave / WN, wn = wave % WN;
     const int col0 = in * T::BN + 32 * TN * wn + 4 * (lane / 32);
-    const float c = MASK && p.mask.f32 ? 1.0f : p.c;  // y = x c under the mask
     static_assert(MaskBlock<TN>::kLds * WM * WN <= T::kLds, "the mask's blocks fit");
     uint8_t *const mlds = lds + wave * MaskBlock<TN>::kLds;
     const int64_t block = p.block0 + int64_t(in) * WN + wn;
@@ -228,7 +228,7 @@ __global__ __launch_bounds__(S::kThreads, 1) void k_readout_stats(PieceP p) {
             const int64_t row0 = row - lane % 32;
             if (row0 < p.rows)
                 MaskBlock<TN>::in(mlds, p.mask, row0, p.rows - row0 < 32 ? int(p.rows - row0) : 32, in * T::BN + 32 * TN * wn, p.n, lane, i == 0);
-            MaskBlock<TN>::out(mlds, p.mask, p.c, lane, x);
+            MaskBlock<TN>::out(mlds, p.mask, p.invt, lane, x);
         } else if (in * T::BN + T::BN > p.n) {
             ended(x, p.n - col0);
         }
@@ -237,14 +237,14 @@ __global__ __launch_bounds__(S::kThreads, 1) void k_readout_stats(PieceP p) {
         for (int q = 0; q < 4 * TN; q++)
 #pragma unroll
             for (int e = 0; e < 4; e++) m = fmaxf(m, x[q][e]);
-        m = fmaxf(m, __shfl_xor(m, 32, 64)) * c;
+        m = fmaxf(m, __shfl_xor(m, 32, 64));
         const float ref = m == -INFINITY ? 0.0f : m;
         float s = 0.0f, es = 0.0f;
 #pragma unroll
         for (int q = 0; q < 4 * TN; q++)
 #pragma unroll
             for (int e = 0; e < 4; e++) {
-                const float d = fmaf(x[q][e], c, -ref), w = __builtin_amdgcn_exp2f(d);
+                const float d = (x[q][e] - ref) * p.c, w = __builtin_amdgcn_exp2f(d);
                 s += w;
                 if constexpr (ENT) es += w > 0.0f ? w * d : 0.0f;
             }
@@ -267,6 +267,7 @@ struct MergeP {
     const int32_t *tokens;
     MaskP mask;
     double tau;
+    float c, invt;
     float *logp, *entropy, *base, *rest;
     uint8_t *status;
 };
@@ -297,8 +298,9 @@ __global__ __launch_bounds__(1024) void k_readout_merge(MergeP p) {
         for (int k = 0; k < kBatch; k++) top = fmaxf(top, r[k]);
         const float base = top == -INFINITY ? 0.0f : top;
         if (m > -INFINITY) {
-            const double d = double(m) - double(base), f = double(__builtin_amdgcn_exp2f(float(d)));
-            t = f * (t + d * s);
+            const float d = (m - base) * p.c;
+            const double f = double(__builtin_amdgcn_exp2f(d));
+            t = f * (t + double(d) * s);
             s *= f;
         }
         m = top;
@@ -306,7 +308,7 @@ __global__ __launch_bounds__(1024) void k_readout_merge(MergeP p) {
         for (int k = 0; k < kBatch; k++) {
             // (a block with nothing allowed has ref -inf and sum 0; with NaNs alone, sum NaN)
             if (r[k] == -INFINITY && q[k] == 0.0f) continue;
-            const float d = r[k] - base;
+            const float d = (r[k] - base) * p.c;
             const double f = r[k] == -INFINITY ? 1.0 : double(__builtin_amdgcn_exp2f(d));
             s += f * double(q[k]);
             t += f * (double(e[k]) + double(d) * double(q[k]));
@@ -325,27 +327,29 @@ __global__ __launch_bounds__(1024) void k_readout_merge(MergeP p) {
             s += q;  // 0, or NaN
             continue;
         }
-        const float d = sm[k][lr] - m;
+        const float d = (sm[k][lr] - m) * p.c;
         const double f = double(__builtin_amdgcn_exp2f(d));
         s += f * q;
         t += f * (st[k][lr] + double(d) * q);
     }
     const int64_t tok = p.tokens[row];
     const bool bad = tok < 0 || tok >= p.vocab;
-    const bool none = m == -INFINITY && s == 0.0;
-    const bool ok = !none && s > 0.0 && s < INFINITY && m < INFINITY;
+    // The largest z and, relative to it, the log of the sum: apart, since under a large bias in every column (a mask of
+    // the type's lowest value) the sum's last bits are not the logits'.
+    const double zmax = p.mask.f32 ? double(m) : double(m) / p.tau, lns = kLn2 * log2(s);
+    const float base = float(zmax);
+    const bool none = base == -INFINITY && s == s;  // (or every value below what z holds)
+    const bool ok = !none && s > 0.0 && s < INFINITY && base < INFINITY;
     uint8_t status = ok ? NT_ROW_OK : (none ? NT_ROW_NO_TOKEN : NT_ROW_NAN);
-    const double lse2 = double(m) + log2(s), lse = lse2 * kLn2;
-    float base = float(double(m) * kLn2);
     if (p.base) p.base[row] = ok ? base : (none ? -INFINITY : NAN);
-    if (p.rest) p.rest[row] = ok ? float(lse - double(base)) : (none ? 0.0f : NAN);
-    if (p.entropy) p.entropy[row] = ok ? float(kLn2 * (log2(s) - t / s)) : NAN;
+    if (p.rest) p.rest[row] = ok ? float((zmax - double(base)) + lns) : (none ? 0.0f : NAN);
+    if (p.entropy) p.entropy[row] = ok ? float(lns - kLn2 * t / s) : NAN;
     float lp = NAN;
     if (ok && !bad) {
         double z = double(p.xtok[row]) / p.tau;
         if (p.mask.u8 && !p.mask.u8[row * p.mask.ld + tok]) z = -INFINITY;
-        else if (p.mask.f32) z += double(p.mask.f32[row * p.mask.ld + tok]);
-        lp = float(z - lse);
+        else if (p.mask.f32) z = double(p.xtok[row] * p.invt + p.mask.f32[row * p.mask.ld + tok]);  // (as its column's value)
+        lp = float((z - zmax) - lns);
     }
     p.logp[row] = lp;
     if (ok && bad) status = NT_ROW_BAD_TOKEN;
@@ -359,14 +363,15 @@ struct CoefP {
     const int32_t *tokens;
     int64_t rows, vocab;
     double tau;
-    int f16;
+    int f32mask, f16;
     float4 *coef;
     float *left;   // [rows] zeros here, or null
     float *up;     // [rows] f16: what a row of G was divided by
     float *top;    // [1] f16: the largest of them
 };
 
-// What a row's upstream gradients make of it (f16: one workgroup, the largest row's scale is a maximum over all).
+// What a row's upstream gradients make of it: with l = (value - largest) c, so that p = 2^l q, q = e^-rest, and ln p =
+// l ln 2 - rest, G = 2^l (a + b l) + the token's term (f16: one workgroup, the largest row's scale is a maximum over all).
 __global__ __launch_bounds__(1024) void k_readout_coef(CoefP p) {
     __shared__ float s_top[16];
     float top = 0.0f;
@@ -376,8 +381,10 @@ __global__ __launch_bounds__(1024) void k_readout_coef(CoefP p) {
         if (tok < 0 || tok >= p.vocab) gl = 0.0;
         const double ge = p.g_entropy ? double(p.g_entropy[r]) : 0.0;
         const double h = p.g_entropy ? double(p.entropy[r]) : 0.0;
-        const double lse = double(p.base[r]) + double(p.rest[r]);
-        const bool dead = (gl == 0.0 && ge == 0.0) || lse == -INFINITY;
+        // the largest value as the columns have it: z's (an additive mask), or x's, whose rounding goes to the rest
+        const float base = p.base[r], top_x = p.f32mask ? base : float(double(base) * p.tau);
+        const double rest = double(p.rest[r]) + (p.f32mask ? 0.0 : double(base) - double(top_x) / p.tau), q = exp(-rest);
+        const bool dead = (gl == 0.0 && ge == 0.0) || base == -INFINITY;
         double unit = 1.0;  // f16: G's unit, a power of two
         float up = 0.0f;
         if (p.f16 && !dead) {
@@ -395,8 +402,8 @@ __global__ __launch_bounds__(1024) void k_readout_coef(CoefP p) {
         }
         if (p.f16) p.up[r] = up;
         if (p.left) p.left[r] = 0.0f;
-        const float a = float(-(gl + ge * h) * unit), b = float(-ge * kLn2 * unit);
-        p.coef[r] = dead ? float4{INFINITY, 0.0f, 0.0f, 0.0f} : float4{float(lse * kLog2eD), a, b, float(gl * unit)};
+        const float a = float(-(gl + ge * (h - rest)) * q * unit), b = float(-ge * kLn2 * q * unit);
+        p.coef[r] = dead ? float4{INFINITY, 0.0f, 0.0f, 0.0f} : float4{top_x, a, b, float(gl * unit)};
     }
     if (!p.f16) return;
 #pragma unroll
@@ -459,7 +466,6 @@ __global__ __launch_bounds__(S::kThreads, 1) void k_readout_g(PieceP p) {
           weight_rows<T, BTR>(p, in), p.kbytes, wave, lane);
     const int wm = wave / WN, wn = wave % WN;
     const int col0 = in * T::BN + 32 * TN * wn + 4 * (lane / 32);
-    const float c = MASK && p.mask.f32 ? 1.0f : p.c;
     const int64_t bytes = p.gbytes - (in * T::BN + 32 * TN * wn) * 2;
     // (a mask's 32 rows are read before G's block is written over them; a row that all share stays in front of it)
     constexpr int kShared = MASK ? MaskBlock<TN>::kShared : 0, kMask = MASK ? MaskBlock<TN>::kLds : 0;
@@ -492,7 +498,7 @@ __global__ __launch_bounds__(S::kThreads, 1) void k_readout_g(PieceP p) {
             for (int e = 0; e < 4; e++) x[q][e] = t.acc[i][q / 4][4 * (q % 4) + e];
         if constexpr (MASK) {
             MaskBlock<TN>::in(mlds, p.mask, row0, p.rows - row0 < 32 ? int(p.rows - row0) : 32, in * T::BN + 32 * TN * wn, p.n, lane, i == 0);
-            MaskBlock<TN>::out(mlds, p.mask, p.c, lane, x);
+            MaskBlock<TN>::out(mlds, p.mask, p.invt, lane, x);
         } else if (in * T::BN + T::BN > p.n) {
             ended(x, p.n - col0);
         }
@@ -501,8 +507,8 @@ __global__ __launch_bounds__(S::kThreads, 1) void k_readout_g(PieceP p) {
             float g[4];
 #pragma unroll
             for (int e = 0; e < 4; e++) {
-                const float lp = fmaf(x[q][e], c, -k.x), pr = __builtin_amdgcn_exp2f(lp);  // log2 p, p
-                g[e] = pr * fmaf(k.z, fmaxf(lp, -200.0f), k.y);  // (p 0: 0, and a NaN stays in p)
+                const float l = (x[q][e] - k.x) * p.c, w = __builtin_amdgcn_exp2f(l);
+                g[e] = w * fmaf(k.z, fmaxf(l, -200.0f), k.y);  // (p 0: 0, and a NaN stays in w)
             }
             if (mine)
 #pragma unroll
@@ -939,7 +945,8 @@ int forward(const NtRlReadoutStatsArgs *a) {
     p.rows = R;
     p.dim = d;
     p.kbytes = kp * 2;
-    p.c = float(kLog2eD / a->temperature);
+    p.c = a->mask_kind == NT_MASK_F32 ? kLog2e : float(kLog2eD / a->temperature);
+    p.invt = float(1.0 / a->temperature);
     p.tokens = a->tokens;
     p.ref = s.at<float>(o_ref);
     p.sum = s.at<float>(o_sum);
@@ -970,6 +977,8 @@ int forward(const NtRlReadoutStatsArgs *a) {
     q.tokens = a->tokens;
     q.mask = mask_at(a->mask_kind, a->mask, a->mask_ld, 0);
     q.tau = a->temperature;
+    q.c = p.c;
+    q.invt = p.invt;
     q.logp = a->logp;
     q.entropy = a->entropy;
     q.base = a->lse_base;
@@ -1131,6 +1140,7 @@ int backward(const NtRlReadoutStatsGradArgs *a) {
     c.rows = R;
     c.vocab = V;
     c.tau = a->temperature;
+    c.f32mask = a->mask_kind == NT_MASK_F32;
     c.f16 = f16;
     c.coef = s.at<float4>(o_coef);
     c.left = kept ? s.at<float>(o_left) : nullptr;
@@ -1151,7 +1161,8 @@ int backward(const NtRlReadoutStatsGradArgs *a) {
     p.rows = R;
     p.dim = d;
     p.kbytes = kp * 2;
-    p.c = float(kLog2eD / a->temperature);
+    p.c = a->mask_kind == NT_MASK_F32 ? kLog2e : float(kLog2eD / a->temperature);
+    p.invt = float(1.0 / a->temperature);
     p.tokens = a->tokens;
     p.coef = c.coef;
     p.g = s.at<uint8_t>(o_g);

@@ -548,3 +548,59 @@ def test_offsets_past_32_bits():
     u = HALF_STEP["bf16"]
     # (dp under 2^-12; each piece's sum of 40000 f32 terms)
     assert ((gw.cuda()[cols] - want).abs() <= (u + 2.0 ** -12 + R * 2.0 ** -24) * size + u * want.abs()).all()
+
+
+# ----------------------------------------------------------------------------- far from zero
+
+def exact_case(rows, V, d, dtype, layout, mask, tau, grid, seed=0):
+    """A case whose logits are exact in f32 in any order of their sums: integers times multiples of `grid`, all held in
+    the operands' type, and a temperature that is a power of two."""
+    c = Case(rows, V, d, dtype, layout, mask, tau=tau, seed=seed)
+    g = torch.Generator().manual_seed(seed + rows + V)
+    c.h = torch.randint(-3, 4, (rows, d), generator=g).to(TORCH[dtype])
+    w = (torch.randint(-250, 251, (V, d), generator=g).double() * grid).to(TORCH[dtype])
+    c.w = w if layout == "vd" else w.t().contiguous()
+    return c
+
+
+def logits64(c):
+    return c.h.double() @ (c.w.double().t() if c.layout == "vd" else c.w.double())
+
+
+@pytest.mark.parametrize("bias", [-1e4, -65504.0, -1e9, torch.finfo(torch.float32).min, 1e9])
+@pytest.mark.parametrize("rows,V,d,dtype,layout,kind", [(70, 1000, 8, "bf16", "dv", "f32"), (5, 640, 16, "f16", "vd", "f32_shared"),
+                                                        (300, 33000, 24, "bf16", "vd", "f32_shared"),
+                                                        (600, 5001, 8, "bf16", "dv", "bf16_bias")])
+def test_a_large_bias_in_every_column(rows, V, d, dtype, layout, kind, bias):
+    """tempered_logits' own f32 values, x / T + mask rounded once (the quotient is exact here), and the softmax of those:
+    the same but for the base when the row's largest is taken off them."""
+    c = exact_case(rows, V, d, dtype, layout, kind, 2.0, 2.0 ** -9)
+    c.mask = torch.full_like(c.mask, max(bias, torch.finfo(c.mask.dtype).min))
+    z = (logits64(c) / c.tau).float() + c.mask.float()  # f32
+    assert z.isfinite().all()
+    top = z.amax(1, keepdim=True)
+    c.add = (z - top).double() - logits64(c) / c.tau
+    got, (want, tol) = c.run(), c.want()
+    assert torch.equal(values(got["base"]), top[:, 0].double())
+    for k in ("logp", "rest", "entropy", "grad_hidden", "grad_weight"):
+        agree(values(got[k]), want[k], tol[k], k)
+
+
+@pytest.mark.parametrize("rows,V,d,dtype,layout,kind", [(70, 1000, 8, "bf16", "dv", "none"), (5, 640, 16, "f16", "vd", "u8"),
+                                                        (520, 5000, 8, "bf16", "vd", "u8_shared"), (40, 901, 12, "bf16", "vd", "f32")])
+def test_a_large_logit_in_every_column(rows, V, d, dtype, layout, kind):
+    """2^17 added to every logit by a column of H and a row of W: the scores and the gradients of all other columns as
+    without them."""
+    c = exact_case(rows, V, d, dtype, layout, kind, 1.0, 2.0 ** -6)
+    want, tol = c.want()
+    one = torch.full((rows, 1), 256.0, dtype=c.h.dtype)
+    row = torch.full((V, 1), 512.0, dtype=c.h.dtype)
+    far = exact_case(rows, V, d, dtype, layout, kind, 1.0, 2.0 ** -6)
+    far.h = torch.cat([one, c.h], 1)
+    far.w = torch.cat([row, c.w], 1) if layout == "vd" else torch.cat([row.t(), c.w], 0)
+    got = {k: values(v) for k, v in far.run().items()}
+    assert torch.equal(got["base"], want["base"] + 2.0 ** 17)
+    got["grad_hidden"] = got["grad_hidden"][:, 1:]
+    got["grad_weight"] = got["grad_weight"][:, 1:] if layout == "vd" else got["grad_weight"][1:]
+    for k in ("logp", "rest", "entropy", "grad_hidden", "grad_weight"):
+        agree(got[k], want[k], tol[k], k)
