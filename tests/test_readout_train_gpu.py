@@ -604,3 +604,34 @@ def test_a_large_logit_in_every_column(rows, V, d, dtype, layout, kind):
     got["grad_weight"] = got["grad_weight"][:, 1:] if layout == "vd" else got["grad_weight"][1:]
     for k in ("logp", "rest", "entropy", "grad_hidden", "grad_weight"):
         agree(got[k], want[k], tol[k], k)
+
+
+@pytest.mark.parametrize("kind", ["none", "u8", "f32", "f32_shared"])
+@pytest.mark.parametrize("layout", ["dv", "vd"])
+@pytest.mark.parametrize("rows,V,d", [(75, 328, 40), (300, 1288, 72), (40, 264, 33)])
+def test_row_padding_that_is_not_a_number(rows, V, d, layout, kind):
+    """Aligned operands read in place, NaN behind the last value of each row: none of it reaches an output."""
+    c = Case(rows, V, d, "bf16", layout, kind, tau=0.8)
+
+    def padded(x):
+        b = torch.full((x.shape[0], x.shape[1] + 8), math.nan, dtype=x.dtype)
+        b[:, :x.shape[1]] = x
+        return given(b), x.shape[1] + 8
+
+    (h, ldh), (w, ldw) = padded(c.h), padded(c.w)
+    m = None if c.mask is None else padded(c.mask) if c.mask.dtype == torch.float32 else (given(c.mask), V)
+    kinds = {"n": nr.NT_MASK_NONE, "u": nr.NT_MASK_U8, "f": nr.NT_MASK_F32}
+    t, gl, ge = given(c.tokens), given(c.g_logp), given(c.g_entropy)
+    rowf = lambda: nr.Tensor((c.rows,), "f32")  # noqa: E731
+    lp, ent, base, rest, st = rowf(), rowf(), rowf(), rowf(), nr.Tensor((c.rows,), "u8")
+    lay = nr.NT_READOUT_W_DV if layout == "dv" else nr.NT_READOUT_W_VD
+    head = (h.ptr, w.ptr, nr.NT_BF16, lay, c.rows, c.V, c.d, ldh, ldw, m[0].ptr if m else None,
+            m[1] if m and c.mask.shape[0] > 1 else 0, kinds[kind[0]], 0, c.tau, t.ptr)
+    a = nr.NtRlReadoutStatsArgs(*head, lp.ptr, ent.ptr, base.ptr, rest.ptr, st.ptr)
+    nr._check(nr.lib().nt_hip_rl_readout_score_stats(C.byref(a)), "stats")
+    gh, gw = nr.Tensor(tuple(c.h.shape), "bf16"), nr.Tensor(tuple(c.w.shape), "bf16")
+    b = nr.NtRlReadoutStatsGradArgs(*head, base.ptr, rest.ptr, ent.ptr, gl.ptr, ge.ptr, gh.ptr, gw.ptr, c.d, c.w.shape[1])
+    nr._check(nr.lib().nt_hip_rl_readout_score_backward(C.byref(b)), "backward")
+    want, tol = c.want()
+    for k, v in (("logp", lp), ("entropy", ent), ("base", base), ("rest", rest), ("grad_hidden", gh), ("grad_weight", gw)):
+        agree(values(v), want[k], tol[k], k)
