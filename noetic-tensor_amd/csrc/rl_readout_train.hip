@@ -25,7 +25,9 @@
 //  token's row of W and the row of H (128 x 1024 x 32000 bf16: the error is 0.0017 of the norm, which is the written
 //  values' own, instead of 0.0022, for 112 us instead of 104). For f16, whose range G would leave, a row of G is
 //  held in units of 2^(e - 14), 2^e over |g_logp| + 16 |g_entropy| (p |ln p + entropy| is under 14 for a
-//  vocabulary of 2^20), its share of dW being scaled through the row of H by a power of two.
+//  vocabulary of 2^20), and for dW the row of H is scaled by 2^e and the one power of two that puts the largest value of
+//  all scaled rows under 2^15: what rows far below the largest lose to f16's smallest steps is 2^-40 of that
+//  value, less than the smallest step of a gradient that holds the largest row's.
 //
 //  Bound by the matrix cores for many rows, and those by power: 4096 x 4096 x 128256 bf16 is scored in 3.2-3.3 ms (1.33
 //  PFLOP/s at a clock near 1.5 GHz; a library product alone 2.99) and scored and differentiated in 13.4 ms (1.29 at its 8
@@ -366,15 +368,16 @@ struct CoefP {
     int f32mask, f16;
     float4 *coef;
     float *left;   // [rows] zeros here, or null
-    float *up;     // [rows] f16: what a row of G was divided by
-    float *top;    // [1] f16: the largest of them
+    float *up;     // [rows] f16: 2^e, what a row of G was divided by (0: nothing flows)
+    int *top;      // [1] f16: cleared here, for k_readout_top
 };
 
+constexpr int kNoTop = -(1 << 30);
+
 // What a row's upstream gradients make of it: with l = (value - largest) c, so that p = 2^l q, q = e^-rest, and ln p =
-// l ln 2 - rest, G = 2^l (a + b l) + the token's term (f16: one workgroup, the largest row's scale is a maximum over all).
+// l ln 2 - rest, G = 2^l (a + b l) + the token's term.
 __global__ __launch_bounds__(1024) void k_readout_coef(CoefP p) {
-    __shared__ float s_top[16];
-    float top = 0.0f;
+    if (p.f16 && blockIdx.x == 0 && threadIdx.x == 0) *p.top = kNoTop;
     for (int64_t r = blockIdx.x * int64_t(1024) + threadIdx.x; r < p.rows; r += int64_t(gridDim.x) * 1024) {
         const int64_t tok = p.tokens[r];
         double gl = p.g_logp ? double(p.g_logp[r]) : 0.0;
@@ -392,11 +395,10 @@ __global__ __launch_bounds__(1024) void k_readout_coef(CoefP p) {
             int e = 0;
             if (size > 0.0 && size < INFINITY) {
                 (void)frexp(size, &e);  // size < 2^e
-                e = e < -126 ? -126 : (e > 127 ? 127 : e);
+                e = e < -126 ? -126 : (e > 126 ? 126 : e);
             }
             up = ldexpf(1.0f, e);
             unit = ldexp(1.0, 14 - e);
-            top = fmaxf(top, up);
         } else if (!p.f16) {
             unit = 1.0 / p.tau;
         }
@@ -405,23 +407,51 @@ __global__ __launch_bounds__(1024) void k_readout_coef(CoefP p) {
         const float a = float(-(gl + ge * (h - rest)) * q * unit), b = float(-ge * kLn2 * q * unit);
         p.coef[r] = dead ? float4{INFINITY, 0.0f, 0.0f, 0.0f} : float4{top_x, a, b, float(gl * unit)};
     }
-    if (!p.f16) return;
+}
+
+// Of a normal power of two.
+__device__ __forceinline__ int exponent(float p) { return int(__builtin_bit_cast(uint32_t, p) >> 23) - 127; }
+
+// f16: the exponent that the largest |h| 2^e of all rows is under, a wave a row. (A maximum of integers: the same in any
+// order. Infinities and NaNs do not count.)
+__global__ __launch_bounds__(256) void k_readout_top(const uint16_t *h, int64_t rows, int64_t cols, int64_t ld, const float *up,
+                                                     int *top) {
+    const int lane = threadIdx.x % 64;
+    const int64_t row = blockIdx.x * int64_t(4) + threadIdx.x / 64;
+    if (row >= rows || up[row] == 0.0f) return;
+    uint32_t most = 0;  // (magnitudes order as their bits do)
+    auto see = [&](uint32_t b) {
+        b &= 0x7fffu;
+        if (b < 0x7c00u && b > most) most = b;
+    };
+    const uint16_t *s = h + row * ld;
+    for (int64_t c = lane * 8; c < cols; c += 512) {
+        if (c + 8 <= cols) {
+            const u32x4 v = *reinterpret_cast<const u32x4u *>(s + c);
 #pragma unroll
-    for (int d = 32; d; d /= 2) top = fmaxf(top, __shfl_xor(top, d, 64));
-    if (threadIdx.x % 64 == 0) s_top[threadIdx.x / 64] = top;
-    __syncthreads();
-    if (threadIdx.x == 0) {
-        for (int k = 1; k < 16; k++) top = fmaxf(top, s_top[k]);
-        *p.top = top == 0.0f ? 1.0f : top;
+            for (int e = 0; e < 4; e++) see(v[e]), see(v[e] >> 16);
+        } else {
+            for (int e = 0; c + e < cols; e++) see(s[c + e]);
+        }
+    }
+#pragma unroll
+    for (int d = 32; d; d /= 2) most = max(most, uint32_t(__shfl_xor(int(most), d, 64)));
+    if (lane == 0 && most > 0) {
+        int e;  // |h| < 2^e
+        (void)frexpf(float(__builtin_bit_cast(_Float16, uint16_t(most))), &e);
+        atomicMax(top, e + exponent(up[row]));
     }
 }
 
+// What f16 rows of H are scaled by besides their own 2^e, and its inverse for dW.
+__device__ __forceinline__ int lift(const int *top) { return 15 - (*top == kNoTop ? 0 : *top); }
+
 // Rows of 16-bit values into rows of `ldo` bytes, zeros from `cols` to their end: an operand that is not laid
 // out as the copies need it. With `coef`, the rows that nothing flows through are zeros (whatever they hold, a
-// NaN too, stays out of dW) and with `up`, f16 rows are scaled by up / top, a power of two.
+// NaN too, stays out of dW) and with `up`, f16 rows are scaled by up 2^lift, a power of two.
 __global__ __launch_bounds__(256) void k_readout_rows(const uint16_t *src, int64_t rows, int64_t cols, int64_t ld,
                                                       uint8_t *out, int64_t ldo, const float4 *coef, const float *up,
-                                                      const float *top) {
+                                                      const int *top) {
     const int64_t per = ldo / 16, total = rows * per;
     for (int64_t i = blockIdx.x * int64_t(256) + threadIdx.x; i < total; i += int64_t(gridDim.x) * 256) {
         const int64_t r = i / per, c = (i - r * per) * 8;
@@ -437,9 +467,9 @@ __global__ __launch_bounds__(256) void k_readout_rows(const uint16_t *src, int64
             else
                 for (int e = 0; e < 8; e++) x.h[e] = c + e < cols ? s[e] : uint16_t(0);
             if (up) {
-                const float f = up[r] / *top;
+                const int l = exponent(up[r]) + lift(top);  // (f32 need not hold 2^l)
 #pragma unroll
-                for (int e = 0; e < 8; e++) x.f[e] = _Float16(float(x.f[e]) * f);
+                for (int e = 0; e < 8; e++) x.f[e] = _Float16(ldexpf(float(x.f[e]), l));
             }
         }
         *reinterpret_cast<u32x4 *>(out + r * ldo + c * 2) = x.v;
@@ -539,7 +569,7 @@ struct GradP {
     float *slab;              // [splits][m][n] f32
     int add;
     const float *row_scale;   // f16: [m] or null
-    const float *scale;       // f16: [1] or null
+    const int *top;           // f16: [1] or null
     float fixed;
     // dW: what the rounding of G left of the tokens' entries (null: dH)
     const float *left;        // [k]
@@ -632,7 +662,7 @@ __global__ __launch_bounds__(S::kThreads, S::TM == 1 ? 2 : 1) void k_readout_gra
             else add_left<E, false>(t.acc[0], p, mine, lefts, p.v0 + row0, p.b, p.ldb, p.wb, row0, c0, lane);
         }
     }
-    const float whole = p.scale ? *p.scale * p.fixed : p.fixed;
+    const float whole = p.top ? ldexpf(p.fixed, -lift(p.top)) : p.fixed;
     const int64_t col0 = n0 + 32 * TN * wn;
     if (col0 >= p.n) return;
     float f[TM];
@@ -696,7 +726,7 @@ struct LeftP {
 
 template <class E>
 __global__ __launch_bounds__(256) void k_readout_fold(const float *slab, int splits, int64_t m, int64_t n, LeftP p, uint16_t *out,
-                                                      int64_t ldo, const float *row_scale, const float *scale, float fixed) {
+                                                      int64_t ldo, const float *row_scale, const int *top, float fixed) {
     const int64_t per = (n + 3) / 4, total = m * per;
     for (int64_t i = blockIdx.x * int64_t(256) + threadIdx.x; i < total; i += int64_t(gridDim.x) * 256) {
         const int64_t r = i / per, c = (i - r * per) * 4;
@@ -721,7 +751,7 @@ __global__ __launch_bounds__(256) void k_readout_fold(const float *slab, int spl
             }
         for (; z < splits; z++)
             for (int e = 0; e < have; e++) x[e] += at(z)[e];
-        float f = scale ? *scale * fixed : fixed;
+        float f = top ? ldexpf(fixed, -lift(top)) : fixed;
         if (row_scale) f *= row_scale[r];
         uint16_t *o = out + r * ldo + c;
         const uint32_t w[2] = {pair16<E>(x[0] * f, x[1] * f), pair16<E>(x[2] * f, x[3] * f)};
@@ -810,7 +840,7 @@ bool aligned(const void *p, int64_t cols, int64_t ld) {
 }
 
 int copy_rows(const void *src, int64_t rows, int64_t cols, int64_t ld, uint8_t *out, int64_t ldo, const float4 *coef,
-              const float *up, const float *top) {
+              const float *up, const int *top) {
     const int64_t n = rows * (ldo / 16);
     hipLaunchKernelGGL(k_readout_rows, dim3(unsigned(std::min<int64_t>(ceil_div(n, 256), 8192))), dim3(256), 0,
                        ctx().stream, static_cast<const uint16_t *>(src), rows, cols, ld, out, ldo, coef, up, top);
@@ -991,7 +1021,7 @@ template <class E>
 int fold(const GradP &p, int64_t splits, uint16_t *out, const LeftP &left = {}) {
     const int64_t n = p.m * ceil_div(p.n, 4);
     hipLaunchKernelGGL(k_readout_fold<E>, dim3(unsigned(std::min<int64_t>(ceil_div(n, 256), 8192))), dim3(256), 0,
-                       ctx().stream, p.slab, int(splits), p.m, p.n, left, out, p.ldo, p.row_scale, p.scale, p.fixed);
+                       ctx().stream, p.slab, int(splits), p.m, p.n, left, out, p.ldo, p.row_scale, p.top, p.fixed);
     return launched("k_readout_fold");
 }
 
@@ -1022,7 +1052,8 @@ struct BackP {
     const uint8_t *hs;  // the scaled hidden states, [rows, ldhs bytes]
     int64_t ldhs;
     float *slab_h, *slab_w;
-    const float *up, *top;
+    const float *up;
+    const int *top;
     float fixed;
     bool last;
 };
@@ -1049,7 +1080,7 @@ int piece(const BackP &b) {
         w.ldo = a->grad_weight_ld;
         w.out = b.sw.splits > 1 ? nullptr : out;
         w.slab = b.slab_w;
-        w.scale = b.top;
+        w.top = b.top;
         w.fixed = b.fixed;
         const int64_t c = b.sw.splits > 1 || p.left ? 0 : whole_rounds(DV ? w.m : w.n, DV ? w.n : w.m, w.k * 2);
         if (c) {  // whole rounds of the vocabulary's side, and its rest
@@ -1127,7 +1158,8 @@ int backward(const NtRlReadoutStatsGradArgs *a) {
     const int o_sh = s.add(a->grad_hidden && hslab ? sh.splits * R * d * 4 : 0);
     const int o_sw = s.add(a->grad_weight && sw.splits > 1 ? sw.splits * std::min(cols, V) * d * 4 : 0);
     if (int rc = s.allocate()) return rc;
-    const float *up = f16 ? s.at<float>(o_up) : nullptr, *top = f16 ? s.at<float>(o_top) : nullptr;
+    const float *up = f16 ? s.at<float>(o_up) : nullptr;
+    int *top = f16 ? s.at<int>(o_top) : nullptr;
     const float fixed = f16 ? float(ldexp(1.0, -14) / a->temperature) : 1.0f;
     CoefP c{};
     c.base = a->lse_base;
@@ -1144,9 +1176,14 @@ int backward(const NtRlReadoutStatsGradArgs *a) {
     c.coef = s.at<float4>(o_coef);
     c.left = kept ? s.at<float>(o_left) : nullptr;
     c.up = s.at<float>(o_up);
-    c.top = s.at<float>(o_top);
-    hipLaunchKernelGGL(k_readout_coef, dim3(f16 ? 1 : unsigned(std::min<int64_t>(ceil_div(R, 1024), 256))), dim3(1024), 0, ctx().stream, c);
+    c.top = top;
+    hipLaunchKernelGGL(k_readout_coef, dim3(unsigned(std::min<int64_t>(ceil_div(R, 1024), 256))), dim3(1024), 0, ctx().stream, c);
     if (int rc = launched("k_readout_coef")) return rc;
+    if (a->grad_weight && f16) {
+        hipLaunchKernelGGL(k_readout_top, dim3(unsigned(ceil_div(R, 4))), dim3(256), 0, ctx().stream,
+                           static_cast<const uint16_t *>(a->hidden), R, d, a->ldh, up, top);
+        if (int rc = launched("k_readout_top")) return rc;
+    }
     if (a->grad_weight)
         if (int rc = copy_rows(a->hidden, R, d, a->ldh, s.at<uint8_t>(o_hs), kp * 2, c.coef, up, top)) return rc;
     PieceP p{};

@@ -635,3 +635,37 @@ def test_row_padding_that_is_not_a_number(rows, V, d, layout, kind):
     want, tol = c.want()
     for k, v in (("logp", lp), ("entropy", ent), ("base", base), ("rest", rest), ("grad_hidden", gh), ("grad_weight", gw)):
         agree(values(v), want[k], tol[k], k)
+
+
+@pytest.mark.parametrize("layout", ["dv", "vd"])
+@pytest.mark.parametrize("rows,V,d,spread", [(64, 400, 32, 20), (33, 1001, 45, 30), (600, 3001, 40, 20), (300, 9000, 72, 24)])
+def test_f16_weight_gradients_of_rows_far_apart(rows, V, d, spread, layout):
+    """Upstream gradients over many powers of two: the weight's gradient keeps each row's own bits. Besides G's rounding
+    and its own, a value of H scaled next to the largest (2^15 at most, and over 2^14) is off by half a step of 2^-24
+    where that leaves no more: 2^-39 of the largest |h| 2^e, times the row's G in its units of 2^e."""
+    c = Case(rows, V, d, "f16", layout, entropy=False, scale=6.0)
+    g = torch.Generator().manual_seed(rows)
+    c.g_logp = (2.0 ** torch.linspace(-spread / 2, spread / 2, rows))[torch.randperm(rows, generator=g)].float()
+    if rows == 64:
+        c.h[5] *= 2.0 ** -8  # (a small row, and one past half of f16's range)
+        c.h[7] *= 2.0 ** 4
+    h = c.h.double()
+    z = logits64(c) / c.tau
+    dz = (d + 8) * 2.0 ** -24 * (h.abs() @ (c.w.double().abs().t() if layout == "vd" else c.w.double().abs())).amax(1, keepdim=True)
+    p = torch.softmax(z, 1)
+    gl = c.g_logp.double()[:, None]
+    G = -gl * p
+    G[torch.arange(rows), c.tokens.long()] += gl[:, 0]
+    up = 2.0 ** (torch.floor(torch.log2(gl.abs())) + 1)
+    u = HALF_STEP["f16"]
+    dG = (u + 2.0 ** -22) * G.abs() + (4 * dz + 2.0 ** -20) * gl.abs() * p + 2.0 ** -38 * up
+    want = h.t() @ G
+    tol = h.abs().t() @ dG + rows * 2.0 ** -24 * (h.abs().t() @ G.abs()) + u * want.abs() + 2.0 ** -25
+    tol = tol + 2.0 ** -39 * float((h.abs().amax(1, keepdim=True) * up).max()) * (G.abs() / up).sum(0)[None, :]
+    # (an f16 of 65520 or more, half a step past the largest, is infinite; none is too near to tell)
+    past = want.abs() - tol >= 65520.0
+    assert (past | (want.abs() + tol < 65520.0)).all()
+    want = torch.where(past, want.sign() * math.inf, want)
+    if layout == "vd":
+        want, tol = want.t(), tol.t()
+    agree(values(c.run()["grad_weight"]), want, tol, "grad_weight")
