@@ -988,7 +988,8 @@ def _readout_vocab_mask(mask: Optional[Tensor], logits_shape, rows: int, V: int,
         raise ValueError(f"vocabulary mask of dtype {mask.dtype} (u8 keep-mask, or additive f32, bf16 or f16)")
     kind = NT_MASK_U8 if mask.dtype == "u8" else NT_MASK_F32
     sh, full = tuple(mask.shape), tuple(logits_shape)
-    by_row = kind, mask, V, (rows // seeds) * V
+    seed = rows // seeds * V if seeds else 0
+    by_row = kind, mask, V, seed
     if sh and sh[-1] == V and mask.numel == V:
         return kind, mask, 0, 0
     if len(sh) != len(full):  # rows of another rank: one per logits row
@@ -999,7 +1000,7 @@ def _readout_vocab_mask(mask: Optional[Tensor], logits_shape, rows: int, V: int,
     elif seeds > 1 and sh == (seeds, 1, V):
         return kind, mask, 0, V
     elif all(a == b or a == 1 for a, b in zip(sh, full)):
-        return kind, ops.copy(mask, ops.Layout.contiguous(sh).broadcast(full)), V, (rows // seeds) * V
+        return kind, ops.copy(mask, ops.Layout.contiguous(sh).broadcast(full)) if rows else mask, V, seed
     raise ValueError(f"readout: a mask {list(sh)} that does not broadcast to the logits {list(full)}")
 
 

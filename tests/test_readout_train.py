@@ -139,6 +139,15 @@ def test_scales_of_rows_without_elements_are_counted(rows, scales):
             call()
 
 
+@pytest.mark.parametrize("shape", [(0, 5, 32), (1, 5, 32), (0, 1, 32), (1, 1, 32), (32,)])
+def test_masks_of_no_seeds(shape):
+    """No seeds, a mask: shapes that broadcast are taken, others refused."""
+    kind, mask, _, _ = nr._readout_vocab_mask(Fake(shape, "u8"), (0, 5, 32), 0, 32, 0)
+    assert kind == nr.NT_MASK_U8 and mask.shape == shape
+    with pytest.raises(ValueError, match="does not broadcast"):
+        nr._readout_vocab_mask(Fake((2, 5, 32), "u8"), (0, 5, 32), 0, 32, 0)
+
+
 def test_argument_struct_layouts_match_the_header(tmp_path):
     names = ("NtRlReadoutStatsArgs", "NtRlReadoutStatsGradArgs")
     lines = []

@@ -669,3 +669,13 @@ def test_f16_weight_gradients_of_rows_far_apart(rows, V, d, spread, layout):
     if layout == "vd":
         want, tol = want.t(), tol.t()
     agree(values(c.run()["grad_weight"]), want, tol, "grad_weight")
+
+
+@pytest.mark.parametrize("shape", [(0, 5, 300), (1, 5, 300), (300,), None])
+def test_no_seeds(shape):
+    """A weight of no seeds: empty results and gradients, with a mask and without."""
+    h, w, t = nr.Tensor((0, 5, 16), "bf16"), nr.Tensor((0, 16, 300), "bf16"), nr.Tensor((0, 5), "i32")
+    m = None if shape is None else nr.Tensor(shape, "u8")
+    lp, ent, stats = nr.readout_score_with_stats(h, w, 1.0, m, t)
+    gh, gw = nr.readout_score_grad(h, w, 1.0, m, t, stats, ent, lp, ent)
+    assert lp.shape == ent.shape == (0, 5) and gh.shape == (0, 5, 16) and gw.shape == (0, 16, 300)
