@@ -1151,9 +1151,9 @@ int backward(const NtRlReadoutStatsGradArgs *a) {
     const Plan sw = dv ? plan(d, width, R * 2, true, most_w) : plan(width, d, R * 2, true, most_w);
     const bool hslab = sh.splits > 1 || cols < V || kept;
     Scratch s;
-    const int o_h = s.add(hdirect ? 0 : R * kp * 2), o_hs = s.add(R * kp * 2);
+    const int o_h = s.add(hdirect ? 0 : R * kp * 2), o_hs = s.add(a->grad_weight ? R * kp * 2 : 0);
     const int o_w = s.add(wdirect ? 0 : (dv ? d * cols : cols * kp) * 2);
-    const int o_coef = s.add(R * 16), o_left = s.add(kept ? R * 4 : 0), o_up = s.add(R * 4), o_top = s.add(4);
+    const int o_coef = s.add(R * 16), o_left = s.add(kept ? R * 4 : 0), o_up = s.add(f16 ? R * 4 : 0), o_top = s.add(f16 ? 4 : 0);
     const int o_g = s.add(R * cols * 2);
     const int o_sh = s.add(a->grad_hidden && hslab ? sh.splits * R * d * 4 : 0);
     const int o_sw = s.add(a->grad_weight && sw.splits > 1 ? sw.splits * std::min(cols, V) * d * 4 : 0);
@@ -1175,7 +1175,7 @@ int backward(const NtRlReadoutStatsGradArgs *a) {
     c.f16 = f16;
     c.coef = s.at<float4>(o_coef);
     c.left = kept ? s.at<float>(o_left) : nullptr;
-    c.up = s.at<float>(o_up);
+    c.up = f16 ? s.at<float>(o_up) : nullptr;
     c.top = top;
     hipLaunchKernelGGL(k_readout_coef, dim3(unsigned(std::min<int64_t>(ceil_div(R, 1024), 256))), dim3(1024), 0, ctx().stream, c);
     if (int rc = launched("k_readout_coef")) return rc;
