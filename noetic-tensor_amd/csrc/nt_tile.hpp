@@ -15,10 +15,9 @@
 // chunk of 32 rows, or 4 k of 32 columns by ds_read_b64_tr_b16) touch every bank once per pass. The load
 // unit writes LDS lane by lane, so it is the global address of each lane that is permuted.
 //
-// Rows past the operand's last, k past its end and whole stages past it read as zeros through the buffer
-// resource's range and touch no memory; a k-contiguous row's bytes count is a multiple of 16 (callers pad).
-// A transposed operand's columns past its last hold the next row's values: they reach only output columns
-// that are not stored.
+// Rows past the operand's last, k past its end, whole stages past it and a transposed operand's columns past its last
+// (what is behind a row, a NaN too, would pass an additive mask's -inf) read as zeros through the buffer resource's
+// range and touch no memory; a row's bytes count is a multiple of 16 (callers pad).
 #pragma once
 
 #include <hip/hip_runtime.h>
@@ -112,7 +111,8 @@ struct Side {
             } else {
                 constexpr int kRow = 2 * B;  // bytes of a row in LDS
                 const int k = (1024 / kRow) * slot + lane * 16 / kRow;
-                voff[q] = uint32_t(k * ld) + ((lane % (kRow / 16)) ^ (swz(k) << 2)) * 16;
+                const int at = ((lane % (kRow / 16)) ^ (swz(k) << 2)) * 16;
+                voff[q] = at < width ? uint32_t(k * ld) + at : 0x80000000u;
             }
         }
         if constexpr (!TR) {

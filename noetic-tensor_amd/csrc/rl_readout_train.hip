@@ -67,7 +67,7 @@ struct MaskP {
 
 // A wave's block of the mask, 32 rows by 32 TN columns, through LDS: whole 16-byte pieces of its rows in (a lane's
 // own four columns of 32 rows would be 16 scattered loads), a lane's four columns of its row out. Columns past the
-// vocabulary's `n` are not read.
+// vocabulary's `n`, whose logits are 0 (nt_tile.hpp), count as excluded.
 template <int TN>
 struct MaskBlock {
     static constexpr int kU8 = 32 * TN + 16, kF32 = 128 * TN + 16;  // bytes of a row in LDS
@@ -147,8 +147,7 @@ struct MaskBlock {
     }
 };
 
-// The columns past the vocabulary's end, `left` columns from this lane's first: nothing, whatever a weight's row holds
-// behind its last value (a NaN there would pass an additive mask's -inf).
+// Without a mask: the columns past the vocabulary's end, `left` columns from this lane's first.
 template <int Q>
 __device__ __forceinline__ void ended(float (&x)[Q][4], int left) {
 #pragma unroll
@@ -232,8 +231,9 @@ __global__ __launch_bounds__(S::kThreads, 1) void k_readout_stats(PieceP p) {
             if (row0 < p.rows)
                 MaskBlock<TN>::in(mlds, p.mask, row0, p.rows - row0 < 32 ? int(p.rows - row0) : 32, in * T::BN + 32 * TN * wn, p.n, lane, i == 0);
             MaskBlock<TN>::out(mlds, p.mask, p.invt, lane, x);
+        } else if (in * T::BN + T::BN > p.n) {
+            ended(x, p.n - col0);
         }
-        if (in * T::BN + T::BN > p.n) ended(x, p.n - col0);
         float m = -INFINITY;
 #pragma unroll
         for (int q = 0; q < 4 * TN; q++)
@@ -529,8 +529,9 @@ __global__ __launch_bounds__(S::kThreads, 1) void k_readout_g(PieceP p) {
         if constexpr (MASK) {
             MaskBlock<TN>::in(mlds, p.mask, row0, p.rows - row0 < 32 ? int(p.rows - row0) : 32, in * T::BN + 32 * TN * wn, p.n, lane, i == 0);
             MaskBlock<TN>::out(mlds, p.mask, p.invt, lane, x);
+        } else if (in * T::BN + T::BN > p.n) {
+            ended(x, p.n - col0);
         }
-        if (in * T::BN + T::BN > p.n) ended(x, p.n - col0);
 #pragma unroll
         for (int q = 0; q < 4 * TN; q++) {
             float g[4];
