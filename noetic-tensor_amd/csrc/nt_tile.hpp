@@ -30,6 +30,7 @@ namespace nt {
 namespace tile {
 
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef int i32x16 __attribute__((ext_vector_type(16)));
@@ -352,9 +353,16 @@ __device__ __forceinline__ uint32_t pair16(float lo, float hi) {
         asm("v_cvt_pk_bf16_f32 %0, %1, %2" : "=v"(r) : "v"(lo), "v"(hi));
         return r;
     } else {
-        const uint16_t a = __builtin_bit_cast(uint16_t, _Float16(lo)), b = __builtin_bit_cast(uint16_t, _Float16(hi));
-        return uint32_t(a) | (uint32_t(b) << 16);
+        return __builtin_bit_cast(uint32_t, f16x2{_Float16(lo), _Float16(hi)});
     }
+}
+
+// Between the lanes' stores into a wave's own LDS and other lanes' loads from it, and between those loads and the next
+// stores: the LDS takes a wave's accesses in their order, and the compiler, for which a lane's own accesses are all there
+// is, keeps them on their sides of this. No instruction.
+__device__ __forceinline__ void wave_exchange() {
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
 }
 
 // A wave's 32 x 32 TN block of the output as whole cache lines: the tile's layout gives a lane four neighbouring
@@ -378,7 +386,7 @@ __device__ __forceinline__ void store_block(uint8_t *lds, const V (&v)[4 * TN], 
         else
             *reinterpret_cast<u32x4 *>(lds + r * kRow + ((2 * q + h) ^ (r % 16)) * 16) = v[q];
     }
-    // (the compiler orders a wave's own LDS accesses; no other wave touches these)
+    wave_exchange();
     const int c = lane % kPer;
 #pragma unroll
     for (int g = 0; g < 32 / kAt; g++) {
@@ -400,6 +408,7 @@ __device__ __forceinline__ void store_block(uint8_t *lds, const V (&v)[4 * TN], 
             }
         }
     }
+    wave_exchange();
 }
 // The LDS a wave's blocks take.
 template <int TN>

@@ -230,7 +230,9 @@ __global__ __launch_bounds__(S::kThreads, 1) void k_readout_stats(PieceP p) {
             const int64_t row0 = row - lane % 32;
             if (row0 < p.rows)
                 MaskBlock<TN>::in(mlds, p.mask, row0, p.rows - row0 < 32 ? int(p.rows - row0) : 32, in * T::BN + 32 * TN * wn, p.n, lane, i == 0);
+            wave_exchange();
             MaskBlock<TN>::out(mlds, p.mask, p.invt, lane, x);
+            wave_exchange();
         } else if (in * T::BN + T::BN > p.n) {
             ended(x, p.n - col0);
         }
@@ -528,7 +530,9 @@ __global__ __launch_bounds__(S::kThreads, 1) void k_readout_g(PieceP p) {
             for (int e = 0; e < 4; e++) x[q][e] = t.acc[i][q / 4][4 * (q % 4) + e];
         if constexpr (MASK) {
             MaskBlock<TN>::in(mlds, p.mask, row0, p.rows - row0 < 32 ? int(p.rows - row0) : 32, in * T::BN + 32 * TN * wn, p.n, lane, i == 0);
+            wave_exchange();
             MaskBlock<TN>::out(mlds, p.mask, p.invt, lane, x);
+            wave_exchange();
         } else if (in * T::BN + T::BN > p.n) {
             ended(x, p.n - col0);
         }
