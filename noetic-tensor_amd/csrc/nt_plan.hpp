@@ -50,9 +50,10 @@ inline Plan plan(int64_t m, int64_t n, int64_t kb, bool split, Size most = Size:
         for (int64_t r = 0; r <= 4; r++) {  // unsplit, and the splits that give every CU one to four workgroups
             int64_t s = r == 0 ? 1 : 256 * r / tiles;
             s = s > 64 ? 64 : s;
+            // (512 bytes of k a split at the least: 8-bit products of 64 x 1000 x 8192 29 -> 10 us, 16 x 256 x 16384 52 -> 8)
+            s = s > 1 && s > kb / 512 ? kb / 512 : s;
             if (s < 1 || (s > 1 && !split)) continue;
             const int64_t per = round_up(ceil_div(kb, s), 64), splits = ceil_div(kb, per);
-            if (splits > 1 && per < 512) continue;
             const int64_t wgs = tiles * splits, rounds = ceil_div(wgs, c.slots);
             const double cost = double(rounds) * (double(per / 64) * (wgs <= 256 ? c.alone : c.stage) + c.output) +
                                 (splits > 1 ? 4.0 + double(splits) * (0.15 + double(m) * double(n) * 8e-6 / 4.0) : 0.0);

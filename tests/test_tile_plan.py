@@ -1,0 +1,41 @@
+"""The plan of a product's tiles (csrc/nt_plan.hpp), on the CPU: what it promises of every size."""
+import random
+
+from tests.tile_plan import LARGE, MEDIUM, SMALL, int8_product, plan, whole_rounds
+
+
+def sizes(n, seed):
+    rng = random.Random(seed)
+    size = lambda most: int(2 ** rng.uniform(0, most))  # noqa: E731
+    return [(size(16), size(18), 16 * size(13)) for _ in range(n)]
+
+
+def test_splits_cover_k():
+    for m, n, kb in sizes(3000, 1):
+        for split in (False, True):
+            for most in (SMALL, MEDIUM, LARGE):
+                size, per, splits = plan(m, n, kb, split, most)
+                assert size <= most and per % 64 == 0 and 1 <= splits <= 64
+                assert splits * per >= kb > (splits - 1) * per or splits == 1
+                assert splits == 1 or (split and per >= 512)
+
+
+def test_few_tiles_are_split():
+    """Where a product's tiles are a sixteenth of the CUs and less, k of 2048 bytes or more is split: as many parts as have
+    512 bytes, at most 64 and four workgroups a CU, or fewer."""
+    seen = 0
+    for m, n, kb in sizes(20000, 2):
+        tiles = -(-m // 64) * -(-n // 128)
+        if tiles <= 16 and kb >= 2048:
+            _, _, splits = plan(m, n, kb, True)
+            assert 2 <= splits <= kb // 512, (m, n, kb, splits)
+            seen += 1
+    assert seen > 200
+    for m, n, k in ((64, 1000, 8192), (16, 256, 16384), (5, 40, 20000), (64, 2048, 4096)):
+        assert int8_product(m, n, k)[1] >= 8
+
+
+def test_whole_rounds_leave_a_rest():
+    for m, n, kb in sizes(3000, 3):
+        c = whole_rounds(m, n, kb)
+        assert c == 0 or (0 < c < n and c % 256 == 0 and plan(m, n, kb, False)[0] == LARGE)
