@@ -169,6 +169,22 @@ def test_products(m, n, k, dtype):
     agree(y, product(a, sa, b, sb), dtype)
 
 
+# Every tile, split k and not, with sides that end inside one: what each takes is asserted in tests/test_tile_plan.py. (5 to
+# 64 rows against a few columns are 1 to 16 tiles, whose k is split into 512 bytes and more.)
+PLANS = [(5, 40, 48), (5, 40, 2064), (64, 1000, 8192), (17, 500, 1040), (600, 40, 131071), (1000, 4100, 48), (3001, 4100, 300),
+         (1000, 4100, 10496)]
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("m,n,k", PLANS)
+def test_every_plan(m, n, k, dtype):
+    g = torch.Generator().manual_seed(m + 1000 * n + k)
+    a, b = (torch.randint(-127, 128, (r, k), generator=g, dtype=torch.int8) for r in (m, n))
+    sa, sb = torch.rand(m, generator=g) * 1e-3, torch.rand(n, generator=g) * 1e-2
+    y = ops.matmul_int8(given(a), given(sa), given(b), given(sb), dtype)
+    agree(y, product(a, sa, b, sb), dtype)
+
+
 def test_sums_at_their_ends():
     """All of one sign at the largest k: the sums reach 2^31 - 2^14 and its negative, -128 among the values."""
     k = 131071

@@ -679,3 +679,42 @@ def test_no_seeds(shape):
     lp, ent, stats = nr.readout_score_with_stats(h, w, 1.0, m, t)
     gh, gw = nr.readout_score_grad(h, w, 1.0, m, t, stats, ent, lp, ent)
     assert lp.shape == ent.shape == (0, 5) and gh.shape == (0, 5, 16) and gw.shape == (0, 16, 300)
+
+
+# Every tile, split k and unsplit, of each gradient's product (dH's without a split written as it is, with one through slabs),
+# and dW's columns in whole rounds with a rest beside them: what each takes is asserted in tests/test_tile_plan.py.
+PLANS = [(520, 136, 40, "bf16", "dv", "f32"), (520, 130, 40, "f16", "vd", "none"), (1030, 130, 40, "bf16", "dv", "u8"),
+         (520, 1003, 40, "f16", "vd", "none"), (4100, 130, 1001, "f16", "dv", "none"), (4100, 8200, 40, "bf16", "vd", "u8_shared"),
+         (3000, 130, 4100, "bf16", "dv", "none"), (4100, 130, 4100, "f16", "dv", "f32_shared"), (520, 33000, 40, "bf16", "vd", "none"),
+         (4100, 4100, 1001, "bf16", "vd", "none"), (4100, 4104, 1001, "f16", "dv", "none"), (520, 17001, 4100, "bf16", "vd", "none"),
+         (520, 17008, 4100, "f16", "dv", "none")]
+# A row's scores by 256 x 256 tiles, by 128 x 128 ones and by 64 x 128 ones (rows, and as few of them).
+TILES_OF_ROWS = [(300, 32768, 512, 3), (130, 30016, 520, 3), (2100, 32768, 512, 300), (2100, 32768, 512, 130)]
+
+
+@pytest.mark.parametrize("rows,V,d,dtype,layout,mask", PLANS)
+def test_every_plan(rows, V, d, dtype, layout, mask):
+    c = Case(rows, V, d, dtype, layout, mask, tau=0.9)
+    got = c.run()
+    for name in ("h", "w", "tokens", "g_logp", "g_entropy", "add"):
+        setattr(c, name, getattr(c, name).to("cuda"))
+    device = torch.get_default_device()
+    torch.set_default_device("cuda")
+    try:
+        want, tol = c.want()
+    finally:
+        torch.set_default_device(device)
+    for k in got:
+        agree(values(got[k]).to("cuda"), want[k], tol[k], k)
+
+
+@pytest.mark.parametrize("layout", ["dv", "vd"])
+@pytest.mark.parametrize("rows,V,d,few", TILES_OF_ROWS)
+def test_a_rows_scores_are_the_same_by_every_tile(rows, V, d, few, layout):
+    c = Case(rows, V, d, "bf16", layout, "u8_shared", tau=0.7)
+    h, w, m, t = given(c.h), given(c.w), given(c.mask), given(c.tokens)
+    full = nr.readout_score_with_stats(h, w, c.tau, m, t, layout=layout)
+    at = torch.linspace(0, rows - 1, few).long()
+    part = nr.readout_score_with_stats(given(c.h[at]), w, c.tau, m, given(c.tokens[at]), layout=layout)
+    for a, b in ((full[0], part[0]), (full[1], part[1]), (full[2].lse_base, part[2].lse_base), (full[2].lse_rest, part[2].lse_rest)):
+        assert np.array_equal(a.to_numpy()[at.numpy()], b.to_numpy())

@@ -1,7 +1,14 @@
-"""The plan of a product's tiles (csrc/nt_plan.hpp), on the CPU: what it promises of every size."""
+"""The plan of a product's tiles (csrc/nt_plan.hpp), on the CPU: what it promises of every size, and that the sizes of the
+GPU tests take every tile, split and cut there is."""
 import random
 
-from tests.tile_plan import LARGE, MEDIUM, SMALL, int8_product, plan, whole_rounds
+import pytest
+
+from tests import test_int8_gpu, test_readout_train_gpu
+from tests.tile_plan import LARGE, MEDIUM, SMALL, int8_product, plan, readout, whole_rounds
+
+ROWS = {SMALL: 64, MEDIUM: 128, LARGE: 256}
+COLS = {SMALL: 128, MEDIUM: 128, LARGE: 256}
 
 
 def sizes(n, seed):
@@ -39,3 +46,28 @@ def test_whole_rounds_leave_a_rest():
     for m, n, kb in sizes(3000, 3):
         c = whole_rounds(m, n, kb)
         assert c == 0 or (0 < c < n and c % 256 == 0 and plan(m, n, kb, False)[0] == LARGE)
+
+
+def test_int8_sizes_take_every_plan():
+    taken = {(size, splits > 1) for size, splits in (int8_product(*p) for p in test_int8_gpu.PLANS)}
+    assert taken == {(t, s) for t in (SMALL, MEDIUM, LARGE) for s in (False, True)}
+    assert any(m % ROWS[LARGE] and n % COLS[LARGE] and int8_product(m, n, k) == (LARGE, 1) for m, n, k in test_int8_gpu.PLANS)
+
+
+def test_readout_sizes_take_every_plan():
+    logits, hidden, weight, cuts = set(), set(), set(), set()
+    for rows, V, d, _, layout, _ in test_readout_train_gpu.PLANS:
+        l, h, w = readout(rows, V, d, layout)
+        logits.add(l[0])
+        hidden.add((h[0], h[1] > 1))
+        weight.add((w[0], w[1] > 1))
+        if w[2]:
+            cuts.add(layout)
+    both = {(t, s) for t in (SMALL, MEDIUM, LARGE) for s in (False, True)}
+    assert logits == {SMALL, MEDIUM, LARGE} and hidden == both and weight == both and cuts == {"dv", "vd"}
+
+
+@pytest.mark.parametrize("rows,V,d,few", test_readout_train_gpu.TILES_OF_ROWS)
+def test_rows_compared_are_scored_by_different_tiles(rows, V, d, few):
+    full, part = readout(rows, V, d, "vd")[0], readout(few, V, d, "vd")[0]
+    assert full != part, (full, part)
