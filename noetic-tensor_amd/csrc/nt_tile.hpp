@@ -99,6 +99,9 @@ struct Side {
 
     static __device__ __forceinline__ int swz(int k) { return B == 64 ? (k >> 1) & 1 : k & 3; }
 
+    // Where byte `at` of row k of a stage lies (TR).
+    static __device__ __forceinline__ int at(int k, int at) { return k * 2 * B + ((at / 64) ^ swz(k)) * 64 + at % 64; }
+
     __device__ __forceinline__ void init(const Operand &o, int wave, int lane, int first_tile) {
         base = o.base, ld = o.ld, width = o.width;
         rows = !TR && o.rows > B ? B : o.rows;
@@ -116,8 +119,13 @@ struct Side {
                 voff[q] = at < width ? uint32_t(k * ld) + at : 0x80000000u;
             }
         }
-        if constexpr (!TR) {
+        if constexpr (!TR)
             src[0] = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t *>(base), short(0), int((rows - 1) * ld + width), kWord3);
+        reads(lane, first_tile);
+    }
+    // Where the fragments of this lane lie in a stage, from tile `first_tile` of 32 rows on.
+    __device__ __forceinline__ void reads(int lane, int first_tile) {
+        if constexpr (!TR) {
             const int row = 32 * first_tile + lane % 32, s = (row >> 2) & 3;
             addr[0] = row * kStageK + ((lane / 32) ^ s) * 16;
             addr[1] = row * kStageK + ((2 + lane / 32) ^ s) * 16;
@@ -283,9 +291,33 @@ struct Tile {
             landed(x.a, x.b);
             b0 = b2;
         }
-        // every copy has landed, and every wave is past its last read, before the caller uses the LDS
+        // every copy has landed, and every wave is past its last read, before the caller uses the LDS; said so that the
+        // compiler knows it too, which else waits for all memory operations, stores among them, wherever a caller's loop or
+        // branch reads the LDS
         wait_copies<0>();
+        __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0)
         asm volatile("s_barrier" ::: "memory");
+#endif
+    }
+
+    // acc += the product over one more stage, which the caller has put in the first buffer (in front of a barrier).
+    __device__ __forceinline__ void stage(uint8_t *lds, int wave, int lane) {
+#ifdef __HIP_DEVICE_COMPILE__  // (as in run)
+        SideA sa;
+        SideB sb;
+        sa.reads(lane, TM * (wave / WN));
+        sb.reads(lane, TN * (wave % WN));
+        const uint32_t at = uint32_t((uintptr_t)(lds_ptr)(lds));
+        unrolled<2>([&](auto j) {
+            Frags x;
+            unrolled<kReadsA>([&](auto r) { sa.template issue<r, j>(at, x.a[r]); });
+            unrolled<kReadsB>([&](auto r) { sb.template issue<r, j>(at + SideA::kBytes, x.b[r]); });
+            landed(x.a, x.b);
+            unrolled<TM * TN>([&](auto m) {
+                constexpr int I = decltype(m)::value / TN, K = decltype(m)::value % TN;
+                acc[I][K] = E::mfma(SideB::fragment(x.b, K), SideA::fragment(x.a, I), acc[I][K]);
+            });
+        });
 #endif
     }
 

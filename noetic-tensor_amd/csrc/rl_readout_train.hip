@@ -19,15 +19,16 @@
 //  dW = G^T H (the piece's rows of it, whole) and dH += G W^T (f32 sums over the pieces). 8 rows V dim
 //  operations with the forward's, against 6 where the logits are kept: the least there is without them.
 //
-//  Rounding: G is the one value that is rounded on the way (2^-9 of itself for bf16, 2^-12 for f16, as the
-//  gradients are when they are written); every sum is f32. A row's entry at its token is most of G, and its rounding
-//  would show in the gradients as their own does: for up to 512 rows what it left goes into both of them in f32, times the
-//  token's row of W and the row of H (128 x 1024 x 32000 bf16: the error is 0.0017 of the norm, which is the written
-//  values' own, instead of 0.0022, for 112 us instead of 104). For f16, whose range G would leave, a row of G is
-//  held in units of 2^(e - 14), 2^e over |g_logp| + 16 |g_entropy| (p |ln p + entropy| is under 14 for a
-//  vocabulary of 2^20), and for dW the row of H is scaled by 2^e and the one power of two that puts the largest value of
-//  all scaled rows under 2^15: what rows far below the largest lose to f16's smallest steps is 2^-40 of that
-//  value, less than the smallest step of a gradient that holds the largest row's.
+//  Rounding: G is rounded on the way (2^-9 of itself for bf16, 2^-12 for f16, as the gradients are when they are
+//  written), and for f16 the rows of H below; every sum is f32. A row's entry at its token is most of G, and its rounding
+//  would show in the gradients as their own does, so what it left goes into them, times the row of H into dW as a stage
+//  more of its product (LeftRows) and times the token's row of W into dH as its sums are folded: the error is the written
+//  values' own, 0.0017 of the norm for bf16, where it was 0.0023 (2048 x 4096 x 50304 2.93 -> 2.96 ms, 4096 x 4096 x 128256
+//  13.5 -> 13.6). A DV weight's columns are read for it up to 512 rows; dH of more has 0.0023 (kColumnRows).
+//  For f16, whose range G would leave, a row of G is held in units of 2^(e - 14), 2^e over |g_logp| + 16 |g_entropy|
+//  (p |ln p + entropy| is under 14 for a vocabulary of 2^20), and for dW the row of H is scaled by 2^e and the one power
+//  of two that puts the largest value of all scaled rows under 2^15: what rows far below the largest lose to f16's
+//  smallest steps is 2^-40 of that value, less than the smallest step of a gradient that holds the largest row's.
 //
 //  Bound by the matrix cores for many rows, and those by power: 4096 x 4096 x 128256 bf16 is scored in 3.2-3.3 ms (1.33
 //  PFLOP/s at a clock near 1.5 GHz; a library product alone 2.99) and scored and differentiated in 13.4 ms (1.29 at its 8
@@ -178,7 +179,7 @@ struct PieceP {
     const float4 *coef;       // [rows] {the largest value (+inf: nothing flows), a, b, the token's term}
     uint8_t *g;               // [rows, ldg bytes], of which gbytes are written: zeros past n
     int64_t ldg, gbytes;
-    float *left;              // [rows] what the rounding of G's entry at the row's token left, or null
+    float *left;              // [rows] what the rounding of G's entry at the row's token left
 };
 
 template <class T, bool BTR>
@@ -369,18 +370,63 @@ struct CoefP {
     double tau;
     int f32mask, f16;
     float4 *coef;
-    float *left;   // [rows] zeros here, or null
+    float *left;   // [rows] zeros here
+    unsigned coefs;  // workgroups; those behind them list the tokens
+    int2 *place;   // [vocab / 256] a bucket's first entry in `listed`, and how many
+    uint32_t *listed;  // [rows] row << 8 | token % 256
     float *up;     // [rows] f16: 2^e, what a row of G was divided by (0: nothing flows)
     int *top;      // [1] f16: cleared here, for k_readout_top
 };
 
 constexpr int kNoTop = -(1 << 30);
 
+// The rows whose token is in 256 columns of the vocabulary, `bucket`, in their order: a workgroup goes through all the
+// tokens, a wave through consecutive ones, once to count them and those of the buckets in front, once to write them.
+constexpr int kBucket = 256;
+__device__ __forceinline__ void list_tokens(const CoefP &p, int bucket) {
+    __shared__ int s_hits[16], s_less[16];
+    const int lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
+    const int64_t per = ((p.rows + 15) / 16 + 63) / 64 * 64, first = wave * per < p.rows ? wave * per : p.rows;
+    const int64_t last = first + per < p.rows ? first + per : p.rows;
+    const uint32_t from = uint32_t(bucket) * kBucket;
+    auto token = [&](int64_t r) { return r < last ? uint32_t(p.tokens[r]) : ~0u; };
+    int hits = 0, less = 0;
+    for (int64_t r = first + lane; r - lane < last; r += 512) {
+        uint32_t t[8];
+#pragma unroll
+        for (int u = 0; u < 8; u++) t[u] = token(r + 64 * u);  // (eight loads in flight)
+#pragma unroll
+        for (int u = 0; u < 8; u++) {
+            hits += __popcll(__ballot(t[u] < p.vocab && t[u] - from < uint32_t(kBucket)));
+            less += __popcll(__ballot(t[u] < from));
+        }
+    }
+    if (lane == 0) s_hits[wave] = hits, s_less[wave] = less;
+    __syncthreads();
+    int start = 0, all = 0, at = 0;
+    for (int w = 0; w < 16; w++) {
+        start += s_less[w];
+        if (w == wave) at = all;
+        all += s_hits[w];
+    }
+    if (threadIdx.x == 0) p.place[bucket] = int2{start, all};
+    if (hits == 0) return;
+    at += start;
+    for (int64_t r = first + lane; r - lane < last; r += 64) {
+        const uint32_t t = token(r);
+        const bool hit = t < p.vocab && t - from < uint32_t(kBucket);
+        const uint64_t m = __ballot(hit);
+        if (hit) p.listed[at + __popcll(m & ((uint64_t(1) << lane) - 1))] = uint32_t(r) << 8 | (t - from);
+        at += __popcll(m);
+    }
+}
+
 // What a row's upstream gradients make of it: with l = (value - largest) c, so that p = 2^l q, q = e^-rest, and ln p =
 // l ln 2 - rest, G = 2^l (a + b l) + the token's term.
 __global__ __launch_bounds__(1024) void k_readout_coef(CoefP p) {
+    if (blockIdx.x >= p.coefs) return list_tokens(p, int(blockIdx.x - p.coefs));
     if (p.f16 && blockIdx.x == 0 && threadIdx.x == 0) *p.top = kNoTop;
-    for (int64_t r = blockIdx.x * int64_t(1024) + threadIdx.x; r < p.rows; r += int64_t(gridDim.x) * 1024) {
+    for (int64_t r = blockIdx.x * int64_t(1024) + threadIdx.x; r < p.rows; r += int64_t(p.coefs) * 1024) {
         const int64_t tok = p.tokens[r];
         double gl = p.g_logp ? double(p.g_logp[r]) : 0.0;
         if (tok < 0 || tok >= p.vocab) gl = 0.0;
@@ -405,7 +451,7 @@ __global__ __launch_bounds__(1024) void k_readout_coef(CoefP p) {
             unit = 1.0 / p.tau;
         }
         if (p.f16) p.up[r] = up;
-        if (p.left) p.left[r] = 0.0f;
+        p.left[r] = 0.0f;
         const float a = float(-(gl + ge * (h - rest)) * q * unit), b = float(-ge * kLn2 * q * unit);
         p.coef[r] = dead ? float4{INFINITY, 0.0f, 0.0f, 0.0f} : float4{top_x, a, b, float(gl * unit)};
     }
@@ -549,7 +595,7 @@ __global__ __launch_bounds__(S::kThreads, 1) void k_readout_g(PieceP p) {
                 for (int e = 0; e < 4; e++)
                     if (tok[i] == 8 * q + e) g[e] += k.w;
             v[q] = dead ? u32x2{0, 0} : u32x2{pair16<E>(g[0], g[1]), pair16<E>(g[2], g[3])};
-            if (mine && p.left)
+            if (mine)
 #pragma unroll
                 for (int e = 0; e < 4; e++)
                     if (tok[i] == 8 * q + e && !dead)
@@ -576,57 +622,79 @@ struct GradP {
     const float *row_scale;   // f16: [m] or null
     const int *top;           // f16: [1] or null
     float fixed;
-    // dW: what the rounding of G left of the tokens' entries (null: dH)
+    // dW: what the rounding of G left of the tokens' entries
     const float *left;        // [k]
-    const int32_t *tokens;    // [k]
+    const int2 *place;        // the rows of each 256 tokens
+    const uint32_t *listed;
     int64_t v0;               // the vocabulary's first row of the output (VD) or column (DV)
     bool dv;
 };
 
-// acc += left[r] H(r, .) at row r's token, for the rows whose token is among this wave's vocabulary from v0 on (its 32 rows,
-// or its columns, DV), in the order of r. `h` is H as the product reads it, [k, ldh bytes], `wh` bytes of each row.
-// `mine` and `lefts`: those of rows lane, lane + 64, .. (token -1 past the last), loaded in front of the product: a tile of so
-// few k takes no longer than a load.
-//
-// More than kLeftRows rows average their entries' roundings: the gradients' error is the written values' own and as much
-// again, within 6% of 1.41 of it, where with 128 rows a few upstream gradients far larger than the others make it 1.5 and
-// more; and the 256 x 256 tiles, which take over there, have no registers to add it in.
-constexpr int kLeftRows = 512, kLefts = kLeftRows / 64;
-template <class E, bool DV, int TN, class Acc>
-__device__ __forceinline__ void add_left(Acc (&acc)[TN], const GradP &p, const int (&mine)[kLefts], const float (&lefts)[kLefts],
-                                         int64_t v0, const uint8_t *h, int64_t ldh, int64_t wh, int64_t row0, int64_t col0, int lane) {
-    constexpr int BV = DV ? 32 * TN : 32;
-    const int first = int(v0);
-#pragma unroll
-    for (int b = 0; b < kLefts; b++) {
-        uint64_t hits = __ballot(mine[b] >= first && mine[b] < first + BV);
-        while (hits) {
-            const int at = __builtin_ctzll(hits), c = __builtin_amdgcn_readlane(mine[b], at) - first, k0 = 64 * b;
-            hits &= hits - 1;
-            const float left = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, lefts[b]), at));
-            const uint16_t *hr = reinterpret_cast<const uint16_t *>(h + (k0 + at) * ldh);
-            if constexpr (DV) {
-                const int64_t row = row0 + lane % 32;
-                const float x = left * widened<E>(hr[row < p.m ? row : 0]);
-                const int k = lane / 32 == c / 4 % 2 ? c / 8 * 4 + c % 4 : -1;
-#pragma unroll
-                for (int q = 0; q < 16 * TN; q++) acc[q / 16][q % 16] += k == q ? x : 0.0f;
-            } else {
-                uint16_t w[4 * TN][4];
-#pragma unroll
-                for (int q = 0; q < 4 * TN; q++) {  // (every load before the first use; columns past the end are not stored)
-                    const int64_t col = col0 + 8 * q + 4 * (lane / 32);
-                    __builtin_memcpy(w[q], hr + (col * 2 + 8 <= wh ? col : 0), 8);
-                }
-                const float f = lane % 32 == c ? left : 0.0f;
-#pragma unroll
-                for (int q = 0; q < 4 * TN; q++)
-#pragma unroll
-                    for (int e = 0; e < 4; e++) acc[q / 4][4 * (q % 4) + e] = fmaf(f, widened<E>(w[q][e]), acc[q / 4][4 * (q % 4) + e]);
-            }
+// dW's share of what the rounding of G left of each row's entry at its token, left[r] H(r, .) to the token's row of dW
+// (column, DV), as more k of the product: 32 of the rows whose token is in the tile's bucket at a time, one side of a stage
+// their rows of H, the other zeros but for each row's left (rounded to the operands' type: 2^-9 of what G's rounding
+// left) at its token. (Few rows have their token in a tile: of 4096, 8 in 256 columns of 128256, one stage beside 128.)
+template <class S>
+struct LeftRows {
+    static_assert(S::kRows <= kBucket && S::kCols <= kBucket, "a tile in a bucket");
+    int2 place;
+    int in;       // the tile's first column in its bucket
+    uint32_t e;   // this lane's of the first 64 rows, and what is left (0: none)
+    float left;
+
+    __device__ __forceinline__ void entry(const GradP &p, int j, uint32_t &e, float &left) const {
+        e = j < place.y ? p.listed[place.x + j] : 0u;
+        left = j < place.y ? p.left[e >> 8] : 0.0f;
+    }
+    // In front of the product (its latency beside the product's).
+    __device__ __forceinline__ void init(const GradP &p, int64_t m0, int64_t n0, int lane) {
+        const int64_t v = p.v0 + (p.dv ? n0 : m0);
+        place = p.place[v / kBucket];
+        in = int(v % kBucket);
+        entry(p, lane, e, left);
+    }
+    // One operand's panel of a stage (nt_tile.hpp), B columns: H's rows of lane j0 + k's entries, or the lefts.
+    template <int B>
+    __device__ __forceinline__ void rows(uint8_t *panel, const uint8_t *h, int64_t ldh, int64_t wh, uint32_t e, int j0) const {
+        typedef Side<B, S::WM * S::WN, true> P;
+        constexpr int kPer = 2 * B / 16;  // chunks of 16 bytes a row
+        for (int x = threadIdx.x; x < 32 * kPer; x += S::kThreads) {
+            const int k = x / kPer, at = x % kPer * 16;
+            const int64_t r = uint32_t(__shfl(int(e), j0 + k, 64)) >> 8;
+            u32x4 v = {0, 0, 0, 0};
+            if (at < wh) v = *reinterpret_cast<const u32x4 *>(h + r * ldh + at);
+            *reinterpret_cast<u32x4 *>(panel + P::at(k, at)) = v;
         }
     }
-}
+    template <class E, int B>
+    __device__ __forceinline__ void tokens(uint8_t *panel, uint32_t e, float left, int j0, int lane) const {
+        typedef Side<B, S::WM * S::WN, true> P;
+        for (int x = threadIdx.x; x < 4 * B; x += S::kThreads) *reinterpret_cast<u32x4 *>(panel + x * 16) = u32x4{0, 0, 0, 0};
+        __syncthreads();
+        const uint32_t c = (e & 255u) - uint32_t(in);
+        if (threadIdx.x < 64 && lane - j0 >= 0 && lane - j0 < 32 && left != 0.0f && c < uint32_t(B))
+            *reinterpret_cast<uint16_t *>(panel + P::at(lane - j0, int(c) * 2)) = uint16_t(pair16<E>(left, 0.0f));
+    }
+    template <class E, class T>
+    __device__ __forceinline__ void add(T &t, uint8_t *lds, const GradP &p, int64_t m0, int64_t n0, int wave, int lane) {
+        constexpr int BM = T::BM, BN = T::BN;
+        uint8_t *const a = lds, *const b = lds + T::SideA::kBytes;
+        for (int j = 0; j < place.y; j += 32) {
+            if (j > 0 && j % 64 == 0) entry(p, j + lane, e, left);
+            const int j0 = j % 64;
+            if (p.dv) {
+                rows<BM>(a, p.a + m0 * 2, p.lda, p.wa - m0 * 2, e, j0);
+                tokens<E, BN>(b, e, left, j0, lane);
+            } else {
+                rows<BN>(b, p.b + n0 * 2, p.ldb, p.wb - n0 * 2, e, j0);
+                tokens<E, BM>(a, e, left, j0, lane);
+            }
+            __syncthreads();
+            t.stage(lds, wave, lane);
+            __syncthreads();
+        }
+    }
+};
 
 // (Two waves a SIMD, 256 registers each, or the smaller tiles' second workgroup waits: dW 128 x 1024 x 32000 54 -> 30 us.)
 template <class E, class S, bool ATR, bool BTR>
@@ -645,28 +713,14 @@ __global__ __launch_bounds__(S::kThreads, S::TM == 1 ? 2 : 1) void k_readout_gra
                           : Operand{p.a + m0 * p.lda + k0 * 2, p.lda, p.m - m0, kb};
     const Operand b = BTR ? Operand{p.b + k0 * p.ldb + n0 * 2, p.ldb, kn, p.wb - n0 * 2}
                           : Operand{p.b + n0 * p.ldb + k0 * 2, p.ldb, p.n - n0, kb};
-    constexpr bool kLeft = ATR && BTR && TM == 1;
-    int mine[kLeft ? kLefts : 1];
-    float lefts[kLeft ? kLefts : 1];
-    if (kLeft && p.left) {
-#pragma unroll
-        for (int q = 0; q < kLefts; q++) {
-            const int r = 64 * q + lane < p.k ? 64 * q + lane : 0;
-            mine[q] = p.tokens[r];
-            lefts[q] = p.left[r];
-            if (64 * q + lane >= p.k) mine[q] = -1;
-        }
-    }
+    constexpr bool kDW = ATR && BTR;
+    LeftRows<S> lefts;
+    if (kDW) lefts.init(p, m0, n0, lane);
     T t;
     t.run(lds, a, b, kb, wave, lane);
+    if constexpr (kDW)
+        if (blockIdx.y == 0) lefts.template add<E>(t, lds, p, m0, n0, wave, lane);
     const int wm = wave / WN, wn = wave % WN;
-    if constexpr (kLeft) {
-        if (p.left && blockIdx.y == 0) {
-            const int64_t row0 = m0 + 32 * wm, c0 = n0 + 32 * TN * wn;
-            if (p.dv) add_left<E, true>(t.acc[0], p, mine, lefts, p.v0 + c0, p.a, p.lda, p.wa, row0, c0, lane);
-            else add_left<E, false>(t.acc[0], p, mine, lefts, p.v0 + row0, p.b, p.ldb, p.wb, row0, c0, lane);
-        }
-    }
     const float whole = p.top ? ldexpf(p.fixed, -lift(p.top)) : p.fixed;
     const int64_t col0 = n0 + 32 * TN * wn;
     if (col0 >= p.n) return;
@@ -729,6 +783,11 @@ struct LeftP {
     int dv;
 };
 
+// Rows up to which a DV weight's columns are read for it: a column's every value is a line of its own, and for 2048 rows of
+// dim 4096 (V 50304) they took 90 us of 2930. Without it a row of dH is off by a factor within 2^-9 of 1 (bf16; f16 2^-12),
+// the rounding of its G at its token, beside its values' own.
+constexpr int64_t kColumnRows = 512;
+
 template <class E>
 __global__ __launch_bounds__(256) void k_readout_fold(const float *slab, int splits, int64_t m, int64_t n, LeftP p, uint16_t *out,
                                                       int64_t ldo, const float *row_scale, const int *top, float fixed) {
@@ -772,7 +831,7 @@ __global__ __launch_bounds__(256) void k_readout_fold(const float *slab, int spl
 // blocks of up to 128 MiB for the next call; a larger one is the device pool's, and its allocation may wait for the
 // stream), then the places.
 struct Scratch {
-    static constexpr int kMost = 12;
+    static constexpr int kMost = 16;
     static constexpr size_t kAlone = size_t(1) << 20;
     size_t size[kMost], together = 0;
     void *place[kMost], *shared = nullptr;
@@ -1053,7 +1112,9 @@ struct BackP {
     const NtRlReadoutStatsGradArgs *a;
     PieceP p;
     Plan sh, sw;
-    bool hslab;
+    bool hslab, hleft;
+    const int2 *place;
+    const uint32_t *listed;
     const uint8_t *hs;  // the scaled hidden states, [rows, ldhs bytes]
     int64_t ldhs;
     float *slab_h, *slab_w;
@@ -1078,7 +1139,8 @@ int piece(const BackP &b) {
         w.n = DV ? p.n : p.dim;
         w.k = p.rows;
         w.left = p.left;
-        w.tokens = p.tokens;
+        w.place = b.place;
+        w.listed = b.listed;
         w.v0 = p.v0;
         w.dv = DV;
         uint16_t *out = static_cast<uint16_t *>(a->grad_weight) + (DV ? p.v0 : p.v0 * a->grad_weight_ld);
@@ -1087,7 +1149,7 @@ int piece(const BackP &b) {
         w.slab = b.slab_w;
         w.top = b.top;
         w.fixed = b.fixed;
-        const int64_t c = b.sw.splits > 1 || p.left ? 0 : whole_rounds(DV ? w.m : w.n, DV ? w.n : w.m, w.k * 2);
+        const int64_t c = b.sw.splits > 1 ? 0 : whole_rounds(DV ? w.m : w.n, DV ? w.n : w.m, w.k * 2);
         if (c) {  // whole rounds of the vocabulary's side, and its rest
             GradP first = w, rest = w;
             (DV ? first.n : first.m) = c;
@@ -1123,7 +1185,7 @@ int piece(const BackP &b) {
         h.fixed = b.fixed;
         if (int rc = product<E, false, !DV>(h, b.sh)) return rc;
         if (b.hslab && b.last) {
-            const LeftP left{p.left, p.tokens, static_cast<const uint16_t *>(a->weight), a->ldw, DV};
+            const LeftP left{b.hleft ? p.left : nullptr, p.tokens, static_cast<const uint16_t *>(a->weight), a->ldw, DV};
             if (int rc = fold<E>(h, b.sh.splits, out, left)) return rc;
         }
     }
@@ -1150,15 +1212,14 @@ int backward(const NtRlReadoutStatsGradArgs *a) {
     const int64_t cols = piece_cols(V, most);
     // dH: [rows, dim], k the piece's columns; dW: [vocab, dim] or [dim, vocab], k the rows
     const int64_t width = std::min(cols, V);
-    const bool kept = R <= kLeftRows;
     const Plan sh = plan(R, d, round_up(width, 8) * 2, true);
-    const Size most_w = kept ? Size::kMedium : Size::kLarge;
-    const Plan sw = dv ? plan(d, width, R * 2, true, most_w) : plan(width, d, R * 2, true, most_w);
-    const bool hslab = sh.splits > 1 || cols < V || kept;
+    const Plan sw = dv ? plan(d, width, R * 2, true) : plan(width, d, R * 2, true);
+    const bool hleft = !dv || R <= kColumnRows, hslab = hleft || sh.splits > 1 || cols < V;
     Scratch s;
     const int o_h = s.add(hdirect ? 0 : R * kp * 2), o_hs = s.add(a->grad_weight ? R * kp * 2 : 0);
     const int o_w = s.add(wdirect ? 0 : (dv ? d * cols : cols * kp) * 2);
-    const int o_coef = s.add(R * 16), o_left = s.add(kept ? R * 4 : 0), o_up = s.add(f16 ? R * 4 : 0), o_top = s.add(f16 ? 4 : 0);
+    const int o_coef = s.add(R * 16), o_left = s.add(R * 4), o_up = s.add(f16 ? R * 4 : 0), o_top = s.add(f16 ? 4 : 0);
+    const int o_place = s.add(ceil_div(V, kBucket) * 8), o_listed = s.add(R * 4);
     const int o_g = s.add(R * cols * 2);
     const int o_sh = s.add(a->grad_hidden && hslab ? sh.splits * R * d * 4 : 0);
     const int o_sw = s.add(a->grad_weight && sw.splits > 1 ? sw.splits * std::min(cols, V) * d * 4 : 0);
@@ -1179,10 +1240,13 @@ int backward(const NtRlReadoutStatsGradArgs *a) {
     c.f32mask = a->mask_kind == NT_MASK_F32;
     c.f16 = f16;
     c.coef = s.at<float4>(o_coef);
-    c.left = kept ? s.at<float>(o_left) : nullptr;
+    c.left = s.at<float>(o_left);
     c.up = f16 ? s.at<float>(o_up) : nullptr;
     c.top = top;
-    hipLaunchKernelGGL(k_readout_coef, dim3(unsigned(std::min<int64_t>(ceil_div(R, 1024), 256))), dim3(1024), 0, ctx().stream, c);
+    c.coefs = unsigned(std::min<int64_t>(ceil_div(R, 1024), 256));
+    c.place = s.at<int2>(o_place);
+    c.listed = s.at<uint32_t>(o_listed);
+    hipLaunchKernelGGL(k_readout_coef, dim3(c.coefs + unsigned(ceil_div(V, kBucket))), dim3(1024), 0, ctx().stream, c);
     if (int rc = launched("k_readout_coef")) return rc;
     if (a->grad_weight && f16) {
         hipLaunchKernelGGL(k_readout_top, dim3(unsigned(ceil_div(R, 4))), dim3(256), 0, ctx().stream,
@@ -1215,8 +1279,8 @@ int backward(const NtRlReadoutStatsGradArgs *a) {
         p.v0 = v0;
         p.ldg = p.gbytes = round_up(n, 8) * 2;
         p.mask = mask_at(a->mask_kind, a->mask, a->mask_ld, v0);
-        BackP b{a, p, sh, sw, hslab, s.at<uint8_t>(o_hs), kp * 2, s.at<float>(o_sh), s.at<float>(o_sw), up, top, fixed,
-                v0 + cols >= V};
+        BackP b{a, p, sh, sw, hslab, hleft, c.place, c.listed, s.at<uint8_t>(o_hs), kp * 2, s.at<float>(o_sh), s.at<float>(o_sw),
+                up, top, fixed, v0 + cols >= V};
         const int rc = dv ? (f16 ? piece<F16, true>(b) : piece<Bf16, true>(b)) : (f16 ? piece<F16, false>(b) : piece<Bf16, false>(b));
         if (rc) return rc;
     }

@@ -681,8 +681,8 @@ def test_no_seeds(shape):
     assert lp.shape == ent.shape == (0, 5) and gh.shape == (0, 5, 16) and gw.shape == (0, 16, 300)
 
 
-# Every tile, split k and unsplit, of each gradient's product (dH's without a split written as it is, with one through slabs),
-# and dW's columns in whole rounds with a rest beside them: what each takes is asserted in tests/test_tile_plan.py.
+# Every tile, split k and unsplit, of each gradient's product (unsplit: dW, and dH of a DV weight, written as they are), and
+# dW's columns in whole rounds with a rest beside them: what each takes is asserted in tests/test_tile_plan.py.
 PLANS = [(520, 136, 40, "bf16", "dv", "f32"), (520, 130, 40, "f16", "vd", "none"), (1030, 130, 40, "bf16", "dv", "u8"),
          (520, 1003, 40, "f16", "vd", "none"), (4100, 130, 1001, "f16", "dv", "none"), (4100, 8200, 40, "bf16", "vd", "u8_shared"),
          (3000, 130, 4100, "bf16", "dv", "none"), (4100, 130, 4100, "f16", "dv", "f32_shared"), (520, 33000, 40, "bf16", "vd", "none"),
@@ -718,3 +718,47 @@ def test_a_rows_scores_are_the_same_by_every_tile(rows, V, d, few, layout):
     part = nr.readout_score_with_stats(given(c.h[at]), w, c.tau, m, given(c.tokens[at]), layout=layout)
     for a, b in ((full[0], part[0]), (full[1], part[1]), (full[2].lse_base, part[2].lse_base), (full[2].lse_rest, part[2].lse_rest)):
         assert np.array_equal(a.to_numpy()[at.numpy()], b.to_numpy())
+
+
+@pytest.mark.parametrize("dtype,layout", [("bf16", "dv"), ("bf16", "vd"), ("f16", "dv"), ("f16", "vd")])
+@pytest.mark.parametrize("rows,V,d,live", [(700, 3001, 264, 700), (2100, 9000, 520, 2100), (2100, 9000, 520, 40), (5000, 40000, 72, 300),
+                                           (130, 3001, 264, 7), (600, 70, 40, 600)])
+def test_the_tokens_entries_are_whole_however_many_rows(rows, V, d, live, dtype, layout):
+    """The gradients' error in norm: the written values' own rounding (a half step u at the most, u / sqrt(3) of it in
+    the mean) and that of G's entries off the tokens, whatever the number of rows, of them those that something flows
+    through, and a few upstream gradients far larger than the others. (dH of a DV weight past 512 rows: each row by a factor
+    within u of 1 besides, another u / sqrt(3) at the most.)"""
+    c = Case(rows, V, d, dtype, layout, entropy=False)
+    g = torch.Generator().manual_seed(rows + live)
+    c.g_logp = torch.randn(rows, generator=g).exp() * (8.0 if dtype == "f16" else 1.0)
+    c.g_logp[torch.randperm(rows, generator=g)[live:]] = 0.0
+    got = {k: values(v).cuda() for k, v in c.run().items() if k.startswith("grad")}
+    h, w = c.h.double().cuda(), c.w.double().cuda()
+    w = w.t() if layout == "vd" else w
+    gl = c.g_logp.double().cuda()[:, None]
+    G = torch.softmax(h @ w, 1).mul_(-gl)
+    G[torch.arange(rows, device="cuda"), c.tokens.long().cuda()] += gl[:, 0]
+    gw = h.t() @ G
+    for name, want in (("grad_hidden", G @ w.t()), ("grad_weight", gw if layout == "dv" else gw.t())):
+        off = (got[name] - want).norm() / want.norm()
+        most = 0.85 if name == "grad_hidden" and layout == "dv" and rows > 512 else 0.6
+        assert off <= most * HALF_STEP[dtype], (name, float(off) / HALF_STEP[dtype])
+
+
+def test_every_row_has_one_of_two_tokens():
+    """All rows in one 256 of the vocabulary, at each tile."""
+    for rows, V, d, layout in ((9000, 400, 40, "vd"), (14000, 300, 520, "dv"), (30000, 256, 1032, "vd")):
+        c = Case(rows, V, d, "bf16", layout, entropy=False)
+        c.tokens[:] = V - 3
+        c.tokens[::7] = V - 1
+        got = c.run()
+        for name in ("h", "w", "tokens", "g_logp", "g_entropy", "add"):
+            setattr(c, name, getattr(c, name).to("cuda"))
+        device = torch.get_default_device()
+        torch.set_default_device("cuda")
+        try:
+            want, tol = c.want()
+        finally:
+            torch.set_default_device(device)
+        for k in got:
+            agree(values(got[k]).to("cuda"), want[k], tol[k], k)

@@ -56,11 +56,10 @@ def readout(rows, V, d, layout):
     whole rounds; dH's tile and splits; dW's tile, splits and columns in whole rounds)."""
     kp = (d + 7) // 8 * 8
     wide = (V + 7) // 8 * 8
-    kept = rows <= 512
     assert (V + 255) // 256 * 256 * rows <= 1 << 28
     logits = plan(rows, V, kp * 2, False)[0], whole_rounds(rows, V, kp * 2)
     hidden = plan(rows, d, wide * 2, True)
     shape = (d, V) if layout == "dv" else (V, d)
-    weight = plan(*shape, rows * 2, True, MEDIUM if kept else LARGE)
-    cut = 0 if weight[2] > 1 or kept else whole_rounds(d, V, rows * 2)
+    weight = plan(*shape, rows * 2, True)
+    cut = 0 if weight[2] > 1 else whole_rounds(d, V, rows * 2)
     return logits, (hidden[0], hidden[2]), (weight[0], weight[2], cut)
