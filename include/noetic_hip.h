@@ -329,8 +329,8 @@ int nt_hip_rl_readout_score_stats(const NtRlReadoutStatsArgs *a);
  *   grad_hidden = G W^T  [rows, grad_hidden_ld],   grad_weight = H^T G, laid out as the weight.
  * The logits are computed again, a piece of the vocabulary at a time; G, at most 512 MiB of it (256 columns
  * at the least), is rounded to the operands' type (what that leaves of a row's entry at its token goes into both
- * gradients; into grad_hidden of a [dim, vocab] weight for up to 512 rows), every sum is f32 and in a fixed order. The
- * gradients overlap no input. A row whose
+ * gradients; of a [dim, vocab] weight past 512 rows, into grad_hidden as a scale of the row within 2^-9 of 1), every
+ * sum is f32 and in a fixed order. The gradients overlap no input. A row whose
  * upstream gradients are zero, and one that has no allowed token, adds nothing, whatever its hidden states
  * hold; a token outside [0, vocab) has no log-probability to differentiate. rows 0 gives a zero
  * grad_weight. Inputs as the forward's, with its outputs. */

@@ -27,13 +27,13 @@ struct Plan {
     double cost;          // us
 };
 
-// The tile of the least cost (`most`: and at most that size) for `kb` bytes of k, split where `split` allows it: rounds of the workgroups that run
+// The tile of the least cost for `kb` bytes of k, split where `split` allows it: rounds of the workgroups that run
 // at once, each its stages of 64 bytes and its output. Measured (us a stage, a round full): 0.92, 0.57 and 0.36 for
 // Large, Medium and Small, or 0.33 and 0.25 in a round of one workgroup a CU; an output of Large about 6 us, of
 // Medium and Small less than their share of it, since it goes on beside the other workgroup's products; the slabs of a
 // split k 4 us, 0.15 a slab and their bytes, written and read, at 4 TB/s. So 4096 x 128256 takes Large, 333 x 50257 x 1001 Medium (a
 // pass over the logits 99 -> 77 us), 64 rows Small (29 -> 16 us at 32000 x 1024).
-inline Plan plan(int64_t m, int64_t n, int64_t kb, bool split, Size most = Size::kLarge) {
+inline Plan plan(int64_t m, int64_t n, int64_t kb, bool split) {
     if (kb < 64) kb = 64;
     struct Kind {
         Size size;
@@ -45,7 +45,6 @@ inline Plan plan(int64_t m, int64_t n, int64_t kb, bool split, Size most = Size:
                                  {Size::kSmall, Small::kRows, Small::kCols, 512, 0.36, 0.25, 1.5}};
     Plan best{};
     for (const Kind &c : kinds) {
-        if (c.size > most) continue;
         const int64_t tiles = ceil_div(m, c.rows) * ceil_div(n, c.cols);
         for (int64_t r = 0; r <= 4; r++) {  // unsplit, and the splits that give every CU one to four workgroups
             int64_t s = r == 0 ? 1 : 256 * r / tiles;

@@ -24,7 +24,7 @@
 //  would show in the gradients as their own does, so what it left goes into them, times the row of H into dW as a stage
 //  more of its product (LeftRows) and times the token's row of W into dH as its sums are folded: the error is the written
 //  values' own, 0.0017 of the norm for bf16, where it was 0.0023 (2048 x 4096 x 50304 2.93 -> 2.96 ms, 4096 x 4096 x 128256
-//  13.5 -> 13.6). A DV weight's columns are read for it up to 512 rows; dH of more has 0.0023 (kColumnRows).
+//  13.5 -> 13.6). A DV weight's columns are read for it up to 512 rows; more rows of dH are scaled for it (kColumnRows).
 //  For f16, whose range G would leave, a row of G is held in units of 2^(e - 14), 2^e over |g_logp| + 16 |g_entropy|
 //  (p |ln p + entropy| is under 14 for a vocabulary of 2^20), and for dW the row of H is scaled by 2^e and the one power
 //  of two that puts the largest value of all scaled rows under 2^15: what rows far below the largest lose to f16's
@@ -179,7 +179,8 @@ struct PieceP {
     const float4 *coef;       // [rows] {the largest value (+inf: nothing flows), a, b, the token's term}
     uint8_t *g;               // [rows, ldg bytes], of which gbytes are written: zeros past n
     int64_t ldg, gbytes;
-    float *left;              // [rows] what the rounding of G's entry at the row's token left
+    float *left;              // [rows] what the rounding of G's entry at the row's token left (first: see CoefP)
+    float *turn;              // [rows] what makes up for it in the row of dH (1: nothing), or null
 };
 
 template <class T, bool BTR>
@@ -370,7 +371,8 @@ struct CoefP {
     double tau;
     int f32mask, f16;
     float4 *coef;
-    float *left;   // [rows] zeros here
+    float *left;   // [rows] 0 where nothing flows; else 8 |g_entropy| in G's units until G is there
+    float *turn;   // [rows] ones here, or null
     unsigned coefs;  // workgroups; those behind them list the tokens
     int2 *place;   // [vocab / 256] a bucket's first entry in `listed`, and how many
     uint32_t *listed;  // [rows] row << 8 | token % 256
@@ -451,7 +453,9 @@ __global__ __launch_bounds__(1024) void k_readout_coef(CoefP p) {
             unit = 1.0 / p.tau;
         }
         if (p.f16) p.up[r] = up;
-        p.left[r] = 0.0f;
+        const bool term = !dead && tok >= 0 && tok < p.vocab;
+        p.left[r] = term ? float(8.0 * fabs(ge) * unit) : 0.0f;
+        if (p.turn) p.turn[r] = 1.0f;
         const float a = float(-(gl + ge * (h - rest)) * q * unit), b = float(-ge * kLn2 * q * unit);
         p.coef[r] = dead ? float4{INFINITY, 0.0f, 0.0f, 0.0f} : float4{top_x, a, b, float(gl * unit)};
     }
@@ -568,6 +572,7 @@ __global__ __launch_bounds__(S::kThreads, 1) void k_readout_g(PieceP p) {
         const bool dead = k.x == INFINITY;
         // (of 32 rows few have their token among this wave's columns)
         const bool mine = __any(tok[i] >= 0 && tok[i] < 32 * TN);
+        float at_token = 0.0f, held = 0.0f;  // the row's entry at its token, and as it is written
         u32x2 v[4 * TN];
         float x[4 * TN][4];
 #pragma unroll
@@ -593,13 +598,18 @@ __global__ __launch_bounds__(S::kThreads, 1) void k_readout_g(PieceP p) {
             if (mine)
 #pragma unroll
                 for (int e = 0; e < 4; e++)
-                    if (tok[i] == 8 * q + e) g[e] += k.w;
+                    if (tok[i] == 8 * q + e) at_token = g[e] += k.w;
             v[q] = dead ? u32x2{0, 0} : u32x2{pair16<E>(g[0], g[1]), pair16<E>(g[2], g[3])};
             if (mine)
 #pragma unroll
                 for (int e = 0; e < 4; e++)
-                    if (tok[i] == 8 * q + e && !dead)
-                        p.left[row0 + lane % 32] = g[e] - widened<E>((e < 2 ? v[q].x : v[q].y) >> (16 * (e % 2)) & 0xffffu);
+                    if (tok[i] == 8 * q + e) held = widened<E>((e < 2 ? v[q].x : v[q].y) >> (16 * (e % 2)) & 0xffffu);
+        }
+        if (mine && tok[i] >= 0 && tok[i] < 32 * TN && (tok[i] & 4) == 0 && !dead) {
+            const int64_t r = row0 + lane % 32;
+            const float left = at_token - held;
+            if (p.turn && fabsf(held) > p.left[r] && fabsf(left) <= 0x1p-8f * fabsf(held)) p.turn[r] = at_token / held;
+            p.left[r] = left;
         }
         const int rows = p.rows - row0 < 32 ? int(p.rows - row0) : 32, have = bytes < 64 * TN ? int(bytes) : 64 * TN;
         uint8_t *o = p.g + row0 * p.ldg + (in * T::BN + 32 * TN * wn) * 2;
@@ -620,6 +630,7 @@ struct GradP {
     float *slab;              // [splits][m][n] f32
     int add;
     const float *row_scale;   // f16: [m] or null
+    const float *turn;        // [m] or null: another scale of the rows (dH)
     const int *top;           // f16: [1] or null
     float fixed;
     // dW: what the rounding of G left of the tokens' entries
@@ -728,7 +739,9 @@ __global__ __launch_bounds__(S::kThreads, S::TM == 1 ? 2 : 1) void k_readout_gra
 #pragma unroll
     for (int i = 0; i < TM; i++) {
         const int64_t row = m0 + 32 * (TM * wm + i) + lane % 32;
-        f[i] = p.row_scale ? p.row_scale[row < p.m ? row : p.m - 1] * whole : whole;
+        const int64_t r = row < p.m ? row : p.m - 1;
+        f[i] = p.row_scale ? p.row_scale[r] * whole : whole;
+        if (!kDW && p.turn) f[i] *= p.turn[r];
     }
 #pragma unroll
     for (int i = 0; i < TM; i++) {
@@ -784,13 +797,17 @@ struct LeftP {
 };
 
 // Rows up to which a DV weight's columns are read for it: a column's every value is a line of its own, and for 2048 rows of
-// dim 4096 (V 50304) they took 90 us of 2930. Without it a row of dH is off by a factor within 2^-9 of 1 (bf16; f16 2^-12),
-// the rounding of its G at its token, beside its values' own.
+// dim 4096 (V 50304) they took 90 us of 2930. A row of dH of more is scaled instead, by the exact entry over the rounded
+// one: its token's part is then right, and the others' off by that factor, within 2^-9 of 1 (bf16; f16 2^-12). Without an
+// entropy's gradient the others are no larger than the token's (a row of G sums to zero, so their part is the token's entry
+// times a mean of W's columns); with one the row is scaled where its token's entry is over 8 |g_entropy|, which the other
+// entries' norm by p (ln p + entropy), sqrt(max p Var ln p) at the most, is under up to vocabularies of 2^20.
 constexpr int64_t kColumnRows = 512;
 
 template <class E>
 __global__ __launch_bounds__(256) void k_readout_fold(const float *slab, int splits, int64_t m, int64_t n, LeftP p, uint16_t *out,
-                                                      int64_t ldo, const float *row_scale, const int *top, float fixed) {
+                                                      int64_t ldo, const float *row_scale, const float *turn, const int *top,
+                                                      float fixed) {
     const int64_t per = (n + 3) / 4, total = m * per;
     for (int64_t i = blockIdx.x * int64_t(256) + threadIdx.x; i < total; i += int64_t(gridDim.x) * 256) {
         const int64_t r = i / per, c = (i - r * per) * 4;
@@ -817,6 +834,7 @@ __global__ __launch_bounds__(256) void k_readout_fold(const float *slab, int spl
             for (int e = 0; e < have; e++) x[e] += at(z)[e];
         float f = top ? ldexpf(fixed, -lift(top)) : fixed;
         if (row_scale) f *= row_scale[r];
+        if (turn) f *= turn[r];
         uint16_t *o = out + r * ldo + c;
         const uint32_t w[2] = {pair16<E>(x[0] * f, x[1] * f), pair16<E>(x[2] * f, x[3] * f)};
         if (have == 4) __builtin_memcpy(o, w, 8);
@@ -1085,7 +1103,7 @@ template <class E>
 int fold(const GradP &p, int64_t splits, uint16_t *out, const LeftP &left = {}) {
     const int64_t n = p.m * ceil_div(p.n, 4);
     hipLaunchKernelGGL(k_readout_fold<E>, dim3(unsigned(std::min<int64_t>(ceil_div(n, 256), 8192))), dim3(256), 0,
-                       ctx().stream, p.slab, int(splits), p.m, p.n, left, out, p.ldo, p.row_scale, p.top, p.fixed);
+                       ctx().stream, p.slab, int(splits), p.m, p.n, left, out, p.ldo, p.row_scale, p.turn, p.top, p.fixed);
     return launched("k_readout_fold");
 }
 
@@ -1182,6 +1200,7 @@ int piece(const BackP &b) {
         h.slab = b.slab_h;
         h.add = p.v0 > 0;
         h.row_scale = b.up;
+        h.turn = p.turn;
         h.fixed = b.fixed;
         if (int rc = product<E, false, !DV>(h, b.sh)) return rc;
         if (b.hslab && b.last) {
@@ -1219,7 +1238,9 @@ int backward(const NtRlReadoutStatsGradArgs *a) {
     const int o_h = s.add(hdirect ? 0 : R * kp * 2), o_hs = s.add(a->grad_weight ? R * kp * 2 : 0);
     const int o_w = s.add(wdirect ? 0 : (dv ? d * cols : cols * kp) * 2);
     const int o_coef = s.add(R * 16), o_left = s.add(R * 4), o_up = s.add(f16 ? R * 4 : 0), o_top = s.add(f16 ? 4 : 0);
-    const int o_place = s.add(ceil_div(V, kBucket) * 8), o_listed = s.add(R * 4);
+    const int64_t buckets = a->grad_weight ? ceil_div(V, kBucket) : 0;
+    const int o_turn = s.add(a->grad_hidden && !hleft ? R * 4 : 0);
+    const int o_place = s.add(buckets * 8), o_listed = s.add(buckets ? R * 4 : 0);
     const int o_g = s.add(R * cols * 2);
     const int o_sh = s.add(a->grad_hidden && hslab ? sh.splits * R * d * 4 : 0);
     const int o_sw = s.add(a->grad_weight && sw.splits > 1 ? sw.splits * std::min(cols, V) * d * 4 : 0);
@@ -1241,12 +1262,13 @@ int backward(const NtRlReadoutStatsGradArgs *a) {
     c.f16 = f16;
     c.coef = s.at<float4>(o_coef);
     c.left = s.at<float>(o_left);
+    c.turn = a->grad_hidden && !hleft ? s.at<float>(o_turn) : nullptr;
     c.up = f16 ? s.at<float>(o_up) : nullptr;
     c.top = top;
     c.coefs = unsigned(std::min<int64_t>(ceil_div(R, 1024), 256));
     c.place = s.at<int2>(o_place);
     c.listed = s.at<uint32_t>(o_listed);
-    hipLaunchKernelGGL(k_readout_coef, dim3(c.coefs + unsigned(ceil_div(V, kBucket))), dim3(1024), 0, ctx().stream, c);
+    hipLaunchKernelGGL(k_readout_coef, dim3(c.coefs + unsigned(buckets)), dim3(1024), 0, ctx().stream, c);
     if (int rc = launched("k_readout_coef")) return rc;
     if (a->grad_weight && f16) {
         hipLaunchKernelGGL(k_readout_top, dim3(unsigned(ceil_div(R, 4))), dim3(256), 0, ctx().stream,
@@ -1272,6 +1294,7 @@ int backward(const NtRlReadoutStatsGradArgs *a) {
     p.coef = c.coef;
     p.g = s.at<uint8_t>(o_g);
     p.left = c.left;
+    p.turn = c.turn;
     for (int64_t v0 = 0; v0 < V; v0 += cols) {
         const int64_t n = std::min(cols, V - v0);
         if (int rc = piece_weight(a->weight, dv, wdirect, v0, n, d, a->ldw, s.at<uint8_t>(o_w), &p)) return rc;

@@ -20,11 +20,10 @@ def sizes(n, seed):
 def test_splits_cover_k():
     for m, n, kb in sizes(3000, 1):
         for split in (False, True):
-            for most in (SMALL, MEDIUM, LARGE):
-                size, per, splits = plan(m, n, kb, split, most)
-                assert size <= most and per % 64 == 0 and 1 <= splits <= 64
-                assert splits * per >= kb > (splits - 1) * per or splits == 1
-                assert splits == 1 or (split and per >= 512)
+            _, per, splits = plan(m, n, kb, split)
+            assert per % 64 == 0 and 1 <= splits <= 64
+            assert splits * per >= kb > (splits - 1) * per or splits == 1
+            assert splits == 1 or (split and per >= 512)
 
 
 def test_few_tiles_are_split():

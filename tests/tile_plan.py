@@ -11,8 +11,8 @@ SMALL, MEDIUM, LARGE = range(3)
 SOURCE = """
 #include "nt_plan.hpp"
 using namespace nt::tile;
-extern "C" void plan_of(int64_t m, int64_t n, int64_t kb, int split, int most, int64_t *out) {
-    const Plan p = plan(m, n, kb, split != 0, Size(most));
+extern "C" void plan_of(int64_t m, int64_t n, int64_t kb, int split, int64_t *out) {
+    const Plan p = plan(m, n, kb, split != 0);
     out[0] = int64_t(p.size), out[1] = p.per, out[2] = p.splits;
 }
 extern "C" int64_t whole(int64_t m, int64_t n, int64_t kb) { return whole_rounds(m, n, kb); }
@@ -28,16 +28,16 @@ def _lib():
     subprocess.run(["g++", "-std=c++17", "-O1", "-shared", "-fPIC", "-I", os.path.join(ROOT, "noetic-tensor_amd", "csrc"), src,
                     "-o", so], check=True)
     lib = C.CDLL(so)
-    lib.plan_of.argtypes = [C.c_int64, C.c_int64, C.c_int64, C.c_int, C.c_int, C.POINTER(C.c_int64)]
+    lib.plan_of.argtypes = [C.c_int64, C.c_int64, C.c_int64, C.c_int, C.POINTER(C.c_int64)]
     lib.plan_of.restype = None
     lib.whole.argtypes, lib.whole.restype = [C.c_int64] * 3, C.c_int64
     return lib
 
 
-def plan(m, n, kb, split, most=LARGE):
+def plan(m, n, kb, split):
     """(tile, bytes of k of a split, splits) of [m, k] x [n, k], kb bytes of k."""
     out = (C.c_int64 * 3)()
-    _lib().plan_of(m, n, kb, int(split), most, out)
+    _lib().plan_of(m, n, kb, int(split), out)
     return tuple(out)
 
 
