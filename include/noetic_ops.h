@@ -187,7 +187,7 @@ int nt_hip_dequantize_int8(const int8_t *q, const float *scale, int64_t rows, in
  * (k <= 131071), then rounded to f32, scaled, and rounded into dtype (f32, bf16 or f16). Row strides lda, ldb
  * (at most 2^22) and ldo in elements. Operands whose base and stride are not multiples of 16, or whose k is not, are first
  * copied to scratch rows that are; where the output's tiles are few, k is split and the splits' sums (32 bits) go through
- * scratch, which changes no result. k = 0 gives zeros. */
+ * scratch, which changes no result. Under stream capture a call with 1 MiB of scratch or more is refused. k = 0 gives zeros. */
 int nt_hip_matmul_int8(const int8_t *a, int64_t lda, const float *a_scale, const int8_t *b, int64_t ldb, const float *b_scale,
                        int64_t m, int64_t n, int64_t k, int32_t dtype, void *out, int64_t ldo);
 

@@ -666,6 +666,11 @@ int product(const int8_t *a, int64_t lda, const float *sa, const int8_t *b, int6
     const bool slabs = m > 4 && s.splits > 1;
     const int64_t need = abytes + bbytes + (slabs ? s.splits * m * n * 4 : 0);
     void *ws = nullptr;
+    bool cap = false;
+    if (need >= (int64_t(1) << 20))
+        if (int rc = stream_capturing(&cap)) return rc;
+    if (cap)  // (as the training readout's: replays with scratch of this size have faulted)
+        return fail(NT_E_UNSUPPORTED, "matmul_int8: " + std::to_string(need) + " bytes of scratch under stream capture (under 1 MiB)");
     if (need > 0)
         if (int rc = scratch_alloc(size_t(need), &ws)) return rc;
     uint8_t *pa = static_cast<uint8_t *>(ws), *pb = pa + abytes;

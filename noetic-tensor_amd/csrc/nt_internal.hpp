@@ -42,6 +42,9 @@ int enter_nofree(std::unique_lock<std::mutex> *out);
 int scratch_alloc(size_t bytes, void **out);
 int scratch_release(void *ptr);
 
+// Whether the library stream is being captured into a graph.
+int stream_capturing(bool *out);
+
 // Clear n u32 words of device memory with a kernel on the library stream (a kernel, so that a
 // caller capturing the stream into a graph records no memset node).
 int zero_words(uint32_t *p, size_t n);

@@ -860,7 +860,16 @@ struct Scratch {
         if (size[n] < kAlone) together += size[n];
         return n++;
     }
-    int allocate() {
+    // `large`: the call takes 256 x 256 tiles. Under stream capture such a call, and one with a block of its own, is refused: a
+    // captured step of 2100 x 512 x 32768 faulted in its replays, for a cause not found, where it runs as it should
+    // outside of a graph; captured steps of smaller tiles whose scratch is one block replay rightly.
+    int allocate(const char *who, bool large) {
+        bool cap = false;
+        if (int rc = stream_capturing(&cap)) return rc;
+        for (int i = 0; i < n; i++) large |= size[i] >= kAlone;
+        if (cap && large)
+            return fail(NT_E_UNSUPPORTED, std::string(who) + ": too large for stream capture (256 x 256 tiles, or scratch of 1 MiB "
+                                                             "and more)");
         if (int rc = scratch_alloc(together, &shared)) return rc;
         uint8_t *at = static_cast<uint8_t *>(shared);
         for (int i = 0; i < n; i++) {
@@ -1044,7 +1053,7 @@ int forward(const NtRlReadoutStatsArgs *a) {
     const int o_w = s.add(wdirect ? 0 : (dv ? d * cols : cols * kp) * 2);
     const int o_ref = s.add(blocks * rows_p * 4), o_sum = s.add(blocks * rows_p * 4);
     const int o_es = s.add(a->entropy ? blocks * rows_p * 4 : 0), o_x = s.add(R * 4);
-    if (int rc = s.allocate()) return rc;
+    if (int rc = s.allocate("nt_hip_rl_readout_score_stats", plan(R, std::min(cols, V), kp * 2, false).size == Size::kLarge)) return rc;
     PieceP p{};
     p.h = static_cast<const uint8_t *>(a->hidden);
     p.ldh = a->ldh * 2;
@@ -1244,7 +1253,9 @@ int backward(const NtRlReadoutStatsGradArgs *a) {
     const int o_g = s.add(R * cols * 2);
     const int o_sh = s.add(a->grad_hidden && hslab ? sh.splits * R * d * 4 : 0);
     const int o_sw = s.add(a->grad_weight && sw.splits > 1 ? sw.splits * std::min(cols, V) * d * 4 : 0);
-    if (int rc = s.allocate()) return rc;
+    const bool large = plan(R, width, kp * 2, false).size == Size::kLarge || (a->grad_hidden && sh.size == Size::kLarge) ||
+                       (a->grad_weight && sw.size == Size::kLarge);
+    if (int rc = s.allocate("nt_hip_rl_readout_score_backward", large)) return rc;
     const float *up = f16 ? s.at<float>(o_up) : nullptr;
     int *top = f16 ? s.at<int>(o_top) : nullptr;
     const float fixed = f16 ? float(ldexp(1.0, -14) / a->temperature) : 1.0f;

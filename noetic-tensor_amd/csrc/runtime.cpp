@@ -66,8 +66,7 @@ struct KeptBlock {
     bool used;
 };
 
-// Whether the library stream is being captured.
-static int capturing(bool *out) {
+int stream_capturing(bool *out) {
     hipStreamCaptureStatus cap = hipStreamCaptureStatusNone;
     if (int rc = hip_check(hipStreamIsCapturing(ctx().stream, &cap), "hipStreamIsCapturing")) return rc;
     *out = cap != hipStreamCaptureStatusNone;
@@ -122,7 +121,7 @@ static int take_block(size_t bytes, void **out) {
     size_t size = bytes;
     int cls = -1;
     bool cap = false;
-    if (int rc = capturing(&cap)) return rc;
+    if (int rc = stream_capturing(&cap)) return rc;
     if (bytes <= kKeepBlock && !cap) {
         cls = size_class(bytes, &size);
         if (!k.lists[cls].empty()) {
@@ -156,7 +155,7 @@ static int give_block(void *p, bool in_capture) {
     k.bytes += class_bytes(it->second.cls);
     if (k.bytes <= kKeepTotal) return 0;
     bool cap = false;
-    if (int rc = capturing(&cap)) return rc;
+    if (int rc = stream_capturing(&cap)) return rc;
     if (cap) return 0;  // (a later release trims them)
     // the larger blocks first: from 1 MiB (class 8 * 20) up, then all
     if (int rc = drop_kept(8 * 20)) return rc;
@@ -369,7 +368,7 @@ int nt_hip_alloc(size_t bytes, void **out) {
 int nt_hip_free(void *ptr) {
     if (!ptr) return 0;
     bool cap = false;
-    if (ctx().stream && capturing(&cap)) cap = true;  // (not known: as if it were)
+    if (ctx().stream && stream_capturing(&cap)) cap = true;  // (not known: as if it were)
     std::lock_guard<std::mutex> pl(g_pending_mu);
     g_pending.push_back(Pending{ptr, cap});
     return 0;

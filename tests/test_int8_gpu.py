@@ -283,3 +283,23 @@ def test_captured_calls_replay():
         nr.sync()
         assert np.array_equal(y.to_numpy(), want)
     cap.close()
+
+
+def test_a_product_with_much_scratch_is_refused_under_capture():
+    """k of no whole chunks against a weight of 1.1 MB, whose copy is scratch: refused under stream capture before
+    anything is queued, and right outside of one."""
+    m, n, k = 8, 1100, 1001
+    g = torch.Generator().manual_seed(5)
+    a, b = (torch.randint(-127, 128, (r, k), generator=g, dtype=torch.int8) for r in (m, n))
+    sa, sb = torch.rand(m, generator=g), torch.rand(n, generator=g)
+    ta, tb, tsa, tsb, y = given(a), given(b), given(sa), given(sb), nr.Tensor((m, n), "f32")
+    call = lambda: nr.lib().nt_hip_matmul_int8(ta.ptr, k, tsa.ptr, tb.ptr, k, tsb.ptr, m, n, k, 0, y.ptr, n)  # noqa: E731
+    nr.sync()
+    cap = Capture()
+    with cap:
+        rc = call()
+        text = nr.lib().nt_hip_last_error().decode()
+    assert rc == -4 and "under stream capture" in text and cap.nodes() == 0
+    cap.close()
+    assert call() == 0
+    agree(y, product(a, sa, b, sb), "f32")

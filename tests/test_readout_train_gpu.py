@@ -792,3 +792,82 @@ def test_rows_of_a_wide_weight_under_an_entropys_gradient(rows, V, d, dtype):
     for k in ("grad_hidden", "grad_weight"):
         off = (values(got[k]).to("cuda") - want[k]).norm() / want[k].norm()
         assert off <= 0.85 * HALF_STEP[dtype], (k, float(off) / HALF_STEP[dtype])  # (sqrt(0.6^2 + 1 / 3))
+
+
+@pytest.mark.parametrize("rows,V,d,dtype,layout,mask", [(2100, 9000, 520, "bf16", "dv", "f32_shared"), (2100, 32768, 512, "bf16", "vd", "none"),
+                                                        (333, 5003, 1001, "f16", "dv", "u8"), (4100, 70000, 72, "bf16", "dv", "none")])
+def test_large_reruns_are_the_same_bytes(rows, V, d, dtype, layout, mask):
+    c = Case(rows, V, d, dtype, layout, mask)
+    a = {k: v.to_numpy() for k, v in c.run().items()}
+    for _ in range(3):
+        b = c.run()
+        for k in a:
+            assert np.array_equal(a[k], b[k].to_numpy()), k
+
+
+@pytest.mark.skip(reason="faulted in a replay (illegal address), its cause not found: such calls are refused under capture")
+def test_captured_calls_of_a_large_step_replay():
+    """The same with 256 x 256 tiles, whole rounds and their rest, a mask and an entropy, replayed over other inputs."""
+    R, V, d = 2100, 32768, 512
+    c = Case(R, V, d, "bf16", "dv", "u8")
+    bufs = [given(x) for x in (c.h, c.w, c.mask, c.tokens, c.g_logp, c.g_entropy)]
+    h, w, m, t, gl, ge = bufs
+    rowf = lambda: nr.Tensor((R,), "f32")  # noqa: E731
+    lp, ent, base, rest, st = rowf(), rowf(), rowf(), rowf(), nr.Tensor((R,), "u8")
+    gh, gw = nr.Tensor((R, d), "bf16"), nr.Tensor((d, V), "bf16")
+    head = (h.ptr, w.ptr, nr.NT_BF16, nr.NT_READOUT_W_DV, R, V, d, d, V, m.ptr, V, nr.NT_MASK_U8, 0, c.tau, t.ptr)
+    a = nr.NtRlReadoutStatsArgs(*head, lp.ptr, ent.ptr, base.ptr, rest.ptr, st.ptr)
+    b = nr.NtRlReadoutStatsGradArgs(*head, base.ptr, rest.ptr, ent.ptr, gl.ptr, ge.ptr, gh.ptr, gw.ptr, d, V)
+
+    def calls():
+        nr._check(nr.lib().nt_hip_rl_readout_score_stats(C.byref(a)), "stats")
+        nr._check(nr.lib().nt_hip_rl_readout_score_backward(C.byref(b)), "backward")
+
+    calls()
+    nr.sync()
+    g = Capture()
+    with g:
+        calls()
+    for k in range(3):
+        other = Case(R, V, d, "bf16", "dv", "u8", seed=k + 1)
+        want = other.run()  # eager, between the replays
+        for dst, src in zip(bufs, (other.h, other.w, other.mask, other.tokens, other.g_logp, other.g_entropy)):
+            s = given(src)
+            view = ops.Layout.contiguous(s.shape)
+            ops.write(dst, view, s, view)
+        g.replay()
+        nr.sync()
+        for name, got in (("logp", lp), ("entropy", ent), ("grad_hidden", gh), ("grad_weight", gw)):
+            assert np.array_equal(got.to_numpy(), want[name].to_numpy()), (k, name)
+    g.close()
+
+
+def test_a_step_too_large_for_capture_is_refused():
+    """256 x 256 tiles, or scratch of 1 MiB and more, under stream capture: refused before anything is queued; the same
+    calls run outside of one, and the next smaller step is captured."""
+    for R, V, d, fits in ((2100, 32768, 512, False), (130, 30016, 64, False), (90, 1000, 64, True)):
+        c = Case(R, V, d, "bf16", "vd")
+        h, w, t, gl, ge = (given(x) for x in (c.h, c.w, c.tokens, c.g_logp, c.g_entropy))
+        rowf = lambda: nr.Tensor((R,), "f32")  # noqa: E731
+        lp, ent, base, rest, st = rowf(), rowf(), rowf(), rowf(), nr.Tensor((R,), "u8")
+        gh, gw = nr.Tensor((R, d), "bf16"), nr.Tensor((V, d), "bf16")
+        head = (h.ptr, w.ptr, nr.NT_BF16, nr.NT_READOUT_W_VD, R, V, d, d, d, None, 0, nr.NT_MASK_NONE, 0, c.tau, t.ptr)
+        a = nr.NtRlReadoutStatsArgs(*head, lp.ptr, ent.ptr, base.ptr, rest.ptr, st.ptr)
+        b = nr.NtRlReadoutStatsGradArgs(*head, base.ptr, rest.ptr, ent.ptr, gl.ptr, ge.ptr, gh.ptr, gw.ptr, d, d)
+        L = nr.lib()
+        assert L.nt_hip_rl_readout_score_stats(C.byref(a)) == 0 and L.nt_hip_rl_readout_score_backward(C.byref(b)) == 0
+        nr.sync()
+        g = Capture()
+        with g:
+            if fits:
+                assert L.nt_hip_rl_readout_score_stats(C.byref(a)) == 0
+            rc = L.nt_hip_rl_readout_score_backward(C.byref(b))
+            text = L.nt_hip_last_error().decode()
+        if fits:
+            assert rc == 0 and g.nodes() > 5
+        else:
+            assert rc == -4 and "too large for stream capture" in text and g.nodes() == 0
+        nr.sync()
+        assert L.nt_hip_rl_readout_score_stats(C.byref(a)) == 0 and L.nt_hip_rl_readout_score_backward(C.byref(b)) == 0
+        nr.sync()
+        g.close()
