@@ -175,7 +175,7 @@ int nt_hip_half_gemm_key(char *buf, size_t cap);
  * and its scale s = max |x| / 127 in f32: q contiguous over the view's shape, scale over its leading
  * dimensions. A row of zeros has scale 0; one that holds a NaN or an infinity has scale NaN and zeros; a row
  * of no elements scale 0. A view whose leading dimensions do not fold into one stride, or whose rows are not
- * contiguous (nor its columns), is first copied to scratch. */
+ * contiguous (nor its columns), is first copied to scratch (under stream capture only under 1 MiB). */
 int nt_hip_quantize_int8(const void *x, const NtLayout *xl, int32_t dtype, int8_t *q, float *scale);
 
 /* out = q scale, the values the 8 bits stand for, rounded to nearest even into dtype: q and out [rows, cols]

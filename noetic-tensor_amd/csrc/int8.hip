@@ -655,6 +655,15 @@ bool aligned(const void *p, int64_t cols, int64_t ld) {
     return reinterpret_cast<uintptr_t>(p) % 16 == 0 && ld % 16 == 0 && cols % 16 == 0;
 }
 
+// Scratch of 1 MiB and more is refused under stream capture, as the training readout's is (rl_readout_train.hip).
+int fits_capture(const char *who, int64_t need) {
+    bool cap = false;
+    if (need < (int64_t(1) << 20)) return 0;
+    if (int rc = stream_capturing(&cap)) return rc;
+    return cap ? fail(NT_E_UNSUPPORTED, std::string(who) + ": " + std::to_string(need) + " bytes of scratch under stream capture (under 1 MiB)")
+               : 0;
+}
+
 constexpr int64_t kMaxK = 131071, kMaxLd = int64_t(1) << 22;
 
 int product(const int8_t *a, int64_t lda, const float *sa, const int8_t *b, int64_t ldb, const float *sb, int64_t m, int64_t n,
@@ -666,11 +675,7 @@ int product(const int8_t *a, int64_t lda, const float *sa, const int8_t *b, int6
     const bool slabs = m > 4 && s.splits > 1;
     const int64_t need = abytes + bbytes + (slabs ? s.splits * m * n * 4 : 0);
     void *ws = nullptr;
-    bool cap = false;
-    if (need >= (int64_t(1) << 20))
-        if (int rc = stream_capturing(&cap)) return rc;
-    if (cap)  // (as the training readout's: replays with scratch of this size have faulted)
-        return fail(NT_E_UNSUPPORTED, "matmul_int8: " + std::to_string(need) + " bytes of scratch under stream capture (under 1 MiB)");
+    if (int rc = fits_capture("matmul_int8", need)) return rc;
     if (need > 0)
         if (int rc = scratch_alloc(size_t(need), &ws)) return rc;
     uint8_t *pa = static_cast<uint8_t *>(ws), *pb = pa + abytes;
@@ -746,6 +751,7 @@ int nt_hip_quantize_int8(const void *x, const NtLayout *xl, int32_t dtype, int8_
     const bool folds = as_rows(xl, &v);
     const bool columns = folds && v.rows > 1 && v.cols > 1 && v.row_stride == 1 && v.col_stride != 1;
     if (!columns && !(folds && (v.col_stride == 1 || v.cols == 1))) {  // any other view: its values in order first
+        if (int rc = fits_capture(who, total * size_of(dtype))) return rc;
         if (int rc = scratch_alloc(size_t(total) * size_of(dtype), &ws)) return rc;
         lk.unlock();
         int rc = nt_hip_copy(x, xl, size_of(dtype), ws);

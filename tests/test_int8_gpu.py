@@ -303,3 +303,13 @@ def test_a_product_with_much_scratch_is_refused_under_capture():
     cap.close()
     assert call() == 0
     agree(y, product(a, sa, b, sb), "f32")
+    x = given(torch.randn(70, 70, 70, generator=g))  # (a view that is neither rows nor columns: its copy is scratch)
+    lay, q, s = ops.Layout.contiguous((70, 70, 70)).swapped(0, 2).c(), nr.Tensor((70, 70, 70), "i8"), nr.Tensor((70, 70), "f32")
+    quantize = lambda: nr.lib().nt_hip_quantize_int8(x.ptr, C.byref(lay), 0, q.ptr, s.ptr)  # noqa: E731
+    nr.sync()
+    cap = Capture()
+    with cap:
+        rc = quantize()
+    assert rc == -4 and cap.nodes() == 0
+    cap.close()
+    assert quantize() == 0
