@@ -8,7 +8,7 @@
 // Quantizing: the quotient's nearest integer, ties to even, of the exact x / s, so that the integers depend on
 // no rounding of the quotient: r = round(x (1/s)) is at most one off next to a border, and the remainder
 // x - r s, exact in one fma, says which side x is on. Bounded by HBM: the values in, a byte each out (4096 x 4096 bf16
-// there and back 25 us of 21 at a copy's rate, 4.73 TB/s; 1024 x 50304 f32 by columns 145 of 109).
+// there and back 25 us of 21 at a copy's rate, 4.73 TB/s; 1024 x 50304 f32 by columns 147 of 109).
 //
 // The product: v_mfma_i32_32x32x32_i8 sums exactly in 32 bits (k up to 131071 keeps |sum| under 2^31), so the
 // only roundings are the sum's to f32, the two scales' products and the output type's. Up to four tokens are bound by the

@@ -23,17 +23,17 @@
 //  written), and for f16 the rows of H below; every sum is f32. A row's entry at its token is most of G, and its rounding
 //  would show in the gradients as their own does, so what it left goes into them, times the row of H into dW as a stage
 //  more of its product (LeftRows) and times the token's row of W into dH as its sums are folded: the error is the written
-//  values' own, 0.0017 of the norm for bf16, where it was 0.0023 (2048 x 4096 x 50304 2.93 -> 2.96 ms, 4096 x 4096 x 128256
-//  13.5 -> 13.6). A DV weight's columns are read for it up to 512 rows; more rows of dH are scaled for it (kColumnRows).
+//  values' own, 0.0017 of the norm for bf16, where it was 0.0023 (2048 x 4096 x 50304 +1%, 4096 x 4096 x
+//  128256 +0.8%). A DV weight's columns are read for it up to 512 rows; more rows of dH are scaled for it (kColumnRows).
 //  For f16, whose range G would leave, a row of G is held in units of 2^(e - 14), 2^e over |g_logp| + 16 |g_entropy|
 //  (p |ln p + entropy| is under 14 for a vocabulary of 2^20), and for dW the row of H is scaled by 2^e and the one power
 //  of two that puts the largest value of all scaled rows under 2^15: what rows far below the largest lose to f16's
 //  smallest steps is 2^-40 of that value, less than the smallest step of a gradient that holds the largest row's.
 //
-//  Bound by the matrix cores for many rows, and those by power: 4096 x 4096 x 128256 bf16 is scored in 3.2-3.3 ms (1.33
-//  PFLOP/s at a clock near 1.5 GHz; a library product alone 2.99) and scored and differentiated in 13.4 ms (1.29 at its 8
-//  R V dim). Few rows are bound by the weight's bytes and the launches: 64 x 1024 x 32000 scored in 26.5 us
-//  (of 14 at a copy's rate), 128 rows differentiated with it in 112 (28).
+//  Bound by the matrix cores for many rows, and those by power: 4096 x 4096 x 128256 bf16 is scored in 3.3 ms (1.3
+//  PFLOP/s at a clock near 1.5 GHz; a library product alone 2.99) and scored and differentiated in 13.5 to 13.8 ms (1.25
+//  to 1.27 at its 8 R V dim). Few rows are bound by the weight's bytes and the launches: 64 x 1024 x 32000 scored in 27 us
+//  (of 14 at a copy's rate), 128 rows differentiated with it in 113 (28).
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
