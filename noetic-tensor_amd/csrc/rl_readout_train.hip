@@ -382,9 +382,12 @@ struct CoefP {
 
 constexpr int kNoTop = -(1 << 30);
 
-// The rows whose token is in 256 columns of the vocabulary, `bucket`, in their order: a workgroup goes through all the
-// tokens, a wave through consecutive ones, once to count them and those of the buckets in front, once to write them.
+// The rows whose token is in 256 columns of the vocabulary, `bucket`, in their order, but for those that nothing flows
+// through (a batch's padding may hold one token many times): a workgroup goes through all the tokens, a wave through
+// consecutive ones, once to count them and those of the buckets in front, whose places they may not fill, once to
+// write them.
 constexpr int kBucket = 256;
+__device__ __forceinline__ bool nothing_flows(double gl, double ge, float base) { return (gl == 0.0 && ge == 0.0) || base == -INFINITY; }
 __device__ __forceinline__ void list_tokens(const CoefP &p, int bucket) {
     __shared__ int s_hits[16], s_less[16];
     const int lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
@@ -392,6 +395,10 @@ __device__ __forceinline__ void list_tokens(const CoefP &p, int bucket) {
     const int64_t last = first + per < p.rows ? first + per : p.rows;
     const uint32_t from = uint32_t(bucket) * kBucket;
     auto token = [&](int64_t r) { return r < last ? uint32_t(p.tokens[r]) : ~0u; };
+    auto listed = [&](int64_t r, uint32_t t) {
+        return t < p.vocab && t - from < uint32_t(kBucket) &&
+               !nothing_flows(p.g_logp ? p.g_logp[r] : 0.0, p.g_entropy ? p.g_entropy[r] : 0.0, p.base[r]);
+    };
     int hits = 0, less = 0;
     for (int64_t r = first + lane; r - lane < last; r += 512) {
         uint32_t t[8];
@@ -399,7 +406,7 @@ __device__ __forceinline__ void list_tokens(const CoefP &p, int bucket) {
         for (int u = 0; u < 8; u++) t[u] = token(r + 64 * u);  // (eight loads in flight)
 #pragma unroll
         for (int u = 0; u < 8; u++) {
-            hits += __popcll(__ballot(t[u] < p.vocab && t[u] - from < uint32_t(kBucket)));
+            hits += __popcll(__ballot(listed(r + 64 * u, t[u])));
             less += __popcll(__ballot(t[u] < from));
         }
     }
@@ -416,7 +423,7 @@ __device__ __forceinline__ void list_tokens(const CoefP &p, int bucket) {
     at += start;
     for (int64_t r = first + lane; r - lane < last; r += 64) {
         const uint32_t t = token(r);
-        const bool hit = t < p.vocab && t - from < uint32_t(kBucket);
+        const bool hit = listed(r, t);
         const uint64_t m = __ballot(hit);
         if (hit) p.listed[at + __popcll(m & ((uint64_t(1) << lane) - 1))] = uint32_t(r) << 8 | (t - from);
         at += __popcll(m);
@@ -437,7 +444,7 @@ __global__ __launch_bounds__(1024) void k_readout_coef(CoefP p) {
         // the largest value as the columns have it: z's (an additive mask), or x's, whose rounding goes to the rest
         const float base = p.base[r], top_x = p.f32mask ? base : float(double(base) * p.tau);
         const double rest = double(p.rest[r]) + (p.f32mask ? 0.0 : double(base) - double(top_x) / p.tau), q = exp(-rest);
-        const bool dead = (gl == 0.0 && ge == 0.0) || base == -INFINITY;
+        const bool dead = nothing_flows(gl, ge, base);
         double unit = 1.0;  // f16: G's unit, a power of two
         float up = 0.0f;
         if (p.f16 && !dead) {

@@ -871,3 +871,15 @@ def test_a_step_too_large_for_capture_is_refused():
         assert L.nt_hip_rl_readout_score_stats(C.byref(a)) == 0 and L.nt_hip_rl_readout_score_backward(C.byref(b)) == 0
         nr.sync()
         g.close()
+
+
+@pytest.mark.parametrize("layout", ["dv", "vd"])
+def test_padding_of_one_token(layout):
+    """Most positions padded with one token, which live ones have too: the gradients of those that are not."""
+    R, V, d = 3000, 5000, 264
+    c = Case(R, V, d, "bf16", layout)
+    pad = torch.rand(R, generator=torch.Generator().manual_seed(4)) < 0.9
+    c.tokens[pad], c.g_logp[pad], c.g_entropy[pad] = 7, 0.0, 0.0
+    live = (~pad).nonzero().ravel()
+    c.tokens[live[::5]] = 7
+    check(c)
