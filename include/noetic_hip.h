@@ -302,7 +302,7 @@ int nt_hip_rl_readout_score(const NtRlReadoutScoreArgs *a);
  * whose allowed logits hold a NaN or +inf has NaNs and NT_ROW_NAN. Rows of 16-byte-aligned operands whose
  * strides and contiguous lengths are multiples of 8 are read in place; others are first copied into such rows.
  * The workspace is 8 (12 with the entropy) bytes per row and 128 columns, and those copies. Under stream capture a call
- * of 256 x 256 tiles, or with a part of the workspace of 1 MiB or more, is refused (NT_E_UNSUPPORTED), and so is such
+ * of 256 x 256 tiles, or with a workspace of 1 MiB or more, is refused (NT_E_UNSUPPORTED), and so is such
  * a backward. */
 typedef struct NtRlReadoutStatsArgs {
     const void *hidden;        /* [rows, ldh] */

@@ -867,12 +867,13 @@ struct Scratch {
         if (size[n] < kAlone) together += size[n];
         return n++;
     }
-    // `large`: the call takes 256 x 256 tiles. Under stream capture such a call, and one with a block of its own, is refused: a
+    // `large`: the call takes 256 x 256 tiles. Under stream capture such a call, and one with 1 MiB of scratch, is refused: a
     // captured step of 2100 x 512 x 32768 faulted in its replays, for a cause not found, where it runs as it should
     // outside of a graph; captured steps of smaller tiles whose scratch is one block replay rightly.
     int allocate(const char *who, bool large) {
         bool cap = false;
         if (int rc = stream_capturing(&cap)) return rc;
+        large |= together >= kAlone;
         for (int i = 0; i < n; i++) large |= size[i] >= kAlone;
         if (cap && large)
             return fail(NT_E_UNSUPPORTED, std::string(who) + ": too large for stream capture (256 x 256 tiles, or scratch of 1 MiB "
