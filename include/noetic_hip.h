@@ -432,6 +432,137 @@ typedef struct NtRlScoreGradArgs {
 } NtRlScoreGradArgs;
 int nt_hip_rl_score_backward(const NtRlScoreGradArgs *a);
 
+/* Verification of drafted tokens (speculative decoding; no counterpart in the reference, beside its samplers,
+ * rl.rs:488-529). A sequence has K = drafted tokens of a cheaper drafter and the target's logits at K + 1
+ * positions: row s (K + 1) + t holds the distribution after the first t drafts. With z = x / T + mask evaluated
+ * in f64, p = softmax(z) of the target and q = softmax(z) of the drafter's own logits (row s K + t, under the
+ * target row's mask and draft_temperature; no draft_logits: the drafter is certain, q = 1 at its token), the
+ * token x drafted at t is accepted while uniforms[s, t] q(x) < p(x). At the first position a that is not, the
+ * token is drawn from r = max(p - q, 0) (from p where that is zero everywhere), at a = lengths[s] (all drafts
+ * accepted) from p itself: the first v with sum_{j <= v} r_j > uniforms[s, K] sum r, or the last with r > 0.
+ * What is kept is then distributed as the target's own samples are. Temperature 0 is greedy: a draft is
+ * accepted where it is the first argmax of the target's masked logits (in f32), which is also the token at a;
+ * no uniforms and no draft logits are read, and logp is that of the temperature-1 distribution, as
+ * nt_hip_rl_sample's.
+ *   accepted[s] = a;  ids[s, 0 .. a] = the accepted drafts and the drawn token, -1 after them;
+ *   logp[s, t] = ln p(ids[s, t]), 0 after them.
+ * Rows past a do not matter, whatever they hold. A row that does and has no allowed token (target or drafter:
+ * NT_ROW_NO_TOKEN), a NaN or +inf among its allowed logits (NT_ROW_NAN), or a draft outside [0, vocab)
+ * (NT_ROW_BAD_TOKEN) ends its sequence there: accepted is its position, its id -1 and its logp NaN. A length
+ * outside [0, K] accepts nothing (NT_ROW_BAD_TOKEN). The workspace is under 32 bytes per row of each of its
+ * pieces and 8 per sequence and 512 columns; under stream capture a call with 1 MiB of it or more is refused
+ * (NT_E_UNSUPPORTED). */
+typedef struct NtRlVerifyArgs {
+    const void *logits;        /* [seqs (drafted + 1), ld] */
+    const void *draft_logits;  /* [seqs drafted, draft_ld] of the same dtype, or NULL: certain drafts */
+    int32_t dtype;             /* NT_F32 | NT_BF16 | NT_F16 */
+    int32_t mask_kind;         /* NT_MASK_* */
+    int64_t seqs, drafted;     /* drafted 0 .. 127, seqs (drafted + 1) < 2^22 */
+    int64_t vocab, ld, draft_ld;
+    const void *mask;          /* rows of vocab entries for the target's rows; NULL with NT_MASK_NONE */
+    int64_t mask_ld;           /* mask row stride; 0 = one row shared */
+    double temperature;        /* >= 0 and finite; 0 = greedy */
+    double draft_temperature;  /* > 0 and finite where draft logits are read */
+    const int32_t *tokens;     /* [seqs, drafted] */
+    const int32_t *lengths;    /* [seqs] drafts of each sequence, or NULL (all) */
+    const double *uniforms;    /* [seqs, drafted + 1], each in (0,1); unused when greedy */
+    int32_t *ids;              /* [seqs, drafted + 1] out */
+    int32_t *accepted;         /* [seqs] out */
+    float *logp;               /* [seqs, drafted + 1] out or NULL */
+    uint8_t *status;           /* [seqs] out: NT_ROW_* */
+    NtMaskRows mask_rows;      /* a mask broadcast over leading dimensions of the target's rows */
+} NtRlVerifyArgs;
+int nt_hip_rl_verify_drafted(const NtRlVerifyArgs *a);
+
+/* The k most likely tokens of each row with their log-probabilities: what a served token's alternatives or a
+ * teacher's record for nt_hip_rl_distill are (topk_with_indices, float.rs:1070-1080, of the tempered logits, and
+ * token_log_probs, rl.rs:134-141, at them, in one pass over the row). Ordered by z = tempered_logits(logits, T,
+ * mask) from the largest down, ties (-0 and +0 among them) to the lowest index; without an additive mask by the
+ * logits themselves, which a quotient's rounding could make equal. ids and logp are [rows, k]. A row of
+ * fewer allowed tokens than k has ids -1 and logp -inf after them; one with none (NT_ROW_NO_TOKEN), or
+ * with a NaN or +inf among its allowed logits (NT_ROW_NAN), ids -1 and logp NaN throughout. A call of few rows
+ * has a workspace of under 32 (k + 1) bytes per 2048 columns; under stream capture 1 MiB or more of it is
+ * refused (NT_E_UNSUPPORTED). */
+typedef struct NtRlTopArgs {
+    const void *logits;       /* [rows, ld] f32, bf16 or f16 */
+    int32_t dtype;
+    int32_t mask_kind;
+    int64_t rows, vocab, ld;  /* vocab < 2^31 */
+    const void *mask;
+    int64_t mask_ld;
+    double temperature;       /* > 0 and finite */
+    int64_t k;                /* 1 .. min(vocab, 1024) */
+    int32_t *ids;             /* [rows, k] out */
+    float *logp;              /* [rows, k] out */
+    uint8_t *status;          /* [rows] out: NT_ROW_* */
+    NtMaskRows mask_rows;
+} NtRlTopArgs;
+int nt_hip_rl_top_logprobs(const NtRlTopArgs *a);
+
+/* Distillation from a teacher's recorded tokens: the divergence of each row's softmax q (of the student's
+ * tempered logits) from the teacher's weights w_j = exp(teacher_logp[r, j]) at tokens ids[r, j]:
+ *   NT_TAIL_REST         what the list leaves, rest = max(1 - sum w, 0), is one outcome more:
+ *                        loss = sum w (ln w - ln q) + rest (ln rest - ln of the sum of q off the list)
+ *   NT_TAIL_DROP         loss = sum w (ln w - ln q)
+ *   NT_TAIL_RENORMALIZE  the same with w = softmax(teacher_logp) over the list (any logits do)
+ * A listed id of -1 is padding. One outside [-1, vocab) or listed twice gives NT_ROW_BAD_TOKEN and loss NaN; a
+ * row with no allowed token or with a NaN or +inf, its status and NaN. A weight at a token that the mask
+ * excludes makes the loss +inf, as logp is -inf there; a weight of 0 adds nothing, and neither does a rest
+ * where no allowed token is off the list. Sums over the row are of f32 exponentials, held in f64;
+ * everything per listed token is f64. stats, [rows, NT_DISTILL_STATS] f64, is for the backward. Vocabulary below
+ * 2^31. The workspace (a call of few rows, or of rows past 2^18 columns) is 32 bytes per piece of a row; under stream
+ * capture 1 MiB or more of it is refused (NT_E_UNSUPPORTED). */
+#define NT_TAIL_REST 0
+#define NT_TAIL_DROP 1
+#define NT_TAIL_RENORMALIZE 2
+#define NT_DISTILL_STATS 5
+typedef struct NtRlDistillArgs {
+    const void *logits;         /* [rows, ld] the student's: f32, bf16 or f16 */
+    int32_t dtype;
+    int32_t mask_kind;
+    int64_t rows, vocab, ld;
+    const void *mask;
+    int64_t mask_ld;
+    double temperature;         /* > 0 and finite */
+    int64_t k;                  /* tokens listed per row: 1 .. 1024 */
+    const int32_t *ids;         /* [rows, k] */
+    const float *teacher_logp;  /* [rows, k] */
+    int32_t tail;               /* NT_TAIL_* */
+    int32_t pad0;
+    float *loss;                /* [rows] out */
+    double *stats;              /* [rows, NT_DISTILL_STATS] out */
+    uint8_t *status;            /* [rows] out: NT_ROW_* */
+    NtMaskRows mask_rows;
+} NtRlDistillArgs;
+int nt_hip_rl_distill(const NtRlDistillArgs *a);
+
+/* Its backward: grad = d (sum_r g_loss[r] loss[r]) / d logits. With M = sum w (+ rest),
+ *   d loss / d z_v = M q_v - w_v                             on the list
+ *                  = M q_v - rest q_v / (sum of q off the list)    off it (rest 0 but for NT_TAIL_REST)
+ * and d / d x = d / d z / T; a listed token that the mask excludes gets its -w term alone, as a scored one's
+ * does (nt_hip_rl_score_backward). Written in grad_dtype, rounded once. A row whose g_loss is 0 gets zeros,
+ * whatever it holds; a refused one NaN. stats is the forward's for the same inputs. */
+typedef struct NtRlDistillGradArgs {
+    const void *logits;
+    int32_t dtype;
+    int32_t mask_kind;
+    int64_t rows, vocab, ld;
+    const void *mask;
+    int64_t mask_ld;
+    double temperature;
+    int64_t k;
+    const int32_t *ids;
+    const float *teacher_logp;
+    const double *stats;        /* [rows, NT_DISTILL_STATS] from the forward */
+    const float *g_loss;        /* [rows] */
+    void *grad;                 /* [rows, grad_ld] out */
+    int32_t grad_dtype;         /* NT_F32 | NT_BF16 | NT_F16 */
+    int32_t pad0;
+    int64_t grad_ld;
+    NtMaskRows mask_rows;
+} NtRlDistillGradArgs;
+int nt_hip_rl_distill_backward(const NtRlDistillGradArgs *a);
+
 /* kl_estimate per sampled token (rl.rs:380-400), elementwise over n = S*B*T values:
  * delta = ref_logp - logp, zeroed where mask == 0 (a select, rl.rs:100-102), clamped to
  * [-clamp, clamp] when clamp > 0; estimator 1: -delta, 2: delta^2/2, 3: exp(delta)-delta-1;

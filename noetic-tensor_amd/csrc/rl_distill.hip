@@ -1,0 +1,517 @@
+// nt_hip_rl_distill and nt_hip_rl_distill_backward: a row's divergence from a teacher's listed tokens, and its
+// gradient.
+//
+// Forward: a workgroup (several a row where rows are few) streams the logits once. A bitmap in LDS, a bit a column,
+// says which columns the list holds: that keeps the sum off the list a sum of its own (the whole less
+// the listed part would lose what is left to the rounding of the whole), and finds an id listed twice. Exponentials
+// are f32 relative to a wave's running maximum; a lane's sums are f64.
+// A divergence is a small difference of large sums, so it is taken as one of its second order: with
+// d = ln q - ln w, sum w (-d) = sum w (e^d - 1 - d) over a whole distribution (sum q = sum w = 1), whose terms
+// are all positive and whose derivative by an error of ln q, sum (q - w), vanishes. The f32
+// exponentials' error then does not reach it.
+//
+// Backward: every column's gradient is its exponential times one factor of the row, written as it streams
+// by; then the listed ones, in f64 and rounded once, are written over it.
+#include <algorithm>
+
+#include "nt_exp64.hpp"
+#include "nt_rows.hpp"
+
+namespace nt {
+namespace {
+
+constexpr int kDistillThreads = 256;
+constexpr int kDistillWaves = kDistillThreads / kWave;
+constexpr int kDistillBatch = 4;              // chunks a wave takes together
+constexpr int kMaxListed = 1024;
+constexpr int kMapChunks = 512;               // chunks a workgroup's bitmap covers: 2^18 columns, 32 KiB
+
+struct DistillRec {
+    double S, R;   // sum over the piece, and over its columns off the list, relative to a
+    float a;
+    int32_t bad;   // an id outside the vocabulary, or one listed twice
+    int64_t pad;
+};
+
+struct DistillP {
+    const void *x, *mask;
+    int64_t V, ld;
+    MaskMap mm;
+    float c;            // exponent scale of a value: log2(e) / T (none, u8) or log2(e) (f32 mask)
+    float tau;
+    int tau_one;
+    double inv_t;       // 1 / T
+    int nc, segs, per;
+    int k, tail;
+    const int32_t *ids;
+    const float *teacher;
+    float *loss;
+    double *stats;
+    uint8_t *status;
+    DistillRec *rec;    // segs > 1
+    // backward
+    const float *g;
+    void *grad;
+    int64_t gld;
+};
+
+// z - base of one listed token in f64 (the base a value: see c), -inf where it is excluded.
+template <int DT, int MK>
+__device__ __forceinline__ double listed_z(const DistillP &p, const void *xrow, const void *mrow, int64_t v, double base) {
+    float x;
+    if constexpr (DT == NT_F32) x = static_cast<const float *>(xrow)[v];
+    else x = widen16<DT>(uint32_t(static_cast<const uint16_t *>(xrow)[v]));
+    if constexpr (MK == NT_MASK_U8) {
+        if (static_cast<const uint8_t *>(mrow)[v] == 0) return -INFINITY;
+    } else if constexpr (MK == NT_MASK_F32) {
+        return (double(x) * p.inv_t + double(static_cast<const float *>(mrow)[v])) - base;
+    }
+    return (double(x) - base) * p.inv_t;
+}
+
+// A sum over the workgroup in f64; every thread gets it. `s` holds a value per wave.
+__device__ __forceinline__ double group_sum_d(double v, double *s) {
+    v = wave_sum_d(v);
+    __syncthreads();
+    if ((threadIdx.x & (kWave - 1)) == 0) s[threadIdx.x / kWave] = v;
+    __syncthreads();
+    double t = s[0];
+    for (int w = 1; w < kDistillWaves; w++) t += s[w];
+    return t;
+}
+
+// A row's loss, statistics and status from its merged sums. The whole workgroup.
+template <int DT, int MK>
+__device__ void distill_finish(const DistillP &p, int64_t row, const DistillRec &r, double *s) {
+    const void *xrow = static_cast<const char *>(p.x) + row * p.ld * Elem<DT>::kBytes;
+    const void *mrow = nullptr;
+    if constexpr (MK != NT_MASK_NONE) mrow = static_cast<const char *>(p.mask) + mask_row_at(p.mm, row) * MaskWords<MK>::kBytes;
+    int st = NT_ROW_OK;
+    if (!(r.S == r.S)) st = NT_ROW_NAN;
+    else if (r.a == -INFINITY) st = NT_ROW_NO_TOKEN;
+    else if (r.bad) st = NT_ROW_BAD_TOKEN;
+    const int32_t *ids = p.ids + row * p.k;
+    const float *teacher = p.teacher + row * p.k;
+    double ln_norm = 0.0;
+    if (p.tail == NT_TAIL_RENORMALIZE) {
+        float m = -INFINITY;
+        for (int j = threadIdx.x; j < p.k; j += kDistillThreads) m = ids[j] >= 0 ? fmaxf(m, teacher[j]) : m;
+        m = wave_max(m);
+        __syncthreads();
+        if ((threadIdx.x & (kWave - 1)) == 0) s[threadIdx.x / kWave] = double(m);
+        __syncthreads();
+        for (int w = 0; w < kDistillWaves; w++) m = fmaxf(m, float(s[w]));
+        double t = 0.0;
+        for (int j = threadIdx.x; j < p.k; j += kDistillThreads)
+            if (ids[j] >= 0) t += exp(double(teacher[j]) - double(m));
+        ln_norm = double(m) + log(group_sum_d(t, s));
+    }
+    const double ln_s = log(r.S);
+    double loss = 0.0, mass = 0.0;
+    if (st == NT_ROW_OK) {
+        for (int j = threadIdx.x; j < p.k; j += kDistillThreads) {
+            if (ids[j] < 0) continue;
+            const double lw = double(teacher[j]) - ln_norm, w = exp(lw);
+            const double lq = listed_z<DT, MK>(p, xrow, mrow, ids[j], double(r.a)) - ln_s, d = lq - lw;
+            mass += w;
+            if (p.tail != NT_TAIL_REST) {
+                if (!(w == 0.0)) loss -= w * d;
+            } else if (w == 0.0) {
+                loss += exp(lq);
+            } else {
+                loss += fabs(d) < 1.0 ? w * (expm1(d) - d) : exp(lq) - w - w * d;
+            }
+        }
+    }
+    loss = group_sum_d(loss, s);
+    mass = group_sum_d(mass, s);
+    if (threadIdx.x != 0) return;
+    double total = mass, share = 0.0;
+    if (p.tail == NT_TAIL_REST) {
+        const double rest = mass < 1.0 ? 1.0 - mass : 0.0, q = r.R / r.S;
+        total = mass < 1.0 ? 1.0 : mass;
+        if (rest > 0.0 && q > 0.0) {
+            const double d = log(q) - log(rest);
+            loss += fabs(d) < 1.0 ? rest * (expm1(d) - d) : q - rest - rest * d;
+            share = rest / q;
+        } else {
+            // (an outcome of one side alone: the terms' sum is then over other masses than 1 and 1)
+            loss += q - rest;
+        }
+        loss += total - 1.0;
+    }
+    p.loss[row] = st == NT_ROW_OK ? float(loss) : NAN;
+    p.status[row] = uint8_t(st);
+    double *o = p.stats + row * NT_DISTILL_STATS;
+    o[0] = double(r.a);
+    o[1] = st == NT_ROW_OK ? r.S : NAN;
+    o[2] = total - share;
+    o[3] = total;
+    o[4] = ln_norm;
+}
+
+template <int DT, int MK, bool AL>
+__global__ __launch_bounds__(kDistillThreads) void k_distill(DistillP p) {
+    extern __shared__ uint32_t map[];
+    __shared__ double red[kDistillWaves];
+    __shared__ DistillRec ws[kDistillWaves];
+    __shared__ int bad;
+    const int64_t row = blockIdx.x / unsigned(p.segs);
+    const int seg = int(blockIdx.x % unsigned(p.segs));
+    const int lane = threadIdx.x & (kWave - 1), wave = __builtin_amdgcn_readfirstlane(int(threadIdx.x / kWave));
+    const void *xrow = static_cast<const char *>(p.x) + row * p.ld * Elem<DT>::kBytes;
+    const void *mrow = nullptr;
+    if constexpr (MK != NT_MASK_NONE) mrow = static_cast<const char *>(p.mask) + mask_row_at(p.mm, row) * MaskWords<MK>::kBytes;
+    const bool tau_one = p.tau_one != 0;
+    const int c0 = seg * p.per, c1 = min(p.nc, c0 + p.per);
+
+    for (int i = threadIdx.x; i < (c1 - c0) * (kChunk / 32); i += kDistillThreads) map[i] = 0;
+    if (threadIdx.x == 0) bad = 0;
+    __syncthreads();
+    for (int j = threadIdx.x; j < p.k; j += kDistillThreads) {
+        const int32_t id = p.ids[row * p.k + j];
+        if (id < -1 || id >= p.V) {
+            bad = 1;
+        } else if (id >= c0 * kChunk && id - c0 * kChunk < (c1 - c0) * kChunk) {
+            const uint32_t at = uint32_t(id - c0 * kChunk), bit = 1u << (at % 32);
+            if (atomicOr(&map[at / 32], bit) & bit) bad = 1;
+        }
+    }
+    __syncthreads();
+    const uint8_t *bytes = reinterpret_cast<const uint8_t *>(map);
+
+    double S = 0.0, R = 0.0;
+    float a = -INFINITY;
+    for (int t0 = c0 + wave; t0 < c1; t0 += kDistillBatch * kDistillWaves) {
+        Raw<DT, MK> raw[kDistillBatch];
+#pragma unroll
+        for (int i = 0; i < kDistillBatch; i++) {
+            const int ch = t0 + i * kDistillWaves;
+            load_raw<DT, MK, AL>(raw[i], xrow, mrow, ch < c1 ? int64_t(ch) * kChunk + lane * kEpl : p.V, p.V);
+        }
+        float v[kDistillBatch][kEpl];
+        float m = -INFINITY;
+#pragma unroll
+        for (int i = 0; i < kDistillBatch; i++) {
+            decode<DT, MK>(raw[i], v[i], p.tau, tau_one);
+            m = fmaxf(m, max8(v[i]));
+        }
+        m = fmaxf(wave_max(m), a);
+        const float sh = m == -INFINITY ? 0.0f : m;
+        float sum = 0.0f, off = 0.0f;
+#pragma unroll
+        for (int i = 0; i < kDistillBatch; i++) {
+            const int ch = t0 + i * kDistillWaves;
+            float w[kEpl];
+#pragma unroll
+            for (int j = 0; j < kEpl; j++) w[j] = exp2_hw((v[i][j] - sh) * p.c);
+            const float t = tree8(w);
+            sum += t;
+            const uint32_t on = ch < c1 ? bytes[(ch - c0) * kWave + lane] : 0u;
+            if (__ballot(on != 0) == 0) {
+                off += t;
+            } else {
+#pragma unroll
+                for (int j = 0; j < kEpl; j++) w[j] = (on >> j) & 1u ? 0.0f : w[j];
+                off += tree8(w);
+            }
+        }
+        if (a != m && a != -INFINITY) {
+            const double f = exp2((double(a) - double(m)) * double(p.c));
+            S *= f;
+            R *= f;
+        }
+        S += double(sum);
+        R += double(off);
+        a = m;
+    }
+    S = wave_sum_d(S);
+    R = wave_sum_d(R);
+    if (lane == 0) ws[wave] = DistillRec{S, R, a, 0, 0};
+    __syncthreads();
+    DistillRec r{0.0, 0.0, ws[0].a, bad, 0};
+    for (int w = 1; w < kDistillWaves; w++) r.a = fmaxf(r.a, ws[w].a);
+    for (int w = 0; w < kDistillWaves; w++) {
+        const double f = ws[w].a == -INFINITY ? 1.0 : exp2((double(ws[w].a) - double(r.a)) * double(p.c));
+        r.S += ws[w].S * f;
+        r.R += ws[w].R * f;
+    }
+    if (p.segs > 1) {
+        if (threadIdx.x == 0) p.rec[row * p.segs + seg] = r;
+        return;
+    }
+    distill_finish<DT, MK>(p, row, r, red);
+}
+
+// The rows of a launch with several workgroups a row.
+template <int DT, int MK>
+__global__ __launch_bounds__(kDistillThreads) void k_distill_finish(DistillP p) {
+    __shared__ double red[kDistillWaves];
+    const int64_t row = blockIdx.x;
+    const DistillRec *rec = p.rec + row * p.segs;
+    DistillRec r{0.0, 0.0, -INFINITY, 0, 0};
+    for (int g = 0; g < p.segs; g++) {
+        r.a = fmaxf(r.a, rec[g].a);
+        r.bad |= rec[g].bad;
+    }
+    for (int g = 0; g < p.segs; g++) {
+        const double f = rec[g].a == -INFINITY ? 1.0 : exp2((double(rec[g].a) - double(r.a)) * double(p.c));
+        r.S += rec[g].S * f;
+        r.R += rec[g].R * f;
+    }
+    distill_finish<DT, MK>(p, row, r, red);
+}
+
+// Two gradients in a 16-bit dtype, a in the low half, to nearest even.
+template <int GDT>
+__device__ __forceinline__ uint32_t pack2(float a, float b) {
+    if constexpr (GDT == NT_BF16) {
+        uint32_t r;
+        asm("v_cvt_pk_bf16_f32 %0, %1, %2" : "=v"(r) : "v"(a), "v"(b));
+        return r;
+    } else {
+        return uint32_t(__builtin_bit_cast(uint16_t, _Float16(a))) | (uint32_t(__builtin_bit_cast(uint16_t, _Float16(b))) << 16);
+    }
+}
+
+// 8 gradients at column e0; AL: 16-byte aligned, all inside the row.
+template <int GDT, bool AL>
+__device__ __forceinline__ void store8(void *grow, int64_t e0, int64_t V, const float *o) {
+    if (e0 >= V) return;
+    if (AL || e0 + kEpl <= V) {
+        if constexpr (GDT == NT_F32) {
+            auto *d = reinterpret_cast<u32x4_f32 *>(static_cast<float *>(grow) + e0);
+            if constexpr (AL) {
+                auto *q = reinterpret_cast<v4u *>(d);
+                __builtin_nontemporal_store(v4u{__float_as_uint(o[0]), __float_as_uint(o[1]), __float_as_uint(o[2]), __float_as_uint(o[3])}, q);
+                __builtin_nontemporal_store(v4u{__float_as_uint(o[4]), __float_as_uint(o[5]), __float_as_uint(o[6]), __float_as_uint(o[7])}, q + 1);
+            } else {
+                d[0] = u32x4_f32{__float_as_uint(o[0]), __float_as_uint(o[1]), __float_as_uint(o[2]), __float_as_uint(o[3])};
+                d[1] = u32x4_f32{__float_as_uint(o[4]), __float_as_uint(o[5]), __float_as_uint(o[6]), __float_as_uint(o[7])};
+            }
+        } else {
+            const uint32_t w0 = pack2<GDT>(o[0], o[1]), w1 = pack2<GDT>(o[2], o[3]), w2 = pack2<GDT>(o[4], o[5]), w3 = pack2<GDT>(o[6], o[7]);
+            if constexpr (AL) __builtin_nontemporal_store(v4u{w0, w1, w2, w3}, reinterpret_cast<v4u *>(static_cast<uint16_t *>(grow) + e0));
+            else *reinterpret_cast<u32x4_f16 *>(static_cast<uint16_t *>(grow) + e0) = u32x4_f16{w0, w1, w2, w3};
+        }
+        return;
+    }
+    for (int j = 0; j < kEpl && e0 + j < V; j++) {
+        if constexpr (GDT == NT_F32) static_cast<float *>(grow)[e0 + j] = o[j];
+        else static_cast<uint16_t *>(grow)[e0 + j] = uint16_t(pack2<GDT>(o[j], o[j]));
+    }
+}
+
+template <int DT, int MK, int GDT, bool AL>
+__global__ __launch_bounds__(kDistillThreads) void k_distill_grad(DistillP p) {
+    const int64_t row = blockIdx.x / unsigned(p.segs);
+    const int seg = int(blockIdx.x % unsigned(p.segs));
+    const int lane = threadIdx.x & (kWave - 1), wave = __builtin_amdgcn_readfirstlane(int(threadIdx.x / kWave));
+    const void *xrow = static_cast<const char *>(p.x) + row * p.ld * Elem<DT>::kBytes;
+    const void *mrow = nullptr;
+    if constexpr (MK != NT_MASK_NONE) mrow = static_cast<const char *>(p.mask) + mask_row_at(p.mm, row) * MaskWords<MK>::kBytes;
+    void *grow = static_cast<char *>(p.grad) + row * p.gld * (GDT == NT_F32 ? 4 : 2);
+    const int c0 = seg * p.per, c1 = min(p.nc, c0 + p.per);
+    const float g = p.g[row];
+    if (g == 0.0f) {
+        const float zero[kEpl] = {};
+        for (int ch = c0 + wave; ch < c1; ch += kDistillWaves) store8<GDT, AL>(grow, int64_t(ch) * kChunk + lane * kEpl, p.V, zero);
+        return;
+    }
+    const double *st = p.stats + row * NT_DISTILL_STATS;
+    const double base = st[0], S = st[1], scale = double(g) * p.inv_t;
+    const float a = float(base), factor = float(scale * st[2] / S);
+    const bool tau_one = p.tau_one != 0;
+    for (int t0 = c0 + wave; t0 < c1; t0 += 2 * kDistillWaves) {
+        Raw<DT, MK> raw[2];
+#pragma unroll
+        for (int i = 0; i < 2; i++) {
+            const int ch = t0 + i * kDistillWaves;
+            load_raw<DT, MK, AL>(raw[i], xrow, mrow, ch < c1 ? int64_t(ch) * kChunk + lane * kEpl : p.V, p.V);
+        }
+#pragma unroll
+        for (int i = 0; i < 2; i++) {
+            const int ch = t0 + i * kDistillWaves;
+            float v[kEpl], o[kEpl];
+            decode<DT, MK>(raw[i], v, p.tau, tau_one);
+#pragma unroll
+            for (int j = 0; j < kEpl; j++) o[j] = fmaf(exp2_hw((v[j] - a) * p.c), factor, 0.0f);
+            if (ch < c1) store8<GDT, AL>(grow, int64_t(ch) * kChunk + lane * kEpl, p.V, o);
+        }
+    }
+    // the listed columns of this piece, over what was just written there
+    wait_vmcnt<0>();
+    __syncthreads();
+    for (int j = threadIdx.x; j < p.k; j += kDistillThreads) {
+        const int64_t id = p.ids[row * p.k + j];
+        if (id < int64_t(c0) * kChunk || id >= int64_t(c1) * kChunk || id >= p.V) continue;
+        const double w = exp(double(p.teacher[row * p.k + j]) - st[4]);
+        const double q = exp(listed_z<DT, MK>(p, xrow, mrow, id, base)) / S;
+        const double o = scale * (st[3] * q - w);
+        if constexpr (GDT == NT_F32) {
+            static_cast<float *>(grow)[id] = float(o);
+        } else if constexpr (GDT == NT_F16) {
+            static_cast<uint16_t *>(grow)[id] = __builtin_bit_cast(uint16_t, _Float16(o));
+        } else {
+            // (to f32 with the last bit odd where that was not exact, so that the second rounding is the only one)
+            float f = float(o);
+            if (double(f) != o && f == f) {
+                const uint32_t b = __float_as_uint(f);
+                const bool past = fabs(double(f)) > fabs(o);
+                f = __uint_as_float((past ? b - 1 : b) | 1u);
+            }
+            static_cast<uint16_t *>(grow)[id] = uint16_t(pack2<GDT>(f, f));
+        }
+    }
+}
+
+// Pieces of a row for `rows` rows of nc chunks: about `groups` workgroups, of a chunk per wave or more, and
+// at most `most` chunks each.
+void cut_rows(int64_t rows, int nc, int64_t groups, int most, int *segs, int *per) {
+    const int64_t few = std::max<int64_t>(1, std::min<int64_t>(groups / std::max<int64_t>(rows, 1), (nc + kDistillWaves - 1) / kDistillWaves));
+    *per = int(std::min<int64_t>(most, (nc + few - 1) / few));
+    *segs = (nc + *per - 1) / *per;
+}
+
+int distill_check(const char *who, int64_t rows, int64_t vocab, int64_t k, double temperature) {
+    if (!(temperature > 0.0) || !std::isfinite(temperature))
+        return fail(NT_E_ARG, "tempered_logits: temperature " + std::to_string(temperature) + " (must be positive)");
+    if (k < 1 || k > kMaxListed)
+        return fail(NT_E_ARG, std::string(who) + ": " + std::to_string(k) + " listed tokens a row (1 to " + std::to_string(kMaxListed) + ")");
+    // (a launch holds fewer than 2^32 threads; columns are counted in 32 bits)
+    if (vocab > 0x7fffffffLL - 16 * kChunk || rows > 0xffffffLL || rows * ((vocab + (int64_t(1) << 18) - 1) >> 18) > 0xffffffLL)
+        return fail(NT_E_ARG, std::string(who) + ": rows past 2^24 (of 2^18 columns) or vocab past 2^31");
+    return 0;
+}
+
+template <class F>
+void by_dtype(int dtype, int mk, F &&f) {
+    auto by_mk = [&](auto dt) {
+        if (mk == NT_MASK_U8) f(dt, std::integral_constant<int, NT_MASK_U8>{});
+        else if (mk == NT_MASK_F32) f(dt, std::integral_constant<int, NT_MASK_F32>{});
+        else f(dt, std::integral_constant<int, NT_MASK_NONE>{});
+    };
+    if (dtype == NT_F32) by_mk(std::integral_constant<int, NT_F32>{});
+    else if (dtype == NT_BF16) by_mk(std::integral_constant<int, NT_BF16>{});
+    else by_mk(std::integral_constant<int, NT_F16>{});
+}
+
+}  // namespace
+}  // namespace nt
+
+using namespace nt;
+
+extern "C" {
+
+int nt_hip_rl_distill(const NtRlDistillArgs *a) {
+    const char *who = "nt_hip_rl_distill";
+    if (!a) return fail(NT_E_ARG, std::string(who) + ": null args");
+    if (int rc = check_rows(a->rows, a->vocab, a->ld, a->dtype, a->mask_kind, a->mask, a->mask_ld, who)) return rc;
+    MaskMap mm;
+    if (int rc = mask_map(a->mask_rows, a->rows, a->vocab, a->mask_kind, a->mask_ld, who, &mm)) return rc;
+    if (int rc = distill_check(who, a->rows, a->vocab, a->k, a->temperature)) return rc;
+    if (a->tail < NT_TAIL_REST || a->tail > NT_TAIL_RENORMALIZE)
+        return fail(NT_E_ARG, std::string(who) + ": tail " + std::to_string(a->tail));
+    if (!a->logits || !a->ids || !a->teacher_logp || !a->loss || !a->stats || !a->status)
+        return fail(NT_E_ARG, std::string(who) + ": null logits, ids, teacher_logp or outputs");
+    std::unique_lock<std::mutex> lk;
+    if (int rc = enter(&lk)) return rc;
+    if (a->rows == 0) return 0;
+    DistillP p{};
+    p.x = a->logits;
+    p.mask = a->mask;
+    p.V = a->vocab;
+    p.ld = a->ld;
+    p.mm = mm;
+    p.tau = float(a->temperature);
+    p.tau_one = a->temperature == 1.0;
+    p.c = a->mask_kind == NT_MASK_F32 || p.tau_one ? kLog2e : float(kLog2e64 / a->temperature);
+    p.inv_t = 1.0 / a->temperature;
+    p.nc = int((a->vocab + kChunk - 1) / kChunk);
+    cut_rows(a->rows, p.nc, 1024, kMapChunks, &p.segs, &p.per);
+    p.k = int(a->k);
+    p.tail = a->tail;
+    p.ids = a->ids;
+    p.teacher = a->teacher_logp;
+    p.loss = a->loss;
+    p.stats = a->stats;
+    p.status = a->status;
+    void *ws = nullptr;
+    if (p.segs > 1) {
+        const size_t need = sizeof(DistillRec) * size_t(a->rows) * size_t(p.segs);
+        bool cap = false;
+        if (int rc = stream_capturing(&cap)) return rc;
+        if (cap && need >= size_t(1) << 20)
+            return fail(NT_E_UNSUPPORTED, std::string(who) + ": a workspace of " + std::to_string(need) +
+                                              " bytes under stream capture (less than 1 MiB)");
+        if (int rc = scratch_alloc(need, &ws)) return rc;
+        p.rec = static_cast<DistillRec *>(ws);
+    }
+    const bool al = aligned_rows(a->logits, a->vocab, a->ld, a->dtype, a->mask_kind, a->mask, mm);
+    hipStream_t s = ctx().stream;
+    by_dtype(a->dtype, a->mask_kind, [&](auto dt, auto mk) {
+        constexpr int DT = decltype(dt)::value, MK = decltype(mk)::value;
+        const dim3 grid(unsigned(a->rows * p.segs));
+        const size_t lds = size_t(p.per) * (kChunk / 8);
+        if (al) hipLaunchKernelGGL((k_distill<DT, MK, true>), grid, dim3(kDistillThreads), lds, s, p);
+        else hipLaunchKernelGGL((k_distill<DT, MK, false>), grid, dim3(kDistillThreads), lds, s, p);
+        if (p.segs > 1) hipLaunchKernelGGL((k_distill_finish<DT, MK>), dim3(unsigned(a->rows)), dim3(kDistillThreads), 0, s, p);
+    });
+    const int rc = launched(who);
+    const int rc2 = scratch_release(ws);
+    return rc ? rc : rc2;
+}
+
+int nt_hip_rl_distill_backward(const NtRlDistillGradArgs *a) {
+    const char *who = "nt_hip_rl_distill_backward";
+    if (!a) return fail(NT_E_ARG, std::string(who) + ": null args");
+    if (int rc = check_rows(a->rows, a->vocab, a->ld, a->dtype, a->mask_kind, a->mask, a->mask_ld, who)) return rc;
+    MaskMap mm;
+    if (int rc = mask_map(a->mask_rows, a->rows, a->vocab, a->mask_kind, a->mask_ld, who, &mm)) return rc;
+    if (int rc = distill_check(who, a->rows, a->vocab, a->k, a->temperature)) return rc;
+    if (!a->logits || !a->ids || !a->teacher_logp || !a->stats || !a->g_loss || !a->grad)
+        return fail(NT_E_ARG, std::string(who) + ": null logits, ids, teacher_logp, stats, g_loss or grad");
+    if (a->grad_dtype != NT_F32 && a->grad_dtype != NT_BF16 && a->grad_dtype != NT_F16)
+        return fail(NT_E_ARG, std::string(who) + ": grad dtype " + std::to_string(a->grad_dtype));
+    if (a->grad_ld < a->vocab) return fail(NT_E_ARG, std::string(who) + ": grad_ld < vocab");
+    std::unique_lock<std::mutex> lk;
+    if (int rc = enter(&lk)) return rc;
+    if (a->rows == 0) return 0;
+    DistillP p{};
+    p.x = a->logits;
+    p.mask = a->mask;
+    p.V = a->vocab;
+    p.ld = a->ld;
+    p.mm = mm;
+    p.tau = float(a->temperature);
+    p.tau_one = a->temperature == 1.0;
+    p.c = a->mask_kind == NT_MASK_F32 || p.tau_one ? kLog2e : float(kLog2e64 / a->temperature);
+    p.inv_t = 1.0 / a->temperature;
+    p.nc = int((a->vocab + kChunk - 1) / kChunk);
+    cut_rows(a->rows, p.nc, 4096, kMapChunks, &p.segs, &p.per);
+    p.k = int(a->k);
+    p.ids = a->ids;
+    p.teacher = a->teacher_logp;
+    p.stats = const_cast<double *>(a->stats);
+    p.g = a->g_loss;
+    p.grad = a->grad;
+    p.gld = a->grad_ld;
+    const bool al = aligned_rows(a->logits, a->vocab, a->ld, a->dtype, a->mask_kind, a->mask, mm) &&
+                    a->grad_ld % kEpl == 0 && reinterpret_cast<uintptr_t>(a->grad) % 16 == 0;
+    hipStream_t s = ctx().stream;
+    by_dtype(a->dtype, a->mask_kind, [&](auto dt, auto mk) {
+        constexpr int DT = decltype(dt)::value, MK = decltype(mk)::value;
+        const dim3 grid(unsigned(a->rows * p.segs));
+        auto launch = [&](auto gdt) {
+            constexpr int GDT = decltype(gdt)::value;
+            if (al) hipLaunchKernelGGL((k_distill_grad<DT, MK, GDT, true>), grid, dim3(kDistillThreads), 0, s, p);
+            else hipLaunchKernelGGL((k_distill_grad<DT, MK, GDT, false>), grid, dim3(kDistillThreads), 0, s, p);
+        };
+        if (a->grad_dtype == NT_F32) launch(std::integral_constant<int, NT_F32>{});
+        else if (a->grad_dtype == NT_BF16) launch(std::integral_constant<int, NT_BF16>{});
+        else launch(std::integral_constant<int, NT_F16>{});
+    });
+    return launched(who);
+}
+
+}  // extern "C"

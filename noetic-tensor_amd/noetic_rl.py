@@ -202,6 +202,41 @@ class NtRlPolicyLossArgs(C.Structure):
 NT_LOSS_PG, NT_LOSS_PPO = 0, 1
 
 
+class NtRlVerifyArgs(C.Structure):
+    _fields_ = [("logits", C.c_void_p), ("draft_logits", C.c_void_p), ("dtype", C.c_int32), ("mask_kind", C.c_int32),
+                ("seqs", C.c_int64), ("drafted", C.c_int64), ("vocab", C.c_int64), ("ld", C.c_int64),
+                ("draft_ld", C.c_int64), ("mask", C.c_void_p), ("mask_ld", C.c_int64), ("temperature", C.c_double),
+                ("draft_temperature", C.c_double), ("tokens", C.c_void_p), ("lengths", C.c_void_p),
+                ("uniforms", C.c_void_p), ("ids", C.c_void_p), ("accepted", C.c_void_p), ("logp", C.c_void_p),
+                ("status", C.c_void_p), ("mask_rows", NtMaskRows)]
+
+
+class NtRlTopArgs(C.Structure):
+    _fields_ = [("logits", C.c_void_p), ("dtype", C.c_int32), ("mask_kind", C.c_int32), ("rows", C.c_int64),
+                ("vocab", C.c_int64), ("ld", C.c_int64), ("mask", C.c_void_p), ("mask_ld", C.c_int64),
+                ("temperature", C.c_double), ("k", C.c_int64), ("ids", C.c_void_p), ("logp", C.c_void_p),
+                ("status", C.c_void_p), ("mask_rows", NtMaskRows)]
+
+
+class NtRlDistillArgs(C.Structure):
+    _fields_ = [("logits", C.c_void_p), ("dtype", C.c_int32), ("mask_kind", C.c_int32), ("rows", C.c_int64),
+                ("vocab", C.c_int64), ("ld", C.c_int64), ("mask", C.c_void_p), ("mask_ld", C.c_int64),
+                ("temperature", C.c_double), ("k", C.c_int64), ("ids", C.c_void_p), ("teacher_logp", C.c_void_p),
+                ("tail", C.c_int32), ("pad0", C.c_int32), ("loss", C.c_void_p), ("stats", C.c_void_p),
+                ("status", C.c_void_p), ("mask_rows", NtMaskRows)]
+
+
+class NtRlDistillGradArgs(C.Structure):
+    _fields_ = [("logits", C.c_void_p), ("dtype", C.c_int32), ("mask_kind", C.c_int32), ("rows", C.c_int64),
+                ("vocab", C.c_int64), ("ld", C.c_int64), ("mask", C.c_void_p), ("mask_ld", C.c_int64),
+                ("temperature", C.c_double), ("k", C.c_int64), ("ids", C.c_void_p), ("teacher_logp", C.c_void_p),
+                ("stats", C.c_void_p), ("g_loss", C.c_void_p), ("grad", C.c_void_p), ("grad_dtype", C.c_int32),
+                ("pad0", C.c_int32), ("grad_ld", C.c_int64), ("mask_rows", NtMaskRows)]
+
+
+NT_DISTILL_STATS = 5
+
+
 class NtLayout(C.Structure):
     """include/noetic_ops.h NtLayout: a view (element offset, shape, element strides)."""
     _fields_ = [("rank", C.c_int32), ("pad_", C.c_int32), ("offset", C.c_int64), ("shape", C.c_int64 * 8),
@@ -248,6 +283,10 @@ _SIGS = {
     "nt_hip_rl_sample_noalloc": (C.c_int, [C.POINTER(NtRlSampleArgs)]),
     "nt_hip_rl_score": (C.c_int, [C.POINTER(NtRlScoreArgs)]),
     "nt_hip_rl_score_backward": (C.c_int, [C.POINTER(NtRlScoreGradArgs)]),
+    "nt_hip_rl_verify_drafted": (C.c_int, [C.POINTER(NtRlVerifyArgs)]),
+    "nt_hip_rl_top_logprobs": (C.c_int, [C.POINTER(NtRlTopArgs)]),
+    "nt_hip_rl_distill": (C.c_int, [C.POINTER(NtRlDistillArgs)]),
+    "nt_hip_rl_distill_backward": (C.c_int, [C.POINTER(NtRlDistillGradArgs)]),
     "nt_hip_rl_kl_estimate": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_int64, C.c_int32, C.c_double,
                                         C.c_void_p]),
     "nt_hip_rl_zero_masked": (C.c_int, [C.c_void_p, C.c_void_p, C.c_int64, C.c_void_p]),
@@ -750,6 +789,64 @@ def sample_categorical_inv_cdf(logits: Tensor, temperature: float, mask: Optiona
     return sample_logp(logits, temperature, mask, rng)[0]
 
 
+def verify_drafted(logits: Tensor, draft_logits: Optional[Tensor], tokens: Tensor, temperature: float,
+                   mask: Optional[Tensor], rng: Optional[Rng], uniforms: Optional[Tensor] = None,
+                   lengths: Optional[Tensor] = None, draft_temperature: Optional[float] = None, check: bool = True):
+    """A new nn::rl entry beside the samplers (rl.rs:488-529): verification of K drafted tokens (speculative
+    decoding). `logits` [.., K + 1, V] are the target's after 0 .. K drafts, `draft_logits` [.., K, V] the drafter's
+    own at the drafted `tokens` [.., K] (None: drafts that are certain, a lookup's or a greedy drafter's);
+    `mask` is the target rows' vocabulary mask, and the drafter's. A draft x is accepted while u q(x) < p(x); at the first
+    refused one the token is drawn from max(p - q, 0), after the last from p, so that what is kept is distributed as
+    the target's own samples. Temperature 0 accepts the first argmax. `rng` gives K + 1 uniforms a sequence, the
+    last one the drawn token's (or `uniforms`, device f64 [.., K + 1]); `lengths` i32 [..] says how many drafts a
+    sequence has, `draft_temperature` the drafter's where it is another. Returns (ids [.., K + 1], accepted [..],
+    logp [.., K + 1]): the accepted drafts and the drawn token, then -1, and their log-probabilities, then 0.
+    Everything is evaluated in f64. `check` reads the sequences' status and refuses what cannot be drawn from."""
+    if not (temperature >= 0.0 and math.isfinite(temperature)):
+        raise ValueError(f"verify_drafted: temperature {temperature} (must be ≥ 0)")
+    t = Tempered(logits, 1.0 if temperature == 0.0 else temperature, mask)
+    if len(logits.shape) < 2 or logits.shape[-2] < 1:
+        raise ValueError(f"verify_drafted: logits {list(logits.shape)} ([.., K + 1, V])")
+    rows, V = _rows(logits)
+    lead, K = tuple(logits.shape[:-2]), logits.shape[-2] - 1
+    seqs = math.prod(lead)
+    if tokens.dtype != "i32" or tuple(tokens.shape) != lead + (K,):
+        raise ValueError(f"verify_drafted: tokens {list(tokens.shape)} of {tokens.dtype} (i32 {list(lead + (K,))})")
+    if draft_logits is not None:
+        if tuple(draft_logits.shape) != lead + (K, V):
+            raise ValueError(f"verify_drafted: draft logits {list(draft_logits.shape)} ({list(lead + (K, V))})")
+        same_dtype(logits.dtype, draft_logits.dtype, "verify_drafted")
+    dtemp = temperature if draft_temperature is None else draft_temperature
+    if draft_temperature is not None and not (dtemp > 0.0 and math.isfinite(dtemp)):
+        raise ValueError(f"verify_drafted: draft temperature {dtemp} (must be positive)")
+    if lengths is not None:
+        lengths = _row_arg(lengths, seqs, "i32", "verify_drafted: lengths")
+    if temperature != 0.0 and uniforms is None:
+        if rng is None:
+            raise ValueError("verify_drafted: a stream is needed at temperature > 0")
+        uniforms = Tensor.from_numpy(rng.uniforms(rows), "f64")
+    uniforms = _row_arg(uniforms, rows, "f64", "verify_drafted: uniforms")
+    ids, accepted, lp = IntTensor(lead + (K + 1,)), IntTensor(lead), Tensor(lead + (K + 1,), "f32")
+    status = Tensor(lead, "u8")
+    kind, mptr, mld, mrows, _keep = _mask_fields(t, rows, V)
+    ptr = lambda x: None if x is None else x.ptr  # noqa: E731
+    a = NtRlVerifyArgs(logits.ptr, ptr(draft_logits), _dtype_code(logits), kind, seqs, K, V, V, V, mptr, mld,
+                       float(temperature), float(dtemp), tokens.ptr, ptr(lengths), ptr(uniforms), ids.ptr,
+                       accepted.ptr, lp.ptr, status.ptr, mrows)
+    _check(lib().nt_hip_rl_verify_drafted(C.byref(a)), "verify_drafted")
+    if check:
+        st = status.to_numpy().ravel()
+        bad = np.nonzero(st != NT_ROW_OK)[0]
+        if bad.size:
+            i = int(bad[0])
+            if st[i] == NT_ROW_BAD_TOKEN:
+                raise IndexError(f"verify_drafted: sequence {i} has a draft outside [0, {V}) or a length outside "
+                                 f"[0, {K}]")
+            raise ValueError(f"verify_drafted: sequence {i} has a position with no allowed token (every logit −∞ or a "
+                             "NaN)")
+    return ids, accepted, lp
+
+
 NT_READOUT_W_DV, NT_READOUT_W_VD = 0, 1
 _ESIZE = {"f32": 4, "bf16": 2, "f16": 2}
 _DTCODE = {"f32": NT_F32, "bf16": NT_BF16, "f16": NT_F16}
@@ -1171,6 +1268,101 @@ def score_grad(logits, ref_logits, tokens: Optional[Tensor], stats: RowStats, kl
     return grad
 
 
+def top_logprobs(logits, k: int, check: bool = True):
+    """The k most likely tokens of each position and their log-probabilities, (ids [.., k] i32, logp [.., k]
+    f32), from the largest down: topk_with_indices (float.rs:1070-1080) of the tempered logits with token_log_probs
+    (rl.rs:134-141) at them, in one pass. `logits` may be a `Tempered` (temperature and vocabulary mask); 16-bit logits
+    are widened exactly. Ties go to the lowest index; a position of fewer allowed tokens has -1 and -inf
+    after them. k up to 1024. What `distill_with_stats` takes as a teacher's record. `check` reads the
+    positions' status and refuses one with no allowed token, as sample_categorical does (rl.rs:516-519)."""
+    x = _as_tempered(logits)
+    rows, V = _rows(x.logits)
+    lead = tuple(x.logits.shape[:-1])
+    if not 1 <= k <= min(V, 1024):
+        raise ValueError(f"top_logprobs: k {k} of {V} tokens (1 to min(V, 1024))")
+    ids, lp, status = IntTensor(lead + (k,)), Tensor(lead + (k,), "f32"), Tensor(lead, "u8")
+    kind, mptr, mld, mrows, _keep = _mask_fields(x, rows, V)
+    a = NtRlTopArgs(x.logits.ptr, _dtype_code(x.logits), kind, rows, V, V, mptr, mld, x.temperature, k, ids.ptr, lp.ptr,
+                    status.ptr, mrows)
+    _check(lib().nt_hip_rl_top_logprobs(C.byref(a)), "top_logprobs")
+    if check:
+        bad = np.nonzero(status.to_numpy().ravel() != NT_ROW_OK)[0]
+        if bad.size:
+            raise ValueError(f"top_logprobs: position {bad[0]} has no allowed token (every logit −∞ or a NaN)")
+    return ids, lp
+
+
+class TeacherTail(enum.IntEnum):
+    """What a teacher's list leaves of its distribution: one outcome more (REST), nothing (DROP), or the list's own
+    weights divided by their sum (RENORMALIZE, for which any logits do)."""
+    REST = 0
+    DROP = 1
+    RENORMALIZE = 2
+
+
+class DistillStats:
+    """A distillation pass's per-position sums (f64), saved for `distill_grad` in place of a log_softmax."""
+
+    def __init__(self, rows: Tensor):
+        self.rows = rows
+
+
+def _distill_args(x: Tempered, ids: Tensor, teacher_logp: Tensor):
+    """(rows, V, k, teacher f32), checked."""
+    rows, V = _rows(x.logits)
+    lead = tuple(x.logits.shape[:-1])
+    if ids.dtype != "i32" or len(ids.shape) != len(lead) + 1 or tuple(ids.shape[:-1]) != lead or ids.shape[-1] < 1 or \
+            ids.shape[-1] > 1024:
+        raise ValueError(f"distill: ids {list(ids.shape)} of {ids.dtype} (i32 {list(lead)} and 1 to 1024 listed tokens)")
+    if tuple(teacher_logp.shape) != tuple(ids.shape):
+        raise ValueError(f"distill: teacher log-probabilities {list(teacher_logp.shape)} for ids {list(ids.shape)}")
+    return rows, V, ids.shape[-1], _f32_storage(teacher_logp, "distill: teacher log-probabilities")
+
+
+def distill_with_stats(logits, ids: Tensor, teacher_logp: Tensor, tail: TeacherTail = TeacherTail.REST,
+                       check: bool = True):
+    """Distillation from a teacher's recorded tokens: per position, the divergence KL(teacher || student) of
+    softmax(`logits`) (a `Tempered` for a temperature and vocabulary mask) from the weights exp(`teacher_logp`)
+    [.., k] at `ids` [.., k] i32 (`top_logprobs`'s; an id of -1 is padding), with `tail` saying what becomes of the
+    rest of the teacher's distribution. Returns (loss [..] f32, DistillStats) for `distill_grad`. A weight at a token
+    that the mask excludes makes the loss +inf. `check` reads the positions' status and refuses an id outside
+    the vocabulary or listed twice."""
+    x = _as_tempered(logits)
+    rows, V, k, teacher = _distill_args(x, ids, teacher_logp)
+    lead = tuple(x.logits.shape[:-1])
+    loss, stats, status = Tensor(lead, "f32"), Tensor(lead + (NT_DISTILL_STATS,), "f64"), Tensor(lead, "u8")
+    kind, mptr, mld, mrows, _keep = _mask_fields(x, rows, V)
+    a = NtRlDistillArgs(x.logits.ptr, _dtype_code(x.logits), kind, rows, V, V, mptr, mld, x.temperature, k, ids.ptr,
+                        teacher.ptr, int(TeacherTail(tail)), 0, loss.ptr, stats.ptr, status.ptr, mrows)
+    _check(lib().nt_hip_rl_distill(C.byref(a)), "distill")
+    if check:
+        bad = np.nonzero(status.to_numpy().ravel() == NT_ROW_BAD_TOKEN)[0]
+        if bad.size:
+            raise IndexError(f"distill: position {bad[0]} lists a token outside [0, {V}), or one twice")
+    return loss, DistillStats(stats)
+
+
+def distill_grad(logits, ids: Tensor, teacher_logp: Tensor, stats: DistillStats, g_loss: Tensor,
+                 grad_dtype: Optional[str] = None) -> Tensor:
+    """The backward of `distill_with_stats`: d(sum_r g_loss[r] loss[r]) / d logits (the raw logits), one pass.
+    A position whose g_loss is 0 (padding) gets zeros, whatever it holds. `grad_dtype` defaults to the
+    logits' dtype."""
+    x = _as_tempered(logits)
+    rows, V, k, teacher = _distill_args(x, ids, teacher_logp)
+    g_loss = _row_arg(g_loss, rows, "f32", "distill backward: g_loss")
+    _row_arg(stats.rows, rows * NT_DISTILL_STATS, "f64", "distill backward: stats")
+    kind, mptr, mld, mrows, _keep = _mask_fields(x, rows, V)
+    gdt = grad_dtype or x.logits.dtype
+    gcode = _DTCODE.get(gdt)
+    if gcode is None:
+        raise ValueError(f"gradient dtype {gdt}")
+    grad = Tensor(x.logits.shape, gdt)
+    a = NtRlDistillGradArgs(x.logits.ptr, _dtype_code(x.logits), kind, rows, V, V, mptr, mld, x.temperature, k, ids.ptr,
+                            teacher.ptr, stats.rows.ptr, g_loss.ptr, grad.ptr, gcode, 0, V, mrows)
+    _check(lib().nt_hip_rl_distill_backward(C.byref(a)), "distill backward")
+    return grad
+
+
 def token_log_probs(logits, tokens: Tensor) -> Tensor:
     """rl.rs:134-141: log_softmax(logits)[…, tokens[…]]; `logits` may be a `tempered_logits`.
     16-bit logits are refused as the reference's log_softmax refuses them (at τ == 1, or
@@ -1265,6 +1457,16 @@ def categorical_entropy(logits, mask: Optional[Tensor] = None,
     log_softmax_dtype(_logits_dtype(logits))
     ent = _score(logits, None, None, False, False, False, True)[3]
     return _reduce(_zero_masked(ent, mask), mask, reduction)
+
+
+def distillation_loss(logits, ids: Tensor, teacher_logp: Tensor, tail: TeacherTail = TeacherTail.REST,
+                      mask: Optional[Tensor] = None, reduction: TokenReduction = TokenReduction.TOKEN_MEAN) -> Tensor:
+    """`distill_with_stats` of logits [S, B, T, V], reduced as the other losses are (categorical_kl, rl.rs:327-338). Its
+    gradient is `distill_grad` with `reduce_tokens_backward` as g_loss."""
+    if len(_as_tempered(logits).logits.shape) != 4:
+        raise ValueError("distillation_loss: logits [S, B, T, V]")
+    loss = distill_with_stats(logits, ids, teacher_logp, tail)[0]
+    return _reduce(_zero_masked(loss, mask), mask, reduction)
 
 
 def kl_estimate(logp: Tensor, ref_logp: Tensor, estimator: KlEstimator, delta_clamp: Optional[float] = None,
