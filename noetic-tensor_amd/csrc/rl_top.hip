@@ -1,14 +1,14 @@
 // nt_hip_rl_top_logprobs: the k most likely tokens of each row and their log-probabilities, in one pass.
 //
-// A workgroup streams its row (or, where rows are few, a piece of one) in tiles that its registers hold. It keeps
-// a list of candidates in LDS and a threshold that the k-th largest so far is known to reach, and a tile adds the few
-// elements above it; the same registers give the tile's part of the log-sum-exp. The first threshold comes from
-// the largest value of each lane's groups of eight: k groups that reach it are k elements that do. A value is
-// compared as 64 bits, the f32 made an ordered integer over the complement of its column, so that no two are equal and ties
-// go to the lowest column. When the list grows past kKeep, a threshold between the k-th and the 2k-th of it is
-// found by bisection and the rest dropped; where many values are equal or the row rises (a tile may then
-// bring more than the list holds), the tile goes in by groups and the list is cut to its k largest exactly.
-// At the end a candidate's place is the number of candidates above it.
+// A workgroup streams its row (or, where rows are few, a piece of one) once, and takes from it the log-sum-exp and the
+// largest value of each group of columns: a lane's columns in a quarter (of 256 k: a sixteenth) of the row. With
+// t the k-th largest of those 1024 (4096) maxima, k groups reach t, so k columns do, and the columns
+// that reach it lie in groups whose maximum does: those few groups are read again, from the caches, and hardly more than k
+// columns (1.15 k at k = 256 of 1024 groups) go on a list in LDS. A column's place is the number of listed ones above it.
+// Values are compared as 64 bits, the f32 made an ordered integer over the complement of its column, so that
+// no two are equal and ties go to the lowest column. Where the list does not hold what reaches t (many equal
+// values), the row goes through it in order, a few hundred columns at a time, and it is cut to its k
+// largest whenever it fills.
 //
 // What bounds it: the row's bytes, and for the log-sum-exp f32 exponentials as the scorer takes them.
 #include <algorithm>
@@ -20,10 +20,17 @@ namespace {
 
 constexpr int kTopThreads = 256;
 constexpr int kTopWaves = kTopThreads / kWave;
-constexpr int kList = 4096;          // candidates in LDS (a full group of a tile over kMaxK fits: 1024 + 2048)
-constexpr int kKeep = 1024;          // the list is cut when it is longer (or longer than 2 k)
 constexpr int kMaxK = 1024;
+constexpr int kFewK = 256;           // up to here the small form: 1024 groups, a list of 1024
 constexpr int kTopSegs = 64;         // pieces of a row, at most
+constexpr int kTopBatch = 4;         // chunks a wave takes together
+
+// The two forms: G groups a lane, the list's length, and the chunks that go through it at a time in order.
+template <bool BIG>
+struct TopForm {
+    static constexpr int G = BIG ? 16 : 4, kList = BIG ? 4096 : 1024, kRound = BIG ? 4 : 1;
+    static_assert((BIG ? kMaxK : kFewK) + kRound * kChunk <= kList, "a cut list and a round more");
+};
 
 // A piece's part of the row's log-sum-exp: S relative to a; n candidates follow.
 struct TopRec {
@@ -47,8 +54,11 @@ struct TopP {
     float *logp;
     uint8_t *status;
     TopRec *rec;        // segs > 1: [rows][segs]
-    uint64_t *cand;     // segs > 1: [rows][segs][2 k]
+    uint64_t *cand;     // segs > 1: [rows][segs][cand_of(k)]
 };
+
+// How many candidates a piece hands on, at most.
+__host__ __device__ __forceinline__ int cand_of(int k) { return k + k / 4 + 32; }
 
 // An f32 as an integer of the same order (-0 and +0 alike), and back.
 __device__ __forceinline__ uint32_t ordered(float v) {
@@ -61,17 +71,19 @@ __device__ __forceinline__ float unordered(uint32_t k) {
 constexpr uint32_t kNone = 0x007fffffu;  // ordered(-inf): an excluded token's, never a candidate
 
 // LDS of a workgroup.
+template <bool BIG>
 struct TopS {
-    uint64_t list[kList];
-    uint64_t least;          // a candidate is above it
+    uint64_t list[TopForm<BIG>::kList];
+    float gmax[TopForm<BIG>::G * kTopThreads];  // the groups' maxima
     uint32_t sums[2][kTopWaves];
-    int count;
+    int count, groups;
     double S[kTopWaves];
     float a[kTopWaves];
 };
 
 // The sum over the workgroup of a count that each lane's wave already agrees on (one barrier: two buffers in turn).
-__device__ __forceinline__ uint32_t group_sum(TopS &s, uint32_t wave_count, int turn) {
+template <bool BIG>
+__device__ __forceinline__ uint32_t group_sum(TopS<BIG> &s, uint32_t wave_count, int turn) {
     if ((threadIdx.x & (kWave - 1)) == 0) s.sums[turn & 1][threadIdx.x / kWave] = wave_count;
     __syncthreads();
     uint32_t n = 0;
@@ -81,10 +93,9 @@ __device__ __forceinline__ uint32_t group_sum(TopS &s, uint32_t wave_count, int 
 }
 
 // The largest found t such that at least k of the workgroup's N keys a lane are t or more, as soon as no more than
-// `most` are (bit by bit from the top; exact when it reaches the last). 0 where fewer than k are above `floor`
-// (floor: what a lane holds in place of nothing).
-template <class T, int N>
-__device__ __forceinline__ T kth_bound(TopS &s, const T (&key)[N], int k, int most) {
+// `most` are (bit by bit from the top; exact when it reaches the last). 0 where there are not k keys but 0.
+template <class T, int N, bool BIG>
+__device__ __forceinline__ T kth_bound(TopS<BIG> &s, const T (&key)[N], int k, int most) {
     T t = 0;
     int turn = 0;
     for (int bit = int(sizeof(T)) * 8 - 1; bit >= 0; bit--) {
@@ -102,9 +113,18 @@ __device__ __forceinline__ T kth_bound(TopS &s, const T (&key)[N], int k, int mo
     return t;
 }
 
-// Keep of the list what is `bound` or more. Every thread holds its entries (list[i * 256 + thread]) in `mine`.
-template <int N>
-__device__ __forceinline__ void keep_from(TopS &s, const uint64_t (&mine)[N], uint64_t bound) {
+// Cut the list of `n` entries to its k largest; the k-th of them. The whole workgroup.
+template <bool BIG>
+__device__ __forceinline__ uint64_t cut_list(TopS<BIG> &s, int n, int k) {
+    constexpr int N = TopForm<BIG>::kList / kTopThreads;
+    uint64_t mine[N];
+    const int lane = threadIdx.x & (kWave - 1);
+#pragma unroll
+    for (int i = 0; i < N; i++) {
+        const int at = i * kTopThreads + int(threadIdx.x);
+        mine[i] = at < n ? s.list[at] : 0;
+    }
+    const uint64_t bound = kth_bound<uint64_t, N, BIG>(s, mine, k, k);
     if (threadIdx.x == 0) s.count = 0;
     __syncthreads();
 #pragma unroll
@@ -113,55 +133,23 @@ __device__ __forceinline__ void keep_from(TopS &s, const uint64_t (&mine)[N], ui
         const uint64_t b = __ballot(in);
         if (b == 0) continue;
         int at = 0;
-        if ((threadIdx.x & (kWave - 1)) == unsigned(__builtin_ctzll(b))) at = atomicAdd(&s.count, int(__popcll(b)));
+        if (lane == int(__builtin_ctzll(b))) at = atomicAdd(&s.count, int(__popcll(b)));
         at = __builtin_amdgcn_readlane(at, __builtin_ctzll(b));
-        if (in) s.list[at + __popcll(b & ((uint64_t(1) << (threadIdx.x & (kWave - 1))) - 1))] = mine[i];
+        if (in) s.list[at + __popcll(b & ((uint64_t(1) << lane) - 1))] = mine[i];
     }
     __syncthreads();
+    return bound;
 }
 
-// Cut the list of `count` > k to at most max(2 k, ..) entries that hold its k largest (`exact`: to those k), and
-// raise the threshold to it.
-__device__ __attribute__((noinline)) void cut_list(TopS &s, int count, int k, bool exact) {
-    constexpr int N = kList / kTopThreads;
-    uint64_t mine[N];
-#pragma unroll
-    for (int i = 0; i < N; i++) {
-        const int at = i * kTopThreads + int(threadIdx.x);
-        mine[i] = at < count ? s.list[at] : 0;
-    }
-    uint64_t bound = 0;
-    if (!exact) {
-        uint32_t hi[N];
-#pragma unroll
-        for (int i = 0; i < N; i++) hi[i] = uint32_t(mine[i] >> 32);
-        bound = uint64_t(kth_bound<uint32_t, N>(s, hi, k, 2 * k)) << 32;
-        uint32_t n = 0;
-#pragma unroll
-        for (int i = 0; i < N; i++) n += uint32_t(__popcll(__ballot(mine[i] >= bound)));
-        n = group_sum(s, n, 0);
-        __syncthreads();
-        exact = int(n) > 2 * k;  // (equal values: by their columns too)
-    }
-    if (exact) bound = kth_bound<uint64_t, N>(s, mine, k, k);
-    keep_from<N>(s, mine, bound);
-    if (threadIdx.x == 0 && bound > 0 && bound - 1 > s.least) s.least = bound - 1;
-    __syncthreads();
-}
-
-// The row's tokens from the list and its log-sum-exp (base in z, rest ln of the sum). Every thread.
-__device__ __forceinline__ void top_finish(TopS &s, const TopP &p, int64_t row, double S, float a) {
+// The row's tokens from the list of n and its log-sum-exp. Every thread.
+template <bool BIG>
+__device__ __forceinline__ void top_finish(TopS<BIG> &s, const TopP &p, int64_t row, int n, double S, float a) {
     int32_t *ids = p.ids + row * p.k;
     float *logp = p.logp + row * p.k;
     int st = NT_ROW_OK;
     if (!(S == S)) st = NT_ROW_NAN;
     else if (a == -INFINITY) st = NT_ROW_NO_TOKEN;
     if (threadIdx.x == 0) p.status[row] = uint8_t(st);
-    int n = s.count;
-    if (n > kKeep) {
-        cut_list(s, n, p.k, false);
-        n = s.count;
-    }
     if (st != NT_ROW_OK) n = 0;
     const double lse = double(a) * p.inv_t + log(S);
     for (int i = threadIdx.x; i < n; i += kTopThreads) {
@@ -179,23 +167,17 @@ __device__ __forceinline__ void top_finish(TopS &s, const TopP &p, int64_t row, 
     }
 }
 
-// A workgroup's waves' sums.
-__device__ __forceinline__ void waves_sum(const TopS &s, float c, double *S, float *a) {
-    float m = s.a[0];
-    for (int w = 1; w < kTopWaves; w++) m = fmaxf(m, s.a[w]);
-    double t = 0.0;
-    for (int w = 0; w < kTopWaves; w++)
-        t += s.a[w] == -INFINITY ? s.S[w] : s.S[w] * exp2((double(s.a[w]) - double(m)) * double(c));
-    *S = t;
-    *a = m;
+// A lane's sum relative to a of its own, over the wave: S relative to the wave's a.
+__device__ __forceinline__ void wave_merge(double &S, float &a, float c) {
+    const float m = wave_max(a);
+    S = wave_sum_d(a == -INFINITY ? S : S * exp2((double(a) - double(m)) * double(c)));
+    a = m;
 }
 
-template <int DT, int MK, bool AL>
+template <int DT, int MK, bool AL, bool BIG>
 __global__ __launch_bounds__(kTopThreads) void k_top(TopP p) {
-    // a tile: NC chunks a wave, held as 16-bit logits with the u8 mask folded in, or as f32 values
-    constexpr bool HALF = DT != NT_F32 && MK != NT_MASK_F32;
-    constexpr int NC = HALF ? 8 : 4, W = HALF ? 4 : 8, HDT = HALF ? DT : NT_F32;
-    __shared__ TopS s;
+    using F = TopForm<BIG>;
+    __shared__ TopS<BIG> s;
     const int64_t row = blockIdx.x / unsigned(p.segs);
     const int seg = int(blockIdx.x % unsigned(p.segs));
     const int lane = threadIdx.x & (kWave - 1), wave = __builtin_amdgcn_readfirstlane(int(threadIdx.x / kWave));
@@ -203,166 +185,195 @@ __global__ __launch_bounds__(kTopThreads) void k_top(TopP p) {
     const void *mrow = nullptr;
     if constexpr (MK != NT_MASK_NONE) mrow = static_cast<const char *>(p.mask) + mask_row_at(p.mm, row) * MaskWords<MK>::kBytes;
     const bool tau_one = p.tau_one != 0;
-    const int c1 = min(p.nc, (seg + 1) * p.per);
-    if (threadIdx.x == 0) {
-        s.count = 0;
-        s.least = (uint64_t(kNone) << 32) | 0xffffffffu;
-    }
-    __syncthreads();
+    const int c0 = seg * p.per, c1 = min(p.nc, c0 + p.per);
+    // the wave's chunks are c0 + wave + 4 j; group q of a lane has j in [q cpg, q cpg + cpg)
+    const int J = (c1 - c0 + kTopWaves - 1) / kTopWaves, cpg = (J + F::G - 1) / F::G;
+    if (threadIdx.x == 0) s.count = s.groups = 0;
     double S = 0.0;
     float a = -INFINITY;
-    bool bounded = false;  // (the list has a threshold of its own)
-    for (int t0 = seg * p.per; t0 < c1; t0 += NC * kTopWaves) {
-        Raw<DT, MK> raw[NC];
+    for (int q = 0; q < F::G; q++) {
+        float gm = -INFINITY;
+        const int j1 = min(J, (q + 1) * cpg);
+        for (int j = q * cpg; j < j1; j += kTopBatch) {
+            Raw<DT, MK> raw[kTopBatch];
 #pragma unroll
-        for (int i = 0; i < NC; i++) {
-            const int ch = t0 + i * kTopWaves + wave;
-            load_raw<DT, MK, AL>(raw[i], xrow, mrow, ch < c1 ? int64_t(ch) * kChunk + lane * kEpl : p.V, p.V);
-        }
-        uint32_t held[NC][W];
-        float gm[NC];
-        float m = -INFINITY;
-#pragma unroll
-        for (int i = 0; i < NC; i++) {
-            float v[kEpl];
-            decode<DT, MK>(raw[i], v, p.tau, tau_one);
-#pragma unroll
-            for (int j = 0; j < W; j++) held[i][j] = HALF ? raw[i].x[j] : __float_as_uint(v[j]);
-            if constexpr (HALF && MK == NT_MASK_U8) fold_values<DT>(held[i], v);
-            gm[i] = max8(v);
-            m = fmaxf(m, gm[i]);
-        }
-        // the log-sum-exp's part, relative to the larger of the wave's maximum so far and the tile's
-        m = fmaxf(wave_max(m), a);
-        const float sh = m == -INFINITY ? 0.0f : m;
-        float sum = 0.0f;
-#pragma unroll
-        for (int i = 0; i < NC; i++) {
-            float w[kEpl];
-#pragma unroll
-            for (int j = 0; j < kEpl; j++) w[j] = exp2_hw((logit<HDT>(held[i], j) - sh) * p.c);
-            sum += tree8(w);
-        }
-        if (a != m && a != -INFINITY) S *= exp2((double(a) - double(m)) * double(p.c));
-        S += wave_sum_d(double(sum));
-        a = m;
-
-        // the threshold, once k groups' maxima give one
-        auto bound_by_groups = [&]() {
-            uint32_t g[NC];
-#pragma unroll
-            for (int i = 0; i < NC; i++) g[i] = ordered(gm[i]);
-            const uint32_t b = kth_bound<uint32_t, NC>(s, g, p.k, 2 * p.k);
-            if (threadIdx.x == 0 && b > kNone && (uint64_t(b) << 32) - 1 > s.least) s.least = (uint64_t(b) << 32) - 1;
-            __syncthreads();
-            return b > kNone;
-        };
-        // the elements of chunks i0 .. i1 - 1 above the threshold, as far as the list holds them
-        auto append = [&](int i0, int i1) {
-            const uint64_t least = s.least;
-            const float lf = unordered(uint32_t(least >> 32));
-#pragma unroll
-            for (int i = 0; i < NC; i++) {
-                if (i < i0 || i >= i1 || __ballot(gm[i] >= lf) == 0) continue;
-                const uint32_t e0 = uint32_t(t0 + i * kTopWaves + wave) * kChunk + lane * kEpl;
-#pragma unroll
-                for (int j = 0; j < kEpl; j++) {
-                    const float v = logit<HDT>(held[i], j);
-                    const uint64_t key = (uint64_t(ordered(v)) << 32) | uint32_t(~(e0 + j));
-                    const bool in = v >= lf && key > least;
-                    const uint64_t b = __ballot(in);
-                    if (b == 0) continue;
-                    int at = 0;
-                    if (lane == int(__builtin_ctzll(b))) at = atomicAdd(&s.count, int(__popcll(b)));
-                    at = __builtin_amdgcn_readlane(at, __builtin_ctzll(b)) + int(__popcll(b & ((uint64_t(1) << lane) - 1)));
-                    if (in && at < kList) s.list[at] = key;
-                }
+            for (int i = 0; i < kTopBatch; i++) {
+                const int ch = c0 + wave + (j + i) * kTopWaves;
+                load_raw<DT, MK, AL>(raw[i], xrow, mrow, j + i < j1 && ch < c1 ? int64_t(ch) * kChunk + lane * kEpl : p.V, p.V);
             }
-        };
-        if (!bounded) bounded = bound_by_groups();
-        const int before = s.count;
-        __syncthreads();
-        append(0, NC);
-        __syncthreads();
-        int n = s.count;
-        __syncthreads();
-        if (n > kList) {
-            // more than the list holds: once more with the tile's own threshold, and if that does not help in groups
-            if (threadIdx.x == 0) s.count = before;
-            __syncthreads();
-            bounded = bound_by_groups() || bounded;
-            append(0, NC);
-            __syncthreads();
-            n = s.count;
-            __syncthreads();
-            if (n > kList) {
-                if (threadIdx.x == 0) s.count = before;
-                n = before;
-                __syncthreads();
-                for (int i = 0; i < NC; i++) {
-                    if (n > p.k) cut_list(s, n, p.k, true);
-                    append(i, i + 1);
-                    __syncthreads();
-                    n = s.count;
-                    __syncthreads();
-                }
+            float v[kTopBatch][kEpl];
+            float m = -INFINITY;
+#pragma unroll
+            for (int i = 0; i < kTopBatch; i++) {
+                decode<DT, MK>(raw[i], v[i], p.tau, tau_one);
+                m = fmaxf(m, max8(v[i]));
             }
+            gm = fmaxf(gm, m);
+            // relative to the lane's maximum so far
+            m = fmaxf(m, a);
+            const float sh = m == -INFINITY ? 0.0f : m;
+            float sum = 0.0f;
+#pragma unroll
+            for (int i = 0; i < kTopBatch; i++) {
+                float w[kEpl];
+#pragma unroll
+                for (int e = 0; e < kEpl; e++) w[e] = exp2_hw((v[i][e] - sh) * p.c);
+                sum += tree8(w);
+            }
+            S = S * double(exp2_hw((a - sh) * p.c)) + double(sum);
+            a = m;
         }
-        if (n > max(kKeep, 2 * p.k)) {
-            cut_list(s, n, p.k, false);
-            bounded = true;
-        }
+        s.gmax[q * kTopThreads + threadIdx.x] = gm;
     }
+    wave_merge(S, a, p.c);
     if (lane == 0) {
         s.S[wave] = S;
         s.a[wave] = a;
     }
+    // the threshold: what is on the list is above `least`
+    uint32_t g[F::G];
+#pragma unroll
+    for (int q = 0; q < F::G; q++) g[q] = ordered(s.gmax[q * kTopThreads + threadIdx.x]);  // (this thread's own)
+    uint32_t bound = kth_bound<uint32_t, F::G, BIG>(s, g, p.k, p.k + p.k / 8 + 16);
+    if (bound <= kNone) bound = kNone + 1;
+    const float lf = unordered(bound);
+    uint64_t least = (uint64_t(bound) << 32) - 1;
+    // the groups that reach it, their numbers where their maxima were
+    uint16_t *group = reinterpret_cast<uint16_t *>(s.gmax);
     __syncthreads();
-    waves_sum(s, p.c, &S, &a);
+#pragma unroll
+    for (int q = 0; q < F::G; q++) {
+        const bool in = g[q] >= bound;
+        const uint64_t b = __ballot(in);
+        if (b == 0) continue;
+        int at = 0;
+        if (lane == int(__builtin_ctzll(b))) at = atomicAdd(&s.groups, int(__popcll(b)));
+        at = __builtin_amdgcn_readlane(at, __builtin_ctzll(b));
+        if (in) group[at + __popcll(b & ((uint64_t(1) << lane) - 1))] = uint16_t(q * kTopThreads + threadIdx.x);
+    }
+    __syncthreads();
+    // v and its column, if it goes on the list: where, or kList and more where that is full
+    auto append = [&](float v, int64_t e) {
+        const uint64_t key = (uint64_t(ordered(v)) << 32) | uint32_t(~uint32_t(e));
+        if (!(v >= lf) || key <= least) return;
+        const int at = atomicAdd(&s.count, 1);
+        if (at < F::kList) s.list[at] = key;
+    };
+    const int items = s.groups * cpg;
+    for (int it = threadIdx.x; it < items; it += kTopThreads) {
+        const int id = group[it / cpg], q = id / kTopThreads, thread = id % kTopThreads;
+        const int j = q * cpg + it % cpg, ch = c0 + thread / kWave + j * kTopWaves;
+        if (j >= J || ch >= c1 || s.count > F::kList) continue;
+        const int64_t e0 = int64_t(ch) * kChunk + (thread % kWave) * kEpl;
+        Raw<DT, MK> raw;
+        float v[kEpl];
+        load_raw<DT, MK, AL>(raw, xrow, mrow, e0, p.V);
+        decode<DT, MK>(raw, v, p.tau, tau_one);
+#pragma unroll
+        for (int e = 0; e < kEpl; e++) append(v[e], e0 + e);
+    }
+    __syncthreads();
+    int n = s.count;
+    __syncthreads();
+    if (n > F::kList) {
+        // too many reach it (equal values): in the columns' order, the list cut whenever a round might not fit
+        if (threadIdx.x == 0) s.count = 0;
+        n = 0;
+        __syncthreads();
+        for (int t0 = c0; t0 < c1; t0 += F::kRound) {
+            if (n > F::kList - F::kRound * kChunk) {
+                least = cut_list(s, n, p.k);
+                __syncthreads();
+            }
+            if (wave < F::kRound && t0 + wave < c1) {
+                const int64_t e0 = int64_t(t0 + wave) * kChunk + lane * kEpl;
+                Raw<DT, MK> raw;
+                float v[kEpl];
+                load_raw<DT, MK, AL>(raw, xrow, mrow, e0, p.V);
+                decode<DT, MK>(raw, v, p.tau, tau_one);
+#pragma unroll
+                for (int e = 0; e < kEpl; e++) append(v[e], e0 + e);
+            }
+            __syncthreads();
+            n = s.count;
+            __syncthreads();
+        }
+    }
+    // (placing 512 entries costs less than cutting them)
+    if (n > (p.segs > 1 ? cand_of(p.k) : max(2 * p.k, 512))) {
+        cut_list(s, n, p.k);
+        n = p.k;
+    }
+    a = s.a[0];
+    for (int w = 1; w < kTopWaves; w++) a = fmaxf(a, s.a[w]);
+    S = 0.0;
+    for (int w = 0; w < kTopWaves; w++) S += s.a[w] == -INFINITY ? s.S[w] : s.S[w] * exp2((double(s.a[w]) - double(a)) * double(p.c));
     if (p.segs == 1) {
-        top_finish(s, p, row, S, a);
+        top_finish(s, p, row, n, S, a);
         return;
     }
-    int n = s.count;
-    if (n > 2 * p.k) {
-        cut_list(s, n, p.k, false);
-        n = s.count;
-    }
     const int64_t at = row * p.segs + seg;
-    for (int i = threadIdx.x; i < n; i += kTopThreads) p.cand[at * 2 * p.k + i] = s.list[i];
+    for (int i = threadIdx.x; i < n; i += kTopThreads) p.cand[at * cand_of(p.k) + i] = s.list[i];
     if (threadIdx.x == 0) p.rec[at] = TopRec{S, a, n};
 }
 
 // The rows of a launch with several workgroups a row.
+template <bool BIG>
 __global__ __launch_bounds__(kTopThreads) void k_top_finish(TopP p) {
-    __shared__ TopS s;
+    using F = TopForm<BIG>;
+    __shared__ TopS<BIG> s;
+    __shared__ int first[kTopSegs + 1];
     const int64_t row = blockIdx.x;
+    const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
     const TopRec *rec = p.rec + row * p.segs;
-    if (threadIdx.x == 0) {
-        s.count = 0;
-        s.least = 0;
+    // (every wave the same: a piece a lane)
+    TopRec r{0.0, -INFINITY, 0};
+    if (lane < p.segs) r = rec[lane];
+    double S = r.S;
+    float a = r.a;
+    wave_merge(S, a, p.c);
+    int before = r.n;
+#pragma unroll
+    for (int o = 1; o < kWave; o <<= 1) {
+        const int m = __shfl_up(before, o, kWave);
+        if (lane >= o) before += m;
     }
-    float a = -INFINITY;
-    for (int g = 0; g < p.segs; g++) a = fmaxf(a, rec[g].a);
-    double S = 0.0;
-    for (int g = 0; g < p.segs; g++)
-        S += rec[g].a == -INFINITY ? rec[g].S : rec[g].S * exp2((double(rec[g].a) - double(a)) * double(p.c));
-    int n = 0;
+    if (wave == 0) first[lane + 1] = before;
+    if (threadIdx.x == 0) first[0] = s.count = 0;
     __syncthreads();
-    for (int g = 0; g < p.segs; g++) {
-        const int more = rec[g].n;
-        if (n + more > kList) {
-            cut_list(s, n, p.k, true);
-            n = s.count;
-            __syncthreads();
+    const int stride = cand_of(p.k);
+    const uint64_t *cand = p.cand + row * p.segs * stride;
+    const int all = first[kTopSegs];
+    int n;
+    if (all <= F::kList) {
+        for (int g = wave; g < p.segs; g += kTopWaves)
+            for (int i = lane; i < first[g + 1] - first[g]; i += kWave) s.list[first[g] + i] = cand[g * stride + i];
+        n = all;
+        __syncthreads();
+    } else {
+        // a round of the list's free places at a time
+        n = 0;
+        for (int g = 0; g < p.segs; g++) {
+            const int more = first[g + 1] - first[g];
+            for (int i0 = 0; i0 < more;) {
+                if (n == F::kList) {
+                    cut_list(s, n, p.k);
+                    n = p.k;
+                    __syncthreads();
+                }
+                const int take = min(more - i0, F::kList - n);
+                for (int i = threadIdx.x; i < take; i += kTopThreads) s.list[n + i] = cand[g * stride + i0 + i];
+                n += take;
+                i0 += take;
+                __syncthreads();
+            }
         }
-        for (int i = threadIdx.x; i < more; i += kTopThreads) s.list[n + i] = p.cand[(row * p.segs + g) * 2 * p.k + i];
-        n += more;
-        __syncthreads();
-        if (threadIdx.x == 0) s.count = n;
-        __syncthreads();
     }
-    top_finish(s, p, row, S, a);
+    if (n > max(2 * p.k, 512)) {
+        cut_list(s, n, p.k);
+        n = p.k;
+    }
+    top_finish(s, p, row, n, S, a);
 }
 
 }  // namespace
@@ -410,7 +421,7 @@ extern "C" int nt_hip_rl_top_logprobs(const NtRlTopArgs *a) {
     p.status = a->status;
     void *ws = nullptr;
     if (p.segs > 1) {
-        const size_t n = size_t(a->rows) * size_t(p.segs), recs = n * sizeof(TopRec), need = recs + n * 16 * size_t(p.k);
+        const size_t n = size_t(a->rows) * size_t(p.segs), recs = n * sizeof(TopRec), need = recs + n * 8 * size_t(cand_of(p.k));
         bool cap = false;
         if (int rc = stream_capturing(&cap)) return rc;
         if (cap && need >= size_t(1) << 20)
@@ -425,8 +436,14 @@ extern "C" int nt_hip_rl_top_logprobs(const NtRlTopArgs *a) {
     const dim3 grid(unsigned(a->rows * p.segs));
     auto by_al = [&](auto dt, auto mk) {
         constexpr int DT = decltype(dt)::value, MK = decltype(mk)::value;
-        if (al) hipLaunchKernelGGL((k_top<DT, MK, true>), grid, dim3(kTopThreads), 0, s, p);
-        else hipLaunchKernelGGL((k_top<DT, MK, false>), grid, dim3(kTopThreads), 0, s, p);
+        auto by_k = [&](auto big) {
+            constexpr bool BIG = decltype(big)::value;
+            if (al) hipLaunchKernelGGL((k_top<DT, MK, true, BIG>), grid, dim3(kTopThreads), 0, s, p);
+            else hipLaunchKernelGGL((k_top<DT, MK, false, BIG>), grid, dim3(kTopThreads), 0, s, p);
+            if (p.segs > 1) hipLaunchKernelGGL(k_top_finish<BIG>, dim3(unsigned(a->rows)), dim3(kTopThreads), 0, s, p);
+        };
+        if (p.k > kFewK) by_k(std::true_type{});
+        else by_k(std::false_type{});
     };
     auto by_mk = [&](auto dt) {
         if (a->mask_kind == NT_MASK_U8) by_al(dt, std::integral_constant<int, NT_MASK_U8>{});
@@ -436,7 +453,6 @@ extern "C" int nt_hip_rl_top_logprobs(const NtRlTopArgs *a) {
     if (a->dtype == NT_F32) by_mk(std::integral_constant<int, NT_F32>{});
     else if (a->dtype == NT_BF16) by_mk(std::integral_constant<int, NT_BF16>{});
     else by_mk(std::integral_constant<int, NT_F16>{});
-    if (p.segs > 1) hipLaunchKernelGGL(k_top_finish, dim3(unsigned(a->rows)), dim3(kTopThreads), 0, s, p);
     const int rc = launched(who);
     const int rc2 = scratch_release(ws);
     return rc ? rc : rc2;
