@@ -1,8 +1,10 @@
 """Drafted tokens' verification (verify_drafted) against a plain f64 form of its definition.
 
-The kernels evaluate everything in f64, with exponentials within 2e-14: every id and count has to be equal (a draw lies
-within 1e-13 of a token's border with a probability of about 1e-9 a test). A log-probability is a difference of f64
-values within 1e-12, rounded once: half an f32 step of its value and 1e-12."""
+Everything that decides a token is evaluated in f64, with exponentials within 2e-14: every id and count has to be equal (a
+draw lies within 1e-13 of a token's border with a probability of about 1e-9 a test). A log-probability is a
+difference of f64 values within 1e-12, rounded once: half an f32 step of its value and 1e-12. From 256 positions on, and
+greedily, an accepted draft's (and the greedy token's) log-sum-exp is of f32 exponentials: within 6e-6 in log2 units, 4.2e-6
+here, and of an additive mask's f32 sums within half a step of the largest, 2^-24 of it."""
 import ctypes as C
 
 import numpy as np
@@ -43,12 +45,15 @@ def run(x, y, mt, tokens, u, lengths, dtype, T, **kw):
                              lengths=None if lengths is None else nr.Tensor.from_numpy(lengths), **kw)
 
 
-def compare(got, want):
+def compare(got, want, greedy=False, largest=0.0):
     ids, acc, lp = (t.to_numpy() for t in got)
     wi, wa, wl = want
     assert np.array_equal(acc, wa)
     assert np.array_equal(ids, wi)
-    assert (np.abs(lp - wl) <= 2.0 ** -24 * np.abs(wl) + 1e-12).all()
+    f32 = np.full(wl.shape, greedy or wl.size >= 256)
+    if not greedy:
+        f32[np.arange(len(wl)), wa] = False
+    assert (np.abs(lp - wl) <= 2.0 ** -24 * np.abs(wl) + np.where(f32, 4.2e-6 + 2.0 ** -24 * largest, 1e-12)).all()
 
 
 CASES = [
@@ -80,7 +85,7 @@ def test_against_the_definition(case):
     x, y, z, zq, mt, tokens, u, lengths = inputs(S, K, V, dtype, kind, T, rng, shared, draft and K > 0, ragged)
     want = ref.verify(z, zq, tokens, u, lengths, T == 0.0)
     got = run(x, y, mt, tokens, u, lengths if ragged else None, dtype, T)
-    compare(got, want)
+    compare(got, want, T == 0.0, np.abs(z.max()) if kind == "f32" else 0.0)
     again = run(x, y, mt, tokens, u, lengths if ragged else None, dtype, T)
     for a, b in zip(got, again):
         assert a.to_numpy().tobytes() == b.to_numpy().tobytes()
