@@ -8,30 +8,30 @@
 namespace nt {
 namespace {
 
-// 2^t for t <= 1000 within 2e-14 relative; t below -1100 (and a NaN: the callers look for those
-// themselves) gives 0. 2^n by v_ldexp_f64 with n = t to the nearest whole number, taken by the addition of
-// 1.5 2^52, which leaves n in the sum's low word, times 2^f for f in [-1/2, 1/2]: the polynomial that
-// agrees with 2^f at the ten Chebyshev nodes of that interval (its largest relative error is 1.8e-14). f64 fma, add
-// and max run at the f32 rate here, 16 lanes a clock and SIMD, so that 16 instructions are 64 clocks a wave.
-__device__ __forceinline__ double exp2_64(double t) {
-    t = fmax(t, -1100.0);
-    const double y = t + 0x1.8p52;
+constexpr double kLog2e64 = 1.4426950408889634074;
+
+// 2^(d c) for d c <= 1000 within 2e-12 relative and 0 for d at least `low` below 0 (low c is -1100; a NaN gives 0 too: the
+// callers look for those themselves). 2^n by v_ldexp_f64 with n = d c to the nearest whole number, taken by an fma
+// onto 1.5 2^52, which leaves n in the low word, times 2^f for f in [-1/2, 1/2]: the polynomial that agrees with
+// 2^f at the nine Chebyshev nodes of that interval (its largest relative error is 1.1e-12). An f64 instruction of
+// any of these kinds takes 4.5 clocks a wave where an f32 fma takes 2.4 and v_exp_f32 8.2 (measured), so that a weight with
+// its conversion, difference and addition is 72 clocks, against about 20 in f32.
+__device__ __forceinline__ double exp2_64(double d, double c, double low) {
+    d = fmax(d, low);
+    const double y = fma(d, c, 0x1.8p52);
     const int n = int(uint32_t(uint64_t(__double_as_longlong(y))));
-    const double f = t - (y - 0x1.8p52);
-    double p = 0x1.b6571de2f2351p-24;
-    p = fma(p, f, 0x1.63ef969a64d3cp-20);
-    p = fma(p, f, 0x1.ffcb76789860fp-17);
-    p = fma(p, f, 0x1.43088e257f341p-13);
-    p = fma(p, f, 0x1.5d87fe908f88ap-10);
-    p = fma(p, f, 0x1.3b2ab72b175eep-7);
-    p = fma(p, f, 0x1.c6b08d7044119p-5);
-    p = fma(p, f, 0x1.ebfbdff8149f2p-3);
-    p = fma(p, f, 0x1.62e42fefa39f7p-1);
-    p = fma(p, f, 0x1.000000000003dp+0);
+    const double f = fma(d, c, 0x1.8p52 - y);
+    double p = 0x1.63d136366db24p-20;
+    p = fma(p, f, 0x1.00dc4a532fb8ep-16);
+    p = fma(p, f, 0x1.4308ac85aa947p-13);
+    p = fma(p, f, 0x1.5d8745a728441p-10);
+    p = fma(p, f, 0x1.3b2ab7181b755p-7);
+    p = fma(p, f, 0x1.c6b08dd6fd234p-5);
+    p = fma(p, f, 0x1.ebfbdff823cedp-3);
+    p = fma(p, f, 0x1.62e42fef84cf0p-1);
+    p = fma(p, f, 1.0);
     return __builtin_ldexp(p, n);
 }
-
-constexpr double kLog2e64 = 1.4426950408889634074;
 
 }  // namespace
 }  // namespace nt

@@ -1,0 +1,175 @@
+// A row's chunks loaded without a branch, and sums of 2^(v c) over its values v in f32 exponentials, one lane's share,
+// with f64 totals.
+#pragma once
+
+#include "nt_exp64.hpp"
+#include "nt_rows.hpp"
+
+namespace nt {
+namespace {
+
+// A row's loads, none under a condition: with one, the compiler lets every load wait for the one before it, whose registers
+// the other branch would write (64 of 4096 x 50304: 108 us; without 72). AL (aligned_rows, row bytes below 2^31): buffer
+// loads, zeros past the row's end. Otherwise loads at the elements' own alignment, the row's last ones from 8 columns
+// before its end, so that a lane there holds columns of its neighbour too; rows of under 8 columns by elements.
+// Lane l of chunk ch has columns first() .. first() + 7, of which those below own() or not below V are not its own:
+// only in the row's last chunk, where clean() gives them -inf.
+template <int DT, int MK, bool AL>
+struct RowLoad {
+    const void *x, *m;
+    __amdgpu_buffer_rsrc_t xr, mr;
+    int64_t V;
+    int last;
+
+    __device__ __forceinline__ RowLoad(const void *xrow, const void *mrow, int64_t V_, int nc) : x(xrow), m(mrow), V(V_), last(nc - 1) {
+        if constexpr (AL) {
+            xr = __builtin_amdgcn_make_buffer_rsrc(const_cast<void *>(xrow), short(0), int(V) * Elem<DT>::kBytes, kBufferWord3);
+            mr = xr;
+            if constexpr (MK != NT_MASK_NONE)
+                mr = __builtin_amdgcn_make_buffer_rsrc(const_cast<void *>(mrow), short(0), int(V) * MaskWords<MK>::kBytes, kBufferWord3);
+        }
+    }
+    static __device__ __forceinline__ int64_t own(int ch, int lane) { return int64_t(ch) * kChunk + lane * kEpl; }
+    __device__ __forceinline__ int64_t first(int ch, int lane) const {
+        const int64_t e0 = own(ch, lane);
+        if constexpr (AL) return e0;
+        else return V < kEpl ? e0 : (e0 + kEpl <= V ? e0 : V - kEpl);
+    }
+    // The raw words of chunk ch (in: the row has it; otherwise anything).
+    __device__ __forceinline__ void load(Raw<DT, MK> &r, int ch, int lane, bool in = true) const {
+        if constexpr (AL) {
+            const int e0 = in ? int(own(ch, lane)) : int(V);
+#pragma unroll
+            for (int q = 0; q < Elem<DT>::kWords / 4; q++) {
+                const auto a = __builtin_amdgcn_raw_buffer_load_b128(xr, e0 * Elem<DT>::kBytes + 16 * q, 0, 0);
+#pragma unroll
+                for (int i = 0; i < 4; i++) r.x[4 * q + i] = a[i];
+            }
+            if constexpr (MK == NT_MASK_U8) {
+                const auto k = __builtin_amdgcn_raw_buffer_load_b64(mr, e0, 0, 0);
+                r.m[0] = k[0];
+                r.m[1] = k[1];
+            } else if constexpr (MK == NT_MASK_F32) {
+#pragma unroll
+                for (int q = 0; q < 2; q++) {
+                    const auto a = __builtin_amdgcn_raw_buffer_load_b128(mr, e0 * 4 + 16 * q, 0, 0);
+#pragma unroll
+                    for (int i = 0; i < 4; i++) r.m[4 * q + i] = a[i];
+                }
+            }
+        } else if (V < kEpl) {
+            load_raw<DT, MK, false>(r, x, m, in ? own(ch, lane) : V, V);
+        } else {
+            const int64_t e = in ? first(ch, lane) : 0;
+            if constexpr (DT == NT_F32) {
+                const u32x4_f32 *q = reinterpret_cast<const u32x4_f32 *>(static_cast<const float *>(x) + e);
+                const u32x4_f32 a = q[0], b = q[1];
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    r.x[i] = a[i];
+                    r.x[4 + i] = b[i];
+                }
+            } else {
+                const u32x4_f16 a = *reinterpret_cast<const u32x4_f16 *>(static_cast<const uint16_t *>(x) + e);
+#pragma unroll
+                for (int i = 0; i < 4; i++) r.x[i] = a[i];
+            }
+            if constexpr (MK == NT_MASK_U8) {
+                const u32x2_u8 k = *reinterpret_cast<const u32x2_u8 *>(static_cast<const uint8_t *>(m) + e);
+                r.m[0] = k[0];
+                r.m[1] = k[1];
+            } else if constexpr (MK == NT_MASK_F32) {
+                const u32x4_f32 *q = reinterpret_cast<const u32x4_f32 *>(static_cast<const float *>(m) + e);
+                const u32x4_f32 a = q[0], b = q[1];
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    r.m[i] = a[i];
+                    r.m[4 + i] = b[i];
+                }
+            }
+        }
+    }
+    // Whether column first() + j of the lane is its own.
+    __device__ __forceinline__ bool mine(int ch, int lane, int j) const {
+        const int64_t e = first(ch, lane) + j;
+        return e >= own(ch, lane) && e < V;
+    }
+    __device__ __forceinline__ void clean(float v[kEpl], int ch, int lane) const {
+        if (ch != last) return;
+#pragma unroll
+        for (int j = 0; j < kEpl; j++) v[j] = mine(ch, lane, j) ? v[j] : -INFINITY;
+    }
+};
+
+// N sums (of all weights, of some) relative to the lane's reference: the first maximum it met, moved only where a later
+// value lies 60 log2 units above it, so that most chunks cost a weight one fma, one exponential and one addition. The
+// reference is kept as the f32 product -ref c that the fma adds, and what its rounding and c's leave of it goes
+// into at(). Products past 2^20, whose f32 steps are no small part of a log2 unit, are taken by differences.
+// A weight is within 2^-23 (the instruction) and |t| 2^-23 ln 2 of its argument t (the fma's rounding and
+// c's); a NaN or +inf leaves a NaN in S[0].
+template <int N>
+struct LaneSums {
+    double S[N] = {};
+    float ref = -INFINITY, neg = 0.0f, lim = -INFINITY;
+
+    // Takes `top`, not below the limit (a NaN among others), into the reference; whether weights go by the fma.
+    __device__ __forceinline__ bool settle(float top, float c) {
+        if (!(top < INFINITY)) {
+            S[0] = NAN;
+            return true;
+        }
+        const float r = fmaxf(ref, top), now = -(r * c);
+        const bool far = fabsf(now) > 0x1p20f;
+        if (ref != -INFINITY) {
+            const double was = lim == -INFINITY ? -double(ref) * double(c) : double(neg);
+            const double f = exp2_64((far ? -double(r) * double(c) : double(now)) - was, 1.0, -1100.0);
+#pragma unroll
+            for (int i = 0; i < N; i++) S[i] *= f;
+        }
+        ref = r;
+        neg = now;
+        lim = far ? -INFINITY : r + 60.0f / c;
+        return !far;
+    }
+    // The weights of 8 values; their maximum.
+    __device__ __forceinline__ float weigh(const float v[kEpl], float c, float w[kEpl]) {
+        const float top = max8_hw(v);
+        bool fast = top <= lim;
+        // (lanes without a token so far have none here either: their weights are 0)
+        if (!fast && !(top == -INFINITY)) fast = settle(top, c);
+        else fast = true;
+        if (fast) {
+#pragma unroll
+            for (int j = 0; j < kEpl; j++) w[j] = exp2_hw(fmaf(v[j], c, neg));
+        } else {
+#pragma unroll
+            for (int j = 0; j < kEpl; j++) w[j] = exp2_hw((v[j] - ref) * c);
+        }
+        return top;
+    }
+    __device__ __forceinline__ float add(const float v[kEpl], float c) {
+        float w[kEpl];
+        const float top = weigh(v, c, w);
+        S[0] += double(tree8(w));
+        return top;
+    }
+    // The value whose weight is 1 (c: what c32 is the f32 of); -inf where the lane met no token.
+    __device__ __forceinline__ double at(double c, float c32) const {
+        if (ref == -INFINITY || lim == -INFINITY) return double(ref);
+        return -(double(neg) + double(ref) * (double(c32) - c)) / c;
+    }
+};
+
+__device__ __forceinline__ double wave_max_d(double v) {
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) v = fmax(v, __shfl_xor(v, o, kWave));
+    return v;
+}
+
+// S relative to a, moved to the reference `to` (at least a); low: -1100 / c.
+__device__ __forceinline__ double moved(double S, double a, double to, double c, double low) {
+    return a == -INFINITY || a == to ? S : S * exp2_64(a - to, c, low);
+}
+
+}  // namespace
+}  // namespace nt

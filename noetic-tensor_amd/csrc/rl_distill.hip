@@ -16,6 +16,7 @@
 
 #include "nt_exp64.hpp"
 #include "nt_rows.hpp"
+#include "nt_rowsum.hpp"
 
 namespace nt {
 namespace {
@@ -27,18 +28,16 @@ constexpr int kMaxListed = 1024;
 constexpr int kMapChunks = 512;               // chunks a workgroup's bitmap covers: 2^18 columns, 32 KiB
 
 struct DistillRec {
-    double S, R;   // sum over the piece, and over its columns off the list, relative to a
-    float a;
-    int32_t bad;   // an id outside the vocabulary, or one listed twice
-    int64_t pad;
+    double S, R, a;  // sum over the piece, and over its columns off the list, relative to a
+    int64_t bad;     // an id outside the vocabulary, or one listed twice
 };
 
 struct DistillP {
     const void *x, *mask;
     int64_t V, ld;
     MaskMap mm;
-    float c;            // exponent scale of a value: log2(e) / T (none, u8) or log2(e) (f32 mask)
-    float tau;
+    double c, low;      // exponent scale of a value: log2(e) / T (none, u8) or log2(e) (f32 mask); -1100 / c
+    float c32, tau;
     int tau_one;
     double inv_t;       // 1 / T
     int nc, segs, per;
@@ -112,7 +111,7 @@ __device__ void distill_finish(const DistillP &p, int64_t row, const DistillRec 
         for (int j = threadIdx.x; j < p.k; j += kDistillThreads) {
             if (ids[j] < 0) continue;
             const double lw = double(teacher[j]) - ln_norm, w = exp(lw);
-            const double lq = listed_z<DT, MK>(p, xrow, mrow, ids[j], double(r.a)) - ln_s, d = lq - lw;
+            const double lq = listed_z<DT, MK>(p, xrow, mrow, ids[j], r.a) - ln_s, d = lq - lw;
             mass += w;
             if (p.tail != NT_TAIL_REST) {
                 if (!(w == 0.0)) loss -= w * d;
@@ -143,8 +142,10 @@ __device__ void distill_finish(const DistillP &p, int64_t row, const DistillRec 
     p.loss[row] = st == NT_ROW_OK ? float(loss) : NAN;
     p.status[row] = uint8_t(st);
     double *o = p.stats + row * NT_DISTILL_STATS;
-    o[0] = double(r.a);
-    o[1] = st == NT_ROW_OK ? r.S : NAN;
+    // (the backward's f32 base: a value)
+    const double base = double(float(r.a));
+    o[0] = base;
+    o[1] = st == NT_ROW_OK ? r.S * exp2((r.a - base) * p.c) : NAN;
     o[2] = total - share;
     o[3] = total;
     o[4] = ln_norm;
@@ -180,61 +181,45 @@ __global__ __launch_bounds__(kDistillThreads) void k_distill(DistillP p) {
     __syncthreads();
     const uint8_t *bytes = reinterpret_cast<const uint8_t *>(map);
 
-    double S = 0.0, R = 0.0;
-    float a = -INFINITY;
+    const RowLoad<DT, MK, AL> in(xrow, mrow, p.V, p.nc);
+    LaneSums<2> sum;
     for (int t0 = c0 + wave; t0 < c1; t0 += kDistillBatch * kDistillWaves) {
         Raw<DT, MK> raw[kDistillBatch];
 #pragma unroll
         for (int i = 0; i < kDistillBatch; i++) {
             const int ch = t0 + i * kDistillWaves;
-            load_raw<DT, MK, AL>(raw[i], xrow, mrow, ch < c1 ? int64_t(ch) * kChunk + lane * kEpl : p.V, p.V);
+            in.load(raw[i], ch, lane, ch < c1);
         }
-        float v[kDistillBatch][kEpl];
-        float m = -INFINITY;
-#pragma unroll
-        for (int i = 0; i < kDistillBatch; i++) {
-            decode<DT, MK>(raw[i], v[i], p.tau, tau_one);
-            m = fmaxf(m, max8(v[i]));
-        }
-        m = fmaxf(wave_max(m), a);
-        const float sh = m == -INFINITY ? 0.0f : m;
-        float sum = 0.0f, off = 0.0f;
 #pragma unroll
         for (int i = 0; i < kDistillBatch; i++) {
             const int ch = t0 + i * kDistillWaves;
-            float w[kEpl];
+            if (ch < c1) {
+                float v[kEpl], w[kEpl];
+                decode<DT, MK>(raw[i], v, p.tau, tau_one);
+                in.clean(v, ch, lane);
+                sum.weigh(v, p.c32, w);
+                float t = tree8(w);
+                sum.S[0] += double(t);
+                // (bit j for column first() + j: past the row's end a lane's own columns come after its neighbour's)
+                const uint32_t on = uint32_t(bytes[(ch - c0) * kWave + lane]) << min(int64_t(8), in.own(ch, lane) - in.first(ch, lane));
+                if (__ballot(on != 0) != 0) {
 #pragma unroll
-            for (int j = 0; j < kEpl; j++) w[j] = exp2_hw((v[i][j] - sh) * p.c);
-            const float t = tree8(w);
-            sum += t;
-            const uint32_t on = ch < c1 ? bytes[(ch - c0) * kWave + lane] : 0u;
-            if (__ballot(on != 0) == 0) {
-                off += t;
-            } else {
-#pragma unroll
-                for (int j = 0; j < kEpl; j++) w[j] = (on >> j) & 1u ? 0.0f : w[j];
-                off += tree8(w);
+                    for (int j = 0; j < kEpl; j++) w[j] = (on >> j) & 1u ? 0.0f : w[j];
+                    t = tree8(w);
+                }
+                sum.S[1] += double(t);
             }
         }
-        if (a != m && a != -INFINITY) {
-            const double f = exp2((double(a) - double(m)) * double(p.c));
-            S *= f;
-            R *= f;
-        }
-        S += double(sum);
-        R += double(off);
-        a = m;
     }
-    S = wave_sum_d(S);
-    R = wave_sum_d(R);
-    if (lane == 0) ws[wave] = DistillRec{S, R, a, 0, 0};
+    const double at = sum.at(p.c, p.c32), top = wave_max_d(at);
+    const double S = wave_sum_d(moved(sum.S[0], at, top, p.c, p.low)), R = wave_sum_d(moved(sum.S[1], at, top, p.c, p.low));
+    if (lane == 0) ws[wave] = DistillRec{S, R, top, 0};
     __syncthreads();
-    DistillRec r{0.0, 0.0, ws[0].a, bad, 0};
-    for (int w = 1; w < kDistillWaves; w++) r.a = fmaxf(r.a, ws[w].a);
+    DistillRec r{0.0, 0.0, ws[0].a, bad};
+    for (int w = 1; w < kDistillWaves; w++) r.a = fmax(r.a, ws[w].a);
     for (int w = 0; w < kDistillWaves; w++) {
-        const double f = ws[w].a == -INFINITY ? 1.0 : exp2((double(ws[w].a) - double(r.a)) * double(p.c));
-        r.S += ws[w].S * f;
-        r.R += ws[w].R * f;
+        r.S += moved(ws[w].S, ws[w].a, r.a, p.c, p.low);
+        r.R += moved(ws[w].R, ws[w].a, r.a, p.c, p.low);
     }
     if (p.segs > 1) {
         if (threadIdx.x == 0) p.rec[row * p.segs + seg] = r;
@@ -249,15 +234,14 @@ __global__ __launch_bounds__(kDistillThreads) void k_distill_finish(DistillP p) 
     __shared__ double red[kDistillWaves];
     const int64_t row = blockIdx.x;
     const DistillRec *rec = p.rec + row * p.segs;
-    DistillRec r{0.0, 0.0, -INFINITY, 0, 0};
+    DistillRec r{0.0, 0.0, -INFINITY, 0};
     for (int g = 0; g < p.segs; g++) {
-        r.a = fmaxf(r.a, rec[g].a);
+        r.a = fmax(r.a, rec[g].a);
         r.bad |= rec[g].bad;
     }
     for (int g = 0; g < p.segs; g++) {
-        const double f = rec[g].a == -INFINITY ? 1.0 : exp2((double(rec[g].a) - double(r.a)) * double(p.c));
-        r.S += rec[g].S * f;
-        r.R += rec[g].R * f;
+        r.S += moved(rec[g].S, rec[g].a, r.a, p.c, p.low);
+        r.R += moved(rec[g].R, rec[g].a, r.a, p.c, p.low);
     }
     distill_finish<DT, MK>(p, row, r, red);
 }
@@ -272,6 +256,12 @@ __device__ __forceinline__ uint32_t pack2(float a, float b) {
     } else {
         return uint32_t(__builtin_bit_cast(uint16_t, _Float16(a))) | (uint32_t(__builtin_bit_cast(uint16_t, _Float16(b))) << 16);
     }
+}
+
+template <int GDT>
+__device__ __forceinline__ void store1(void *grow, int64_t e, float o) {
+    if constexpr (GDT == NT_F32) static_cast<float *>(grow)[e] = o;
+    else static_cast<uint16_t *>(grow)[e] = uint16_t(pack2<GDT>(o, o));
 }
 
 // 8 gradients at column e0; AL: 16-byte aligned, all inside the row.
@@ -296,10 +286,7 @@ __device__ __forceinline__ void store8(void *grow, int64_t e0, int64_t V, const 
         }
         return;
     }
-    for (int j = 0; j < kEpl && e0 + j < V; j++) {
-        if constexpr (GDT == NT_F32) static_cast<float *>(grow)[e0 + j] = o[j];
-        else static_cast<uint16_t *>(grow)[e0 + j] = uint16_t(pack2<GDT>(o[j], o[j]));
-    }
+    for (int j = 0; j < kEpl && e0 + j < V; j++) store1<GDT>(grow, e0 + j, o[j]);
 }
 
 template <int DT, int MK, int GDT, bool AL>
@@ -322,21 +309,29 @@ __global__ __launch_bounds__(kDistillThreads) void k_distill_grad(DistillP p) {
     const double base = st[0], S = st[1], scale = double(g) * p.inv_t;
     const float a = float(base), factor = float(scale * st[2] / S);
     const bool tau_one = p.tau_one != 0;
-    for (int t0 = c0 + wave; t0 < c1; t0 += 2 * kDistillWaves) {
-        Raw<DT, MK> raw[2];
+    const RowLoad<DT, MK, AL> in(xrow, mrow, p.V, p.nc);
+    for (int t0 = c0 + wave; t0 < c1; t0 += kDistillBatch * kDistillWaves) {
+        Raw<DT, MK> raw[kDistillBatch];
 #pragma unroll
-        for (int i = 0; i < 2; i++) {
+        for (int i = 0; i < kDistillBatch; i++) {
             const int ch = t0 + i * kDistillWaves;
-            load_raw<DT, MK, AL>(raw[i], xrow, mrow, ch < c1 ? int64_t(ch) * kChunk + lane * kEpl : p.V, p.V);
+            in.load(raw[i], ch, lane, ch < c1);
         }
 #pragma unroll
-        for (int i = 0; i < 2; i++) {
+        for (int i = 0; i < kDistillBatch; i++) {
             const int ch = t0 + i * kDistillWaves;
-            float v[kEpl], o[kEpl];
-            decode<DT, MK>(raw[i], v, p.tau, tau_one);
+            if (ch < c1) {
+                float v[kEpl], o[kEpl];
+                decode<DT, MK>(raw[i], v, p.tau, tau_one);
 #pragma unroll
-            for (int j = 0; j < kEpl; j++) o[j] = fmaf(exp2_hw((v[j] - a) * p.c), factor, 0.0f);
-            if (ch < c1) store8<GDT, AL>(grow, int64_t(ch) * kChunk + lane * kEpl, p.V, o);
+                for (int j = 0; j < kEpl; j++) o[j] = fmaf(exp2_hw((v[j] - a) * p.c32), factor, 0.0f);
+                if (AL || in.first(ch, lane) == in.own(ch, lane)) {
+                    store8<GDT, AL>(grow, in.own(ch, lane), p.V, o);
+                } else {
+                    for (int j = 0; j < kEpl; j++)
+                        if (in.mine(ch, lane, j)) store1<GDT>(grow, in.first(ch, lane) + j, o[j]);
+                }
+            }
         }
     }
     // the listed columns of this piece, over what was just written there
@@ -425,7 +420,9 @@ int nt_hip_rl_distill(const NtRlDistillArgs *a) {
     p.mm = mm;
     p.tau = float(a->temperature);
     p.tau_one = a->temperature == 1.0;
-    p.c = a->mask_kind == NT_MASK_F32 || p.tau_one ? kLog2e : float(kLog2e64 / a->temperature);
+    p.c = a->mask_kind == NT_MASK_F32 ? kLog2e64 : kLog2e64 / a->temperature;
+    p.c32 = float(p.c);
+    p.low = -1100.0 / p.c;
     p.inv_t = 1.0 / a->temperature;
     p.nc = int((a->vocab + kChunk - 1) / kChunk);
     cut_rows(a->rows, p.nc, 1024, kMapChunks, &p.segs, &p.per);
@@ -447,7 +444,7 @@ int nt_hip_rl_distill(const NtRlDistillArgs *a) {
         if (int rc = scratch_alloc(need, &ws)) return rc;
         p.rec = static_cast<DistillRec *>(ws);
     }
-    const bool al = aligned_rows(a->logits, a->vocab, a->ld, a->dtype, a->mask_kind, a->mask, mm);
+    const bool al = aligned_rows(a->logits, a->vocab, a->ld, a->dtype, a->mask_kind, a->mask, mm) && a->vocab * 4 <= 0x7fffffffLL;
     hipStream_t s = ctx().stream;
     by_dtype(a->dtype, a->mask_kind, [&](auto dt, auto mk) {
         constexpr int DT = decltype(dt)::value, MK = decltype(mk)::value;
@@ -485,7 +482,9 @@ int nt_hip_rl_distill_backward(const NtRlDistillGradArgs *a) {
     p.mm = mm;
     p.tau = float(a->temperature);
     p.tau_one = a->temperature == 1.0;
-    p.c = a->mask_kind == NT_MASK_F32 || p.tau_one ? kLog2e : float(kLog2e64 / a->temperature);
+    p.c = a->mask_kind == NT_MASK_F32 ? kLog2e64 : kLog2e64 / a->temperature;
+    p.c32 = float(p.c);
+    p.low = -1100.0 / p.c;
     p.inv_t = 1.0 / a->temperature;
     p.nc = int((a->vocab + kChunk - 1) / kChunk);
     cut_rows(a->rows, p.nc, 4096, kMapChunks, &p.segs, &p.per);
@@ -496,7 +495,7 @@ int nt_hip_rl_distill_backward(const NtRlDistillGradArgs *a) {
     p.g = a->g_loss;
     p.grad = a->grad;
     p.gld = a->grad_ld;
-    const bool al = aligned_rows(a->logits, a->vocab, a->ld, a->dtype, a->mask_kind, a->mask, mm) &&
+    const bool al = aligned_rows(a->logits, a->vocab, a->ld, a->dtype, a->mask_kind, a->mask, mm) && a->vocab * 4 <= 0x7fffffffLL &&
                     a->grad_ld % kEpl == 0 && reinterpret_cast<uintptr_t>(a->grad) % 16 == 0;
     hipStream_t s = ctx().stream;
     by_dtype(a->dtype, a->mask_kind, [&](auto dt, auto mk) {

@@ -1,10 +1,10 @@
 // nt_hip_rl_top_logprobs: the k most likely tokens of each row and their log-probabilities, in one pass.
 //
 // A workgroup streams its row (or, where rows are few, a piece of one) once, and takes from it the log-sum-exp and the
-// largest value of each group of columns: a lane's columns in a quarter (of 256 k: a sixteenth) of the row. With
-// t the k-th largest of those 1024 (4096) maxima, k groups reach t, so k columns do, and the columns
+// largest value of each group of columns: a lane's columns in an eighth (past 256 k: a sixteenth) of the row.
+// With t the k-th largest of those 2048 (4096) maxima, k groups reach t, so k columns do, and the columns
 // that reach it lie in groups whose maximum does: those few groups are read again, from the caches, and hardly more than k
-// columns (1.15 k at k = 256 of 1024 groups) go on a list in LDS. A column's place is the number of listed ones above it.
+// columns (1.07 k at k = 256 of 2048 groups) go on a list in LDS. A column's place is the number of listed ones above it.
 // Values are compared as 64 bits, the f32 made an ordered integer over the complement of its column, so that
 // no two are equal and ties go to the lowest column. Where the list does not hold what reaches t (many equal
 // values), the row goes through it in order, a few hundred columns at a time, and it is cut to its k
@@ -14,6 +14,7 @@
 #include <algorithm>
 
 #include "nt_rows.hpp"
+#include "nt_rowsum.hpp"
 
 namespace nt {
 namespace {
@@ -21,30 +22,29 @@ namespace {
 constexpr int kTopThreads = 256;
 constexpr int kTopWaves = kTopThreads / kWave;
 constexpr int kMaxK = 1024;
-constexpr int kFewK = 256;           // up to here the small form: 1024 groups, a list of 1024
+constexpr int kFewK = 256;           
 constexpr int kTopSegs = 64;         // pieces of a row, at most
 constexpr int kTopBatch = 4;         // chunks a wave takes together
 
-// The two forms: G groups a lane, the list's length, and the chunks that go through it at a time in order.
+// The two forms, k up to kFewK and past it: G groups a lane, the list's length, and the chunks that go through it at a time in order.
 template <bool BIG>
 struct TopForm {
-    static constexpr int G = BIG ? 16 : 4, kList = BIG ? 4096 : 1024, kRound = BIG ? 4 : 1;
+    static constexpr int G = BIG ? 16 : 8, kList = BIG ? 4096 : 1024, kRound = BIG ? 4 : 1;
     static_assert((BIG ? kMaxK : kFewK) + kRound * kChunk <= kList, "a cut list and a round more");
 };
 
 // A piece's part of the row's log-sum-exp: S relative to a; n candidates follow.
 struct TopRec {
-    double S;
-    float a;
-    int32_t n;
+    double S, a;
+    int64_t n;
 };
 
 struct TopP {
     const void *x, *mask;
     int64_t V, ld;
     MaskMap mm;
-    float c;            // exponent scale of a value: log2(e) / T (none, u8) or log2(e) (f32 mask)
-    float tau;
+    double c, low;      // exponent scale of a value: log2(e) / T (none, u8) or log2(e) (f32 mask); -1100 / c
+    float c32, tau;
     int tau_one;
     double inv_t;       // value -> z: 1 / T, or 1 with an f32 mask
     int k;
@@ -75,39 +75,38 @@ template <bool BIG>
 struct TopS {
     uint64_t list[TopForm<BIG>::kList];
     float gmax[TopForm<BIG>::G * kTopThreads];  // the groups' maxima
-    uint32_t sums[2][kTopWaves];
+    uint64_t sums[2][kTopWaves];
     int count, groups;
-    double S[kTopWaves];
-    float a[kTopWaves];
+    double S[kTopWaves], a[kTopWaves];
 };
 
-// The sum over the workgroup of a count that each lane's wave already agrees on (one barrier: two buffers in turn).
-template <bool BIG>
-__device__ __forceinline__ uint32_t group_sum(TopS<BIG> &s, uint32_t wave_count, int turn) {
-    if ((threadIdx.x & (kWave - 1)) == 0) s.sums[turn & 1][threadIdx.x / kWave] = wave_count;
-    __syncthreads();
-    uint32_t n = 0;
-#pragma unroll
-    for (int w = 0; w < kTopWaves; w++) n += s.sums[turn & 1][w];
-    return n;
-}
-
 // The largest found t such that at least k of the workgroup's N keys a lane are t or more, as soon as no more than
-// `most` are (bit by bit from the top; exact when it reaches the last). 0 where there are not k keys but 0.
+// `most` are (two bits at a time from the top; exact when it reaches the last). 0 where there are not k keys but 0.
 template <class T, int N, bool BIG>
 __device__ __forceinline__ T kth_bound(TopS<BIG> &s, const T (&key)[N], int k, int most) {
     T t = 0;
     int turn = 0;
-    for (int bit = int(sizeof(T)) * 8 - 1; bit >= 0; bit--) {
-        const T up = t | (T(1) << bit);
-        uint32_t n = 0;
+    for (int bit = int(sizeof(T)) * 8 - 2; bit >= 0; bit -= 2) {
+        // (three counts of at most 2^10 x 4 waves in a word)
+        uint64_t n = 0;
 #pragma unroll
-        for (int i = 0; i < N; i++) n += uint32_t(__popcll(__ballot(key[i] >= up)));
-        n = group_sum(s, n, turn++);
-        if (int(n) >= k) {
-            t = up;
-            if (int(n) <= most) break;
+        for (int d = 1; d < 4; d++) {
+            const T up = t | (T(d) << bit);
+            uint32_t one = 0;
+#pragma unroll
+            for (int i = 0; i < N; i++) one += uint32_t(__popcll(__ballot(key[i] >= up)));
+            n |= uint64_t(one) << (16 * d);
         }
+        if ((threadIdx.x & (kWave - 1)) == 0) s.sums[turn & 1][threadIdx.x / kWave] = n;
+        __syncthreads();
+        n = 0;
+#pragma unroll
+        for (int w = 0; w < kTopWaves; w++) n += s.sums[turn & 1][w];
+        turn++;
+        int d = 3;
+        while (d > 0 && int((n >> (16 * d)) & 0xffff) < k) d--;
+        t |= T(d) << bit;
+        if (d > 0 && int((n >> (16 * d)) & 0xffff) <= most) break;
     }
     __syncthreads();  // (the sums' buffers are free again)
     return t;
@@ -143,7 +142,7 @@ __device__ __forceinline__ uint64_t cut_list(TopS<BIG> &s, int n, int k) {
 
 // The row's tokens from the list of n and its log-sum-exp. Every thread.
 template <bool BIG>
-__device__ __forceinline__ void top_finish(TopS<BIG> &s, const TopP &p, int64_t row, int n, double S, float a) {
+__device__ __forceinline__ void top_finish(TopS<BIG> &s, const TopP &p, int64_t row, int n, double S, double a) {
     int32_t *ids = p.ids + row * p.k;
     float *logp = p.logp + row * p.k;
     int st = NT_ROW_OK;
@@ -151,14 +150,15 @@ __device__ __forceinline__ void top_finish(TopS<BIG> &s, const TopP &p, int64_t 
     else if (a == -INFINITY) st = NT_ROW_NO_TOKEN;
     if (threadIdx.x == 0) p.status[row] = uint8_t(st);
     if (st != NT_ROW_OK) n = 0;
-    const double lse = double(a) * p.inv_t + log(S);
+    const double ln_s = log(S);
     for (int i = threadIdx.x; i < n; i += kTopThreads) {
         const uint64_t key = s.list[i];
         int rank = 0;
+#pragma unroll 8
         for (int j = 0; j < n; j++) rank += s.list[j] > key;
         if (rank < p.k) {
             ids[rank] = int32_t(~uint32_t(key));
-            logp[rank] = float(double(unordered(uint32_t(key >> 32))) * p.inv_t - lse);
+            logp[rank] = float((double(unordered(uint32_t(key >> 32))) - a) * p.inv_t - ln_s);
         }
     }
     for (int i = n + threadIdx.x; i < p.k; i += kTopThreads) {
@@ -167,10 +167,10 @@ __device__ __forceinline__ void top_finish(TopS<BIG> &s, const TopP &p, int64_t 
     }
 }
 
-// A lane's sum relative to a of its own, over the wave: S relative to the wave's a.
-__device__ __forceinline__ void wave_merge(double &S, float &a, float c) {
-    const float m = wave_max(a);
-    S = wave_sum_d(a == -INFINITY ? S : S * exp2((double(a) - double(m)) * double(c)));
+// Sums relative to a of the lanes' own, over the wave.
+__device__ __forceinline__ void wave_merge(const TopP &p, double &S, double &a) {
+    const double m = wave_max_d(a);
+    S = wave_sum_d(moved(S, a, m, p.c, p.low));
     a = m;
 }
 
@@ -184,13 +184,13 @@ __global__ __launch_bounds__(kTopThreads) void k_top(TopP p) {
     const void *xrow = static_cast<const char *>(p.x) + row * p.ld * Elem<DT>::kBytes;
     const void *mrow = nullptr;
     if constexpr (MK != NT_MASK_NONE) mrow = static_cast<const char *>(p.mask) + mask_row_at(p.mm, row) * MaskWords<MK>::kBytes;
+    const RowLoad<DT, MK, AL> in(xrow, mrow, p.V, p.nc);
     const bool tau_one = p.tau_one != 0;
     const int c0 = seg * p.per, c1 = min(p.nc, c0 + p.per);
     // the wave's chunks are c0 + wave + 4 j; group q of a lane has j in [q cpg, q cpg + cpg)
     const int J = (c1 - c0 + kTopWaves - 1) / kTopWaves, cpg = (J + F::G - 1) / F::G;
     if (threadIdx.x == 0) s.count = s.groups = 0;
-    double S = 0.0;
-    float a = -INFINITY;
+    LaneSums<1> sum;
     for (int q = 0; q < F::G; q++) {
         float gm = -INFINITY;
         const int j1 = min(J, (q + 1) * cpg);
@@ -199,33 +199,24 @@ __global__ __launch_bounds__(kTopThreads) void k_top(TopP p) {
 #pragma unroll
             for (int i = 0; i < kTopBatch; i++) {
                 const int ch = c0 + wave + (j + i) * kTopWaves;
-                load_raw<DT, MK, AL>(raw[i], xrow, mrow, j + i < j1 && ch < c1 ? int64_t(ch) * kChunk + lane * kEpl : p.V, p.V);
+                in.load(raw[i], ch, lane, j + i < j1 && ch < c1);
             }
-            float v[kTopBatch][kEpl];
-            float m = -INFINITY;
 #pragma unroll
             for (int i = 0; i < kTopBatch; i++) {
-                decode<DT, MK>(raw[i], v[i], p.tau, tau_one);
-                m = fmaxf(m, max8(v[i]));
+                const int ch = c0 + wave + (j + i) * kTopWaves;
+                if (j + i < j1 && ch < c1) {
+                    float v[kEpl];
+                    decode<DT, MK>(raw[i], v, p.tau, tau_one);
+                    in.clean(v, ch, lane);
+                    const float top = sum.add(v, p.c32);
+                    gm = max3_hw(gm, top, top);
+                }
             }
-            gm = fmaxf(gm, m);
-            // relative to the lane's maximum so far
-            m = fmaxf(m, a);
-            const float sh = m == -INFINITY ? 0.0f : m;
-            float sum = 0.0f;
-#pragma unroll
-            for (int i = 0; i < kTopBatch; i++) {
-                float w[kEpl];
-#pragma unroll
-                for (int e = 0; e < kEpl; e++) w[e] = exp2_hw((v[i][e] - sh) * p.c);
-                sum += tree8(w);
-            }
-            S = S * double(exp2_hw((a - sh) * p.c)) + double(sum);
-            a = m;
         }
         s.gmax[q * kTopThreads + threadIdx.x] = gm;
     }
-    wave_merge(S, a, p.c);
+    double S = sum.S[0], a = sum.at(p.c, p.c32);
+    wave_merge(p, S, a);
     if (lane == 0) {
         s.S[wave] = S;
         s.a[wave] = a;
@@ -305,9 +296,9 @@ __global__ __launch_bounds__(kTopThreads) void k_top(TopP p) {
         n = p.k;
     }
     a = s.a[0];
-    for (int w = 1; w < kTopWaves; w++) a = fmaxf(a, s.a[w]);
+    for (int w = 1; w < kTopWaves; w++) a = fmax(a, s.a[w]);
     S = 0.0;
-    for (int w = 0; w < kTopWaves; w++) S += s.a[w] == -INFINITY ? s.S[w] : s.S[w] * exp2((double(s.a[w]) - double(a)) * double(p.c));
+    for (int w = 0; w < kTopWaves; w++) S += moved(s.S[w], s.a[w], a, p.c, p.low);
     if (p.segs == 1) {
         top_finish(s, p, row, n, S, a);
         return;
@@ -329,10 +320,9 @@ __global__ __launch_bounds__(kTopThreads) void k_top_finish(TopP p) {
     // (every wave the same: a piece a lane)
     TopRec r{0.0, -INFINITY, 0};
     if (lane < p.segs) r = rec[lane];
-    double S = r.S;
-    float a = r.a;
-    wave_merge(S, a, p.c);
-    int before = r.n;
+    double S = r.S, a = r.a;
+    wave_merge(p, S, a);
+    int before = int(r.n);
 #pragma unroll
     for (int o = 1; o < kWave; o <<= 1) {
         const int m = __shfl_up(before, o, kWave);
@@ -408,12 +398,16 @@ extern "C" int nt_hip_rl_top_logprobs(const NtRlTopArgs *a) {
     p.tau = float(a->temperature);
     p.tau_one = a->temperature == 1.0;
     const bool added = a->mask_kind == NT_MASK_F32;
-    p.c = added || p.tau_one ? kLog2e : float(double(kLog2e) / a->temperature);
+    p.c = added ? kLog2e64 : kLog2e64 / a->temperature;
+    p.c32 = float(p.c);
+    p.low = -1100.0 / p.c;
     p.inv_t = added ? 1.0 : 1.0 / a->temperature;
     p.k = int(a->k);
     p.nc = int((a->vocab + kChunk - 1) / kChunk);
-    // About 1024 workgroups, each of a chunk per wave or more.
-    p.segs = int(std::max<int64_t>(1, std::min<int64_t>({1024 / a->rows, int64_t(kTopSegs), (p.nc + kTopWaves - 1) / kTopWaves})));
+    // About 1024 workgroups, each of a chunk per wave or more, and no more of them than their candidates (k and an eighth and
+    // 16 each) can be placed together.
+    p.segs = int(std::max<int64_t>(1, std::min<int64_t>({1024 / a->rows, int64_t(kTopSegs), (p.nc + kTopWaves - 1) / kTopWaves,
+                                                         (p.k > kFewK ? 4096 : 512) / (p.k + p.k / 8 + 16)})));
     p.per = (p.nc + p.segs - 1) / p.segs;
     p.segs = (p.nc + p.per - 1) / p.per;
     p.ids = a->ids;
@@ -431,7 +425,7 @@ extern "C" int nt_hip_rl_top_logprobs(const NtRlTopArgs *a) {
         p.rec = static_cast<TopRec *>(ws);
         p.cand = reinterpret_cast<uint64_t *>(static_cast<char *>(ws) + recs);
     }
-    const bool al = aligned_rows(a->logits, a->vocab, a->ld, a->dtype, a->mask_kind, a->mask, mm);
+    const bool al = aligned_rows(a->logits, a->vocab, a->ld, a->dtype, a->mask_kind, a->mask, mm) && a->vocab * 4 <= 0x7fffffffLL;
     hipStream_t s = ctx().stream;
     const dim3 grid(unsigned(a->rows * p.segs));
     auto by_al = [&](auto dt, auto mk) {

@@ -13,36 +13,41 @@
 //    (kNarrow), bound by the rows' bytes; they go by position first and sequence second, each judges its
 //    draft, and one whose sequence has had a draft refused before it leaves at once (what it would compute is not
 //    used, so whether it saw the refusal in time changes no result).
-//  * k_verify_sums (kNarrow): the first refused position, any row that was too close to call, and the f64
-//    log-sum-exps of the rows at that position, over several workgroups a sequence.
-//  * k_verify_draw: r = max(p - q, 0) of that position summed by chunks of 512 columns, over several workgroups.
-//  * k_verify_pick: one wave a sequence finds the chunk that holds u sum r, and in it the token.
+//  * k_verify_draw: the first refused position (any row that was too close to call summed in f64), and in one f64 pass
+//    over the rows there, by several workgroups a sequence, their sums and what r = max(p - q, 0) needs of
+//    them: per chunk of 512 columns the sums of both over the columns with p > q. Which those are is known before the
+//    sums are, from the sums of k_verify_rows, but for columns where p / q lies too near 1; a chunk that has such a
+//    column is left to the next kernel, and all are where those sums turn out to be further off.
+//  * k_verify_pick: the chunks' sums of r, then the chunk that holds u sum r, and in it the token.
 #include <algorithm>
 
 #include "nt_exp64.hpp"
 #include "nt_rows.hpp"
+#include "nt_rowsum.hpp"
 
 namespace nt {
 namespace {
 
 constexpr int kRowThreads = 512;              // k_verify_rows
 constexpr int kRowWaves = kRowThreads / kWave;
-constexpr int kDrawThreads = 256;             // k_verify_sums, k_verify_draw
+constexpr int kDrawThreads = 256;             // k_verify_draw, k_verify_pick
 constexpr int kDrawWaves = kDrawThreads / kWave;
 constexpr int kMaxDrafts = 127;
 constexpr int kVerifySegs = 64;               // workgroups a position or a drawn row, at most (one lane each)
 // How k_verify_rows sums: in f64, in f32 (see judge), or in f32 with the first largest value.
 enum { kWide, kNarrow, kGreedy };
-// What f32 sums may be off in a draft's log2 ratio: each of the two log-sum-exps by 6e-6 (exponentials within 2^-23 and
-// |t| 3 2^-24 ln 2 of arguments t, |t| < 24 where it matters; the lanes' references move a few times), and with an additive
-// mask, whose values are f32 tempered logits, by half an f32 step of the largest of each.
+// What f32 sums may be off in a log2 ratio of p and q: each of the two log-sum-exps by 6e-6 (weights within 2^-23 and |t| 2^-23
+// ln 2 of arguments t, |t| < 24 where it matters, in trees of 8), and with an additive mask, whose values are f32
+// tempered logits, by half an f32 step of the largest of each. f64 sums: 1e-11.
 constexpr double kClose32 = 2e-5;
+// How near 1 a column's p / q is left to k_verify_pick: far more than f64 sums are off, and more than f32 sums of these rows
+// usually are (1e-7; with a wider one, equal 16-bit differences of many columns fall into it: one row in 200 at kClose32).
+constexpr double kNear64 = 1e-9, kNear32 = 1e-6;
 
-// What a workgroup found in its piece of a position's rows: sums S relative to the reference a (value space,
-// as decoded below), of the target and of the drafter; greedy: the target's first largest value and its place.
+// What a workgroup found in its piece of a position's rows: sums S relative to the reference a (in tempered logits,
+// or with no additive mask logits), of the target and of the drafter; greedy: the target's first largest value and its place.
 struct VerifyRec {
-    double S, Sd;
-    float a, ad;
+    double S, Sd, a, ad;
     int32_t at;
     float top;
 };
@@ -52,15 +57,16 @@ struct VerifyRec {
 enum { kAccept = 0, kDraw = 1, kTooClose = 2, kBad = 3 };
 struct Verdict {
     int what;
-    int32_t at;     // greedy: the first largest
-    double lp, lq;  // log-sum-exps in log2 units (lq 0 without draft logits)
-    double logp;    // ln p of the draft
+    int32_t at;            // greedy: the first largest; otherwise whether the sums are f64
+    double a, ls, ad, lsd; // the log-sum-exps: references and log2 of the sums (drafter's 0 without its logits)
+    double logp;           // ln p of the draft
 };
 
-// What is drawn from at a sequence's last position: p's and q's log-sum-exps (log2 units) and how.
+// What is drawn from at a sequence's last position: references of p and q (their sums are k_verify_draw's) and how, and the
+// ratio of the sums that k_verify_draw went by, with how far it may be off.
 enum { kDrawNone = -1, kDrawTarget = 0, kDrawRest = 1, kDrawOthers = 2 };
 struct VerifyPick {
-    double lp, lq;
+    double a, ad, ratio, near;
     int32_t pos, mode;
 };
 
@@ -68,10 +74,11 @@ struct VerifyP {
     const void *x, *y, *mask;
     int64_t V, ld, ldy;
     MaskMap mm;
-    double c, cd;             // log2(e) / T of the target and the drafter
-    double inv_t, inv_td;     // 1 / T
-    float cap, capd;          // 2^500 in value units
-    float s32, sd32;          // log2 units of one unit of value
+    double inv_t, inv_td;     // 1 / T of the target and the drafter
+    double c, cd;             // log2 units of one unit of value: log2(e) / T, with an additive mask log2(e)
+    double low, lowd;         // -1100 / c
+    float cap, capd;          // 500 / c
+    float c32, cd32;
     int nc;                   // chunks of a row
     int seqs, K;
     int segs, per;            // workgroups a position, chunks each
@@ -81,11 +88,12 @@ struct VerifyP {
     int32_t *ids, *accepted;
     float *logp;
     uint8_t *status;
-    VerifyRec *rec;           // [seqs][K + 1][segs], or of the drawn rows [seqs][dsegs]
-    Verdict *verdict;         // one workgroup a position: [seqs][K + 1]
-    double *sums;             // [seqs][nc]
+    VerifyRec *rec;           // several workgroups a position: [seqs][K + 1][segs]
+    Verdict *verdict;         // one: [seqs][K + 1]
+    int32_t *first;           //      [seqs] the first position known to be refused
+    double2 *total;           // [seqs][dsegs] the drawn rows' sums
+    double2 *sums;            // [seqs][nc] of their chunks: of P - ratio Q, and of Q, where that is above 0 (y NaN: left)
     VerifyPick *pick;         // [seqs]
-    int32_t *first;           // one workgroup a position: [seqs] the first one known to be refused
 };
 
 // The larger, a NaN if there is one.
@@ -94,97 +102,95 @@ __device__ __forceinline__ float max8_nan(const float v[kEpl]) {
     return max_nan(max_nan(max_nan(v[0], v[1]), max_nan(v[2], v[3])), max_nan(max_nan(v[4], v[5]), max_nan(v[6], v[7])));
 }
 
-// One lane's logits and what stands for them: value v (a logit, -inf where a u8 mask excludes it; with an
-// additive mask the f32 nearest to the tempered logit, kGreedy: the f32 sum), and in f64 the exponent
-// v c - A, of an additive mask x c + m log2(e) - A.
+// One lane's 8 values: a logit, -inf where a u8 mask excludes it; with an additive mask the tempered logit in f64
+// (v: the f32 nearest to it; kGreedy: the f32 sum).
 template <int DT, int MK, int HOW>
 struct Lane8 {
+    static constexpr bool kTwo = MK == NT_MASK_F32 && HOW == kWide;
     float v[kEpl];
-    float x[MK == NT_MASK_F32 ? kEpl : 1], m[MK == NT_MASK_F32 ? kEpl : 1];
+    double z[kTwo ? kEpl : 1];
 
     __device__ __forceinline__ void decode(const uint32_t *xw, const uint32_t *mw, double inv_t) {
         if constexpr (MK == NT_MASK_F32) {
 #pragma unroll
             for (int j = 0; j < kEpl; j++) {
-                x[j] = logit<DT>(xw, j);
-                m[j] = __uint_as_float(mw[j]);
-                v[j] = HOW == kGreedy ? x[j] + m[j] : float(fma(double(x[j]), inv_t, double(m[j])));
+                const float x = logit<DT>(xw, j), m = __uint_as_float(mw[j]);
+                if constexpr (HOW == kGreedy) {
+                    v[j] = x + m;
+                } else {
+                    const double t = fma(double(x), inv_t, double(m));
+                    if constexpr (kTwo) z[j] = t;
+                    v[j] = float(t);
+                }
             }
         } else {
             decode_words<DT, MK>(xw, mw, v, 1.0f, true);
         }
     }
-    __device__ __forceinline__ double arg(int j, double c, double neg_a) const {
-        if constexpr (MK == NT_MASK_F32) return fma(double(x[j]), c, fma(double(m[j]), kLog2e64, neg_a));
-        else return fma(double(v[j]), c, neg_a);
+    template <class R>
+    __device__ __forceinline__ void clean(const R &row, int ch, int lane) {
+        row.clean(v, ch, lane);
+        if constexpr (kTwo) {
+#pragma unroll
+            for (int j = 0; j < kEpl; j++) z[j] = v[j] == -INFINITY ? -INFINITY : z[j];
+        }
+    }
+    __device__ __forceinline__ double at(int j) const {
+        if constexpr (kTwo) return z[j];
+        else return double(v[j]);
     }
 };
 
-// The log2 units of one unit of value.
-template <int MK>
-__device__ __forceinline__ double value_scale(double c) {
-    return MK == NT_MASK_F32 ? kLog2e64 : c;
+__device__ __forceinline__ double sum8(const double r[kEpl]) {
+    return ((r[0] + r[1]) + (r[2] + r[3])) + ((r[4] + r[5]) + (r[6] + r[7]));
 }
 
-// A lane's f64 sum of 2^(arg) relative to its reference: the first maximum it met, moved only where a later logit lies
-// 2^500 above it, which f64 holds and logits hardly reach.
+// A lane's f64 sum relative to its reference: the first maximum it met, moved only where a later value lies 2^500 above
+// it, which f64 holds and logits hardly reach. A NaN or +inf leaves a NaN.
 struct LaneSum {
-    double S = 0.0, neg_a = 0.0;
-    float ref = -INFINITY, lim = -INFINITY;
+    double S[1] = {}, ref = -INFINITY;
+    float lim = -INFINITY;
 
-    template <int DT, int MK, int H>
-    __device__ __forceinline__ void add(const Lane8<DT, MK, H> &l, double c, float cap) {
+    template <class L>
+    __device__ __forceinline__ void add(const L &l, double c, double low, float cap) {
         const float top = max8_nan(l.v);
-        if (!(top <= lim)) {
+        double high = double(top);
+        bool over = !(top <= lim);
+        if constexpr (L::kTwo) {  // (an f32 step may be more than 2^500: in f64)
+            high = l.z[0];
+#pragma unroll
+            for (int j = 1; j < kEpl; j++) high = fmax(high, l.z[j]);
+            over = high > ref + double(cap) || !(top < INFINITY);
+        }
+        if (over) {
             if (top < INFINITY) {
-                const double s = value_scale<MK>(c);
-                if (ref != -INFINITY) S *= exp2_64((double(ref) - double(top)) * s);
-                ref = top;
+                if (ref != -INFINITY) S[0] *= exp2_64(ref - high, c, low);
+                ref = high;
                 lim = top + cap;
-                neg_a = -double(ref) * s;
             } else {
-                S = NAN;
+                S[0] = NAN;
             }
         }
         double w[kEpl];
 #pragma unroll
-        for (int j = 0; j < kEpl; j++) w[j] = exp2_64(l.arg(j, c, neg_a));
-        S += ((w[0] + w[1]) + (w[2] + w[3])) + ((w[4] + w[5]) + (w[6] + w[7]));
+        for (int j = 0; j < kEpl; j++) w[j] = exp2_64(l.at(j) - ref, c, low);
+        S[0] += sum8(w);
     }
+    __device__ __forceinline__ double at(double, float) const { return ref; }
 };
 
-// The same of f32 exponentials, relative to the lane's maximum so far. A NaN or +inf leaves a NaN.
-struct LaneSum32 {
-    double S = 0.0;
-    float ref = -INFINITY;
-
-    __device__ __forceinline__ void add(const float v[kEpl], float scale) {
-        const float top = fmaxf(ref, max8(v)), sh = top == -INFINITY ? 0.0f : top;
-        float w[kEpl];
-#pragma unroll
-        for (int j = 0; j < kEpl; j++) w[j] = exp2_hw((v[j] - sh) * scale);
-        S = fma(S, double(exp2_hw((ref - sh) * scale)), double(tree8(w)));
-        ref = top;
-    }
-};
-
-// S relative to a, moved to the reference at (at least a).
-__device__ __forceinline__ double moved(double S, float a, float at, double scale) {
-    return a == -INFINITY || a == at ? S : S * exp2_64((double(a) - double(at)) * scale);
-}
-
-// The tempered logit of one token in log2 units, -inf where it is excluded.
+// The value of one token (see Lane8), -inf where it is excluded.
 template <int DT, int MK>
-__device__ __forceinline__ double token_arg(const void *xrow, const void *mrow, int64_t v, double c) {
+__device__ __forceinline__ double token_value(const void *xrow, const void *mrow, int64_t v, double inv_t) {
     float x;
     if constexpr (DT == NT_F32) x = static_cast<const float *>(xrow)[v];
     else x = widen16<DT>(uint32_t(static_cast<const uint16_t *>(xrow)[v]));
     if constexpr (MK == NT_MASK_U8) {
         if (static_cast<const uint8_t *>(mrow)[v] == 0) return -INFINITY;
     } else if constexpr (MK == NT_MASK_F32) {
-        return fma(double(x), c, double(static_cast<const float *>(mrow)[v]) * kLog2e64);
+        return fma(double(x), inv_t, double(static_cast<const float *>(mrow)[v]));
     }
-    return double(x) * c;
+    return double(x);
 }
 
 template <int DT, int MK>
@@ -205,7 +211,7 @@ __device__ __forceinline__ int drafts_of(const VerifyP &p, int64_t s) { return p
 // Position t of a sequence of n drafts, from its merged sums.
 template <int DT, int MK, int HOW>
 __device__ __forceinline__ Verdict judge(const VerifyP &p, int64_t s, int t, int n, const VerifyRec &r) {
-    Verdict d{kDraw, r.at, 0.0, 0.0, 0.0};
+    Verdict d{kDraw, HOW == kGreedy ? r.at : HOW == kWide, r.a, 0.0, 0.0, 0.0, 0.0};
     const VerifyRows<DT, MK> rows(p, s, t);
     if (!(r.S == r.S)) {
         d.what = kBad + NT_ROW_NAN;
@@ -215,14 +221,17 @@ __device__ __forceinline__ Verdict judge(const VerifyP &p, int64_t s, int t, int
         d.what = kBad + NT_ROW_NO_TOKEN;
         return d;
     }
-    d.lp = double(r.a) * value_scale<MK>(p.c) + log2(r.S);
+    d.ls = log2(r.S);
+    // (f32 steps of tempered logits this large are no small part of one, with a reference between them: f64)
+    const bool coarse = HOW == kNarrow && MK == NT_MASK_F32 && fmax(fabs(r.a), r.ad == -INFINITY ? 0.0 : fabs(r.ad)) > 0x1p20;
+    if (coarse) d.what = kTooClose;
     if (t >= n) return d;
     const int32_t tok = p.tokens[s * p.K + t];
     if (tok < 0 || tok >= p.V) {
         d.what = kBad + NT_ROW_BAD_TOKEN;
         return d;
     }
-    const double l = token_arg<DT, MK>(rows.x, rows.m, tok, p.c) - d.lp;
+    const double l = (token_value<DT, MK>(rows.x, rows.m, tok, p.inv_t) - r.a) * p.c - d.ls;
     d.logp = l * kLn2;
     if constexpr (HOW == kGreedy) {
         d.what = r.at == tok ? kAccept : kDraw;
@@ -238,38 +247,40 @@ __device__ __forceinline__ Verdict judge(const VerifyP &p, int64_t s, int t, int
             d.what = kBad + NT_ROW_NO_TOKEN;
             return d;
         }
-        d.lq = double(r.ad) * value_scale<MK>(p.cd) + log2(r.Sd);
-        lq = token_arg<DT, MK>(rows.y, rows.m, tok, p.cd) - d.lq;
+        d.ad = r.ad;
+        d.lsd = log2(r.Sd);
+        lq = (token_value<DT, MK>(rows.y, rows.m, tok, p.inv_td) - r.ad) * p.cd - d.lsd;
     }
     // u q < p: a draft that the drafter gives nothing is accepted where the target gives it something, and one
     // that the target gives nothing never is (inf - inf compares false)
     const double u = p.u[s * (p.K + 1) + t];
     d.what = u < exp2(l - lq) ? kAccept : kDraw;
     if constexpr (HOW == kNarrow) {
-        const double near = kClose32 + (MK == NT_MASK_F32 ? 0x1p-23 * kLog2e64 * (fabs(double(r.a)) + (rows.y ? fabs(double(r.ad)) : 0.0)) : 0.0);
-        if (fabs(log2(u) - (l - lq)) < near) d.what = kTooClose;
+        const double steps = MK == NT_MASK_F32 ? 0x1p-23 * kLog2e64 * (fabs(r.a) + (rows.y ? fabs(r.ad) : 0.0)) : 0.0;
+        if (coarse || fabs(log2(u) - (l - lq)) < kClose32 + steps) d.what = kTooClose;
     }
     return d;
 }
 
 // A wave's sums from its lanes'.
-template <int MK, class L>
+template <class L>
 __device__ __forceinline__ VerifyRec wave_rec(const VerifyP &p, const L &x, const L &y) {
     VerifyRec r{0.0, 0.0, -INFINITY, -INFINITY, 0, 0.0f};
-    r.a = wave_max(x.ref);
-    r.S = wave_sum_d(moved(x.S, x.ref, r.a, value_scale<MK>(p.c)));
-    r.ad = wave_max(y.ref);
-    r.Sd = wave_sum_d(moved(y.S, y.ref, r.ad, value_scale<MK>(p.cd)));
+    const double a = x.at(p.c, p.c32), ad = y.at(p.cd, p.cd32);
+    r.a = wave_max_d(a);
+    r.S = wave_sum_d(moved(x.S[0], a, r.a, p.c, p.low));
+    r.ad = wave_max_d(ad);
+    r.Sd = wave_sum_d(moved(y.S[0], ad, r.ad, p.cd, p.lowd));
     return r;
 }
 
 // The waves' sums in order.
-template <int MK, int WAVES>
+template <int WAVES>
 __device__ __forceinline__ VerifyRec waves_rec(const VerifyP &p, const VerifyRec *ws) {
     VerifyRec r = ws[0];
     for (int w = 1; w < WAVES; w++) {
-        r.a = fmaxf(r.a, ws[w].a);
-        r.ad = fmaxf(r.ad, ws[w].ad);
+        r.a = fmax(r.a, ws[w].a);
+        r.ad = fmax(r.ad, ws[w].ad);
         if (ws[w].top > r.top || (ws[w].top == r.top && ws[w].at < r.at)) {
             r.top = ws[w].top;
             r.at = ws[w].at;
@@ -277,44 +288,49 @@ __device__ __forceinline__ VerifyRec waves_rec(const VerifyP &p, const VerifyRec
     }
     r.S = r.Sd = 0.0;
     for (int w = 0; w < WAVES; w++) {
-        r.S += moved(ws[w].S, ws[w].a, r.a, value_scale<MK>(p.c));
-        r.Sd += moved(ws[w].Sd, ws[w].ad, r.ad, value_scale<MK>(p.cd));
+        r.S += moved(ws[w].S, ws[w].a, r.a, p.c, p.low);
+        r.Sd += moved(ws[w].Sd, ws[w].ad, r.ad, p.cd, p.lowd);
     }
     return r;
 }
 
-// Chunks c, c + step, .. below c1 of a position's rows (BOTH: and the drafter's) into the lane's sums.
-template <int DT, int MK, bool AL, int HOW, class L>
-__device__ __forceinline__ void add_rows(const VerifyP &p, const VerifyRows<DT, MK> &rows, bool both, int c, int step, int c1,
-                                         int lane, L &sx, L &sy, float *top, int32_t *at) {
+// One wave: the sums of `segs` pieces.
+__device__ __forceinline__ VerifyRec merge_recs(const VerifyP &p, const VerifyRec *rec, int segs, int lane) {
+    VerifyRec r{0.0, 0.0, -INFINITY, -INFINITY, 0x7fffffff, -INFINITY};
+    if (lane < segs) r = rec[lane];
+    VerifyRec f;
+    f.a = wave_max_d(r.a);
+    f.ad = wave_max_d(r.ad);
+    f.S = wave_sum_d(moved(r.S, r.a, f.a, p.c, p.low));
+    f.Sd = wave_sum_d(moved(r.Sd, r.ad, f.ad, p.cd, p.lowd));
+    f.top = wave_max(r.top);
+    f.at = wave_min_i(r.top == f.top ? r.at : 0x7fffffff);
+    return f;
+}
+
+// f(chunk, target's values, drafter's values) for chunks c, c + step, .. below c1 of a position's rows (both: the
+// drafter's are read), two loaded ahead.
+template <int DT, int MK, bool AL, int HOW, class F>
+__device__ __forceinline__ void over_rows(const VerifyP &p, const VerifyRows<DT, MK> &rows, bool both, int c, int step, int c1,
+                                          int lane, F &&f) {
     Raw<DT, MK> rx[2];
     Raw<DT, NT_MASK_NONE> ry[2];
+    const RowLoad<DT, MK, AL> x(rows.x, rows.m, p.V, p.nc);
+    const RowLoad<DT, NT_MASK_NONE, AL> y(rows.y, nullptr, p.V, p.nc);
     auto load = [&](int k, int ch) {
-        if (ch >= c1) return;
-        const int64_t e0 = int64_t(ch) * kChunk + lane * kEpl;
-        load_raw<DT, MK, AL>(rx[k], rows.x, rows.m, e0, p.V);
-        if (both) load_raw<DT, NT_MASK_NONE, AL>(ry[k], rows.y, nullptr, e0, p.V);
+        x.load(rx[k], ch, lane, ch < c1);
+        if (both) y.load(ry[k], ch, lane, ch < c1);
     };
     auto take = [&](int k, int ch, int next) {
         Lane8<DT, MK, HOW> lx, ly;
         lx.decode(rx[k].x, rx[k].m, p.inv_t);
-        if (both) ly.decode(ry[k].x, rx[k].m, p.inv_td);
+        lx.clean(x, ch, lane);
+        if (both) {
+            ly.decode(ry[k].x, rx[k].m, p.inv_td);
+            ly.clean(y, ch, lane);
+        }
         load(k, next);
-        if constexpr (HOW == kGreedy) {
-#pragma unroll
-            for (int j = 0; j < kEpl; j++) {
-                const bool up = lx.v[j] > *top;
-                *top = up ? lx.v[j] : *top;
-                *at = up ? ch * kChunk + lane * kEpl + j : *at;
-            }
-        }
-        if constexpr (HOW == kWide) {
-            sx.add(lx, p.c, p.cap);
-            if (both) sy.add(ly, p.cd, p.capd);
-        } else {
-            sx.add(lx.v, p.s32);
-            if (both) sy.add(ly.v, p.sd32);
-        }
+        f(ch, lx, ly);
     };
     load(0, c);
     load(1, c + step);
@@ -324,8 +340,32 @@ __device__ __forceinline__ void add_rows(const VerifyP &p, const VerifyRows<DT, 
     }
 }
 
+// The lanes' sums of a position's rows.
+template <int DT, int MK, bool AL, int HOW, class L>
+__device__ __forceinline__ void add_rows(const VerifyP &p, const VerifyRows<DT, MK> &rows, bool both, int c, int step, int c1,
+                                         int lane, L &sx, L &sy, float *top, int32_t *at) {
+    over_rows<DT, MK, AL, HOW>(p, rows, both, c, step, c1, lane, [&](int ch, const auto &lx, const auto &ly) {
+        if constexpr (HOW == kGreedy) {
+            const int64_t first = RowLoad<DT, MK, AL>(rows.x, rows.m, p.V, p.nc).first(ch, lane);
+#pragma unroll
+            for (int j = 0; j < kEpl; j++) {
+                const bool up = lx.v[j] > *top;
+                *top = up ? lx.v[j] : *top;
+                *at = up ? int32_t(first + j) : *at;
+            }
+        }
+        if constexpr (HOW == kWide) {
+            sx.add(lx, p.c, p.low, p.cap);
+            if (both) sy.add(ly, p.cd, p.lowd, p.capd);
+        } else {
+            sx.add(lx.v, p.c32);
+            if (both) sy.add(ly.v, p.cd32);
+        }
+    });
+}
+
 template <int HOW>
-using Sum = std::conditional_t<HOW == kWide, LaneSum, LaneSum32>;
+using Sum = std::conditional_t<HOW == kWide, LaneSum, LaneSums<1>>;
 
 template <int DT, int MK, bool AL, int HOW>
 __global__ __launch_bounds__(kRowThreads) void k_verify_rows(VerifyP p) {
@@ -352,7 +392,7 @@ __global__ __launch_bounds__(kRowThreads) void k_verify_rows(VerifyP p) {
     float top = -INFINITY;
     int32_t at = 0x7fffffff;
     add_rows<DT, MK, AL, HOW>(p, rows, both, seg * p.per + wave, kRowWaves, c1, lane, sx, sy, &top, &at);
-    VerifyRec r = wave_rec<MK>(p, sx, sy);
+    VerifyRec r = wave_rec(p, sx, sy);
     if constexpr (HOW == kGreedy) {
         r.top = wave_max(top);
         r.at = wave_min_i(top == r.top ? at : 0x7fffffff);
@@ -360,7 +400,7 @@ __global__ __launch_bounds__(kRowThreads) void k_verify_rows(VerifyP p) {
     if (lane == 0) ws[wave] = r;
     __syncthreads();
     if (threadIdx.x != 0) return;
-    r = waves_rec<MK, kRowWaves>(p, ws);
+    r = waves_rec<kRowWaves>(p, ws);
     if (!p.first) {
         p.rec[(s * (p.K + 1) + t) * p.segs + seg] = r;
         return;
@@ -385,63 +425,32 @@ __device__ __forceinline__ void refuse_length(const VerifyP &p, int64_t s) {
     }
 }
 
-// What a sequence ends with at position a, of verdict d.
-template <bool GREEDY>
-__device__ __forceinline__ VerifyPick pick_of(const VerifyP &p, const Verdict &d, int a, int n) {
-    VerifyPick k{d.lp, d.lq, a, kDrawNone};
-    if (d.what < kBad && !GREEDY) k.mode = a == n ? kDrawTarget : (p.y ? kDrawRest : kDrawOthers);
-    return k;
-}
-
-// The sequence's outputs but for the drawn token (k_verify_pick's), from its verdicts up to a. One workgroup.
-template <int DT, int MK, bool GREEDY>
-__device__ __forceinline__ void write_kept(const VerifyP &p, int64_t s, const Verdict *vs, const VerifyPick &k) {
-    const int K1 = p.K + 1, a = k.pos;
-    const Verdict &d = vs[a];
-    for (int t = threadIdx.x; t < K1; t += blockDim.x) {
-        if (t == a && k.mode != kDrawNone) continue;
-        float lp = 0.0f;
-        int32_t id = -1;
-        if (t < a) {
-            id = p.tokens[s * p.K + t];
-            lp = float(vs[t].logp);
-        } else if (t == a) {
-            lp = NAN;
-            if (GREEDY && d.what < kBad) {
-                const VerifyRows<DT, MK> rows(p, s, a);
-                id = d.at;
-                lp = float((token_arg<DT, MK>(rows.x, rows.m, id, p.c) - d.lp) * kLn2);
-            }
-        }
-        p.ids[s * K1 + t] = id;
-        if (p.logp) p.logp[s * K1 + t] = lp;
-    }
-    if (threadIdx.x == 0) {
-        p.accepted[s] = a;
-        p.status[s] = uint8_t(d.what < kBad ? NT_ROW_OK : d.what - kBad);
-        if constexpr (!GREEDY) p.pick[s] = k;
-    }
-}
-
-// One workgroup a position: a sequence's verdicts into vs, those too close to call (not greedy) summed in f64,
-// and its last position.
+// The sequence's verdicts into vs, and its last position. One workgroup.
 template <int DT, int MK, bool AL, bool GREEDY>
 __device__ __forceinline__ int settle(const VerifyP &p, int64_t s, int n, Verdict *vs, VerifyRec *ws) {
-    const int upto = min(n, p.first[s]), lane = threadIdx.x & (kWave - 1);
-    const int wave = __builtin_amdgcn_readfirstlane(int(threadIdx.x / kWave));
-    for (int t = threadIdx.x; t <= upto; t += kDrawThreads) vs[t] = p.verdict[s * (p.K + 1) + t];
+    const int lane = threadIdx.x & (kWave - 1), wave = __builtin_amdgcn_readfirstlane(int(threadIdx.x / kWave));
+    int upto = n;
+    if (p.first) {
+        upto = min(n, p.first[s]);
+        for (int t = threadIdx.x; t <= upto; t += kDrawThreads) vs[t] = p.verdict[s * (p.K + 1) + t];
+    } else {
+        for (int t = wave; t <= n; t += kDrawWaves) {
+            const VerifyRec r = merge_recs(p, p.rec + (s * (p.K + 1) + t) * p.segs, p.segs, lane);
+            const Verdict d = judge<DT, MK, GREEDY ? kGreedy : kWide>(p, s, t, n, r);
+            if (lane == 0) vs[t] = d;
+        }
+    }
     __syncthreads();
-    int a = 0;
-    for (;; a++) {
+    for (int a = 0;; a++) {
         if constexpr (!GREEDY) {
             if (vs[a].what == kTooClose) {
                 const VerifyRows<DT, MK> rows(p, s, a);
                 LaneSum sx, sy;
                 add_rows<DT, MK, AL, kWide>(p, rows, rows.y != nullptr, wave, kDrawWaves, p.nc, lane, sx, sy, nullptr, nullptr);
-                const VerifyRec r = wave_rec<MK>(p, sx, sy);
+                const VerifyRec r = wave_rec(p, sx, sy);
                 if (lane == 0) ws[wave] = r;
                 __syncthreads();
-                const Verdict d = judge<DT, MK, kWide>(p, s, a, n, waves_rec<MK, kDrawWaves>(p, ws));
+                const Verdict d = judge<DT, MK, kWide>(p, s, a, n, waves_rec<kDrawWaves>(p, ws));
                 if (threadIdx.x == 0) vs[a] = d;
                 __syncthreads();
             }
@@ -451,168 +460,172 @@ __device__ __forceinline__ int settle(const VerifyP &p, int64_t s, int n, Verdic
     }
 }
 
-template <int DT, int MK, bool AL>
-__global__ __launch_bounds__(kDrawThreads) void k_verify_sums(VerifyP p) {
+template <int DT, int MK, bool AL, bool GREEDY>
+__global__ __launch_bounds__(kDrawThreads, 4) void k_verify_draw(VerifyP p) {
     __shared__ Verdict vs[kMaxDrafts + 1];
     __shared__ VerifyRec ws[kDrawWaves];
     const int64_t s = blockIdx.x / unsigned(p.dsegs);
     const int seg = int(blockIdx.x % unsigned(p.dsegs));
-    const int n = drafts_of(p, s);
+    const int lane = threadIdx.x & (kWave - 1), wave = __builtin_amdgcn_readfirstlane(int(threadIdx.x / kWave));
+    const int n = drafts_of(p, s), K1 = p.K + 1;
     if (n < 0 || n > p.K) {
         if (seg == 0) refuse_length(p, s);
         return;
     }
-    const int a = settle<DT, MK, AL, false>(p, s, n, vs, ws);
-    const VerifyPick k = pick_of<false>(p, vs[a], a, n);
-    if (seg == 0) write_kept<DT, MK, false>(p, s, vs, k);
-    if (k.mode == kDrawNone) return;
-    const int lane = threadIdx.x & (kWave - 1), wave = __builtin_amdgcn_readfirstlane(int(threadIdx.x / kWave));
+    const int a = settle<DT, MK, AL, GREEDY>(p, s, n, vs, ws);
+    const Verdict d = vs[a];
     const VerifyRows<DT, MK> rows(p, s, a);
-    LaneSum sx, sy;
-    add_rows<DT, MK, AL, kWide>(p, rows, k.mode == kDrawRest, seg * p.dper + wave, kDrawWaves, min(p.nc, (seg + 1) * p.dper), lane,
-                                sx, sy, nullptr, nullptr);
+    const double ratio = exp2(d.ls - d.lsd), near = d.at ? kNear64 : kNear32;
+    int mode = kDrawNone;
+    if (d.what < kBad && !GREEDY) mode = a == n ? kDrawTarget : (p.y ? kDrawRest : kDrawOthers);
+    if (seg == 0) {
+        // what is kept, but for the drawn token (k_verify_pick's)
+        for (int t = threadIdx.x; t < K1; t += kDrawThreads) {
+            if (t == a && mode != kDrawNone) continue;
+            float lp = 0.0f;
+            int32_t id = -1;
+            if (t < a) {
+                id = p.tokens[s * p.K + t];
+                lp = float(vs[t].logp);
+            } else if (t == a) {
+                lp = NAN;
+                if (GREEDY && d.what < kBad) {
+                    id = d.at;
+                    lp = float(((token_value<DT, MK>(rows.x, rows.m, id, p.inv_t) - d.a) * p.c - d.ls) * kLn2);
+                }
+            }
+            p.ids[s * K1 + t] = id;
+            if (p.logp) p.logp[s * K1 + t] = lp;
+        }
+        if (threadIdx.x == 0) {
+            p.accepted[s] = a;
+            p.status[s] = uint8_t(d.what < kBad ? NT_ROW_OK : d.what - kBad);
+            if constexpr (!GREEDY) p.pick[s] = VerifyPick{d.a, d.ad, ratio, near, a, mode};
+        }
+    }
+    if (GREEDY || mode == kDrawNone) return;
+
+    // p and q are P = 2^((x - a) c) and Q = 2^((y - ad) cd) over their sums, r = max(P - ratio Q, 0) over P's with the ratio of
+    // the sums
+    const int32_t tok = mode == kDrawOthers ? p.tokens[s * p.K + a] : -1;
+    double2 total{0.0, 0.0};
+    over_rows<DT, MK, AL, kWide>(p, rows, mode == kDrawRest, seg * p.dper + wave, kDrawWaves, min(p.nc, (seg + 1) * p.dper), lane,
+                                 [&](int ch, const auto &lx, const auto &ly) {
+        double P[kEpl];
+#pragma unroll
+        for (int j = 0; j < kEpl; j++) P[j] = exp2_64(lx.at(j) - d.a, p.c, p.low);
+        total.x += sum8(P);
+        bool left = false;
+        double q = 0.0;
+        if (mode == kDrawRest) {
+            double Q[kEpl];
+#pragma unroll
+            for (int j = 0; j < kEpl; j++) Q[j] = exp2_64(ly.at(j) - d.ad, p.cd, p.lowd);
+            total.y += sum8(Q);
+#pragma unroll
+            for (int j = 0; j < kEpl; j++) {
+                const double over = fma(-ratio, Q[j], P[j]);
+                left = left || fabs(over) < P[j] * near;
+                P[j] = fmax(over, 0.0);
+                Q[j] = over > 0.0 ? Q[j] : 0.0;
+            }
+            q = wave_sum_d(sum8(Q));
+        } else if (mode == kDrawOthers) {
+            const int64_t e0 = RowLoad<DT, MK, AL>(rows.x, rows.m, p.V, p.nc).first(ch, lane);
+#pragma unroll
+            for (int j = 0; j < kEpl; j++) P[j] = e0 + j == tok ? 0.0 : P[j];
+        }
+        const double x = wave_sum_d(sum8(P));
+        if (__ballot(left)) q = NAN;
+        if (lane == 0) p.sums[s * p.nc + ch] = double2{x, q};
+    });
+    total.x = wave_sum_d(total.x);
+    total.y = wave_sum_d(total.y);
     __syncthreads();
-    const VerifyRec r = wave_rec<MK>(p, sx, sy);
-    if (lane == 0) ws[wave] = r;
+    if (lane == 0) {
+        ws[wave].S = total.x;
+        ws[wave].Sd = total.y;
+    }
     __syncthreads();
-    if (threadIdx.x == 0) p.rec[s * p.dsegs + seg] = waves_rec<MK, kDrawWaves>(p, ws);
+    if (threadIdx.x == 0) {
+        for (int w = 1; w < kDrawWaves; w++) {
+            total.x += ws[w].S;
+            total.y += ws[w].Sd;
+        }
+        p.total[s * p.dsegs + seg] = total;
+    }
 }
 
-// One wave: the sums of `segs` pieces.
-template <int MK>
-__device__ __forceinline__ VerifyRec merge_recs(const VerifyP &p, const VerifyRec *rec, int segs, int lane) {
-    VerifyRec r{0.0, 0.0, -INFINITY, -INFINITY, 0x7fffffff, -INFINITY};
-    if (lane < segs) r = rec[lane];
-    VerifyRec f;
-    f.a = wave_max(r.a);
-    f.ad = wave_max(r.ad);
-    f.S = wave_sum_d(moved(r.S, r.a, f.a, value_scale<MK>(p.c)));
-    f.Sd = wave_sum_d(moved(r.Sd, r.ad, f.ad, value_scale<MK>(p.cd)));
-    f.top = wave_max(r.top);
-    f.at = wave_min_i(r.top == f.top ? r.at : 0x7fffffff);
-    return f;
-}
-
-// r of one lane's 8 columns of a chunk.
-template <int DT, int MK>
-__device__ __forceinline__ void rest8(const VerifyP &p, const VerifyPick &k, int32_t tok, const Raw<DT, MK> &rx,
-                                      const Raw<DT, NT_MASK_NONE> &ry, int64_t e0, double r[kEpl]) {
+// r of one lane's 8 columns: p = 2^((x - a) c) / sums.x less q.
+template <int DT, int MK, bool AL>
+__device__ __forceinline__ void rest8(const VerifyP &p, const VerifyRows<DT, MK> &rows, const VerifyPick &k, double2 inv, int32_t tok,
+                                      int64_t e0, double r[kEpl]) {
+    Raw<DT, MK> rx;
+    Raw<DT, NT_MASK_NONE> ry;
+    load_raw<DT, MK, AL>(rx, rows.x, rows.m, e0, p.V);
+    if (k.mode == kDrawRest) load_raw<DT, NT_MASK_NONE, AL>(ry, rows.y, nullptr, e0, p.V);
     Lane8<DT, MK, kWide> l;
     l.decode(rx.x, rx.m, p.inv_t);
 #pragma unroll
-    for (int j = 0; j < kEpl; j++) r[j] = exp2_64(l.arg(j, p.c, -k.lp));
+    for (int j = 0; j < kEpl; j++) r[j] = exp2_64(l.at(j) - k.a, p.c, p.low) * inv.x;
     if (k.mode == kDrawRest) {
         l.decode(ry.x, rx.m, p.inv_td);
 #pragma unroll
-        for (int j = 0; j < kEpl; j++) r[j] = fmax(r[j] - exp2_64(l.arg(j, p.cd, -k.lq)), 0.0);
+        for (int j = 0; j < kEpl; j++) r[j] = fmax(r[j] - exp2_64(l.at(j) - k.ad, p.cd, p.lowd) * inv.y, 0.0);
     } else if (k.mode == kDrawOthers) {
 #pragma unroll
         for (int j = 0; j < kEpl; j++) r[j] = e0 + j == tok ? 0.0 : r[j];
     }
 }
 
-template <int DT, int MK, bool AL>
-__device__ __forceinline__ void load_rest(const VerifyP &p, const VerifyRows<DT, MK> &rows, int mode, int ch, int lane,
-                                          Raw<DT, MK> &rx, Raw<DT, NT_MASK_NONE> &ry) {
-    const int64_t e0 = int64_t(ch) * kChunk + lane * kEpl;
-    load_raw<DT, MK, AL>(rx, rows.x, rows.m, e0, p.V);
-    if (mode == kDrawRest) load_raw<DT, NT_MASK_NONE, AL>(ry, rows.y, nullptr, e0, p.V);
-}
-
-__device__ __forceinline__ double sum8(const double r[kEpl]) {
-    return ((((((r[0] + r[1]) + r[2]) + r[3]) + r[4]) + r[5]) + r[6]) + r[7];
-}
-
-template <int DT, int MK, bool AL, bool GREEDY>
-__global__ __launch_bounds__(kDrawThreads) void k_verify_draw(VerifyP p) {
-    __shared__ Verdict vs[kMaxDrafts + 1];
-    __shared__ VerifyRec ws[kDrawWaves];
-    const int64_t s = blockIdx.x / unsigned(p.dsegs);
-    const int seg = int(blockIdx.x % unsigned(p.dsegs));
-    const int lane = threadIdx.x & (kWave - 1), wave = __builtin_amdgcn_readfirstlane(int(threadIdx.x / kWave));
-    const int n = drafts_of(p, s);
-    VerifyPick k;
-    if (!GREEDY && p.first) {
-        // k_verify_sums has settled the sequence
-        k = p.pick[s];
-        if (k.mode == kDrawNone) return;
-        const VerifyRec r = merge_recs<MK>(p, p.rec + s * p.dsegs, p.dsegs, lane);
-        k.lp = double(r.a) * value_scale<MK>(p.c) + log2(r.S);
-        if (k.mode == kDrawRest) k.lq = double(r.ad) * value_scale<MK>(p.cd) + log2(r.Sd);
-    } else {
-        if (n < 0 || n > p.K) {
-            if (seg == 0) refuse_length(p, s);
-            return;
-        }
-        int a = 0;
-        if (p.first) {
-            a = settle<DT, MK, AL, true>(p, s, n, vs, ws);
-        } else {
-            for (int t = wave; t <= n; t += kDrawWaves) {
-                const VerifyRec r = merge_recs<MK>(p, p.rec + (s * (p.K + 1) + t) * p.segs, p.segs, lane);
-                const Verdict d = judge<DT, MK, GREEDY ? kGreedy : kWide>(p, s, t, n, r);
-                if (lane == 0) vs[t] = d;
-            }
-            __syncthreads();
-            while (a < n && vs[a].what == kAccept) a++;
-        }
-        k = pick_of<GREEDY>(p, vs[a], a, n);
-        if (seg == 0) write_kept<DT, MK, GREEDY>(p, s, vs, k);
-        if (GREEDY || k.mode == kDrawNone) return;
-    }
-    const int a = k.pos;
-    const VerifyRows<DT, MK> rows(p, s, a);
-    const int32_t tok = k.mode == kDrawOthers ? p.tokens[s * p.K + a] : -1;
-    const int c1 = min(p.nc, (seg + 1) * p.dper);
-    int c = seg * p.dper + wave;
-    Raw<DT, MK> rx, nx;
-    Raw<DT, NT_MASK_NONE> ry, ny;
-    if (c < c1) load_rest<DT, MK, AL>(p, rows, k.mode, c, lane, rx, ry);
-    for (; c < c1; c += kDrawWaves) {
-        if (c + kDrawWaves < c1) load_rest<DT, MK, AL>(p, rows, k.mode, c + kDrawWaves, lane, nx, ny);
-        double r[kEpl];
-        rest8<DT, MK>(p, k, tok, rx, ry, int64_t(c) * kChunk + lane * kEpl, r);
-        const double sum = wave_scan_dpp(sum8(r));
-        if (lane == kWave - 1) p.sums[s * p.nc + c] = sum;
-        rx = nx;
-        ry = ny;
-    }
-}
-
 // The chunk sums' total; each lane holds the same.
-__device__ __forceinline__ double sums_total(const double *sums, int nc, int lane) {
+__device__ __forceinline__ double sums_total(const double2 *sums, int nc, int lane) {
     double total = 0.0;
     for (int c0 = 0; c0 < nc; c0 += kWave)
-        total += readlane_d(wave_scan_dpp(c0 + lane < nc ? sums[c0 + lane] : 0.0), kWave - 1);
+        total += readlane_d(wave_scan_dpp(c0 + lane < nc ? sums[c0 + lane].x : 0.0), kWave - 1);
     return total;
 }
 
 template <int DT, int MK, bool AL>
-__global__ __launch_bounds__(kWave) void k_verify_pick(VerifyP p) {
+__global__ __launch_bounds__(kDrawThreads) void k_verify_pick(VerifyP p) {
     const int64_t s = blockIdx.x;
-    const int lane = threadIdx.x;
+    const int lane = threadIdx.x & (kWave - 1), wave = __builtin_amdgcn_readfirstlane(int(threadIdx.x / kWave));
     VerifyPick k = p.pick[s];
     if (k.mode == kDrawNone) return;
-    if (p.first) {
-        const VerifyRec r = merge_recs<MK>(p, p.rec + s * p.dsegs, p.dsegs, lane);
-        k.lp = double(r.a) * value_scale<MK>(p.c) + log2(r.S);
-        if (k.mode == kDrawRest) k.lq = double(r.ad) * value_scale<MK>(p.cd) + log2(r.Sd);
-    }
     const VerifyRows<DT, MK> rows(p, s, k.pos);
     const int32_t tok = k.mode == kDrawOthers ? p.tokens[s * p.K + k.pos] : -1;
-    double *sums = p.sums + s * p.nc;
-    Raw<DT, MK> rx;
-    Raw<DT, NT_MASK_NONE> ry;
+    double2 *sums = p.sums + s * p.nc, whole{0.0, 0.0};
+    if (lane < p.dsegs) whole = p.total[s * p.dsegs + lane];
+    whole.x = wave_sum_d(whole.x);
+    whole.y = wave_sum_d(whole.y);
+    const double2 inv{1.0 / whole.x, k.mode == kDrawRest ? 1.0 / whole.y : 0.0};
+    // (P - ratio Q of the right ratio, whole.x / whole.y)
+    const double more = k.mode == kDrawRest ? k.ratio - whole.x / whole.y : 0.0;
+    const bool all = fabs(more) > 0.5 * k.near * k.ratio;
     double r[kEpl];
+    // r of each chunk, 64 of them a wave at a time; those that were left are computed here
+    for (int c0 = wave * kWave; c0 < p.nc; c0 += kDrawWaves * kWave) {
+        double2 v{0.0, 0.0};
+        if (c0 + lane < p.nc) v = sums[c0 + lane];
+        double sum = fmax((v.x + more * v.y) * inv.x, 0.0);
+        for (uint64_t left = __ballot(c0 + lane < p.nc && (all || !(v.y == v.y))); left; left &= left - 1) {
+            const int i = __builtin_ctzll(left);
+            rest8<DT, MK, AL>(p, rows, k, inv, tok, int64_t(c0 + i) * kChunk + lane * kEpl, r);
+            const double one = wave_sum_d(sum8(r));
+            if (lane == i) sum = one;
+        }
+        if (c0 + lane < p.nc) sums[c0 + lane].x = sum;
+    }
+    __syncthreads();
+    if (wave != 0) return;
     double total = sums_total(sums, p.nc, lane);
     if (!(total > 0.0)) {
         // refused, and yet p is nowhere above q (a uniform of 1 against a draft of equal p and q): p itself
         k.mode = kDrawTarget;
         for (int c = 0; c < p.nc; c++) {
-            load_rest<DT, MK, AL>(p, rows, k.mode, c, lane, rx, ry);
-            rest8<DT, MK>(p, k, tok, rx, ry, int64_t(c) * kChunk + lane * kEpl, r);
-            const double sum = wave_scan_dpp(sum8(r));
-            if (lane == kWave - 1) sums[c] = sum;
+            rest8<DT, MK, AL>(p, rows, k, inv, -1, int64_t(c) * kChunk + lane * kEpl, r);
+            const double sum = wave_sum_d(sum8(r));
+            if (lane == 0) sums[c].x = sum;
         }
         __threadfence_block();
         total = sums_total(sums, p.nc, lane);
@@ -622,7 +635,7 @@ __global__ __launch_bounds__(kWave) void k_verify_pick(VerifyP p) {
     double run = 0.0, before = 0.0;
     int chunk = -1, last = 0;
     for (int c0 = 0; c0 < p.nc && chunk < 0; c0 += kWave) {
-        const double v = c0 + lane < p.nc ? sums[c0 + lane] : 0.0;
+        const double v = c0 + lane < p.nc ? sums[c0 + lane].x : 0.0;
         const double cum = run + wave_scan_dpp(v);
         const int f = first_lane(__ballot(c0 + lane < p.nc && cum > want));
         const int l = last_lane(__ballot(v > 0.0));
@@ -636,8 +649,7 @@ __global__ __launch_bounds__(kWave) void k_verify_pick(VerifyP p) {
     const bool crossed = chunk >= 0;
     if (!crossed) chunk = last;
     const int64_t e0 = int64_t(chunk) * kChunk + lane * kEpl;
-    load_rest<DT, MK, AL>(p, rows, k.mode, chunk, lane, rx, ry);
-    rest8<DT, MK>(p, k, tok, rx, ry, e0, r);
+    rest8<DT, MK, AL>(p, rows, k, inv, tok, e0, r);
     const double mine = sum8(r);
     double cum = before + (wave_scan_dpp(mine) - mine);
     int here = -1, some = -1;
@@ -653,7 +665,8 @@ __global__ __launch_bounds__(kWave) void k_verify_pick(VerifyP p) {
         const int64_t v = e0 + (f >= 0 ? here : some);
         p.ids[s * (p.K + 1) + k.pos] = int32_t(v);
         if (p.logp)
-            p.logp[s * (p.K + 1) + k.pos] = float((token_arg<DT, MK>(rows.x, rows.m, v, p.c) - k.lp) * kLn2);
+            p.logp[s * (p.K + 1) + k.pos] =
+                float(((token_value<DT, MK>(rows.x, rows.m, v, p.inv_t) - k.a) * p.c - log2(whole.x)) * kLn2);
     }
 }
 
@@ -674,12 +687,11 @@ void verify_launch(const VerifyP &p, bool greedy, hipStream_t s) {
     }
     if (p.first) {
         hipLaunchKernelGGL((k_verify_rows<DT, MK, AL, kNarrow>), rows, dim3(kRowThreads), 0, s, p);
-        hipLaunchKernelGGL((k_verify_sums<DT, MK, AL>), draw, dim3(kDrawThreads), 0, s, p);
     } else {
         hipLaunchKernelGGL((k_verify_rows<DT, MK, AL, kWide>), rows, dim3(kRowThreads), 0, s, p);
     }
     hipLaunchKernelGGL((k_verify_draw<DT, MK, AL, false>), draw, dim3(kDrawThreads), 0, s, p);
-    hipLaunchKernelGGL((k_verify_pick<DT, MK, AL>), dim3(unsigned(p.seqs)), dim3(kWave), 0, s, p);
+    hipLaunchKernelGGL((k_verify_pick<DT, MK, AL>), dim3(unsigned(p.seqs)), dim3(kDrawThreads), 0, s, p);
 }
 
 }  // namespace
@@ -721,15 +733,17 @@ extern "C" int nt_hip_rl_verify_drafted(const NtRlVerifyArgs *a) {
     p.ldy = a->draft_ld;
     p.mm = mm;
     const double T = greedy ? 1.0 : a->temperature, Td = draft ? a->draft_temperature : 1.0;
-    p.c = kLog2e64 / T;
-    p.cd = kLog2e64 / Td;
     p.inv_t = 1.0 / T;
     p.inv_td = 1.0 / Td;
     const bool added = a->mask_kind == NT_MASK_F32;
-    p.cap = float(500.0 / (added ? kLog2e64 : p.c));
-    p.capd = float(500.0 / (added ? kLog2e64 : p.cd));
-    p.s32 = added ? kLog2e : float(p.c);
-    p.sd32 = added ? kLog2e : float(p.cd);
+    p.c = added ? kLog2e64 : kLog2e64 / T;
+    p.cd = added ? kLog2e64 : kLog2e64 / Td;
+    p.low = -1100.0 / p.c;
+    p.lowd = -1100.0 / p.cd;
+    p.cap = float(500.0 / p.c);
+    p.capd = float(500.0 / p.cd);
+    p.c32 = float(p.c);
+    p.cd32 = float(p.cd);
     p.nc = int((a->vocab + kChunk - 1) / kChunk);
     p.seqs = int(seqs);
     p.K = int(K);
@@ -754,11 +768,13 @@ extern "C" int nt_hip_rl_verify_drafted(const NtRlVerifyArgs *a) {
     p.status = a->status;
 
     const auto round = [](size_t n) { return (n + 255) / 256 * 256; };
-    const size_t recs = round(sizeof(VerifyRec) * size_t(one ? seqs * p.dsegs : rows * p.segs));
+    const size_t recs = one ? 0 : round(sizeof(VerifyRec) * size_t(rows) * size_t(p.segs));
     const size_t verdicts = one ? round(sizeof(Verdict) * size_t(rows)) : 0;
-    const size_t sums = greedy ? 0 : round(sizeof(double) * size_t(seqs) * size_t(p.nc));
-    const size_t picks = round(sizeof(VerifyPick) * size_t(seqs)), firsts = one ? round(sizeof(int32_t) * size_t(seqs)) : 0;
-    const size_t need = recs + verdicts + sums + picks + firsts;
+    const size_t firsts = one ? round(sizeof(int32_t) * size_t(seqs)) : 0;
+    const size_t totals = greedy ? 0 : round(sizeof(double2) * size_t(seqs) * size_t(p.dsegs));
+    const size_t sums = greedy ? 0 : round(sizeof(double2) * size_t(seqs) * size_t(p.nc));
+    const size_t picks = round(sizeof(VerifyPick) * size_t(seqs));
+    const size_t need = recs + verdicts + firsts + totals + sums + picks;
     bool cap = false;
     if (int rc = stream_capturing(&cap)) return rc;
     if (cap && need >= size_t(1) << 20)
@@ -768,12 +784,13 @@ extern "C" int nt_hip_rl_verify_drafted(const NtRlVerifyArgs *a) {
     if (int rc = scratch_alloc(need, &ws)) return rc;
     char *at = static_cast<char *>(ws);
     p.rec = reinterpret_cast<VerifyRec *>(at);
-    p.verdict = reinterpret_cast<Verdict *>(at + recs);
-    p.sums = reinterpret_cast<double *>(at + recs + verdicts);
-    p.pick = reinterpret_cast<VerifyPick *>(at + recs + verdicts + sums);
-    if (one) p.first = reinterpret_cast<int32_t *>(at + recs + verdicts + sums + picks);
+    p.verdict = reinterpret_cast<Verdict *>(at += recs);
+    if (one) p.first = reinterpret_cast<int32_t *>(at + verdicts);
+    p.total = reinterpret_cast<double2 *>(at += verdicts + firsts);
+    p.sums = reinterpret_cast<double2 *>(at += totals);
+    p.pick = reinterpret_cast<VerifyPick *>(at + sums);
 
-    bool al = aligned_rows(a->logits, a->vocab, a->ld, a->dtype, a->mask_kind, a->mask, mm);
+    bool al = aligned_rows(a->logits, a->vocab, a->ld, a->dtype, a->mask_kind, a->mask, mm) && a->vocab * 4 <= 0x7fffffffLL;
     if (draft) al = al && a->draft_ld % kEpl == 0 && reinterpret_cast<uintptr_t>(a->draft_logits) % 16 == 0;
     hipStream_t s = ctx().stream;
     auto by_al = [&](auto dt, auto mk) {

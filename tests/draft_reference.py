@@ -57,7 +57,7 @@ def tempered(x, T, add, off):
 def log_softmax(z):
     with np.errstate(invalid="ignore", divide="ignore"):
         m = z.max(-1, keepdims=True)
-        return z - (m + np.log(np.exp(z - m).sum(-1, keepdims=True)))
+        return (z - m) - np.log(np.exp(z - m).sum(-1, keepdims=True))  # (in this order: m may be far larger)
 
 
 def verify(z, zq, tokens, u, lengths, greedy):

@@ -151,6 +151,25 @@ def test_far_logits_and_masks_of_the_lowest_value():
     compare(run(x, y, nr.Tensor.from_numpy(add), tokens, u, None, "f32", 1.0), want)
 
 
+@pytest.mark.parametrize("S", [4, 150])  # several workgroups a position, and one
+@pytest.mark.parametrize("value", [-1e9, -1e13, float(np.finfo(np.float32).min)])
+def test_masks_that_lower_every_token(S, value):
+    """A row whose mask leaves nothing but lowers all by one value: what f64 keeps of the logits beside it decides."""
+    rng = np.random.default_rng(12)
+    K, V = 2, 1100
+    x = rng.normal(0, 2, (S, K + 1, V)).astype(np.float32)
+    y = (x[:, :K] + rng.normal(0, 0.5, (S, K, V))).astype(np.float32)
+    add = np.full((1, 1, V), value, np.float32)
+    z, zq = x.astype(np.float64) + add, y.astype(np.float64) + add
+    tokens = np.argmax(zq + rng.gumbel(size=zq.shape), 2).astype(np.int32)
+    u = rng.random((S, K + 1))
+    want = ref.verify(z, zq, tokens, u, np.full(S, K), False)
+    ids, acc, lp = (t.to_numpy() for t in run(x, y, nr.Tensor.from_numpy(add), tokens, u, None, "f32", 1.0))
+    assert np.array_equal(ids, want[0]) and np.array_equal(acc, want[1])
+    at = np.arange(S), acc
+    assert (np.abs(lp - want[2])[at] <= 2.0 ** -24 * np.abs(want[2])[at] + 1e-12).all()
+
+
 def raw(x, y, tokens, u, dtype="f32", T=1.0, lengths=None, mt=None, S=None, K=None, V=None):
     """A direct call with every output larger by a row, filled beforehand; (rc, ids, accepted, logp, status)."""
     S1, K1, V1 = x.shape
