@@ -9,13 +9,15 @@ namespace nt {
 namespace {
 
 // A row's loads, none under a condition: with one, the compiler lets every load wait for the one before it, whose registers
-// the other branch would write (64 of 4096 x 50304: 108 us; without 72). AL (aligned_rows, row bytes below 2^31): buffer
-// loads, zeros past the row's end. Otherwise loads at the elements' own alignment, the row's last ones from 8 columns
-// before its end, so that a lane there holds columns of its neighbour too; rows of under 8 columns by elements.
-// Lane l of chunk ch has columns first() .. first() + 7, of which those below own() or not below V are not its own:
-// only in the row's last chunk, where clean() gives them -inf.
+// the other branch would write. AL (aligned_rows, row bytes below 2^31): non-temporal buffer loads, zeros past the row's
+// end; f32 rows in two groups of four columns a lane, 256 apart, so that each instruction reads one contiguous kilobyte.
+// Otherwise loads at the elements' own alignment, the row's last ones from 8 columns before its end, so that a lane there
+// holds columns of its neighbour too; rows of under 8 columns by elements. Column j of lane l in chunk ch is col(); those
+// that are not the lane's own (its neighbour's, or past the row) are in the row's last chunk only, where clean() gives them -inf.
 template <int DT, int MK, bool AL>
 struct RowLoad {
+    static constexpr bool kSplit = AL && DT == NT_F32;
+    static constexpr int kHalf = kChunk / 2;
     const void *x, *m;
     __amdgpu_buffer_rsrc_t xr, mr;
     int64_t V;
@@ -35,24 +37,43 @@ struct RowLoad {
         if constexpr (AL) return e0;
         else return V < kEpl ? e0 : (e0 + kEpl <= V ? e0 : V - kEpl);
     }
+    __device__ __forceinline__ int64_t col(int ch, int lane, int j) const {
+        if constexpr (kSplit) return int64_t(ch) * kChunk + lane * 4 + (j < 4 ? j : kHalf - 4 + j);
+        else return first(ch, lane) + j;
+    }
     // The raw words of chunk ch (in: the row has it; otherwise anything).
     __device__ __forceinline__ void load(Raw<DT, MK> &r, int ch, int lane, bool in = true) const {
-        if constexpr (AL) {
+        if constexpr (kSplit) {
+            const int e0 = in ? ch * kChunk + lane * 4 : int(V);
+#pragma unroll
+            for (int q = 0; q < 2; q++) {
+                const auto a = __builtin_amdgcn_raw_buffer_load_b128(xr, (e0 + q * kHalf) * 4, 0, kCachePolicyNT);
+#pragma unroll
+                for (int i = 0; i < 4; i++) r.x[4 * q + i] = a[i];
+                if constexpr (MK == NT_MASK_U8) {
+                    r.m[q] = __builtin_amdgcn_raw_buffer_load_b32(mr, e0 + q * kHalf, 0, kCachePolicyNT);
+                } else if constexpr (MK == NT_MASK_F32) {
+                    const auto k = __builtin_amdgcn_raw_buffer_load_b128(mr, (e0 + q * kHalf) * 4, 0, kCachePolicyNT);
+#pragma unroll
+                    for (int i = 0; i < 4; i++) r.m[4 * q + i] = k[i];
+                }
+            }
+        } else if constexpr (AL) {
             const int e0 = in ? int(own(ch, lane)) : int(V);
 #pragma unroll
             for (int q = 0; q < Elem<DT>::kWords / 4; q++) {
-                const auto a = __builtin_amdgcn_raw_buffer_load_b128(xr, e0 * Elem<DT>::kBytes + 16 * q, 0, 0);
+                const auto a = __builtin_amdgcn_raw_buffer_load_b128(xr, e0 * Elem<DT>::kBytes + 16 * q, 0, kCachePolicyNT);
 #pragma unroll
                 for (int i = 0; i < 4; i++) r.x[4 * q + i] = a[i];
             }
             if constexpr (MK == NT_MASK_U8) {
-                const auto k = __builtin_amdgcn_raw_buffer_load_b64(mr, e0, 0, 0);
+                const auto k = __builtin_amdgcn_raw_buffer_load_b64(mr, e0, 0, kCachePolicyNT);
                 r.m[0] = k[0];
                 r.m[1] = k[1];
             } else if constexpr (MK == NT_MASK_F32) {
 #pragma unroll
                 for (int q = 0; q < 2; q++) {
-                    const auto a = __builtin_amdgcn_raw_buffer_load_b128(mr, e0 * 4 + 16 * q, 0, 0);
+                    const auto a = __builtin_amdgcn_raw_buffer_load_b128(mr, e0 * 4 + 16 * q, 0, kCachePolicyNT);
 #pragma unroll
                     for (int i = 0; i < 4; i++) r.m[4 * q + i] = a[i];
                 }
@@ -89,10 +110,11 @@ struct RowLoad {
             }
         }
     }
-    // Whether column first() + j of the lane is its own.
+    // Whether column col(j) of the lane is its own.
     __device__ __forceinline__ bool mine(int ch, int lane, int j) const {
-        const int64_t e = first(ch, lane) + j;
-        return e >= own(ch, lane) && e < V;
+        const int64_t e = col(ch, lane, j);
+        if constexpr (AL) return e < V;
+        else return e >= own(ch, lane) && e < V;
     }
     __device__ __forceinline__ void clean(float v[kEpl], int ch, int lane) const {
         if (ch != last) return;
@@ -100,6 +122,18 @@ struct RowLoad {
         for (int j = 0; j < kEpl; j++) v[j] = mine(ch, lane, j) ? v[j] : -INFINITY;
     }
 };
+
+// take(slot, chunk, next) for chunks c, c + step, .. below c1 with D of them loaded ahead by load(slot, chunk): take uses
+// the slot's words and then loads `next` into it.
+template <int D, class L, class F>
+__device__ __forceinline__ void stream(int c, int step, int c1, L &&load, F &&take) {
+    static_for<0, D>([&](auto k) { load(k, c + k.value * step); });
+    for (; c < c1; c += D * step)
+        static_for<0, D>([&](auto k) {
+            const int ch = c + k.value * step;
+            if (ch < c1) take(k, ch, ch + D * step);
+        });
+}
 
 // N sums (of all weights, of some) relative to the lane's reference: the first maximum it met, moved only where a later
 // value lies 60 log2 units above it, so that most chunks cost a weight one fma, one exponential and one addition. The

@@ -23,7 +23,7 @@ namespace {
 
 constexpr int kDistillThreads = 256;
 constexpr int kDistillWaves = kDistillThreads / kWave;
-constexpr int kDistillBatch = 4;              // chunks a wave takes together
+constexpr int kDistillAhead = 4;              // chunks a wave loads ahead
 constexpr int kMaxListed = 1024;
 constexpr int kMapChunks = 512;               // chunks a workgroup's bitmap covers: 2^18 columns, 32 KiB
 
@@ -183,34 +183,32 @@ __global__ __launch_bounds__(kDistillThreads) void k_distill(DistillP p) {
 
     const RowLoad<DT, MK, AL> in(xrow, mrow, p.V, p.nc);
     LaneSums<2> sum;
-    for (int t0 = c0 + wave; t0 < c1; t0 += kDistillBatch * kDistillWaves) {
-        Raw<DT, MK> raw[kDistillBatch];
-#pragma unroll
-        for (int i = 0; i < kDistillBatch; i++) {
-            const int ch = t0 + i * kDistillWaves;
-            in.load(raw[i], ch, lane, ch < c1);
+    Raw<DT, MK> raw[kDistillAhead];
+    auto load = [&](auto i, int ch) { in.load(raw[i.value], ch, lane, ch < c1); };
+    stream<kDistillAhead>(c0 + wave, kDistillWaves, c1, load, [&](auto i, int ch, int next) {
+        float v[kEpl], w[kEpl];
+        decode<DT, MK>(raw[i.value], v, p.tau, tau_one);
+        in.clean(v, ch, lane);
+        load(i, next);
+        sum.weigh(v, p.c32, w);
+        float t = tree8(w);
+        sum.S[0] += double(t);
+        // bit j for column j
+        uint32_t on;
+        if constexpr (decltype(in)::kSplit) {
+            const int at = (ch - c0) * kWave + lane / 2, shift = 4 * (lane & 1);
+            on = ((bytes[at] >> shift) & 15u) | (((bytes[at + kWave / 2] >> shift) & 15u) << 4);
+        } else {
+            // (past the row's end a lane's own columns come after its neighbour's)
+            on = uint32_t(bytes[(ch - c0) * kWave + lane]) << (AL ? 0 : min(int64_t(8), in.own(ch, lane) - in.first(ch, lane)));
         }
+        if (__ballot(on != 0) != 0) {
 #pragma unroll
-        for (int i = 0; i < kDistillBatch; i++) {
-            const int ch = t0 + i * kDistillWaves;
-            if (ch < c1) {
-                float v[kEpl], w[kEpl];
-                decode<DT, MK>(raw[i], v, p.tau, tau_one);
-                in.clean(v, ch, lane);
-                sum.weigh(v, p.c32, w);
-                float t = tree8(w);
-                sum.S[0] += double(t);
-                // (bit j for column first() + j: past the row's end a lane's own columns come after its neighbour's)
-                const uint32_t on = uint32_t(bytes[(ch - c0) * kWave + lane]) << min(int64_t(8), in.own(ch, lane) - in.first(ch, lane));
-                if (__ballot(on != 0) != 0) {
-#pragma unroll
-                    for (int j = 0; j < kEpl; j++) w[j] = (on >> j) & 1u ? 0.0f : w[j];
-                    t = tree8(w);
-                }
-                sum.S[1] += double(t);
-            }
+            for (int j = 0; j < kEpl; j++) w[j] = (on >> j) & 1u ? 0.0f : w[j];
+            t = tree8(w);
         }
-    }
+        sum.S[1] += double(t);
+    });
     const double at = sum.at(p.c, p.c32), top = wave_max_d(at);
     const double S = wave_sum_d(moved(sum.S[0], at, top, p.c, p.low)), R = wave_sum_d(moved(sum.S[1], at, top, p.c, p.low));
     if (lane == 0) ws[wave] = DistillRec{S, R, top, 0};
@@ -289,6 +287,20 @@ __device__ __forceinline__ void store8(void *grow, int64_t e0, int64_t V, const 
     for (int j = 0; j < kEpl && e0 + j < V; j++) store1<GDT>(grow, e0 + j, o[j]);
 }
 
+// 4 gradients at column e, aligned, all inside the row or none.
+template <int GDT>
+__device__ __forceinline__ void store4(void *grow, int64_t e, int64_t V, const float *o) {
+    if (e >= V) return;
+    if constexpr (GDT == NT_F32) {
+        __builtin_nontemporal_store(v4u{__float_as_uint(o[0]), __float_as_uint(o[1]), __float_as_uint(o[2]), __float_as_uint(o[3])},
+                                    reinterpret_cast<v4u *>(static_cast<float *>(grow) + e));
+    } else {
+        typedef uint32_t v2u __attribute__((ext_vector_type(2)));
+        __builtin_nontemporal_store(v2u{pack2<GDT>(o[0], o[1]), pack2<GDT>(o[2], o[3])},
+                                    reinterpret_cast<v2u *>(static_cast<uint16_t *>(grow) + e));
+    }
+}
+
 template <int DT, int MK, int GDT, bool AL>
 __global__ __launch_bounds__(kDistillThreads) void k_distill_grad(DistillP p) {
     const int64_t row = blockIdx.x / unsigned(p.segs);
@@ -310,30 +322,24 @@ __global__ __launch_bounds__(kDistillThreads) void k_distill_grad(DistillP p) {
     const float a = float(base), factor = float(scale * st[2] / S);
     const bool tau_one = p.tau_one != 0;
     const RowLoad<DT, MK, AL> in(xrow, mrow, p.V, p.nc);
-    for (int t0 = c0 + wave; t0 < c1; t0 += kDistillBatch * kDistillWaves) {
-        Raw<DT, MK> raw[kDistillBatch];
+    Raw<DT, MK> raw[kDistillAhead];
+    auto load = [&](auto i, int ch) { in.load(raw[i.value], ch, lane, ch < c1); };
+    stream<kDistillAhead>(c0 + wave, kDistillWaves, c1, load, [&](auto i, int ch, int next) {
+        float v[kEpl], o[kEpl];
+        decode<DT, MK>(raw[i.value], v, p.tau, tau_one);
+        load(i, next);
 #pragma unroll
-        for (int i = 0; i < kDistillBatch; i++) {
-            const int ch = t0 + i * kDistillWaves;
-            in.load(raw[i], ch, lane, ch < c1);
+        for (int j = 0; j < kEpl; j++) o[j] = fmaf(exp2_hw((v[j] - a) * p.c32), factor, 0.0f);
+        if constexpr (decltype(in)::kSplit) {
+            store4<GDT>(grow, in.col(ch, lane, 0), p.V, o);
+            store4<GDT>(grow, in.col(ch, lane, 4), p.V, o + 4);
+        } else if (AL || in.first(ch, lane) == in.own(ch, lane)) {
+            store8<GDT, AL>(grow, in.own(ch, lane), p.V, o);
+        } else {
+            for (int j = 0; j < kEpl; j++)
+                if (in.mine(ch, lane, j)) store1<GDT>(grow, in.first(ch, lane) + j, o[j]);
         }
-#pragma unroll
-        for (int i = 0; i < kDistillBatch; i++) {
-            const int ch = t0 + i * kDistillWaves;
-            if (ch < c1) {
-                float v[kEpl], o[kEpl];
-                decode<DT, MK>(raw[i], v, p.tau, tau_one);
-#pragma unroll
-                for (int j = 0; j < kEpl; j++) o[j] = fmaf(exp2_hw((v[j] - a) * p.c32), factor, 0.0f);
-                if (AL || in.first(ch, lane) == in.own(ch, lane)) {
-                    store8<GDT, AL>(grow, in.own(ch, lane), p.V, o);
-                } else {
-                    for (int j = 0; j < kEpl; j++)
-                        if (in.mine(ch, lane, j)) store1<GDT>(grow, in.first(ch, lane) + j, o[j]);
-                }
-            }
-        }
-    }
+    });
     // the listed columns of this piece, over what was just written there
     wait_vmcnt<0>();
     __syncthreads();

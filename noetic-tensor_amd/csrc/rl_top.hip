@@ -2,9 +2,9 @@
 //
 // A workgroup streams its row (or, where rows are few, a piece of one) once, and takes from it the log-sum-exp and the
 // largest value of each group of columns: a lane's columns in an eighth (past 256 k: a sixteenth) of the row.
-// With t the k-th largest of those 2048 (4096) maxima, k groups reach t, so k columns do, and the columns
+// With t the k-th largest of those maxima (joined to 256, 512 or 1024 for few k), k groups reach t, so k columns do, and the columns
 // that reach it lie in groups whose maximum does: those few groups are read again, from the caches, and hardly more than k
-// columns (1.07 k at k = 256 of 2048 groups) go on a list in LDS. A column's place is the number of listed ones above it.
+// columns (1.4 k at the most) go on a list in LDS. A column's place is the number of listed ones above it.
 // Values are compared as 64 bits, the f32 made an ordered integer over the complement of its column, so that
 // no two are equal and ties go to the lowest column. Where the list does not hold what reaches t (many equal
 // values), the row goes through it in order, a few hundred columns at a time, and it is cut to its k
@@ -24,7 +24,7 @@ constexpr int kTopWaves = kTopThreads / kWave;
 constexpr int kMaxK = 1024;
 constexpr int kFewK = 256;           
 constexpr int kTopSegs = 64;         // pieces of a row, at most
-constexpr int kTopBatch = 4;         // chunks a wave takes together
+constexpr int kTopAhead = 4;         // chunks a wave loads ahead
 
 // The two forms, k up to kFewK and past it: G groups a lane, the list's length, and the chunks that go through it at a time in order.
 template <bool BIG>
@@ -191,29 +191,26 @@ __global__ __launch_bounds__(kTopThreads) void k_top(TopP p) {
     const int J = (c1 - c0 + kTopWaves - 1) / kTopWaves, cpg = (J + F::G - 1) / F::G;
     if (threadIdx.x == 0) s.count = s.groups = 0;
     LaneSums<1> sum;
-    for (int q = 0; q < F::G; q++) {
-        float gm = -INFINITY;
-        const int j1 = min(J, (q + 1) * cpg);
-        for (int j = q * cpg; j < j1; j += kTopBatch) {
-            Raw<DT, MK> raw[kTopBatch];
-#pragma unroll
-            for (int i = 0; i < kTopBatch; i++) {
-                const int ch = c0 + wave + (j + i) * kTopWaves;
-                in.load(raw[i], ch, lane, j + i < j1 && ch < c1);
-            }
-#pragma unroll
-            for (int i = 0; i < kTopBatch; i++) {
-                const int ch = c0 + wave + (j + i) * kTopWaves;
-                if (j + i < j1 && ch < c1) {
-                    float v[kEpl];
-                    decode<DT, MK>(raw[i], v, p.tau, tau_one);
-                    in.clean(v, ch, lane);
-                    const float top = sum.add(v, p.c32);
-                    gm = max3_hw(gm, top, top);
-                }
-            }
+    float gm = -INFINITY;
+    int q = 0, left = cpg;
+    Raw<DT, MK> raw[kTopAhead];
+    auto load = [&](auto i, int ch) { in.load(raw[i.value], ch, lane, ch < c1); };
+    stream<kTopAhead>(c0 + wave, kTopWaves, c1, load, [&](auto i, int ch, int next) {
+        float v[kEpl];
+        decode<DT, MK>(raw[i.value], v, p.tau, tau_one);
+        in.clean(v, ch, lane);
+        load(i, next);
+        const float top = sum.add(v, p.c32);
+        gm = max3_hw(gm, top, top);
+        if (--left == 0) {
+            s.gmax[q++ * kTopThreads + threadIdx.x] = gm;
+            gm = -INFINITY;
+            left = cpg;
         }
+    });
+    for (; q < F::G; q++) {
         s.gmax[q * kTopThreads + threadIdx.x] = gm;
+        gm = -INFINITY;
     }
     double S = sum.S[0], a = sum.at(p.c, p.c32);
     wave_merge(p, S, a);
@@ -221,11 +218,25 @@ __global__ __launch_bounds__(kTopThreads) void k_top(TopP p) {
         s.S[wave] = S;
         s.a[wave] = a;
     }
-    // the threshold: what is on the list is above `least`
+    // the threshold: what is on the list is above `least`. Of the largest of all a lane's groups where there are four lanes for
+    // each of the k, of pairs or fours of them else: k of those reach it too, and they are fewer to count.
     uint32_t g[F::G];
 #pragma unroll
-    for (int q = 0; q < F::G; q++) g[q] = ordered(s.gmax[q * kTopThreads + threadIdx.x]);  // (this thread's own)
-    uint32_t bound = kth_bound<uint32_t, F::G, BIG>(s, g, p.k, p.k + p.k / 8 + 16);
+    for (int i = 0; i < F::G; i++) g[i] = ordered(s.gmax[i * kTopThreads + threadIdx.x]);  // (this thread's own)
+    const auto of_groups = [&](auto n) {
+        constexpr int N = decltype(n)::value;
+        uint32_t h[N];
+#pragma unroll
+        for (int i = 0; i < N; i++) h[i] = g[i];
+#pragma unroll
+        for (int i = N; i < F::G; i++) h[i % N] = max(h[i % N], g[i]);
+        return kth_bound<uint32_t, N, BIG>(s, h, p.k, p.k + p.k / 8 + 16);
+    };
+    uint32_t bound;
+    if constexpr (BIG) bound = of_groups(std::integral_constant<int, F::G>{});
+    else if (p.k <= 64) bound = of_groups(std::integral_constant<int, 1>{});
+    else if (p.k <= 128) bound = of_groups(std::integral_constant<int, 2>{});
+    else bound = of_groups(std::integral_constant<int, 4>{});
     if (bound <= kNone) bound = kNone + 1;
     const float lf = unordered(bound);
     uint64_t least = (uint64_t(bound) << 32) - 1;
@@ -246,22 +257,22 @@ __global__ __launch_bounds__(kTopThreads) void k_top(TopP p) {
     // v and its column, if it goes on the list: where, or kList and more where that is full
     auto append = [&](float v, int64_t e) {
         const uint64_t key = (uint64_t(ordered(v)) << 32) | uint32_t(~uint32_t(e));
-        if (!(v >= lf) || key <= least) return;
+        if (!(v >= lf) || v == -INFINITY || key <= least) return;
         const int at = atomicAdd(&s.count, 1);
         if (at < F::kList) s.list[at] = key;
     };
     const int items = s.groups * cpg;
     for (int it = threadIdx.x; it < items; it += kTopThreads) {
         const int id = group[it / cpg], q = id / kTopThreads, thread = id % kTopThreads;
-        const int j = q * cpg + it % cpg, ch = c0 + thread / kWave + j * kTopWaves;
+        const int j = q * cpg + it % cpg, ch = c0 + thread / kWave + j * kTopWaves, l = thread % kWave;
         if (j >= J || ch >= c1 || s.count > F::kList) continue;
-        const int64_t e0 = int64_t(ch) * kChunk + (thread % kWave) * kEpl;
         Raw<DT, MK> raw;
         float v[kEpl];
-        load_raw<DT, MK, AL>(raw, xrow, mrow, e0, p.V);
+        in.load(raw, ch, l);
         decode<DT, MK>(raw, v, p.tau, tau_one);
+        in.clean(v, ch, l);
 #pragma unroll
-        for (int e = 0; e < kEpl; e++) append(v[e], e0 + e);
+        for (int e = 0; e < kEpl; e++) append(v[e], in.col(ch, l, e));
     }
     __syncthreads();
     int n = s.count;
@@ -404,10 +415,10 @@ extern "C" int nt_hip_rl_top_logprobs(const NtRlTopArgs *a) {
     p.inv_t = added ? 1.0 : 1.0 / a->temperature;
     p.k = int(a->k);
     p.nc = int((a->vocab + kChunk - 1) / kChunk);
-    // About 1024 workgroups, each of a chunk per wave or more, and no more of them than their candidates (k and an eighth and
+    // About 1024 workgroups, each of a chunk per wave or more, and no more of them than their candidates (k and a quarter and
     // 16 each) can be placed together.
     p.segs = int(std::max<int64_t>(1, std::min<int64_t>({1024 / a->rows, int64_t(kTopSegs), (p.nc + kTopWaves - 1) / kTopWaves,
-                                                         (p.k > kFewK ? 4096 : 512) / (p.k + p.k / 8 + 16)})));
+                                                         (p.k > kFewK ? 4096 : 512) / (p.k + p.k / 4 + 16)})));
     p.per = (p.nc + p.segs - 1) / p.segs;
     p.segs = (p.nc + p.per - 1) / p.per;
     p.ids = a->ids;

@@ -33,6 +33,7 @@ constexpr int kRowWaves = kRowThreads / kWave;
 constexpr int kDrawThreads = 256;             // k_verify_draw, k_verify_pick
 constexpr int kDrawWaves = kDrawThreads / kWave;
 constexpr int kMaxDrafts = 127;
+constexpr int kAhead = 4;                     // chunks loaded ahead of f32 sums
 constexpr int kVerifySegs = 64;               // workgroups a position or a drawn row, at most (one lane each)
 // How k_verify_rows sums: in f64, in f32 (see judge), or in f32 with the first largest value.
 enum { kWide, kNarrow, kGreedy };
@@ -208,11 +209,26 @@ struct VerifyRows {
 
 __device__ __forceinline__ int drafts_of(const VerifyP &p, int64_t s) { return p.lengths ? p.lengths[s] : p.K; }
 
+// The draft at position t < n, its values and its uniform, loaded before the sums are known.
+struct Draft {
+    int32_t tok = -1;
+    double x = 0.0, y = 0.0, u = 0.0;
+
+    template <int DT, int MK, bool GREEDY>
+    __device__ __forceinline__ void load(const VerifyP &p, const VerifyRows<DT, MK> &rows, int64_t s, int t, int n) {
+        if (t >= n) return;
+        tok = p.tokens[s * p.K + t];
+        if constexpr (!GREEDY) u = p.u[s * (p.K + 1) + t];
+        if (tok < 0 || tok >= p.V) return;
+        x = token_value<DT, MK>(rows.x, rows.m, tok, p.inv_t);
+        if (rows.y) y = token_value<DT, MK>(rows.y, rows.m, tok, p.inv_td);
+    }
+};
+
 // Position t of a sequence of n drafts, from its merged sums.
 template <int DT, int MK, int HOW>
-__device__ __forceinline__ Verdict judge(const VerifyP &p, int64_t s, int t, int n, const VerifyRec &r) {
+__device__ __forceinline__ Verdict judge(const VerifyP &p, const VerifyRows<DT, MK> &rows, const Draft &w, int t, int n, const VerifyRec &r) {
     Verdict d{kDraw, HOW == kGreedy ? r.at : HOW == kWide, r.a, 0.0, 0.0, 0.0, 0.0};
-    const VerifyRows<DT, MK> rows(p, s, t);
     if (!(r.S == r.S)) {
         d.what = kBad + NT_ROW_NAN;
         return d;
@@ -226,15 +242,14 @@ __device__ __forceinline__ Verdict judge(const VerifyP &p, int64_t s, int t, int
     const bool coarse = HOW == kNarrow && MK == NT_MASK_F32 && fmax(fabs(r.a), r.ad == -INFINITY ? 0.0 : fabs(r.ad)) > 0x1p20;
     if (coarse) d.what = kTooClose;
     if (t >= n) return d;
-    const int32_t tok = p.tokens[s * p.K + t];
-    if (tok < 0 || tok >= p.V) {
+    if (w.tok < 0 || w.tok >= p.V) {
         d.what = kBad + NT_ROW_BAD_TOKEN;
         return d;
     }
-    const double l = (token_value<DT, MK>(rows.x, rows.m, tok, p.inv_t) - r.a) * p.c - d.ls;
+    const double l = (w.x - r.a) * p.c - d.ls;
     d.logp = l * kLn2;
     if constexpr (HOW == kGreedy) {
-        d.what = r.at == tok ? kAccept : kDraw;
+        d.what = r.at == w.tok ? kAccept : kDraw;
         return d;
     }
     double lq = 0.0;
@@ -249,15 +264,14 @@ __device__ __forceinline__ Verdict judge(const VerifyP &p, int64_t s, int t, int
         }
         d.ad = r.ad;
         d.lsd = log2(r.Sd);
-        lq = (token_value<DT, MK>(rows.y, rows.m, tok, p.inv_td) - r.ad) * p.cd - d.lsd;
+        lq = (w.y - r.ad) * p.cd - d.lsd;
     }
     // u q < p: a draft that the drafter gives nothing is accepted where the target gives it something, and one
     // that the target gives nothing never is (inf - inf compares false)
-    const double u = p.u[s * (p.K + 1) + t];
-    d.what = u < exp2(l - lq) ? kAccept : kDraw;
+    d.what = w.u < exp2(l - lq) ? kAccept : kDraw;
     if constexpr (HOW == kNarrow) {
         const double steps = MK == NT_MASK_F32 ? 0x1p-23 * kLog2e64 * (fabs(r.a) + (rows.y ? fabs(r.ad) : 0.0)) : 0.0;
-        if (coarse || fabs(log2(u) - (l - lq)) < kClose32 + steps) d.what = kTooClose;
+        if (coarse || fabs(log2(w.u) - (l - lq)) < kClose32 + steps) d.what = kTooClose;
     }
     return d;
 }
@@ -271,26 +285,6 @@ __device__ __forceinline__ VerifyRec wave_rec(const VerifyP &p, const L &x, cons
     r.S = wave_sum_d(moved(x.S[0], a, r.a, p.c, p.low));
     r.ad = wave_max_d(ad);
     r.Sd = wave_sum_d(moved(y.S[0], ad, r.ad, p.cd, p.lowd));
-    return r;
-}
-
-// The waves' sums in order.
-template <int WAVES>
-__device__ __forceinline__ VerifyRec waves_rec(const VerifyP &p, const VerifyRec *ws) {
-    VerifyRec r = ws[0];
-    for (int w = 1; w < WAVES; w++) {
-        r.a = fmax(r.a, ws[w].a);
-        r.ad = fmax(r.ad, ws[w].ad);
-        if (ws[w].top > r.top || (ws[w].top == r.top && ws[w].at < r.at)) {
-            r.top = ws[w].top;
-            r.at = ws[w].at;
-        }
-    }
-    r.S = r.Sd = 0.0;
-    for (int w = 0; w < WAVES; w++) {
-        r.S += moved(ws[w].S, ws[w].a, r.a, p.c, p.low);
-        r.Sd += moved(ws[w].Sd, ws[w].ad, r.ad, p.cd, p.lowd);
-    }
     return r;
 }
 
@@ -309,35 +303,30 @@ __device__ __forceinline__ VerifyRec merge_recs(const VerifyP &p, const VerifyRe
 }
 
 // f(chunk, target's values, drafter's values) for chunks c, c + step, .. below c1 of a position's rows (both: the
-// drafter's are read), two loaded ahead.
+// drafter's are read).
 template <int DT, int MK, bool AL, int HOW, class F>
 __device__ __forceinline__ void over_rows(const VerifyP &p, const VerifyRows<DT, MK> &rows, bool both, int c, int step, int c1,
                                           int lane, F &&f) {
-    Raw<DT, MK> rx[2];
-    Raw<DT, NT_MASK_NONE> ry[2];
+    constexpr int D = HOW == kWide ? 2 : kAhead;
+    Raw<DT, MK> rx[D];
+    Raw<DT, NT_MASK_NONE> ry[D];
     const RowLoad<DT, MK, AL> x(rows.x, rows.m, p.V, p.nc);
     const RowLoad<DT, NT_MASK_NONE, AL> y(rows.y, nullptr, p.V, p.nc);
-    auto load = [&](int k, int ch) {
-        x.load(rx[k], ch, lane, ch < c1);
-        if (both) y.load(ry[k], ch, lane, ch < c1);
+    auto load = [&](auto k, int ch) {
+        x.load(rx[k.value], ch, lane, ch < c1);
+        if (both) y.load(ry[k.value], ch, lane, ch < c1);
     };
-    auto take = [&](int k, int ch, int next) {
+    stream<D>(c, step, c1, load, [&](auto k, int ch, int next) {
         Lane8<DT, MK, HOW> lx, ly;
-        lx.decode(rx[k].x, rx[k].m, p.inv_t);
+        lx.decode(rx[k.value].x, rx[k.value].m, p.inv_t);
         lx.clean(x, ch, lane);
         if (both) {
-            ly.decode(ry[k].x, rx[k].m, p.inv_td);
+            ly.decode(ry[k.value].x, rx[k.value].m, p.inv_td);
             ly.clean(y, ch, lane);
         }
         load(k, next);
         f(ch, lx, ly);
-    };
-    load(0, c);
-    load(1, c + step);
-    for (; c < c1; c += 2 * step) {
-        take(0, c, c + 2 * step);
-        if (c + step < c1) take(1, c + step, c + 3 * step);
-    }
+    });
 }
 
 // The lanes' sums of a position's rows.
@@ -346,12 +335,12 @@ __device__ __forceinline__ void add_rows(const VerifyP &p, const VerifyRows<DT, 
                                          int lane, L &sx, L &sy, float *top, int32_t *at) {
     over_rows<DT, MK, AL, HOW>(p, rows, both, c, step, c1, lane, [&](int ch, const auto &lx, const auto &ly) {
         if constexpr (HOW == kGreedy) {
-            const int64_t first = RowLoad<DT, MK, AL>(rows.x, rows.m, p.V, p.nc).first(ch, lane);
+            const RowLoad<DT, MK, AL> row(rows.x, rows.m, p.V, p.nc);
 #pragma unroll
             for (int j = 0; j < kEpl; j++) {
                 const bool up = lx.v[j] > *top;
                 *top = up ? lx.v[j] : *top;
-                *at = up ? int32_t(first + j) : *at;
+                *at = up ? int32_t(row.col(ch, lane, j)) : *at;
             }
         }
         if constexpr (HOW == kWide) {
@@ -388,6 +377,8 @@ __global__ __launch_bounds__(kRowThreads) void k_verify_rows(VerifyP p) {
     const bool both = HOW != kGreedy && rows.y != nullptr && t < n;
     const int lane = threadIdx.x & (kWave - 1), wave = __builtin_amdgcn_readfirstlane(int(threadIdx.x / kWave));
     const int c1 = min(p.nc, (seg + 1) * p.per);
+    Draft w;
+    if (p.first) w.load<DT, MK, HOW == kGreedy>(p, rows, s, t, n);
     Sum<HOW> sx, sy;
     float top = -INFINITY;
     int32_t at = 0x7fffffff;
@@ -399,13 +390,14 @@ __global__ __launch_bounds__(kRowThreads) void k_verify_rows(VerifyP p) {
     }
     if (lane == 0) ws[wave] = r;
     __syncthreads();
-    if (threadIdx.x != 0) return;
-    r = waves_rec<kRowWaves>(p, ws);
+    if (wave != 0) return;
+    r = merge_recs(p, ws, kRowWaves, lane);
     if (!p.first) {
-        p.rec[(s * (p.K + 1) + t) * p.segs + seg] = r;
+        if (lane == 0) p.rec[(s * (p.K + 1) + t) * p.segs + seg] = r;
         return;
     }
-    const Verdict d = judge<DT, MK, HOW>(p, s, t, n, r);
+    if (lane != 0) return;
+    const Verdict d = judge<DT, MK, HOW>(p, rows, w, t, n, r);
     p.verdict[s * (p.K + 1) + t] = d;
     if (d.what != kAccept && d.what != kTooClose)
         __hip_atomic_fetch_min(&p.first[s], t, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
@@ -435,8 +427,11 @@ __device__ __forceinline__ int settle(const VerifyP &p, int64_t s, int n, Verdic
         for (int t = threadIdx.x; t <= upto; t += kDrawThreads) vs[t] = p.verdict[s * (p.K + 1) + t];
     } else {
         for (int t = wave; t <= n; t += kDrawWaves) {
+            const VerifyRows<DT, MK> rows(p, s, t);
+            Draft w;
+            w.load<DT, MK, GREEDY>(p, rows, s, t, n);
             const VerifyRec r = merge_recs(p, p.rec + (s * (p.K + 1) + t) * p.segs, p.segs, lane);
-            const Verdict d = judge<DT, MK, GREEDY ? kGreedy : kWide>(p, s, t, n, r);
+            const Verdict d = judge<DT, MK, GREEDY ? kGreedy : kWide>(p, rows, w, t, n, r);
             if (lane == 0) vs[t] = d;
         }
     }
@@ -450,7 +445,9 @@ __device__ __forceinline__ int settle(const VerifyP &p, int64_t s, int n, Verdic
                 const VerifyRec r = wave_rec(p, sx, sy);
                 if (lane == 0) ws[wave] = r;
                 __syncthreads();
-                const Verdict d = judge<DT, MK, kWide>(p, s, a, n, waves_rec<kDrawWaves>(p, ws));
+                Draft w;
+                w.load<DT, MK, false>(p, rows, s, a, n);
+                const Verdict d = judge<DT, MK, kWide>(p, rows, w, a, n, merge_recs(p, ws, kDrawWaves, lane));
                 if (threadIdx.x == 0) vs[a] = d;
                 __syncthreads();
             }
@@ -531,9 +528,9 @@ __global__ __launch_bounds__(kDrawThreads, 4) void k_verify_draw(VerifyP p) {
             }
             q = wave_sum_d(sum8(Q));
         } else if (mode == kDrawOthers) {
-            const int64_t e0 = RowLoad<DT, MK, AL>(rows.x, rows.m, p.V, p.nc).first(ch, lane);
+            const RowLoad<DT, MK, AL> row(rows.x, rows.m, p.V, p.nc);
 #pragma unroll
-            for (int j = 0; j < kEpl; j++) P[j] = e0 + j == tok ? 0.0 : P[j];
+            for (int j = 0; j < kEpl; j++) P[j] = row.col(ch, lane, j) == tok ? 0.0 : P[j];
         }
         const double x = wave_sum_d(sum8(P));
         if (__ballot(left)) q = NAN;
