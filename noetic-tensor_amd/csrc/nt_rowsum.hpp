@@ -124,15 +124,17 @@ struct RowLoad {
 };
 
 // take(slot, chunk, next) for chunks c, c + step, .. below c1 with D of them loaded ahead by load(slot, chunk): take uses
-// the slot's words and then loads `next` into it.
+// the slot's words and then loads `next` into it. The loop takes D chunks at a time with no condition between them, without
+// which the compiler knows how many loads came after the one that it waits for (and else waits for all of them).
 template <int D, class L, class F>
 __device__ __forceinline__ void stream(int c, int step, int c1, L &&load, F &&take) {
     static_for<0, D>([&](auto k) { load(k, c + k.value * step); });
-    for (; c < c1; c += D * step)
-        static_for<0, D>([&](auto k) {
-            const int ch = c + k.value * step;
-            if (ch < c1) take(k, ch, ch + D * step);
-        });
+    for (; c + (D - 1) * step < c1; c += D * step)
+        static_for<0, D>([&](auto k) { take(k, c + k.value * step, c + (k.value + D) * step); });
+    static_for<0, D>([&](auto k) {
+        const int ch = c + k.value * step;
+        if (ch < c1) take(k, ch, c1);
+    });
 }
 
 // N sums (of all weights, of some) relative to the lane's reference: the first maximum it met, moved only where a later
