@@ -187,7 +187,7 @@ __global__ __launch_bounds__(kDistillThreads) void k_distill(DistillP p) {
     auto load = [&](auto i, int ch) { in.load(raw[i.value], ch, lane, ch < c1); };
     stream<kDistillAhead>(c0 + wave, kDistillWaves, c1, load, [&](auto i, int ch, int next) {
         float v[kEpl], w[kEpl];
-        decode<DT, MK>(raw[i.value], v, p.tau, tau_one);
+        decode_e<DT, MK, kEpl>(raw[i.value].x, raw[i.value].m, v, p.tau, tau_one);
         in.clean(v, ch, lane);
         load(i, next);
         sum.weigh(v, p.c32, w);
@@ -326,7 +326,7 @@ __global__ __launch_bounds__(kDistillThreads) void k_distill_grad(DistillP p) {
     auto load = [&](auto i, int ch) { in.load(raw[i.value], ch, lane, ch < c1); };
     stream<kDistillAhead>(c0 + wave, kDistillWaves, c1, load, [&](auto i, int ch, int next) {
         float v[kEpl], o[kEpl];
-        decode<DT, MK>(raw[i.value], v, p.tau, tau_one);
+        decode_e<DT, MK, kEpl>(raw[i.value].x, raw[i.value].m, v, p.tau, tau_one);
         load(i, next);
 #pragma unroll
         for (int j = 0; j < kEpl; j++) o[j] = fmaf(exp2_hw((v[j] - a) * p.c32), factor, 0.0f);

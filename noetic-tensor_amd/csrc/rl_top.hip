@@ -1,7 +1,7 @@
 // nt_hip_rl_top_logprobs: the k most likely tokens of each row and their log-probabilities, in one pass.
 //
 // A workgroup streams its row (or, where rows are few, a piece of one) once, and takes from it the log-sum-exp and the
-// largest value of each group of columns: a lane's columns in an eighth (past 256 k: a sixteenth) of the row.
+// largest value of each group of columns: a lane's columns in a sixteenth of the row.
 // With t the k-th largest of those maxima (joined to 256, 512 or 1024 for few k), k groups reach t, so k columns do, and the columns
 // that reach it lie in groups whose maximum does: those few groups are read again, from the caches, and hardly more than k
 // columns (1.4 k at the most) go on a list in LDS. A column's place is the number of listed ones above it.
@@ -29,7 +29,7 @@ constexpr int kTopAhead = 4;         // chunks a wave loads ahead
 // The two forms, k up to kFewK and past it: G groups a lane, the list's length, and the chunks that go through it at a time in order.
 template <bool BIG>
 struct TopForm {
-    static constexpr int G = BIG ? 16 : 8, kList = BIG ? 4096 : 1024, kRound = BIG ? 4 : 1;
+    static constexpr int G = 16, kList = BIG ? 4096 : 1024, kRound = BIG ? 4 : 1;
     static_assert((BIG ? kMaxK : kFewK) + kRound * kChunk <= kList, "a cut list and a round more");
 };
 
@@ -197,7 +197,7 @@ __global__ __launch_bounds__(kTopThreads) void k_top(TopP p) {
     auto load = [&](auto i, int ch) { in.load(raw[i.value], ch, lane, ch < c1); };
     stream<kTopAhead>(c0 + wave, kTopWaves, c1, load, [&](auto i, int ch, int next) {
         float v[kEpl];
-        decode<DT, MK>(raw[i.value], v, p.tau, tau_one);
+        decode_e<DT, MK, kEpl>(raw[i.value].x, raw[i.value].m, v, p.tau, tau_one);
         in.clean(v, ch, lane);
         load(i, next);
         const float top = sum.add(v, p.c32);
@@ -261,18 +261,30 @@ __global__ __launch_bounds__(kTopThreads) void k_top(TopP p) {
         const int at = atomicAdd(&s.count, 1);
         if (at < F::kList) s.list[at] = key;
     };
+    // (four of their chunks a thread at a time: each costs a load's latency otherwise, 11 us of a row of 151936 f32)
     const int items = s.groups * cpg;
-    for (int it = threadIdx.x; it < items; it += kTopThreads) {
-        const int id = group[it / cpg], q = id / kTopThreads, thread = id % kTopThreads;
-        const int j = q * cpg + it % cpg, ch = c0 + thread / kWave + j * kTopWaves, l = thread % kWave;
-        if (j >= J || ch >= c1 || s.count > F::kList) continue;
-        Raw<DT, MK> raw;
-        float v[kEpl];
-        in.load(raw, ch, l);
-        decode<DT, MK>(raw, v, p.tau, tau_one);
-        in.clean(v, ch, l);
+    constexpr int kItems = 4;
+    for (int t0 = threadIdx.x; t0 < items; t0 += kItems * kTopThreads) {
+        Raw<DT, MK> part[kItems];
+        int at[kItems], of[kItems];
 #pragma unroll
-        for (int e = 0; e < kEpl; e++) append(v[e], in.col(ch, l, e));
+        for (int i = 0; i < kItems; i++) {
+            const int it = min(t0 + i * kTopThreads, items - 1), id = group[it / cpg], thread = id % kTopThreads;
+            const int j = id / kTopThreads * cpg + it % cpg, ch = c0 + thread / kWave + j * kTopWaves;
+            const bool some = t0 + i * kTopThreads < items && j < J && ch < c1;
+            at[i] = some ? ch : -1;
+            of[i] = thread % kWave;
+            in.load(part[i], some ? ch : c0, of[i]);
+        }
+#pragma unroll
+        for (int i = 0; i < kItems; i++) {
+            if (at[i] < 0 || s.count > F::kList) continue;
+            float v[kEpl];
+            decode_e<DT, MK, kEpl>(part[i].x, part[i].m, v, p.tau, tau_one);
+            in.clean(v, at[i], of[i]);
+#pragma unroll
+            for (int e = 0; e < kEpl; e++) append(v[e], in.col(at[i], of[i], e));
+        }
     }
     __syncthreads();
     int n = s.count;
@@ -292,7 +304,7 @@ __global__ __launch_bounds__(kTopThreads) void k_top(TopP p) {
                 Raw<DT, MK> raw;
                 float v[kEpl];
                 load_raw<DT, MK, AL>(raw, xrow, mrow, e0, p.V);
-                decode<DT, MK>(raw, v, p.tau, tau_one);
+                decode_e<DT, MK, kEpl>(raw.x, raw.m, v, p.tau, tau_one);
 #pragma unroll
                 for (int e = 0; e < kEpl; e++) append(v[e], e0 + e);
             }

@@ -125,7 +125,7 @@ struct Lane8 {
                 }
             }
         } else {
-            decode_words<DT, MK>(xw, mw, v, 1.0f, true);
+            decode_e<DT, MK, kEpl>(xw, mw, v, 1.0f, true);
         }
     }
     template <class R>
