@@ -541,7 +541,7 @@ int nt_hip_rl_distill(const NtRlDistillArgs *a);
  *                  = M q_v - rest q_v / (sum of q off the list)    off it (rest 0 but for NT_TAIL_REST)
  * and d / d x = d / d z / T; a listed token that the mask excludes gets its -w term alone, as a scored one's
  * does (nt_hip_rl_score_backward). Written in grad_dtype, rounded once. A row whose g_loss is 0 gets zeros,
- * whatever it holds; a refused one NaN. stats is the forward's for the same inputs. */
+ * whatever it holds; a refused one NaN. stats is the forward's for the same inputs; grad overlaps no input. */
 typedef struct NtRlDistillGradArgs {
     const void *logits;
     int32_t dtype;

@@ -164,7 +164,7 @@ struct LaneSums {
         }
         ref = r;
         neg = now;
-        lim = far ? -INFINITY : r + 60.0f / c;
+        lim = far ? -INFINITY : fminf(r + 60.0f / c, FLT_MAX);  // (an infinity is past it at any temperature)
         return !far;
     }
     // The weights of 8 values; their maximum.

@@ -167,7 +167,7 @@ struct LaneSum {
             if (top < INFINITY) {
                 if (ref != -INFINITY) S[0] *= exp2_64(ref - high, c, low);
                 ref = high;
-                lim = top + cap;
+                lim = fminf(top + cap, FLT_MAX);
             } else {
                 S[0] = NAN;
             }
@@ -737,8 +737,8 @@ extern "C" int nt_hip_rl_verify_drafted(const NtRlVerifyArgs *a) {
     p.cd = added ? kLog2e64 : kLog2e64 / Td;
     p.low = -1100.0 / p.c;
     p.lowd = -1100.0 / p.cd;
-    p.cap = float(500.0 / p.c);
-    p.capd = float(500.0 / p.cd);
+    p.cap = float(std::min(500.0 / p.c, 1e38));  // (an infinity is past it at any temperature)
+    p.capd = float(std::min(500.0 / p.cd, 1e38));
     p.c32 = float(p.c);
     p.cd32 = float(p.cd);
     p.nc = int((a->vocab + kChunk - 1) / kChunk);
