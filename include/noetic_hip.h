@@ -480,8 +480,8 @@ int nt_hip_rl_verify_drafted(const NtRlVerifyArgs *a);
  * mask) from the largest down, ties (-0 and +0 among them) to the lowest index; without an additive mask by the
  * logits themselves, which a quotient's rounding could make equal. ids and logp are [rows, k]. A row of
  * fewer allowed tokens than k has ids -1 and logp -inf after them; one with none (NT_ROW_NO_TOKEN), or
- * with a NaN or +inf among its allowed logits (NT_ROW_NAN), ids -1 and logp NaN throughout. A call of few rows
- * has a workspace of under 10 k + 272 bytes per 2048 columns (64 pieces a row at most); under stream capture 1 MiB or more of it is
+ * with a NaN or +inf among its allowed logits (NT_ROW_NAN), ids -1 and logp NaN throughout. A call of few long
+ * rows has a workspace of under 10 k + 300 bytes per 61440 columns; under stream capture 1 MiB or more of it is
  * refused (NT_E_UNSUPPORTED). */
 typedef struct NtRlTopArgs {
     const void *logits;       /* [rows, ld] f32, bf16 or f16 */

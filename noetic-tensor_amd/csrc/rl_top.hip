@@ -427,9 +427,10 @@ extern "C" int nt_hip_rl_top_logprobs(const NtRlTopArgs *a) {
     p.inv_t = added ? 1.0 : 1.0 / a->temperature;
     p.k = int(a->k);
     p.nc = int((a->vocab + kChunk - 1) / kChunk);
-    // About 1024 workgroups, each of a chunk per wave or more, and no more of them than their candidates (k and a quarter and
-    // 16 each) can be placed together.
-    p.segs = int(std::max<int64_t>(1, std::min<int64_t>({1024 / a->rows, int64_t(kTopSegs), (p.nc + kTopWaves - 1) / kTopWaves,
+    // Up to 512 workgroups, each of 120 chunks or more (the finishing launch is worth about as many: 1 row of 50257 bf16 16.7 us in
+    // one piece, 23.3 in four; 64 of 128256 24.2 in one, 22.9 in two, 31 in four), and no more of a row than what they hand on (k
+    // and a quarter and 16 each) can be placed together.
+    p.segs = int(std::max<int64_t>(1, std::min<int64_t>({512 / a->rows, int64_t(kTopSegs), int64_t(p.nc / 120),
                                                          (p.k > kFewK ? 4096 : 512) / (p.k + p.k / 4 + 16)})));
     p.per = (p.nc + p.segs - 1) / p.segs;
     p.segs = (p.nc + p.per - 1) / p.per;
