@@ -449,9 +449,10 @@ int nt_hip_rl_score_backward(const NtRlScoreGradArgs *a);
  * Rows past a do not matter, whatever they hold. A row that does and has no allowed token (target or drafter:
  * NT_ROW_NO_TOKEN), a NaN or +inf among its allowed logits (NT_ROW_NAN), or a draft outside [0, vocab)
  * (NT_ROW_BAD_TOKEN) ends its sequence there: accepted is its position, its id -1 and its logp NaN. A length
- * outside [0, K] accepts nothing (NT_ROW_BAD_TOKEN). The workspace is under 32 bytes per row of each of its
- * pieces and 8 per sequence and 512 columns; under stream capture a call with 1 MiB of it or more is refused
- * (NT_E_UNSUPPORTED). */
+ * outside [0, K] accepts nothing (NT_ROW_BAD_TOKEN). What decides a token is f64; the
+ * log-probabilities of accepted drafts are, from 256 positions on and greedily, from f32 exponentials (within 4.2e-6). The
+ * workspace is under 64 bytes per row or piece of one and 16 per sequence and 512 columns; under stream capture a call with
+ * 1 MiB of it or more is refused (NT_E_UNSUPPORTED). */
 typedef struct NtRlVerifyArgs {
     const void *logits;        /* [seqs (drafted + 1), ld] */
     const void *draft_logits;  /* [seqs drafted, draft_ld] of the same dtype, or NULL: certain drafts */

@@ -4,14 +4,15 @@
 // Forward: a workgroup (several a row where rows are few) streams the logits once. A bitmap in LDS, a bit a column,
 // says which columns the list holds: that keeps the sum off the list a sum of its own (the whole less
 // the listed part would lose what is left to the rounding of the whole), and finds an id listed twice. Exponentials
-// are f32 relative to a wave's running maximum; a lane's sums are f64.
+// are f32, a lane's sums f64 (LaneSums). HBM bounds it: 4096 x 128256 bf16 162 us, 6.4 TB/s.
 // A divergence is a small difference of large sums, so it is taken as one of its second order: with
 // d = ln q - ln w, sum w (-d) = sum w (e^d - 1 - d) over a whole distribution (sum q = sum w = 1), whose terms
 // are all positive and whose derivative by an error of ln q, sum (q - w), vanishes. The f32
 // exponentials' error then does not reach it.
 //
 // Backward: every column's gradient is its exponential times one factor of the row, written as it streams
-// by; then the listed ones, in f64 and rounded once, are written over it.
+// by; then the listed ones, in f64 and rounded once, are written over it (after a barrier, by the same workgroup).
+// 4096 x 128256 bf16: 408 us, 5.1 TB/s of reads and writes, where a plain copy reaches 4.7.
 #include <algorithm>
 
 #include "nt_exp64.hpp"

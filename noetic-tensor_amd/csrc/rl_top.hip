@@ -10,7 +10,8 @@
 // values), the row goes through it in order, a few hundred columns at a time, and it is cut to its k
 // largest whenever it fills.
 //
-// What bounds it: the row's bytes, and for the log-sum-exp f32 exponentials as the scorer takes them.
+// What bounds it: the row's bytes (64 of 4096 x 50304 bf16: 86 us, 4.8 TB/s), and after each row's stream some 8 us of
+// counting, reading again and placing, which other workgroups' streams hide where there are rounds of them.
 #include <algorithm>
 
 #include "nt_rows.hpp"

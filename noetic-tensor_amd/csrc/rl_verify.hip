@@ -19,6 +19,9 @@
 //    sums are, from the sums of k_verify_rows, but for columns where p / q lies too near 1; a chunk that has such a
 //    column is left to the next kernel, and all are where those sums turn out to be further off.
 //  * k_verify_pick: the chunks' sums of r, then the chunk that holds u sum r, and in it the token.
+//
+// 256 sequences of 7 drafts over 128256 bf16: 110, 58 and 8 to 16 us of them; the first is bound by HBM, the second by
+// f64 exponentials (two a column, 40 us of instructions).
 #include <algorithm>
 
 #include "nt_exp64.hpp"

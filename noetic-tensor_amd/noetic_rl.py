@@ -801,7 +801,7 @@ def verify_drafted(logits: Tensor, draft_logits: Optional[Tensor], tokens: Tenso
     last one the drawn token's (or `uniforms`, device f64 [.., K + 1]); `lengths` i32 [..] says how many drafts a
     sequence has, `draft_temperature` the drafter's where it is another. Returns (ids [.., K + 1], accepted [..],
     logp [.., K + 1]): the accepted drafts and the drawn token, then -1, and their log-probabilities, then 0.
-    Everything is evaluated in f64. `check` reads the sequences' status and refuses what cannot be drawn from."""
+    What decides a token is evaluated in f64. `check` reads the sequences' status and refuses what cannot be drawn from."""
     if not (temperature >= 0.0 and math.isfinite(temperature)):
         raise ValueError(f"verify_drafted: temperature {temperature} (must be ≥ 0)")
     t = Tempered(logits, 1.0 if temperature == 0.0 else temperature, mask)

@@ -70,3 +70,41 @@ def test_captured_calls_of_long_rows_replay(op):
             assert got.to_numpy().tobytes() == w.to_numpy().tobytes()
     for cap in caps:
         cap.close()
+
+
+def test_offsets_past_32_bits():
+    """70000 rows of 65536 bf16 columns, 4.6e9 of them: zeros but for the last two rows."""
+    R, V, k = 70000, 65536, 3
+    rng = np.random.default_rng(2)
+    L = nr.lib()
+    x, grad = nr.Tensor((R, V), "bf16"), nr.Tensor((R, V), "bf16")
+    nr._check(L.nt_hip_memset(C.c_void_p(x.ptr), 0, x.nbytes), "memset")
+    tail = ref.rounded(rng.normal(0, 2, (2, V)), "bf16")
+    bits = ref.bits_of(tail, "bf16")
+    nr._check(L.nt_hip_upload(C.c_void_p(x.ptr + (R - 2) * V * 2), bits.ctypes.data_as(C.c_void_p), bits.nbytes), "upload")
+    ids, lp = (t.to_numpy() for t in nr.top_logprobs(x, k))
+    assert (ids[:-2] == np.arange(k)).all() and (np.abs(lp[:-2] + np.log(V)) <= 2.0 ** -24 * 12 + 4e-6).all()
+    wi, wl = ref.top(tail, tail, k)
+    assert np.array_equal(ids[-2:], wi) and (np.abs(lp[-2:] - wl) <= 2.0 ** -24 * np.abs(wl) + 4e-6).all()
+    it, lt = nr.Tensor.from_numpy(ids), nr.Tensor.from_numpy(np.full((R, k), -2.0, np.float32))
+    loss, stats = nr.distill_with_stats(x, it, lt)
+    g = nr.Tensor.from_numpy(np.ones(R, np.float32))
+    a = nr.NtRlDistillGradArgs(x.ptr, nr.NT_BF16, 0, R, V, V, None, 0, 1.0, k, it.ptr, lt.ptr, stats.rows.ptr, g.ptr, grad.ptr,
+                               nr.NT_BF16, 0, V)
+    nr._check(L.nt_hip_rl_distill_backward(C.byref(a)), "backward")
+    wl, wg, (q, listed, w, rest, q_off, mass, share) = ref.distill(tail, ids[-2:], np.full((2, k), -2.0, np.float32), "REST")
+    assert (np.abs(loss.to_numpy()[-2:] - wl) <= 2.0 ** -24 * np.abs(wl) + 8e-6).all()
+    out = np.empty((2, V), np.uint16)
+    nr._check(L.nt_hip_download(out.ctypes.data_as(C.c_void_p), C.c_void_p(grad.ptr + (R - 2) * V * 2), out.nbytes), "download")
+    got = (out.astype(np.uint32) << 16).view(np.float32).astype(np.float64)
+    tol = np.where(listed, mass[:, None] * q * 8e-6 + 1e-12, (mass + share)[:, None] * q * 2.8e-5) * 1.01
+    assert (np.abs(got - wg) <= tol + 2.0 ** -8 * np.abs(wg) + 2.0 ** -126).all()
+    # sequences of one draft: the last one's rows are the last two
+    S = R // 2
+    u = np.full((S, 2), 0.37)
+    tokens = np.zeros((S, 1), np.int32)
+    got = nr.verify_drafted(nr.Tensor((S, 2, V), "bf16", x.buf), None, nr.Tensor.from_numpy(tokens), 1.0, None, None,
+                            uniforms=nr.Tensor.from_numpy(u, "f64"))
+    want = ref.verify(tail[None], None, tokens[-1:], u[-1:], [1], False)
+    assert np.array_equal(got[0].to_numpy()[-1:], want[0]) and got[1].to_numpy()[-1] == want[1][0]
+    assert (got[1].to_numpy()[:-1] == 0).all()
