@@ -163,7 +163,7 @@ struct LaneSums {
             for (int i = 0; i < N; i++) S[i] *= f;
         }
         ref = r;
-        neg = now;
+        neg = far ? 0.0f : now;  // (unused there, and maybe infinite: an excluded value's weight is 0 and no NaN)
         lim = far ? -INFINITY : fminf(r + 60.0f / c, FLT_MAX);  // (an infinity is past it at any temperature)
         return !far;
     }
