@@ -137,38 +137,36 @@ __device__ __forceinline__ void stream(int c, int step, int c1, L &&load, F &&ta
     });
 }
 
-// N sums (of all weights, of some) relative to the lane's reference: the first maximum it met, moved only where a later
+// A sum relative to the lane's reference: the first maximum it met, moved only where a later
 // value lies 60 log2 units above it, so that most chunks cost a weight one fma, one exponential and one addition. The
 // reference is kept as the f32 product -ref c that the fma adds, and what its rounding and c's leave of it goes
 // into at(). Products past 2^20, whose f32 steps are no small part of a log2 unit, are taken by differences.
 // A weight is within 2^-23 (the instruction) and |t| 2^-23 ln 2 of its argument t (the fma's rounding and
-// c's); a NaN or +inf leaves a NaN in S[0].
-template <int N>
+// c's); a NaN or +inf leaves a NaN in S.
 struct LaneSums {
-    double S[N] = {};
+    double S = 0.0;
     float ref = -INFINITY, neg = 0.0f, lim = -INFINITY;
 
     // Takes `top`, not below the limit (a NaN among others), into the reference; whether weights go by the fma.
     __device__ __forceinline__ bool settle(float top, float c) {
         if (!(top < INFINITY)) {
-            S[0] = NAN;
+            S = NAN;
             return true;
         }
         const float r = fmaxf(ref, top), now = -(r * c);
         const bool far = fabsf(now) > 0x1p20f;
         if (ref != -INFINITY) {
             const double was = lim == -INFINITY ? -double(ref) * double(c) : double(neg);
-            const double f = exp2_64((far ? -double(r) * double(c) : double(now)) - was, 1.0, -1100.0);
-#pragma unroll
-            for (int i = 0; i < N; i++) S[i] *= f;
+            S *= exp2_64((far ? -double(r) * double(c) : double(now)) - was, 1.0, -1100.0);
         }
         ref = r;
         neg = far ? 0.0f : now;  // (unused there, and maybe infinite: an excluded value's weight is 0 and no NaN)
         lim = far ? -INFINITY : fminf(r + 60.0f / c, FLT_MAX);  // (an infinity is past it at any temperature)
         return !far;
     }
-    // The weights of 8 values; their maximum.
-    __device__ __forceinline__ float weigh(const float v[kEpl], float c, float w[kEpl]) {
+    // Takes 8 values; their maximum.
+    __device__ __forceinline__ float add(const float v[kEpl], float c) {
+        float w[kEpl];
         const float top = max8_hw(v);
         bool fast = top <= lim;
         // (lanes without a token so far have none here either: their weights are 0)
@@ -181,12 +179,7 @@ struct LaneSums {
 #pragma unroll
             for (int j = 0; j < kEpl; j++) w[j] = exp2_hw((v[j] - ref) * c);
         }
-        return top;
-    }
-    __device__ __forceinline__ float add(const float v[kEpl], float c) {
-        float w[kEpl];
-        const float top = weigh(v, c, w);
-        S[0] += double(tree8(w));
+        S += double(tree8(w));
         return top;
     }
     // The value whose weight is 1 (c: what c32 is the f32 of); -inf where the lane met no token.

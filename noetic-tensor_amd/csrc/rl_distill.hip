@@ -2,9 +2,10 @@
 // gradient.
 //
 // Forward: a workgroup (several a row where rows are few) streams the logits once. A bitmap in LDS, a bit a column,
-// says which columns the list holds: that keeps the sum off the list a sum of its own (the whole less
-// the listed part would lose what is left to the rounding of the whole), and finds an id listed twice. Exponentials
-// are f32, a lane's sums f64 (LaneSums). HBM bounds it: 4096 x 128256 bf16 162 us, 6.4 TB/s.
+// says which columns the list holds, and finds an id listed twice: the stream sums what is off the list, relative to a
+// maximum off the list (next to that of a listed token its exponentials could all be 0, and the whole less the listed
+// part would lose what is left to the rounding of the whole), and the listed ones join it in f64. Exponentials of the
+// stream are f32, a lane's sum f64 (LaneSums). HBM bounds it: 4096 x 128256 bf16 162 us, 6.4 TB/s.
 // A divergence is a small difference of large sums, so it is taken as one of its second order: with
 // d = ln q - ln w, sum w (-d) = sum w (e^d - 1 - d) over a whole distribution (sum q = sum w = 1), whose terms
 // are all positive and whose derivative by an error of ln q, sum (q - w), vanishes. The f32
@@ -29,7 +30,7 @@ constexpr int kMaxListed = 1024;
 constexpr int kMapChunks = 512;               // chunks a workgroup's bitmap covers: 2^18 columns, 32 KiB
 
 struct DistillRec {
-    double S, R, a;  // sum over the piece, and over its columns off the list, relative to a
+    double R, a;     // sum over the piece's columns off the list, relative to a (-inf: none is allowed)
     int64_t bad;     // an id outside the vocabulary, or one listed twice
 };
 
@@ -41,6 +42,7 @@ struct DistillP {
     float c32, tau;
     int tau_one;
     double inv_t;       // 1 / T
+    double unit;        // z of one unit of value: 1 / T, or 1 with an f32 mask
     int nc, segs, per;
     int k, tail;
     const int32_t *ids;
@@ -55,18 +57,18 @@ struct DistillP {
     int64_t gld;
 };
 
-// z - base of one listed token in f64 (the base a value: see c), -inf where it is excluded.
+// The value of one listed token (see c) in f64, -inf where it is excluded.
 template <int DT, int MK>
-__device__ __forceinline__ double listed_z(const DistillP &p, const void *xrow, const void *mrow, int64_t v, double base) {
+__device__ __forceinline__ double listed_value(const DistillP &p, const void *xrow, const void *mrow, int64_t v) {
     float x;
     if constexpr (DT == NT_F32) x = static_cast<const float *>(xrow)[v];
     else x = widen16<DT>(uint32_t(static_cast<const uint16_t *>(xrow)[v]));
     if constexpr (MK == NT_MASK_U8) {
         if (static_cast<const uint8_t *>(mrow)[v] == 0) return -INFINITY;
     } else if constexpr (MK == NT_MASK_F32) {
-        return (double(x) * p.inv_t + double(static_cast<const float *>(mrow)[v])) - base;
+        return double(x) * p.inv_t + double(static_cast<const float *>(mrow)[v]);
     }
-    return (double(x) - base) * p.inv_t;
+    return double(x);
 }
 
 // A sum over the workgroup in f64; every thread gets it. `s` holds a value per wave.
@@ -80,39 +82,60 @@ __device__ __forceinline__ double group_sum_d(double v, double *s) {
     return t;
 }
 
+// A maximum over the workgroup, likewise.
+__device__ __forceinline__ double group_max_d(double v, double *s) {
+    v = wave_max_d(v);
+    __syncthreads();
+    if ((threadIdx.x & (kWave - 1)) == 0) s[threadIdx.x / kWave] = v;
+    __syncthreads();
+    double t = s[0];
+    for (int w = 1; w < kDistillWaves; w++) t = fmax(t, s[w]);
+    return t;
+}
+
 // A row's loss, statistics and status from its merged sums. The whole workgroup.
 template <int DT, int MK>
 __device__ void distill_finish(const DistillP &p, int64_t row, const DistillRec &r, double *s) {
     const void *xrow = static_cast<const char *>(p.x) + row * p.ld * Elem<DT>::kBytes;
     const void *mrow = nullptr;
     if constexpr (MK != NT_MASK_NONE) mrow = static_cast<const char *>(p.mask) + mask_row_at(p.mm, row) * MaskWords<MK>::kBytes;
-    int st = NT_ROW_OK;
-    if (!(r.S == r.S)) st = NT_ROW_NAN;
-    else if (r.a == -INFINITY) st = NT_ROW_NO_TOKEN;
-    else if (r.bad) st = NT_ROW_BAD_TOKEN;
     const int32_t *ids = p.ids + row * p.k;
     const float *teacher = p.teacher + row * p.k;
     double ln_norm = 0.0;
     if (p.tail == NT_TAIL_RENORMALIZE) {
-        float m = -INFINITY;
-        for (int j = threadIdx.x; j < p.k; j += kDistillThreads) m = ids[j] >= 0 ? fmaxf(m, teacher[j]) : m;
-        m = wave_max(m);
-        __syncthreads();
-        if ((threadIdx.x & (kWave - 1)) == 0) s[threadIdx.x / kWave] = double(m);
-        __syncthreads();
-        for (int w = 0; w < kDistillWaves; w++) m = fmaxf(m, float(s[w]));
-        double t = 0.0;
+        double m = -INFINITY, t = 0.0;
+        for (int j = threadIdx.x; j < p.k; j += kDistillThreads) m = ids[j] >= 0 ? fmax(m, double(teacher[j])) : m;
+        m = group_max_d(m, s);
         for (int j = threadIdx.x; j < p.k; j += kDistillThreads)
-            if (ids[j] >= 0) t += exp(double(teacher[j]) - double(m));
-        ln_norm = double(m) + log(group_sum_d(t, s));
+            if (ids[j] >= 0) t += exp(double(teacher[j]) - m);
+        ln_norm = m + log(group_sum_d(t, s));
     }
-    const double ln_s = log(r.S);
+    // the listed tokens' values (a thread's are kDistillThreads apart), and with their sum the whole row's
+    constexpr int kEach = kMaxListed / kDistillThreads;
+    double v[kEach], a = r.a, listed = 0.0;
+#pragma unroll
+    for (int i = 0; i < kEach; i++) {
+        const int j = i * kDistillThreads + int(threadIdx.x), id = j < p.k ? ids[j] : -1;
+        v[i] = id >= 0 && id < p.V ? listed_value<DT, MK>(p, xrow, mrow, id) : -INFINITY;
+        a = fmax(a, v[i]);
+    }
+    a = group_max_d(a, s);
+#pragma unroll
+    for (int i = 0; i < kEach; i++)
+        if (v[i] != -INFINITY) listed += exp((v[i] - a) * p.unit);  // (a NaN, or +inf less itself: a NaN)
+    const double S = moved(r.R, r.a, a, p.c, p.low) + group_sum_d(listed, s), ln_s = log(S);
+    int st = NT_ROW_OK;
+    if (!(S == S)) st = NT_ROW_NAN;
+    else if (a == -INFINITY) st = NT_ROW_NO_TOKEN;
+    else if (r.bad) st = NT_ROW_BAD_TOKEN;
     double loss = 0.0, mass = 0.0;
     if (st == NT_ROW_OK) {
-        for (int j = threadIdx.x; j < p.k; j += kDistillThreads) {
-            if (ids[j] < 0) continue;
+#pragma unroll
+        for (int i = 0; i < kEach; i++) {
+            const int j = i * kDistillThreads + int(threadIdx.x);
+            if (j >= p.k || ids[j] < 0) continue;
             const double lw = double(teacher[j]) - ln_norm, w = exp(lw);
-            const double lq = listed_z<DT, MK>(p, xrow, mrow, ids[j], r.a) - ln_s, d = lq - lw;
+            const double lq = (v[i] - a) * p.unit - ln_s, d = lq - lw;
             mass += w;
             if (p.tail != NT_TAIL_REST) {
                 if (!(w == 0.0)) loss -= w * d;
@@ -128,10 +151,11 @@ __device__ void distill_finish(const DistillP &p, int64_t row, const DistillRec 
     if (threadIdx.x != 0) return;
     double total = mass, share = 0.0;
     if (p.tail == NT_TAIL_REST) {
-        const double rest = mass < 1.0 ? 1.0 - mass : 0.0, q = r.R / r.S;
+        const double rest = mass < 1.0 ? 1.0 - mass : 0.0;
+        const double lq = r.a == -INFINITY ? -INFINITY : log(r.R) + (r.a - a) * p.unit - ln_s, q = exp(lq);
         total = mass < 1.0 ? 1.0 : mass;
-        if (rest > 0.0 && q > 0.0) {
-            const double d = log(q) - log(rest);
+        if (rest > 0.0 && r.a != -INFINITY) {
+            const double d = lq - log(rest);
             loss += fabs(d) < 1.0 ? rest * (expm1(d) - d) : q - rest - rest * d;
             share = rest / q;
         } else {
@@ -144,9 +168,9 @@ __device__ void distill_finish(const DistillP &p, int64_t row, const DistillRec 
     p.status[row] = uint8_t(st);
     double *o = p.stats + row * NT_DISTILL_STATS;
     // (the backward's f32 base: a value)
-    const double base = double(float(r.a));
+    const double base = double(float(a));
     o[0] = base;
-    o[1] = st == NT_ROW_OK ? r.S * exp2((r.a - base) * p.c) : NAN;
+    o[1] = st == NT_ROW_OK ? S * exp2((a - base) * p.c) : NAN;
     o[2] = total - share;
     o[3] = total;
     o[4] = ln_norm;
@@ -183,17 +207,14 @@ __global__ __launch_bounds__(kDistillThreads) void k_distill(DistillP p) {
     const uint8_t *bytes = reinterpret_cast<const uint8_t *>(map);
 
     const RowLoad<DT, MK, AL> in(xrow, mrow, p.V, p.nc);
-    LaneSums<2> sum;
+    LaneSums sum;
     Raw<DT, MK> raw[kDistillAhead];
     auto load = [&](auto i, int ch) { in.load(raw[i.value], ch, lane, ch < c1); };
     stream<kDistillAhead>(c0 + wave, kDistillWaves, c1, load, [&](auto i, int ch, int next) {
-        float v[kEpl], w[kEpl];
+        float v[kEpl];
         decode_e<DT, MK, kEpl>(raw[i.value].x, raw[i.value].m, v, p.tau, tau_one);
         in.clean(v, ch, lane);
         load(i, next);
-        sum.weigh(v, p.c32, w);
-        float t = tree8(w);
-        sum.S[0] += double(t);
         // bit j for column j
         uint32_t on;
         if constexpr (decltype(in)::kSplit) {
@@ -205,21 +226,17 @@ __global__ __launch_bounds__(kDistillThreads) void k_distill(DistillP p) {
         }
         if (__ballot(on != 0) != 0) {
 #pragma unroll
-            for (int j = 0; j < kEpl; j++) w[j] = (on >> j) & 1u ? 0.0f : w[j];
-            t = tree8(w);
+            for (int j = 0; j < kEpl; j++) v[j] = (on >> j) & 1u ? -INFINITY : v[j];
         }
-        sum.S[1] += double(t);
+        sum.add(v, p.c32);
     });
     const double at = sum.at(p.c, p.c32), top = wave_max_d(at);
-    const double S = wave_sum_d(moved(sum.S[0], at, top, p.c, p.low)), R = wave_sum_d(moved(sum.S[1], at, top, p.c, p.low));
-    if (lane == 0) ws[wave] = DistillRec{S, R, top, 0};
+    const double R = wave_sum_d(moved(sum.S, at, top, p.c, p.low));
+    if (lane == 0) ws[wave] = DistillRec{R, top, 0};
     __syncthreads();
-    DistillRec r{0.0, 0.0, ws[0].a, bad};
+    DistillRec r{0.0, ws[0].a, bad};
     for (int w = 1; w < kDistillWaves; w++) r.a = fmax(r.a, ws[w].a);
-    for (int w = 0; w < kDistillWaves; w++) {
-        r.S += moved(ws[w].S, ws[w].a, r.a, p.c, p.low);
-        r.R += moved(ws[w].R, ws[w].a, r.a, p.c, p.low);
-    }
+    for (int w = 0; w < kDistillWaves; w++) r.R += moved(ws[w].R, ws[w].a, r.a, p.c, p.low);
     if (p.segs > 1) {
         if (threadIdx.x == 0) p.rec[row * p.segs + seg] = r;
         return;
@@ -233,15 +250,12 @@ __global__ __launch_bounds__(kDistillThreads) void k_distill_finish(DistillP p) 
     __shared__ double red[kDistillWaves];
     const int64_t row = blockIdx.x;
     const DistillRec *rec = p.rec + row * p.segs;
-    DistillRec r{0.0, 0.0, -INFINITY, 0};
+    DistillRec r{0.0, -INFINITY, 0};
     for (int g = 0; g < p.segs; g++) {
         r.a = fmax(r.a, rec[g].a);
         r.bad |= rec[g].bad;
     }
-    for (int g = 0; g < p.segs; g++) {
-        r.S += moved(rec[g].S, rec[g].a, r.a, p.c, p.low);
-        r.R += moved(rec[g].R, rec[g].a, r.a, p.c, p.low);
-    }
+    for (int g = 0; g < p.segs; g++) r.R += moved(rec[g].R, rec[g].a, r.a, p.c, p.low);
     distill_finish<DT, MK>(p, row, r, red);
 }
 
@@ -348,7 +362,7 @@ __global__ __launch_bounds__(kDistillThreads) void k_distill_grad(DistillP p) {
         const int64_t id = p.ids[row * p.k + j];
         if (id < int64_t(c0) * kChunk || id >= int64_t(c1) * kChunk || id >= p.V) continue;
         const double w = exp(double(p.teacher[row * p.k + j]) - st[4]);
-        const double q = exp(listed_z<DT, MK>(p, xrow, mrow, id, base)) / S;
+        const double q = exp((listed_value<DT, MK>(p, xrow, mrow, id) - base) * p.unit) / S;
         const double o = scale * (st[3] * q - w);
         if constexpr (GDT == NT_F32) {
             static_cast<float *>(grow)[id] = float(o);
@@ -430,6 +444,7 @@ int nt_hip_rl_distill(const NtRlDistillArgs *a) {
     p.c32 = float(p.c);
     p.low = -1100.0 / p.c;
     p.inv_t = 1.0 / a->temperature;
+    p.unit = a->mask_kind == NT_MASK_F32 ? 1.0 : p.inv_t;
     p.nc = int((a->vocab + kChunk - 1) / kChunk);
     // (the finishing launch is worth 120 chunks: 128 rows of 32000 bf16 16.4 us in one piece, 18.9 in two; 1 of 128256 19.7 and 19.1)
     cut_rows(a->rows, p.nc, 512, 120, &p.segs, &p.per);
@@ -493,6 +508,7 @@ int nt_hip_rl_distill_backward(const NtRlDistillGradArgs *a) {
     p.c32 = float(p.c);
     p.low = -1100.0 / p.c;
     p.inv_t = 1.0 / a->temperature;
+    p.unit = a->mask_kind == NT_MASK_F32 ? 1.0 : p.inv_t;
     p.nc = int((a->vocab + kChunk - 1) / kChunk);
     cut_rows(a->rows, p.nc, 4096, kDistillWaves, &p.segs, &p.per);
     p.k = int(a->k);

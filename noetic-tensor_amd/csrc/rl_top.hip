@@ -191,7 +191,7 @@ __global__ __launch_bounds__(kTopThreads) void k_top(TopP p) {
     // the wave's chunks are c0 + wave + 4 j; group q of a lane has j in [q cpg, q cpg + cpg)
     const int J = (c1 - c0 + kTopWaves - 1) / kTopWaves, cpg = (J + F::G - 1) / F::G;
     if (threadIdx.x == 0) s.count = s.groups = 0;
-    LaneSums<1> sum;
+    LaneSums sum;
     float gm = -INFINITY;
     int q = 0, left = cpg;
     Raw<DT, MK> raw[kTopAhead];
@@ -213,7 +213,7 @@ __global__ __launch_bounds__(kTopThreads) void k_top(TopP p) {
         s.gmax[q * kTopThreads + threadIdx.x] = gm;
         gm = -INFINITY;
     }
-    double S = sum.S[0], a = sum.at(p.c, p.c32);
+    double S = sum.S, a = sum.at(p.c, p.c32);
     wave_merge(p, S, a);
     if (lane == 0) {
         s.S[wave] = S;

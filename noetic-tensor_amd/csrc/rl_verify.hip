@@ -152,7 +152,7 @@ __device__ __forceinline__ double sum8(const double r[kEpl]) {
 // A lane's f64 sum relative to its reference: the first maximum it met, moved only where a later value lies 2^500 above
 // it, which f64 holds and logits hardly reach. A NaN or +inf leaves a NaN.
 struct LaneSum {
-    double S[1] = {}, ref = -INFINITY;
+    double S = 0.0, ref = -INFINITY;
     float lim = -INFINITY;
 
     template <class L>
@@ -168,17 +168,17 @@ struct LaneSum {
         }
         if (over) {
             if (top < INFINITY) {
-                if (ref != -INFINITY) S[0] *= exp2_64(ref - high, c, low);
+                if (ref != -INFINITY) S *= exp2_64(ref - high, c, low);
                 ref = high;
                 lim = fminf(top + cap, FLT_MAX);
             } else {
-                S[0] = NAN;
+                S = NAN;
             }
         }
         double w[kEpl];
 #pragma unroll
         for (int j = 0; j < kEpl; j++) w[j] = exp2_64(l.at(j) - ref, c, low);
-        S[0] += sum8(w);
+        S += sum8(w);
     }
     __device__ __forceinline__ double at(double, float) const { return ref; }
 };
@@ -285,9 +285,9 @@ __device__ __forceinline__ VerifyRec wave_rec(const VerifyP &p, const L &x, cons
     VerifyRec r{0.0, 0.0, -INFINITY, -INFINITY, 0, 0.0f};
     const double a = x.at(p.c, p.c32), ad = y.at(p.cd, p.cd32);
     r.a = wave_max_d(a);
-    r.S = wave_sum_d(moved(x.S[0], a, r.a, p.c, p.low));
+    r.S = wave_sum_d(moved(x.S, a, r.a, p.c, p.low));
     r.ad = wave_max_d(ad);
-    r.Sd = wave_sum_d(moved(y.S[0], ad, r.ad, p.cd, p.lowd));
+    r.Sd = wave_sum_d(moved(y.S, ad, r.ad, p.cd, p.lowd));
     return r;
 }
 
@@ -357,7 +357,7 @@ __device__ __forceinline__ void add_rows(const VerifyP &p, const VerifyRows<DT, 
 }
 
 template <int HOW>
-using Sum = std::conditional_t<HOW == kWide, LaneSum, LaneSums<1>>;
+using Sum = std::conditional_t<HOW == kWide, LaneSum, LaneSums>;
 
 template <int DT, int MK, bool AL, int HOW>
 __global__ __launch_bounds__(kRowThreads) void k_verify_rows(VerifyP p) {
