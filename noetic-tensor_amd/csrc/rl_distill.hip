@@ -11,7 +11,8 @@
 // are all positive and whose derivative by an error of ln q, sum (q - w), vanishes. The f32
 // exponentials' error then does not reach it.
 //
-// Backward: every column's gradient is its exponential times one factor of the row, written as it streams
+// Backward: every column's gradient is its exponential times one factor of the row, both relative to a maximum off the list
+// (relative to a listed token's the exponentials could be 0 and the factor past f32), written as it streams
 // by; then the listed ones, in f64 and rounded once, are written over it (after a barrier, by the same workgroup).
 // 4096 x 128256 bf16: 408 us, 5.1 TB/s of reads and writes, where a plain copy reaches 4.7.
 #include <algorithm>
@@ -128,7 +129,7 @@ __device__ void distill_finish(const DistillP &p, int64_t row, const DistillRec 
     if (!(S == S)) st = NT_ROW_NAN;
     else if (a == -INFINITY) st = NT_ROW_NO_TOKEN;
     else if (r.bad) st = NT_ROW_BAD_TOKEN;
-    double loss = 0.0, mass = 0.0;
+    double loss = 0.0, mass = 0.0, rest = 0.0;
     if (st == NT_ROW_OK) {
 #pragma unroll
         for (int i = 0; i < kEach; i++) {
@@ -149,15 +150,14 @@ __device__ void distill_finish(const DistillP &p, int64_t row, const DistillRec 
     loss = group_sum_d(loss, s);
     mass = group_sum_d(mass, s);
     if (threadIdx.x != 0) return;
-    double total = mass, share = 0.0;
+    double total = mass;
     if (p.tail == NT_TAIL_REST) {
-        const double rest = mass < 1.0 ? 1.0 - mass : 0.0;
+        rest = mass < 1.0 ? 1.0 - mass : 0.0;
         const double lq = r.a == -INFINITY ? -INFINITY : log(r.R) + (r.a - a) * p.unit - ln_s, q = exp(lq);
         total = mass < 1.0 ? 1.0 : mass;
         if (rest > 0.0 && r.a != -INFINITY) {
             const double d = lq - log(rest);
             loss += fabs(d) < 1.0 ? rest * (expm1(d) - d) : q - rest - rest * d;
-            share = rest / q;
         } else {
             // (an outcome of one side alone: the terms' sum is then over other masses than 1 and 1)
             loss += q - rest;
@@ -167,12 +167,15 @@ __device__ void distill_finish(const DistillP &p, int64_t row, const DistillRec 
     p.loss[row] = st == NT_ROW_OK ? float(loss) : NAN;
     p.status[row] = uint8_t(st);
     double *o = p.stats + row * NT_DISTILL_STATS;
-    // (the backward's f32 base: a value)
-    const double base = double(float(a));
+    // For the backward, off the list: an f32 value as the base of its exponentials, and the factor of one,
+    // total q_off / R - rest / R with R relative to the base. On it: the reference of q, and total over the sum relative to that.
+    const bool off = r.a != -INFINITY;
+    const double base = off ? double(float(fmin(fmax(r.a, -double(FLT_MAX)), double(FLT_MAX)))) : 0.0;
+    const double factor = off ? (total * exp((r.a - a) * p.unit) / S - rest / r.R) * exp2((base - r.a) * p.c) : 0.0;
     o[0] = base;
-    o[1] = st == NT_ROW_OK ? S * exp2((a - base) * p.c) : NAN;
-    o[2] = total - share;
-    o[3] = total;
+    o[1] = st == NT_ROW_OK ? factor : NAN;
+    o[2] = a;
+    o[3] = st == NT_ROW_OK ? total / S : NAN;
     o[4] = ln_norm;
 }
 
@@ -333,8 +336,8 @@ __global__ __launch_bounds__(kDistillThreads) void k_distill_grad(DistillP p) {
         return;
     }
     const double *st = p.stats + row * NT_DISTILL_STATS;
-    const double base = st[0], S = st[1], scale = double(g) * p.inv_t;
-    const float a = float(base), factor = float(scale * st[2] / S);
+    const double scale = double(g) * p.inv_t;
+    const float base = float(st[0]), factor = float(scale * st[1]);
     const bool tau_one = p.tau_one != 0;
     const RowLoad<DT, MK, AL> in(xrow, mrow, p.V, p.nc);
     Raw<DT, MK> raw[kDistillAhead];
@@ -344,7 +347,7 @@ __global__ __launch_bounds__(kDistillThreads) void k_distill_grad(DistillP p) {
         decode_e<DT, MK, kEpl>(raw[i.value].x, raw[i.value].m, v, p.tau, tau_one);
         load(i, next);
 #pragma unroll
-        for (int j = 0; j < kEpl; j++) o[j] = fmaf(exp2_hw((v[j] - a) * p.c32), factor, 0.0f);
+        for (int j = 0; j < kEpl; j++) o[j] = fmaf(exp2_hw((v[j] - base) * p.c32), factor, 0.0f);
         if constexpr (decltype(in)::kSplit) {
             store4<GDT>(grow, in.col(ch, lane, 0), p.V, o);
             store4<GDT>(grow, in.col(ch, lane, 4), p.V, o + 4);
@@ -362,8 +365,8 @@ __global__ __launch_bounds__(kDistillThreads) void k_distill_grad(DistillP p) {
         const int64_t id = p.ids[row * p.k + j];
         if (id < int64_t(c0) * kChunk || id >= int64_t(c1) * kChunk || id >= p.V) continue;
         const double w = exp(double(p.teacher[row * p.k + j]) - st[4]);
-        const double q = exp((listed_value<DT, MK>(p, xrow, mrow, id) - base) * p.unit) / S;
-        const double o = scale * (st[3] * q - w);
+        const double q = exp((listed_value<DT, MK>(p, xrow, mrow, id) - st[2]) * p.unit) * st[3];  // (times the total)
+        const double o = scale * (q - w);
         if constexpr (GDT == NT_F32) {
             static_cast<float *>(grow)[id] = float(o);
         } else if constexpr (GDT == NT_F16) {

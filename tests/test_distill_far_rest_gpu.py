@@ -95,3 +95,36 @@ def test_one_unlisted_token_that_the_mask_allows():
                                     nr.Tensor.from_numpy(ids), nr.Tensor.from_numpy(lp))
     want, _, _, first = form(z, ids, lp, "REST")
     assert (np.abs(loss.to_numpy() - want) <= 2.0 ** -24 * np.abs(want) + 2 * E * first + 1e-9).all() and (want > 20).all()
+
+
+@pytest.mark.parametrize("tail", ["REST", "DROP"])
+@pytest.mark.parametrize("V, gap, T, dtype", CASES)
+def test_its_gradient(V, gap, T, dtype, tail):
+    rng = np.random.default_rng(V + abs(gap) + 1)
+    for R in (2, 300) if V < 100000 else (2,):
+        x, z, ids, lp = rows(V, gap, T, dtype, R, min(4, V // 3), rng)
+        logits, it, lt = nr.Tempered(ref.tensor(x, dtype), T, None), nr.Tensor.from_numpy(ids), nr.Tensor.from_numpy(lp)
+        _, stats = nr.distill_with_stats(logits, it, lt, nr.TeacherTail[tail])
+        # (f16: a loss scale)
+        g = (rng.uniform(0.5, 1.0, R) * (4096.0 if dtype == "f16" else 1.0)).astype(np.float32)
+        got = ref.values(nr.distill_grad(logits, it, lt, stats, nr.Tensor.from_numpy(g)))
+        _, want, tol, _ = form(z, ids, lp, tail)
+        s = g.astype(np.float64)[:, None] / T
+        err = np.abs(got - want * s)
+        assert (err <= tol * s * (1 + 2.0 ** -7) + ref.HALF_ULP[dtype] * np.abs(want * s) + TINY[dtype]).all()
+
+
+def test_excluded_columns_beside_a_far_rest_have_no_gradient():
+    rng = np.random.default_rng(2)
+    for gap in (50.0, 100.0, 1000.0):
+        R, V, k = 4, 2003, 2
+        x, z, ids, lp = rows(V, gap, 1.0, "f32", R, k, rng)
+        keep = (rng.random((R, V)) < 0.5).astype(np.uint8)
+        np.put_along_axis(keep, ids, 1, 1)
+        logits = nr.Tempered(ref.tensor(x, "f32"), 1.0, nr.Tensor.from_numpy(keep, "u8"))
+        it, lt = nr.Tensor.from_numpy(ids), nr.Tensor.from_numpy(lp)
+        _, stats = nr.distill_with_stats(logits, it, lt)
+        got = nr.distill_grad(logits, it, lt, stats, nr.Tensor.from_numpy(np.ones(R, np.float32))).to_numpy()
+        _, want, tol, _ = form(np.where(keep == 0, -np.inf, z), ids, lp, "REST")
+        assert (got[keep == 0] == 0.0).all()
+        assert (np.abs(got - want) <= tol + 2.0 ** -24 * np.abs(want) + TINY["f32"]).all()
