@@ -501,7 +501,7 @@ typedef struct NtRlTopArgs {
 int nt_hip_rl_top_logprobs(const NtRlTopArgs *a);
 
 /* Distillation from a teacher's recorded tokens: the divergence of each row's softmax q (of the student's
- * tempered logits) from the teacher's weights w_j = exp(teacher_logp[r, j]) at tokens ids[r, j]:
+ * tempered logits z = x / T + mask in f64) from the teacher's weights w_j = exp(teacher_logp[r, j]) at tokens ids[r, j]:
  *   NT_TAIL_REST         what the list leaves, rest = max(1 - sum w, 0), is one outcome more:
  *                        loss = sum w (ln w - ln q) + rest (ln rest - ln of the sum of q off the list)
  *   NT_TAIL_DROP         loss = sum w (ln w - ln q)

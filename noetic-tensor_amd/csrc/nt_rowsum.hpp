@@ -116,10 +116,11 @@ struct RowLoad {
         if constexpr (AL) return e < V;
         else return e >= own(ch, lane) && e < V;
     }
-    __device__ __forceinline__ void clean(float v[kEpl], int ch, int lane) const {
+    template <class T>
+    __device__ __forceinline__ void clean(T (&v)[kEpl], int ch, int lane) const {
         if (ch != last) return;
 #pragma unroll
-        for (int j = 0; j < kEpl; j++) v[j] = mine(ch, lane, j) ? v[j] : -INFINITY;
+        for (int j = 0; j < kEpl; j++) v[j] = mine(ch, lane, j) ? v[j] : T(-INFINITY);
     }
 };
 

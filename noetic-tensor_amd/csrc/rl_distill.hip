@@ -5,7 +5,8 @@
 // says which columns the list holds, and finds an id listed twice: the stream sums what is off the list, relative to a
 // maximum off the list (next to that of a listed token its exponentials could all be 0, and the whole less the listed
 // part would lose what is left to the rounding of the whole), and the listed ones join it in f64. Exponentials of the
-// stream are f32, a lane's sum f64 (LaneSums). HBM bounds it: 4096 x 128256 bf16 162 us, 6.4 TB/s.
+// stream are f32, a lane's sum f64 (LaneSums). HBM bounds it: 4096 x 128256 bf16 162 us, 6.4 TB/s. With an additive mask z is f64
+// throughout, as it is for the listed tokens (FarSum).
 // A divergence is a small difference of large sums, so it is taken as one of its second order: with
 // d = ln q - ln w, sum w (-d) = sum w (e^d - 1 - d) over a whole distribution (sum q = sum w = 1), whose terms
 // are all positive and whose derivative by an error of ln q, sum (q - w), vanishes. The f32
@@ -40,8 +41,7 @@ struct DistillP {
     int64_t V, ld;
     MaskMap mm;
     double c, low;      // exponent scale of a value: log2(e) / T (none, u8) or log2(e) (f32 mask); -1100 / c
-    float c32, tau;
-    int tau_one;
+    float c32;
     double inv_t;       // 1 / T
     double unit;        // z of one unit of value: 1 / T, or 1 with an f32 mask
     int nc, segs, per;
@@ -58,6 +58,41 @@ struct DistillP {
     int64_t gld;
 };
 
+// A tempered logit under an additive mask. In f64: a mask may lower a whole row so far (-1e9) that an f32 step is no small part
+// of its logits' differences, and the sums and the listed tokens have to be of the same values.
+__device__ __forceinline__ double tempered64(const DistillP &p, float x, float m) { return fma(double(x), p.inv_t, double(m)); }
+
+// A lane's sum of 2^(z log2(e)) over such z, as LaneSums: of f32 exponentials, their arguments f64 differences from the reference
+// rounded once, the reference moved where a value lies 16 above it. A NaN or +inf leaves a NaN.
+struct FarSum {
+    static constexpr double kNothing = -0x1p1000;  // below every finite z
+    double S = 0.0, ref = kNothing;
+
+    __device__ __forceinline__ void add(const double z[kEpl], double low) {
+        float d[kEpl];
+#pragma unroll
+        for (int j = 0; j < kEpl; j++) d[j] = float(z[j] - ref);
+        if (!(max8_hw(d) <= 16.0f)) {
+            double high = z[0];
+#pragma unroll
+            for (int j = 1; j < kEpl; j++) high = fmax(high, z[j]);
+            if (high < INFINITY) {
+                S *= exp2_64(ref - high, kLog2e64, low);
+                ref = high;
+#pragma unroll
+                for (int j = 0; j < kEpl; j++) d[j] = float(z[j] - ref);
+            } else {
+                S = NAN;
+            }
+        }
+#pragma unroll
+        for (int j = 0; j < kEpl; j++) d[j] = exp2_hw(d[j] * kLog2e);
+        S += double(tree8(d));
+    }
+    // The z whose weight is 1; -inf where the lane met no token.
+    __device__ __forceinline__ double at(double, float) const { return ref == kNothing ? -INFINITY : ref; }
+};
+
 // The value of one listed token (see c) in f64, -inf where it is excluded.
 template <int DT, int MK>
 __device__ __forceinline__ double listed_value(const DistillP &p, const void *xrow, const void *mrow, int64_t v) {
@@ -67,7 +102,7 @@ __device__ __forceinline__ double listed_value(const DistillP &p, const void *xr
     if constexpr (MK == NT_MASK_U8) {
         if (static_cast<const uint8_t *>(mrow)[v] == 0) return -INFINITY;
     } else if constexpr (MK == NT_MASK_F32) {
-        return double(x) * p.inv_t + double(static_cast<const float *>(mrow)[v]);
+        return tempered64(p, x, static_cast<const float *>(mrow)[v]);
     }
     return double(x);
 }
@@ -167,10 +202,11 @@ __device__ void distill_finish(const DistillP &p, int64_t row, const DistillRec 
     p.loss[row] = st == NT_ROW_OK ? float(loss) : NAN;
     p.status[row] = uint8_t(st);
     double *o = p.stats + row * NT_DISTILL_STATS;
-    // For the backward, off the list: an f32 value as the base of its exponentials, and the factor of one,
-    // total q_off / R - rest / R with R relative to the base. On it: the reference of q, and total over the sum relative to that.
+    // For the backward, off the list: the base of its exponentials (a value that f32 holds but under an additive mask), and the
+    // factor of one, total q_off / R - rest / R with R relative to the base. On it: the reference of q, and total over the sum relative to that.
     const bool off = r.a != -INFINITY;
-    const double base = off ? double(float(fmin(fmax(r.a, -double(FLT_MAX)), double(FLT_MAX)))) : 0.0;
+    const double held = MK == NT_MASK_F32 ? r.a : double(float(fmin(fmax(r.a, -double(FLT_MAX)), double(FLT_MAX))));
+    const double base = off ? held : 0.0;
     const double factor = off ? (total * exp((r.a - a) * p.unit) / S - rest / r.R) * exp2((base - r.a) * p.c) : 0.0;
     o[0] = base;
     o[1] = st == NT_ROW_OK ? factor : NAN;
@@ -191,7 +227,6 @@ __global__ __launch_bounds__(kDistillThreads) void k_distill(DistillP p) {
     const void *xrow = static_cast<const char *>(p.x) + row * p.ld * Elem<DT>::kBytes;
     const void *mrow = nullptr;
     if constexpr (MK != NT_MASK_NONE) mrow = static_cast<const char *>(p.mask) + mask_row_at(p.mm, row) * MaskWords<MK>::kBytes;
-    const bool tau_one = p.tau_one != 0;
     const int c0 = seg * p.per, c1 = min(p.nc, c0 + p.per);
 
     for (int i = threadIdx.x; i < (c1 - c0) * (kChunk / 32); i += kDistillThreads) map[i] = 0;
@@ -210,12 +245,17 @@ __global__ __launch_bounds__(kDistillThreads) void k_distill(DistillP p) {
     const uint8_t *bytes = reinterpret_cast<const uint8_t *>(map);
 
     const RowLoad<DT, MK, AL> in(xrow, mrow, p.V, p.nc);
-    LaneSums sum;
+    std::conditional_t<MK == NT_MASK_F32, FarSum, LaneSums> sum;
     Raw<DT, MK> raw[kDistillAhead];
     auto load = [&](auto i, int ch) { in.load(raw[i.value], ch, lane, ch < c1); };
     stream<kDistillAhead>(c0 + wave, kDistillWaves, c1, load, [&](auto i, int ch, int next) {
-        float v[kEpl];
-        decode_e<DT, MK, kEpl>(raw[i.value].x, raw[i.value].m, v, p.tau, tau_one);
+        std::conditional_t<MK == NT_MASK_F32, double, float> v[kEpl];
+        if constexpr (MK == NT_MASK_F32) {
+#pragma unroll
+            for (int j = 0; j < kEpl; j++) v[j] = tempered64(p, logit<DT>(raw[i.value].x, j), __uint_as_float(raw[i.value].m[j]));
+        } else {
+            decode_e<DT, MK, kEpl>(raw[i.value].x, raw[i.value].m, v, 1.0f, true);
+        }
         in.clean(v, ch, lane);
         load(i, next);
         // bit j for column j
@@ -231,7 +271,8 @@ __global__ __launch_bounds__(kDistillThreads) void k_distill(DistillP p) {
 #pragma unroll
             for (int j = 0; j < kEpl; j++) v[j] = (on >> j) & 1u ? -INFINITY : v[j];
         }
-        sum.add(v, p.c32);
+        if constexpr (MK == NT_MASK_F32) sum.add(v, p.low);
+        else sum.add(v, p.c32);
     });
     const double at = sum.at(p.c, p.c32), top = wave_max_d(at);
     const double R = wave_sum_d(moved(sum.S, at, top, p.c, p.low));
@@ -337,17 +378,25 @@ __global__ __launch_bounds__(kDistillThreads) void k_distill_grad(DistillP p) {
     }
     const double *st = p.stats + row * NT_DISTILL_STATS;
     const double scale = double(g) * p.inv_t;
-    const float base = float(st[0]), factor = float(scale * st[1]);
-    const bool tau_one = p.tau_one != 0;
+    const double far = st[0];
+    const float base = float(far), factor = float(scale * st[1]);
     const RowLoad<DT, MK, AL> in(xrow, mrow, p.V, p.nc);
     Raw<DT, MK> raw[kDistillAhead];
     auto load = [&](auto i, int ch) { in.load(raw[i.value], ch, lane, ch < c1); };
     stream<kDistillAhead>(c0 + wave, kDistillWaves, c1, load, [&](auto i, int ch, int next) {
         float v[kEpl], o[kEpl];
-        decode_e<DT, MK, kEpl>(raw[i.value].x, raw[i.value].m, v, p.tau, tau_one);
+        if constexpr (MK == NT_MASK_F32) {
+#pragma unroll
+            for (int j = 0; j < kEpl; j++)
+                v[j] = float(tempered64(p, logit<DT>(raw[i.value].x, j), __uint_as_float(raw[i.value].m[j])) - far);
+        } else {
+            decode_e<DT, MK, kEpl>(raw[i.value].x, raw[i.value].m, v, 1.0f, true);
+#pragma unroll
+            for (int j = 0; j < kEpl; j++) v[j] -= base;
+        }
         load(i, next);
 #pragma unroll
-        for (int j = 0; j < kEpl; j++) o[j] = fmaf(exp2_hw((v[j] - base) * p.c32), factor, 0.0f);
+        for (int j = 0; j < kEpl; j++) o[j] = fmaf(exp2_hw(v[j] * p.c32), factor, 0.0f);
         if constexpr (decltype(in)::kSplit) {
             store4<GDT>(grow, in.col(ch, lane, 0), p.V, o);
             store4<GDT>(grow, in.col(ch, lane, 4), p.V, o + 4);
@@ -441,8 +490,6 @@ int nt_hip_rl_distill(const NtRlDistillArgs *a) {
     p.V = a->vocab;
     p.ld = a->ld;
     p.mm = mm;
-    p.tau = float(a->temperature);
-    p.tau_one = a->temperature == 1.0;
     p.c = a->mask_kind == NT_MASK_F32 ? kLog2e64 : kLog2e64 / a->temperature;
     p.c32 = float(p.c);
     p.low = -1100.0 / p.c;
@@ -505,8 +552,6 @@ int nt_hip_rl_distill_backward(const NtRlDistillGradArgs *a) {
     p.V = a->vocab;
     p.ld = a->ld;
     p.mm = mm;
-    p.tau = float(a->temperature);
-    p.tau_one = a->temperature == 1.0;
     p.c = a->mask_kind == NT_MASK_F32 ? kLog2e64 : kLog2e64 / a->temperature;
     p.c32 = float(p.c);
     p.low = -1100.0 / p.c;

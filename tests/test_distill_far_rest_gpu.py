@@ -21,8 +21,9 @@ def device():
 
 
 def lse(z):
+    """The largest and what the log-sum-exp is above it, apart: the largest may be of any size."""
     m = z.max(1, keepdims=True)
-    return (m + np.log(np.exp(z - m).sum(1, keepdims=True)))[:, 0]
+    return m, np.log(np.exp(z - m).sum(1, keepdims=True))
 
 
 def form(z, ids, lp, tail):
@@ -31,8 +32,8 @@ def form(z, ids, lp, tail):
     w, rest = ref.teacher_weights(lp, ids, tail)
     on = np.zeros((R, V), bool)
     np.put_along_axis(on, ids, True, 1)
-    whole, off = lse(z), lse(np.where(on, -np.inf, z))
-    lnq, ln_off = z - whole[:, None], off - whole
+    (m, above), (m_off, above_off) = lse(z), lse(np.where(on, -np.inf, z))
+    lnq, ln_off = (z - m) - above, ((m_off - m) + (above_off - above))[:, 0]
     dense = np.zeros((R, V))
     np.put_along_axis(dense, ids, w, 1)
     mass = w.sum(1) + rest
@@ -40,7 +41,7 @@ def form(z, ids, lp, tail):
         loss = np.where(w > 0, w * (np.log(w) - np.take_along_axis(lnq, ids, 1)), 0.0).sum(1)
         loss = loss + np.where(rest > 0, rest * (np.log(rest) - ln_off), 0.0)
     q = np.exp(lnq)
-    alone = rest[:, None] * np.exp(np.minimum(z - off[:, None], 0.0))
+    alone = rest[:, None] * np.exp(np.minimum((z - m_off) - above_off, 0.0))
     grad = np.where(on, mass[:, None] * q - dense, mass[:, None] * q - alone)
     tol = np.where(on, mass[:, None] * q * 2 * E + 1e-12, (mass[:, None] * q + alone) * (2 * E + 2e-5))
     first = np.abs(np.exp(ln_off) - rest) if tail == "REST" else mass
