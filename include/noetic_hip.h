@@ -442,8 +442,8 @@ int nt_hip_rl_score_backward(const NtRlScoreGradArgs *a);
  * accepted) from p itself: the first v with sum_{j <= v} r_j > uniforms[s, K] sum r, or the last with r > 0.
  * What is kept is then distributed as the target's own samples are. Temperature 0 is greedy: a draft is
  * accepted where it is the first argmax of the target's masked logits (in f32), which is also the token at a;
- * no uniforms and no draft logits are read, and logp is that of the temperature-1 distribution, as
- * nt_hip_rl_sample's.
+ * no uniforms and no draft logits are read, and logp is that of the temperature-1 distribution of those f32
+ * values, as nt_hip_rl_sample's.
  *   accepted[s] = a;  ids[s, 0 .. a] = the accepted drafts and the drawn token, -1 after them;
  *   logp[s, t] = ln p(ids[s, t]), 0 after them.
  * Rows past a do not matter, whatever they hold. A row that does and has no allowed token (target or drafter:

@@ -183,8 +183,9 @@ struct LaneSum {
     __device__ __forceinline__ double at(double, float) const { return ref; }
 };
 
-// The value of one token (see Lane8), -inf where it is excluded.
-template <int DT, int MK>
+// The value of one token (see Lane8), -inf where it is excluded. Greedy under an additive mask: the f32 sum, as the row's sums
+// take it (where a mask lowers a whole row, its rounding is no small part of the differences).
+template <int DT, int MK, bool GREEDY>
 __device__ __forceinline__ double token_value(const void *xrow, const void *mrow, int64_t v, double inv_t) {
     float x;
     if constexpr (DT == NT_F32) x = static_cast<const float *>(xrow)[v];
@@ -192,7 +193,9 @@ __device__ __forceinline__ double token_value(const void *xrow, const void *mrow
     if constexpr (MK == NT_MASK_U8) {
         if (static_cast<const uint8_t *>(mrow)[v] == 0) return -INFINITY;
     } else if constexpr (MK == NT_MASK_F32) {
-        return fma(double(x), inv_t, double(static_cast<const float *>(mrow)[v]));
+        const float m = static_cast<const float *>(mrow)[v];
+        if constexpr (GREEDY) return double(x + m);
+        else return fma(double(x), inv_t, double(m));
     }
     return double(x);
 }
@@ -223,8 +226,8 @@ struct Draft {
         tok = p.tokens[s * p.K + t];
         if constexpr (!GREEDY) u = p.u[s * (p.K + 1) + t];
         if (tok < 0 || tok >= p.V) return;
-        x = token_value<DT, MK>(rows.x, rows.m, tok, p.inv_t);
-        if (rows.y) y = token_value<DT, MK>(rows.y, rows.m, tok, p.inv_td);
+        x = token_value<DT, MK, GREEDY>(rows.x, rows.m, tok, p.inv_t);
+        if (rows.y) y = token_value<DT, MK, GREEDY>(rows.y, rows.m, tok, p.inv_td);
     }
 };
 
@@ -491,7 +494,7 @@ __global__ __launch_bounds__(kDrawThreads, 4) void k_verify_draw(VerifyP p) {
                 lp = NAN;
                 if (GREEDY && d.what < kBad) {
                     id = d.at;
-                    lp = float(((token_value<DT, MK>(rows.x, rows.m, id, p.inv_t) - d.a) * p.c - d.ls) * kLn2);
+                    lp = float(((token_value<DT, MK, true>(rows.x, rows.m, id, p.inv_t) - d.a) * p.c - d.ls) * kLn2);
                 }
             }
             p.ids[s * K1 + t] = id;
@@ -666,7 +669,7 @@ __global__ __launch_bounds__(kDrawThreads) void k_verify_pick(VerifyP p) {
         p.ids[s * (p.K + 1) + k.pos] = int32_t(v);
         if (p.logp)
             p.logp[s * (p.K + 1) + k.pos] =
-                float(((token_value<DT, MK>(rows.x, rows.m, v, p.inv_t) - k.a) * p.c - log2(whole.x)) * kLn2);
+                float(((token_value<DT, MK, false>(rows.x, rows.m, v, p.inv_t) - k.a) * p.c - log2(whole.x)) * kLn2);
     }
 }
 

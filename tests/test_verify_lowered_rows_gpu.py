@@ -1,0 +1,55 @@
+"""Greedy verification under an additive mask that lowers a whole row: the log-probabilities are those of the f32 masked logits
+that its tokens are the first largest of, as the sampler's are. Ids and counts are equal; a log-probability is within half an
+f32 step of its value and 4.2e-6 (its sums' f32 exponentials)."""
+import numpy as np
+import pytest
+
+import noetic_rl as nr
+from tests import draft_reference as ref
+from tests.test_verify_drafted_gpu import run
+
+pytestmark = pytest.mark.gpu
+LOWEST = float(np.finfo(np.float32).min)
+
+
+@pytest.fixture(scope="module", autouse=True)
+def device():
+    nr.claim(0)
+    yield
+
+
+def lowered(x, add):
+    """x + add rounded to f32, as f64."""
+    return (np.asarray(x, np.float32) + add).astype(np.float64)
+
+
+@pytest.mark.parametrize("S", [4, 150])  # several workgroups a position, and one
+@pytest.mark.parametrize("V", [7, 1100, 5003])
+@pytest.mark.parametrize("value", [-1e5, -1e9, -1e13, LOWEST])
+def test_greedy(S, V, value):
+    rng = np.random.default_rng(V)
+    K = 2
+    x = ref.rounded(rng.normal(0, 2, (S, K + 1, V)), "f32")
+    add = np.full((1, 1, V), value, np.float32)
+    z = lowered(x, add)
+    tokens = np.where(rng.random((S, K)) < 0.7, np.argmax(z[:, :K], 2), rng.integers(0, V, (S, K))).astype(np.int32)
+    wi, wa, wl = ref.verify(z, None, tokens, None, np.full(S, K), True)
+    u, mt = rng.random((S, K + 1)), nr.Tensor.from_numpy(add)
+    ids, acc, lp = (t.to_numpy() for t in run(x, None, mt, tokens, u, None, "f32", 0.0))
+    assert np.array_equal(ids, wi) and np.array_equal(acc, wa)
+    assert (np.abs(lp - wl) <= 2.0 ** -24 * np.abs(wl) + 4.2e-6).all()
+    # the sampler's, of the same rows (within its own 4.2e-6 too)
+    sampled, slp = (t.to_numpy() for t in nr.sample_logp(ref.tensor(x, "f32"), 0.0, mt, None))
+    kept = np.arange(K + 1) <= wa[:, None]
+    assert np.array_equal(sampled[kept], wi[kept])
+    assert (np.abs(lp - slp)[kept] <= 2.0 ** -23 * np.abs(wl)[kept] + 8.4e-6).all()
+
+
+@pytest.mark.parametrize("S", [4, 150])
+def test_greedy_with_one_token_left(S):
+    x = np.full((S, 2, 900), 3.7, np.float32)
+    add = np.full((1, 1, 900), -np.inf, np.float32)
+    add[..., 77] = -1e9
+    tokens = np.full((S, 1), 77, np.int32)
+    ids, acc, lp = (t.to_numpy() for t in run(x, None, nr.Tensor.from_numpy(add), tokens, np.full((S, 2), 0.5), None, "f32", 0.0))
+    assert (ids == 77).all() and (acc == 1).all() and (lp == 0.0).all()
