@@ -450,7 +450,8 @@ int nt_hip_rl_score_backward(const NtRlScoreGradArgs *a);
  * NT_ROW_NO_TOKEN), a NaN or +inf among its allowed logits (NT_ROW_NAN), or a draft outside [0, vocab)
  * (NT_ROW_BAD_TOKEN) ends its sequence there: accepted is its position, its id -1 and its logp NaN. A length
  * outside [0, K] accepts nothing (NT_ROW_BAD_TOKEN). What decides a token is f64; the
- * log-probabilities of accepted drafts are, from 256 positions on and greedily, from f32 exponentials (within 4.2e-6). The
+ * log-probabilities of accepted drafts are, from 256 positions on and greedily, from f32 exponentials (within 4.2e-6), and
+ * under an additive mask from 256 positions on of z rounded to f32 where the largest is under 256 in magnitude (7.6e-6 more). The
  * workspace is under 64 bytes per row or piece of one and 16 per sequence and 512 columns; under stream capture a call with
  * 1 MiB of it or more is refused (NT_E_UNSUPPORTED). */
 typedef struct NtRlVerifyArgs {

@@ -44,6 +44,8 @@ enum { kWide, kNarrow, kGreedy };
 // ln 2 of arguments t, |t| < 24 where it matters, in trees of 8), and with an additive mask, whose values are f32
 // tempered logits, by half an f32 step of the largest of each. f64 sums: 1e-11.
 constexpr double kClose32 = 2e-5;
+// The largest tempered logit under an additive mask from which on a row of many is summed in f64 all the same.
+constexpr double kCoarse = 256.0;
 // How near 1 a column's p / q is left to k_verify_pick: far more than f64 sums are off, and more than f32 sums of these rows
 // usually are (1e-7; with a wider one, equal 16-bit differences of many columns fall into it: one row in 200 at kClose32).
 constexpr double kNear64 = 1e-9, kNear32 = 1e-6;
@@ -244,8 +246,8 @@ __device__ __forceinline__ Verdict judge(const VerifyP &p, const VerifyRows<DT, 
         return d;
     }
     d.ls = log2(r.S);
-    // (f32 steps of tempered logits this large are no small part of one, with a reference between them: f64)
-    const bool coarse = HOW == kNarrow && MK == NT_MASK_F32 && fmax(fabs(r.a), r.ad == -INFINITY ? 0.0 : fabs(r.ad)) > 0x1p20;
+    // (half an f32 step of tempered logits up to here is 7.6e-6, no smaller than what else a log-probability is off: past it f64)
+    const bool coarse = HOW == kNarrow && MK == NT_MASK_F32 && fmax(fabs(r.a), r.ad == -INFINITY ? 0.0 : fabs(r.ad)) >= kCoarse;
     if (coarse) d.what = kTooClose;
     if (t >= n) return d;
     if (w.tok < 0 || w.tok >= p.V) {

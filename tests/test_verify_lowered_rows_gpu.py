@@ -53,3 +53,34 @@ def test_greedy_with_one_token_left(S):
     tokens = np.full((S, 1), 77, np.int32)
     ids, acc, lp = (t.to_numpy() for t in run(x, None, nr.Tensor.from_numpy(add), tokens, np.full((S, 2), 0.5), None, "f32", 0.0))
     assert (ids == 77).all() and (acc == 1).all() and (lp == 0.0).all()
+
+
+@pytest.mark.parametrize("value", [-200.3, -1e3, -1e5, -4e5, -1e9])
+def test_accepted_drafts_of_many_positions(value):
+    """450 positions, one workgroup each: what is decided is f64's, where the f32 sums that it starts from are off by half an
+    f32 step of the mask (at -200.3 more than 5e-7 of the drawn row's, which k_verify_pick then computes throughout). An accepted
+    draft's log-probability is from those sums, half a step of |z| up to 256, and from f64 sums past it."""
+    rng = np.random.default_rng(3)
+    S, K, V = 150, 2, 1100
+    x = ref.rounded(rng.normal(0, 2, (S, K + 1, V)), "f32")
+    y = ref.rounded(x[:, :K] + rng.normal(0, 0.5, (S, K, V)), "f32")
+    add = np.full((1, 1, V), value, np.float32)
+    z, zq = x + add.astype(np.float64), y + add.astype(np.float64)
+    tokens = np.argmax(zq + rng.gumbel(size=zq.shape), 2).astype(np.int32)
+    u = rng.random((S, K + 1))
+    wi, wa, wl = ref.verify(z, zq, tokens, u, np.full(S, K), False)
+    ids, acc, lp = (t.to_numpy() for t in run(x, y, nr.Tensor.from_numpy(add), tokens, u, None, "f32", 1.0))
+    assert np.array_equal(ids, wi) and np.array_equal(acc, wa) and (wa > 0).any()
+    largest = np.abs(z).max() if value > -256 else 0.0
+    assert (np.abs(lp - wl) <= 2.0 ** -24 * np.abs(wl) + 4.2e-6 + 2.0 ** -24 * largest).all()
+
+
+def test_a_certain_token_of_many_positions():
+    """The only token that the mask leaves, at -1e5: its log-probability is 0."""
+    S = 300
+    x = np.full((S, 2, 900), 3.7, np.float32)
+    add = np.full((1, 1, 900), -np.inf, np.float32)
+    add[..., 77] = -1e5
+    ids, acc, lp = (t.to_numpy() for t in run(x, None, nr.Tensor.from_numpy(add), np.full((S, 1), 77, np.int32), np.full((S, 2), 0.5),
+                                              None, "f32", 1.0))
+    assert (ids == 77).all() and (acc == 1).all() and (np.abs(lp) <= 4.2e-6).all()
