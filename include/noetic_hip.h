@@ -492,7 +492,7 @@ typedef struct NtRlTopArgs {
     int64_t rows, vocab, ld;  /* vocab < 2^31 */
     const void *mask;
     int64_t mask_ld;
-    double temperature;       /* > 0 and finite */
+    double temperature;       /* a positive normal f32 */
     int64_t k;                /* 1 .. min(vocab, 1024) */
     int32_t *ids;             /* [rows, k] out */
     float *logp;              /* [rows, k] out */
@@ -525,7 +525,7 @@ typedef struct NtRlDistillArgs {
     int64_t rows, vocab, ld;
     const void *mask;
     int64_t mask_ld;
-    double temperature;         /* > 0 and finite */
+    double temperature;         /* a positive normal f32 */
     int64_t k;                  /* tokens listed per row: 1 .. 1024 */
     const int32_t *ids;         /* [rows, k] */
     const float *teacher_logp;  /* [rows, k] */

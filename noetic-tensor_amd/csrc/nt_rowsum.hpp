@@ -201,5 +201,14 @@ __device__ __forceinline__ double moved(double S, double a, double to, double c,
     return a == -INFINITY || a == to ? S : S * exp2_64(a - to, c, low);
 }
 
+// A temperature whose scale of the exponentials, log2(e) / T, f32 holds: T itself one of its normal numbers.
+inline int check_scale(double T) {
+    if (T >= double(FLT_MIN) && T <= double(FLT_MAX)) return 0;
+    char buf[128];
+    std::snprintf(buf, sizeof buf, "tempered_logits: temperature %g (%s)", T,
+                  T > 0.0 && std::isfinite(T) ? "must be a normal f32" : "must be positive");
+    return fail(NT_E_ARG, buf);
+}
+
 }  // namespace
 }  // namespace nt

@@ -441,8 +441,7 @@ void cut_rows(int64_t rows, int nc, int64_t groups, int least, int *segs, int *p
 }
 
 int distill_check(const char *who, int64_t rows, int64_t vocab, int64_t k, double temperature) {
-    if (!(temperature > 0.0) || !std::isfinite(temperature))
-        return fail(NT_E_ARG, "tempered_logits: temperature " + std::to_string(temperature) + " (must be positive)");
+    if (int rc = check_scale(temperature)) return rc;
     if (k < 1 || k > kMaxListed)
         return fail(NT_E_ARG, std::string(who) + ": " + std::to_string(k) + " listed tokens a row (1 to " + std::to_string(kMaxListed) + ")");
     // (a launch holds fewer than 2^32 threads; columns are counted in 32 bits)

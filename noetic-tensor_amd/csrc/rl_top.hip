@@ -401,8 +401,7 @@ extern "C" int nt_hip_rl_top_logprobs(const NtRlTopArgs *a) {
     if (int rc = check_rows(a->rows, a->vocab, a->ld, a->dtype, a->mask_kind, a->mask, a->mask_ld, who)) return rc;
     MaskMap mm;
     if (int rc = mask_map(a->mask_rows, a->rows, a->vocab, a->mask_kind, a->mask_ld, who, &mm)) return rc;
-    if (!(a->temperature > 0.0) || !std::isfinite(a->temperature))
-        return fail(NT_E_ARG, "tempered_logits: temperature " + std::to_string(a->temperature) + " (must be positive)");
+    if (int rc = check_scale(a->temperature)) return rc;
     if (a->k < 1 || a->k > kMaxK || a->k > a->vocab)
         return fail(NT_E_ARG, "top_logprobs: k " + std::to_string(a->k) + " of " + std::to_string(a->vocab) +
                                   " tokens (1 to min(vocab, " + std::to_string(kMaxK) + "))");

@@ -753,8 +753,10 @@ extern "C" int nt_hip_rl_verify_drafted(const NtRlVerifyArgs *a) {
     p.seqs = int(seqs);
     p.K = int(K);
     // One workgroup a position where the positions alone fill the chip's 256 CUs, so that a refusal can spare the
-    // later ones; otherwise about two a CU, each of a chunk per wave or more.
-    const bool one = rows >= 256;
+    // later ones; otherwise about two a CU, each of a chunk per wave or more. (A temperature whose scale f32 does not
+    // hold goes the f64 way too.)
+    const auto held = [](double c) { return c >= double(FLT_MIN) && c <= double(FLT_MAX); };
+    const bool one = rows >= 256 && held(p.c) && held(p.cd);
     p.segs = one ? 1
                  : int(std::min<int64_t>({int64_t(kVerifySegs), (512 + rows - 1) / rows,
                                           (p.nc + kRowWaves - 1) / kRowWaves}));
