@@ -279,7 +279,8 @@ __global__ __launch_bounds__(kTopThreads) void k_top(TopP p) {
         }
 #pragma unroll
         for (int i = 0; i < kItems; i++) {
-            if (at[i] < 0 || s.count > F::kList) continue;
+            // (other threads are adding to the count: a look at it, which only ends work early)
+            if (at[i] < 0 || __hip_atomic_load(&s.count, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP) > F::kList) continue;
             float v[kEpl];
             decode_e<DT, MK, kEpl>(part[i].x, part[i].m, v, p.tau, tau_one);
             in.clean(v, at[i], of[i]);
