@@ -129,6 +129,13 @@ __device__ __forceinline__ double group_max_d(double v, double *s) {
     return t;
 }
 
+// Two f32 in eight bytes.
+__device__ __forceinline__ double two_floats(float a, float b) {
+    return __longlong_as_double(int64_t((uint64_t(__float_as_uint(a)) << 32) | __float_as_uint(b)));
+}
+__device__ __forceinline__ float first_float(double v) { return __uint_as_float(uint32_t(uint64_t(__double_as_longlong(v)) >> 32)); }
+__device__ __forceinline__ float second_float(double v) { return __uint_as_float(uint32_t(uint64_t(__double_as_longlong(v)))); }
+
 // A row's loss, statistics and status from its merged sums. The whole workgroup.
 template <int DT, int MK>
 __device__ void distill_finish(const DistillP &p, int64_t row, const DistillRec &r, double *s) {
@@ -137,14 +144,17 @@ __device__ void distill_finish(const DistillP &p, int64_t row, const DistillRec 
     if constexpr (MK != NT_MASK_NONE) mrow = static_cast<const char *>(p.mask) + mask_row_at(p.mm, row) * MaskWords<MK>::kBytes;
     const int32_t *ids = p.ids + row * p.k;
     const float *teacher = p.teacher + row * p.k;
-    double ln_norm = 0.0;
+    // What a weight's logarithm is less: the largest, a teacher's f32, and the logarithm of the sum relative to it, apart (of
+    // logits that a mask lowered far enough their sum would keep the first alone).
+    double most = 0.0, ln_norm = 0.0;
     if (p.tail == NT_TAIL_RENORMALIZE) {
-        double m = -INFINITY, t = 0.0;
-        for (int j = threadIdx.x; j < p.k; j += kDistillThreads) m = ids[j] >= 0 ? fmax(m, double(teacher[j])) : m;
-        m = group_max_d(m, s);
+        double t = 0.0;
+        most = -INFINITY;
+        for (int j = threadIdx.x; j < p.k; j += kDistillThreads) most = ids[j] >= 0 ? fmax(most, double(teacher[j])) : most;
+        most = group_max_d(most, s);
         for (int j = threadIdx.x; j < p.k; j += kDistillThreads)
-            if (ids[j] >= 0) t += exp(double(teacher[j]) - m);
-        ln_norm = m + log(group_sum_d(t, s));
+            if (ids[j] >= 0) t += exp(double(teacher[j]) - most);
+        ln_norm = log(group_sum_d(t, s));
     }
     // the listed tokens' values (a thread's are kDistillThreads apart), and with their sum the whole row's
     constexpr int kEach = kMaxListed / kDistillThreads;
@@ -170,7 +180,7 @@ __device__ void distill_finish(const DistillP &p, int64_t row, const DistillRec 
         for (int i = 0; i < kEach; i++) {
             const int j = i * kDistillThreads + int(threadIdx.x);
             if (j >= p.k || ids[j] < 0) continue;
-            const double lw = double(teacher[j]) - ln_norm, w = exp(lw);
+            const double lw = (double(teacher[j]) - most) - ln_norm, w = exp(lw);
             const double lq = (v[i] - a) * p.unit - ln_s, d = lq - lw;
             mass += w;
             if (p.tail != NT_TAIL_REST) {
@@ -209,7 +219,7 @@ __device__ void distill_finish(const DistillP &p, int64_t row, const DistillRec 
     const double base = off ? held : 0.0;
     const double factor = off ? (total * exp((r.a - a) * p.unit) / S - rest / r.R) * exp2((base - r.a) * p.c) : 0.0;
     o[0] = base;
-    o[1] = st == NT_ROW_OK ? factor : NAN;
+    o[1] = two_floats(st == NT_ROW_OK ? float(factor) : NAN, float(most));
     o[2] = a;
     o[3] = st == NT_ROW_OK ? total / S : NAN;
     o[4] = ln_norm;
@@ -379,7 +389,8 @@ __global__ __launch_bounds__(kDistillThreads) void k_distill_grad(DistillP p) {
     const double *st = p.stats + row * NT_DISTILL_STATS;
     const double scale = double(g) * p.inv_t;
     const double far = st[0];
-    const float base = float(far), factor = float(scale * st[1]);
+    const float base = float(far), factor = float(scale * double(first_float(st[1])));
+    const double most = double(second_float(st[1]));
     const RowLoad<DT, MK, AL> in(xrow, mrow, p.V, p.nc);
     Raw<DT, MK> raw[kDistillAhead];
     auto load = [&](auto i, int ch) { in.load(raw[i.value], ch, lane, ch < c1); };
@@ -413,7 +424,7 @@ __global__ __launch_bounds__(kDistillThreads) void k_distill_grad(DistillP p) {
     for (int j = threadIdx.x; j < p.k; j += kDistillThreads) {
         const int64_t id = p.ids[row * p.k + j];
         if (id < int64_t(c0) * kChunk || id >= int64_t(c1) * kChunk || id >= p.V) continue;
-        const double w = exp(double(p.teacher[row * p.k + j]) - st[4]);
+        const double w = exp((double(p.teacher[row * p.k + j]) - most) - st[4]);
         const double q = exp((listed_value<DT, MK>(p, xrow, mrow, id) - st[2]) * p.unit) * st[3];  // (times the total)
         const double o = scale * (q - w);
         if constexpr (GDT == NT_F32) {
