@@ -40,9 +40,10 @@ constexpr int kAhead = 4;                     // chunks loaded ahead of f32 sums
 constexpr int kVerifySegs = 64;               // workgroups a position or a drawn row, at most (one lane each)
 // How k_verify_rows sums: in f64, in f32 (see judge), or in f32 with the first largest value.
 enum { kWide, kNarrow, kGreedy };
-// What f32 sums may be off in a log2 ratio of p and q: each of the two log-sum-exps by 6e-6 (weights within 2^-23 and |t| 2^-23
-// ln 2 of arguments t, |t| < 24 where it matters, in trees of 8), and with an additive mask, whose values are f32
-// tempered logits, by half an f32 step of the largest of each. f64 sums: 1e-11.
+// What f32 sums may be off in a log2 ratio of p and q: each of the two log-sum-exps by 6e-6 (of an argument t, up to 60 where a
+// reference trails its lane's largest value: half a step of it 1.9e-6, the rounding of c 60 2^-24 = 3.6e-6; the instruction and trees of 8
+// 0.5e-6), and with an additive mask, whose values are f32 tempered logits, by half an f32 step of the largest of each. f64 sums:
+// 1e-11.
 constexpr double kClose32 = 2e-5;
 // The largest tempered logit under an additive mask from which on a row of many is summed in f64 all the same.
 constexpr double kCoarse = 256.0;
@@ -753,8 +754,9 @@ extern "C" int nt_hip_rl_verify_drafted(const NtRlVerifyArgs *a) {
     p.seqs = int(seqs);
     p.K = int(K);
     // One workgroup a position where the positions alone fill the chip's 256 CUs, so that a refusal can spare the
-    // later ones; otherwise about two a CU, each of a chunk per wave or more. (A temperature whose scale f32 does not
-    // hold goes the f64 way too.)
+    // later ones; otherwise about two a CU, each of a chunk per wave or more. (3 drafts, in several and in one: 128 positions of
+    // 32000 bf16 29.9 and 32.2 us, of 128256 47.6 and 44.3; 256 positions 35.9 and 32.7, 70.5 and 54.6; 512 of 128256 117 and
+    // 87.) A temperature whose scale f32 does not hold goes the f64 way too.
     const auto held = [](double c) { return c >= double(FLT_MIN) && c <= double(FLT_MAX); };
     const bool one = rows >= 256 && held(p.c) && held(p.cd);
     p.segs = one ? 1

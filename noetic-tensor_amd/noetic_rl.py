@@ -1324,9 +1324,9 @@ def distill_with_stats(logits, ids: Tensor, teacher_logp: Tensor, tail: TeacherT
     """Distillation from a teacher's recorded tokens: per position, the divergence KL(teacher || student) of
     softmax(`logits`) (a `Tempered` for a temperature and vocabulary mask) from the weights exp(`teacher_logp`)
     [.., k] at `ids` [.., k] i32 (`top_logprobs`'s; an id of -1 is padding), with `tail` saying what becomes of the
-    rest of the teacher's distribution. Returns (loss [..] f32, DistillStats) for `distill_grad`. A weight at a token
-    that the mask excludes makes the loss +inf. `check` reads the positions' status and refuses an id outside
-    the vocabulary or listed twice."""
+    rest of the teacher's distribution. Under an additive mask x / T + mask is f64. Returns (loss [..] f32, DistillStats)
+    for `distill_grad`. A weight at a token that the mask excludes makes the loss +inf. `check` reads the positions'
+    status and refuses an id outside the vocabulary or listed twice."""
     x = _as_tempered(logits)
     rows, V, k, teacher = _distill_args(x, ids, teacher_logp)
     lead = tuple(x.logits.shape[:-1])
