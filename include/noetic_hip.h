@@ -435,8 +435,8 @@ int nt_hip_rl_score_backward(const NtRlScoreGradArgs *a);
 /* Verification of drafted tokens (speculative decoding; no counterpart in the reference, beside its samplers,
  * rl.rs:488-529). A sequence has K = drafted tokens of a cheaper drafter and the target's logits at K + 1
  * positions: row s (K + 1) + t holds the distribution after the first t drafts. With z = x / T + mask evaluated
- * in f64, p = softmax(z) of the target and q = softmax(z) of the drafter's own logits (row s K + t, under the
- * target row's mask and draft_temperature; no draft_logits: the drafter is certain, q = 1 at its token), the
+ * in f64 (infinite where f32 would be), p = softmax(z) of the target and q = softmax(z) of the drafter's own logits
+ * (row s K + t, under the target row's mask and draft_temperature; no draft_logits: the drafter is certain, q = 1 at its token), the
  * token x drafted at t is accepted while uniforms[s, t] q(x) < p(x). At the first position a that is not, the
  * token is drawn from r = max(p - q, 0) (from p where that is zero everywhere), at a = lengths[s] (all drafts
  * accepted) from p itself: the first v with sum_{j <= v} r_j > uniforms[s, K] sum r, or the last with r > 0.
@@ -450,8 +450,7 @@ int nt_hip_rl_score_backward(const NtRlScoreGradArgs *a);
  * NT_ROW_NO_TOKEN), a NaN or +inf among its allowed logits (NT_ROW_NAN), or a draft outside [0, vocab)
  * (NT_ROW_BAD_TOKEN) ends its sequence there: accepted is its position, its id -1 and its logp NaN. A length
  * outside [0, K] accepts nothing (NT_ROW_BAD_TOKEN). What decides a token is f64; the
- * log-probabilities of accepted drafts are, from 256 positions on and greedily, from f32 exponentials (within 4.2e-6), and
- * under an additive mask from 256 positions on of z rounded to f32 where the largest is under 256 in magnitude (7.6e-6 more). The
+ * log-probabilities of accepted drafts are, from 256 positions on and greedily, from f32 exponentials (within 4.2e-6). The
  * workspace is under 64 bytes per row or piece of one and 16 per sequence and 512 columns; under stream capture a call with
  * 1 MiB of it or more is refused (NT_E_UNSUPPORTED): past about 230 sequences of 7 drafts over 128256 columns. */
 typedef struct NtRlVerifyArgs {
@@ -502,7 +501,7 @@ typedef struct NtRlTopArgs {
 int nt_hip_rl_top_logprobs(const NtRlTopArgs *a);
 
 /* Distillation from a teacher's recorded tokens: the divergence of each row's softmax q (of the student's
- * tempered logits z = x / T + mask in f64) from the teacher's weights w_j = exp(teacher_logp[r, j]) at tokens ids[r, j]:
+ * tempered logits z = x / T + mask in f64, infinite where f32 would be) from the teacher's weights w_j = exp(teacher_logp[r, j]) at tokens ids[r, j]:
  *   NT_TAIL_REST         what the list leaves, rest = max(1 - sum w, 0), is one outcome more:
  *                        loss = sum w (ln w - ln q) + rest (ln rest - ln of the sum of q off the list)
  *   NT_TAIL_DROP         loss = sum w (ln w - ln q)

@@ -190,6 +190,39 @@ struct LaneSums {
     }
 };
 
+// The same over f64 values z of unit scale (tempered logits under an additive mask, which may lower a row so far that an f32 step is
+// no small part of their differences): the exponentials' arguments are f64 differences from the reference, rounded to f32,
+// and the reference is moved where a value lies 16 above it. A weight is within 2^-23 and |t| 3 2^-24 ln 2. What f32 would round to an
+// infinity (kPast on) is one: excluded, or a NaN in S.
+struct FarSum {
+    static constexpr double kPast = 0x1.ffffffp127, kNothing = -0x1.fffffefffffffp127;  // (the next one to -kPast)
+    double S = 0.0, ref = kNothing;
+
+    __device__ __forceinline__ void add(const double z[kEpl], double low) {
+        float d[kEpl];
+#pragma unroll
+        for (int j = 0; j < kEpl; j++) d[j] = float(z[j] - ref);
+        if (!(max8_hw(d) <= 16.0f)) {
+            double high = z[0];
+#pragma unroll
+            for (int j = 1; j < kEpl; j++) high = fmax(high, z[j]);
+            if (high < kPast) {
+                S *= exp2_64(ref - high, kLog2e64, low);
+                ref = high;
+#pragma unroll
+                for (int j = 0; j < kEpl; j++) d[j] = float(z[j] - ref);
+            } else {
+                S = NAN;
+            }
+        }
+#pragma unroll
+        for (int j = 0; j < kEpl; j++) d[j] = exp2_hw(d[j] * kLog2e);
+        S += double(tree8(d));
+    }
+    // The z whose weight is 1; -inf where the lane met no token.
+    __device__ __forceinline__ double at(double, float) const { return ref == kNothing ? -INFINITY : ref; }
+};
+
 __device__ __forceinline__ double wave_max_d(double v) {
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) v = fmax(v, __shfl_xor(v, o, kWave));

@@ -62,37 +62,6 @@ struct DistillP {
 // of its logits' differences, and the sums and the listed tokens have to be of the same values.
 __device__ __forceinline__ double tempered64(const DistillP &p, float x, float m) { return fma(double(x), p.inv_t, double(m)); }
 
-// A lane's sum of 2^(z log2(e)) over such z, as LaneSums: of f32 exponentials, their arguments f64 differences from the reference
-// rounded once, the reference moved where a value lies 16 above it. A NaN or +inf leaves a NaN.
-struct FarSum {
-    static constexpr double kNothing = -0x1p1000;  // below every finite z
-    double S = 0.0, ref = kNothing;
-
-    __device__ __forceinline__ void add(const double z[kEpl], double low) {
-        float d[kEpl];
-#pragma unroll
-        for (int j = 0; j < kEpl; j++) d[j] = float(z[j] - ref);
-        if (!(max8_hw(d) <= 16.0f)) {
-            double high = z[0];
-#pragma unroll
-            for (int j = 1; j < kEpl; j++) high = fmax(high, z[j]);
-            if (high < INFINITY) {
-                S *= exp2_64(ref - high, kLog2e64, low);
-                ref = high;
-#pragma unroll
-                for (int j = 0; j < kEpl; j++) d[j] = float(z[j] - ref);
-            } else {
-                S = NAN;
-            }
-        }
-#pragma unroll
-        for (int j = 0; j < kEpl; j++) d[j] = exp2_hw(d[j] * kLog2e);
-        S += double(tree8(d));
-    }
-    // The z whose weight is 1; -inf where the lane met no token.
-    __device__ __forceinline__ double at(double, float) const { return ref == kNothing ? -INFINITY : ref; }
-};
-
 // The value of one listed token (see c) in f64, -inf where it is excluded.
 template <int DT, int MK>
 __device__ __forceinline__ double listed_value(const DistillP &p, const void *xrow, const void *mrow, int64_t v) {

@@ -42,11 +42,8 @@ constexpr int kVerifySegs = 64;               // workgroups a position or a draw
 enum { kWide, kNarrow, kGreedy };
 // What f32 sums may be off in a log2 ratio of p and q: each of the two log-sum-exps by 6e-6 (of an argument t, up to 60 where a
 // reference trails its lane's largest value: half a step of it 1.9e-6, the rounding of c 60 2^-24 = 3.6e-6; the instruction and trees of 8
-// 0.5e-6), and with an additive mask, whose values are f32 tempered logits, by half an f32 step of the largest of each. f64 sums:
-// 1e-11.
+// 0.5e-6; under an additive mask f64 differences of up to 23 above theirs, 4.6e-6). f64 sums: 1e-11.
 constexpr double kClose32 = 2e-5;
-// The largest tempered logit under an additive mask from which on a row of many is summed in f64 all the same.
-constexpr double kCoarse = 256.0;
 // How near 1 a column's p / q is left to k_verify_pick: far more than f64 sums are off, and more than f32 sums of these rows
 // usually are (1e-7; with a wider one, equal 16-bit differences of many columns fall into it: one row in 200 at kClose32).
 constexpr double kNear64 = 1e-9, kNear32 = 1e-6;
@@ -110,10 +107,10 @@ __device__ __forceinline__ float max8_nan(const float v[kEpl]) {
 }
 
 // One lane's 8 values: a logit, -inf where a u8 mask excludes it; with an additive mask the tempered logit in f64
-// (v: the f32 nearest to it; kGreedy: the f32 sum).
+// (v: the f32 nearest to it, infinite past f32, which FarSum sees to; kGreedy: the f32 sum).
 template <int DT, int MK, int HOW>
 struct Lane8 {
-    static constexpr bool kTwo = MK == NT_MASK_F32 && HOW == kWide;
+    static constexpr bool kTwo = MK == NT_MASK_F32 && HOW != kGreedy;
     float v[kEpl];
     double z[kTwo ? kEpl : 1];
 
@@ -136,10 +133,14 @@ struct Lane8 {
     }
     template <class R>
     __device__ __forceinline__ void clean(const R &row, int ch, int lane) {
-        row.clean(v, ch, lane);
-        if constexpr (kTwo) {
+        if constexpr (kTwo && HOW == kNarrow) {
+            row.clean(z, ch, lane);
+        } else {
+            row.clean(v, ch, lane);
+            if constexpr (kTwo) {
 #pragma unroll
-            for (int j = 0; j < kEpl; j++) z[j] = v[j] == -INFINITY ? -INFINITY : z[j];
+                for (int j = 0; j < kEpl; j++) z[j] = v[j] == -INFINITY ? -INFINITY : z[j];
+            }
         }
     }
     __device__ __forceinline__ double at(int j) const {
@@ -247,9 +248,6 @@ __device__ __forceinline__ Verdict judge(const VerifyP &p, const VerifyRows<DT, 
         return d;
     }
     d.ls = log2(r.S);
-    // (half an f32 step of tempered logits up to here is 7.6e-6, no smaller than what else a log-probability is off: past it f64)
-    const bool coarse = HOW == kNarrow && MK == NT_MASK_F32 && fmax(fabs(r.a), r.ad == -INFINITY ? 0.0 : fabs(r.ad)) >= kCoarse;
-    if (coarse) d.what = kTooClose;
     if (t >= n) return d;
     if (w.tok < 0 || w.tok >= p.V) {
         d.what = kBad + NT_ROW_BAD_TOKEN;
@@ -279,8 +277,7 @@ __device__ __forceinline__ Verdict judge(const VerifyP &p, const VerifyRows<DT, 
     // that the target gives nothing never is (inf - inf compares false)
     d.what = w.u < exp2(l - lq) ? kAccept : kDraw;
     if constexpr (HOW == kNarrow) {
-        const double steps = MK == NT_MASK_F32 ? 0x1p-23 * kLog2e64 * (fabs(r.a) + (rows.y ? fabs(r.ad) : 0.0)) : 0.0;
-        if (coarse || fabs(log2(w.u) - (l - lq)) < kClose32 + steps) d.what = kTooClose;
+        if (fabs(log2(w.u) - (l - lq)) < kClose32) d.what = kTooClose;
     }
     return d;
 }
@@ -355,6 +352,9 @@ __device__ __forceinline__ void add_rows(const VerifyP &p, const VerifyRows<DT, 
         if constexpr (HOW == kWide) {
             sx.add(lx, p.c, p.low, p.cap);
             if (both) sy.add(ly, p.cd, p.lowd, p.capd);
+        } else if constexpr (std::is_same_v<L, FarSum>) {
+            sx.add(lx.z, p.low);
+            if (both) sy.add(ly.z, p.lowd);
         } else {
             sx.add(lx.v, p.c32);
             if (both) sy.add(ly.v, p.cd32);
@@ -362,8 +362,8 @@ __device__ __forceinline__ void add_rows(const VerifyP &p, const VerifyRows<DT, 
     });
 }
 
-template <int HOW>
-using Sum = std::conditional_t<HOW == kWide, LaneSum, LaneSums>;
+template <int HOW, int MK>
+using Sum = std::conditional_t<HOW == kWide, LaneSum, std::conditional_t<HOW == kNarrow && MK == NT_MASK_F32, FarSum, LaneSums>>;
 
 template <int DT, int MK, bool AL, int HOW>
 __global__ __launch_bounds__(kRowThreads) void k_verify_rows(VerifyP p) {
@@ -388,7 +388,7 @@ __global__ __launch_bounds__(kRowThreads) void k_verify_rows(VerifyP p) {
     const int c1 = min(p.nc, (seg + 1) * p.per);
     Draft w;
     if (p.first) w.load<DT, MK, HOW == kGreedy>(p, rows, s, t, n);
-    Sum<HOW> sx, sy;
+    Sum<HOW, MK> sx, sy;
     float top = -INFINITY;
     int32_t at = 0x7fffffff;
     add_rows<DT, MK, AL, HOW>(p, rows, both, seg * p.per + wave, kRowWaves, c1, lane, sx, sy, &top, &at);
