@@ -71,7 +71,8 @@ __device__ __forceinline__ double listed_value(const DistillP &p, const void *xr
     if constexpr (MK == NT_MASK_U8) {
         if (static_cast<const uint8_t *>(mrow)[v] == 0) return -INFINITY;
     } else if constexpr (MK == NT_MASK_F32) {
-        return tempered64(p, x, static_cast<const float *>(mrow)[v]);
+        const double z = tempered64(p, x, static_cast<const float *>(mrow)[v]);
+        return fabs(z) < FarSum::kPast ? z : z * INFINITY;  // (past f32, as in the sums: infinite; a NaN stays one)
     }
     return double(x);
 }

@@ -38,3 +38,42 @@ def test_verification_of_few_and_many_positions(temperature):
     assert (many[1] == K).all() and np.array_equal(many[0][:, :K], tokens)   # (the drafter's logits are the target's)
     if temperature < 1:
         assert np.array_equal(many[0][:, K], np.argmax(z[:, K], 1))
+
+
+@pytest.mark.gpu
+def test_tempered_logits_past_f32():
+    """Under an additive mask a tempered logit that f32 would round to -inf is excluded and one that it would round to +inf refuses
+    its row, in every operator and for few and many positions (1e-37: 5 is held, 50 is not)."""
+    nr.claim(0)
+    T, V, S, K = 1e-37, 3000, 200, 1
+    x = np.full((S, K + 1, V), -50.0, np.float32)
+    x[:, :, 7], x[:, :, 2900] = 5.0, 5.0
+    x[1, 0, 11] = 50.0
+    add = nr.Tensor.from_numpy(np.zeros((1, 1, V), np.float32))
+    tokens = np.full((S, K), 2900, np.int32)
+    u = np.full((S, K + 1), 0.4)
+    bad = np.arange(S) == 1
+    for n in (3, S):
+        ids, acc, lp = (t.to_numpy() for t in nr.verify_drafted(
+            nr.Tensor.from_numpy(x[:n]), None, nr.Tensor.from_numpy(tokens[:n]), T, add, None, uniforms=nr.Tensor.from_numpy(u[:n], "f64"),
+            check=False))
+        assert np.array_equal(ids[:, 0] < 0, bad[:n]) and np.array_equal(acc, np.where(bad[:n], 0, 1))
+        assert (ids[~bad[:n]] == [2900, 7]).all() and (np.abs(lp[~bad[:n]] + np.log(2)) < 1e-6).all()
+        rows = nr.Tempered(nr.Tensor.from_numpy(x[:n, 0].copy()), T, nr.Tensor.from_numpy(np.zeros((1, V), np.float32)))
+        top, lp = (t.to_numpy() for t in nr.top_logprobs(rows, 3, check=False))
+        assert np.array_equal(np.isnan(lp).all(1), bad[:n]) and (top[~bad[:n]] == [7, 2900, -1]).all()
+        for listed, loss in (([7, 11], np.inf), ([7, 2900], 0.0)):
+            it = nr.Tensor.from_numpy(np.tile(np.array(listed, np.int32), (n, 1)))
+            lt = nr.Tensor.from_numpy(np.full((n, 2), np.log(0.5), np.float32))
+            got, stats = nr.distill_with_stats(rows, it, lt, check=False)
+            got = got.to_numpy()
+            assert np.isnan(got[bad[:n]]).all()
+            good = got[~bad[:n]]
+            assert (good == loss).all() if loss else (np.abs(good) < 1e-6).all()
+            grad = nr.distill_grad(rows, it, lt, stats, nr.Tensor.from_numpy(np.full(n, 1e-37, np.float32))).to_numpy()
+            assert np.isnan(grad[bad[:n]]).all()
+            want = np.zeros(V)
+            want[7] += 0.5
+            want[2900] += 0.5
+            want[listed] -= 0.5
+            assert (np.abs(grad[~bad[:n]] - want) < 1e-6).all()
